@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define XL_ABI_VERSION 2
+#define XL_ABI_VERSION 3
 
 enum xl_dtype { XL_DTYPE_F32 = 0, XL_DTYPE_BF16 = 1, XL_DTYPE_F16 = 2 };
 
@@ -364,6 +364,32 @@ int xl_mlstm_chunkwise_bwd(const void* q, const void* k, const void* v, const vo
  */
 int xl_lm_head_softcap_fwd(const void* x, const void* weight, void* y, int M, int D, int V, float cap,
                            int dtype, void* stream);
+
+/*
+ * Layer norm of rows of D values, y = (x - mean) / sqrt(var + eps) * weight + bias, in float32, rounded once.  The
+ * rows are n0 * n1 tokens of H heads; H = 1 is the plain layer norm over the last axis, H > 1 the per-head norm with
+ * weights of each head (nn.LayerNorm per head; MultiHeadLayerNorm, xlstm_metal/torch_native/blocks/mlstm/
+ * multihead_norm/multihead_norm.py:5-40).
+ *   x: token (i0, i1) of head h at i0 * x_strides[0] + i1 * x_strides[1] + h * x_strides[2] (elements; values
+ *   contiguous; NULL: [n0, n1, H, D] contiguous); y [n0, n1, H, D] contiguous; weight, bias [H, D] of param_dtype
+ *   (dtype or XL_DTYPE_F32) or NULL; mean, rstd [n0, n1, H] float32 or NULL (what the backward needs).  Pointers
+ *   aligned to their elements.  y must not overlap x.  n0 * n1 * H and H * D below 2^31.
+ */
+int xl_layer_norm_fwd(const void* x, const int64_t* x_strides, const void* weight, const void* bias, void* y,
+                      float* mean, float* rstd, int64_t n0, int64_t n1, int H, int D, float eps, int dtype,
+                      int param_dtype, void* stream);
+
+/*
+ * Its gradients from dy [n0, n1, H, D] contiguous and the forward's x, mean and rstd: dx (dx_strides as x_strides;
+ * rows apart), dweight and dbias [H, D] of param_dtype (sums over the tokens in float32, rounded once; zero without
+ * tokens).  Any of the three may be NULL.  dx must not overlap dy or x.  The workspace
+ * (xl_layer_norm_bwd_workspace_size bytes, 16-byte aligned) is needed for dweight or dbias only.
+ */
+size_t xl_layer_norm_bwd_workspace_size(int64_t n0, int64_t n1, int H, int D);
+int xl_layer_norm_bwd(const void* dy, const void* x, const int64_t* x_strides, const void* weight, const float* mean,
+                      const float* rstd, void* dx, const int64_t* dx_strides, void* dweight, void* dbias, int64_t n0,
+                      int64_t n1, int H, int D, int dtype, int param_dtype, void* workspace, size_t workspace_bytes,
+                      void* stream);
 
 #ifdef __cplusplus
 }

@@ -634,6 +634,157 @@ Tensor silu_mul(const Tensor& g_, const Tensor& u_) {
   return y;
 }
 
+// ------------------------------------------- layer norm and its gradients
+struct NormShape {
+  int64_t H, D, tokens;
+  int param;  // the weights' dtype code
+};
+NormShape norm_shape(const Tensor& x, const OptTensor& w, const OptTensor& b, const char* what) {
+  XL_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, "x must have a last axis of at least one value, got ", x.sizes());
+  const Tensor* p = opt(w) ? opt(w) : opt(b);
+  const int dt = dtype_code(x, what);
+  NormShape s{1, x.size(-1), 0, dt};
+  if (p) {
+    XL_CHECK(p->dim() >= 1 && p->dim() <= 2 && p->dim() <= x.dim() && p->sizes() == x.sizes().slice(x.dim() - p->dim()), what,
+             p == opt(w) ? "weight" : "bias", " must have the shape of x's last axis, or of its last two, got ", p->sizes(),
+             " for x ", x.sizes());
+    if (p->dim() == 2) s.H = p->size(0);
+    XL_CHECK(s.H >= 1, what, "no heads");
+    XL_CHECK(p->scalar_type() == x.scalar_type() || p->scalar_type() == at::kFloat, what,
+             "weight and bias must be of x's dtype ", x.scalar_type(), " or float32, got ", p->scalar_type());
+    s.param = dtype_code(*p, what);
+  }
+  XL_CHECK(!opt(w) || !opt(b) || (w->sizes() == b->sizes() && w->scalar_type() == b->scalar_type()), what,
+           "weight and bias must share shape and dtype");
+  s.tokens = x.numel() / (s.H * s.D);
+  return s;
+}
+
+// The tokens of t [..., H, D] (H only where H > 1) as at most two strided axes: sizes n, strides {n0's, n1's, the
+// head's}.  False where its values are not contiguous or more axes are left.
+bool as_tokens(const Tensor& t, int64_t H, int64_t (&n)[2], int64_t (&strides)[3]) {
+  int64_t outer = t.dim() - 1;
+  if (t.size(-1) > 1 && t.stride(-1) != 1) return false;
+  strides[2] = t.size(-1);
+  if (H > 1) strides[2] = t.stride(--outer);
+  int at = 1;
+  n[0] = n[1] = 1;
+  strides[0] = strides[1] = 0;
+  bool any = false;
+  for (int64_t d = outer - 1; d >= 0; --d) {
+    const int64_t size = t.size(d), stride = t.stride(d);
+    if (size == 1 && t.numel()) continue;
+    if (any && stride == strides[at] * n[at]) {
+      n[at] *= size;
+    } else {
+      if (any && --at < 0) return false;
+      n[at] = size;
+      strides[at] = stride;
+      any = true;
+    }
+  }
+  return true;
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm(const Tensor& x_, const OptTensor& w_, const OptTensor& b_, double eps) {
+  const char* what = "layer_norm";
+  Gpu gpu(what, {&x_, opt(w_), opt(b_)});
+  const NormShape s = norm_shape(x_, w_, b_, what);
+  int64_t n[2], st[3];
+  const bool strided = as_tokens(x_, s.H, n, st);
+  const Tensor x = strided ? x_ : x_.contiguous(), w = prep(w_), b = prep(b_), y = at::empty(x.sizes(), x.options());
+  const auto lead = x.sizes().slice(0, x.dim() - 1);
+  const Tensor mean = at::empty(lead, f32_on(x)), rstd = at::empty(lead, f32_on(x));
+  check_rc(xl_layer_norm_fwd(ptr(x), strided ? st : nullptr, ptr(w), ptr(b), ptr(y), ptr<float>(mean), ptr<float>(rstd),
+                             strided ? n[0] : 1, strided ? n[1] : s.tokens, i32(s.H, what), i32(s.D, what), (float)eps,
+                             dtype_code(x, what), s.param, gpu.st),
+           what);
+  return {y, mean, rstd};
+}
+
+std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& mean_,
+                                                  const Tensor& rstd_, const OptTensor& w_, const OptTensor& b_,
+                                                  std::array<bool, 3> mask) {
+  const char* what = "layer_norm_bwd";
+  Gpu gpu(what, {&dy_, &x_, &mean_, &rstd_, opt(w_), opt(b_)});
+  const NormShape s = norm_shape(x_, w_, b_, what);
+  XL_CHECK(dy_.sizes() == x_.sizes(), what, "dy must have x's shape, got ", dy_.sizes());
+  const auto lead = x_.sizes().slice(0, x_.dim() - 1);
+  for (const Tensor* t : {&mean_, &rstd_})
+    XL_CHECK(t->sizes() == lead && t->scalar_type() == at::kFloat, what, "mean and rstd must be float32 of shape ", lead);
+  int64_t n[2], st[3], dn[2], dst[3];
+  const bool strided = as_tokens(x_, s.H, n, st);
+  const Tensor x = strided ? x_ : x_.contiguous(), w = prep(w_), mean = mean_.contiguous(), rstd = rstd_.contiguous();
+  const Tensor dy = (dy_.scalar_type() == x.scalar_type() ? dy_ : dy_.to(x.scalar_type())).contiguous();
+  const Tensor none = at::empty({0}, x.options());
+  // dx lies as x does where its tokens then fold as x's do: behind the chunkwise kernel it is [B, NH, S, DH] in memory
+  Tensor dx = none;
+  bool dx_strided = false;
+  if (mask[0]) {
+    dx = at::empty_like(x_);
+    dx_strided = strided && as_tokens(dx, s.H, dn, dst) && dn[0] == n[0] && dn[1] == n[1];
+    if (!dx_strided) dx = at::empty(x_.sizes(), x_.options());
+  }
+  const Tensor dw = mask[1] && opt(w_) ? at::empty(w_->sizes(), w_->options()) : at::empty({0}, x.options());
+  const Tensor db = mask[2] && opt(b_) ? at::empty(b_->sizes(), b_->options()) : at::empty({0}, x.options());
+  const bool want_w = mask[1] && opt(w_), want_b = mask[2] && opt(b_);
+  const int64_t n0 = strided ? n[0] : 1, n1 = strided ? n[1] : s.tokens;
+  const int H = i32(s.H, what), D = i32(s.D, what);
+  const size_t ws_bytes = want_w || want_b ? xl_layer_norm_bwd_workspace_size(n0, n1, H, D) : 0;
+  const Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, x.options().dtype(at::kByte)) : Tensor();
+  check_rc(xl_layer_norm_bwd(ptr(dy), ptr(x), strided ? st : nullptr, ptr(w), ptr<float>(mean), ptr<float>(rstd),
+                             mask[0] ? ptr(dx) : nullptr, dx_strided ? dst : nullptr, want_w ? ptr(dw) : nullptr,
+                             want_b ? ptr(db) : nullptr, n0, n1, H, D, dtype_code(x, what), s.param, ptr(ws), ws_bytes,
+                             gpu.st),
+           what);
+  return {dx, dw, db};
+}
+
+using ThreeTensors = std::tuple<Tensor, Tensor, Tensor>;
+
+ThreeTensors call_layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::layer_norm", "").typed<decltype(layer_norm)>();
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, w, b, eps);
+}
+
+// Gradients of y; mean and rstd are not differentiable.
+struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& w,
+                                                const OptTensor& b, double eps) {
+    auto [y, mean, rstd] = call_layer_norm(x, w, b, eps);
+    ctx->save_for_backward({x, w.value_or(Tensor()), b.value_or(Tensor()), mean, rstd});
+    ctx->mark_non_differentiable({mean, rstd});
+    ctx->set_materialize_grads(false);
+    return {y, mean, rstd};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    static const auto bwd = c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::layer_norm_bwd", "")
+                                .typed<decltype(layer_norm_bwd)>();
+    const Tensor none;
+    if (!grads[0].defined()) return {none, none, none, none};
+    const auto saved = ctx->get_saved_variables();
+    auto given = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    std::array<bool, 3> mask = {};
+    for (size_t i = 0, edge = 0; i < 3; ++i)  // an argument left out has no edge
+      if (saved[i].defined()) mask[i] = ctx->needs_input_grad(edge++);
+    auto [dx, dw, db] = bwd.call(grads[0], saved[0], saved[3], saved[4], given(saved[1]), given(saved[2]), mask);
+    return {mask[0] ? dx : none, mask[1] ? dw : none, mask[2] ? db : none, none};
+  }
+};
+
+ThreeTensors layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+  bool any = false;
+  for (const Tensor* t : {&x, opt(w), opt(b)})
+    any = any || (t && t->defined() && (t->requires_grad() || t->_fw_grad(0).defined()));
+  if (!any) return call_layer_norm(x, w, b, eps);
+  const auto r = LayerNormFn::apply(x, w, b, eps);
+  return {r[0], r[1], r[2]};
+}
+
 // The operators that write an argument, under autograd's bookkeeping, on fake tensors as on real ones.  What they
 // write is updated outside autograd, whatever it requires (a leaf too; its own history stays), a backward through
 // the outputs raises, and the written tensors' version counters move (inference tensors have none).
@@ -729,18 +880,21 @@ TORCH_LIBRARY_IMPL(xlstm_hip, CUDA, m) {
   m.impl("rms_norm", rms_norm);
   m.impl("add_rmsnorm", add_rmsnorm);
   m.impl("silu_mul", silu_mul);
+  m.impl("layer_norm", layer_norm);
+  m.impl("layer_norm_bwd", layer_norm_bwd);
 }
 
-// The chunkwise forward differentiates through its own backward; every other operator is forward-only and
-// a backward through it raises.
+// The chunkwise forward and the layer norm differentiate through their own backward; every other operator is
+// forward-only and a backward through it raises.
 #define XL_FORWARD_ONLY(m, kernel)                                                                                     \
   for (const char* op : {"soft_cap", "mlstm_step", "mlstm_chunkwise_bwd", "mlstm_sequence", "slstm_step",              \
                          "slstm_sequence", "causal_conv1d", "group_norm", "mh_rmsnorm_gate", "gate_proj_softcap",      \
-                         "gate_proj2_softcap", "lm_head_softcap", "rms_norm", "silu_mul"})                             \
+                         "gate_proj2_softcap", "lm_head_softcap", "rms_norm", "silu_mul", "layer_norm_bwd"})           \
     m.impl(op, kernel());
 TORCH_LIBRARY_IMPL(xlstm_hip, Autograd, m) {
   if (!abi_matches()) return;
   m.impl("mlstm_chunkwise", mlstm_chunkwise_autograd);
+  m.impl("layer_norm", layer_norm_autograd);
   m.impl("mlstm_step_", mlstm_step__autograd);
   m.impl("add_rmsnorm", add_rmsnorm_autograd);
   XL_FORWARD_ONLY(m, torch::autograd::autogradNotImplementedFallback)

@@ -31,6 +31,7 @@ import torch.nn as nn
 import torch.nn.functional as F
 from torch import Tensor
 
+from .norms import multi_head_layer_norm
 from .ops import gate_proj2_softcap_op, gate_proj_softcap_op, mh_rmsnorm_gate_op
 from .soft_cap import soft_cap
 
@@ -143,7 +144,7 @@ class MultiHeadLayerNorm(nn.Module):
     """``multihead_norm.py:5-40``: per-head LayerNorm of x [B, S, NH, DH] -> [B, S, NH * DH], optional
     weight and bias.  Runs ``group_norm_kernel`` (one group per head) on the [B * S, NH * DH] view,
     with float32 statistics and one rounding of the output; the reference takes the mean and
-    variance in x's own dtype."""
+    variance in x's own dtype.  Where a gradient is wanted it runs ``multi_head_layer_norm``, which has one."""
 
     def __init__(self, num_heads: int, head_dim: int, eps: float = 1e-6, use_weight: bool = True,
                  use_bias: bool = False) -> None:
@@ -166,6 +167,8 @@ class MultiHeadLayerNorm(nn.Module):
         B, S, NH, DH = x.shape
         if NH != self.num_heads or DH != self.head_dim:
             raise ValueError(f"Expected shape [B,S,{self.num_heads},{self.head_dim}], got {x.shape}")
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.weight, self.bias)):
+            return multi_head_layer_norm(x, self.weight, self.bias, self.eps, heads_first=False)
         from .slstm_layers import group_norm
         return group_norm(x.reshape(B * S, NH * DH), NH, self.weight, self.bias, self.eps).view(B, S, NH * DH)
 

@@ -4,8 +4,8 @@ Schemas and fake (meta) kernels are declared here, so the ops are traceable; the
 (csrc/torch_ops.cpp, lib/libxlstm_torch.so): they validate shapes and dtypes, allocate the outputs with
 torch's caching allocator (the library itself never allocates), pass raw pointers and the current HIP
 stream through the C-ABI and return without synchronising.  There is no CPU path: CPU tensors raise.
-``mlstm_chunkwise`` differentiates through the reference's custom backward; a backward through any other
-op raises.
+``mlstm_chunkwise`` differentiates through the reference's custom backward and ``layer_norm`` through its own; a
+backward through any other op raises.
 """
 
 from __future__ import annotations
@@ -22,6 +22,7 @@ __all__ = [
     "soft_cap_op", "mlstm_step_op", "mlstm_step_inplace_op", "mlstm_chunkwise_op", "mlstm_chunkwise_bwd_op", "mlstm_sequence_op",
     "slstm_step_op", "slstm_sequence_op", "causal_conv1d_op", "group_norm_op", "mh_rmsnorm_gate_op",
     "gate_proj_softcap_op", "gate_proj2_softcap_op", "lm_head_softcap_op", "rms_norm_op", "add_rmsnorm_op", "silu_mul_op",
+    "layer_norm_op",
     "chunkwise_workspace_bytes", "chunkwise_algorithm",
 ]
 
@@ -68,6 +69,12 @@ _SCHEMAS = {
                    "copy_dst) -> (Tensor, Tensor)"),
     # silu(gate) * up, the SiLU rounded to the dtype first (bf16 / f16)
     "silu_mul": ("(Tensor gate, Tensor up) -> Tensor"),
+    # (y, mean, rstd) of the norm over the last axis; weight and bias have the last axis' shape, or the last
+    # two axes' (a norm's weights for each head)
+    "layer_norm": ("(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)"),
+    # (dx, dweight, dbias); what the mask leaves out is an empty placeholder
+    "layer_norm_bwd": ("(Tensor dy, Tensor x, Tensor mean, Tensor rstd, Tensor? weight, Tensor? bias, bool[3] "
+                      "output_mask) -> (Tensor, Tensor, Tensor)"),
 }
 
 _library = torch.library.Library("xlstm_hip", "DEF")
@@ -212,6 +219,19 @@ def _(gate, up):
     return torch.empty_like(gate, memory_format=torch.contiguous_format)
 
 
+@_fake("layer_norm")
+def _(x, weight, bias, eps):
+    stats = tuple(x.new_empty(x.shape[:-1], dtype=torch.float32) for _ in range(2))
+    return (torch.empty_like(x, memory_format=torch.contiguous_format),) + stats
+
+
+@_fake("layer_norm_bwd")
+def _(dy, x, mean, rstd, weight, bias, output_mask):
+    dw, db = (torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None and wanted
+              else x.new_empty(_EMPTY_SHAPE) for t, wanted in zip((weight, bias), output_mask[1:]))
+    return torch.empty_like(x) if output_mask[0] else x.new_empty(_EMPTY_SHAPE), dw, db
+
+
 soft_cap_op = torch.ops.xlstm_hip.soft_cap.default
 mlstm_step_op = torch.ops.xlstm_hip.mlstm_step.default
 mlstm_step_inplace_op = torch.ops.xlstm_hip.mlstm_step_.default
@@ -227,6 +247,7 @@ lm_head_softcap_op = torch.ops.xlstm_hip.lm_head_softcap.default
 rms_norm_op = torch.ops.xlstm_hip.rms_norm.default
 add_rmsnorm_op = torch.ops.xlstm_hip.add_rmsnorm.default
 silu_mul_op = torch.ops.xlstm_hip.silu_mul.default
+layer_norm_op = torch.ops.xlstm_hip.layer_norm.default
 
 CONV_ACTS = {None: 0, "silu": 1}
 # csrc/torch_ops.cpp's own (0 where no kernel can run): the most rows of lm_head_softcap and the LDS of its
