@@ -385,7 +385,7 @@ int xl_layer_norm_fwd(const void* x, const int64_t* x_strides, const void* weigh
  * tokens).  Any of the three may be NULL.  dx must not overlap dy or x.  The workspace
  * (xl_layer_norm_bwd_workspace_size bytes, 16-byte aligned) is needed for dweight or dbias only.
  */
-size_t xl_layer_norm_bwd_workspace_size(int64_t n0, int64_t n1, int H, int D);
+size_t xl_layer_norm_bwd_workspace_size(int64_t n0, int64_t n1, int H, int D, int dtype);
 int xl_layer_norm_bwd(const void* dy, const void* x, const int64_t* x_strides, const void* weight, const float* mean,
                       const float* rstd, void* dx, const int64_t* dx_strides, void* dweight, void* dbias, int64_t n0,
                       int64_t n1, int H, int D, int dtype, int param_dtype, void* workspace, size_t workspace_bytes,

@@ -43,12 +43,12 @@ def test_backward_refuses(lib):
         assert bwd(lib, dx=big, **bad) == -1 and b"null" in lib.xl_last_error()
     assert bwd(lib, dx=P) == -1 and bwd(lib, dx=Q) == -1
     assert bwd(lib, dx=big, D=0) == -1
-    need = lib.xl_layer_norm_bwd_workspace_size(1, 4, 1, 64)
+    need = lib.xl_layer_norm_bwd_workspace_size(1, 4, 1, 64, 1)
     assert need > 0
     assert bwd(lib, dw=big) == -3 and b"workspace" in lib.xl_last_error()
     assert bwd(lib, dw=big, ws=big, ws_bytes=need - 1) == -3
     assert bwd(lib, dw=big, ws=ctypes.c_void_p(4100), ws_bytes=need) == -3
-    assert lib.xl_layer_norm_bwd_workspace_size(1, 4, 1, 0) == 0
+    assert lib.xl_layer_norm_bwd_workspace_size(1, 4, 1, 0, 1) == 0
 
 
 def test_cpu_tensors_raise():

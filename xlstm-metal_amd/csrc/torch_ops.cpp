@@ -635,45 +635,45 @@ Tensor silu_mul(const Tensor& g_, const Tensor& u_) {
 }
 
 // ------------------------------------------- layer norm and its gradients
+// layout: 0, the norm over x's last axis; 1 and 2, the norm of each head of [B, NH, S, DH] or [B, S, NH, DH], written
+// [B, S, NH * DH].  Statistics: float32 [2, rows], the means and then 1 / sqrt(var + eps).
 struct NormShape {
   int64_t H, D, tokens;
   int param;  // the weights' dtype code
 };
-NormShape norm_shape(const Tensor& x, const OptTensor& w, const OptTensor& b, const char* what) {
+NormShape norm_shape(const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t layout, const char* what) {
+  XL_CHECK(layout >= 0 && layout <= 2, what, "layout must be 0, 1 or 2, got ", layout);
+  XL_CHECK(layout == 0 || x.dim() == 4, what, "heads are of a 4-D tensor, got ", x.sizes());
   XL_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, "x must have a last axis of at least one value, got ", x.sizes());
-  const Tensor* p = opt(w) ? opt(w) : opt(b);
-  const int dt = dtype_code(x, what);
-  NormShape s{1, x.size(-1), 0, dt};
-  if (p) {
-    XL_CHECK(p->dim() >= 1 && p->dim() <= 2 && p->dim() <= x.dim() && p->sizes() == x.sizes().slice(x.dim() - p->dim()), what,
-             p == opt(w) ? "weight" : "bias", " must have the shape of x's last axis, or of its last two, got ", p->sizes(),
-             " for x ", x.sizes());
-    if (p->dim() == 2) s.H = p->size(0);
-    XL_CHECK(s.H >= 1, what, "no heads");
-    XL_CHECK(p->scalar_type() == x.scalar_type() || p->scalar_type() == at::kFloat, what,
-             "weight and bias must be of x's dtype ", x.scalar_type(), " or float32, got ", p->scalar_type());
-    s.param = dtype_code(*p, what);
+  NormShape s{layout ? x.size(layout == 1 ? 1 : 2) : 1, x.size(-1), 0, dtype_code(x, what)};
+  XL_CHECK(s.H >= 1, what, "no heads in ", x.sizes());
+  for (const OptTensor* t : {&w, &b}) {
+    if (!opt(*t)) continue;
+    XL_CHECK((*t)->dim() == 1 && (*t)->size(0) == s.H * s.D, what, t == &w ? "weight" : "bias", " must be (", s.H * s.D,
+             ",), got ", (*t)->sizes());
+    XL_CHECK((*t)->scalar_type() == x.scalar_type() || (*t)->scalar_type() == at::kFloat, what,
+             "weight and bias must be of x's dtype ", x.scalar_type(), " or float32, got ", (*t)->scalar_type());
+    s.param = dtype_code(**t, what);
   }
-  XL_CHECK(!opt(w) || !opt(b) || (w->sizes() == b->sizes() && w->scalar_type() == b->scalar_type()), what,
-           "weight and bias must share shape and dtype");
+  XL_CHECK(!opt(w) || !opt(b) || w->scalar_type() == b->scalar_type(), what, "weight and bias must share a dtype");
   s.tokens = x.numel() / (s.H * s.D);
   return s;
 }
 
-// The tokens of t [..., H, D] (H only where H > 1) as at most two strided axes: sizes n, strides {n0's, n1's, the
+// The tokens of t [..., H, D] (H only where `heads`) as at most two strided axes: sizes n, strides {n0's, n1's, the
 // head's}.  False where its values are not contiguous or more axes are left.
-bool as_tokens(const Tensor& t, int64_t H, int64_t (&n)[2], int64_t (&strides)[3]) {
+bool as_tokens(const Tensor& t, bool heads, int64_t (&n)[2], int64_t (&strides)[3]) {
   int64_t outer = t.dim() - 1;
   if (t.size(-1) > 1 && t.stride(-1) != 1) return false;
   strides[2] = t.size(-1);
-  if (H > 1) strides[2] = t.stride(--outer);
+  if (heads) strides[2] = t.stride(--outer);
   int at = 1;
   n[0] = n[1] = 1;
   strides[0] = strides[1] = 0;
   bool any = false;
   for (int64_t d = outer - 1; d >= 0; --d) {
     const int64_t size = t.size(d), stride = t.stride(d);
-    if (size == 1 && t.numel()) continue;
+    if (size == 1) continue;
     if (any && stride == strides[at] * n[at]) {
       n[at] *= size;
     } else {
@@ -686,103 +686,118 @@ bool as_tokens(const Tensor& t, int64_t H, int64_t (&n)[2], int64_t (&strides)[3
   return true;
 }
 
-std::tuple<Tensor, Tensor, Tensor> layer_norm(const Tensor& x_, const OptTensor& w_, const OptTensor& b_, double eps) {
+std::tuple<Tensor, Tensor> layer_norm(const Tensor& x_, const OptTensor& w_, const OptTensor& b_, double eps,
+                                      int64_t layout) {
   const char* what = "layer_norm";
   Gpu gpu(what, {&x_, opt(w_), opt(b_)});
-  const NormShape s = norm_shape(x_, w_, b_, what);
+  const NormShape s = norm_shape(x_, w_, b_, layout, what);
+  const Tensor view = layout == 1 ? x_.transpose(1, 2) : x_;
   int64_t n[2], st[3];
-  const bool strided = as_tokens(x_, s.H, n, st);
-  const Tensor x = strided ? x_ : x_.contiguous(), w = prep(w_), b = prep(b_), y = at::empty(x.sizes(), x.options());
-  const auto lead = x.sizes().slice(0, x.dim() - 1);
-  const Tensor mean = at::empty(lead, f32_on(x)), rstd = at::empty(lead, f32_on(x));
-  check_rc(xl_layer_norm_fwd(ptr(x), strided ? st : nullptr, ptr(w), ptr(b), ptr(y), ptr<float>(mean), ptr<float>(rstd),
+  const bool strided = as_tokens(view, layout != 0, n, st);
+  const Tensor x = strided ? view : view.contiguous(), w = prep(w_), b = prep(b_);
+  const Tensor y = layout ? at::empty({x.size(0), x.size(1), s.H * s.D}, x.options()) : at::empty(x.sizes(), x.options());
+  const Tensor stats = at::empty({2, s.tokens * s.H}, f32_on(x));
+  float* mean = ptr<float>(stats);
+  check_rc(xl_layer_norm_fwd(ptr(x), strided ? st : nullptr, ptr(w), ptr(b), ptr(y), mean, mean + s.tokens * s.H,
                              strided ? n[0] : 1, strided ? n[1] : s.tokens, i32(s.H, what), i32(s.D, what), (float)eps,
                              dtype_code(x, what), s.param, gpu.st),
            what);
-  return {y, mean, rstd};
+  return {y, stats};
 }
 
-std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& mean_,
-                                                  const Tensor& rstd_, const OptTensor& w_, const OptTensor& b_,
+std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy_, const Tensor& x_, const Tensor& stats_,
+                                                  const OptTensor& w_, const OptTensor& b_, int64_t layout,
                                                   std::array<bool, 3> mask) {
   const char* what = "layer_norm_bwd";
-  Gpu gpu(what, {&dy_, &x_, &mean_, &rstd_, opt(w_), opt(b_)});
-  const NormShape s = norm_shape(x_, w_, b_, what);
-  XL_CHECK(dy_.sizes() == x_.sizes(), what, "dy must have x's shape, got ", dy_.sizes());
-  const auto lead = x_.sizes().slice(0, x_.dim() - 1);
-  for (const Tensor* t : {&mean_, &rstd_})
-    XL_CHECK(t->sizes() == lead && t->scalar_type() == at::kFloat, what, "mean and rstd must be float32 of shape ", lead);
+  Gpu gpu(what, {&dy_, &x_, &stats_, opt(w_), opt(b_)});
+  const NormShape s = norm_shape(x_, w_, b_, layout, what);
+  const Tensor view = layout == 1 ? x_.transpose(1, 2) : x_;
+  const bool fits = layout ? dy_.sizes() == at::IntArrayRef({view.size(0), view.size(1), s.H * s.D}) : dy_.sizes() == x_.sizes();
+  XL_CHECK(fits, what, "dy must have the output's shape, got ", dy_.sizes());
+  XL_CHECK(stats_.sizes() == at::IntArrayRef({2, s.tokens * s.H}) && stats_.scalar_type() == at::kFloat, what,
+           "the statistics must be float32 (2, ", s.tokens * s.H, "), got ", stats_.sizes());
   int64_t n[2], st[3], dn[2], dst[3];
-  const bool strided = as_tokens(x_, s.H, n, st);
-  const Tensor x = strided ? x_ : x_.contiguous(), w = prep(w_), mean = mean_.contiguous(), rstd = rstd_.contiguous();
+  const bool strided = as_tokens(view, layout != 0, n, st);
+  const Tensor x = strided ? view : view.contiguous(), w = prep(w_), stats = stats_.contiguous();
   const Tensor dy = (dy_.scalar_type() == x.scalar_type() ? dy_ : dy_.to(x.scalar_type())).contiguous();
-  const Tensor none = at::empty({0}, x.options());
+  const bool want_w = mask[1] && opt(w_), want_b = mask[2] && opt(b_);
+  auto given_or_empty = [&](bool want, const OptTensor& t) {
+    return want ? at::empty(t->sizes(), t->options()) : at::empty({0}, x.options());
+  };
   // dx lies as x does where its tokens then fold as x's do: behind the chunkwise kernel it is [B, NH, S, DH] in memory
-  Tensor dx = none;
+  Tensor dx;
   bool dx_strided = false;
   if (mask[0]) {
     dx = at::empty_like(x_);
-    dx_strided = strided && as_tokens(dx, s.H, dn, dst) && dn[0] == n[0] && dn[1] == n[1];
-    if (!dx_strided) dx = at::empty(x_.sizes(), x_.options());
+    dx_strided = strided && as_tokens(layout == 1 ? dx.transpose(1, 2) : dx, layout != 0, dn, dst) && dn[0] == n[0] &&
+                 dn[1] == n[1];
+    if (!dx_strided) {
+      dx = at::empty(view.sizes(), x_.options());
+      if (layout == 1) dx = dx.transpose(1, 2);
+    }
+  } else {
+    dx = at::empty({0}, x.options());
   }
-  const Tensor dw = mask[1] && opt(w_) ? at::empty(w_->sizes(), w_->options()) : at::empty({0}, x.options());
-  const Tensor db = mask[2] && opt(b_) ? at::empty(b_->sizes(), b_->options()) : at::empty({0}, x.options());
-  const bool want_w = mask[1] && opt(w_), want_b = mask[2] && opt(b_);
+  const Tensor dw = given_or_empty(want_w, w_), db = given_or_empty(want_b, b_);
   const int64_t n0 = strided ? n[0] : 1, n1 = strided ? n[1] : s.tokens;
-  const int H = i32(s.H, what), D = i32(s.D, what);
-  const size_t ws_bytes = want_w || want_b ? xl_layer_norm_bwd_workspace_size(n0, n1, H, D) : 0;
+  const int H = i32(s.H, what), D = i32(s.D, what), dt = dtype_code(x, what);
+  const size_t ws_bytes = want_w || want_b ? xl_layer_norm_bwd_workspace_size(n0, n1, H, D, dt) : 0;
   const Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, x.options().dtype(at::kByte)) : Tensor();
-  check_rc(xl_layer_norm_bwd(ptr(dy), ptr(x), strided ? st : nullptr, ptr(w), ptr<float>(mean), ptr<float>(rstd),
+  const float* mean = ptr<float>(stats);
+  check_rc(xl_layer_norm_bwd(ptr(dy), ptr(x), strided ? st : nullptr, ptr(w), mean, mean + s.tokens * s.H,
                              mask[0] ? ptr(dx) : nullptr, dx_strided ? dst : nullptr, want_w ? ptr(dw) : nullptr,
-                             want_b ? ptr(db) : nullptr, n0, n1, H, D, dtype_code(x, what), s.param, ptr(ws), ws_bytes,
-                             gpu.st),
+                             want_b ? ptr(db) : nullptr, n0, n1, H, D, dt, s.param, ptr(ws), ws_bytes, gpu.st),
            what);
   return {dx, dw, db};
 }
 
-using ThreeTensors = std::tuple<Tensor, Tensor, Tensor>;
+using TwoTensors = std::tuple<Tensor, Tensor>;
+using CallLayerNorm = TwoTensors(const Tensor&, const OptTensor&, const OptTensor&, double, c10::SymInt);
+using LayerNormBwd = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                                                        const OptTensor&, c10::SymInt, std::array<bool, 3>);
 
-ThreeTensors call_layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
-  static const auto op =
-      c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::layer_norm", "").typed<decltype(layer_norm)>();
+TwoTensors call_layer_norm(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, c10::SymInt layout) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::layer_norm", "").typed<CallLayerNorm>();
   at::AutoDispatchBelowADInplaceOrView below;
-  return op.call(x, w, b, eps);
+  return op.call(x, w, b, eps, layout);
 }
 
-// Gradients of y; mean and rstd are not differentiable.
+// Gradients of y; the statistics are not differentiable.
 struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
   static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const OptTensor& w,
-                                                const OptTensor& b, double eps) {
-    auto [y, mean, rstd] = call_layer_norm(x, w, b, eps);
-    ctx->save_for_backward({x, w.value_or(Tensor()), b.value_or(Tensor()), mean, rstd});
-    ctx->mark_non_differentiable({mean, rstd});
+                                                const OptTensor& b, double eps, c10::SymInt layout) {
+    auto [y, stats] = call_layer_norm(x, w, b, eps, layout);
+    ctx->save_for_backward({x, w.value_or(Tensor()), b.value_or(Tensor()), stats});
+    ctx->saved_data["layout"] = layout;
+    ctx->mark_non_differentiable({stats});
     ctx->set_materialize_grads(false);
-    return {y, mean, rstd};
+    return {y, stats};
   }
 
   static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
                                                  torch::autograd::variable_list grads) {
-    static const auto bwd = c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::layer_norm_bwd", "")
-                                .typed<decltype(layer_norm_bwd)>();
+    static const auto bwd =
+        c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::layer_norm_bwd", "").typed<LayerNormBwd>();
     const Tensor none;
-    if (!grads[0].defined()) return {none, none, none, none};
+    if (!grads[0].defined()) return {none, none, none, none, none};
     const auto saved = ctx->get_saved_variables();
     auto given = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
     std::array<bool, 3> mask = {};
     for (size_t i = 0, edge = 0; i < 3; ++i)  // an argument left out has no edge
       if (saved[i].defined()) mask[i] = ctx->needs_input_grad(edge++);
-    auto [dx, dw, db] = bwd.call(grads[0], saved[0], saved[3], saved[4], given(saved[1]), given(saved[2]), mask);
-    return {mask[0] ? dx : none, mask[1] ? dw : none, mask[2] ? db : none, none};
+    auto [dx, dw, db] = bwd.call(grads[0], saved[0], saved[3], given(saved[1]), given(saved[2]),
+                                 ctx->saved_data["layout"].toSymInt(), mask);
+    return {mask[0] ? dx : none, mask[1] ? dw : none, mask[2] ? db : none, none, none};
   }
 };
 
-ThreeTensors layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps) {
+TwoTensors layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, c10::SymInt layout) {
   bool any = false;
   for (const Tensor* t : {&x, opt(w), opt(b)})
     any = any || (t && t->defined() && (t->requires_grad() || t->_fw_grad(0).defined()));
-  if (!any) return call_layer_norm(x, w, b, eps);
-  const auto r = LayerNormFn::apply(x, w, b, eps);
-  return {r[0], r[1], r[2]};
+  if (!any) return call_layer_norm(x, w, b, eps, layout);
+  const auto r = LayerNormFn::apply(x, w, b, eps, layout);
+  return {r[0], r[1]};
 }
 
 // The operators that write an argument, under autograd's bookkeeping, on fake tensors as on real ones.  What they

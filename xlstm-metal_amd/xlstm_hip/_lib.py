@@ -56,7 +56,7 @@ SIGNATURES = {
     "xl_add_rmsnorm_fwd": (_i, [_vp] * 5 + [_i, _i, _f] + [_fp, _fp, _i] * 2 + [_i, _vp]),
     "xl_silu_mul_fwd": (_i, [_vp] * 3 + [_i64, _i, _vp]),
     "xl_layer_norm_fwd": (_i, [_vp, ctypes.POINTER(_i64)] + [_vp] * 3 + [_fp] * 2 + [_i64] * 2 + [_i] * 2 + [_f, _i, _i, _vp]),
-    "xl_layer_norm_bwd_workspace_size": (_sz, [_i64] * 2 + [_i] * 2),
+    "xl_layer_norm_bwd_workspace_size": (_sz, [_i64] * 2 + [_i] * 3),
     "xl_layer_norm_bwd": (_i, [_vp] * 2 + [ctypes.POINTER(_i64), _vp] + [_fp] * 2 + [_vp, ctypes.POINTER(_i64)] + [_vp] * 2
                           + [_i64] * 2 + [_i] * 4 + [_vp, _sz, _vp]),
 }

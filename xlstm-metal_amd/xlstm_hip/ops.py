@@ -69,11 +69,11 @@ _SCHEMAS = {
                    "copy_dst) -> (Tensor, Tensor)"),
     # silu(gate) * up, the SiLU rounded to the dtype first (bf16 / f16)
     "silu_mul": ("(Tensor gate, Tensor up) -> Tensor"),
-    # (y, mean, rstd) of the norm over the last axis; weight and bias have the last axis' shape, or the last
-    # two axes' (a norm's weights for each head)
-    "layer_norm": ("(Tensor x, Tensor? weight, Tensor? bias, float eps) -> (Tensor, Tensor, Tensor)"),
+    # (y, statistics): layout 0, the norm over the last axis; 1 and 2, of each head of [B, NH, S, DH] or
+    # [B, S, NH, DH], written [B, S, NH * DH]; statistics float32 [2, rows], means and 1 / sqrt(var + eps)
+    "layer_norm": ("(Tensor x, Tensor? weight, Tensor? bias, float eps, SymInt layout) -> (Tensor, Tensor)"),
     # (dx, dweight, dbias); what the mask leaves out is an empty placeholder
-    "layer_norm_bwd": ("(Tensor dy, Tensor x, Tensor mean, Tensor rstd, Tensor? weight, Tensor? bias, bool[3] "
+    "layer_norm_bwd": ("(Tensor dy, Tensor x, Tensor stats, Tensor? weight, Tensor? bias, SymInt layout, bool[3] "
                       "output_mask) -> (Tensor, Tensor, Tensor)"),
 }
 
@@ -220,13 +220,17 @@ def _(gate, up):
 
 
 @_fake("layer_norm")
-def _(x, weight, bias, eps):
-    stats = tuple(x.new_empty(x.shape[:-1], dtype=torch.float32) for _ in range(2))
-    return (torch.empty_like(x, memory_format=torch.contiguous_format),) + stats
+def _(x, weight, bias, eps, layout):
+    if layout == 0:
+        y = torch.empty_like(x, memory_format=torch.contiguous_format)
+    else:
+        B, NH, S, DH = x.shape if layout == 1 else (x.shape[0], x.shape[2], x.shape[1], x.shape[3])
+        y = x.new_empty((B, S, NH * DH))
+    return y, x.new_empty((2, x.numel() // x.shape[-1]), dtype=torch.float32)
 
 
 @_fake("layer_norm_bwd")
-def _(dy, x, mean, rstd, weight, bias, output_mask):
+def _(dy, x, stats, weight, bias, layout, output_mask):
     dw, db = (torch.empty_like(t, memory_format=torch.contiguous_format) if t is not None and wanted
               else x.new_empty(_EMPTY_SHAPE) for t, wanted in zip((weight, bias), output_mask[1:]))
     return torch.empty_like(x) if output_mask[0] else x.new_empty(_EMPTY_SHAPE), dw, db
