@@ -800,6 +800,27 @@ TwoTensors layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTen
   return {r[0], r[1]};
 }
 
+// ------------------------------------------- Newton-Schulz orthogonalisation of [..., m, n]
+Tensor newton_schulz(const Tensor& x_, at::ArrayRef<double> coefficients, double eps) {
+  const char* what = "newton_schulz";
+  Gpu gpu(what, {&x_});
+  XL_CHECK(x_.dim() >= 2, what, "x must be a matrix or a batch of matrices, got ", x_.sizes());
+  XL_CHECK(!coefficients.empty() && coefficients.size() % 3 == 0, what, "coefficients are three for each step, got ",
+           coefficients.size());
+  const int dt = dtype_code(x_, what);
+  const std::vector<float> c(coefficients.begin(), coefficients.end());
+  const int m = i32(x_.size(-2), what), n = i32(x_.size(-1), what);
+  int64_t batch = 1;
+  for (int64_t d = 0; d + 2 < x_.dim(); ++d) batch *= x_.size(d);
+  const Tensor x = x_.contiguous(), y = like(x);
+  const size_t ws_bytes = xl_newton_schulz_workspace_size(batch, m, n, dt);
+  const Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, x.options().dtype(at::kByte)) : Tensor();
+  check_rc(xl_newton_schulz(ptr(x), ptr(y), batch, m, n, c.data(), (int)(c.size() / 3), (float)eps, dt, ptr(ws), ws_bytes,
+                            gpu.st),
+           what);
+  return y;
+}
+
 // The operators that write an argument, under autograd's bookkeeping, on fake tensors as on real ones.  What they
 // write is updated outside autograd, whatever it requires (a leaf too; its own history stays), a backward through
 // the outputs raises, and the written tensors' version counters move (inference tensors have none).
@@ -897,6 +918,7 @@ TORCH_LIBRARY_IMPL(xlstm_hip, CUDA, m) {
   m.impl("silu_mul", silu_mul);
   m.impl("layer_norm", layer_norm);
   m.impl("layer_norm_bwd", layer_norm_bwd);
+  m.impl("newton_schulz", newton_schulz);
 }
 
 // The chunkwise forward and the layer norm differentiate through their own backward; every other operator is
@@ -904,7 +926,8 @@ TORCH_LIBRARY_IMPL(xlstm_hip, CUDA, m) {
 #define XL_FORWARD_ONLY(m, kernel)                                                                                     \
   for (const char* op : {"soft_cap", "mlstm_step", "mlstm_chunkwise_bwd", "mlstm_sequence", "slstm_step",              \
                          "slstm_sequence", "causal_conv1d", "group_norm", "mh_rmsnorm_gate", "gate_proj_softcap",      \
-                         "gate_proj2_softcap", "lm_head_softcap", "rms_norm", "silu_mul", "layer_norm_bwd"})           \
+                         "gate_proj2_softcap", "lm_head_softcap", "rms_norm", "silu_mul", "layer_norm_bwd",             \
+                         "newton_schulz"})                                                                             \
     m.impl(op, kernel());
 TORCH_LIBRARY_IMPL(xlstm_hip, Autograd, m) {
   if (!abi_matches()) return;

@@ -21,6 +21,7 @@ from .mlstm_layers import (
     MultiHeadLayerNorm, MultiHeadRMSNorm, gate_proj_softcap, mh_rmsnorm_gate, mLSTMOutputCell, mLSTMProjectionCell,
 )
 from .norms import layer_norm, multi_head_layer_norm
+from .orthogonalise import newton_schulz
 from .recurrent import (
     mLSTMRecurrentKernelCell, mlstm_recurrent_sequence__native_fw, mlstm_recurrent_step_,
     mlstm_recurrent_step__native, mlstm_recurrent_step__native_fw,
@@ -46,7 +47,7 @@ __all__ = [
     "lm_head_softcap",
     "causal_conv1d", "group_norm", "CausalConv1d", "sLSTMProjectionCell", "sLSTMOutputCell",
     "mh_rmsnorm_gate", "MultiHeadRMSNorm", "MultiHeadLayerNorm", "mLSTMOutputCell", "gate_proj_softcap",
-    "mLSTMProjectionCell", "layer_norm", "multi_head_layer_norm",
+    "mLSTMProjectionCell", "layer_norm", "multi_head_layer_norm", "newton_schulz",
     "get_mlstm_kernel", "get_mlstm_step_kernel", "get_mlstm_sequence_kernel", "available_kernels",
     "wrap_chunkwise__arbitrary_sequence_length", "wrap_chunkwise__pad_zeros", "mLSTMBackendConfig",
     "mLSTMBackend", "load_library", "LIB_PATH",

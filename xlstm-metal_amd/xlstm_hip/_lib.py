@@ -59,6 +59,8 @@ SIGNATURES = {
     "xl_layer_norm_bwd_workspace_size": (_sz, [_i64] * 2 + [_i] * 3),
     "xl_layer_norm_bwd": (_i, [_vp] * 2 + [ctypes.POINTER(_i64), _vp] + [_fp] * 2 + [_vp, ctypes.POINTER(_i64)] + [_vp] * 2
                           + [_i64] * 2 + [_i] * 4 + [_vp, _sz, _vp]),
+    "xl_newton_schulz_workspace_size": (_sz, [_i64] + [_i] * 3),
+    "xl_newton_schulz": (_i, [_vp] * 2 + [_i64, _i, _i, ctypes.POINTER(_f), _i, _f, _i, _vp, _sz, _vp]),
 }
 
 ABI_VERSION = 3

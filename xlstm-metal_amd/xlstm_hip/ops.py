@@ -22,7 +22,7 @@ __all__ = [
     "soft_cap_op", "mlstm_step_op", "mlstm_step_inplace_op", "mlstm_chunkwise_op", "mlstm_chunkwise_bwd_op", "mlstm_sequence_op",
     "slstm_step_op", "slstm_sequence_op", "causal_conv1d_op", "group_norm_op", "mh_rmsnorm_gate_op",
     "gate_proj_softcap_op", "gate_proj2_softcap_op", "lm_head_softcap_op", "rms_norm_op", "add_rmsnorm_op", "silu_mul_op",
-    "layer_norm_op",
+    "layer_norm_op", "newton_schulz_op",
     "chunkwise_workspace_bytes", "chunkwise_algorithm",
 ]
 
@@ -75,6 +75,8 @@ _SCHEMAS = {
     # (dx, dweight, dbias); what the mask leaves out is an empty placeholder
     "layer_norm_bwd": ("(Tensor dy, Tensor x, Tensor stats, Tensor? weight, Tensor? bias, SymInt layout, bool[3] "
                       "output_mask) -> (Tensor, Tensor, Tensor)"),
+    # coefficients: a, b, c of each step
+    "newton_schulz": ("(Tensor x, float[] coefficients, float eps) -> Tensor"),
 }
 
 _library = torch.library.Library("xlstm_hip", "DEF")
@@ -236,6 +238,11 @@ def _(dy, x, stats, weight, bias, layout, output_mask):
     return torch.empty_like(x) if output_mask[0] else x.new_empty(_EMPTY_SHAPE), dw, db
 
 
+@_fake("newton_schulz")
+def _(x, coefficients, eps):
+    return torch.empty_like(x, memory_format=torch.contiguous_format)
+
+
 soft_cap_op = torch.ops.xlstm_hip.soft_cap.default
 mlstm_step_op = torch.ops.xlstm_hip.mlstm_step.default
 mlstm_step_inplace_op = torch.ops.xlstm_hip.mlstm_step_.default
@@ -252,6 +259,7 @@ rms_norm_op = torch.ops.xlstm_hip.rms_norm.default
 add_rmsnorm_op = torch.ops.xlstm_hip.add_rmsnorm.default
 silu_mul_op = torch.ops.xlstm_hip.silu_mul.default
 layer_norm_op = torch.ops.xlstm_hip.layer_norm.default
+newton_schulz_op = torch.ops.xlstm_hip.newton_schulz.default
 
 CONV_ACTS = {None: 0, "silu": 1}
 # csrc/torch_ops.cpp's own (0 where no kernel can run): the most rows of lm_head_softcap and the LDS of its
