@@ -9,9 +9,9 @@
 // hi + lo of f16 (22 bits) and a product three (hi hi + hi lo + lo hi), 4e-7 of the norm.
 //
 // A and P are symmetric: their tiles on and below the diagonal are computed and written to both places.  X is kept
-// as X and X^T, so that all three products have both operands' sums along contiguous rows (X X^T, A A, P (X^T)^T).
-// All matrices are zero-padded to whole tiles in the workspace: no bounds in the loops, and products of zeros stay
-// zero.
+// by rows; P X reads it down its columns with LDS reads that transpose.  All matrices are zero-padded to multiples of
+// 64 in the workspace, and a tile past the end reads its last rows again: no bounds in the loops, and products of
+// zeros stay zero.
 #include <math.h>
 
 #include <type_traits>
@@ -26,30 +26,68 @@ typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef u32x4 u32x4_at2 __attribute__((aligned(2)));
+typedef u32x4 u32x4_at4 __attribute__((aligned(4)));
+template <typename T>
+using raw_at = std::conditional_t<sizeof(T) == 2, u32x4_at2, u32x4_at4>;
+template <typename T>
+struct Vec {  // 16 bytes, at any element's address
+  T e[16 / sizeof(T)];
+};
+template <typename T>
+__device__ __forceinline__ Vec<T> load_vec(const T* p) {
+  const u32x4 raw = *(const raw_at<T>*)p;
+  return __builtin_bit_cast(Vec<T>, raw);
+}
 typedef __attribute__((address_space(3))) char lds_char;
 
 // stored = value * scale: with |singular values| of X up to 8 (checked on the host), |A| <= 64 and |P| <= 250
 constexpr float SCALE_X = 256.f, SCALE_A = 256.f, SCALE_P = 64.f;
+#ifndef CFG
+#define CFG 128
+#endif
 constexpr float MOST_X = 8.f, MOST_P = 250.f;
 
 // ------------------------------------------------------------------------------------------------ norm and first X
-constexpr int NORM_BLOCK = 256, NORM_PARTS = 256;  // partial sums per matrix
+constexpr int NORM_BLOCK = 512, NORM_PARTS = 256;  // most partial sums of a matrix
 
 template <typename T>
 __global__ __launch_bounds__(NORM_BLOCK) void ns_norm_kernel(const T* __restrict__ g, int64_t count, int parts,
                                                              double* __restrict__ part) {
+  constexpr int VW = 16 / sizeof(T), AHEAD = 4;
   __shared__ double sums[NORM_BLOCK / 64];
   const T* p = g + blockIdx.y * count;
+  const int64_t whole = count / VW, step = (int64_t)parts * NORM_BLOCK, at = (int64_t)blockIdx.x * NORM_BLOCK + threadIdx.x;
   double s = 0.0;  // no float32 value's square overflows it
-  for (int64_t i = (int64_t)blockIdx.x * NORM_BLOCK + threadIdx.x; i < count; i += (int64_t)parts * NORM_BLOCK) {
-    const double v = (double)to_f32(p[i]);
+  auto add = [&](float f) {
+    const double v = (double)f;
     s = fma(v, v, s);
+  };
+  int64_t i = at;
+  for (; i + (AHEAD - 1) * step < whole; i += AHEAD * step) {
+    Vec<T> v[AHEAD];
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u) v[u] = load_vec(p + (i + u * step) * VW);
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+      for (int j = 0; j < VW; ++j) add(to_f32(v[u].e[j]));
   }
+  for (; i < whole; i += step) {
+    const Vec<T> v = load_vec(p + i * VW);
+#pragma unroll
+    for (int j = 0; j < VW; ++j) add(to_f32(v.e[j]));
+  }
+  if (at < count - whole * VW) add(to_f32(p[whole * VW + at]));
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = s;
   __syncthreads();
-  if (threadIdx.x == 0) part[(int64_t)blockIdx.y * parts + blockIdx.x] = sums[0] + sums[1] + sums[2] + sums[3];
+  if (threadIdx.x != 0) return;
+  s = 0.0;
+#pragma unroll
+  for (int w = 0; w < NORM_BLOCK / 64; ++w) s += sums[w];
+  part[(int64_t)blockIdx.y * parts + blockIdx.x] = s;
 }
 
 // A matrix's factors: X0 = stored * first, later X = stored * later.
@@ -78,13 +116,26 @@ __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
   lo = (_Float16)(v - (float)hi);
 }
 
-// G [R, C] into `same` [Rp, Cp] and `turned` [Cp, Rp] (f16 planes, zero past G), 64 x 64 a workgroup
-template <typename T, int PL>
-__global__ __launch_bounds__(256) void ns_enter_kernel(const T* __restrict__ g, int R, int C, int Rp, int Cp,
+__device__ __forceinline__ void store_planes(f16_t* to, int64_t lo_plane, bool with_lo, const float (&v)[8]) {
+  f16x8 hi, lo;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    _Float16 h, l;
+    split(v[q], h, l);
+    hi[q] = h;
+    lo[q] = l;
+  }
+  *(f16x8*)to = hi;
+  if (with_lo) *(f16x8*)(to + lo_plane) = lo;
+}
+
+// X [Mp, Np] (f16 planes, zero past the matrix) from G [M, N], or from G [N, M] (TALL); 64 x 64 a workgroup
+template <typename T, int PL, bool TALL>
+__global__ __launch_bounds__(256) void ns_enter_kernel(const T* __restrict__ g, int M, int N, int Mp, int Np,
                                                        const double* __restrict__ part, int parts, double eps,
-                                                       double growth, f16_t* __restrict__ same, int64_t same_plane,
-                                                       f16_t* __restrict__ turned, int64_t turned_plane,
+                                                       double growth, f16_t* __restrict__ x, int64_t x_plane,
                                                        Factors* __restrict__ factors) {
+  constexpr int VW = 16 / sizeof(T);
   __shared__ float tile[64][65];
   __shared__ double sums[4];
   const int tid = threadIdx.x, b = blockIdx.z;
@@ -96,34 +147,44 @@ __global__ __launch_bounds__(256) void ns_enter_kernel(const T* __restrict__ g, 
   double enter;
   const Factors f = factors_of(sqrt(sums[0] + sums[1] + sums[2] + sums[3]), eps, growth, enter);
   if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) factors[b] = f;
-  const int r0 = blockIdx.y * 64, c0 = blockIdx.x * 64, x = tid & 63, y = tid >> 6;
-  const T* gp = g + (int64_t)b * R * C;
-  const int64_t at = (int64_t)b * Rp * Cp;
+  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, R = TALL ? N : M, C = TALL ? M : N;
+  const int r0 = TALL ? n0 : m0, c0 = TALL ? m0 : n0;
+  const T* gp = g + (int64_t)b * M * N;
+  f16_t* xp = x + (int64_t)b * Mp * Np;
+  const int r = tid >> 2, c = (tid & 3) * 16;  // 16 values of one row of G's tile, and of X's
+  float v[16];
+  const T* from = gp + (int64_t)(r0 + r) * C + c0 + c;
+  if (r0 + r < R && c0 + c + 16 <= C) {
 #pragma unroll
-  for (int i = 0; i < 64; i += 4) {
-    const int r = r0 + i + y, c = c0 + x;
-    const float v = r < R && c < C ? (float)((double)to_f32(gp[(int64_t)r * C + c]) * enter) : 0.f;
-    tile[i + y][x] = v;
-    _Float16 hi, lo;
-    split(v, hi, lo);
-    same[at + (int64_t)r * Cp + c] = hi;
-    if constexpr (PL == 2) same[same_plane + at + (int64_t)r * Cp + c] = lo;
+    for (int q = 0; q < 16; q += VW) {
+      const Vec<T> u = load_vec(from + q);
+#pragma unroll
+      for (int j = 0; j < VW; ++j) v[q + j] = to_f32(u.e[j]);
+    }
+  } else {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) v[q] = r0 + r < R && c0 + c + q < C ? to_f32(from[q]) : 0.f;
   }
-  __syncthreads();
 #pragma unroll
-  for (int i = 0; i < 64; i += 4) {
-    _Float16 hi, lo;
-    split(tile[x][i + y], hi, lo);
-    const int64_t to = at + (int64_t)(c0 + i + y) * Rp + r0 + x;
-    turned[to] = hi;
-    if constexpr (PL == 2) turned[turned_plane + to] = lo;
+  for (int q = 0; q < 16; ++q) v[q] = (float)((double)v[q] * enter);
+  if constexpr (TALL) {
+#pragma unroll
+    for (int q = 0; q < 16; ++q) tile[r][c + q] = v[q];
+    __syncthreads();
+#pragma unroll
+    for (int q = 0; q < 16; ++q) v[q] = tile[c + q][r];
+  }
+#pragma unroll
+  for (int q = 0; q < 16; q += 8) {
+    const float half[8] = {v[q], v[q + 1], v[q + 2], v[q + 3], v[q + 4], v[q + 5], v[q + 6], v[q + 7]};
+    store_planes(xp + (int64_t)(m0 + r) * Np + n0 + c + q, x_plane, PL == 2, half);
   }
 }
 
 // ------------------------------------------------------------------------------------------------ the products
 // 16 bytes a lane from global memory into LDS, at lds + 16 * lane (lds the same in the whole wave)
 __device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const void* base) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory", "m0");
+  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -131,125 +192,174 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-enum Product { XXT, AA, PX, LAST };  // A; P; X and X^T; the result
+enum Product { XXT, AA, PX, LAST };  // A; P; X; the result
 
+// sum[l][r] over k of left[l][k] right[r][k]
 struct Args {
-  // left [tm BM, K] and right [tn BN, K], planes hi and (plane elements on) lo
+  // left [lefts, K] by rows (A, X), or X [K, lefts] by columns (PX, LAST); right [rights, K]; planes hi, and lo a plane on
   const f16_t *left, *right;
   int64_t left_plane, right_plane, left_batch, right_batch;
-  int K, tm, tn;
-  // value = beta * e + alpha * sum; e transposed, [tn BN, tm BM], of e_planes
+  int lefts, rights, K;     // multiples of 64
+  int left_tiles, right_tiles;
+  // value = beta * e + alpha * sum; e as out
   const f16_t* e;
   int64_t e_plane, e_batch;
   int e_planes;
   float alpha, beta;
   const Factors* factors;
   bool first;
-  // out [tm BM, tn BN] and turned [tn BN, tm BM], with out_planes and turned_planes
-  f16_t *out, *turned;
-  int64_t out_plane, turned_plane, out_batch, turned_batch;
-  int out_planes, turned_planes;
-  // LAST: the result, [rows, cols], or [cols, rows] where it is turned
+  // out [rights, lefts] (A, P: [lefts, rights] too, which is the other triangle)
+  f16_t* out;
+  int64_t out_plane, out_batch;
+  int out_planes;
+  // LAST: the result [rows, cols] of X's own shape, or its transpose
   void* result;
   int rows, cols;
   bool result_turned;
 };
 
-// One workgroup a tile of BM x BN, WM x WN waves, the sums in registers (16 x 16 blocks of v_mfma_f32_16x16x32_f16).
-// Slices of 64 of both operands are in LDS twice: the next one is on its way (straight from memory, no registers)
-// while this one is multiplied; one barrier a slice.  A row's 8 pieces of 16 bytes lie at piece ^ (row % 8), so that the
-// rows that the matrix cores' lanes read together fall on different banks; as the loads write LDS in lane order,
-// each lane fetches the piece that belongs at its place.
-template <int BM, int BN, int WM, int WN, int PL, int MODE, typename T>
-__global__ __launch_bounds__(64 * WM * WN) void ns_product_kernel(Args p) {
-  constexpr int THREADS = 64 * WM * WN, BK = 64, TM = BM / WM / 16, TN = BN / WN / 16;
-  constexpr int STAGE = (BM + BN) * BK * 2 * PL, PER = THREADS / 8;  // rows by one load of the workgroup
-  constexpr int STRIP = 16 * (TN * 16 + 4) * 4;
-  constexpr int LDS = 2 * STAGE > WM * WN * STRIP ? 2 * STAGE : WM * WN * STRIP;
-  static_assert(BM % PER == 0 && BN % PER == 0);
+// One workgroup a tile of BL x BR, WL x WR waves, the sums in registers (16 x 16 blocks of v_mfma_f32_16x16x32_f16).
+// Slices of 64 of both operands lie in LDS, STAGES of them, filled straight from memory (no registers) STAGES - 1 slices
+// ahead.  A wave holds the operands of 32 of a slice's 64 and multiplies them while it reads those of the next 32, so
+// LDS and the matrix cores work at once; one barrier a slice.
+//
+// LDS, an operand by rows: [row][8 pieces of 16 bytes], piece p at p ^ (row % 8): the 8 rows that are read together fall
+// on different banks.  X by columns: [k][pieces of 32 bytes = 16 columns], piece p at p ^ key(k), likewise for the 4 + 4
+// rows k of a transposing read.  The loads write LDS in lane order, so each lane fetches what belongs at its place.
+template <int BL, int BR, int WL, int WR, int STAGES, int PL, int MODE, typename T>
+__global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
+  constexpr int THREADS = 64 * WL * WR, BK = 64, TL = BL / WL / 16, TR = BR / WR / 16;
+  constexpr bool SYM = MODE == XXT || MODE == AA, COLUMNS = !SYM;  // left by columns
+  constexpr int PLANE = (BL + BR) * 128, STAGE = PLANE * PL;
+  constexpr int PER = THREADS / 8;         // rows of 128 bytes by one load of the workgroup
+  constexpr int PER_K = THREADS * 8 / BL;  // rows k of BL columns by one
+  constexpr int LOADS_L = BL / PER, LOADS_P = LOADS_L + BR / PER, LOADS = LOADS_P * PL, READS = PL * (TL + TR);
+  static_assert(BL % PER == 0 && BR % PER == 0 && (!COLUMNS || PER_K % 16 == 0) && LOADS * (STAGES - 2) < 64);
   extern __shared__ __align__(1024) char lds[];
-  static_assert(LDS <= 160 * 1024);
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int wm = wave / WN, wn = wave % WN;
-  constexpr bool SYM = MODE == XXT || MODE == AA;
+  const int wl = wave / WR, wr = wave % WR;
 
-  // neighbours share rows and columns of tiles, on one XCD
-  const int t = mfma::xcd_contiguous(blockIdx.x, gridDim.x), b = blockIdx.y;
-  int bi, bj;
+  // neighbours share operands, on one XCD
+  const int tiles = SYM ? p.left_tiles * (p.left_tiles + 1) / 2 : p.left_tiles * p.right_tiles;
+  const int g = mfma::xcd_contiguous(blockIdx.x, gridDim.x), b = __builtin_amdgcn_readfirstlane(g / tiles), t = g - b * tiles;
+  int bl, br;
   if constexpr (SYM) {
-    bi = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
-    while ((bi + 1) * (bi + 2) / 2 <= t) ++bi;
-    while (bi * (bi + 1) / 2 > t) --bi;
-    bj = t - bi * (bi + 1) / 2;
+    bl = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
+    while ((bl + 1) * (bl + 2) / 2 <= t) ++bl;
+    while (bl * (bl + 1) / 2 > t) --bl;
+    br = t - bl * (bl + 1) / 2;
   } else {
     constexpr int G = 4;
-    const int group = t / (G * p.tn), rows = min(G, p.tm - group * G), in = t - group * G * p.tn;
-    bi = group * G + in % rows;
-    bj = in / rows;
+    const int group = t / (G * p.left_tiles), rows = min(G, p.right_tiles - group * G), in = t - group * G * p.left_tiles;
+    br = group * G + in % rows;
+    bl = in / rows;
   }
-  bi = __builtin_amdgcn_readfirstlane(bi);
-  bj = __builtin_amdgcn_readfirstlane(bj);
+  bl = __builtin_amdgcn_readfirstlane(bl);
+  br = __builtin_amdgcn_readfirstlane(br);
 
-  const int64_t ld = (int64_t)p.K * 2;
-  const uint32_t offset = (uint32_t)((tid >> 3) * ld) + (uint32_t)(((tid & 7) ^ ((tid >> 3) & 7)) * 16);
-  const char *lp = (const char*)(p.left + b * p.left_batch) + bi * BM * ld,
-             *rp = (const char*)(p.right + b * p.right_batch) + bj * BN * ld;
-  const uint32_t at = (uint32_t)(uintptr_t)(lds_char*)lds + wave * 1024;
-  auto fetch = [&](int k, int stage) {
-    uint32_t to = at + stage * STAGE;
+  // where this lane's loads come from: byte offsets from the operands' first slice
+  const int64_t ld = (int64_t)p.K * 2, ldx = (int64_t)p.lefts * 2;
+  const int piece = ((tid & 7) ^ ((tid >> 3) & 7)) * 16;
+  constexpr int PIECES = BL / 8, KEYS = BL >= 128 ? 7 : 3;  // 16-byte pieces of a row k; the key's bits
+  uint32_t from_l[LOADS_L], from_r[BR / PER];
+  const char *lp = (const char*)(p.left + b * p.left_batch), *rp = (const char*)(p.right + b * p.right_batch) + br * BR * ld;
+  if constexpr (COLUMNS) {
+    const int k = tid / PIECES, at = tid % PIECES, key = ((k & 3) | ((k >> 1) & 4)) & KEYS;
+    const int column = bl * BL + ((((at >> 1) ^ key) << 1) | (at & 1)) * 8;
+    from_l[0] = (uint32_t)(k * ldx + min(column, p.lefts - 8) * 2);
+  } else {
+    lp += bl * BL * ld;
 #pragma unroll
-    for (int pl = 0; pl < PL; ++pl) {
+    for (int i = 0; i < LOADS_L; ++i)
+      from_l[i] = (uint32_t)(min(i * PER + (tid >> 3), p.lefts - 1 - bl * BL) * ld + piece);
+  }
 #pragma unroll
-      for (int i = 0; i < BM / PER; ++i, to += PER * 128)
-        to_lds(to, offset, lp + pl * p.left_plane * 2 + i * PER * ld + k * (BK * 2));
-#pragma unroll
-      for (int i = 0; i < BN / PER; ++i, to += PER * 128)
-        to_lds(to, offset, rp + pl * p.right_plane * 2 + i * PER * ld + k * (BK * 2));
-    }
+  for (int i = 0; i < BR / PER; ++i)
+    from_r[i] = (uint32_t)(min(i * PER + (tid >> 3), p.rights - 1 - br * BR) * ld + piece);
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds + wave * 1024;
+  auto fetch_one = [&](auto I, int k, int stage) {
+    constexpr int pl = I.value / LOADS_P, i = I.value % LOADS_P;
+    const uint32_t to = lds_at + stage * STAGE + I.value * (PER * 128);
+    if constexpr (i >= LOADS_L)
+      to_lds(to, from_r[i - LOADS_L], rp + pl * p.right_plane * 2 + k * (BK * 2));
+    else if constexpr (COLUMNS)
+      to_lds(to, from_l[0], lp + pl * p.left_plane * 2 + (int64_t)(k * BK + i * PER_K) * ldx);
+    else
+      to_lds(to, from_l[i], lp + pl * p.left_plane * 2 + k * (BK * 2));
   };
-  f32x4 acc[TM][TN];
+
+  f32x4 acc[TL][TR];
 #pragma unroll
-  for (int i = 0; i < TM; ++i)
+  for (int i = 0; i < TL; ++i)
 #pragma unroll
-    for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < TR; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
   const int row = lane & 15, quad = lane >> 4;
-  auto operand = [&](int base, int r, int s) {  // 8 values of row r, from 32 s + 8 quad
-    return *(const f16x8*)(lds + base + r * 128 + (((s * 4 + quad) ^ (r & 7)) << 4));
+  struct Half {  // a wave's operands of 32 of a slice's 64
+    f16x8 l[PL][TL], r[PL][TR];
   };
-  const int slices = p.K / BK;
-  fetch(0, 0);
-  for (int k = 0; k < slices; ++k) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");  // slice k is there, slice k - 1 has been read
+  const int by_row = row * 128 + ((quad ^ (row & 7)) << 4);
+  const int by_column = (quad * 8 + (row >> 2)) * (BL * 2) + ((((row >> 2) | ((quad & 1) << 2)) & KEYS) ^ (wl * TL)) * 32 + (row & 3) * 8;
+  // read I of half s of the slice at LDS offset `base`: 8 values along k, from 32 s + 8 quad, of a row or a column
+  auto read_one = [&](auto I, Half& h, int base, int s) {
+    constexpr int pl = I.value / (TL + TR), i = I.value % (TL + TR);
+    const char* plane = lds + base + pl * PLANE;
+    if constexpr (i >= TL) {
+      h.r[pl][i - TL] = *(const f16x8*)(plane + BL * 128 + (wr * TR + i - TL) * 2048 + (by_row ^ (s * 64)));
+    } else if constexpr (COLUMNS) {
+      const char* at = plane + s * (32 * BL * 2) + (by_column ^ (i * 32));
+      h.l[pl][i] = __builtin_bit_cast(f16x8, mfma::tr_pair(at, at + 4 * BL * 2));
+    } else {
+      h.l[pl][i] = *(const f16x8*)(plane + (wl * TL + i) * 2048 + (by_row ^ (s * 64)));
+    }
+  };
+  // one half's products, a row of blocks at a time, each with its share of the next half's reads and of `more`
+  auto multiply = [&](const Half& h, Half& next, int next_base, int next_s, auto&& more) {
+    mfma::static_for<0, TL>([&](auto I) {
+      constexpr int i = I.value;
+      mfma::static_for<READS * i / TL, READS * (i + 1) / TL>([&](auto R) { read_one(R, next, next_base, next_s); });
+      more(I);
+#pragma unroll
+      for (int j = 0; j < TR; ++j) {
+        if constexpr (PL == 2) {
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.l[1][i], h.r[0][j], acc[i][j], 0, 0, 0);
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.l[0][i], h.r[1][j], acc[i][j], 0, 0, 0);
+        }
+        acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.l[0][i], h.r[0][j], acc[i][j], 0, 0, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    });
+  };
+  // all but this wave's last LEFT loads are in LDS, and its reads done; then everybody's
+  auto landed = [&](auto LEFT) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(LEFT.value) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    if (k + 1 < slices) fetch(k + 1, (k + 1) & 1);
-    const int base = (k & 1) * STAGE;
+  };
+  // Past the end the last slice is loaded again, into a place that is not read: the same number of loads is under way
+  // after every slice.
+  const int slices = p.K / BK;
+  using Behind = std::integral_constant<int, LOADS*(STAGES - 2)>;
+  Half h0, h1;
 #pragma unroll
-    for (int s = 0; s < BK / 32; ++s) {
-      f16x8 l[PL][TM], r[PL][TN];
-#pragma unroll
-      for (int pl = 0; pl < PL; ++pl) {
-        const int at_plane = base + pl * (BM + BN) * 128;
-#pragma unroll
-        for (int i = 0; i < TM; ++i) l[pl][i] = operand(at_plane, (wm * TM + i) * 16 + row, s);
-#pragma unroll
-        for (int j = 0; j < TN; ++j) r[pl][j] = operand(at_plane + BM * 128, (wn * TN + j) * 16 + row, s);
-      }
-#pragma unroll
-      for (int i = 0; i < TM; ++i)
-#pragma unroll
-        for (int j = 0; j < TN; ++j) {
-          if constexpr (PL == 2) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[1][i], r[0][j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[1][j], acc[i][j], 0, 0, 0);
-          }
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0][i], r[0][j], acc[i][j], 0, 0, 0);
-        }
-    }
+  for (int k = 0; k < STAGES - 1; ++k)
+    mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(k, slices - 1), k); });
+  landed(Behind{});
+  mfma::static_for<0, READS>([&](auto R) { read_one(R, h0, 0, 0); });
+  mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(STAGES - 1, slices - 1), STAGES - 1); });
+  int stage = 0;
+  for (int k = 0; k < slices; ++k) {
+    const int next = stage + 1 == STAGES ? 0 : stage + 1, ahead = min(k + STAGES, slices - 1);
+    multiply(h0, h1, stage * STAGE, 1, [](auto) {});
+    landed(Behind{});  // slice k + 1 is there, slice k has been read
+    multiply(h1, h0, next * STAGE, 0, [&](auto I) {
+      mfma::static_for<LOADS * I.value / TL, LOADS * (I.value + 1) / TL>([&](auto L) { fetch_one(L, ahead, stage); });
+    });
+    stage = next;
   }
+  landed(std::integral_constant<int, 0>{});
 
-  // A lane has rows 4 quad .. 4 quad + 3 of column `row` of each block: four neighbours of a row of the transposed.
+  // A lane has left 4 quad .. 4 quad + 3 of right `row` of each block.
   const Factors f = p.factors[b];
   const float u = p.first ? f.first : f.later;
   float alpha = p.alpha, beta = p.beta;
@@ -262,104 +372,89 @@ __global__ __launch_bounds__(64 * WM * WN) void ns_product_kernel(Args p) {
     alpha *= u;
     beta *= u;
   }
-  const int m0 = bi * BM + wm * TM * 16, n0 = bj * BN + wn * TN * 16;
-  const int64_t ldt = (int64_t)p.tm * BM, ldo = (int64_t)p.tn * BN;
-  if constexpr (MODE != XXT) {
-    const f16_t* e = p.e + b * p.e_batch;
+  const int l0 = bl * BL + wl * TL * 16, r0 = br * BR + wr * TR * 16;
+  const f16_t* e = p.e + b * p.e_batch;
+  // 16 rows of [rows, 8 * EACH columns] at a time, turned in the wave's own part of LDS: 16 bytes a lane, whole lines
+  constexpr int WIDE = TL > TR ? TL : TR, STRIP = 16 * (WIDE * 16 + 4);
+  float* strip = (float*)lds + wave * STRIP;
+  auto out_rows = [&](auto BLOCKS, int row0, int rows, int col0, int cols, bool with_e) {
+    constexpr int EACH = BLOCKS.value * 2, LDW = BLOCKS.value * 16 + 4;
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+    for (int h = 0; h < (16 * EACH + 63) / 64; ++h) {
+      const int r = h * (64 / EACH) + lane / EACH, c = lane % EACH * 8, m = row0 + r, n = col0 + c;
+      if (r >= 16 || m >= rows || n >= cols) continue;
+      const f32x4 v0 = *(const f32x4*)(strip + r * LDW + c), v1 = *(const f32x4*)(strip + r * LDW + c + 4);
+      float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+      if (with_e) {
+        const int64_t from = (int64_t)m * cols + n;
+        const f16x8 hi = *(const f16x8*)(e + from);
+        f16x8 lo = {};
+        if (p.e_planes == 2) lo = *(const f16x8*)(e + p.e_plane + from);
 #pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int64_t from = (n0 + j * 16 + row) * ldt + m0 + i * 16 + quad * 4;
-        const f16x4 hi = *(const f16x4*)(e + from);
-        f16x4 lo = {};
-        if (p.e_planes == 2) lo = *(const f16x4*)(e + p.e_plane + from);
-#pragma unroll
-        for (int q = 0; q < 4; ++q) acc[i][j][q] = fmaf(beta, (float)hi[q] + (float)lo[q], alpha * acc[i][j][q]);
+        for (int q = 0; q < 8; ++q) v[q] = fmaf(beta, (float)hi[q] + (float)lo[q], v[q]);
       }
-  } else {
+      if constexpr (MODE == LAST) {
+        const int R = p.result_turned ? p.cols : p.rows, C = p.result_turned ? p.rows : p.cols;
+        if (m >= R || n >= C) continue;
+        T* to = (T*)p.result + (int64_t)b * R * C + (int64_t)m * C + n;
+        if (n + 8 <= C) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i)
+          for (int q = 0; q < 8; q += 16 / sizeof(T)) {
+            Vec<T> o;
 #pragma unroll
-      for (int j = 0; j < TN; ++j) acc[i][j] *= alpha;
-  }
-
-  const bool by_columns = MODE == LAST ? p.result_turned : true, by_rows = MODE == LAST ? !p.result_turned : true;
-  if (by_columns && !(SYM && bi == bj)) {
-#pragma unroll
-    for (int i = 0; i < TM; ++i)
-#pragma unroll
-      for (int j = 0; j < TN; ++j) {
-        const int n = n0 + j * 16 + row, m = m0 + i * 16 + quad * 4;
-        if constexpr (MODE == LAST) {
-          T* to = (T*)p.result + (int64_t)b * p.rows * p.cols + (int64_t)n * p.rows + m;
-          if (n < p.cols) {
-#pragma unroll
-            for (int q = 0; q < 4; ++q)
-              if (m + q < p.rows) to[q] = from_f32<T>(acc[i][j][q]);
+            for (int z = 0; z < 16 / (int)sizeof(T); ++z) o.e[z] = from_f32<T>(v[q + z]);
+            *(raw_at<T>*)(to + q) = __builtin_bit_cast(u32x4, o);
           }
         } else {
-          f16_t* to = p.turned + b * p.turned_batch + n * ldt + m;
-          f16x4 hi, lo;
 #pragma unroll
-          for (int q = 0; q < 4; ++q) {
-            _Float16 h, l;
-            split(acc[i][j][q], h, l);
-            hi[q] = h;
-            lo[q] = l;
-          }
-          *(f16x4*)to = hi;
-          if (p.turned_planes == 2) *(f16x4*)(to + p.turned_plane) = lo;
+          for (int q = 0; q < 8; ++q)
+            if (n + q < C) to[q] = from_f32<T>(v[q]);
         }
+      } else {
+        store_planes(p.out + b * p.out_batch + (int64_t)m * cols + n, p.out_plane, p.out_planes == 2, v);
       }
+    }
+  };
+  if (!(MODE == LAST && p.result_turned)) {
+#pragma unroll
+    for (int j = 0; j < TR; ++j) {
+      wave_fence();
+#pragma unroll
+      for (int i = 0; i < TL; ++i) *(f32x4*)(strip + row * (TL * 16 + 4) + i * 16 + quad * 4) = acc[i][j] * alpha;
+      wave_fence();
+      out_rows(std::integral_constant<int, TL>{}, r0 + j * 16, p.rights, l0, p.lefts, MODE != XXT);
+    }
   }
-  if (by_rows) {  // 16 rows at a time turned in the wave's own part of LDS
-    __syncthreads();
-    float* strip = (float*)(lds + wave * STRIP);
-    constexpr int LDW = TN * 16 + 4, EACH = TN * 16 / 8;  // 8 values a lane: EACH lanes a row
+  if ((SYM && bl != br) || (MODE == LAST && p.result_turned)) {
 #pragma unroll
-    for (int i = 0; i < TM; ++i) {
+    for (int i = 0; i < TL; ++i) {
       wave_fence();
 #pragma unroll
-      for (int j = 0; j < TN; ++j)
+      for (int j = 0; j < TR; ++j) {
+        f32x4 v = acc[i][j] * alpha;
+        const int l = l0 + i * 16 + quad * 4, r = r0 + j * 16 + row;
+        if (MODE == LAST && l < p.lefts && r < p.rights) {  // e lies the other way round
+          const int64_t from = (int64_t)r * p.lefts + l;
+          const f16x4 hi = *(const f16x4*)(e + from);
+          f16x4 lo = {};
+          if (p.e_planes == 2) lo = *(const f16x4*)(e + p.e_plane + from);
 #pragma unroll
-        for (int q = 0; q < 4; ++q) strip[(quad * 4 + q) * LDW + j * 16 + row] = acc[i][j][q];
-      wave_fence();
-#pragma unroll
-      for (int h = 0; h < 16 * EACH / 64; ++h) {
-        const int r = h * (64 / EACH) + lane / EACH, c = lane % EACH * 8;
-        const f32x4 v0 = *(const f32x4*)(strip + r * LDW + c), v1 = *(const f32x4*)(strip + r * LDW + c + 4);
-        const int m = m0 + i * 16 + r, n = n0 + c;
-        if constexpr (MODE == LAST) {
-          if (m < p.rows) {
-            T* to = (T*)p.result + (int64_t)b * p.rows * p.cols + (int64_t)m * p.cols + n;
-#pragma unroll
-            for (int q = 0; q < 8; ++q)
-              if (n + q < p.cols) to[q] = from_f32<T>(q < 4 ? v0[q] : v1[q - 4]);
-          }
-        } else {
-          f16_t* to = p.out + b * p.out_batch + m * ldo + n;
-          f16x8 hi, lo;
-#pragma unroll
-          for (int q = 0; q < 8; ++q) {
-            _Float16 a, l;
-            split(q < 4 ? v0[q] : v1[q - 4], a, l);
-            hi[q] = a;
-            lo[q] = l;
-          }
-          *(f16x8*)to = hi;
-          if (p.out_planes == 2) *(f16x8*)(to + p.out_plane) = lo;
+          for (int q = 0; q < 4; ++q) v[q] = fmaf(beta, (float)hi[q] + (float)lo[q], v[q]);
         }
+#pragma unroll
+        for (int q = 0; q < 4; ++q) strip[(quad * 4 + q) * (TR * 16 + 4) + j * 16 + row] = v[q];
       }
+      wave_fence();
+      out_rows(std::integral_constant<int, TR>{}, l0 + i * 16, p.lefts, r0, p.rights, MODE == AA);
     }
   }
 }
 
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
-  int planes, tile, M, N, Mp, Np;  // M <= N; padded to whole tiles
-  int64_t x, xt, a;                // elements of a plane of X (X^T), of A (P), all matrices
-  int64_t parts_at, factors_at, x_at, xt_at[2], a_at, p_at;  // bytes into the workspace
+  int planes, M, N, Mp, Np;  // M <= N; padded to multiples of 64
+  int64_t x, a;              // elements of a plane of X, of A (P), all matrices
+  int64_t parts_at, factors_at, x_at[2], a_at, p_at;  // bytes into the workspace
   size_t bytes;
 };
 
@@ -370,11 +465,9 @@ Plan plan_of(int64_t batch, int m, int n, int dtype) {
   p.planes = dtype == XL_DTYPE_BF16 ? 1 : 2;
   p.M = m < n ? m : n;
   p.N = m < n ? n : m;
-  p.tile = 128;
-  p.Mp = round_up(p.M, p.tile);
-  p.Np = round_up(p.N, p.tile);
+  p.Mp = round_up(p.M, 64);
+  p.Np = round_up(p.N, 64);
   p.x = batch * p.Mp * p.Np;
-  p.xt = p.x;
   p.a = batch * p.Mp * p.Mp;
   int64_t at = 0;
   auto take = [&](int64_t bytes) {
@@ -384,26 +477,40 @@ Plan plan_of(int64_t batch, int m, int n, int dtype) {
   };
   p.parts_at = take(batch * NORM_PARTS * 8);
   p.factors_at = take(batch * (int64_t)sizeof(Factors));
-  p.x_at = take(2 * p.x * p.planes);
-  for (int64_t& t : p.xt_at) t = take(2 * p.xt * 2);  // X^T has its lo plane in some steps of one-plane products too
+  for (int64_t& x : p.x_at) x = take(2 * p.x * 2);  // X has its lo plane in some steps of one-plane products too
   p.a_at = take(2 * p.a * p.planes);
   p.p_at = take(2 * p.a * p.planes);
   p.bytes = (size_t)at;
   return p;
 }
 
-template <int BM, int BN, int WM, int WN, int PL, int MODE, typename T>
-int launch_product(const Args& a, int64_t batch, hipStream_t st) {
-  constexpr int STAGE = (BM + BN) * 128 * PL, STRIP = 16 * (BN / WN + 4) * 4;
-  constexpr int LDS = 2 * STAGE > WM * WN * STRIP ? 2 * STAGE : WM * WN * STRIP;
-  auto kernel = ns_product_kernel<BM, BN, WM, WN, PL, MODE, T>;
+template <int BL, int BR, int WL, int WR, int STAGES, int PL, int MODE, typename T>
+int launch_tiles(Args a, int64_t batch, hipStream_t st) {
+  constexpr int TL = BL / WL / 16, TR = BR / WR / 16;
+  constexpr int STRIPS = WL * WR * 16 * ((TL > TR ? TL : TR) * 16 + 4) * 4, SLICES = STAGES * (BL + BR) * 128 * PL;
+  constexpr int LDS = SLICES > STRIPS ? SLICES : STRIPS;
+  static_assert(LDS <= 160 * 1024);
+  auto kernel = ns_product_kernel<BL, BR, WL, WR, STAGES, PL, MODE, T>;
   if (LDS > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (e != hipSuccess) return set_error(XL_ERR_LAUNCH, "xl_newton_schulz: %s", hipGetErrorString(e));
   }
-  const int tiles = MODE == XXT || MODE == AA ? a.tm * (a.tm + 1) / 2 : a.tm * a.tn;
-  hipLaunchKernelGGL(kernel, dim3((unsigned)tiles, (unsigned)batch), dim3(64 * WM * WN), LDS, st, a);
+  a.left_tiles = (a.lefts + BL - 1) / BL;
+  a.right_tiles = (a.rights + BR - 1) / BR;
+  const int64_t tiles = MODE == XXT || MODE == AA ? (int64_t)a.left_tiles * (a.left_tiles + 1) / 2
+                                                  : (int64_t)a.left_tiles * a.right_tiles;
+  if (tiles * batch > 0x7fffff) return set_error(XL_ERR_UNSUPPORTED, "xl_newton_schulz: batch too large");
+  hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * batch)), dim3(64 * WL * WR), LDS, st, a);
   return check_launch("xl_newton_schulz");
+}
+
+template <int PL, int MODE, typename T>
+int launch_product(const Args& a, int64_t batch, hipStream_t st) {
+  const int force = CFG;
+  if constexpr (PL == 1)
+    if (force == 256) return launch_tiles<256, 256, 2, 4, 2, PL, MODE, T>(a, batch, st);
+  if (force == 64) return launch_tiles<64, 64, 2, 2, PL == 1 ? 4 : 2, PL, MODE, T>(a, batch, st);
+  return launch_tiles<128, 128, 2, 2, 2, PL, MODE, T>(a, batch, st);
 }
 
 template <typename T, int PL>
@@ -412,10 +519,9 @@ int run(const void* g, void* x, int64_t batch, int m, int n, const float* coeffi
   const bool tall = m > n;
   double* part = (double*)(ws + p.parts_at);
   Factors* factors = (Factors*)(ws + p.factors_at);
-  f16_t *X = (f16_t*)(ws + p.x_at), *XT[2] = {(f16_t*)(ws + p.xt_at[0]), (f16_t*)(ws + p.xt_at[1])};
-  f16_t *A = (f16_t*)(ws + p.a_at), *P = (f16_t*)(ws + p.p_at);
+  f16_t *X[2] = {(f16_t*)(ws + p.x_at[0]), (f16_t*)(ws + p.x_at[1])}, *A = (f16_t*)(ws + p.a_at), *P = (f16_t*)(ws + p.p_at);
   const int64_t count = (int64_t)m * n;
-  const int64_t want = (count + 16 * NORM_BLOCK - 1) / (16 * NORM_BLOCK);
+  const int64_t want = (count + 64 * NORM_BLOCK - 1) / (64 * NORM_BLOCK);
   const int parts = (int)(want < NORM_PARTS ? want : NORM_PARTS);
   double growth = 1.0;
   for (int s = 0; s < steps; ++s) {
@@ -424,12 +530,9 @@ int run(const void* g, void* x, int64_t batch, int m, int n, const float* coeffi
   }
   hipLaunchKernelGGL(ns_norm_kernel<T>, dim3((unsigned)parts, (unsigned)batch), dim3(NORM_BLOCK), 0, st, (const T*)g, count,
                      parts, part);
-  const int Rp = tall ? p.Np : p.Mp, Cp = tall ? p.Mp : p.Np;
-  f16_t *same = tall ? XT[0] : X, *turned = tall ? X : XT[0];
-  const int64_t x_plane = p.x, xt_plane = p.xt;
-  hipLaunchKernelGGL((ns_enter_kernel<T, PL>), dim3((unsigned)(Cp / 64), (unsigned)(Rp / 64), (unsigned)batch), dim3(256), 0, st,
-                     (const T*)g, m, n, Rp, Cp, part, parts, (double)eps, growth, same, tall ? xt_plane : x_plane, turned,
-                     tall ? x_plane : xt_plane, factors);
+  auto enter = tall ? ns_enter_kernel<T, PL, true> : ns_enter_kernel<T, PL, false>;
+  hipLaunchKernelGGL(enter, dim3((unsigned)(p.Np / 64), (unsigned)(p.Mp / 64), (unsigned)batch), dim3(256), 0, st, (const T*)g,
+                     p.M, p.N, p.Mp, p.Np, part, parts, (double)eps, growth, X[0], p.x, factors);
   if (const int rc = check_launch("xl_newton_schulz")) return rc;
   const int64_t xb = (int64_t)p.Mp * p.Np, ab = (int64_t)p.Mp * p.Mp;
   for (int s = 0; s < steps; ++s) {
@@ -438,22 +541,21 @@ int run(const void* g, void* x, int64_t batch, int m, int n, const float* coeffi
     // a X in more bits than the products' while the smallest singular values grow: to the step before the last two.
     // Later the rounding of X is better the same in both terms: there the steps contract, and correct it.
     auto fine = [&](int step) { return PL == 2 || (step >= 1 && step <= steps - 3); };
-    const f16_t* old = XT[s & 1];
-    f16_t* next = XT[(s + 1) & 1];
+    const f16_t* old = X[s & 1];
     Args k{};
     k.factors = factors;
     k.first = s == 0;
-    k.left = k.right = X;
+    k.left = k.right = old;
     k.left_plane = k.right_plane = p.x;
     k.left_batch = k.right_batch = xb;
+    k.lefts = k.rights = p.Mp;
     k.K = p.Np;
-    k.tm = k.tn = p.Mp / p.tile;
     k.alpha = SCALE_A;
-    k.out = k.turned = A;
-    k.out_plane = k.turned_plane = p.a;
-    k.out_batch = k.turned_batch = ab;
-    k.out_planes = k.turned_planes = PL;
-    if (const int rc = launch_product<128, 128, 2, 2, PL, XXT, T>(k, batch, st)) return rc;
+    k.out = A;
+    k.out_plane = p.a;
+    k.out_batch = ab;
+    k.out_planes = PL;
+    if (const int rc = launch_product<PL, XXT, T>(k, batch, st)) return rc;
     k.left = k.right = k.e = A;
     k.left_plane = k.right_plane = k.e_plane = p.a;
     k.left_batch = k.right_batch = k.e_batch = ab;
@@ -461,30 +563,25 @@ int run(const void* g, void* x, int64_t batch, int m, int n, const float* coeffi
     k.K = p.Mp;
     k.alpha = SCALE_P * c / (SCALE_A * SCALE_A);
     k.beta = SCALE_P * b / SCALE_A;
-    k.out = k.turned = P;
-    if (const int rc = launch_product<128, 128, 2, 2, PL, AA, T>(k, batch, st)) return rc;
-    k.left = P;
-    k.right = k.e = old;
-    k.right_plane = k.e_plane = p.xt;
-    k.right_batch = k.e_batch = xb;
+    k.out = P;
+    if (const int rc = launch_product<PL, AA, T>(k, batch, st)) return rc;
+    k.left = k.e = old;
+    k.left_plane = k.e_plane = p.x;
+    k.left_batch = k.e_batch = xb;
     k.e_planes = fine(s) ? 2 : 1;
-    k.tn = p.Np / p.tile;
+    k.right = P;
+    k.lefts = p.Np;
     k.alpha = 1.f / SCALE_P;
     k.beta = a;
-    k.out = X;
+    k.out = X[(s + 1) & 1];
     k.out_plane = p.x;
     k.out_batch = xb;
-    k.turned = next;
-    k.turned_plane = p.xt;
-    k.turned_batch = xb;
-    k.turned_planes = fine(s + 1) ? 2 : 1;
+    k.out_planes = fine(s + 1) ? 2 : 1;
     k.result = x;
     k.rows = p.M;
     k.cols = p.N;
     k.result_turned = tall;
-    const int rc = last ? launch_product<128, 128, 2, 2, PL, LAST, T>(k, batch, st)
-                        : launch_product<128, 128, 2, 2, PL, PX, T>(k, batch, st);
-    if (rc) return rc;
+    if (const int rc = last ? launch_product<PL, LAST, T>(k, batch, st) : launch_product<PL, PX, T>(k, batch, st)) return rc;
   }
   return XL_OK;
 }
