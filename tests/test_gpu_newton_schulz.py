@@ -79,9 +79,9 @@ def gradient(shape, dtype, seed=0, kind="spread"):
     return x.to(dtype).to(dev())
 
 
-# one value; vectors; less than a tile, a tile, just past it; odd; wide and tall; a long sum for few rows; batches
+# one value; vectors; less than a tile, a tile, just past it; odd; the largest in one workgroup and just past them; wide and tall; a long sum for few rows; batches
 SHAPES = [(1, 1), (1, 9), (200, 1), (3, 5), (33, 17), (64, 64), (128, 128), (127, 129), (129, 128), (130, 257), (200, 333),
-          (31, 2050), (2050, 31), (100, 5000), (513, 700), (1000, 777), (3, 65, 130), (2, 2, 140, 96), (17, 64, 64), (0, 8, 8),
+          (31, 2050), (2050, 31), (100, 5000), (513, 700), (1000, 777), (64, 256), (65, 200), (128, 256), (257, 128), (60, 257), (128, 130), (256, 64), (3, 65, 130), (2, 2, 140, 96), (17, 64, 64), (0, 8, 8),
           (8, 0)]
 
 
@@ -97,7 +97,8 @@ def test_sizes(gpu_case, shape, dtype):
         check(got, G)
 
 
-@pytest.mark.parametrize("shape", [(1536, 1100), (2048, 2304), (2, 1300, 2600), (640, 6000)], ids=str)
+# every size of tile and depth of stages
+@pytest.mark.parametrize("shape", [(1536, 1100), (2048, 2304), (2, 1300, 2600), (640, 6000), (4100, 2900), (6, 1000, 2000)], ids=str)
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_large(gpu_case, shape, dtype):
     import xlstm_hip

@@ -43,9 +43,6 @@ typedef __attribute__((address_space(3))) char lds_char;
 
 // stored = value * scale: with |singular values| of X up to 8 (checked on the host), |A| <= 64 and |P| <= 250
 constexpr float SCALE_X = 256.f, SCALE_A = 256.f, SCALE_P = 64.f;
-#ifndef CFG
-#define CFG 128
-#endif
 constexpr float MOST_X = 8.f, MOST_P = 250.f;
 
 // ------------------------------------------------------------------------------------------------ norm and first X
@@ -89,6 +86,11 @@ __global__ __launch_bounds__(NORM_BLOCK) void ns_norm_kernel(const T* __restrict
   for (int w = 0; w < NORM_BLOCK / 64; ++w) s += sums[w];
   part[(int64_t)blockIdx.y * parts + blockIdx.x] = s;
 }
+
+constexpr int MOST_STEPS = 64;
+struct Coefficients {  // a kernel's argument
+  float v[3 * MOST_STEPS];
+};
 
 // A matrix's factors: X0 = stored * first, later X = stored * later.
 struct Factors {
@@ -381,7 +383,7 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
     constexpr int EACH = BLOCKS.value * 2, LDW = BLOCKS.value * 16 + 4;
 #pragma unroll
     for (int h = 0; h < (16 * EACH + 63) / 64; ++h) {
-      const int r = h * (64 / EACH) + lane / EACH, c = lane % EACH * 8, m = row0 + r, n = col0 + c;
+      const int at = h * 64 + lane, r = at / EACH, c = at % EACH * 8, m = row0 + r, n = col0 + c;
       if (r >= 16 || m >= rows || n >= cols) continue;
       const f32x4 v0 = *(const f32x4*)(strip + r * LDW + c), v1 = *(const f32x4*)(strip + r * LDW + c + 4);
       float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
@@ -450,6 +452,178 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
   }
 }
 
+// ------------------------------------------------------------------------------------------------ small matrices
+// A whole matrix in one workgroup and one launch: X [D, N] by rows in LDS (f16 planes), A and then P [D, D] beside it,
+// and every wave's part of X in float32 registers.  A lane has left 4 quad .. + 3 of right `row` of a block, which is four
+// neighbours of a row of X in P X and, as A and P are symmetric, of theirs: no block is turned.  Pieces of 16 bytes lie
+// at piece ^ (row % 8).  Bound by the latency of 3 products and 5 barriers a step: 128 x 128 bf16 in %SMALL% us, where
+// the separate launches of the tiled form take 60.
+constexpr int SMALL_THREADS = 512, SMALL_WL = 2, SMALL_WR = 4;
+
+template <int D, int N, int PL, bool TALL, typename T>
+__global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __restrict__ g, T* __restrict__ out, int rows,
+                                                                 int cols, Coefficients co, int steps, double eps,
+                                                                 double growth) {
+  constexpr int TA = D / SMALL_WL / 16, TX = N / SMALL_WL / 16, TR = D / SMALL_WR / 16;  // blocks of a wave
+  constexpr int X_PLANE = D * N * 2, A_PLANE = D * D * 2;
+  extern __shared__ __align__(1024) char lds[];
+  char *xs = lds, *as = lds + PL * X_PLANE;
+  double* sums = (double*)as;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / SMALL_WR, wr = wave % SMALL_WR;
+  const int row = lane & 15, quad = lane >> 4;
+  g += (int64_t)blockIdx.x * rows * cols;
+  out += (int64_t)blockIdx.x * rows * cols;
+
+  // X[m][n .. n + 3] of block (i, j): n = (wl TX + i) 16 + 4 quad, m = (wr TR + j) 16 + row
+  float x[TX][TR][4];
+  double s = 0.0;
+#pragma unroll
+  for (int i = 0; i < TX; ++i)
+#pragma unroll
+    for (int j = 0; j < TR; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = (wl * TX + i) * 16 + 4 * quad + q, m = (wr * TR + j) * 16 + row;
+        const bool in = m < rows && n < cols;
+        x[i][j][q] = in ? to_f32(g[TALL ? (int64_t)n * rows + m : (int64_t)m * cols + n]) : 0.f;
+        s = fma((double)x[i][j][q], (double)x[i][j][q], s);
+      }
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
+  if (lane == 0) sums[wave] = s;
+  __syncthreads();
+  s = 0.0;
+#pragma unroll
+  for (int w = 0; w < SMALL_THREADS / 64; ++w) s += sums[w];
+  double enter;
+  const Factors f = factors_of(sqrt(s), eps, growth, enter);
+#pragma unroll
+  for (int i = 0; i < TX; ++i)
+#pragma unroll
+    for (int j = 0; j < TR; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) x[i][j][q] = (float)((double)x[i][j][q] * enter);
+
+  // 8 values along k of a row, from 32 s + 8 quad
+  auto by_row = [&](const char* base, int width, int block, int k32) {
+    const int r = block * 16 + row;
+    return *(const f16x8*)(base + r * (width * 2) + (((k32 * 4 + quad) ^ (r & 7)) << 4));
+  };
+  // of a column of X
+  auto by_column = [&](const char* base, int block, int k32) {
+    const int k = k32 * 32 + quad * 8 + (row >> 2), piece = (2 * block + ((row & 3) >> 1)) ^ (row >> 2);
+    const char* at = base + k * (N * 2) + (row & 1) * 8;
+    return __builtin_bit_cast(f16x8, mfma::tr_pair(at + (piece << 4), at + 4 * (N * 2) + ((piece ^ 4) << 4)));
+  };
+  auto place = [&](char* base, int width, int r, int c) {  // 4 values at (r, c)
+    return base + r * (width * 2) + (((c >> 3) ^ (r & 7)) << 4) + (c & 4) * 2;
+  };
+  auto put = [&](char* base, int plane, int width, int r, int c, const f32x4& v) {
+    f16x4 hi, lo;
+#pragma unroll
+    for (int q = 0; q < 4; ++q) {
+      _Float16 h, l;
+      split(v[q], h, l);
+      hi[q] = h;
+      lo[q] = l;
+    }
+    *(f16x4*)place(base, width, r, c) = hi;
+    if constexpr (PL == 2) *(f16x4*)(place(base, width, r, c) + plane) = lo;
+  };
+  // acc[i][j] = sum over K of the wave's left blocks and its right rows
+  auto product = [&](auto& acc, auto BLOCKS, auto K, auto&& left, const char* right, int right_plane, int right_width) {
+#pragma unroll
+    for (int i = 0; i < BLOCKS.value; ++i)
+#pragma unroll
+      for (int j = 0; j < TR; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll 2
+    for (int k = 0; k < K.value / 32; ++k) {
+      f16x8 r[PL][TR];
+#pragma unroll
+      for (int pl = 0; pl < PL; ++pl)
+#pragma unroll
+        for (int j = 0; j < TR; ++j) r[pl][j] = by_row(right + pl * right_plane, right_width, wr * TR + j, k);
+#pragma unroll
+      for (int i = 0; i < BLOCKS.value; ++i) {
+        f16x8 l[PL];
+#pragma unroll
+        for (int pl = 0; pl < PL; ++pl) l[pl] = left(pl, wl * BLOCKS.value + i, k);
+#pragma unroll
+        for (int j = 0; j < TR; ++j) {
+          if constexpr (PL == 2) {
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[1], r[0][j], acc[i][j], 0, 0, 0);
+            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0], r[1][j], acc[i][j], 0, 0, 0);
+          }
+          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0], r[0][j], acc[i][j], 0, 0, 0);
+        }
+      }
+    }
+  };
+  using IntA = std::integral_constant<int, TA>;
+  using IntX = std::integral_constant<int, TX>;
+  using KX = std::integral_constant<int, N>;
+  using KA = std::integral_constant<int, D>;
+  for (int step = 0; step < steps; ++step) {
+    const float u = step ? f.later : f.first;
+    __syncthreads();  // X has been read
+#pragma unroll
+    for (int i = 0; i < TX; ++i)
+#pragma unroll
+      for (int j = 0; j < TR; ++j)
+        put(xs, X_PLANE, N, (wr * TR + j) * 16 + row, (wl * TX + i) * 16 + 4 * quad,
+            f32x4{x[i][j][0], x[i][j][1], x[i][j][2], x[i][j][3]});
+    __syncthreads();
+    f32x4 acc[TA][TR];
+    product(acc, IntA{}, KX{}, [&](int pl, int block, int k) { return by_row(xs + pl * X_PLANE, N, block, k); }, xs, X_PLANE, N);
+#pragma unroll
+    for (int i = 0; i < TA; ++i)
+#pragma unroll
+      for (int j = 0; j < TR; ++j) {
+        acc[i][j] *= SCALE_A * u * u;
+        put(as, A_PLANE, D, (wr * TR + j) * 16 + row, (wl * TA + i) * 16 + 4 * quad, acc[i][j]);
+      }
+    __syncthreads();
+    f32x4 sq[TA][TR];
+    product(sq, IntA{}, KA{}, [&](int pl, int block, int k) { return by_row(as + pl * A_PLANE, D, block, k); }, as, A_PLANE, D);
+    __syncthreads();  // A has been read
+    const float pb = SCALE_P * co.v[3 * step + 1] / SCALE_A, pc = SCALE_P * co.v[3 * step + 2] / (SCALE_A * SCALE_A);
+#pragma unroll
+    for (int i = 0; i < TA; ++i)
+#pragma unroll
+      for (int j = 0; j < TR; ++j) {
+        f32x4 v;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          // one plane: A as it was multiplied
+          const float a = PL == 1 ? (float)(_Float16)acc[i][j][q] : acc[i][j][q];
+          v[q] = fmaf(pb, a, pc * sq[i][j][q]);
+        }
+        put(as, A_PLANE, D, (wr * TR + j) * 16 + row, (wl * TA + i) * 16 + 4 * quad, v);
+      }
+    __syncthreads();
+    f32x4 px[TX][TR];
+    product(px, IntX{}, KA{}, [&](int pl, int block, int k) { return by_column(xs + pl * X_PLANE, block, k); }, as, A_PLANE, D);
+    const bool last = step + 1 == steps, fine = PL == 2 || (step >= 1 && step <= steps - 3);
+    const float to = last ? u : u / f.later, a = co.v[3 * step] * to, b = to / SCALE_P;
+#pragma unroll
+    for (int i = 0; i < TX; ++i)
+#pragma unroll
+      for (int j = 0; j < TR; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          x[i][j][q] = fmaf(a, fine ? x[i][j][q] : (float)(_Float16)x[i][j][q], b * px[i][j][q]);
+  }
+#pragma unroll
+  for (int i = 0; i < TX; ++i)
+#pragma unroll
+    for (int j = 0; j < TR; ++j)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int n = (wl * TX + i) * 16 + 4 * quad + q, m = (wr * TR + j) * 16 + row;
+        if (m < rows && n < cols) out[TALL ? (int64_t)n * rows + m : (int64_t)m * cols + n] = from_f32<T>(x[i][j][q]);
+      }
+}
+
 // ------------------------------------------------------------------------------------------------ host
 struct Plan {
   int planes, M, N, Mp, Np;  // M <= N; padded to multiples of 64
@@ -460,11 +634,20 @@ struct Plan {
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
+// Whether ns_small_kernel takes matrices of these sizes: a row of X more fills the LDS or the registers.
+bool is_small(int M, int N, int planes) {
+  return M <= 64 ? N <= 256 : M <= 128 && N <= (planes == 1 ? 256 : 128);
+}
+
 Plan plan_of(int64_t batch, int m, int n, int dtype) {
   Plan p;
   p.planes = dtype == XL_DTYPE_BF16 ? 1 : 2;
   p.M = m < n ? m : n;
   p.N = m < n ? n : m;
+  if (is_small(p.M, p.N, p.planes)) {  // no workspace
+    p.bytes = 0;
+    return p;
+  }
   p.Mp = round_up(p.M, 64);
   p.Np = round_up(p.N, 64);
   p.x = batch * p.Mp * p.Np;
@@ -504,18 +687,101 @@ int launch_tiles(Args a, int64_t batch, hipStream_t st) {
   return check_launch("xl_newton_schulz");
 }
 
+// Which tiles.  A tile of 256 x 256 has the best rate of a full chip, smaller ones fill it where there are few tiles, and
+// deep stages hide the loads' latency where a CU has one workgroup.  cost: time of a slice of K, in 0.96 us of a 4096^3
+// product, from the tiles a CU gets (r); measured (us):
+//   bf16, X of 4096 x 4096, P X:   256: 110;  128, 2 stages: 133, 4 stages: 159;  64, 2 stages: 205, 4 stages: 204
+//   X X^T there:                   192 (253 tiles): 67;  256 (136): 76;  128 (528): 96;  64 (2080): 128
+//   12 of 1024 x 2048, P X:        128 (1536): 69;  256 (384): 72;  64: 90;   X X^T: 128 (432): 33;  192 (252): 36
+//   2048 x 5504, P X:              256 (176): 52;  128 (688): 60;  64 (2752): 73
+//   X X^T there:                   128, 4 stages (136): 41, 2 stages: 55;  64, 2 stages (528): 47, 4 stages: 62
+//   1024 x 1024, P X:              64, 4 stages (256): 8.1, 2 stages: 10.9;  128, 4 stages (64): 14.6
+//   float32, 2048 x 2048, P X:     128 (256): 48;  64, 2 stages (1024): 59, 4 stages: 64
+//   float32, 1000 x 1777, P X:     64, 2 stages (448): 16.7, 4 stages: 19.3;  128 (112): 26;   X X^T: 64, 4 stages
+//                                  (136): 14.0, 2 stages: 20;  128 (36): 37
 template <int PL, int MODE, typename T>
 int launch_product(const Args& a, int64_t batch, hipStream_t st) {
-  const int force = CFG;
-  if constexpr (PL == 1)
-    if (force == 256) return launch_tiles<256, 256, 2, 4, 2, PL, MODE, T>(a, batch, st);
-  if (force == 64) return launch_tiles<64, 64, 2, 2, PL == 1 ? 4 : 2, PL, MODE, T>(a, batch, st);
+  constexpr bool SYM = MODE == XXT || MODE == AA;
+  constexpr int CUS = 256;
+  auto tiles = [&](int tile) {
+    const int64_t l = (a.lefts + tile - 1) / tile, r = (a.rights + tile - 1) / tile;
+    return (SYM ? l * (l + 1) / 2 : l * r) * batch;
+  };
+  auto rounds = [&](int tile) { return (double)((tiles(tile) + CUS - 1) / CUS); };
+  auto at_least = [](double v, double least) { return v > least ? v : least; };
+  enum { T256, T192, T128_2, T128_4, T64_2, T64_4, CHOICES };
+  double cost[CHOICES];
+  for (double& c : cost) c = INFINITY;
+  if (PL == 1) {
+    const double r = rounds(256);
+    cost[T256] = 52.4 * r * (0.75 + 0.25 * (double)tiles(256) / (CUS * r));  // a chip not full runs faster
+    if (SYM) cost[T192] = 32.3 * rounds(192);
+    cost[T128_2] = at_least(16.2 * rounds(128), 19.3);
+    cost[T128_4] = (rounds(128) > 1 ? 19.0 : 14.6) * rounds(128);
+    cost[T64_2] = at_least(6.1 * rounds(64), 12.8);
+    cost[T64_4] = (rounds(64) > 1 ? 7.0 : 8.0) * rounds(64);
+  } else {
+    cost[T128_2] = 16.4 * rounds(128);
+    cost[T64_2] = at_least(5.6 * rounds(64), 9.1);
+    cost[T64_4] = 6.2 * rounds(64);
+  }
+  int best = T128_2;
+  for (int c = 0; c < CHOICES; ++c)
+    if (cost[c] < cost[best]) best = c;
+  if constexpr (PL == 1) {
+    if (best == T256) return launch_tiles<256, 256, 2, 4, 2, PL, MODE, T>(a, batch, st);
+    if constexpr (SYM)
+      if (best == T192) return launch_tiles<192, 192, 2, 4, 2, PL, MODE, T>(a, batch, st);
+    if (best == T128_4) return launch_tiles<128, 128, 2, 2, 4, PL, MODE, T>(a, batch, st);
+  }
+  if (best == T64_2) return launch_tiles<64, 64, 2, 2, 2, PL, MODE, T>(a, batch, st);
+  if (best == T64_4) return launch_tiles<64, 64, 2, 2, 4, PL, MODE, T>(a, batch, st);
   return launch_tiles<128, 128, 2, 2, 2, PL, MODE, T>(a, batch, st);
+}
+
+template <int D, int N, int PL, typename T>
+int launch_small(const void* g, void* x, int64_t batch, int m, int n, const Coefficients& co, int steps, float eps,
+                 double growth, hipStream_t st) {
+  constexpr int LDS = PL * (D * N + D * D) * 2;
+  static_assert(LDS <= 160 * 1024);
+  auto kernel = m > n ? ns_small_kernel<D, N, PL, true, T> : ns_small_kernel<D, N, PL, false, T>;
+  if (LDS > 64 * 1024) {
+    const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
+    if (e != hipSuccess) return set_error(XL_ERR_LAUNCH, "xl_newton_schulz: %s", hipGetErrorString(e));
+  }
+  hipLaunchKernelGGL(kernel, dim3((unsigned)batch), dim3(SMALL_THREADS), LDS, st, (const T*)g, (T*)x, m < n ? m : n,
+                     m < n ? n : m, co, steps, (double)eps, growth);
+  return check_launch("xl_newton_schulz");
+}
+
+template <typename T, int PL>
+int run_small(const void* g, void* x, int64_t batch, int m, int n, const Coefficients& co, int steps, float eps, double growth,
+              hipStream_t st) {
+  const int M = m < n ? m : n, N = m < n ? n : m;
+  if (M <= 64) {
+    if (N <= 64) return launch_small<64, 64, PL, T>(g, x, batch, m, n, co, steps, eps, growth, st);
+    if (N <= 128) return launch_small<64, 128, PL, T>(g, x, batch, m, n, co, steps, eps, growth, st);
+    return launch_small<64, 256, PL, T>(g, x, batch, m, n, co, steps, eps, growth, st);
+  }
+  if constexpr (PL == 1) {
+    if (N > 128) return launch_small<128, 256, PL, T>(g, x, batch, m, n, co, steps, eps, growth, st);
+  }
+  return launch_small<128, 128, PL, T>(g, x, batch, m, n, co, steps, eps, growth, st);
 }
 
 template <typename T, int PL>
 int run(const void* g, void* x, int64_t batch, int m, int n, const float* coefficients, int steps, float eps, const Plan& p,
         char* ws, hipStream_t st) {
+  double growth = 1.0;
+  for (int s = 0; s < steps; ++s) {
+    const double a = fabs((double)coefficients[3 * s]);
+    if (a > 1.0) growth *= a;
+  }
+  if (is_small(p.M, p.N, PL)) {
+    Coefficients co;
+    for (int i = 0; i < 3 * steps; ++i) co.v[i] = coefficients[i];
+    return run_small<T, PL>(g, x, batch, m, n, co, steps, eps, growth, st);
+  }
   const bool tall = m > n;
   double* part = (double*)(ws + p.parts_at);
   Factors* factors = (Factors*)(ws + p.factors_at);
@@ -523,11 +789,6 @@ int run(const void* g, void* x, int64_t batch, int m, int n, const float* coeffi
   const int64_t count = (int64_t)m * n;
   const int64_t want = (count + 64 * NORM_BLOCK - 1) / (64 * NORM_BLOCK);
   const int parts = (int)(want < NORM_PARTS ? want : NORM_PARTS);
-  double growth = 1.0;
-  for (int s = 0; s < steps; ++s) {
-    const double a = fabs((double)coefficients[3 * s]);
-    if (a > 1.0) growth *= a;
-  }
   hipLaunchKernelGGL(ns_norm_kernel<T>, dim3((unsigned)parts, (unsigned)batch), dim3(NORM_BLOCK), 0, st, (const T*)g, count,
                      parts, part);
   auto enter = tall ? ns_enter_kernel<T, PL, true> : ns_enter_kernel<T, PL, false>;
@@ -611,7 +872,8 @@ extern "C" int xl_newton_schulz(const void* g, void* x, int64_t batch, int m, in
   clear_error();
   const char* who = "xl_newton_schulz";
   if (const int rc = check_sizes(who, batch, m, n, dtype)) return rc;
-  if (steps < 1 || !coefficients) return set_error(XL_ERR_INVALID_ARG, "%s: steps=%d (at least 1, with coefficients)", who, steps);
+  if (steps < 1 || steps > MOST_STEPS || !coefficients)
+    return set_error(XL_ERR_INVALID_ARG, "%s: steps=%d (1 to %d, with coefficients)", who, steps, MOST_STEPS);
   if (!(eps >= 0.f)) return set_error(XL_ERR_INVALID_ARG, "%s: eps=%g (not negative)", who, (double)eps);
   // singular values start in [0, 1]: the most that a step's polynomial makes of them
   double most = 1.0;
@@ -632,7 +894,7 @@ extern "C" int xl_newton_schulz(const void* g, void* x, int64_t batch, int m, in
   if (!g || !x) return set_error(XL_ERR_INVALID_ARG, "%s: null pointer", who);
   if (g == x) return set_error(XL_ERR_INVALID_ARG, "%s: x must not alias g", who);
   const Plan p = plan_of(batch, m, n, dtype);
-  if (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255u))
+  if (p.bytes && (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255u)))
     return set_error(XL_ERR_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", who, p.bytes,
                      workspace_bytes);
   char* ws = (char*)workspace;
