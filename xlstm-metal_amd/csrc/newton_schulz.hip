@@ -39,6 +39,37 @@ __device__ __forceinline__ Vec<T> load_vec(const T* p) {
   const u32x4 raw = *(const raw_at<T>*)p;
   return __builtin_bit_cast(Vec<T>, raw);
 }
+// 16 bytes of T from float32, two values by one conversion
+template <typename T>
+__device__ __forceinline__ u32x4 rounded_vec(const float* v) {
+  if constexpr (is_f32<T>::value) {
+    return __builtin_bit_cast(u32x4, (f32x4{v[0], v[1], v[2], v[3]}));
+  } else {
+    using pair = std::conditional_t<std::is_same_v<T, f16_t>, xl_f16x2, xl_bf16x2>;
+    u32x4 raw;
+#pragma unroll
+    for (int j = 0; j < 4; ++j)
+      raw[j] = __builtin_bit_cast(uint32_t, __builtin_convertvector((xl_f32x2{v[2 * j], v[2 * j + 1]}), pair));
+    return raw;
+  }
+}
+template <typename T>
+struct Four {
+  T e[4];
+};
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef u32x2 u32x2_at2 __attribute__((aligned(2)));
+template <typename T>
+using raw_four = std::conditional_t<sizeof(T) == 2, u32x2_at2, u32x4_at4>;
+template <typename T>
+__device__ __forceinline__ Four<T> load_four(const T* p) {
+  const std::conditional_t<sizeof(T) == 2, u32x2, u32x4> raw = *(const raw_four<T>*)p;
+  return __builtin_bit_cast(Four<T>, raw);
+}
+template <typename T>
+__device__ __forceinline__ void store_four(T* p, const Four<T>& v) {
+  *(raw_four<T>*)p = __builtin_bit_cast(std::conditional_t<sizeof(T) == 2, u32x2, u32x4>, v);
+}
 typedef __attribute__((address_space(3))) char lds_char;
 
 // stored = value * scale: with |singular values| of X up to 8 (checked on the host), |A| <= 64 and |P| <= 250
@@ -138,49 +169,62 @@ __global__ __launch_bounds__(256) void ns_enter_kernel(const T* __restrict__ g, 
                                                        double growth, f16_t* __restrict__ x, int64_t x_plane,
                                                        Factors* __restrict__ factors) {
   constexpr int VW = 16 / sizeof(T);
-  __shared__ float tile[64][65];
-  __shared__ double sums[4];
+  __shared__ float tile[TALL ? 64 : 1][65];
+  __shared__ double sums[4], scale;
   const int tid = threadIdx.x, b = blockIdx.z;
+  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, R = TALL ? N : M, C = TALL ? M : N;
+  const int r0 = TALL ? n0 : m0, c0 = TALL ? m0 : n0;
+  const T* gp = g + (int64_t)b * M * N;
+  f16_t* xp = x + (int64_t)b * Mp * Np;
+  const int r = tid >> 3, c = (tid & 7) * 8;  // 8 values of rows r and r + 32, of G's tile and of X's
+  float v[2][8];
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    const int rr = r0 + r + 32 * h;
+    const T* from = gp + (int64_t)rr * C + c0 + c;
+    if (rr < R && c0 + c + 8 <= C) {
+#pragma unroll
+      for (int q = 0; q < 8; q += VW) {
+        const Vec<T> u = load_vec(from + q);
+#pragma unroll
+        for (int j = 0; j < VW; ++j) v[h][q + j] = to_f32(u.e[j]);
+      }
+    } else {
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[h][q] = rr < R && c0 + c + q < C ? to_f32(from[q]) : 0.f;
+    }
+  }
   double s = tid < parts ? part[(int64_t)b * parts + tid] : 0.0;
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if ((tid & 63) == 0) sums[tid >> 6] = s;
   __syncthreads();
-  double enter;
-  const Factors f = factors_of(sqrt(sums[0] + sums[1] + sums[2] + sums[3]), eps, growth, enter);
-  if (blockIdx.x == 0 && blockIdx.y == 0 && tid == 0) factors[b] = f;
-  const int m0 = blockIdx.y * 64, n0 = blockIdx.x * 64, R = TALL ? N : M, C = TALL ? M : N;
-  const int r0 = TALL ? n0 : m0, c0 = TALL ? m0 : n0;
-  const T* gp = g + (int64_t)b * M * N;
-  f16_t* xp = x + (int64_t)b * Mp * Np;
-  const int r = tid >> 2, c = (tid & 3) * 16;  // 16 values of one row of G's tile, and of X's
-  float v[16];
-  const T* from = gp + (int64_t)(r0 + r) * C + c0 + c;
-  if (r0 + r < R && c0 + c + 16 <= C) {
-#pragma unroll
-    for (int q = 0; q < 16; q += VW) {
-      const Vec<T> u = load_vec(from + q);
-#pragma unroll
-      for (int j = 0; j < VW; ++j) v[q + j] = to_f32(u.e[j]);
-    }
-  } else {
-#pragma unroll
-    for (int q = 0; q < 16; ++q) v[q] = r0 + r < R && c0 + c + q < C ? to_f32(from[q]) : 0.f;
+  if (tid == 0) {
+    double enter;
+    const Factors f = factors_of(sqrt(sums[0] + sums[1] + sums[2] + sums[3]), eps, growth, enter);
+    if (blockIdx.x == 0 && blockIdx.y == 0) factors[b] = f;
+    scale = enter;
   }
+  __syncthreads();
+  const double enter = scale;
 #pragma unroll
-  for (int q = 0; q < 16; ++q) v[q] = (float)((double)v[q] * enter);
+  for (int h = 0; h < 2; ++h)
+#pragma unroll
+    for (int q = 0; q < 8; ++q) v[h][q] = (float)((double)v[h][q] * enter);
   if constexpr (TALL) {
 #pragma unroll
-    for (int q = 0; q < 16; ++q) tile[r][c + q] = v[q];
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) tile[r + 32 * h][c + q] = v[h][q];
     __syncthreads();
 #pragma unroll
-    for (int q = 0; q < 16; ++q) v[q] = tile[c + q][r];
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int q = 0; q < 8; ++q) v[h][q] = tile[c + q][r + 32 * h];
   }
 #pragma unroll
-  for (int q = 0; q < 16; q += 8) {
-    const float half[8] = {v[q], v[q + 1], v[q + 2], v[q + 3], v[q + 4], v[q + 5], v[q + 6], v[q + 7]};
-    store_planes(xp + (int64_t)(m0 + r) * Np + n0 + c + q, x_plane, PL == 2, half);
-  }
+  for (int h = 0; h < 2; ++h)
+    store_planes(xp + (int64_t)(m0 + r + 32 * h) * Np + n0 + c, x_plane, PL == 2, v[h]);
 }
 
 // ------------------------------------------------------------------------------------------------ the products
@@ -402,10 +446,7 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
         if (n + 8 <= C) {
 #pragma unroll
           for (int q = 0; q < 8; q += 16 / sizeof(T)) {
-            Vec<T> o;
-#pragma unroll
-            for (int z = 0; z < 16 / (int)sizeof(T); ++z) o.e[z] = from_f32<T>(v[q + z]);
-            *(raw_at<T>*)(to + q) = __builtin_bit_cast(u32x4, o);
+            *(raw_at<T>*)(to + q) = rounded_vec<T>(v + q);
           }
         } else {
 #pragma unroll
@@ -456,7 +497,7 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
 // A whole matrix in one workgroup and one launch: X [D, N] by rows in LDS (f16 planes), A and then P [D, D] beside it,
 // and every wave's part of X in float32 registers.  A lane has left 4 quad .. + 3 of right `row` of a block, which is four
 // neighbours of a row of X in P X and, as A and P are symmetric, of theirs: no block is turned.  Pieces of 16 bytes lie
-// at piece ^ (row % 8).  Bound by the latency of 3 products and 5 barriers a step: 128 x 128 bf16 in %SMALL% us, where
+// at piece ^ (row % 8).  Bound by the latency of 3 products and 5 barriers a step: 128 x 128 bf16 in 27 us, where
 // the separate launches of the tiled form take 60.
 constexpr int SMALL_THREADS = 512, SMALL_WL = 2, SMALL_WR = 4;
 
@@ -477,17 +518,32 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
   // X[m][n .. n + 3] of block (i, j): n = (wl TX + i) 16 + 4 quad, m = (wr TR + j) 16 + row
   float x[TX][TR][4];
   double s = 0.0;
+  // Four neighbours by one access where the block is whole (a wide matrix); the loads of all blocks are under way at once.
+  // (Value by value they took 16 us of 37 at 128 x 128: 16 lines an access.)
+#pragma unroll
+  for (int i = 0; i < TX; ++i)
+#pragma unroll
+    for (int j = 0; j < TR; ++j) {
+      const int n = (wl * TX + i) * 16 + 4 * quad, m = (wr * TR + j) * 16 + row, mc = min(m, rows - 1);
+      if (!TALL && (wl * TX + i) * 16 + 16 <= cols) {
+        const Four<T> v = load_four(g + mc * cols + n);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) x[i][j][q] = m < rows ? to_f32(v.e[q]) : 0.f;
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+          const int nc = min(n + q, cols - 1);
+          const float v = to_f32(g[TALL ? nc * rows + mc : mc * cols + nc]);
+          x[i][j][q] = m < rows && n + q < cols ? v : 0.f;
+        }
+      }
+    }
 #pragma unroll
   for (int i = 0; i < TX; ++i)
 #pragma unroll
     for (int j = 0; j < TR; ++j)
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = (wl * TX + i) * 16 + 4 * quad + q, m = (wr * TR + j) * 16 + row;
-        const bool in = m < rows && n < cols;
-        x[i][j][q] = in ? to_f32(g[TALL ? (int64_t)n * rows + m : (int64_t)m * cols + n]) : 0.f;
-        s = fma((double)x[i][j][q], (double)x[i][j][q], s);
-      }
+      for (int q = 0; q < 4; ++q) s = fma((double)x[i][j][q], (double)x[i][j][q], s);
 #pragma unroll
   for (int o = 32; o > 0; o >>= 1) s += __shfl_xor(s, o, 64);
   if (lane == 0) sums[wave] = s;
@@ -536,7 +592,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
     for (int i = 0; i < BLOCKS.value; ++i)
 #pragma unroll
       for (int j = 0; j < TR; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll 2
+#pragma unroll 4
     for (int k = 0; k < K.value / 32; ++k) {
       f16x8 r[PL][TR];
 #pragma unroll
@@ -616,12 +672,20 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
 #pragma unroll
   for (int i = 0; i < TX; ++i)
 #pragma unroll
-    for (int j = 0; j < TR; ++j)
+    for (int j = 0; j < TR; ++j) {
+      const int n = (wl * TX + i) * 16 + 4 * quad, m = (wr * TR + j) * 16 + row;
+      if (m >= rows) continue;
+      if (!TALL && n + 4 <= cols) {
+        Four<T> v;
 #pragma unroll
-      for (int q = 0; q < 4; ++q) {
-        const int n = (wl * TX + i) * 16 + 4 * quad + q, m = (wr * TR + j) * 16 + row;
-        if (m < rows && n < cols) out[TALL ? (int64_t)n * rows + m : (int64_t)m * cols + n] = from_f32<T>(x[i][j][q]);
+        for (int q = 0; q < 4; ++q) v.e[q] = from_f32<T>(x[i][j][q]);
+        store_four(out + m * cols + n, v);
+      } else {
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          if (n + q < cols) out[TALL ? (n + q) * rows + m : m * cols + n + q] = from_f32<T>(x[i][j][q]);
       }
+    }
 }
 
 // ------------------------------------------------------------------------------------------------ host
@@ -715,7 +779,7 @@ int launch_product(const Args& a, int64_t batch, hipStream_t st) {
   if (PL == 1) {
     const double r = rounds(256);
     cost[T256] = 52.4 * r * (0.75 + 0.25 * (double)tiles(256) / (CUS * r));  // a chip not full runs faster
-    if (SYM) cost[T192] = 32.3 * rounds(192);
+    if (SYM) cost[T192] = 33.5 * rounds(192);
     cost[T128_2] = at_least(16.2 * rounds(128), 19.3);
     cost[T128_4] = (rounds(128) > 1 ? 19.0 : 14.6) * rounds(128);
     cost[T64_2] = at_least(6.1 * rounds(64), 12.8);
