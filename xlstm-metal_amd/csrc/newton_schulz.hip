@@ -238,7 +238,7 @@ __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
 }
 
-enum Product { XXT, AA, PX, LAST };  // A; P; X; the result
+enum Product { XXT, XXT_PART, XXT_JOIN, AA, PX, LAST };  // A, a part of its sums, A from the parts; P; X; the result
 
 // sum[l][r] over k of left[l][k] right[r][k]
 struct Args {
@@ -247,6 +247,9 @@ struct Args {
   int64_t left_plane, right_plane, left_batch, right_batch;
   int lefts, rights, K;     // multiples of 64
   int left_tiles, right_tiles;
+  // XXT_PART, XXT_JOIN: parts of K, their sums by [tile][split]
+  int splits;
+  float* partial;
   // value = beta * e + alpha * sum; e as out
   const f16_t* e;
   int64_t e_plane, e_batch;
@@ -275,7 +278,7 @@ struct Args {
 template <int BL, int BR, int WL, int WR, int STAGES, int PL, int MODE, typename T>
 __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
   constexpr int THREADS = 64 * WL * WR, BK = 64, TL = BL / WL / 16, TR = BR / WR / 16;
-  constexpr bool SYM = MODE == XXT || MODE == AA, COLUMNS = !SYM;  // left by columns
+  constexpr bool IS_A = MODE == XXT || MODE == XXT_PART || MODE == XXT_JOIN, SYM = IS_A || MODE == AA, COLUMNS = !SYM;  // left by columns
   constexpr int PLANE = (BL + BR) * 128, STAGE = PLANE * PL;
   constexpr int PER = THREADS / 8;         // rows of 128 bytes by one load of the workgroup
   constexpr int PER_K = THREADS * 8 / BL;  // rows k of BL columns by one
@@ -287,7 +290,9 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
 
   // neighbours share operands, on one XCD
   const int tiles = SYM ? p.left_tiles * (p.left_tiles + 1) / 2 : p.left_tiles * p.right_tiles;
-  const int g = mfma::xcd_contiguous(blockIdx.x, gridDim.x), b = __builtin_amdgcn_readfirstlane(g / tiles), t = g - b * tiles;
+  const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
+  const int g = MODE == XXT_PART ? __builtin_amdgcn_readfirstlane(all / p.splits) : all;
+  const int b = __builtin_amdgcn_readfirstlane(g / tiles), t = g - b * tiles;
   int bl, br;
   if constexpr (SYM) {
     bl = (int)((sqrtf(8.f * t + 1.f) - 1.f) * 0.5f);
@@ -309,6 +314,14 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
   constexpr int PIECES = BL / 8, KEYS = BL >= 128 ? 7 : 3;  // 16-byte pieces of a row k; the key's bits
   uint32_t from_l[LOADS_L], from_r[BR / PER];
   const char *lp = (const char*)(p.left + b * p.left_batch), *rp = (const char*)(p.right + b * p.right_batch) + br * BR * ld;
+  int slices = p.K / BK, split = 0;
+  if constexpr (MODE == XXT_PART) {
+    split = all - g * p.splits;
+    const int first = __builtin_amdgcn_readfirstlane(slices * split / p.splits);
+    slices = __builtin_amdgcn_readfirstlane(slices * (split + 1) / p.splits) - first;
+    lp += first * (BK * 2);
+    rp += first * (BK * 2);
+  }
   if constexpr (COLUMNS) {
     const int k = tid / PIECES, at = tid % PIECES, key = ((k & 3) | ((k >> 1) & 4)) & KEYS;
     const int column = bl * BL + ((((at >> 1) ^ key) << 1) | (at & 1)) * 8;
@@ -384,8 +397,18 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
   };
   // Past the end the last slice is loaded again, into a place that is not read: the same number of loads is under way
   // after every slice.
-  const int slices = p.K / BK;
   using Behind = std::integral_constant<int, LOADS*(STAGES - 2)>;
+  // a lane's sums of a part: one f32x4 a block, the workgroup's side by side
+  auto part_at = [&](int of, int block) {
+    return (f32x4*)p.partial + (((int64_t)g * p.splits + of) * (TL * TR) + block) * THREADS + tid;
+  };
+  if constexpr (MODE == XXT_JOIN) {
+    for (int of = 0; of < p.splits; ++of)
+#pragma unroll
+      for (int i = 0; i < TL; ++i)
+#pragma unroll
+        for (int j = 0; j < TR; ++j) acc[i][j] += *part_at(of, i * TR + j);
+  } else {
   Half h0, h1;
 #pragma unroll
   for (int k = 0; k < STAGES - 1; ++k)
@@ -404,12 +427,20 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
     stage = next;
   }
   landed(std::integral_constant<int, 0>{});
+  }
+  if constexpr (MODE == XXT_PART) {
+#pragma unroll
+    for (int i = 0; i < TL; ++i)
+#pragma unroll
+      for (int j = 0; j < TR; ++j) *part_at(split, i * TR + j) = acc[i][j];
+    return;
+  }
 
   // A lane has left 4 quad .. 4 quad + 3 of right `row` of each block.
   const Factors f = p.factors[b];
   const float u = p.first ? f.first : f.later;
   float alpha = p.alpha, beta = p.beta;
-  if constexpr (MODE == XXT) alpha *= u * u;
+  if constexpr (IS_A) alpha *= u * u;
   if constexpr (MODE == PX) {
     alpha *= u / f.later;
     beta *= u / f.later;
@@ -465,7 +496,7 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
 #pragma unroll
       for (int i = 0; i < TL; ++i) *(f32x4*)(strip + row * (TL * 16 + 4) + i * 16 + quad * 4) = acc[i][j] * alpha;
       wave_fence();
-      out_rows(std::integral_constant<int, TL>{}, r0 + j * 16, p.rights, l0, p.lefts, MODE != XXT);
+      out_rows(std::integral_constant<int, TL>{}, r0 + j * 16, p.rights, l0, p.lefts, !IS_A);
     }
   }
   if ((SYM && bl != br) || (MODE == LAST && p.result_turned)) {
@@ -689,10 +720,23 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
 }
 
 // ------------------------------------------------------------------------------------------------ host
+constexpr int CUS = 256;
+// Parts of X X^T's long sums, where its tiles of 64 x 64 leave CUs idle: a slice of K takes 0.2 us (a pair 0.43) on its
+// own, the second launch that adds the parts up 4; a part keeps some slices.  64 x 8000 bf16 153 us whole, 114 so;
+// 300 x 5000 152 and 136; 200 x 3000, near the limit, the same.
+int splits_of(int64_t batch, int Mp, int Np, int planes) {
+  const int64_t t = Mp / 64, tiles = t * (t + 1) / 2 * batch;
+  const int slices = Np / 64, least = planes == 1 ? 6 : 4;
+  if (slices < (planes == 1 ? 28 : 14) || tiles > CUS / 2) return 1;
+  const int64_t most = CUS / tiles;
+  return (int)(most < slices / least ? most : slices / least);
+}
+
 struct Plan {
+  int splits;
   int planes, M, N, Mp, Np;  // M <= N; padded to multiples of 64
   int64_t x, a;              // elements of a plane of X, of A (P), all matrices
-  int64_t parts_at, factors_at, x_at[2], a_at, p_at;  // bytes into the workspace
+  int64_t parts_at, factors_at, x_at[2], a_at, p_at, partial_at;  // bytes into the workspace
   size_t bytes;
 };
 
@@ -727,6 +771,9 @@ Plan plan_of(int64_t batch, int m, int n, int dtype) {
   for (int64_t& x : p.x_at) x = take(2 * p.x * 2);  // X has its lo plane in some steps of one-plane products too
   p.a_at = take(2 * p.a * p.planes);
   p.p_at = take(2 * p.a * p.planes);
+  p.splits = splits_of(batch, p.Mp, p.Np, p.planes);
+  const int64_t t = p.Mp / 64;
+  p.partial_at = take(p.splits > 1 ? batch * (t * (t + 1) / 2) * p.splits * 64 * 64 * 4 : 0);
   p.bytes = (size_t)at;
   return p;
 }
@@ -744,8 +791,9 @@ int launch_tiles(Args a, int64_t batch, hipStream_t st) {
   }
   a.left_tiles = (a.lefts + BL - 1) / BL;
   a.right_tiles = (a.rights + BR - 1) / BR;
-  const int64_t tiles = MODE == XXT || MODE == AA ? (int64_t)a.left_tiles * (a.left_tiles + 1) / 2
-                                                  : (int64_t)a.left_tiles * a.right_tiles;
+  const bool sym = MODE != PX && MODE != LAST;
+  const int64_t tiles = (sym ? (int64_t)a.left_tiles * (a.left_tiles + 1) / 2 : (int64_t)a.left_tiles * a.right_tiles) *
+                        (MODE == XXT_PART ? a.splits : 1);
   if (tiles * batch > 0x7fffff) return set_error(XL_ERR_UNSUPPORTED, "xl_newton_schulz: batch too large");
   hipLaunchKernelGGL(kernel, dim3((unsigned)(tiles * batch)), dim3(64 * WL * WR), LDS, st, a);
   return check_launch("xl_newton_schulz");
@@ -766,7 +814,11 @@ int launch_tiles(Args a, int64_t batch, hipStream_t st) {
 template <int PL, int MODE, typename T>
 int launch_product(const Args& a, int64_t batch, hipStream_t st) {
   constexpr bool SYM = MODE == XXT || MODE == AA;
-  constexpr int CUS = 256;
+  if constexpr (MODE == XXT)
+    if (a.splits > 1) {
+      const int rc = launch_tiles<64, 64, 2, 2, 4, PL, XXT_PART, T>(a, batch, st);
+      return rc ? rc : launch_tiles<64, 64, 2, 2, 4, PL, XXT_JOIN, T>(a, batch, st);
+    }
   auto tiles = [&](int tile) {
     const int64_t l = (a.lefts + tile - 1) / tile, r = (a.rights + tile - 1) / tile;
     return (SYM ? l * (l + 1) / 2 : l * r) * batch;
@@ -875,6 +927,8 @@ int run(const void* g, void* x, int64_t batch, int m, int n, const float* coeffi
     k.left_batch = k.right_batch = xb;
     k.lefts = k.rights = p.Mp;
     k.K = p.Np;
+    k.splits = p.splits;
+    k.partial = (float*)(ws + p.partial_at);
     k.alpha = SCALE_A;
     k.out = A;
     k.out_plane = p.a;
