@@ -30,7 +30,7 @@ def iterate(G, triples, eps=1e-7):
 
 def rounded(G, triples, pairs):
     """The iteration in 64 bits with the kernels' stored matrices: X, A and P in f16 (X and the linear term of the middle
-    steps as a pair; with `pairs` all of them)."""
+    steps as a pair, P's diagonal apart; with `pairs` all of them as pairs)."""
     def store(x, scale):
         hi = (x * scale).to(F16).double()
         return hi / scale, (x * scale - hi).to(F16).double() / scale
@@ -46,9 +46,11 @@ def rounded(G, triples, pairs):
     for k, (a, b, c) in enumerate(triples):
         A = store(product(S, S), 256.0)
         full = A[0] + (A[1] if pairs else 0.0)
-        P = store(b * full + c * product(A, A), 64.0)
+        P = b * full + c * product(A, A)
+        D = torch.zeros_like(P[..., :1]) if pairs else torch.diagonal(P, dim1=-2, dim2=-1).unsqueeze(-1)
+        P = store(P - torch.diag_embed(D.squeeze(-1)), 64.0)
         linear = S[0] + (S[1] if pairs or 1 <= k <= len(triples) - 3 else 0.0)
-        X = a * linear + product(P, tuple(t.mT for t in S))
+        X = (a + D) * linear + product(P, tuple(t.mT for t in S))
         S = store(X, 256.0)
     return X.mT if G.shape[-2] > G.shape[-1] else X
 

@@ -5,7 +5,8 @@
 // on the side with fewer rows (G^T for a tall G), so that every singular value s goes to s (a + b s^2 + c s^4) a step.
 // The products are on the matrix cores in f16 with float32 sums.  Every matrix is kept at a power-of-two scale that
 // holds it in f16's range; a bf16 G enters exactly, its results' own rounding (1.65e-3 of the norm) is larger than what
-// the f16 intermediates add (bf16 intermediates: 1e-2 to 3e-2).  For f16 and float32 every matrix is a pair
+// the f16 intermediates add (1.95e-3 in all; bf16 intermediates: 1e-2 to 3e-2).  P's diagonal, its largest values, stays
+// in float32 beside it and joins a (2.35e-3 with it in f16).  For f16 and float32 every matrix is a pair
 // hi + lo of f16 (22 bits) and a product three (hi hi + hi lo + lo hi), 4e-7 of the norm.
 //
 // A and P are symmetric: their tiles on and below the diagonal are computed and written to both places.  X is kept
@@ -255,6 +256,7 @@ struct Args {
   int64_t e_plane, e_batch;
   int e_planes;
   float alpha, beta;
+  float* diagonal;  // one plane: P's [batch, Mp], at P's scale; AA writes it and zeros in P, PX and LAST add it to beta
   const Factors* factors;
   bool first;
   // out [rights, lefts] (A, P: [lefts, rights] too, which is the other triangle)
@@ -451,6 +453,7 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
   }
   const int l0 = bl * BL + wl * TL * 16, r0 = br * BR + wr * TR * 16;
   const f16_t* e = p.e + b * p.e_batch;
+  float* diagonal = p.diagonal + (int64_t)b * p.rights;
   // 16 rows of [rows, 8 * EACH columns] at a time, turned in the wave's own part of LDS: 16 bytes a lane, whole lines
   constexpr int WIDE = TL > TR ? TL : TR, STRIP = 16 * (WIDE * 16 + 4);
   float* strip = (float*)lds + wave * STRIP;
@@ -467,9 +470,19 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
         const f16x8 hi = *(const f16x8*)(e + from);
         f16x8 lo = {};
         if (p.e_planes == 2) lo = *(const f16x8*)(e + p.e_plane + from);
+        const float rate = MODE == AA || PL == 2 ? beta : fmaf(alpha, diagonal[m], beta);
 #pragma unroll
-        for (int q = 0; q < 8; ++q) v[q] = fmaf(beta, (float)hi[q] + (float)lo[q], v[q]);
+        for (int q = 0; q < 8; ++q) v[q] = fmaf(rate, (float)hi[q] + (float)lo[q], v[q]);
       }
+      if constexpr (MODE == AA && PL == 1)
+        if (bl == br) {
+#pragma unroll
+          for (int q = 0; q < 8; ++q)
+            if (m == n + q) {
+              diagonal[m] = v[q];
+              v[q] = 0.f;
+            }
+        }
       if constexpr (MODE == LAST) {
         const int R = p.result_turned ? p.cols : p.rows, C = p.result_turned ? p.rows : p.cols;
         if (m >= R || n >= C) continue;
@@ -512,8 +525,9 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
           const f16x4 hi = *(const f16x4*)(e + from);
           f16x4 lo = {};
           if (p.e_planes == 2) lo = *(const f16x4*)(e + p.e_plane + from);
+          const float rate = PL == 2 ? beta : fmaf(alpha, diagonal[r], beta);
 #pragma unroll
-          for (int q = 0; q < 4; ++q) v[q] = fmaf(beta, (float)hi[q] + (float)lo[q], v[q]);
+          for (int q = 0; q < 4; ++q) v[q] = fmaf(rate, (float)hi[q] + (float)lo[q], v[q]);
         }
 #pragma unroll
         for (int q = 0; q < 4; ++q) strip[(quad * 4 + q) * (TR * 16 + 4) + j * 16 + row] = v[q];
@@ -541,6 +555,7 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
   extern __shared__ __align__(1024) char lds[];
   char *xs = lds, *as = lds + PL * X_PLANE;
   double* sums = (double*)as;
+  float* diagonal = (float*)(as + PL * A_PLANE);  // P's
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, wl = wave / SMALL_WR, wr = wave % SMALL_WR;
   const int row = lane & 15, quad = lane >> 4;
   g += (int64_t)blockIdx.x * rows * cols;
@@ -684,6 +699,10 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
           // one plane: A as it was multiplied
           const float a = PL == 1 ? (float)(_Float16)acc[i][j][q] : acc[i][j][q];
           v[q] = fmaf(pb, a, pc * sq[i][j][q]);
+          if (PL == 1 && (wr * TR + j) * 16 + row == (wl * TA + i) * 16 + 4 * quad + q) {
+            diagonal[(wr * TR + j) * 16 + row] = v[q];
+            v[q] = 0.f;
+          }
         }
         put(as, A_PLANE, D, (wr * TR + j) * 16 + row, (wl * TA + i) * 16 + 4 * quad, v);
       }
@@ -693,12 +712,14 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
     const bool last = step + 1 == steps, fine = PL == 2 || (step >= 1 && step <= steps - 3);
     const float to = last ? u : u / f.later, a = co.v[3 * step] * to, b = to / SCALE_P;
 #pragma unroll
-    for (int i = 0; i < TX; ++i)
+    for (int j = 0; j < TR; ++j) {
+      const float rate = PL == 1 ? fmaf(b, diagonal[(wr * TR + j) * 16 + row], a) : a;
 #pragma unroll
-      for (int j = 0; j < TR; ++j)
+      for (int i = 0; i < TX; ++i)
 #pragma unroll
         for (int q = 0; q < 4; ++q)
-          x[i][j][q] = fmaf(a, fine ? x[i][j][q] : (float)(_Float16)x[i][j][q], b * px[i][j][q]);
+          x[i][j][q] = fmaf(rate, fine ? x[i][j][q] : (float)(_Float16)x[i][j][q], b * px[i][j][q]);
+    }
   }
 #pragma unroll
   for (int i = 0; i < TX; ++i)
@@ -736,7 +757,7 @@ struct Plan {
   int splits;
   int planes, M, N, Mp, Np;  // M <= N; padded to multiples of 64
   int64_t x, a;              // elements of a plane of X, of A (P), all matrices
-  int64_t parts_at, factors_at, x_at[2], a_at, p_at, partial_at;  // bytes into the workspace
+  int64_t parts_at, factors_at, x_at[2], a_at, p_at, diagonal_at, partial_at;  // bytes into the workspace
   size_t bytes;
 };
 
@@ -771,6 +792,7 @@ Plan plan_of(int64_t batch, int m, int n, int dtype) {
   for (int64_t& x : p.x_at) x = take(2 * p.x * 2);  // X has its lo plane in some steps of one-plane products too
   p.a_at = take(2 * p.a * p.planes);
   p.p_at = take(2 * p.a * p.planes);
+  p.diagonal_at = take(p.planes == 1 ? batch * p.Mp * 4 : 0);
   p.splits = splits_of(batch, p.Mp, p.Np, p.planes);
   const int64_t t = p.Mp / 64;
   p.partial_at = take(p.splits > 1 ? batch * (t * (t + 1) / 2) * p.splits * 64 * 64 * 4 : 0);
@@ -858,7 +880,7 @@ int launch_product(const Args& a, int64_t batch, hipStream_t st) {
 template <int D, int N, int PL, typename T>
 int launch_small(const void* g, void* x, int64_t batch, int m, int n, const Coefficients& co, int steps, float eps,
                  double growth, hipStream_t st) {
-  constexpr int LDS = PL * (D * N + D * D) * 2;
+  constexpr int LDS = PL * (D * N + D * D) * 2 + D * 4;
   static_assert(LDS <= 160 * 1024);
   auto kernel = m > n ? ns_small_kernel<D, N, PL, true, T> : ns_small_kernel<D, N, PL, false, T>;
   if (LDS > 64 * 1024) {
@@ -922,6 +944,7 @@ int run(const void* g, void* x, int64_t batch, int m, int n, const float* coeffi
     Args k{};
     k.factors = factors;
     k.first = s == 0;
+    k.diagonal = (float*)(ws + p.diagonal_at);
     k.left = k.right = old;
     k.left_plane = k.right_plane = p.x;
     k.left_batch = k.right_batch = xb;
