@@ -49,7 +49,7 @@ def rounded(G, triples, pairs):
         P = b * full + c * product(A, A)
         D = torch.zeros_like(P[..., :1]) if pairs else torch.diagonal(P, dim1=-2, dim2=-1).unsqueeze(-1)
         P = store(P - torch.diag_embed(D.squeeze(-1)), 64.0)
-        linear = S[0] + (S[1] if pairs or 1 <= k <= len(triples) - 3 else 0.0)
+        linear = S[0] + (S[1] if pairs or 1 <= k <= len(triples) - 2 else 0.0)
         X = (a + D) * linear + product(P, tuple(t.mT for t in S))
         S = store(X, 256.0)
     return X.mT if G.shape[-2] > G.shape[-1] else X
