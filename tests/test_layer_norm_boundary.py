@@ -27,7 +27,8 @@ def test_forward_refuses(lib):
     assert fwd(lib, x=None) == -1 and b"null" in lib.xl_last_error()
     assert fwd(lib, y=P) == -1 and b"alias" in lib.xl_last_error()
     assert fwd(lib, n=(1 << 16, 1 << 16)) == -2
-    assert fwd(lib, H=1 << 16, D=1 << 16) == -2
+    assert fwd(lib, H=1 << 13, D=1 << 14) == -2
+    assert fwd(lib, H=(1 << 20) + 1, D=1) == -2
     assert fwd(lib, n=(1 << 62, 1 << 62)) == -2
     assert fwd(lib, n=(0, 7)) == 0  # no rows
 

@@ -565,9 +565,9 @@ int shape_of(const char* who, int64_t n0, int64_t n1, int H, int D, int dtype, i
   if (!dtype_ok(dtype) || (param_dtype != dtype && param_dtype != XL_DTYPE_F32))
     return set_error(XL_ERR_INVALID_ARG, "%s: dtype %d with weights of dtype %d (the same one, or float32)", who, dtype,
                      param_dtype);
-  const int64_t most = 0x7fffffff;
-  if (n0 > most || n1 > most || n0 * n1 > most / H || (int64_t)H * D > most)
-    return set_error(XL_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows, or values per token", who);
+  const int64_t most = 0x7fffffff, widest = 1 << 26;  // what the grids of the column kernels take
+  if (n0 > most || n1 > most || n0 * n1 > most / H || H > (1 << 20) || (int64_t)H * D > widest)
+    return set_error(XL_ERR_UNSUPPORTED, "%s: more than 2^31 - 1 rows, 2^20 heads or 2^26 values per token", who);
   s = Shape{(int)(n0 * n1), (int)(n1 ? n1 : 1), H, D};
   p32 = param_dtype == XL_DTYPE_F32;
   return XL_OK;

@@ -229,7 +229,9 @@ __global__ __launch_bounds__(256) void ns_enter_kernel(const T* __restrict__ g, 
 }
 
 // ------------------------------------------------------------------------------------------------ the products
-// 16 bytes a lane from global memory into LDS, at lds + 16 * lane (lds the same in the whole wave)
+// 16 bytes a lane from global memory into LDS, at lds + 16 * lane (lds the same in the whole wave).  Written out, so that
+// the compiler does not wait for it before the next LDS read; nothing else here uses m0.  Whoever reads what it writes
+// waits for it by vmcnt, and then for everybody at a barrier.
 __device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const void* base) {
   asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
@@ -313,7 +315,10 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
   // where this lane's loads come from: byte offsets from the operands' first slice
   const int64_t ld = (int64_t)p.K * 2, ldx = (int64_t)p.lefts * 2;
   const int piece = ((tid & 7) ^ ((tid >> 3) & 7)) * 16;
-  constexpr int PIECES = BL / 8, KEYS = BL >= 128 ? 7 : 3;  // 16-byte pieces of a row k; the key's bits
+  constexpr int PIECES = BL / 8;  // 16-byte pieces of a row k
+  // 64 columns: a row is half the banks, so rows of one parity need the keys (with k % 4 a third of the LDS cycles of a
+  // float32 P X were conflicts; 4 of 768 x 2048 2 % slower)
+  auto key_of = [](int k) { return BL >= 128 ? (k & 3) | ((k >> 1) & 4) : ((k >> 1) & 1) | ((k >> 2) & 2); };
   uint32_t from_l[LOADS_L], from_r[BR / PER];
   const char *lp = (const char*)(p.left + b * p.left_batch), *rp = (const char*)(p.right + b * p.right_batch) + br * BR * ld;
   int slices = p.K / BK, split = 0;
@@ -325,7 +330,7 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
     rp += first * (BK * 2);
   }
   if constexpr (COLUMNS) {
-    const int k = tid / PIECES, at = tid % PIECES, key = ((k & 3) | ((k >> 1) & 4)) & KEYS;
+    const int k = tid / PIECES, at = tid % PIECES, key = key_of(k);
     const int column = bl * BL + ((((at >> 1) ^ key) << 1) | (at & 1)) * 8;
     from_l[0] = (uint32_t)(k * ldx + min(column, p.lefts - 8) * 2);
   } else {
@@ -360,7 +365,7 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
     f16x8 l[PL][TL], r[PL][TR];
   };
   const int by_row = row * 128 + ((quad ^ (row & 7)) << 4);
-  const int by_column = (quad * 8 + (row >> 2)) * (BL * 2) + ((((row >> 2) | ((quad & 1) << 2)) & KEYS) ^ (wl * TL)) * 32 + (row & 3) * 8;
+  const int by_column = (quad * 8 + (row >> 2)) * (BL * 2) + (key_of(quad * 8 + (row >> 2)) ^ (wl * TL)) * 32 + (row & 3) * 8;
   // read I of half s of the slice at LDS offset `base`: 8 values along k, from 32 s + 8 quad, of a row or a column
   auto read_one = [&](auto I, Half& h, int base, int s) {
     constexpr int pl = I.value / (TL + TR), i = I.value % (TL + TR);

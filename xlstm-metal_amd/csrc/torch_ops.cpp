@@ -793,8 +793,9 @@ struct LayerNormFn : public torch::autograd::Function<LayerNormFn> {
 
 TwoTensors layer_norm_autograd(const Tensor& x, const OptTensor& w, const OptTensor& b, double eps, c10::SymInt layout) {
   bool any = false;
+  const bool recorded = c10::GradMode::is_enabled();
   for (const Tensor* t : {&x, opt(w), opt(b)})
-    any = any || (t && t->defined() && (t->requires_grad() || t->_fw_grad(0).defined()));
+    any = any || (t && t->defined() && ((recorded && t->requires_grad()) || t->_fw_grad(0).defined()));
   if (!any) return call_layer_norm(x, w, b, eps, layout);
   const auto r = LayerNormFn::apply(x, w, b, eps, layout);
   return {r[0], r[1]};
