@@ -13,6 +13,12 @@
 // by rows; P X reads it down its columns with LDS reads that transpose.  All matrices are zero-padded to multiples of
 // 64 in the workspace, and a tile past the end reads its last rows again: no bounds in the loops, and products of
 // zeros stay zero.
+//
+// Large matrices are bound by the matrix cores (4096 x 4096 bf16: P X 111 us, 1240 TFLOP/s, where a library f16 product
+// takes 109) and, in the symmetric products' smaller tiles, by LDS reads; middling ones in batches by memory (12 of
+// 1024 x 2048: P X 70 us, 300 MB); small ones by latency and launches.  us for five steps: 4096 x 4096 1300, 10944 x 4096
+// 2900, 12 of 1024 x 2048 700, 1777 x 1000 float32 225, 512 x 512 90, 128 x 128 28 (the products with torch in float32:
+// 14410, 32260, 5564, 633, 490, 491).
 #include <math.h>
 
 #include <type_traits>
