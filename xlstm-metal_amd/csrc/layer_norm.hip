@@ -10,9 +10,9 @@
 // Both passes are streams: x in, y out (2 values moved a value), then x, dy in, dx out (3).  A row is read once into the
 // registers of a team of lanes, so mean and variance cost no second read; weights stay in registers over a workgroup's
 // rows; the backward keeps the columns' sums there too and writes them once (float32, a workgroup's rows), for a short
-// second launch to join.  Measured (us; torch's copy of the same bytes runs at 5.13 TB/s): 8192 x 4096 bf16 forward 25.0
-// (5.4 TB/s), backward 50.3 (4.0 TB/s; x + dy -> dx as torch.add takes 36.7, without the weight's gradient 45.9);
-// 8192 tokens of 8 heads of 512 forward 26.1, backward 45.6; 8 x 4096, one token each, 3.8 (latency).
+// second launch to join.  Measured (us; torch's copy of the same bytes runs at 5.13 TB/s): 8192 x 4096 bf16 forward 23.6
+// (5.7 TB/s), backward 49.3 (4.1 TB/s; x + dy -> dx as torch.add takes 36.7, without the weight's gradient 42.1);
+// 8192 tokens of 8 heads of 512 forward 26.8, backward 45.6; 8 x 4096, one token each, 3.8 (latency).
 #include <type_traits>
 
 #include "common.h"
@@ -225,7 +225,7 @@ __global__ __launch_bounds__(BLOCK) void ln_fwd_kernel(const T* __restrict__ x, 
 
 // The backward pass of the same teams: dx of a row from its registers, and over the rows of a workgroup the sums of dy h
 // and dy for every column, written once as part[slice][0 / 1][H * D].
-template <typename T, int VW, int TL, int NV, int BLOCK, bool AHEAD>
+template <typename T, int VW, int TL, int NV, int BLOCK, bool AHEAD, bool STREAM>
 __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(const T* __restrict__ dy, const T* __restrict__ x, Rows xr,
                                                        const void* __restrict__ w, bool p32, const float* __restrict__ mean,
                                                        const float* __restrict__ rstd, T* __restrict__ dx, Rows dxr,
@@ -297,7 +297,7 @@ __global__ __launch_bounds__(BLOCK) void ln_bwd_kernel(const T* __restrict__ dy,
         const float h = (to_f32(xv[k].e[j]) - mu) * rs;
         f[j] = rs * (to_f32(dv[k].e[j]) * wv[k][j] - c1 - h * c2);
       }
-      store_vec<false>(op + c.at[k], f);
+      store_vec<STREAM>(op + c.at[k], f);
     }
   }
   if (!part) return;
@@ -508,6 +508,14 @@ void with_layout(const Layout& l, F&& f) {
 #undef XL_LN
 }
 
+// An output of half the L2 caches (8 of 4 MiB) or more goes past them.  us through them and past them, bf16: forward
+// 8192 x 4096 27.9 and 23.6, 8192 x 2048 14.0 and 12.7, 8192 x 1536 11.6 and 9.5; backward 50.4 and 49.3, 30.7 and 27.8,
+// 27.2 and 24.3.  What is smaller stays for its reader.
+template <typename T>
+bool streams(const Shape& s) {
+  return (int64_t)s.tokens * s.H * s.D * (int64_t)sizeof(T) >= (int64_t)16 << 20;
+}
+
 template <typename T>
 int launch_fwd(const void* x, const Rows& xr, const void* w, const void* b, bool p32, void* y, float* mean, float* rstd,
                const Shape& s, float eps, int dtype, hipStream_t st) {
@@ -517,9 +525,7 @@ int launch_fwd(const void* x, const Rows& xr, const void* w, const void* b, bool
                        w, b, p32, (T*)y, mean, rstd, s, eps);
   } else {
     const int slices = fwd_slices(s, l);
-    // An output larger than the L2 caches (8 of 4 MiB) goes past them: 64 MiB of bf16 at 4096 / 8192 columns 26.3 / 23.2 us
-    // so, 28.1 / 28.4 through them (the backward's dx: no difference).  What is smaller stays for its reader.
-    const bool stream = (int64_t)s.tokens * s.H * s.D * (int64_t)sizeof(T) > (int64_t)32 << 20;
+    const bool stream = streams<T>(s);
     with_layout<T, false>(l, [&](auto VW, auto TL, auto NV, auto BLOCK) {
       auto kernel = stream ? ln_fwd_kernel<T, VW.value, TL.value, NV.value, BLOCK.value, true>
                            : ln_fwd_kernel<T, VW.value, TL.value, NV.value, BLOCK.value, false>;
@@ -546,9 +552,11 @@ int launch_bwd(const void* dy, const void* x, const Rows& xr, const void* w, boo
                          dim3(LN_BLOCK), 0, st, (const T*)dy, (const T*)x, xr, mean, rstd, part, s, slices);
   } else {
     with_layout<T, true>(l, [&](auto VW, auto TL, auto NV, auto BLOCK) {
-      hipLaunchKernelGGL((ln_bwd_kernel<T, VW.value, TL.value, NV.value, BLOCK.value, (BLOCK.value < 1024)>), dim3((unsigned)slices * s.H),
-                         dim3(BLOCK.value), 0, st, (const T*)dy, (const T*)x, xr, w, p32, mean, rstd, (T*)dx, dxr, part, s,
-                         slices);
+      constexpr bool AHEAD = BLOCK.value < 1024;
+      auto kernel = streams<T>(s) ? ln_bwd_kernel<T, VW.value, TL.value, NV.value, BLOCK.value, AHEAD, true>
+                                  : ln_bwd_kernel<T, VW.value, TL.value, NV.value, BLOCK.value, AHEAD, false>;
+      hipLaunchKernelGGL(kernel, dim3((unsigned)slices * s.H), dim3(BLOCK.value), 0, st, (const T*)dy, (const T*)x, xr, w, p32,
+                         mean, rstd, (T*)dx, dxr, part, s, slices);
     });
   }
   if (part)

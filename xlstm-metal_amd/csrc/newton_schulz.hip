@@ -5,7 +5,7 @@
 // on the side with fewer rows (G^T for a tall G), so that every singular value s goes to s (a + b s^2 + c s^4) a step.
 // The products are on the matrix cores in f16 with float32 sums.  Every matrix is kept at a power-of-two scale that
 // holds it in f16's range; a bf16 G enters exactly, its results' own rounding (1.65e-3 of the norm) is larger than what
-// the f16 intermediates add (1.95e-3 in all; bf16 intermediates: 1e-2 to 3e-2).  P's diagonal, its largest values, stays
+// the f16 intermediates add (2.0e-3 in all; bf16 intermediates: 1e-2 to 3e-2).  P's diagonal, its largest values, stays
 // in float32 beside it and joins a (2.35e-3 with it in f16).  For f16 and float32 every matrix is a pair
 // hi + lo of f16 (22 bits) and a product three (hi hi + hi lo + lo hi), 4e-7 of the norm.
 //
@@ -17,8 +17,8 @@
 // Large matrices are bound by the matrix cores (4096 x 4096 bf16: P X 111 us, 1240 TFLOP/s, where a library f16 product
 // takes 109) and, in the symmetric products' smaller tiles, by LDS reads; middling ones in batches by memory (12 of
 // 1024 x 2048: P X 70 us, 300 MB); small ones by latency and launches.  us for five steps: 4096 x 4096 1300, 10944 x 4096
-// 2900, 12 of 1024 x 2048 700, 1777 x 1000 float32 225, 512 x 512 90, 128 x 128 28 (the products with torch in float32:
-// 14410, 32260, 5564, 633, 490, 491).
+// 2900, 12 of 1024 x 2048 700, 1777 x 1000 float32 225, 128 x 128 28 (the products with torch in float32:
+// 14410, 32260, 5564, 633, 491).
 #include <math.h>
 
 #include <type_traits>
