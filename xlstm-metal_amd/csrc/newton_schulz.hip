@@ -236,10 +236,10 @@ __global__ __launch_bounds__(256) void ns_enter_kernel(const T* __restrict__ g, 
 
 // ------------------------------------------------------------------------------------------------ the products
 // 16 bytes a lane from global memory into LDS, at lds + 16 * lane (lds the same in the whole wave).  Written out, so that
-// the compiler does not wait for it before the next LDS read; nothing else here uses m0.  Whoever reads what it writes
-// waits for it by vmcnt, and then for everybody at a barrier.
+// the compiler does not wait for it before the next LDS read; nothing else here uses m0, which has to be written one
+// wait state before the load.  Whoever reads what it writes waits for it by vmcnt, and then for everybody at a barrier.
 __device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const void* base) {
-  asm volatile("s_mov_b32 m0, %0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 __device__ __forceinline__ void wave_fence() {
   __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
@@ -288,7 +288,8 @@ struct Args {
 template <int BL, int BR, int WL, int WR, int STAGES, int PL, int MODE, typename T>
 __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
   constexpr int THREADS = 64 * WL * WR, BK = 64, TL = BL / WL / 16, TR = BR / WR / 16;
-  constexpr bool IS_A = MODE == XXT || MODE == XXT_PART || MODE == XXT_JOIN, SYM = IS_A || MODE == AA, COLUMNS = !SYM;  // left by columns
+  constexpr bool IS_A = MODE == XXT || MODE == XXT_PART || MODE == XXT_JOIN, SYM = IS_A || MODE == AA;
+  constexpr bool COLUMNS = !SYM;  // left by columns
   constexpr int PLANE = (BL + BR) * 128, STAGE = PLANE * PL;
   constexpr int PER = THREADS / 8;         // rows of 128 bytes by one load of the workgroup
   constexpr int PER_K = THREADS * 8 / BL;  // rows k of BL columns by one
@@ -371,7 +372,7 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
     f16x8 l[PL][TL], r[PL][TR];
   };
   const int by_row = row * 128 + ((quad ^ (row & 7)) << 4);
-  const int by_column = (quad * 8 + (row >> 2)) * (BL * 2) + (key_of(quad * 8 + (row >> 2)) ^ (wl * TL)) * 32 + (row & 3) * 8;
+  const int first_k = quad * 8 + (row >> 2), by_column = first_k * (BL * 2) + (key_of(first_k) ^ (wl * TL)) * 32 + (row & 3) * 8;
   // read I of half s of the slice at LDS offset `base`: 8 values along k, from 32 s + 8 quad, of a row or a column
   auto read_one = [&](auto I, Half& h, int base, int s) {
     constexpr int pl = I.value / (TL + TR), i = I.value % (TL + TR);
@@ -408,8 +409,8 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
   };
-  // Past the end the last slice is loaded again, into a place that is not read: the same number of loads is under way
-  // after every slice.
+  // Past the end the last slice is loaded again, and read, but not multiplied: the same number of loads is under way after
+  // every slice.
   using Behind = std::integral_constant<int, LOADS*(STAGES - 2)>;
   // a lane's sums of a part: one f32x4 a block, the workgroup's side by side
   auto part_at = [&](int of, int block) {
@@ -422,24 +423,24 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
 #pragma unroll
         for (int j = 0; j < TR; ++j) acc[i][j] += *part_at(of, i * TR + j);
   } else {
-  Half h0, h1;
+    Half h0, h1;
 #pragma unroll
-  for (int k = 0; k < STAGES - 1; ++k)
-    mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(k, slices - 1), k); });
-  landed(Behind{});
-  mfma::static_for<0, READS>([&](auto R) { read_one(R, h0, 0, 0); });
-  mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(STAGES - 1, slices - 1), STAGES - 1); });
-  int stage = 0;
-  for (int k = 0; k < slices; ++k) {
-    const int next = stage + 1 == STAGES ? 0 : stage + 1, ahead = min(k + STAGES, slices - 1);
-    multiply(h0, h1, stage * STAGE, 1, [](auto) {});
-    landed(Behind{});  // slice k + 1 is there, slice k has been read
-    multiply(h1, h0, next * STAGE, 0, [&](auto I) {
-      mfma::static_for<LOADS * I.value / TL, LOADS * (I.value + 1) / TL>([&](auto L) { fetch_one(L, ahead, stage); });
-    });
-    stage = next;
-  }
-  landed(std::integral_constant<int, 0>{});
+    for (int k = 0; k < STAGES - 1; ++k)
+      mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(k, slices - 1), k); });
+    landed(Behind{});
+    mfma::static_for<0, READS>([&](auto R) { read_one(R, h0, 0, 0); });
+    mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(STAGES - 1, slices - 1), STAGES - 1); });
+    int stage = 0;
+    for (int k = 0; k < slices; ++k) {
+      const int next = stage + 1 == STAGES ? 0 : stage + 1, ahead = min(k + STAGES, slices - 1);
+      multiply(h0, h1, stage * STAGE, 1, [](auto) {});
+      landed(Behind{});  // slice k + 1 is there, slice k has been read
+      multiply(h1, h0, next * STAGE, 0, [&](auto I) {
+        mfma::static_for<LOADS * I.value / TL, LOADS * (I.value + 1) / TL>([&](auto L) { fetch_one(L, ahead, stage); });
+      });
+      stage = next;
+    }
+    landed(std::integral_constant<int, 0>{});
   }
   if constexpr (MODE == XXT_PART) {
 #pragma unroll
@@ -687,7 +688,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
             f32x4{x[i][j][0], x[i][j][1], x[i][j][2], x[i][j][3]});
     __syncthreads();
     f32x4 acc[TA][TR];
-    product(acc, IntA{}, KX{}, [&](int pl, int block, int k) { return by_row(xs + pl * X_PLANE, N, block, k); }, xs, X_PLANE, N);
+    product(acc, IntA{}, KX{}, [&](int pl, int block, int k) { return by_row(xs + pl * X_PLANE, N, block, k); }, xs, X_PLANE,
+            N);
 #pragma unroll
     for (int i = 0; i < TA; ++i)
 #pragma unroll
@@ -697,7 +699,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
       }
     __syncthreads();
     f32x4 sq[TA][TR];
-    product(sq, IntA{}, KA{}, [&](int pl, int block, int k) { return by_row(as + pl * A_PLANE, D, block, k); }, as, A_PLANE, D);
+    product(sq, IntA{}, KA{}, [&](int pl, int block, int k) { return by_row(as + pl * A_PLANE, D, block, k); }, as, A_PLANE,
+            D);
     __syncthreads();  // A has been read
     const float pb = SCALE_P * co.v[3 * step + 1] / SCALE_A, pc = SCALE_P * co.v[3 * step + 2] / (SCALE_A * SCALE_A);
 #pragma unroll
@@ -719,7 +722,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
       }
     __syncthreads();
     f32x4 px[TX][TR];
-    product(px, IntX{}, KA{}, [&](int pl, int block, int k) { return by_column(xs + pl * X_PLANE, block, k); }, as, A_PLANE, D);
+    product(px, IntX{}, KA{}, [&](int pl, int block, int k) { return by_column(xs + pl * X_PLANE, block, k); }, as, A_PLANE,
+            D);
     const bool last = step + 1 == steps, fine = PL == 2 || (step >= 1 && step <= steps - 2);
     const float to = last ? u : u / f.later, a = co.v[3 * step] * to, b = to / SCALE_P;
 #pragma unroll
