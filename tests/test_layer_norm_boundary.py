@@ -33,6 +33,13 @@ def test_forward_refuses(lib):
     assert fwd(lib, n=(0, 7)) == 0  # no rows
 
 
+@pytest.mark.parametrize("eps", [-1e-6, float("nan"), float("inf")])
+def test_forward_refuses_eps(lib, eps):
+    """As the group norm does, which MultiHeadLayerNorm runs without a gradient."""
+    assert lib.xl_layer_norm_fwd(P, None, None, None, Q, None, None, 1, 4, 1, 64, eps, 1, 0, None) == -1
+    assert b"eps" in lib.xl_last_error()
+
+
 def bwd(lib, dy=P, x=Q, mean=R, rstd=R, dx=None, dw=None, n=(1, 4), H=1, D=64, ws=None, ws_bytes=0):
     return lib.xl_layer_norm_bwd(dy, x, None, None, mean, rstd, dx, None, dw, None, *n, H, D, 1, 0, ws, ws_bytes, None)
 

@@ -13,6 +13,8 @@
 // second launch to join.  Measured (us; torch's copy of the same bytes runs at 5.13 TB/s): 8192 x 4096 bf16 forward 23.6
 // (5.7 TB/s), backward 49.3 (4.1 TB/s; x + dy -> dx as torch.add takes 36.7, without the weight's gradient 42.1);
 // 8192 tokens of 8 heads of 512 forward 26.8, backward 45.6; 8 x 4096, one token each, 3.8 (latency).
+#include <math.h>
+
 #include <type_traits>
 
 #include "common.h"
@@ -598,6 +600,7 @@ extern "C" int xl_layer_norm_fwd(const void* x, const int64_t* x_strides, const 
   Shape s;
   bool p32;
   if (const int rc = shape_of(who, n0, n1, H, D, dtype, param_dtype, s, p32)) return rc;
+  if (!(eps >= 0.0f) || eps == INFINITY) return set_error(XL_ERR_INVALID_ARG, "%s: eps must be finite and >= 0", who);
   if (s.tokens == 0) return XL_OK;
   if (!x || !y) return set_error(XL_ERR_INVALID_ARG, "%s: null pointer", who);
   if (x == y) return set_error(XL_ERR_INVALID_ARG, "%s: y must not alias x", who);
