@@ -373,7 +373,8 @@ int xl_lm_head_softcap_fwd(const void* x, const void* weight, void* y, int M, in
  *   x: token (i0, i1) of head h at i0 * x_strides[0] + i1 * x_strides[1] + h * x_strides[2] (elements; values
  *   contiguous; NULL: [n0, n1, H, D] contiguous); y [n0, n1, H, D] contiguous; weight, bias [H, D] of param_dtype
  *   (dtype or XL_DTYPE_F32) or NULL; mean, rstd [n0, n1, H] float32 or NULL (what the backward needs).  Pointers
- *   aligned to their elements.  y must not overlap x.  n0 * n1 * H below 2^31, H up to 2^20, H * D up to 2^26.
+ *   aligned to their elements.  y must not overlap x.  eps finite and not negative.  n0 * n1 * H below 2^31, H up to
+ *   2^20, H * D up to 2^26.
  */
 int xl_layer_norm_fwd(const void* x, const int64_t* x_strides, const void* weight, const void* bias, void* y,
                       float* mean, float* rstd, int64_t n0, int64_t n1, int H, int D, float eps, int dtype,

@@ -276,6 +276,33 @@ def test_graph_replays(gpu_case):
         assert all(torch.equal(a, c) for a, c in zip(held, step())), f"replay {k}"
 
 
+@pytest.mark.parametrize("layout", [0, 1, 2])
+@pytest.mark.parametrize("order", ["as made", "last axis first", "heads first", "three axes", "every other", "broadcast"])
+def test_gradient_lies_as_traced(gpu_case, layout, order):
+    """dx has the strides that a traced program takes it to have, whatever x's are, and the same bits."""
+    import xlstm_hip  # noqa: F401
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    op = torch.ops.xlstm_hip.layer_norm_bwd.default
+    g = torch.Generator().manual_seed(5)
+    B, M, N, D = 3, 4, 6, 40
+    x = torch.randn(B, M, N, D, generator=g).to(dev())
+    x = {"as made": lambda: x, "last axis first": lambda: x.permute(3, 0, 1, 2).contiguous().permute(1, 2, 3, 0),
+         "heads first": lambda: x.transpose(1, 2).contiguous().transpose(1, 2),
+         "three axes": lambda: x.permute(2, 1, 0, 3).contiguous().permute(2, 1, 0, 3),
+         "every other": lambda: torch.cat([x, x], 2)[:, :, ::2], "broadcast": lambda: x[:, :1].expand(B, M, N, D)}[order]()
+    heads = (1, M, N)[layout]
+    shape = (x.shape, (B, N, M * D), (B, M, N * D))[layout]
+    dy = torch.randn(shape, generator=g).to(dev())
+    w = torch.randn(heads * D, generator=g).to(dev())
+    stats = torch.ops.xlstm_hip.layer_norm.default(x, w, None, 1e-5, layout)[1]
+    dx = op(dy, x, stats, w, None, layout, [True, True, False])[0]
+    with FakeTensorMode() as mode:
+        traced = op(*(mode.from_tensor(t) for t in (dy, x, stats, w)), None, layout, [True, True, False])[0]
+    assert dx.shape == traced.shape and dx.stride() == traced.stride()
+    plain = op(dy, x.contiguous(), stats, w, None, layout, [True, True, False])[0]
+    assert torch.equal(dx, plain)
+
+
 def test_modules_train_on_it(gpu_case):
     """MultiHeadLayerNorm, whose kernel without a gradient has none, differentiates through this norm; without a
     gradient it gives what it gave."""

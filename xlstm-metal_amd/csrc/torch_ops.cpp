@@ -724,17 +724,15 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy_, const Tenso
   auto given_or_empty = [&](bool want, const OptTensor& t) {
     return want ? at::empty(t->sizes(), t->options()) : at::empty({0}, x.options());
   };
-  // dx lies as x does where its tokens then fold as x's do: behind the chunkwise kernel it is [B, NH, S, DH] in memory
-  Tensor dx;
+  // dx lies as empty_like(x) does, written there where its tokens then fold as x's do (behind the chunkwise kernel it is
+  // [B, NH, S, DH] in memory) or are contiguous, and copied there otherwise
+  Tensor dx, to;
   bool dx_strided = false;
   if (mask[0]) {
     dx = at::empty_like(x_);
-    dx_strided = strided && as_tokens(layout == 1 ? dx.transpose(1, 2) : dx, layout != 0, dn, dst) && dn[0] == n[0] &&
-                 dn[1] == n[1];
-    if (!dx_strided) {
-      dx = at::empty(view.sizes(), x_.options());
-      if (layout == 1) dx = dx.transpose(1, 2);
-    }
+    to = layout == 1 ? dx.transpose(1, 2) : dx;
+    dx_strided = strided && as_tokens(to, layout != 0, dn, dst) && dn[0] == n[0] && dn[1] == n[1];
+    if (!dx_strided && !to.is_contiguous()) to = at::empty(view.sizes(), x_.options());
   } else {
     dx = at::empty({0}, x.options());
   }
@@ -745,9 +743,10 @@ std::tuple<Tensor, Tensor, Tensor> layer_norm_bwd(const Tensor& dy_, const Tenso
   const Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, x.options().dtype(at::kByte)) : Tensor();
   const float* mean = ptr<float>(stats);
   check_rc(xl_layer_norm_bwd(ptr(dy), ptr(x), strided ? st : nullptr, ptr(w), mean, mean + s.tokens * s.H,
-                             mask[0] ? ptr(dx) : nullptr, dx_strided ? dst : nullptr, want_w ? ptr(dw) : nullptr,
+                             mask[0] ? ptr(to) : nullptr, dx_strided ? dst : nullptr, want_w ? ptr(dw) : nullptr,
                              want_b ? ptr(db) : nullptr, n0, n1, H, D, dt, s.param, ptr(ws), ws_bytes, gpu.st),
            what);
+  if (mask[0] && to.data_ptr() != dx.data_ptr()) dx.copy_(layout == 1 ? to.transpose(1, 2) : to);
   return {dx, dw, db};
 }
 
