@@ -7,7 +7,8 @@
 // holds it in f16's range; a bf16 G enters exactly, its results' own rounding (1.65e-3 of the norm) is larger than what
 // the f16 intermediates add (2.0e-3 in all; bf16 intermediates: 1e-2 to 3e-2).  P's diagonal, its largest values, stays
 // in float32 beside it and joins a (2.35e-3 with it in f16).  For f16 and float32 every matrix is a pair
-// hi + lo of f16 (22 bits) and a product three (hi hi + hi lo + lo hi), 4e-7 of the norm.
+// hi + lo of f16 (22 bits) and a product three (hi hi + hi lo + lo hi): 1.7e-6 of the norm at 1777 x 1000, where float32
+// products lose 2.6e-6.
 //
 // A and P are symmetric: their tiles on and below the diagonal are computed and written to both places.  X is kept
 // by rows; P X reads it down its columns with LDS reads that transpose.  All matrices are zero-padded to multiples of
@@ -361,11 +362,18 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
       to_lds(to, from_l[i], lp + pl * p.left_plane * 2 + k * (BK * 2));
   };
 
-  f32x4 acc[TL][TR];
+  // A symmetric product of pairs has sums of their own for lo hi and for hi lo: A[l][r] and A[r][l] then have the same
+  // bits, and so have the entries of equal rows of X on either side of the diagonal.  (In one running sum they differ by
+  // a rounding, which gives equal rows directions of their own: 4e-4 of the norm after ten steps, so 5e-6.)
+  constexpr bool APART = SYM && PL == 2 && MODE != XXT_JOIN;
+  f32x4 acc[TL][TR], low[2][APART ? TL : 1][APART ? TR : 1];
 #pragma unroll
   for (int i = 0; i < TL; ++i)
 #pragma unroll
-    for (int j = 0; j < TR; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < TR; ++j) {
+      acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (APART) low[0][i][j] = low[1][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
 
   const int row = lane & 15, quad = lane >> 4;
   struct Half {  // a wave's operands of 32 of a slice's 64
@@ -395,8 +403,10 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
 #pragma unroll
       for (int j = 0; j < TR; ++j) {
         if constexpr (PL == 2) {
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.l[1][i], h.r[0][j], acc[i][j], 0, 0, 0);
-          acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.l[0][i], h.r[1][j], acc[i][j], 0, 0, 0);
+          f32x4 &lo_hi = APART ? low[0][APART ? i : 0][APART ? j : 0] : acc[i][j],
+                &hi_lo = APART ? low[1][APART ? i : 0][APART ? j : 0] : acc[i][j];
+          lo_hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.l[1][i], h.r[0][j], lo_hi, 0, 0, 0);
+          hi_lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.l[0][i], h.r[1][j], hi_lo, 0, 0, 0);
         }
         acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(h.l[0][i], h.r[0][j], acc[i][j], 0, 0, 0);
       }
@@ -441,6 +451,12 @@ __global__ __launch_bounds__(64 * WL * WR) void ns_product_kernel(Args p) {
       stage = next;
     }
     landed(std::integral_constant<int, 0>{});
+    if constexpr (APART) {
+#pragma unroll
+      for (int i = 0; i < TL; ++i)
+#pragma unroll
+        for (int j = 0; j < TR; ++j) acc[i][j] += low[0][i][j] + low[1][i][j];
+    }
   }
   if constexpr (MODE == XXT_PART) {
 #pragma unroll
@@ -644,12 +660,18 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
     *(f16x4*)place(base, width, r, c) = hi;
     if constexpr (PL == 2) *(f16x4*)(place(base, width, r, c) + plane) = lo;
   };
-  // acc[i][j] = sum over K of the wave's left blocks and its right rows
-  auto product = [&](auto& acc, auto BLOCKS, auto K, auto&& left, const char* right, int right_plane, int right_width) {
+  // acc[i][j] = sum over K of the wave's left blocks and its right rows; pairs of a symmetric product as in the tiles
+  auto product = [&](auto& acc, auto BLOCKS, auto K, auto SYM, auto&& left, const char* right, int right_plane,
+                     int right_width) {
+    constexpr bool APART = SYM.value && PL == 2;
+    f32x4 low[2][APART ? BLOCKS.value : 1][APART ? TR : 1];
 #pragma unroll
     for (int i = 0; i < BLOCKS.value; ++i)
 #pragma unroll
-      for (int j = 0; j < TR; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int j = 0; j < TR; ++j) {
+        acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+        if constexpr (APART) low[0][i][j] = low[1][i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+      }
 #pragma unroll 4
     for (int k = 0; k < K.value / 32; ++k) {
       f16x8 r[PL][TR];
@@ -665,12 +687,20 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
 #pragma unroll
         for (int j = 0; j < TR; ++j) {
           if constexpr (PL == 2) {
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[1], r[0][j], acc[i][j], 0, 0, 0);
-            acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0], r[1][j], acc[i][j], 0, 0, 0);
+            f32x4 &lo_hi = APART ? low[0][APART ? i : 0][APART ? j : 0] : acc[i][j],
+                  &hi_lo = APART ? low[1][APART ? i : 0][APART ? j : 0] : acc[i][j];
+            lo_hi = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[1], r[0][j], lo_hi, 0, 0, 0);
+            hi_lo = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0], r[1][j], hi_lo, 0, 0, 0);
           }
           acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x32_f16(l[0], r[0][j], acc[i][j], 0, 0, 0);
         }
       }
+    }
+    if constexpr (APART) {
+#pragma unroll
+      for (int i = 0; i < BLOCKS.value; ++i)
+#pragma unroll
+        for (int j = 0; j < TR; ++j) acc[i][j] += low[0][i][j] + low[1][i][j];
     }
   };
   using IntA = std::integral_constant<int, TA>;
@@ -688,8 +718,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
             f32x4{x[i][j][0], x[i][j][1], x[i][j][2], x[i][j][3]});
     __syncthreads();
     f32x4 acc[TA][TR];
-    product(acc, IntA{}, KX{}, [&](int pl, int block, int k) { return by_row(xs + pl * X_PLANE, N, block, k); }, xs, X_PLANE,
-            N);
+    product(acc, IntA{}, KX{}, std::true_type{},
+            [&](int pl, int block, int k) { return by_row(xs + pl * X_PLANE, N, block, k); }, xs, X_PLANE, N);
 #pragma unroll
     for (int i = 0; i < TA; ++i)
 #pragma unroll
@@ -699,8 +729,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
       }
     __syncthreads();
     f32x4 sq[TA][TR];
-    product(sq, IntA{}, KA{}, [&](int pl, int block, int k) { return by_row(as + pl * A_PLANE, D, block, k); }, as, A_PLANE,
-            D);
+    product(sq, IntA{}, KA{}, std::true_type{},
+            [&](int pl, int block, int k) { return by_row(as + pl * A_PLANE, D, block, k); }, as, A_PLANE, D);
     __syncthreads();  // A has been read
     const float pb = SCALE_P * co.v[3 * step + 1] / SCALE_A, pc = SCALE_P * co.v[3 * step + 2] / (SCALE_A * SCALE_A);
 #pragma unroll
@@ -722,8 +752,8 @@ __global__ __launch_bounds__(SMALL_THREADS) void ns_small_kernel(const T* __rest
       }
     __syncthreads();
     f32x4 px[TX][TR];
-    product(px, IntX{}, KA{}, [&](int pl, int block, int k) { return by_column(xs + pl * X_PLANE, block, k); }, as, A_PLANE,
-            D);
+    product(px, IntX{}, KA{}, std::false_type{},
+            [&](int pl, int block, int k) { return by_column(xs + pl * X_PLANE, block, k); }, as, A_PLANE, D);
     const bool last = step + 1 == steps, fine = PL == 2 || (step >= 1 && step <= steps - 2);
     const float to = last ? u : u / f.later, a = co.v[3 * step] * to, b = to / SCALE_P;
 #pragma unroll
@@ -888,6 +918,13 @@ int launch_product(const Args& a, int64_t batch, hipStream_t st) {
     if (best == T128_4) return launch_tiles<128, 128, 2, 2, 4, PL, MODE, T>(a, batch, st);
   }
   if (best == T64_2) return launch_tiles<64, 64, 2, 2, 2, PL, MODE, T>(a, batch, st);
+  // A symmetric product of pairs has three sums a block: 8 waves, each of half as many blocks.  us for all steps, float32:
+  // 2048 x 2048 662, with 4 waves 819 (more than 256 registers, which the compiler moves about); 1777 x 1000 228 and 235;
+  // two workgroups a CU, 4 of 768 x 2048: 443 and 440.
+  if constexpr (SYM && PL == 2) {
+    if (best == T64_4) return launch_tiles<64, 64, 2, 4, 4, PL, MODE, T>(a, batch, st);
+    return launch_tiles<128, 128, 2, 4, 2, PL, MODE, T>(a, batch, st);
+  }
   if (best == T64_4) return launch_tiles<64, 64, 2, 2, 4, PL, MODE, T>(a, batch, st);
   return launch_tiles<128, 128, 2, 2, 2, PL, MODE, T>(a, batch, st);
 }
