@@ -4,11 +4,13 @@
 //
 // on the side with fewer rows (G^T for a tall G), so that every singular value s goes to s (a + b s^2 + c s^4) a step.
 // The products are on the matrix cores in f16 with float32 sums.  Every matrix is kept at a power-of-two scale that
-// holds it in f16's range; a bf16 G enters exactly, its results' own rounding (1.65e-3 of the norm) is larger than what
-// the f16 intermediates add (2.0e-3 in all; bf16 intermediates: 1e-2 to 3e-2).  P's diagonal, its largest values, stays
-// in float32 beside it and joins a (2.35e-3 with it in f16).  For f16 and float32 every matrix is a pair
-// hi + lo of f16 (22 bits) and a product three (hi hi + hi lo + lo hi): 1.7e-6 of the norm at 1777 x 1000, where float32
-// products lose 2.6e-6.
+// holds it in f16's range.  For f16 and float32 every matrix is a pair hi + lo of f16 (22 bits) and a product three (hi hi
+// + hi lo + lo hi): 1.7e-6 of the norm at 1777 x 1000, where float32 products lose 2.6e-6.  For bf16, which enters
+// exactly, one f16 plane is enough for a few steps: five of Muon's end 1.7e-3 to 2.1e-3 of the norm off for spread
+// singular values (the result's own rounding: 1.65e-3; bf16 intermediates: 1e-2 to 3e-2), up to 5.3e-3 for a matrix of
+// low rank, up to 1e-2 where rows repeat and their roundings add up.  P's diagonal, its largest values, stays in float32
+// beside it and joins a (2.35e-3 with it in f16).  What is rounded away in the directions of small singular values
+// grows with them, so bf16 with coefficients that let it grow further runs pairs too: see MOST_NOISE.
 //
 // A and P are symmetric: their tiles on and below the diagonal are computed and written to both places.  X is kept
 // by rows; P X reads it down its columns with LDS reads that transpose.  All matrices are zero-padded to multiples of
@@ -83,6 +85,12 @@ typedef __attribute__((address_space(3))) char lds_char;
 // stored = value * scale: with |singular values| of X up to 8 (checked on the host), |A| <= 64 and |P| <= 250
 constexpr float SCALE_X = 256.f, SCALE_A = 256.f, SCALE_P = 64.f;
 constexpr float MOST_X = 8.f, MOST_P = 250.f;
+// The most that the roundings of all steps may have grown to, in units of one step's, for products of single planes: each
+// step multiplies what is there by at most its polynomial's largest slope.  Five of Muon's steps: 489; six: 2157; twelve of
+// (1.5, -0.5, 0): 257.  Errors relative to the norm, bf16 matrices of exactly rank 8 or 32, single planes and pairs:
+// five steps 4.3e-3 and 1.7e-3, six 1.4e-2 and 1.7e-3, eight 0.16 and 2.0e-3, ten 1.8 and 1.3e-2 (float32 products, rounded:
+// ten 2.0e-2).  us, six steps: 4096 x 4096 1570 and 4940, 12 of 1024 x 2048 836 and 1950, 128 x 128 32 and 58.
+constexpr double MOST_NOISE = 512.0;
 
 // ------------------------------------------------------------------------------------------------ norm and first X
 constexpr int NORM_BLOCK = 512, NORM_PARTS = 256;  // most partial sums of a matrix
@@ -808,14 +816,15 @@ struct Plan {
 
 int round_up(int v, int to) { return (v + to - 1) / to * to; }
 
-// Whether ns_small_kernel takes matrices of these sizes: a row of X more fills the LDS or the registers.
+// Whether ns_small_kernel takes matrices of these sizes: what is larger has no room in LDS or registers (128 x 256 of one
+// plane spills 34 registers of a lane already).
 bool is_small(int M, int N, int planes) {
   return M <= 64 ? N <= 256 : M <= 128 && N <= (planes == 1 ? 256 : 128);
 }
 
-Plan plan_of(int64_t batch, int m, int n, int dtype) {
+Plan plan_of(int64_t batch, int m, int n, int planes) {
   Plan p;
-  p.planes = dtype == XL_DTYPE_BF16 ? 1 : 2;
+  p.planes = planes;
   p.M = m < n ? m : n;
   p.N = m < n ? n : m;
   if (is_small(p.M, p.N, p.planes)) {  // no workspace
@@ -1051,13 +1060,19 @@ int check_sizes(const char* who, int64_t batch, int m, int n, int dtype) {
   return XL_OK;
 }
 
+// what any coefficients take: bf16 runs one plane or pairs
+size_t workspace_of(int64_t batch, int m, int n, int dtype) {
+  const size_t pairs = plan_of(batch, m, n, 2).bytes, one = dtype == XL_DTYPE_BF16 ? plan_of(batch, m, n, 1).bytes : 0;
+  return one > pairs ? one : pairs;
+}
+
 }  // namespace
 }  // namespace xl
 
 extern "C" size_t xl_newton_schulz_workspace_size(int64_t batch, int m, int n, int dtype) {
   using namespace xl;
   if (check_sizes("xl_newton_schulz_workspace_size", batch, m, n, dtype) || batch == 0 || m == 0 || n == 0) return 0;
-  return plan_of(batch, m, n, dtype).bytes;
+  return workspace_of(batch, m, n, dtype);
 }
 
 extern "C" int xl_newton_schulz(const void* g, void* x, int64_t batch, int m, int n, const float* coefficients, int steps,
@@ -1069,16 +1084,18 @@ extern "C" int xl_newton_schulz(const void* g, void* x, int64_t batch, int m, in
   if (steps < 1 || steps > MOST_STEPS || !coefficients)
     return set_error(XL_ERR_INVALID_ARG, "%s: steps=%d (1 to %d, with coefficients)", who, steps, MOST_STEPS);
   if (!(eps >= 0.f)) return set_error(XL_ERR_INVALID_ARG, "%s: eps=%g (not negative)", who, (double)eps);
-  // singular values start in [0, 1]: the most that a step's polynomial makes of them
-  double most = 1.0;
+  // singular values start in [0, 1]: the most that a step's polynomial makes of them, and of what was rounded before it
+  double most = 1.0, noise = 0.0;
   for (int s = 0; s < steps; ++s) {
     const double a = coefficients[3 * s], b = coefficients[3 * s + 1], c = coefficients[3 * s + 2], x2 = most * most;
     const double in_p = fabs(b) * x2 + fabs(c) * x2 * x2;
-    double next = 0.0;
+    double next = 0.0, slope = 1.0;
     for (int i = 0; i <= 1024; ++i) {
-      const double v = most * i / 1024, y = fabs(v * (a + b * v * v + c * v * v * v * v));
+      const double v = most * i / 1024, v2 = v * v, y = fabs(v * (a + b * v2 + c * v2 * v2));
       if (!(y <= next)) next = y;
+      slope = fmax(slope, fabs(a + 3.0 * b * v2 + 5.0 * c * v2 * v2));
     }
+    noise = noise * slope + 1.0;
     if (!(in_p <= MOST_P) || !(next <= 0.99 * MOST_X))
       return set_error(XL_ERR_INVALID_ARG, "%s: step %d's coefficients (%g, %g, %g) take singular values out of range", who, s, a,
                        b, c);
@@ -1087,15 +1104,18 @@ extern "C" int xl_newton_schulz(const void* g, void* x, int64_t batch, int m, in
   if (batch == 0 || m == 0 || n == 0) return XL_OK;
   if (!g || !x) return set_error(XL_ERR_INVALID_ARG, "%s: null pointer", who);
   if (g == x) return set_error(XL_ERR_INVALID_ARG, "%s: x must not alias g", who);
-  const Plan p = plan_of(batch, m, n, dtype);
-  if (p.bytes && (!workspace || workspace_bytes < p.bytes || ((uintptr_t)workspace & 255u)))
-    return set_error(XL_ERR_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", who, p.bytes,
+  const size_t need = workspace_of(batch, m, n, dtype);
+  if (need && (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255u)))
+    return set_error(XL_ERR_WORKSPACE, "%s: workspace of %zu bytes, 256-byte aligned, needed (got %zu)", who, need,
                      workspace_bytes);
+  const Plan p = plan_of(batch, m, n, dtype == XL_DTYPE_BF16 && noise <= MOST_NOISE ? 1 : 2);
   char* ws = (char*)workspace;
   hipStream_t st = (hipStream_t)stream;
   switch (dtype) {
     case XL_DTYPE_F32: return run<float, 2>(g, x, batch, m, n, coefficients, steps, eps, p, ws, st);
-    case XL_DTYPE_BF16: return run<bf16_t, 1>(g, x, batch, m, n, coefficients, steps, eps, p, ws, st);
+    case XL_DTYPE_BF16:
+      return p.planes == 1 ? run<bf16_t, 1>(g, x, batch, m, n, coefficients, steps, eps, p, ws, st)
+                           : run<bf16_t, 2>(g, x, batch, m, n, coefficients, steps, eps, p, ws, st);
     default: return run<f16_t, 2>(g, x, batch, m, n, coefficients, steps, eps, p, ws, st);
   }
 }
