@@ -121,3 +121,17 @@ def test_batch_stream_and_graph_of_many_steps(gpu_case):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(held, alone.roll(k, 0)), f"replay {k}"
+
+
+@pytest.mark.parametrize("eps", [1e-7, 1e-20, 1e-30])
+@pytest.mark.parametrize("shape", [(40, 60), (3, 130, 257)], ids=str)
+@pytest.mark.parametrize("dtype", [BF16, F16, F32])
+def test_zero_matrix(gpu_case, eps, shape, dtype):
+    """0 / (0 + eps) is 0 for every eps above 0."""
+    import xlstm_hip
+    assert not xlstm_hip.newton_schulz(torch.zeros(shape, dtype=dtype, device=dev()), eps=eps).any()
+    if len(shape) == 3:
+        G = torch.randn(shape, generator=torch.Generator().manual_seed(1)).to(dtype).to(dev())
+        G[1] = 0
+        got = xlstm_hip.newton_schulz(G, eps=eps)
+        assert not got[1].any() and bool(got[[0, 2]].isfinite().all()) and bool(got[[0, 2]].any())

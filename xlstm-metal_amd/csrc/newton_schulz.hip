@@ -157,7 +157,9 @@ __device__ __forceinline__ Factors factors_of(double norm, double eps, double gr
     frexp(share, &up);
     up = up < -100 ? 100 : up < 0 ? -up : 0;
   }
-  return Factors{(float)(1.0 / ((norm + eps) * enter)), (float)ldexp(1.0 / SCALE_X, -up)};
+  // zeros stay zeros however small eps is: the square of 1 / eps would not be finite
+  const double first = norm == 0.0 && eps > 0.0 ? 0.0 : 1.0 / ((norm + eps) * enter);
+  return Factors{(float)first, (float)ldexp(1.0 / SCALE_X, -up)};
 }
 
 __device__ __forceinline__ void split(float v, _Float16& hi, _Float16& lo) {
