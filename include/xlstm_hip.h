@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define XL_ABI_VERSION 3
+#define XL_ABI_VERSION 4
 
 enum xl_dtype { XL_DTYPE_F32 = 0, XL_DTYPE_BF16 = 1, XL_DTYPE_F16 = 2 };
 
@@ -253,6 +253,12 @@ int xl_causal_conv1d_fwd(const void* x, const void* weight, const void* bias, vo
  */
 int xl_group_norm_fwd(const void* x, const void* weight, const void* bias, void* y,
                       int64_t N, int G, int CG, float eps, int dtype, void* stream);
+/*
+ * The same y, and what xl_layer_norm_bwd needs of it (tokens N, heads G): mean
+ * and rstd = 1 / sqrt(var + eps), [N, G] float32, both or neither (NULL).
+ */
+int xl_group_norm_stats_fwd(const void* x, const void* weight, const void* bias, void* y, float* mean, float* rstd,
+                            int64_t N, int G, int CG, float eps, int dtype, void* stream);
 
 /*
  * The mLSTM output cell's stage before its output projection, fused: per-head

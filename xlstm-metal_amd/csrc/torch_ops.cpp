@@ -636,13 +636,13 @@ Tensor silu_mul(const Tensor& g_, const Tensor& u_) {
 
 // ------------------------------------------- layer norm and its gradients
 // layout: 0, the norm over x's last axis; 1 and 2, the norm of each head of [B, NH, S, DH] or [B, S, NH, DH], written
-// [B, S, NH * DH].  Statistics: float32 [2, rows], the means and then 1 / sqrt(var + eps).
+// [B, S, NH * DH]; 3, as 2 by the GroupNorm's kernel, with its bits (weights of x's dtype).  Statistics: float32 [2, rows], the means and then 1 / sqrt(var + eps).
 struct NormShape {
   int64_t H, D, tokens;
   int param;  // the weights' dtype code
 };
 NormShape norm_shape(const Tensor& x, const OptTensor& w, const OptTensor& b, int64_t layout, const char* what) {
-  XL_CHECK(layout >= 0 && layout <= 2, what, "layout must be 0, 1 or 2, got ", layout);
+  XL_CHECK(layout >= 0 && layout <= 3, what, "layout must be 0, 1, 2 or 3, got ", layout);
   XL_CHECK(layout == 0 || x.dim() == 4, what, "heads are of a 4-D tensor, got ", x.sizes());
   XL_CHECK(x.dim() >= 1 && x.size(-1) >= 1, what, "x must have a last axis of at least one value, got ", x.sizes());
   NormShape s{layout ? x.size(layout == 1 ? 1 : 2) : 1, x.size(-1), 0, dtype_code(x, what)};
@@ -656,6 +656,7 @@ NormShape norm_shape(const Tensor& x, const OptTensor& w, const OptTensor& b, in
     s.param = dtype_code(**t, what);
   }
   XL_CHECK(!opt(w) || !opt(b) || w->scalar_type() == b->scalar_type(), what, "weight and bias must share a dtype");
+  XL_CHECK(layout != 3 || s.param == dtype_code(x, what), what, "weight and bias must have x's dtype ", x.scalar_type());
   s.tokens = x.numel() / (s.H * s.D);
   return s;
 }
@@ -692,6 +693,15 @@ std::tuple<Tensor, Tensor> layer_norm(const Tensor& x_, const OptTensor& w_, con
   Gpu gpu(what, {&x_, opt(w_), opt(b_)});
   const NormShape s = norm_shape(x_, w_, b_, layout, what);
   const Tensor view = layout == 1 ? x_.transpose(1, 2) : x_;
+  if (layout == 3) {
+    const Tensor x = prep(view), w = prep(w_), b = prep(b_);
+    const Tensor y = at::empty({x.size(0), x.size(1), s.H * s.D}, x.options()), stats = at::empty({2, s.tokens * s.H}, f32_on(x));
+    float* mean = ptr<float>(stats);
+    check_rc(xl_group_norm_stats_fwd(ptr(x), ptr(w), ptr(b), ptr(y), mean, mean ? mean + s.tokens * s.H : nullptr, s.tokens,
+                                     i32(s.H, what), i32(s.D, what), (float)eps, dtype_code(x, what), gpu.st),
+             what);
+    return {y, stats};
+  }
   int64_t n[2], st[3];
   const bool strided = as_tokens(view, layout != 0, n, st);
   const Tensor x = strided ? view : view.contiguous(), w = prep(w_), b = prep(b_);

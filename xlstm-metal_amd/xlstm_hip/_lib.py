@@ -49,6 +49,7 @@ SIGNATURES = {
     "xl_slstm_seq_fwd": (_i, [_vp] * 4 + [_fp] * 3 + [_vp] + [_fp] * 3 + [_i] * 4 + [_f] + [_i] * 3 + [_vp]),
     "xl_causal_conv1d_fwd": (_i, [_vp] * 4 + [_i] * 6 + [_vp]),
     "xl_group_norm_fwd": (_i, [_vp] * 4 + [_i64, _i, _i, _f, _i, _vp]),
+    "xl_group_norm_stats_fwd": (_i, [_vp] * 4 + [_fp] * 2 + [_i64, _i, _i, _f, _i, _vp]),
     "xl_mh_rmsnorm_gate_fwd": (_i, [_vp] * 4 + [_i] * 5 + [_f, _i, _vp]),
     "xl_gate_proj_softcap_fwd": (_i, [_vp] * 4 + [_i] * 3 + [_f, _i, _i, _vp]),
     "xl_lm_head_softcap_fwd": (_i, [_vp] * 3 + [_i] * 3 + [_f, _i, _vp]),
@@ -63,7 +64,7 @@ SIGNATURES = {
     "xl_newton_schulz": (_i, [_vp] * 2 + [_i64, _i, _i, ctypes.POINTER(_f), _i, _f, _i, _vp, _sz, _vp]),
 }
 
-ABI_VERSION = 3
+ABI_VERSION = 4
 
 _lib = None
 _lock = threading.Lock()

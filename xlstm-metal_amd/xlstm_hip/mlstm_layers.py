@@ -32,7 +32,7 @@ import torch.nn.functional as F
 from torch import Tensor
 
 from .norms import multi_head_layer_norm
-from .ops import gate_proj2_softcap_op, gate_proj_softcap_op, mh_rmsnorm_gate_op
+from .ops import gate_proj2_softcap_op, gate_proj_softcap_op, layer_norm_op, mh_rmsnorm_gate_op
 from .soft_cap import soft_cap
 
 __all__ = ["mh_rmsnorm_gate", "gate_proj_softcap", "gate_pair_softcap", "stacked_linears", "MultiHeadRMSNorm", "MultiHeadLayerNorm",
@@ -144,7 +144,8 @@ class MultiHeadLayerNorm(nn.Module):
     """``multihead_norm.py:5-40``: per-head LayerNorm of x [B, S, NH, DH] -> [B, S, NH * DH], optional
     weight and bias.  Runs ``group_norm_kernel`` (one group per head) on the [B * S, NH * DH] view,
     with float32 statistics and one rounding of the output; the reference takes the mean and
-    variance in x's own dtype.  Where a gradient is wanted it runs ``multi_head_layer_norm``, which has one."""
+    variance in x's own dtype.  Differentiable, with the same output where a gradient is wanted and where none is.
+    Parameters of another dtype than x's (float32 beside 16-bit activations) run ``multi_head_layer_norm``."""
 
     def __init__(self, num_heads: int, head_dim: int, eps: float = 1e-6, use_weight: bool = True,
                  use_bias: bool = False) -> None:
@@ -167,8 +168,11 @@ class MultiHeadLayerNorm(nn.Module):
         B, S, NH, DH = x.shape
         if NH != self.num_heads or DH != self.head_dim:
             raise ValueError(f"Expected shape [B,S,{self.num_heads},{self.head_dim}], got {x.shape}")
-        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, self.weight, self.bias)):
+        given = [t for t in (self.weight, self.bias) if t is not None]
+        if any(t.dtype != x.dtype for t in given):
             return multi_head_layer_norm(x, self.weight, self.bias, self.eps, heads_first=False)
+        if torch.is_grad_enabled() and any(t.requires_grad for t in (x, *given)):
+            return layer_norm_op(x, self.weight, self.bias, self.eps, 3)[0]
         from .slstm_layers import group_norm
         return group_norm(x.reshape(B * S, NH * DH), NH, self.weight, self.bias, self.eps).view(B, S, NH * DH)
 

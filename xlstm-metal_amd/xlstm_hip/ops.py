@@ -70,7 +70,7 @@ _SCHEMAS = {
     # silu(gate) * up, the SiLU rounded to the dtype first (bf16 / f16)
     "silu_mul": ("(Tensor gate, Tensor up) -> Tensor"),
     # (y, statistics): layout 0, the norm over the last axis; 1 and 2, of each head of [B, NH, S, DH] or
-    # [B, S, NH, DH], written [B, S, NH * DH]; statistics float32 [2, rows], means and 1 / sqrt(var + eps)
+    # [B, S, NH, DH], written [B, S, NH * DH]; 3, as 2 by group_norm's kernel, with its bits; statistics float32 [2, rows], means and 1 / sqrt(var + eps)
     "layer_norm": ("(Tensor x, Tensor? weight, Tensor? bias, float eps, SymInt layout) -> (Tensor, Tensor)"),
     # (dx, dweight, dbias); what the mask leaves out is an empty placeholder
     "layer_norm_bwd": ("(Tensor dy, Tensor x, Tensor stats, Tensor? weight, Tensor? bias, SymInt layout, bool[3] "
