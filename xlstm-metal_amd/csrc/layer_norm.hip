@@ -11,8 +11,9 @@
 // registers of a team of lanes, so mean and variance cost no second read; weights stay in registers over a workgroup's
 // rows; the backward keeps the columns' sums there too and writes them once (float32, a workgroup's rows), for a short
 // second launch to join.  Measured (us; torch's copy of the same bytes runs at 5.13 TB/s): 8192 x 4096 bf16 forward 23.6
-// (5.7 TB/s), backward 49.3 (4.1 TB/s; x + dy -> dx as torch.add takes 36.7, without the weight's gradient 42.1);
-// 8192 tokens of 8 heads of 512 forward 26.8, backward 45.6; 8 x 4096, one token each, 3.8 (latency).
+// (5.7 TB/s), backward 44.7 to 47.2 (4.5 to 4.3 TB/s; x + dy -> dx as torch.add takes 36.7, without the weight's gradient
+// 42.1); 8192 tokens of 8 heads of 512 forward 22.7 to 30.4 by machine, backward 45.6 to 47.8; 8 x 4096, one token each,
+// 3.8 (latency).
 #include <math.h>
 
 #include <type_traits>
@@ -510,7 +511,7 @@ void with_layout(const Layout& l, F&& f) {
 #undef XL_LN
 }
 
-// An output of half the L2 caches (8 of 4 MiB) or more goes past them.  us through them and past them, bf16: forward
+// An output of half the L2 caches (8 of 4 MiB) or more goes past them.  us through them and past them, bf16, on one machine: forward
 // 8192 x 4096 27.9 and 23.6, 8192 x 2048 14.0 and 12.7, 8192 x 1536 11.6 and 9.5; backward 50.4 and 49.3, 30.7 and 27.8,
 // 27.2 and 24.3.  What is smaller stays for its reader.
 template <typename T>

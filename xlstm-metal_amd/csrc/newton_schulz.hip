@@ -19,9 +19,10 @@
 //
 // Large matrices are bound by the matrix cores (4096 x 4096 bf16: P X 111 us, 1240 TFLOP/s, where a library f16 product
 // takes 109) and, in the symmetric products' smaller tiles, by LDS reads; middling ones in batches by memory (12 of
-// 1024 x 2048: P X 70 us, 300 MB); small ones by latency and launches.  us for five steps: 4096 x 4096 1300, 10944 x 4096
-// 2900, 12 of 1024 x 2048 700, 1777 x 1000 float32 225, 128 x 128 28 (the products with torch in float32:
-// 14410, 32260, 5564, 633, 491).
+// 1024 x 2048: P X 70 us, 300 MB); small ones by latency and launches.  us for five steps, by machine: 4096 x 4096 1280
+// to 1410, 10944 x 4096 2860 to 3100, 12 of 1024 x 2048 660 to 740, 1777 x 1000 float32 217 to 223, 128 x 128 28 (the
+// products with torch in float32: 14400, 32050, 5550, 627, 492); 4096 x 4096 float32 3940 to 4110, float16 3890 to 4000,
+// 128 x 128 float16 48.
 #include <math.h>
 
 #include <type_traits>
@@ -887,8 +888,9 @@ int launch_tiles(Args a, int64_t batch, hipStream_t st) {
 //   X X^T there:                   128, 4 stages (136): 41, 2 stages: 55;  64, 2 stages (528): 47, 4 stages: 62
 //   1024 x 1024, P X:              64, 4 stages (256): 8.1, 2 stages: 10.9;  128, 4 stages (64): 14.6
 //   float32, 2048 x 2048, P X:     128 (256): 48;  64, 2 stages (1024): 59, 4 stages: 64
-//   float32, 1000 x 1777, P X:     64, 2 stages (448): 16.7, 4 stages: 19.3;  128 (112): 26;   X X^T: 64, 4 stages
-//                                  (136): 14.0, 2 stages: 20;  128 (36): 37
+//   float32, 1000 x 1777, P X:     64, 2 stages (448): 16.7, 4 stages: 19.3;  128 (112): 26
+//   X X^T and A A there:           64, 4 stages (136): 25, 2 stages: 35;  128 (36): 53
+//   2048 x 2048, all five steps, X X^T and A A by 128 (136): 643;  64, 2 stages (528): 758, 4 stages: 791
 template <int PL, int MODE, typename T>
 int launch_product(const Args& a, int64_t batch, hipStream_t st) {
   constexpr bool SYM = MODE == XXT || MODE == AA;
@@ -930,8 +932,8 @@ int launch_product(const Args& a, int64_t batch, hipStream_t st) {
   }
   if (best == T64_2) return launch_tiles<64, 64, 2, 2, 2, PL, MODE, T>(a, batch, st);
   // A symmetric product of pairs has three sums a block: 8 waves, each of half as many blocks.  us for all steps, float32:
-  // 2048 x 2048 662, with 4 waves 819 (more than 256 registers, which the compiler moves about); 1777 x 1000 228 and 235;
-  // two workgroups a CU, 4 of 768 x 2048: 443 and 440.
+  // 2048 x 2048 662, with 4 waves 819 (more than 256 registers, which the compiler moves about); 1777 x 1000 228 and 235.
+  // Tiles of 64 with two stages, two workgroups a CU, stay with 4: 4 of 768 x 2048 440, with 8 443.
   if constexpr (SYM && PL == 2) {
     if (best == T64_4) return launch_tiles<64, 64, 2, 4, 4, PL, MODE, T>(a, batch, st);
     return launch_tiles<128, 128, 2, 4, 2, PL, MODE, T>(a, batch, st);
