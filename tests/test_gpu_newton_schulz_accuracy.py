@@ -135,3 +135,18 @@ def test_zero_matrix(gpu_case, eps, shape, dtype):
         G[1] = 0
         got = xlstm_hip.newton_schulz(G, eps=eps)
         assert not got[1].any() and bool(got[[0, 2]].isfinite().all()) and bool(got[[0, 2]].any())
+
+
+# of eps: far below, where five of Muon's steps (485-fold) just reach 1, and up to it
+@pytest.mark.parametrize("ratio", [1e-30, 1e-12, 1e-6, 1 / 485, 1e-2, 0.03, 0.1, 1.0])
+@pytest.mark.parametrize("shape", [(70, 150), (100, 120), (1024, 2048)], ids=str)
+@pytest.mark.parametrize("coefficients", [MUON, (1.0, 0.8, 0.0)], ids=["Muon", "growing with the value"])
+def test_norm_below_eps(gpu_case, ratio, shape, coefficients):
+    import xlstm_hip
+    x = torch.randn(*shape, generator=torch.Generator().manual_seed(4))
+    G, steps = (x / x.norm() * (ratio * 1e-3)).to(dev()), 5 if coefficients is MUON else 2
+    triples = (coefficients,) * steps
+    want = iterate(G.double(), triples, 1e-3)
+    bar = 2 * error(iterate(G, triples, 1e-3), want) + 2.0 ** -24 + steps * 2.0 ** -21
+    off = error(xlstm_hip.newton_schulz(G, steps, coefficients, eps=1e-3), want)
+    assert off <= bar, f"{off:.2e} over {bar:.2e}"

@@ -83,7 +83,8 @@ __device__ __forceinline__ void store_four(T* p, const Four<T>& v) {
 }
 typedef __attribute__((address_space(3))) char lds_char;
 
-// stored = value * scale: with |singular values| of X up to 8 (checked on the host), |A| <= 64 and |P| <= 250
+// stored = value * scale: with |singular values| of X up to 8 (checked on the host), |A| <= 64 and |P| <= 250.  X is scaled
+// up further where it cannot grow that large (factors_of).
 constexpr float SCALE_X = 256.f, SCALE_A = 256.f, SCALE_P = 64.f;
 constexpr float MOST_X = 8.f, MOST_P = 250.f;
 // The most that the roundings of all steps may have grown to, in units of one step's, for products of single planes: each
@@ -151,12 +152,14 @@ __device__ __forceinline__ Factors factors_of(double norm, double eps, double gr
     frexp(norm, &e);
     enter = ldexp(1.0, 13 - e);  // |stored|_F in [2^12, 2^13)
   }
-  // a G far below eps keeps its smallness: it is scaled up by what the steps cannot make up for
+  // A G far below eps keeps its smallness: it is scaled up by what the steps cannot make up for, to singular values of up
+  // to 128 (2^15 as stored), so that the lo planes keep their bits.  (Up to 1, 4096 x 4096 float32 of a hundredth of eps and
+  // below were up to 8e-5 off.)
   int up = 0;
-  const double share = norm / (norm + eps) * growth;
+  const double share = norm / (norm + eps) * growth / 128.0;
   if (share > 0.0 && share < 1.0) {
     frexp(share, &up);
-    up = up < -100 ? 100 : up < 0 ? -up : 0;
+    up = up < -110 ? 110 : up < 0 ? -up : 0;
   }
   // zeros stay zeros however small eps is: the square of 1 / eps would not be finite
   const double first = norm == 0.0 && eps > 0.0 ? 0.0 : 1.0 / ((norm + eps) * enter);
@@ -973,13 +976,8 @@ int run_small(const void* g, void* x, int64_t batch, int m, int n, const Coeffic
 }
 
 template <typename T, int PL>
-int run(const void* g, void* x, int64_t batch, int m, int n, const float* coefficients, int steps, float eps, const Plan& p,
-        char* ws, hipStream_t st) {
-  double growth = 1.0;
-  for (int s = 0; s < steps; ++s) {
-    const double a = fabs((double)coefficients[3 * s]);
-    if (a > 1.0) growth *= a;
-  }
+int run(const void* g, void* x, int64_t batch, int m, int n, const float* coefficients, int steps, float eps, double growth,
+        const Plan& p, char* ws, hipStream_t st) {
   if (is_small(p.M, p.N, PL)) {
     Coefficients co;
     for (int i = 0; i < 3 * steps; ++i) co.v[i] = coefficients[i];
@@ -1088,18 +1086,21 @@ extern "C" int xl_newton_schulz(const void* g, void* x, int64_t batch, int m, in
   if (steps < 1 || steps > MOST_STEPS || !coefficients)
     return set_error(XL_ERR_INVALID_ARG, "%s: steps=%d (1 to %d, with coefficients)", who, steps, MOST_STEPS);
   if (!(eps >= 0.f)) return set_error(XL_ERR_INVALID_ARG, "%s: eps=%g (not negative)", who, (double)eps);
-  // singular values start in [0, 1]: the most that a step's polynomial makes of them, and of what was rounded before it
-  double most = 1.0, noise = 0.0;
+  // singular values start in [0, 1]: the most that a step's polynomial makes of them, and of what was rounded before it; and
+  // by how much a small one can have grown
+  double most = 1.0, noise = 0.0, growth = 1.0;
   for (int s = 0; s < steps; ++s) {
     const double a = coefficients[3 * s], b = coefficients[3 * s + 1], c = coefficients[3 * s + 2], x2 = most * most;
     const double in_p = fabs(b) * x2 + fabs(c) * x2 * x2;
-    double next = 0.0, slope = 1.0;
+    double next = 0.0, slope = 1.0, rate = 1.0;
     for (int i = 0; i <= 1024; ++i) {
-      const double v = most * i / 1024, v2 = v * v, y = fabs(v * (a + b * v2 + c * v2 * v2));
+      const double v = most * i / 1024, v2 = v * v, by = fabs(a + b * v2 + c * v2 * v2), y = v * by;
       if (!(y <= next)) next = y;
+      rate = fmax(rate, by);
       slope = fmax(slope, fabs(a + 3.0 * b * v2 + 5.0 * c * v2 * v2));
     }
     noise = noise * slope + 1.0;
+    growth *= rate;
     if (!(in_p <= MOST_P) || !(next <= 0.99 * MOST_X))
       return set_error(XL_ERR_INVALID_ARG, "%s: step %d's coefficients (%g, %g, %g) take singular values out of range", who, s, a,
                        b, c);
@@ -1116,10 +1117,10 @@ extern "C" int xl_newton_schulz(const void* g, void* x, int64_t batch, int m, in
   char* ws = (char*)workspace;
   hipStream_t st = (hipStream_t)stream;
   switch (dtype) {
-    case XL_DTYPE_F32: return run<float, 2>(g, x, batch, m, n, coefficients, steps, eps, p, ws, st);
+    case XL_DTYPE_F32: return run<float, 2>(g, x, batch, m, n, coefficients, steps, eps, growth, p, ws, st);
     case XL_DTYPE_BF16:
-      return p.planes == 1 ? run<bf16_t, 1>(g, x, batch, m, n, coefficients, steps, eps, p, ws, st)
-                           : run<bf16_t, 2>(g, x, batch, m, n, coefficients, steps, eps, p, ws, st);
-    default: return run<f16_t, 2>(g, x, batch, m, n, coefficients, steps, eps, p, ws, st);
+      return p.planes == 1 ? run<bf16_t, 1>(g, x, batch, m, n, coefficients, steps, eps, growth, p, ws, st)
+                           : run<bf16_t, 2>(g, x, batch, m, n, coefficients, steps, eps, growth, p, ws, st);
+    default: return run<f16_t, 2>(g, x, batch, m, n, coefficients, steps, eps, growth, p, ws, st);
   }
 }
