@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define XL_ABI_VERSION 4
+#define XL_ABI_VERSION 5
 
 enum xl_dtype { XL_DTYPE_F32 = 0, XL_DTYPE_BF16 = 1, XL_DTYPE_F16 = 2 };
 
@@ -412,6 +412,29 @@ int xl_layer_norm_bwd(const void* dy, const void* x, const int64_t* x_strides, c
 size_t xl_newton_schulz_workspace_size(int64_t batch, int m, int n, int dtype);
 int xl_newton_schulz(const void* g, void* x, int64_t batch, int m, int n, const float* coefficients, int steps,
                      float eps, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Gated delta rule: with a = exp(g), the state C [DQK, DV] goes to a C + k (beta (v - (a C)^T k))^T at every token, and h =
+ * scale C^T q.  q, k [B, NHK, S, DQK], v, h [B, NH, S, DV] of dtype_qkv, head i of v with head i / (NH / NHK) of q and k;
+ * g, beta [B, NH, S] of dtype_gates (g = -inf: a = 0); c0 [B, NH, DQK, DV] float32 or NULL (zeros), c_last the last state or
+ * NULL.  DQK up to 256.  S = 0 copies c0 to c_last.
+ *
+ * Token by token, in float32, everything contiguous; c_last may be c0.
+ */
+int xl_gated_delta_recurrent_fwd(const void* q, const void* k, const void* v, const void* g, const void* beta,
+                                 const float* c0, void* h, float* c_last, int B, int NH, int NHK, int S, int DQK, int DV,
+                                 float scale, int dtype_qkv, int dtype_gates, void* stream);
+
+/*
+ * By chunks of 64 tokens, any S.  strides (host memory): element strides of batch, head and token of q, k and v, values
+ * contiguous, or NULL for contiguous tensors.  h 16-byte aligned, c_last apart from c0.  Workspace:
+ * xl_gated_delta_chunkwise_workspace_size bytes, 256-byte aligned.
+ */
+size_t xl_gated_delta_chunkwise_workspace_size(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv);
+int xl_gated_delta_chunkwise_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* g,
+                                 const void* beta, const float* c0, void* h, float* c_last, int B, int NH, int NHK, int S,
+                                 int DQK, int DV, float scale, int dtype_qkv, int dtype_gates, void* workspace,
+                                 size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,168 @@
+// The gated delta rule by chunks of 64 tokens: what its kernels share (chunkwise forward: delta_chunkwise.hip, backward:
+// delta_backward.hip).
+//
+//   S_t = a_t S_{t-1} + k_t d_t^T,  d_t = beta_t (v_t - (a_t S_{t-1})^T k_t),  h_t = scale S_t^T q_t,  a_t = exp(g_t)
+//
+// In a chunk, with b_i = g_1 + .. + g_i, c_i = exp(b_i), D_ij = exp(b_i - b_j) and S the state before it (rows i, j are tokens):
+//
+//   A_ij = beta_i D_ij k_i.k_j (j < i),  T = (I + A)^-1,  U = T diag(beta) (V - diag(c) K S),  P_ij = scale D_ij q_i.k_j (j <= i)
+//   H = scale diag(c) Q S + P U,   S' = c_L S + (diag(c_L / c_j) K)^T U
+//
+// T and P do not know the state: a first kernel (delta_prep) forms them for all chunks at once.  What is left of a chunk
+// acts on each column of V, U and S by itself: a wave takes 16 columns through the whole sequence, its [DQK, 16] piece
+// of the state in float32 registers, and no wave waits for another.
+//
+// All products are on the matrix cores in f16 with float32 sums.  Every operand stands at a power-of-two scale that
+// puts its largest value high in f16's range (of a chunk's K or Q, of T and P, and of a wave's S, V - diag(c) K S, U), so any
+// input's range is kept; float32 values enter as pairs hi + lo of f16 (22 bits), and a product of two pairs is three.
+//
+// Operand layout of v_mfma_f32_16x16x32_f16: lane l = 16 g + r holds row (A) or column (B) r, k = 8 g .. 8 g + 7; the result's
+// column is r, its rows 4 g .. 4 g + 3.  Two results below each other (16 rows each) hold 4 g + e and 16 + 4 g + e of 32 rows:
+// they are the next product's B operand as they stand if its A operand has k in that order.  "Turned" 32s have it: piece g
+// of 8 values holds 4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3.
+#pragma once
+
+#include "common.h"
+#include "mfma_bf16.h"
+
+namespace xl {
+namespace delta {
+
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) char lds_char;
+
+constexpr int L = 64;           // tokens of a chunk
+constexpr int MAX_DQK = 256;
+constexpr int FRAGS = 8;        // 16 x 32 operands of a 64 x 64 matrix: row tile mt, half s of k at 2 mt + s
+constexpr int FRAG_PLANE = FRAGS * 64 * 8;  // f16 values of one plane
+constexpr float CLAMP_G = -1e4f;  // exp() of it is 0: a reset (-inf) keeps the sums finite
+
+// Per head and chunk, by the first kernel: per-token factors (f16 planes' scales folded in) and scales.
+struct Factors {
+  double b[L];     // running sums of g
+  float in[L];     // c_i 2^k            K S
+  float q[L];      // scale c_i 2^q      Q S
+  float out[L];    // c_L / c_i 2^k      U into the state
+  float back[L];   // beta_i c_i 2^k     Z into the state's gradient
+  float beta[L];
+  float all;       // c_L
+  float t, tt, p;  // T diag(beta), T and P = planes * these
+  float k, qs;     // K, Q = planes * these
+  float pad[2];
+};
+static_assert(sizeof(Factors) % 16 == 0);
+
+__device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+
+// 2^target / 2^exponent(m) and its inverse: m times the first is in [2^target, 2^(target + 1)); m >= 0, the same in the wave
+struct Pow2 {
+  float up, down;
+};
+__device__ __forceinline__ Pow2 pow2_for(float m, int target = 14) {
+  const int e = (int)(__float_as_uint(m) >> 23);
+  int sh = e == 255 ? 0 : target + 127 - e;
+  sh = sh > 100 ? 100 : sh < -100 ? -100 : sh;
+  return {__uint_as_float((uint32_t)(127 + sh) << 23), __uint_as_float((uint32_t)(127 - sh) << 23)};
+}
+
+// max over the wave, in every lane (scalar)
+__device__ __forceinline__ float wave_max_all(float x) {
+#define XL_DPP_MAX(CTRL, ROWMASK) \
+  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWMASK, 0xf, false)));
+  XL_DPP_MAX(0x111, 0xf)  // row_shr:1 (what is shifted in is 0: x is not negative)
+  XL_DPP_MAX(0x112, 0xf)
+  XL_DPP_MAX(0x114, 0xf)
+  XL_DPP_MAX(0x118, 0xf)
+  XL_DPP_MAX(0x142, 0xa)  // row_bcast:15
+  XL_DPP_MAX(0x143, 0xc)  // row_bcast:31
+#undef XL_DPP_MAX
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+}
+
+__device__ __forceinline__ uint32_t pk_f16(float a, float b) {
+  return __builtin_bit_cast(uint32_t, __builtin_convertvector((xl_f32x2{a, b}), xl_f16x2));
+}
+// x * scale as f16 planes, 8 values
+template <bool PAIR>
+__device__ __forceinline__ void split8(const float (&x)[8], float scale, f16x8& hi, f16x8& lo) {
+  u32x4 h, l = {};
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = x[2 * j] * scale, b = x[2 * j + 1] * scale;
+    const xl_f16x2 p = __builtin_convertvector((xl_f32x2{a, b}), xl_f16x2);
+    h[j] = __builtin_bit_cast(uint32_t, p);
+    if constexpr (PAIR) l[j] = pk_f16(a - (float)p[0], b - (float)p[1]);
+  }
+  hi = __builtin_bit_cast(f16x8, h);
+  lo = __builtin_bit_cast(f16x8, l);
+}
+template <bool PAIR>
+__device__ __forceinline__ void split8(f32x4 a, f32x4 b, float scale, f16x8& hi, f16x8& lo) {
+  const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+  split8<PAIR>(x, scale, hi, lo);
+}
+
+// 16 bytes a lane from global memory into LDS, at lds + 16 * lane (lds the same in the whole wave).  Whoever reads what it
+// writes waits for it by vmcnt, and then for everybody at a barrier.  m0 has to be written one wait state before.
+__device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const void* base) {
+  asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
+}
+
+// Images of K and Q: [plane][64 tokens][DKP] f16, each 32 columns turned, the 16-byte piece p of token i at p ^ (i % 8).
+template <int DKP>
+__device__ __forceinline__ int piece_at(int token, int p) {
+  return token * (DKP * 2) + ((p ^ (token & 7)) << 4);
+}
+// A or B operand: tokens 16 mt .. + 15, columns of half s (32 s ..), as turned
+template <int DKP>
+__device__ __forceinline__ f16x8 rows_frag(const char* img, int mt, int s, int r, int g) {
+  return *(const f16x8*)(img + piece_at<DKP>(16 * mt + r, 4 * s + g));
+}
+// A operand: columns 16 t .. + 15 (one a lane), k = tokens 32 s + (4 g .. , 16 + 4 g ..)
+template <int DKP>
+__device__ __forceinline__ f16x8 columns_frag(const char* img, int t, int s, int r, int g) {
+  const int token = 32 * s + 4 * g + (r >> 2), p = 4 * (t >> 1) + (r & 3);
+  const char* a = img + piece_at<DKP>(token, p) + (t & 1) * 8;
+  return __builtin_bit_cast(f16x8, mfma::tr_pair(a, a + 16 * DKP * 2));  // 16 tokens on: the same token % 8
+}
+
+// ------------------------------------------------------------------------------------------------ workspace, shapes
+struct Shape {
+  int B, NH, NHK, S, DK, DV;
+  int64_t qs[3], ks[3], vs[3];  // element strides of batch, head, token
+  float scale;
+  int dtype, dtype_gates;
+  int chunks() const { return (S + L - 1) / L; }
+  int dkp() const { return DK <= 64 ? 64 : DK <= 128 ? 128 : 256; }
+  int planes() const { return dtype == XL_DTYPE_F32 ? 2 : 1; }
+  int64_t images() const { return (int64_t)B * NHK * chunks(); }
+  int64_t parts() const { return (int64_t)B * NH * chunks(); }
+  int64_t image_bytes() const { return (int64_t)planes() * L * dkp() * 2; }
+};
+
+// What the first kernel writes; transposed forms for the backward only.
+struct Prep {
+  char *k, *q;       // images
+  f16_t *t, *p;      // [part][plane][FRAG_PLANE]: T diag(beta) (2 planes), P
+  f16_t *tt, *pt;    // T^T, P^T (2 planes)
+  Factors* f;
+};
+
+int check_shape(const char* who, const Shape& s);
+// q, k, v strides from the caller's nine or of contiguous tensors
+void set_strides(Shape& s, const int64_t* strides);
+size_t prep_bytes(const Shape& s, bool backward);
+Prep prep_at(const Shape& s, bool backward, char* ws);
+int launch_prep(const Shape& s, const void* q, const void* k, const void* g, const void* beta, const Prep& p, bool backward,
+                hipStream_t st, const char* who);
+int launch_recurrent(const Shape& s, const void* q, const void* k, const void* v, const void* g, const void* beta,
+                     const float* c0, void* h, float* c_last, hipStream_t st, const char* who);
+
+}  // namespace delta
+}  // namespace xl

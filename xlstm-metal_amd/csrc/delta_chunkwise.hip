@@ -1,0 +1,294 @@
+// Gated delta rule by chunks, second kernel: the scan over a head's chunks (delta.h has the formulas).
+//
+// A wave takes 16 columns through the sequence, its [DQK, 16] piece of the state in float32 registers; the waves of a
+// workgroup share the chunk's images of K and Q in LDS, filled straight from memory a chunk ahead, and nothing else.  Per
+// chunk: K S and Q S (one pass over the state, which is split into f16 planes on the way), R = V - diag(c) K S, U = T R,
+// H = Q S + P U, S = c_L S + K^T U.  U comes out of T R as the B operand of the next two products; H is formed turned
+// (columns down, tokens across), so that a lane holds four neighbours of a row.
+#include "delta.h"
+
+namespace xl {
+namespace delta {
+namespace {
+
+struct ScanArgs {
+  const void* v;
+  int64_t vs[3];
+  const float* c0;
+  void* h;
+  float* c_last;
+  Prep prep;
+  int NH, group, S, DK, DV, chunks, slices;
+};
+
+// PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32)
+template <typename T, int DKB, int STAGES>
+__global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
+  constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
+  constexpr bool PAIR = !std::is_same_v<T, bf16_t>;
+  extern __shared__ __align__(1024) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int r = lane & 15, gq = lane >> 4;
+  const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
+  const int bh = __builtin_amdgcn_readfirstlane(all / p.slices), slice = all - bh * p.slices;
+  const int b = bh / p.NH, h = bh - b * p.NH;
+  const int64_t image0 = ((int64_t)b * (p.NH / p.group) + h / p.group) * p.chunks, part0 = (int64_t)bh * p.chunks;
+  const int n0 = (slice * waves + wave) * 16, n = n0 + r;
+  const bool column = n < p.DV;
+  const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1] + n;
+  T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
+
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
+  auto fetch = [&](int chunk, int stage) {
+    const char* ki = p.prep.k + (image0 + chunk) * (int64_t)IMG;
+    const char* qi = p.prep.q + (image0 + chunk) * (int64_t)IMG;
+    for (int i = wave; i < IMG / 1024; i += waves) {
+      to_lds(lds_at + stage * STAGE + i * 1024, i * 1024 + lane * 16, ki);
+      to_lds(lds_at + stage * STAGE + IMG + i * 1024, i * 1024 + lane * 16, qi);
+    }
+  };
+  // rows 16 mt + 4 gq + e of column n
+  auto load_v = [&](int chunk, float (&to)[4][4]) {
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int t = chunk * L + 16 * mt + 4 * gq + e;
+        to[mt][e] = column && t < p.S ? to_f32(v[t * p.vs[2]]) : 0.f;
+      }
+  };
+
+  f32x4 st[2 * DKB];
+#pragma unroll
+  for (int t = 0; t < 2 * DKB; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 16 * t + 4 * gq + e;
+      st[t][e] = p.c0 && column && d < p.DK ? p.c0[((int64_t)bh * p.DK + d) * p.DV + n] : 0.f;
+    }
+
+  fetch(0, 0);
+  float vn[4][4];
+  load_v(0, vn);
+  for (int c = 0; c < p.chunks; ++c) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int stage = STAGES == 2 ? c & 1 : 0;
+    if (STAGES == 2 && c + 1 < p.chunks) fetch(c + 1, stage ^ 1);
+    const char *ki = lds + stage * STAGE, *qi = ki + IMG;
+    const Factors* f = p.prep.f + part0 + c;
+    const f16x8* tf = (const f16x8*)(p.prep.t + (part0 + c) * (2 * FRAG_PLANE)) + lane;
+    const f16x8* pf = (const f16x8*)(p.prep.p + (part0 + c) * (2 * FRAG_PLANE)) + lane;
+
+    // ---- K S, and Q S turned
+    float m = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2 * DKB; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(st[t][e]));
+    const float most = wave_max_all(m);
+    const Pow2 ss = pow2_for(most);
+    f32x4 ks[4], hs[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) ks[mt] = hs[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < DKB; ++s) {
+      f16x8 hi, lo;
+      split8<true>(st[2 * s], st[2 * s + 1], ss.up, hi, lo);
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const f16x8 k = rows_frag<DKP>(ki, mt, s, r, gq), q = rows_frag<DKP>(qi, mt, s, r, gq);
+        if constexpr (PK == 2) {
+          ks[mt] = mfma(rows_frag<DKP>(ki + PLANE, mt, s, r, gq), hi, ks[mt]);
+          hs[mt] = mfma(hi, rows_frag<DKP>(qi + PLANE, mt, s, r, gq), hs[mt]);
+        }
+        ks[mt] = mfma(k, lo, ks[mt]);
+        if constexpr (PAIR) hs[mt] = mfma(lo, q, hs[mt]);
+        ks[mt] = mfma(k, hi, ks[mt]);
+        hs[mt] = mfma(hi, q, hs[mt]);
+      }
+    }
+    // ---- R
+    f32x4 rr[4];
+    m = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const f32x4 in = *(const f32x4*)&f->in[16 * mt + 4 * gq];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        rr[mt][e] = vn[mt][e] - in[e] * (ks[mt][e] * ss.down);
+        m = fmaxf(m, fabsf(rr[mt][e]));
+      }
+    }
+    const Pow2 rs = pow2_for(wave_max_all(m));
+    f16x8 rh[2], rl[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) split8<true>(rr[2 * s], rr[2 * s + 1], rs.up, rh[s], rl[s]);
+    // ---- U (T is zero above its diagonal: the second half of k from row tile 2 on)
+    f32x4 u[4];
+    const float back = f->t * rs.down;
+    m = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      u[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s <= mt / 2; ++s) {
+        const f16x8 th = tf[(2 * mt + s) * 64], tl = tf[FRAGS * 64 + (2 * mt + s) * 64];
+        u[mt] = mfma(tl, rh[s], u[mt]);
+        u[mt] = mfma(th, rl[s], u[mt]);
+        u[mt] = mfma(th, rh[s], u[mt]);
+      }
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        u[mt][e] *= back;
+        m = fmaxf(m, fabsf(u[mt][e]));
+      }
+    }
+    const float most_u = wave_max_all(m);
+    const Pow2 us = pow2_for(most_u);
+    if (c + 1 < p.chunks) load_v(c + 1, vn);
+    // ---- H
+    {
+      f16x8 uh[2], ul[2];
+#pragma unroll
+      for (int s = 0; s < 2; ++s) split8<PAIR>(u[2 * s], u[2 * s + 1], us.up, uh[s], ul[s]);
+      const float pu = f->p * us.down;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        f32x4 x = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int s = 0; s <= mt / 2; ++s) {
+          const f16x8 ph = pf[(2 * mt + s) * 64];
+          if constexpr (PAIR) {
+            x = mfma(ul[s], ph, x);
+            x = mfma(uh[s], pf[FRAGS * 64 + (2 * mt + s) * 64], x);
+          }
+          x = mfma(uh[s], ph, x);
+        }
+        const int t = c * L + 16 * mt + r;
+        const float fq = f->q[16 * mt + r] * ss.down;
+        if (t < p.S) {
+          T* to = ho + (int64_t)t * p.DV + n0 + 4 * gq;
+          struct alignas(4 * sizeof(T)) Four { T e[4]; } out;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out.e[e] = from_f32<T>(fmaf(x[e], pu, hs[mt][e] * fq));
+          if (p.DV % 4 == 0) {
+            if (n0 + 4 * gq < p.DV) *(Four*)to = out;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (n0 + 4 * gq + e < p.DV) to[e] = out.e[e];
+          }
+        }
+      }
+    }
+    // ---- the state
+    const float all = f->all;
+    m = most * all;
+    f32x4 w[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      w[mt] = u[mt] * *(const f32x4*)&f->out[16 * mt + 4 * gq];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(w[mt][e]));
+    }
+    const Pow2 ws = pow2_for(wave_max_all(m));
+    f16x8 wh[2], wl[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) split8<true>(w[2 * s], w[2 * s + 1], ws.up, wh[s], wl[s]);
+    const float keep = all * ws.up;
+#pragma unroll
+    for (int t = 0; t < 2 * DKB; ++t) {
+      f32x4 x = st[t] * keep;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const f16x8 k = columns_frag<DKP>(ki, t, s, r, gq);
+        if constexpr (PK == 2) x = mfma(columns_frag<DKP>(ki + PLANE, t, s, r, gq), wh[s], x);
+        x = mfma(k, wl[s], x);
+        x = mfma(k, wh[s], x);
+      }
+      st[t] = x * ws.down;
+    }
+    if (STAGES == 1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (c + 1 < p.chunks) fetch(c + 1, 0);
+    }
+  }
+  if (p.c_last && column) {
+#pragma unroll
+    for (int t = 0; t < 2 * DKB; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 16 * t + 4 * gq + e;
+        if (d < p.DK) p.c_last[((int64_t)bh * p.DK + d) * p.DV + n] = st[t][e];
+      }
+  }
+}
+
+template <typename T>
+const void* pick(int dkp, int& stages) {
+  stages = 2;
+  if (dkp == 64) return (const void*)delta_scan_kernel<T, 2, 2>;
+  if (dkp == 128) return (const void*)delta_scan_kernel<T, 4, 2>;
+  if constexpr (is_f32<T>::value) {
+    stages = 1;
+    return (const void*)delta_scan_kernel<T, 8, 1>;
+  } else {
+    return (const void*)delta_scan_kernel<T, 8, 2>;
+  }
+}
+
+int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* c_last, const Prep& prep, hipStream_t st,
+                const char* who) {
+  ScanArgs a{v, {s.vs[0], s.vs[1], s.vs[2]}, c0, h, c_last, prep, s.NH, s.NH / s.NHK, s.S, s.DK, s.DV, s.chunks(), 0};
+  int stages;
+  const void* kern = s.dtype == XL_DTYPE_F32 ? pick<float>(s.dkp(), stages)
+                     : s.dtype == XL_DTYPE_BF16 ? pick<bf16_t>(s.dkp(), stages) : pick<f16_t>(s.dkp(), stages);
+  const int blocks = (s.DV + 15) / 16, waves = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
+  a.slices = (blocks + waves - 1) / waves;
+  const int64_t lds = stages * 2 * s.image_bytes();
+  void* args[] = {&a};
+  hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (e == hipSuccess)
+    e = hipLaunchKernel(kern, dim3((unsigned)((int64_t)s.B * s.NH * a.slices)), dim3(64 * waves), args, (unsigned)lds, st);
+  if (e != hipSuccess) return set_error(XL_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
+  return check_launch(who);
+}
+
+}  // namespace
+}  // namespace delta
+}  // namespace xl
+
+extern "C" size_t xl_gated_delta_chunkwise_workspace_size(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv) {
+  using namespace xl;
+  delta::Shape s{B, NH, NHK, S, DQK, DV, {}, {}, {}, 1.f, dtype_qkv, dtype_qkv};
+  if (delta::check_shape("xl_gated_delta_chunkwise_workspace_size", s) != XL_OK) return 0;
+  return S == 0 ? 0 : delta::prep_bytes(s, false);
+}
+
+extern "C" int xl_gated_delta_chunkwise_fwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* g,
+                                            const void* beta, const float* c0, void* h, float* c_last, int B, int NH, int NHK,
+                                            int S, int DQK, int DV, float scale, int dtype_qkv, int dtype_gates,
+                                            void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace xl;
+  const char* who = "xl_gated_delta_chunkwise_fwd";
+  clear_error();
+  delta::Shape s{B, NH, NHK, S, DQK, DV, {}, {}, {}, scale, dtype_qkv, dtype_gates};
+  if (const int rc = delta::check_shape(who, s)) return rc;
+  if (S == 0 && !c_last) return XL_OK;
+  if (S == 0) return delta::launch_recurrent(s, q, k, v, g, beta, c0, h, c_last, (hipStream_t)stream, who);
+  if (!q || !k || !v || !g || !beta || !h) return set_error(XL_ERR_INVALID_ARG, "%s: null pointer", who);
+  if ((uintptr_t)h & 15) return set_error(XL_ERR_INVALID_ARG, "%s: h must be 16-byte aligned", who);
+  if (c0 && c0 == c_last) return set_error(XL_ERR_INVALID_ARG, "%s: c_last must not alias c0", who);
+  const size_t need = delta::prep_bytes(s, false);
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))
+    return set_error(XL_ERR_WORKSPACE, "%s: the workspace must be %zu bytes, 256-byte aligned", who, need);
+  delta::set_strides(s, strides);
+  const hipStream_t st = (hipStream_t)stream;
+  const delta::Prep prep = delta::prep_at(s, false, (char*)workspace);
+  if (const int rc = delta::launch_prep(s, q, k, g, beta, prep, false, st, who)) return rc;
+  return delta::launch_scan(s, v, c0, h, c_last, prep, st, who);
+}

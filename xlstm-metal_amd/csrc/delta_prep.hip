@@ -1,0 +1,370 @@
+// Gated delta rule by chunks, first kernel: what of a chunk does not depend on the state (delta.h has the formulas).
+//
+// A workgroup of 4 waves takes one chunk of one head of q and k: it brings K and Q to f16 planes at a power-of-two scale (their
+// images go to memory as the scans' LDS wants them), forms K K^T and Q K^T once, and for each head of v that shares them
+// the sums of g (in float64: differences of sums of strong decays keep their bits), A, T = (I + A)^-1 and P.
+//
+// T by 16 x 16 blocks, in float32: each wave inverts one diagonal block by substitution (a lane a column), then walks down
+// its block column, T_ij = -T_ii sum_l A_il T_lj, with v_mfma_f32_16x16x4_f32, whose result is the next one's operand as it
+// stands.  Everything a scan reads as an operand (T diag(beta), P) is written in operand order, 16 bytes a lane.
+#include "delta.h"
+
+namespace xl {
+namespace delta {
+namespace {
+
+struct PrepArgs {
+  const void *q, *k, *g, *beta;
+  int64_t qs[3], ks[3];
+  int NH, NHK, S, DK, chunks;
+  float scale;
+  int gate_dtype;
+  bool wide;  // 16-byte loads of q and k
+  Prep out;
+};
+
+constexpr int MLD = 68;  // row length of 64 x 64 float32 matrices in LDS
+
+template <typename T>
+__device__ __forceinline__ void load8(const T* p, int from, int n, bool wide, float (&x)[8]) {
+  if (wide && from + 8 <= n) {
+    if constexpr (is_f32<T>::value) {
+      const f32x4 a = *(const f32x4*)(p + from), b = *(const f32x4*)(p + from + 4);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        x[e] = a[e];
+        x[4 + e] = b[e];
+      }
+    } else {
+      const u32x4 raw = *(const u32x4*)(p + from);
+      struct V { T e[8]; };
+      const V v = __builtin_bit_cast(V, raw);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = to_f32(v.e[e]);
+    }
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] = from + e < n ? to_f32(p[from + e]) : 0.f;
+  }
+}
+
+__device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
+  return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
+}
+
+// exp(x): float32's rounding of x alone would cost |x| 2^-24 of the result
+__device__ __forceinline__ float exp_of(double x) {
+  const float hi = (float)x, e = expf(hi);
+  return fmaf(e, (float)(x - (double)hi), e);
+}
+
+// max over the workgroup of N values a thread
+template <int N>
+__device__ __forceinline__ void block_max(float (&m)[N], float (*red)[8]) {
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    m[i] = wave_max_all(m[i]);
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6][i] = m[i];
+  }
+  __syncthreads();
+#pragma unroll
+  for (int i = 0; i < N; ++i) m[i] = fmaxf(fmaxf(red[0][i], red[1][i]), fmaxf(red[2][i], red[3][i]));
+}
+
+template <typename T, int DKB, bool BWD>
+__global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
+  constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, IMG = L * DKP * 2;
+  extern __shared__ __align__(1024) char lds[];  // the images of K and Q; then A, T and P
+  __shared__ double bs[L];
+  __shared__ float betas[L], red[4][8];
+  float *Am = (float*)lds, *Tm = Am + L * MLD, *Pm = Tm + L * MLD;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, gq = lane >> 4;
+  const int64_t img = blockIdx.x;
+  const int bk = (int)(img / p.chunks), chunk = (int)(img - (int64_t)bk * p.chunks);
+  const int b = bk / p.NHK, hk = bk - b * p.NHK, group = p.NH / p.NHK;
+  const int t0 = chunk * L;
+
+  // ---- K and Q: a row's 32 columns are one piece of 8 of each of 4 threads
+  const int row = tid >> 2, c = tid & 3;
+  float scales[2];  // K, Q = planes * these
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const int64_t* st = which ? p.qs : p.ks;
+    const T* from = (const T*)(which ? p.q : p.k) + b * st[0] + hk * st[1] + (int64_t)(t0 + row) * st[2];
+    float x[DKB][8], m[1] = {0.f};
+#pragma unroll
+    for (int s = 0; s < DKB; ++s) {
+      if (t0 + row < p.S) {
+        load8(from, 32 * s + 8 * c, p.DK, p.wide, x[s]);
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[s][e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) m[0] = fmaxf(m[0], fabsf(x[s][e]));
+    }
+    block_max(m, red);
+    const Pow2 sc = pow2_for(m[0], 10);
+    scales[which] = sc.down;
+    char* to = lds + which * PK * IMG;
+#pragma unroll
+    for (int s = 0; s < DKB; ++s) {
+      f16x8 hi, lo;
+      split8<PK == 2>(x[s], sc.up, hi, lo);
+      // values 8 c + 0..3 and 4..7 of the 32: groups 2 c, 2 c + 1 of 4, the second four groups in the upper halves
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int at = piece_at<DKP>(row, 4 * s + ((2 * c + h) & 3)) + (c >> 1) * 8;
+        const u32x4 uh = __builtin_bit_cast(u32x4, hi), ul = __builtin_bit_cast(u32x4, lo);
+        *(u32x2*)(to + at) = u32x2{uh[2 * h], uh[2 * h + 1]};
+        if constexpr (PK == 2) *(u32x2*)(to + IMG + at) = u32x2{ul[2 * h], ul[2 * h + 1]};
+      }
+    }
+  }
+  __syncthreads();
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    char* to = (which ? p.out.q : p.out.k) + img * (PK * IMG);
+    for (int i = tid * 16; i < PK * IMG; i += 256 * 16) *(u32x4*)(to + i) = *(const u32x4*)(lds + which * PK * IMG + i);
+  }
+
+  // ---- K K^T and Q K^T, row tile `wave`, column tiles up to it: lane has column 16 jt + r, rows 4 gq + e
+  f32x4 kk[4], qk[4];
+#pragma unroll
+  for (int jt = 0; jt < 4; ++jt) kk[jt] = qk[jt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int s = 0; s < DKB; ++s) {
+    const f16x8 ka = rows_frag<DKP>(lds, wave, s, r, gq), qa = rows_frag<DKP>(lds + PK * IMG, wave, s, r, gq);
+    f16x8 kal, qal;
+    if constexpr (PK == 2) {
+      kal = rows_frag<DKP>(lds + IMG, wave, s, r, gq);
+      qal = rows_frag<DKP>(lds + 3 * IMG, wave, s, r, gq);
+    }
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt) {
+      if (jt > wave) continue;
+      const f16x8 kb = rows_frag<DKP>(lds, jt, s, r, gq);
+      if constexpr (PK == 2) {
+        const f16x8 kbl = rows_frag<DKP>(lds + IMG, jt, s, r, gq);
+        kk[jt] = mfma(kal, kb, kk[jt]);
+        kk[jt] = mfma(ka, kbl, kk[jt]);
+        qk[jt] = mfma(qal, kb, qk[jt]);
+        qk[jt] = mfma(qa, kbl, qk[jt]);
+      }
+      kk[jt] = mfma(ka, kb, kk[jt]);
+      qk[jt] = mfma(qa, kb, qk[jt]);
+    }
+  }
+  __syncthreads();  // the images' place is A, T and P from here
+
+  for (int rep = 0; rep < group; ++rep) {
+    const int h = hk * group + rep;
+    const int64_t bh = (int64_t)b * p.NH + h, part = bh * p.chunks + chunk;
+    // ---- running sums of g, a lane a token
+    const int token = t0 + lane;
+    float gt = 0.f, bt = 0.f;
+    auto gates = [&](auto type) {
+      using G = decltype(type);
+      if (token < p.S) {
+        gt = to_f32(((const G*)p.g)[bh * p.S + token]);
+        bt = to_f32(((const G*)p.beta)[bh * p.S + token]);
+      }
+    };
+    switch (p.gate_dtype) {
+      case XL_DTYPE_F32: gates(0.f); break;
+      case XL_DTYPE_BF16: gates(bf16_t{}); break;
+      default: gates(f16_t{}); break;
+    }
+    gt = gt < CLAMP_G ? CLAMP_G : gt;
+    double sum = (double)gt;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const double below = __shfl_up(sum, o, 64);
+      if (lane >= o) sum += below;
+    }
+    const double last = __shfl(sum, 63, 64);
+    if (wave == 0) {
+      bs[lane] = sum;
+      betas[lane] = bt;
+      Factors* f = p.out.f + part;
+      const float in = exp_of(sum);
+      f->b[lane] = sum;
+      f->in[lane] = in * scales[0];
+      f->q[lane] = in * scales[1] * p.scale;
+      f->out[lane] = exp_of(last - sum) * scales[0];
+      f->back[lane] = bt * in * scales[0];
+      f->beta[lane] = bt;
+    }
+    __syncthreads();
+    // ---- A and P
+    double bi[4];
+    float be[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      bi[e] = bs[16 * wave + 4 * gq + e];
+      be[e] = betas[16 * wave + 4 * gq + e] * (scales[0] * scales[0]);
+    }
+    const float sp = p.scale * scales[0] * scales[1];
+#pragma unroll
+    for (int jt = 0; jt < 4; ++jt) {
+      const int j = 16 * jt + r;
+      const double bj = bs[j];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int i = 16 * wave + 4 * gq + e;
+        const float dec = jt <= wave && j <= i ? exp_of(bi[e] - bj) : 0.f;
+        Am[i * MLD + j] = j < i ? be[e] * dec * kk[jt][e] : 0.f;
+        Pm[i * MLD + j] = j <= i ? sp * dec * qk[jt][e] : 0.f;
+        Tm[i * MLD + j] = 0.f;
+      }
+    }
+    __syncthreads();
+    // ---- the diagonal blocks' inverses: lane r has column r
+    {
+      const float* a = Am + 16 * wave * MLD + 16 * wave;
+      float t[16];
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        float x = i == r ? 1.f : 0.f;
+#pragma unroll
+        for (int l = 0; l < i; ++l) x = fmaf(-a[i * MLD + l], t[l], x);
+        t[i] = x;
+      }
+      if (lane < 16) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) Tm[(16 * wave + i) * MLD + 16 * wave + r] = t[i];
+      }
+    }
+    __syncthreads();
+    // ---- block column `wave`, downwards
+    f32x4 col[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) col[0][e] = Tm[(16 * wave + 4 * gq + e) * MLD + 16 * wave + r];
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {  // block row wave + d
+      if (wave + d > 3) continue;
+      const int i = wave + d;
+      f32x4 m = {0.f, 0.f, 0.f, 0.f}, n = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int l = 0; l < d; ++l) {
+        const f32x4 a = *(const f32x4*)(Am + (16 * i + r) * MLD + 16 * (wave + l) + 4 * gq);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) m = mfma4(a[e], col[l][e], m);
+      }
+      const f32x4 a = *(const f32x4*)(Tm + (16 * i + r) * MLD + 16 * i + 4 * gq);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) n = mfma4(a[e], m[e], n);
+      col[d] = -n;
+    }
+#pragma unroll
+    for (int d = 1; d < 4; ++d) {
+      if (wave + d > 3) continue;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) Tm[(16 * (wave + d) + 4 * gq + e) * MLD + 16 * wave + r] = col[d][e];
+    }
+    __syncthreads();
+    // ---- operands: wave w has frags w and w + 4 of each matrix
+    constexpr int MATS = BWD ? 4 : 2;  // T diag(beta), P; T^T, P^T
+    float x[MATS][2][8], m[MATS];
+#pragma unroll
+    for (int mat = 0; mat < MATS; ++mat) m[mat] = 0.f;
+#pragma unroll
+    for (int half = 0; half < 2; ++half) {
+      const int frag = wave + 4 * half, i = 16 * (frag >> 1) + r, s = frag & 1;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const int j = 32 * s + (e < 4 ? 4 * gq + e : 12 + 4 * gq + e);
+        x[0][half][e] = Tm[i * MLD + j] * betas[j];
+        x[1][half][e] = Pm[i * MLD + j];
+        if constexpr (BWD) {
+          x[2][half][e] = Tm[j * MLD + i];
+          x[3][half][e] = Pm[j * MLD + i];
+        }
+#pragma unroll
+        for (int mat = 0; mat < MATS; ++mat) m[mat] = fmaxf(m[mat], fabsf(x[mat][half][e]));
+      }
+    }
+    block_max(m, red);
+#pragma unroll
+    for (int mat = 0; mat < MATS; ++mat) {
+      const float up = pow2_for(m[mat], 10).up;
+      f16_t* to = (mat == 0 ? p.out.t : mat == 1 ? p.out.p : mat == 2 ? p.out.tt : p.out.pt) + part * (2 * FRAG_PLANE);
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        f16x8 hi, lo;
+        split8<true>(x[mat][half], up, hi, lo);
+        f16_t* at = to + ((wave + 4 * half) * 64 + lane) * 8;
+        *(f16x8*)at = hi;
+        *(f16x8*)(at + FRAG_PLANE) = lo;
+      }
+    }
+    if (tid == 0) {
+      Factors* f = p.out.f + part;
+      f->all = exp_of(last);
+      f->t = pow2_for(m[0], 10).down;
+      f->p = pow2_for(m[1], 10).down;
+      f->tt = BWD ? pow2_for(m[BWD ? 2 : 0], 10).down : 0.f;
+      f->k = scales[0];
+      f->qs = scales[1];
+    }
+    __syncthreads();
+  }
+}
+
+template <typename T, bool BWD>
+const void* pick(int dkp) {
+  return dkp == 64 ? (const void*)delta_prep_kernel<T, 2, BWD> : dkp == 128 ? (const void*)delta_prep_kernel<T, 4, BWD>
+                                                                           : (const void*)delta_prep_kernel<T, 8, BWD>;
+}
+
+int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+}  // namespace
+
+size_t prep_bytes(const Shape& s, bool backward) {
+  const int64_t frags = up256(s.parts() * 2 * FRAG_PLANE * 2);
+  return 2 * up256(s.images() * s.image_bytes()) + (backward ? 4 : 2) * frags + up256(s.parts() * (int64_t)sizeof(Factors));
+}
+
+Prep prep_at(const Shape& s, bool backward, char* ws) {
+  const int64_t image = up256(s.images() * s.image_bytes()), frags = up256(s.parts() * 2 * FRAG_PLANE * 2);
+  Prep p{};
+  p.k = ws;
+  p.q = p.k + image;
+  char* at = p.q + image;
+  p.t = (f16_t*)at;
+  p.p = (f16_t*)(at + frags);
+  if (backward) {
+    p.tt = (f16_t*)(at + 2 * frags);
+    p.pt = (f16_t*)(at + 3 * frags);
+  }
+  p.f = (Factors*)(at + (backward ? 4 : 2) * frags);
+  return p;
+}
+
+int launch_prep(const Shape& s, const void* q, const void* k, const void* g, const void* beta, const Prep& out, bool backward,
+                hipStream_t st, const char* who) {
+  PrepArgs a{q, k, g, beta, {}, {}, s.NH, s.NHK, s.S, s.DK, s.chunks(), s.scale, s.dtype_gates, false, out};
+  int64_t any = 0;
+  for (int i = 0; i < 3; ++i) {
+    a.qs[i] = s.qs[i];
+    a.ks[i] = s.ks[i];
+    any |= s.qs[i] | s.ks[i];
+  }
+  a.wide = any % (16 / dtype_size(s.dtype)) == 0 && (((uintptr_t)q | (uintptr_t)k) & 15) == 0;
+  const void* kern = s.dtype == XL_DTYPE_F32    ? backward ? pick<float, true>(s.dkp()) : pick<float, false>(s.dkp())
+                     : s.dtype == XL_DTYPE_BF16 ? backward ? pick<bf16_t, true>(s.dkp()) : pick<bf16_t, false>(s.dkp())
+                                                : backward ? pick<f16_t, true>(s.dkp()) : pick<f16_t, false>(s.dkp());
+  int64_t lds = 2 * s.image_bytes();
+  if (lds < 3 * L * MLD * 4) lds = 3 * L * MLD * 4;
+  void* args[] = {&a};
+  hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  if (e == hipSuccess) e = hipLaunchKernel(kern, dim3((unsigned)s.images()), dim3(256), args, (unsigned)lds, st);
+  if (e != hipSuccess) return set_error(XL_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
+  return check_launch(who);
+}
+
+}  // namespace delta
+}  // namespace xl

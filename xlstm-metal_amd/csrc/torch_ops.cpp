@@ -831,6 +831,112 @@ Tensor newton_schulz(const Tensor& x_, at::ArrayRef<double> coefficients, double
   return y;
 }
 
+// ------------------------------------------------------------------ gated delta rule
+struct DeltaShape {
+  int64_t B, NH, NHK, S, DQK, DV;
+};
+// q, k [B, NHK, S, DHQK], v [B, NH, S, DHV], gates [B, NH, S]; without S (tokens false): one token's
+DeltaShape delta_shapes(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Tensor* c0,
+                        bool tokens, const char* what) {
+  const int64_t d = tokens ? 4 : 3;
+  XL_CHECK(q.dim() == d, what, "q must be (B, NHK", tokens ? ", S" : "", ", DHQK), got ", q.sizes());
+  XL_CHECK(k.sizes() == q.sizes(), what, "q and k must have the same shape, got ", q.sizes(), " and ", k.sizes());
+  XL_CHECK(v.dim() == d && v.size(0) == q.size(0) && (!tokens || v.size(2) == q.size(2)), what, "v must be (B, NH",
+           tokens ? ", S" : "", ", DHV), got ", v.sizes());
+  const DeltaShape s{q.size(0), v.size(1), q.size(1), tokens ? q.size(2) : 1, q.size(-1), v.size(-1)};
+  XL_CHECK(s.NHK > 0 && s.NH % s.NHK == 0, what, "v's heads (", s.NH, ") must be a multiple of those of q and k (", s.NHK, ")");
+  XL_CHECK(q.scalar_type() == k.scalar_type() && k.scalar_type() == v.scalar_type(), what, "q, k, v must share a dtype");
+  XL_CHECK(g.sizes() == v.sizes().slice(0, d - 1) && beta.sizes() == g.sizes(), what, "g and beta must be (B, NH",
+           tokens ? ", S" : "", "), got ", g.sizes(), " and ", beta.sizes());
+  XL_CHECK(g.scalar_type() == beta.scalar_type(), what, "g and beta must share a dtype");
+  XL_CHECK(!c0 || c0->sizes() == at::IntArrayRef({s.B, s.NH, s.DQK, s.DV}), what, "c must be (B, NH, DHQK, DHV), got ",
+           c0->sizes());
+  return s;
+}
+struct DeltaSizes {
+  int B, NH, NHK, S, DQK, DV;
+  DeltaSizes(const DeltaShape& s, const char* w)
+      : B(i32(s.B, w)), NH(i32(s.NH, w)), NHK(i32(s.NHK, w)), S(i32(s.S, w)), DQK(i32(s.DQK, w)), DV(i32(s.DV, w)) {}
+};
+// q, k and v as they lie where their last axis is contiguous (strides: batch, head, token of each)
+Tensor delta_rows(const Tensor& t, int64_t* strides) {
+  const Tensor r = t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous();
+  for (int d = 0; d < 3; ++d) strides[d] = r.stride(d);
+  return r;
+}
+
+std::tuple<Tensor, Tensor> gated_delta_recurrent(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_,
+                                                 const Tensor& beta_, const OptTensor& c0_, double scale,
+                                                 bool return_last_states) {
+  const char* what = "gated_delta_recurrent";
+  Gpu gpu(what, {&q_, &k_, &v_, &g_, &beta_, opt(c0_)});
+  const DeltaShape s = delta_shapes(q_, k_, v_, g_, beta_, opt(c0_), true, what);
+  const DeltaSizes n(s, what);
+  const Tensor q = q_.contiguous(), k = k_.contiguous(), v = v_.contiguous(), g = g_.contiguous(), beta = beta_.contiguous();
+  const Tensor c0 = f32(c0_), h = at::empty({s.B, s.NH, s.S, s.DV}, q.options());
+  const Tensor cl = return_last_states ? at::empty({s.B, s.NH, s.DQK, s.DV}, f32_on(q)) : at::empty({0}, f32_on(q));
+  check_rc(xl_gated_delta_recurrent_fwd(ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr<float>(c0), ptr(h),
+                                        return_last_states ? ptr<float>(cl) : nullptr, n.B, n.NH, n.NHK, n.S, n.DQK, n.DV,
+                                        (float)scale, dtype_code(q, what), dtype_code(g, what), gpu.st),
+           what);
+  return {h, cl};
+}
+
+// c_new: where the state goes (c itself for the in-place step)
+Tensor launch_delta_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& beta_,
+                         const Tensor& c, const Tensor& c_new, const DeltaShape& s, double scale, const Gpu& gpu,
+                         const char* what) {
+  const DeltaSizes n(s, what);
+  const Tensor q = q_.contiguous(), k = k_.contiguous(), v = v_.contiguous(), g = g_.contiguous(), beta = beta_.contiguous();
+  const Tensor h = at::empty({s.B, s.NH, s.DV}, q.options());
+  check_rc(xl_gated_delta_recurrent_fwd(ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr<float>(c), ptr(h), ptr<float>(c_new), n.B,
+                                        n.NH, n.NHK, 1, n.DQK, n.DV, (float)scale, dtype_code(q, what), dtype_code(g, what),
+                                        gpu.st),
+           what);
+  return h;
+}
+
+std::tuple<Tensor, Tensor> gated_delta_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                            const Tensor& beta, const Tensor& c_, double scale) {
+  const char* what = "gated_delta_step";
+  Gpu gpu(what, {&q, &k, &v, &g, &beta, &c_});
+  const DeltaShape s = delta_shapes(q, k, v, g, beta, &c_, false, what);
+  const Tensor c = f32(c_), c_new = at::empty({s.B, s.NH, s.DQK, s.DV}, f32_on(q));
+  const Tensor h = launch_delta_step(q, k, v, g, beta, c, c_new, s, scale, gpu, what);
+  return {h, c_new};
+}
+
+Tensor gated_delta_step_(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta, const Tensor& c,
+                         double scale) {
+  const char* what = "gated_delta_step_";
+  Gpu gpu(what, {&q, &k, &v, &g, &beta, &c});
+  const DeltaShape s = delta_shapes(q, k, v, g, beta, &c, false, what);
+  XL_CHECK(c.scalar_type() == at::kFloat && c.is_contiguous(), what, "in-place c must be a contiguous float32 tensor");
+  return launch_delta_step(q, k, v, g, beta, c, c, s, scale, gpu, what);
+}
+
+std::tuple<Tensor, Tensor> gated_delta_chunkwise(const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_,
+                                                 const Tensor& beta_, const OptTensor& c0_, double scale,
+                                                 bool return_last_states) {
+  const char* what = "gated_delta_chunkwise";
+  Gpu gpu(what, {&q_, &k_, &v_, &g_, &beta_, opt(c0_)});
+  const DeltaShape s = delta_shapes(q_, k_, v_, g_, beta_, opt(c0_), true, what);
+  const DeltaSizes n(s, what);
+  int64_t st[9];
+  const Tensor q = delta_rows(q_, st), k = delta_rows(k_, st + 3), v = delta_rows(v_, st + 6);
+  const Tensor g = g_.contiguous(), beta = beta_.contiguous(), c0 = f32(c0_);
+  const Tensor h = at::empty({s.B, s.NH, s.S, s.DV}, q.options());
+  const Tensor cl = return_last_states ? at::empty({s.B, s.NH, s.DQK, s.DV}, f32_on(q)) : at::empty({0}, f32_on(q));
+  const int dt = dtype_code(q, what);
+  const size_t ws_bytes = xl_gated_delta_chunkwise_workspace_size(n.B, n.NH, n.NHK, n.S, n.DQK, n.DV, dt);
+  const Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte)) : Tensor();
+  check_rc(xl_gated_delta_chunkwise_fwd(ptr(q), ptr(k), ptr(v), st, ptr(g), ptr(beta), ptr<float>(c0), ptr(h),
+                                        return_last_states ? ptr<float>(cl) : nullptr, n.B, n.NH, n.NHK, n.S, n.DQK, n.DV,
+                                        (float)scale, dt, dtype_code(g, what), ptr(ws), ws_bytes, gpu.st),
+           what);
+  return {h, cl};
+}
+
 // The operators that write an argument, under autograd's bookkeeping, on fake tensors as on real ones.  What they
 // write is updated outside autograd, whatever it requires (a leaf too; its own history stays), a backward through
 // the outputs raises, and the written tensors' version counters move (inference tensors have none).
@@ -849,7 +955,10 @@ auto without_backward(const char* name, const Op& op, c10::DispatchKeySet ks, at
   if (grad) {
     const auto none = std::make_shared<torch::autograd::NotImplemented>(name);
     none->set_next_edges(torch::autograd::collect_next_edges(given));
-    std::apply([&](const auto&... t) { (torch::autograd::set_history(t, none), ...); }, out);
+    if constexpr (std::is_same_v<decltype(out), Tensor>)
+      torch::autograd::set_history(out, none);
+    else
+      std::apply([&](const auto&... t) { (torch::autograd::set_history(t, none), ...); }, out);
   }
   return out;
 }
@@ -901,6 +1010,23 @@ std::tuple<Tensor, Tensor> add_rmsnorm_inplace(c10::DispatchKeySet ks, const Ten
   return and_count(add_rmsnorm_op(), ks, dst, x, r, w, eps, src, dst);
 }
 
+const auto& delta_step_inplace_op() {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::gated_delta_step_", "").typed<decltype(gated_delta_step_)>();
+  return op;
+}
+
+Tensor gated_delta_step__autograd(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                  const Tensor& beta, const Tensor& c, double scale) {
+  return without_backward("xlstm_hip::gated_delta_step_", delta_step_inplace_op(), ks, {q, k, v, g, beta, c}, q, k, v, g, beta,
+                          c, scale);
+}
+
+Tensor gated_delta_step__inplace(c10::DispatchKeySet ks, const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                 const Tensor& beta, const Tensor& c, double scale) {
+  return and_count(delta_step_inplace_op(), ks, {c}, q, k, v, g, beta, c, scale);
+}
+
 // The kernels below call the library with this build's argument lists: none is registered over one of another ABI
 // (xlstm_hip/_lib.py then says so in their place).
 bool abi_matches() { return xl_abi_version() == XL_ABI_VERSION; }
@@ -929,6 +1055,10 @@ TORCH_LIBRARY_IMPL(xlstm_hip, CUDA, m) {
   m.impl("layer_norm", layer_norm);
   m.impl("layer_norm_bwd", layer_norm_bwd);
   m.impl("newton_schulz", newton_schulz);
+  m.impl("gated_delta_chunkwise", gated_delta_chunkwise);
+  m.impl("gated_delta_recurrent", gated_delta_recurrent);
+  m.impl("gated_delta_step", gated_delta_step);
+  m.impl("gated_delta_step_", gated_delta_step_);
 }
 
 // The chunkwise forward and the layer norm differentiate through their own backward; every other operator is
@@ -937,18 +1067,20 @@ TORCH_LIBRARY_IMPL(xlstm_hip, CUDA, m) {
   for (const char* op : {"soft_cap", "mlstm_step", "mlstm_chunkwise_bwd", "mlstm_sequence", "slstm_step",              \
                          "slstm_sequence", "causal_conv1d", "group_norm", "mh_rmsnorm_gate", "gate_proj_softcap",      \
                          "gate_proj2_softcap", "lm_head_softcap", "rms_norm", "silu_mul", "layer_norm_bwd",             \
-                         "newton_schulz"})                                                                             \
+                         "newton_schulz", "gated_delta_recurrent", "gated_delta_step"})                                                                             \
     m.impl(op, kernel());
 TORCH_LIBRARY_IMPL(xlstm_hip, Autograd, m) {
   if (!abi_matches()) return;
   m.impl("mlstm_chunkwise", mlstm_chunkwise_autograd);
   m.impl("layer_norm", layer_norm_autograd);
   m.impl("mlstm_step_", mlstm_step__autograd);
+  m.impl("gated_delta_step_", gated_delta_step__autograd);
   m.impl("add_rmsnorm", add_rmsnorm_autograd);
   XL_FORWARD_ONLY(m, torch::autograd::autogradNotImplementedFallback)
 }
 TORCH_LIBRARY_IMPL(xlstm_hip, ADInplaceOrView, m) {
   if (!abi_matches()) return;
   m.impl("mlstm_step_", mlstm_step__inplace);
+  m.impl("gated_delta_step_", gated_delta_step__inplace);
   m.impl("add_rmsnorm", add_rmsnorm_inplace);
 }

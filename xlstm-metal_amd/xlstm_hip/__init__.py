@@ -17,6 +17,7 @@ from .backend import (
     mLSTMBackendConfig, wrap_chunkwise__arbitrary_sequence_length, wrap_chunkwise__pad_zeros,
 )
 from .chunkwise import mlstm_chunkwise, mlstm_chunkwise__native_autograd, mlstm_chunkwise__native_custbw
+from .delta import gated_delta_chunkwise, gated_delta_recurrent, gated_delta_step, gated_delta_step_
 from .ops import chunkwise_algorithm
 from .mlstm_layers import (
     MultiHeadLayerNorm, MultiHeadRMSNorm, gate_proj_softcap, mh_rmsnorm_gate, mLSTMOutputCell, mLSTMProjectionCell,
@@ -49,6 +50,7 @@ __all__ = [
     "causal_conv1d", "group_norm", "CausalConv1d", "sLSTMProjectionCell", "sLSTMOutputCell",
     "mh_rmsnorm_gate", "MultiHeadRMSNorm", "MultiHeadLayerNorm", "mLSTMOutputCell", "gate_proj_softcap",
     "mLSTMProjectionCell", "layer_norm", "multi_head_layer_norm", "newton_schulz",
+    "gated_delta_chunkwise", "gated_delta_recurrent", "gated_delta_step", "gated_delta_step_",
     "get_mlstm_kernel", "get_mlstm_step_kernel", "get_mlstm_sequence_kernel", "available_kernels",
     "wrap_chunkwise__arbitrary_sequence_length", "wrap_chunkwise__pad_zeros", "mLSTMBackendConfig",
     "mLSTMBackend", "load_library", "LIB_PATH",

@@ -61,10 +61,14 @@ SIGNATURES = {
     "xl_layer_norm_bwd": (_i, [_vp] * 2 + [ctypes.POINTER(_i64), _vp] + [_fp] * 2 + [_vp, ctypes.POINTER(_i64)] + [_vp] * 2
                           + [_i64] * 2 + [_i] * 4 + [_vp, _sz, _vp]),
     "xl_newton_schulz_workspace_size": (_sz, [_i64] + [_i] * 3),
+    "xl_gated_delta_recurrent_fwd": (_i, [_vp] * 5 + [_fp, _vp, _fp] + [_i] * 6 + [_f] + [_i] * 2 + [_vp]),
+    "xl_gated_delta_chunkwise_workspace_size": (_sz, [_i] * 7),
+    "xl_gated_delta_chunkwise_fwd": (_i, [_vp] * 3 + [ctypes.POINTER(_i64)] + [_vp] * 2 + [_fp, _vp, _fp] + [_i] * 6 + [_f]
+                                     + [_i] * 2 + [_vp, _sz, _vp]),
     "xl_newton_schulz": (_i, [_vp] * 2 + [_i64, _i, _i, ctypes.POINTER(_f), _i, _f, _i, _vp, _sz, _vp]),
 }
 
-ABI_VERSION = 4
+ABI_VERSION = 5
 
 _lib = None
 _lock = threading.Lock()

@@ -22,7 +22,8 @@ __all__ = [
     "soft_cap_op", "mlstm_step_op", "mlstm_step_inplace_op", "mlstm_chunkwise_op", "mlstm_chunkwise_bwd_op", "mlstm_sequence_op",
     "slstm_step_op", "slstm_sequence_op", "causal_conv1d_op", "group_norm_op", "mh_rmsnorm_gate_op",
     "gate_proj_softcap_op", "gate_proj2_softcap_op", "lm_head_softcap_op", "rms_norm_op", "add_rmsnorm_op", "silu_mul_op",
-    "layer_norm_op", "newton_schulz_op",
+    "layer_norm_op", "newton_schulz_op", "gated_delta_chunkwise_op", "gated_delta_recurrent_op", "gated_delta_step_op",
+    "gated_delta_step_inplace_op",
     "chunkwise_workspace_bytes", "chunkwise_algorithm",
 ]
 
@@ -77,6 +78,14 @@ _SCHEMAS = {
                       "output_mask) -> (Tensor, Tensor, Tensor)"),
     # coefficients: a, b, c of each step
     "newton_schulz": ("(Tensor x, float[] coefficients, float eps) -> Tensor"),
+    # (h, the last state, or an empty placeholder); q, k [B, NHK, S, DQK], v [B, NH, S, DV], gates [B, NH, S]
+    "gated_delta_chunkwise": ("(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? c0, float scale, bool "
+                             "return_last_states) -> (Tensor, Tensor)"),
+    "gated_delta_recurrent": ("(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? c0, float scale, bool "
+                             "return_last_states) -> (Tensor, Tensor)"),
+    # one token: no S axis; the in-place form returns h
+    "gated_delta_step": ("(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor c, float scale) -> (Tensor, Tensor)"),
+    "gated_delta_step_": ("(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor(a!) c, float scale) -> Tensor"),
 }
 
 _library = torch.library.Library("xlstm_hip", "DEF")
@@ -243,6 +252,27 @@ def _(x, coefficients, eps):
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
+def _gated_delta(q, k, v, g, beta, c0, scale, return_last_states):
+    B, _, S, DQK = q.shape
+    _, NH, _, DV = v.shape
+    return (q.new_empty((B, NH, S, DV)),
+            q.new_empty((B, NH, DQK, DV) if return_last_states else _EMPTY_SHAPE, dtype=torch.float32))
+
+
+_fake("gated_delta_chunkwise")(_gated_delta)
+_fake("gated_delta_recurrent")(_gated_delta)
+
+
+@_fake("gated_delta_step")
+def _(q, k, v, g, beta, c, scale):
+    return q.new_empty(v.shape), q.new_empty(c.shape, dtype=torch.float32)
+
+
+@_fake("gated_delta_step_")
+def _(q, k, v, g, beta, c, scale):
+    return q.new_empty(v.shape)
+
+
 soft_cap_op = torch.ops.xlstm_hip.soft_cap.default
 mlstm_step_op = torch.ops.xlstm_hip.mlstm_step.default
 mlstm_step_inplace_op = torch.ops.xlstm_hip.mlstm_step_.default
@@ -260,6 +290,10 @@ add_rmsnorm_op = torch.ops.xlstm_hip.add_rmsnorm.default
 silu_mul_op = torch.ops.xlstm_hip.silu_mul.default
 layer_norm_op = torch.ops.xlstm_hip.layer_norm.default
 newton_schulz_op = torch.ops.xlstm_hip.newton_schulz.default
+gated_delta_chunkwise_op = torch.ops.xlstm_hip.gated_delta_chunkwise.default
+gated_delta_recurrent_op = torch.ops.xlstm_hip.gated_delta_recurrent.default
+gated_delta_step_op = torch.ops.xlstm_hip.gated_delta_step.default
+gated_delta_step_inplace_op = torch.ops.xlstm_hip.gated_delta_step_.default
 
 CONV_ACTS = {None: 0, "silu": 1}
 # csrc/torch_ops.cpp's own (0 where no kernel can run): the most rows of lm_head_softcap and the LDS of its
