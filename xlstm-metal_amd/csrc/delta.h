@@ -43,18 +43,18 @@ constexpr float CLAMP_G = -1e4f;  // exp() of it is 0: a reset (-inf) keeps the 
 
 // Per head and chunk, by the first kernel: per-token factors (f16 planes' scales folded in) and scales.
 struct Factors {
-  double b[L];     // running sums of g
   float in[L];     // c_i 2^k            K S
   float q[L];      // scale c_i 2^q      Q S
   float out[L];    // c_L / c_i 2^k      U into the state
-  float back[L];   // beta_i c_i 2^k     Z into the state's gradient
-  float beta[L];
   float all;       // c_L
   float t, tt, p;  // T diag(beta), T and P = planes * these
   float k, qs;     // K, Q = planes * these
-  float pad[2];
+  float pad[58];   // the scans take the first 1 KB into LDS
+  float back[L];   // beta_i c_i 2^k     Z into the state's gradient
+  float beta[L];
+  double b[L];     // running sums of g
 };
-static_assert(sizeof(Factors) % 16 == 0);
+static_assert(sizeof(Factors) == 2048);
 
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -132,6 +132,15 @@ __device__ __forceinline__ f16x8 columns_frag(const char* img, int t, int s, int
   return __builtin_bit_cast(f16x8, mfma::tr_pair(a, a + 16 * DKP * 2));  // 16 tokens on: the same token % 8
 }
 
+// The operands of a 64 x 64 matrix with nothing above its diagonal (below, for a transposed one): 6 of the 8.
+constexpr int LOWER = 6;
+__device__ __host__ constexpr int lower_mt(int i) { return i < 2 ? i : 2 + (i - 2) / 2; }
+__device__ __host__ constexpr int lower_s(int i) { return i < 2 ? 0 : (i - 2) % 2; }
+__device__ __forceinline__ void load_lower(const f16_t* from, int lane, f16x8 (&to)[LOWER]) {
+#pragma unroll
+  for (int i = 0; i < LOWER; ++i) to[i] = *((const f16x8*)from + (2 * lower_mt(i) + lower_s(i)) * 64 + lane);
+}
+
 // ------------------------------------------------------------------------------------------------ workspace, shapes
 struct Shape {
   int B, NH, NHK, S, DK, DV;
@@ -156,7 +165,8 @@ struct Prep {
 
 int check_shape(const char* who, const Shape& s);
 // q, k, v strides from the caller's nine or of contiguous tensors
-void set_strides(Shape& s, const int64_t* strides);
+int set_strides(Shape& s, const int64_t* strides, const char* who);
+constexpr int MAX_TOKEN_STRIDE = 1 << 22;
 size_t prep_bytes(const Shape& s, bool backward);
 Prep prep_at(const Shape& s, bool backward, char* ws);
 int launch_prep(const Shape& s, const void* q, const void* k, const void* g, const void* beta, const Prep& p, bool backward,

@@ -26,7 +26,7 @@ template <typename T, int DKB, int STAGES>
 __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
   constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
   constexpr bool PAIR = !std::is_same_v<T, bf16_t>;
-  extern __shared__ __align__(1024) char lds[];
+  extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, gq = lane >> 4;
   const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
@@ -34,8 +34,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
   const int b = bh / p.NH, h = bh - b * p.NH;
   const int64_t image0 = ((int64_t)b * (p.NH / p.group) + h / p.group) * p.chunks, part0 = (int64_t)bh * p.chunks;
   const int n0 = (slice * waves + wave) * 16, n = n0 + r;
-  const bool column = n < p.DV;
-  const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1] + n;
+  const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
   T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
 
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
@@ -47,15 +46,32 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       to_lds(lds_at + stage * STAGE + IMG + i * 1024, i * 1024 + lane * 16, qi);
     }
   };
-  // rows 16 mt + 4 gq + e of column n
-  auto load_v = [&](int chunk, float (&to)[4][4]) {
+  auto fetch_factors = [&](int chunk) {
+    if (wave == 0) to_lds(lds_at + STAGES * STAGE + (chunk & 1) * 1024, lane * 16, p.prep.f + part0 + chunk);
+  };
+  // Rows 16 mt + 4 gq + e of column n.  Past the last token the last one is read again, for zeros; past the last column the
+  // last one: those columns are computed and not written.
+  const int nc = n < p.DV ? n : p.DV - 1, row_step = (int)p.vs[2];
+  T vn[4][4];
+  auto load_v = [&](int chunk) {
+    const int t0 = chunk * L;
+    const T* base = v + t0 * p.vs[2];
+    if (t0 + L <= p.S) {
+      const uint32_t at = (uint32_t)(4 * gq * row_step + nc) * sizeof(T);
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt)
+      for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int t = chunk * L + 16 * mt + 4 * gq + e;
-        to[mt][e] = column && t < p.S ? to_f32(v[t * p.vs[2]]) : 0.f;
-      }
+        for (int e = 0; e < 4; ++e) vn[mt][e] = *(const T*)((const char*)(base + (16 * mt + e) * p.vs[2]) + at);
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = 16 * mt + 4 * gq + e;
+          const T x = base[(t0 + t < p.S ? t : 0) * p.vs[2] + nc];
+          vn[mt][e] = t0 + t < p.S ? x : from_f32<T>(0.f);
+        }
+    }
   };
 
   f32x4 st[2 * DKB];
@@ -64,22 +80,38 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       const int d = 16 * t + 4 * gq + e;
-      st[t][e] = p.c0 && column && d < p.DK ? p.c0[((int64_t)bh * p.DK + d) * p.DV + n] : 0.f;
+      st[t][e] = p.c0 && d < p.DK ? p.c0[((int64_t)bh * p.DK + d) * p.DV + nc] : 0.f;
     }
 
+  // T and P of the next chunk wait in registers, K, Q and the factors in LDS
+  f16x8 th[LOWER], tl[LOWER], ph[LOWER], pl[PAIR ? LOWER : 1];
+  auto load_t = [&](int chunk) {
+    const f16_t* from = p.prep.t + (part0 + chunk) * (2 * FRAG_PLANE);
+    load_lower(from, lane, th);
+    load_lower(from + FRAG_PLANE, lane, tl);
+  };
+  auto load_p = [&](int chunk) {
+    const f16_t* from = p.prep.p + (part0 + chunk) * (2 * FRAG_PLANE);
+    load_lower(from, lane, ph);
+    if constexpr (PAIR) load_lower(from + FRAG_PLANE, lane, pl);
+  };
   fetch(0, 0);
-  float vn[4][4];
-  load_v(0, vn);
+  fetch_factors(0);
+  load_v(0);
+  load_t(0);
+  load_p(0);
   for (int c = 0; c < p.chunks; ++c) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     const int stage = STAGES == 2 ? c & 1 : 0;
-    if (STAGES == 2 && c + 1 < p.chunks) fetch(c + 1, stage ^ 1);
+    const bool more = c + 1 < p.chunks;
+    if (more) {
+      if (STAGES == 2) fetch(c + 1, stage ^ 1);
+      fetch_factors(c + 1);
+    }
     const char *ki = lds + stage * STAGE, *qi = ki + IMG;
-    const Factors* f = p.prep.f + part0 + c;
-    const f16x8* tf = (const f16x8*)(p.prep.t + (part0 + c) * (2 * FRAG_PLANE)) + lane;
-    const f16x8* pf = (const f16x8*)(p.prep.p + (part0 + c) * (2 * FRAG_PLANE)) + lane;
+    const Factors* f = (const Factors*)(lds + STAGES * STAGE + (c & 1) * 1024);
 
     // ---- K S, and Q S turned
     float m = 0.f;
@@ -117,62 +149,65 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       const f32x4 in = *(const f32x4*)&f->in[16 * mt + 4 * gq];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        rr[mt][e] = vn[mt][e] - in[e] * (ks[mt][e] * ss.down);
+        rr[mt][e] = to_f32(vn[mt][e]) - in[e] * (ks[mt][e] * ss.down);
         m = fmaxf(m, fabsf(rr[mt][e]));
       }
     }
+    if (more) load_v(c + 1);
     const Pow2 rs = pow2_for(wave_max_all(m));
     f16x8 rh[2], rl[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) split8<true>(rr[2 * s], rr[2 * s + 1], rs.up, rh[s], rl[s]);
-    // ---- U (T is zero above its diagonal: the second half of k from row tile 2 on)
+    // ---- U
     f32x4 u[4];
     const float back = f->t * rs.down;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) u[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < LOWER; ++i) {
+      f32x4& x = u[lower_mt(i)];
+      x = mfma(tl[i], rh[lower_s(i)], x);
+      x = mfma(th[i], rl[lower_s(i)], x);
+      x = mfma(th[i], rh[lower_s(i)], x);
+    }
+    if (more) load_t(c + 1);
     m = 0.f;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
-      u[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      u[mt] *= back;
 #pragma unroll
-      for (int s = 0; s <= mt / 2; ++s) {
-        const f16x8 th = tf[(2 * mt + s) * 64], tl = tf[FRAGS * 64 + (2 * mt + s) * 64];
-        u[mt] = mfma(tl, rh[s], u[mt]);
-        u[mt] = mfma(th, rl[s], u[mt]);
-        u[mt] = mfma(th, rh[s], u[mt]);
-      }
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        u[mt][e] *= back;
-        m = fmaxf(m, fabsf(u[mt][e]));
-      }
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(u[mt][e]));
     }
     const float most_u = wave_max_all(m);
     const Pow2 us = pow2_for(most_u);
-    if (c + 1 < p.chunks) load_v(c + 1, vn);
     // ---- H
     {
       f16x8 uh[2], ul[2];
 #pragma unroll
       for (int s = 0; s < 2; ++s) split8<PAIR>(u[2 * s], u[2 * s + 1], us.up, uh[s], ul[s]);
+      f32x4 x[4];
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) x[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < LOWER; ++i) {
+        f32x4& y = x[lower_mt(i)];
+        if constexpr (PAIR) {
+          y = mfma(ul[lower_s(i)], ph[i], y);
+          y = mfma(uh[lower_s(i)], pl[i], y);
+        }
+        y = mfma(uh[lower_s(i)], ph[i], y);
+      }
+      if (more) load_p(c + 1);
       const float pu = f->p * us.down;
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        f32x4 x = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int s = 0; s <= mt / 2; ++s) {
-          const f16x8 ph = pf[(2 * mt + s) * 64];
-          if constexpr (PAIR) {
-            x = mfma(ul[s], ph, x);
-            x = mfma(uh[s], pf[FRAGS * 64 + (2 * mt + s) * 64], x);
-          }
-          x = mfma(uh[s], ph, x);
-        }
         const int t = c * L + 16 * mt + r;
         const float fq = f->q[16 * mt + r] * ss.down;
         if (t < p.S) {
           T* to = ho + (int64_t)t * p.DV + n0 + 4 * gq;
           struct alignas(4 * sizeof(T)) Four { T e[4]; } out;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) out.e[e] = from_f32<T>(fmaf(x[e], pu, hs[mt][e] * fq));
+          for (int e = 0; e < 4; ++e) out.e[e] = from_f32<T>(fmaf(x[mt][e], pu, hs[mt][e] * fq));
           if (p.DV % 4 == 0) {
             if (n0 + 4 * gq < p.DV) *(Four*)to = out;
           } else {
@@ -184,8 +219,8 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       }
     }
     // ---- the state
-    const float all = f->all;
-    m = most * all;
+    const float keep = f->all;
+    m = most * keep;
     f32x4 w[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
@@ -197,10 +232,10 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
     f16x8 wh[2], wl[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) split8<true>(w[2 * s], w[2 * s + 1], ws.up, wh[s], wl[s]);
-    const float keep = all * ws.up;
+    const float up = keep * ws.up;
 #pragma unroll
     for (int t = 0; t < 2 * DKB; ++t) {
-      f32x4 x = st[t] * keep;
+      f32x4 x = st[t] * up;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         const f16x8 k = columns_frag<DKP>(ki, t, s, r, gq);
@@ -214,10 +249,10 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (c + 1 < p.chunks) fetch(c + 1, 0);
+      if (more) fetch(c + 1, 0);
     }
   }
-  if (p.c_last && column) {
+  if (p.c_last && n < p.DV) {
 #pragma unroll
     for (int t = 0; t < 2 * DKB; ++t)
 #pragma unroll
@@ -249,7 +284,7 @@ int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* 
                      : s.dtype == XL_DTYPE_BF16 ? pick<bf16_t>(s.dkp(), stages) : pick<f16_t>(s.dkp(), stages);
   const int blocks = (s.DV + 15) / 16, waves = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
   a.slices = (blocks + waves - 1) / waves;
-  const int64_t lds = stages * 2 * s.image_bytes();
+  const int64_t lds = stages * 2 * s.image_bytes() + 2 * 1024;
   void* args[] = {&a};
   hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (e == hipSuccess)
@@ -286,7 +321,7 @@ extern "C" int xl_gated_delta_chunkwise_fwd(const void* q, const void* k, const 
   const size_t need = delta::prep_bytes(s, false);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255))
     return set_error(XL_ERR_WORKSPACE, "%s: the workspace must be %zu bytes, 256-byte aligned", who, need);
-  delta::set_strides(s, strides);
+  if (const int rc = delta::set_strides(s, strides, who)) return rc;
   const hipStream_t st = (hipStream_t)stream;
   const delta::Prep prep = delta::prep_at(s, false, (char*)workspace);
   if (const int rc = delta::launch_prep(s, q, k, g, beta, prep, false, st, who)) return rc;

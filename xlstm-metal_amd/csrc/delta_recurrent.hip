@@ -169,14 +169,17 @@ int check_shape(const char* who, const Shape& s) {
   return XL_OK;
 }
 
-void set_strides(Shape& s, const int64_t* strides) {
+int set_strides(Shape& s, const int64_t* strides, const char* who) {
   if (strides) {
+    for (int i = 0; i < 3; ++i)  // a token stride is multiplied by up to 63 in 32 bits
+      if (strides[3 * i + 2] < 0 || strides[3 * i + 2] > MAX_TOKEN_STRIDE)
+        return set_error(XL_ERR_UNSUPPORTED, "%s: token strides must be 0 to %d elements", who, MAX_TOKEN_STRIDE);
     for (int i = 0; i < 3; ++i) {
       s.qs[i] = strides[i];
       s.ks[i] = strides[3 + i];
       s.vs[i] = strides[6 + i];
     }
-    return;
+    return XL_OK;
   }
   auto dense = [&](int64_t (&to)[3], int heads, int D) {
     to[2] = D;
@@ -186,6 +189,7 @@ void set_strides(Shape& s, const int64_t* strides) {
   dense(s.qs, s.NHK, s.DK);
   dense(s.ks, s.NHK, s.DK);
   dense(s.vs, s.NH, s.DV);
+  return XL_OK;
 }
 
 int launch_recurrent(const Shape& s, const void* q, const void* k, const void* v, const void* g, const void* beta,

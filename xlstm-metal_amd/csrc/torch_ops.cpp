@@ -860,7 +860,7 @@ struct DeltaSizes {
 };
 // q, k and v as they lie where their last axis is contiguous (strides: batch, head, token of each)
 Tensor delta_rows(const Tensor& t, int64_t* strides) {
-  const Tensor r = t.size(3) <= 1 || t.stride(3) == 1 ? t : t.contiguous();
+  const Tensor r = (t.size(3) <= 1 || t.stride(3) == 1) && t.stride(2) <= (1 << 22) ? t : t.contiguous();
   for (int d = 0; d < 3; ++d) strides[d] = r.stride(d);
   return r;
 }
