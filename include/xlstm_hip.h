@@ -436,6 +436,19 @@ int xl_gated_delta_chunkwise_fwd(const void* q, const void* k, const void* v, co
                                  int DQK, int DV, float scale, int dtype_qkv, int dtype_gates, void* workspace,
                                  size_t workspace_bytes, void* stream);
 
+/*
+ * Its gradients: dq, dk [B, NHK, S, DQK] and dv [B, NH, S, DV] of dtype_qkv, dg, dbeta [B, NH, S] of dtype_gates, all
+ * contiguous (dq, dk and dv 16-byte aligned), and dc0 float32 or NULL, from dh [B, NH, S, DV] of dtype_qkv, contiguous, and
+ * dc_last, the gradient of the last state, float32 or NULL.  S at least 1.  The workspace
+ * (xl_gated_delta_chunkwise_bwd_workspace_size bytes, 256-byte aligned) holds every chunk's state and its gradient.
+ */
+size_t xl_gated_delta_chunkwise_bwd_workspace_size(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv);
+int xl_gated_delta_chunkwise_bwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* g,
+                                 const void* beta, const float* c0, const void* dh, const float* dc_last, void* dq,
+                                 void* dk, void* dv, void* dg, void* dbeta, float* dc0, int B, int NH, int NHK, int S,
+                                 int DQK, int DV, float scale, int dtype_qkv, int dtype_gates, void* workspace,
+                                 size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

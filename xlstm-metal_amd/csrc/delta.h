@@ -60,14 +60,16 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
-// 2^target / 2^exponent(m) and its inverse: m times the first is in [2^target, 2^(target + 1)); m >= 0, the same in the wave
+// 2^target / 2^exponent(m) and its inverse: m times the first is in [2^target, 2^(target + 1)); m >= 0, the same in the wave.
+// At most 2^limit either way (0 gets that); KEPT for scales of which two are multiplied.
+constexpr int KEPT = 60;
 struct Pow2 {
   float up, down;
 };
-__device__ __forceinline__ Pow2 pow2_for(float m, int target = 14) {
+__device__ __forceinline__ Pow2 pow2_for(float m, int target = 14, int limit = 100) {
   const int e = (int)(__float_as_uint(m) >> 23);
   int sh = e == 255 ? 0 : target + 127 - e;
-  sh = sh > 100 ? 100 : sh < -100 ? -100 : sh;
+  sh = sh > limit ? limit : sh < -limit ? -limit : sh;
   return {__uint_as_float((uint32_t)(127 + sh) << 23), __uint_as_float((uint32_t)(127 - sh) << 23)};
 }
 
@@ -140,6 +142,25 @@ __device__ __forceinline__ void load_lower(const f16_t* from, int lane, f16x8 (&
 #pragma unroll
   for (int i = 0; i < LOWER; ++i) to[i] = *((const f16x8*)from + (2 * lower_mt(i) + lower_s(i)) * 64 + lane);
 }
+// of a transposed one: row tiles 0 and 1 have both halves of k, 2 and 3 the second
+__device__ __host__ constexpr int upper_mt(int i) { return i < 4 ? i / 2 : i - 2; }
+__device__ __host__ constexpr int upper_s(int i) { return i < 4 ? i % 2 : 1; }
+__device__ __forceinline__ void load_upper(const f16_t* from, int lane, f16x8 (&to)[LOWER]) {
+#pragma unroll
+  for (int i = 0; i < LOWER; ++i) to[i] = *((const f16x8*)from + (2 * upper_mt(i) + upper_s(i)) * 64 + lane);
+}
+
+// What the backward keeps of a scan for the chunks' gradients, by 16 columns n (a wave's): tokens x n, [plane][16 n][64 tokens,
+// turned], and states, [plane][16 n][DKP, turned], f16 at a scale of their own.  Blocks of 16 are padded to an even number.
+struct Kept {
+  f16_t *u, *z, *dh;   // tokens x n
+  f16_t *s0, *ds;      // the state before the chunk, the gradient of the state behind it
+  float *us, *zs, *dhs, *s0s, *dss;  // values = planes * these (a block of zeros: the least)
+  int blocks;          // of a head, padded
+};
+__device__ __forceinline__ int64_t kept_at(int64_t part, int blocks, int block, int planes, int width) {
+  return ((part * blocks + block) * planes) * (int64_t)(16 * width);
+}
 
 // ------------------------------------------------------------------------------------------------ workspace, shapes
 struct Shape {
@@ -170,6 +191,9 @@ constexpr int MAX_TOKEN_STRIDE = 1 << 22;
 size_t prep_bytes(const Shape& s, bool backward);
 Prep prep_at(const Shape& s, bool backward, char* ws);
 int launch_prep(const Shape& s, const void* q, const void* k, const void* g, const void* beta, const Prep& p, bool backward,
+                hipStream_t st, const char* who);
+// The scan: h (and c_last), or for the backward every chunk's U and state before it.
+int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* c_last, const Prep& prep, const Kept* kept,
                 hipStream_t st, const char* who);
 int launch_recurrent(const Shape& s, const void* q, const void* k, const void* v, const void* g, const void* beta,
                      const float* c0, void* h, float* c_last, hipStream_t st, const char* who);

@@ -1,0 +1,945 @@
+// Gradients of the gated delta rule by chunks (delta.h has the forward's formulas).  From dH and dS, the gradient of the state
+// behind a chunk:
+//
+//   dU = P^T dH + diag(c_L / c_j) K dS,  Z = T^T dU,  dV = diag(beta) Z,
+//   dS_0 = c_L dS + scale (diag(c) Q)^T dH - (diag(c beta) K)^T Z
+//
+// are again of each column by itself: a scan from the last chunk to the first, built as the forward's.  U and the states
+// are formed again by the forward's scan.  Both scans keep U, Z, S_0 and dS in f16 planes for the last kernel, a workgroup a
+// chunk, which sums over the columns:
+//
+//   dP = dH U^T (j <= i),  dA = -Z U^T (j < i),  N_ij = D_ij k_i.k_j,  E_ij = dA_ij beta_i D_ij
+//   dQ = scale (diag(c) dH S_0^T + (D o dP) K)
+//   dK = diag(c_L / c_j) U dS^T - diag(c beta) Z S_0^T + scale (D o dP)^T Q + (E + E^T) K
+//   dbeta_i = Z_i.V_i - c_i k_i.(Z S_0^T)_i + sum_j dA_ij N_ij
+//
+// and for dg every term's exponent b_i - b_j, which b_i gets and b_j loses: rows and columns of dP o P and dA o A, q.dQ's and
+// k.dK's parts with the states, c_L <dS, S_0>; dg_t is the sum of b's gradients from t to the chunk's end.  (The same numbers
+// are added at a term's later token and taken off at its earlier one, so what does not pass t cancels to float32's rounding.)
+//
+// Heads of v that share q and k write their dQ and dK in float32, and a last kernel adds them in order.
+#include "delta.h"
+
+namespace xl {
+namespace delta {
+namespace {
+
+// ------------------------------------------------------------------------------------------------ dH by columns
+struct TurnArgs {
+  const void* dh;
+  Kept kept;
+  int S, DV, chunks;
+};
+
+template <typename T>
+__global__ __launch_bounds__(256) void delta_turn_kernel(TurnArgs p) {
+  constexpr int PK = is_f32<T>::value ? 2 : 1;
+  __shared__ float tile[L][65];
+  const int64_t part = blockIdx.x;
+  const int64_t bh = part / p.chunks;
+  const int t0 = (int)(part - bh * p.chunks) * L, n0 = blockIdx.y * 64;
+  const int row = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
+  const T* from = (const T*)p.dh + (bh * p.S + t0 + row) * p.DV + n0 + c;
+#pragma unroll
+  for (int e = 0; e < 16; ++e) tile[row][c + e] = t0 + row < p.S && n0 + c + e < p.DV ? to_f32(from[e]) : 0.f;
+  __syncthreads();
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, gq = lane >> 4, block = blockIdx.y * 4 + wave;
+  if (block >= p.kept.blocks) return;
+  float x[2][8], m = 0.f;
+#pragma unroll
+  for (int s = 0; s < 2; ++s)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      x[s][e] = tile[32 * s + (e < 4 ? 4 * gq + e : 12 + 4 * gq + e)][16 * wave + r];
+      m = fmaxf(m, fabsf(x[s][e]));
+    }
+  const Pow2 sc = pow2_for(wave_max_all(m), 14, KEPT);
+#pragma unroll
+  for (int s = 0; s < 2; ++s) {
+    f16x8 hi, lo;
+    split8<PK == 2>(x[s], sc.up, hi, lo);
+    f16_t* to = p.kept.dh + kept_at(part, p.kept.blocks, block, PK, L) + r * L + s * 32 + gq * 8;
+    *(f16x8*)to = hi;
+    if constexpr (PK == 2) *(f16x8*)(to + 16 * L) = lo;
+  }
+  if (lane == 0) p.kept.dhs[part * p.kept.blocks + block] = sc.down;
+}
+
+// ------------------------------------------------------------------------------------------------ the scan backwards
+struct BackArgs {
+  const float* dc_last;
+  float* dc0;
+  Prep prep;
+  Kept kept;
+  int NH, group, DK, DV, chunks, slices;
+};
+
+template <typename T, int DKB, int STAGES>
+__global__ __launch_bounds__(256, 1) void delta_back_kernel(BackArgs p) {
+  constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
+  extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int r = lane & 15, gq = lane >> 4;
+  const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
+  const int bh = __builtin_amdgcn_readfirstlane(all / p.slices), slice = all - bh * p.slices;
+  const int b = bh / p.NH, h = bh - b * p.NH;
+  const int64_t image0 = ((int64_t)b * (p.NH / p.group) + h / p.group) * p.chunks, part0 = (int64_t)bh * p.chunks;
+  // past the last block a wave computes it again and writes nothing
+  const int own = slice * waves + wave, block = own < p.kept.blocks ? own : p.kept.blocks - 1, n = block * 16 + r;
+  const bool mine = own < p.kept.blocks;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
+  auto fetch = [&](int chunk, int stage) {
+    const char* ki = p.prep.k + (image0 + chunk) * (int64_t)IMG;
+    const char* qi = p.prep.q + (image0 + chunk) * (int64_t)IMG;
+    for (int i = wave; i < IMG / 1024; i += waves) {
+      to_lds(lds_at + stage * STAGE + i * 1024, i * 1024 + lane * 16, ki);
+      to_lds(lds_at + stage * STAGE + IMG + i * 1024, i * 1024 + lane * 16, qi);
+    }
+  };
+  auto fetch_factors = [&](int chunk) {
+    if (wave != 0) return;
+    to_lds(lds_at + STAGES * STAGE + (chunk & 1) * 2048, lane * 16, p.prep.f + part0 + chunk);
+    to_lds(lds_at + STAGES * STAGE + (chunk & 1) * 2048 + 1024, 1024 + lane * 16, p.prep.f + part0 + chunk);
+  };
+  f32x4 st[2 * DKB];
+#pragma unroll
+  for (int t = 0; t < 2 * DKB; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 16 * t + 4 * gq + e;
+      st[t][e] = p.dc_last && d < p.DK && n < p.DV ? p.dc_last[((int64_t)bh * p.DK + d) * p.DV + n] : 0.f;
+    }
+  f16x8 th[LOWER], tl[LOWER], ph[LOWER], pl[LOWER], dh[2], dl[2];
+  float dh_scale = 0.f;
+  auto load_t = [&](int chunk) {
+    const f16_t* from = p.prep.tt + (part0 + chunk) * (2 * FRAG_PLANE);
+    load_upper(from, lane, th);
+    load_upper(from + FRAG_PLANE, lane, tl);
+  };
+  auto load_p = [&](int chunk) {
+    const f16_t* from = p.prep.pt + (part0 + chunk) * (2 * FRAG_PLANE);
+    load_upper(from, lane, ph);
+    load_upper(from + FRAG_PLANE, lane, pl);
+  };
+  auto load_dh = [&](int chunk) {
+    const f16_t* from = p.kept.dh + kept_at(part0 + chunk, p.kept.blocks, block, PK, L) + r * L + gq * 8;
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      dh[s] = *(const f16x8*)(from + s * 32);
+      if constexpr (PK == 2) dl[s] = *(const f16x8*)(from + s * 32 + 16 * L);
+    }
+    dh_scale = p.kept.dhs[(part0 + chunk) * p.kept.blocks + block];
+  };
+  const int last = p.chunks - 1;
+  fetch(last, STAGES == 2 ? last & 1 : 0);
+  fetch_factors(last);
+  load_t(last);
+  load_p(last);
+  load_dh(last);
+  for (int c = last; c >= 0; --c) {
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int stage = STAGES == 2 ? c & 1 : 0;
+    const bool more = c > 0;
+    if (more) {
+      if (STAGES == 2) fetch(c - 1, stage ^ 1);
+      fetch_factors(c - 1);
+    }
+    const char *ki = lds + stage * STAGE, *qi = ki + IMG;
+    const Factors* f = (const Factors*)(lds + STAGES * STAGE + (c & 1) * 2048);
+    const int64_t at = (part0 + c) * p.kept.blocks + block;
+    // ---- K dS; dS is kept
+    float m = 0.f;
+#pragma unroll
+    for (int t = 0; t < 2 * DKB; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(st[t][e]));
+    const float most = wave_max_all(m);
+    const Pow2 ss = pow2_for(most, 14, KEPT);
+    f32x4 ks[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) ks[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    f16_t* const to_ds = p.kept.ds + kept_at(part0 + c, p.kept.blocks, block, PK, DKP) + r * DKP + gq * 8;
+#pragma unroll
+    for (int s = 0; s < DKB; ++s) {
+      f16x8 hi, lo;
+      split8<true>(st[2 * s], st[2 * s + 1], ss.up, hi, lo);
+      if (mine) {
+        *(f16x8*)(to_ds + s * 32) = hi;
+        if constexpr (PK == 2) *(f16x8*)(to_ds + s * 32 + 16 * DKP) = lo;
+      }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const f16x8 k = rows_frag<DKP>(ki, mt, s, r, gq);
+        if constexpr (PK == 2) ks[mt] = mfma(rows_frag<DKP>(ki + PLANE, mt, s, r, gq), hi, ks[mt]);
+        ks[mt] = mfma(k, lo, ks[mt]);
+        ks[mt] = mfma(k, hi, ks[mt]);
+      }
+    }
+    // ---- dU
+    f32x4 x[4], du[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) x[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < LOWER; ++i) {
+      f32x4& y = x[upper_mt(i)];
+      if constexpr (PK == 2) y = mfma(ph[i], dl[upper_s(i)], y);
+      y = mfma(pl[i], dh[upper_s(i)], y);
+      y = mfma(ph[i], dh[upper_s(i)], y);
+    }
+    if (more) load_p(c - 1);
+    const float px = f->p * dh_scale;
+    m = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const f32x4 out = *(const f32x4*)&f->out[16 * mt + 4 * gq];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        du[mt][e] = fmaf(x[mt][e], px, out[e] * (ks[mt][e] * ss.down));
+        m = fmaxf(m, fabsf(du[mt][e]));
+      }
+    }
+    const Pow2 us = pow2_for(wave_max_all(m));
+    f16x8 uh[2], ul[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) split8<true>(du[2 * s], du[2 * s + 1], us.up, uh[s], ul[s]);
+    // ---- Z
+    f32x4 z[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) z[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < LOWER; ++i) {
+      f32x4& y = z[upper_mt(i)];
+      y = mfma(tl[i], uh[upper_s(i)], y);
+      y = mfma(th[i], ul[upper_s(i)], y);
+      y = mfma(th[i], uh[upper_s(i)], y);
+    }
+    if (more) load_t(c - 1);
+    const float back = f->tt * us.down;
+    m = 0.f;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      z[mt] *= back;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(z[mt][e]));
+    }
+    const Pow2 zs = pow2_for(wave_max_all(m), 14, KEPT);
+    if (mine) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f16x8 zh, zl;
+        split8<PK == 2>(z[2 * s], z[2 * s + 1], zs.up, zh, zl);
+        f16_t* to = p.kept.z + kept_at(part0 + c, p.kept.blocks, block, PK, L) + r * L + s * 32 + gq * 8;
+        *(f16x8*)to = zh;
+        if constexpr (PK == 2) *(f16x8*)(to + 16 * L) = zl;
+      }
+      if (lane == 0) {
+        p.kept.zs[at] = zs.down;
+        p.kept.dss[at] = ss.down;
+      }
+    }
+    // ---- dS: Q^T w1 + K^T w2
+    f32x4 w1[4], w2[4];
+    const float keep = f->all;
+    m = most * keep;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const f32x4 fq = *(const f32x4*)&f->q[16 * mt + 4 * gq], fb = *(const f32x4*)&f->back[16 * mt + 4 * gq];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float d = (float)dh[mt >> 1][(mt & 1) * 4 + e];
+        if constexpr (PK == 2) d += (float)dl[mt >> 1][(mt & 1) * 4 + e];
+        w1[mt][e] = fq[e] * (d * dh_scale);
+        w2[mt][e] = -fb[e] * z[mt][e];
+        m = fmaxf(m, fmaxf(fabsf(w1[mt][e]), fabsf(w2[mt][e])));
+      }
+    }
+    if (more) load_dh(c - 1);
+    const Pow2 ws = pow2_for(wave_max_all(m));
+    f16x8 w1h[2], w1l[2], w2h[2], w2l[2];
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      split8<true>(w1[2 * s], w1[2 * s + 1], ws.up, w1h[s], w1l[s]);
+      split8<true>(w2[2 * s], w2[2 * s + 1], ws.up, w2h[s], w2l[s]);
+    }
+    const float up = keep * ws.up;
+#pragma unroll
+    for (int t = 0; t < 2 * DKB; ++t) {
+      f32x4 y = st[t] * up;
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const f16x8 k = columns_frag<DKP>(ki, t, s, r, gq), q = columns_frag<DKP>(qi, t, s, r, gq);
+        if constexpr (PK == 2) {
+          y = mfma(columns_frag<DKP>(qi + PLANE, t, s, r, gq), w1h[s], y);
+          y = mfma(columns_frag<DKP>(ki + PLANE, t, s, r, gq), w2h[s], y);
+        }
+        y = mfma(q, w1l[s], y);
+        y = mfma(k, w2l[s], y);
+        y = mfma(q, w1h[s], y);
+        y = mfma(k, w2h[s], y);
+      }
+      st[t] = y * ws.down;
+    }
+    if (STAGES == 1) {
+      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (more) fetch(c - 1, 0);
+    }
+  }
+  if (p.dc0 && mine && n < p.DV) {
+#pragma unroll
+    for (int t = 0; t < 2 * DKB; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 16 * t + 4 * gq + e;
+        if (d < p.DK) p.dc0[((int64_t)bh * p.DK + d) * p.DV + n] = st[t][e];
+      }
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ a chunk's gradients
+struct GradArgs {
+  const void* v;
+  int64_t vs[3];
+  void *dq, *dk, *dv, *dg, *dbeta;  // dq, dk: [B, NHK, S, DK], or float32 [B, NH, S, DK] where heads share
+  Prep prep;
+  Kept kept;
+  int NH, group, S, DK, DV, chunks, gate_dtype;
+  float scale;
+  bool wide_v;
+};
+
+constexpr int GLD = 65;
+
+// exp(x): float32's rounding of x alone would cost |x| 2^-24 of the result
+__device__ __forceinline__ float exp_of(double x) {
+  const float hi = (float)x, e = expf(hi);
+  return fmaf(e, (float)(x - (double)hi), e);
+}
+
+template <typename T, int DKB>
+struct GradLds {
+  static constexpr int PK = is_f32<T>::value ? 2 : 1, DKP = DKB * 32;
+  static constexpr int TOK = 32 * L * 2, STA = 32 * DKP * 2;  // 32 columns of one plane
+  static constexpr int STAGE = PK * (3 * TOK + 2 * STA), IMAGE = PK * L * DKP * 2;
+  static constexpr int KK = L * GLD * 4;
+  static constexpr int A = STAGE > IMAGE + KK ? STAGE : IMAGE + KK;  // the columns; then K or Q, and K K^T
+  static constexpr int B = 2 * KK > 6 * L * L * 2 ? 2 * KK : 6 * L * L * 2;  // dP, dA; then their operands
+  static constexpr int SMALL = 6 * 8 * L * 4 + 64 * 4 + L * 8 + 4 * L * 4;
+  static constexpr int BYTES = A + B + SMALL;
+};
+
+// DKB waves: a wave has 32 of DQK's columns of dQ and dK, turned (columns down, tokens across), and its share of the 64 x 64 tiles.
+template <typename T, int DKB>
+__global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
+  using Lds = GradLds<T, DKB>;
+  constexpr int PK = Lds::PK, DKP = Lds::DKP, PLANE = L * DKP * 2, TOK = Lds::TOK, STA = Lds::STA, W = DKB, THREADS = 64 * W;
+  constexpr bool PAIR = !std::is_same_v<T, bf16_t>;
+  extern __shared__ __align__(1024) char lds[];
+  char *areaA = lds, *areaB = lds + Lds::A;
+  float* kkm = (float*)(lds + Lds::IMAGE);
+  float *dpm = (float*)areaB, *dam = (float*)(areaB + Lds::KK);
+  float* red = (float*)(areaB + Lds::B);  // [6][8][L]
+  float* wred = red + 6 * 8 * L;          // [64]
+  double* bs = (double*)(wred + 64);
+  float* betas = (float*)(bs + L);        // [L], then row sums [2][L], spare [L]
+  float* rows = betas + L;
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = lane & 15, gq = lane >> 4;
+  const int64_t part = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
+  const int bh = (int)(part / p.chunks), chunk = (int)(part - (int64_t)bh * p.chunks);
+  const int b = bh / p.NH, h = bh - b * p.NH, t0 = chunk * L;
+  const int64_t image = ((int64_t)b * (p.NH / p.group) + h / p.group) * p.chunks + chunk;
+  const Factors* f = p.prep.f + part;
+  const int blocks = p.kept.blocks;
+  const int64_t blk0 = part * blocks;
+
+  // ---- Blocks of columns have scales of their own; a product's sum over the columns takes the largest of its two scales'
+  // product, and one operand of a smaller block the factor that is left.
+  const float* const scales[5] = {p.kept.dhs + blk0, p.kept.zs + blk0, p.kept.us + blk0, p.kept.s0s + blk0, p.kept.dss + blk0};
+  enum { DH_S, Z_S, U_DS, DH_U, Z_U, S_DS, SUMS };
+  auto products = [&](int block, float (&to)[SUMS]) {
+    const float dh = scales[0][block], z = scales[1][block], u = scales[2][block], s0 = scales[3][block], ds = scales[4][block];
+    to[DH_S] = dh * s0;
+    to[Z_S] = z * s0;
+    to[U_DS] = u * ds;
+    to[DH_U] = dh * u;
+    to[Z_U] = z * u;
+    to[S_DS] = s0 * ds;
+  };
+  float top[SUMS] = {};
+  for (int j = lane; j < blocks; j += 64) {
+    float x[SUMS];
+    products(j, x);
+#pragma unroll
+    for (int i = 0; i < SUMS; ++i) top[i] = fmaxf(top[i], x[i]);
+  }
+#pragma unroll
+  for (int i = 0; i < SUMS; ++i) top[i] = wave_max_all(top[i]);
+  if (tid < L) {
+    bs[tid] = f->b[tid];
+    betas[tid] = f->beta[tid];
+  }
+
+  // ---- staging: pieces of 16 bytes, through registers
+  constexpr int TOK_PIECES = 3 * PK * 256, TOK_PER = (TOK_PIECES + THREADS - 1) / THREADS, STA_PER = 2 * PK;  // of each state
+  u32x4 tok[TOK_PER], sta[2][STA_PER];
+  auto load = [&](int step) {
+#pragma unroll
+    for (int i = 0; i < TOK_PER; ++i) {
+      const int at = i * THREADS + tid;
+      if (at >= TOK_PIECES) continue;
+      const int mat = at / (PK * 256), rest = at - mat * (PK * 256), pl = rest >> 8, row = (rest >> 3) & 31, piece = rest & 7;
+      const int block = 2 * step + (row >> 4);
+      const f16_t* base = mat == 0 ? p.kept.dh : mat == 1 ? p.kept.z : p.kept.u;
+      tok[i] = *(const u32x4*)(base + kept_at(part, blocks, block, PK, L) + pl * 16 * L + (row & 15) * L + piece * 8);
+    }
+#pragma unroll
+    for (int mat = 0; mat < 2; ++mat)
+#pragma unroll
+      for (int i = 0; i < STA_PER; ++i) {
+        const int at = (i / PK) * THREADS + tid, pl = i % PK, row = at / (DKP / 8), piece = at % (DKP / 8);
+        const int block = 2 * step + (row >> 4);
+        sta[mat][i] = *(const u32x4*)((mat ? p.kept.ds : p.kept.s0) + kept_at(part, blocks, block, PK, DKP) + pl * 16 * DKP +
+                                      (row & 15) * DKP + piece * 8);
+      }
+  };
+  float ss_dot = 0.f;  // <dS, S_0>
+  auto store = [&](int step) {
+#pragma unroll
+    for (int i = 0; i < TOK_PER; ++i) {
+      const int at = i * THREADS + tid;
+      if (at >= TOK_PIECES) continue;
+      const int plane = at >> 8, row = (at >> 3) & 31, piece = at & 7;
+      *(u32x4*)(areaA + plane * TOK + row * 128 + ((piece ^ (row & 7)) << 4)) = tok[i];
+    }
+#pragma unroll
+    for (int mat = 0; mat < 2; ++mat)
+#pragma unroll
+      for (int i = 0; i < STA_PER; ++i) {
+        const int at = (i / PK) * THREADS + tid, pl = i % PK, row = at / (DKP / 8), piece = at % (DKP / 8);
+        *(u32x4*)(areaA + 3 * PK * TOK + (mat * PK + pl) * STA + row * (DKP * 2) + ((piece ^ (row & 7)) << 4)) = sta[mat][i];
+      }
+#pragma unroll
+    for (int i = 0; i < STA_PER; i += PK) {
+      const f16x8 a = __builtin_bit_cast(f16x8, sta[0][i]), d = __builtin_bit_cast(f16x8, sta[1][i]);
+      f16x8 al = {}, dl = {};
+      if constexpr (PK == 2) {
+        al = __builtin_bit_cast(f16x8, sta[0][i + 1]);
+        dl = __builtin_bit_cast(f16x8, sta[1][i + 1]);
+      }
+      float x = 0.f;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x = fmaf((float)a[e] + (float)al[e], (float)d[e] + (float)dl[e], x);
+      const int block = 2 * step + ((((i / PK) * THREADS + tid) / (DKP / 8)) >> 4);
+      ss_dot = fmaf(x, scales[3][block] * scales[4][block] / top[S_DS], ss_dot);
+    }
+  };
+  // operands, k = the 32 columns: tokens 16 mt .. of matrix mat (0 dH, 1 Z, 2 U); DQK's columns 16 t .. of S_0 (0), dS (1)
+  const int k0 = 8 * gq + (r >> 2);
+  auto tok_frag = [&](int mat, int pl, int mt) {
+    const char* base = areaA + (mat * PK + pl) * TOK + (mt & 1) * 8;
+    const int piece = 4 * (mt >> 1) + (r & 3);
+    return __builtin_bit_cast(f16x8, mfma::tr_pair(base + k0 * 128 + ((piece ^ (k0 & 7)) << 4),
+                                                   base + (k0 + 4) * 128 + ((piece ^ ((k0 + 4) & 7)) << 4)));
+  };
+  auto sta_frag = [&](int mat, int pl, int t) {
+    const char* base = areaA + 3 * PK * TOK + (mat * PK + pl) * STA + (t & 1) * 8;
+    const int piece = 4 * (t >> 1) + (r & 3);
+    return __builtin_bit_cast(f16x8, mfma::tr_pair(base + k0 * (DKP * 2) + ((piece ^ (k0 & 7)) << 4),
+                                                   base + (k0 + 4) * (DKP * 2) + ((piece ^ ((k0 + 4) & 7)) << 4)));
+  };
+
+  f32x4 g1[2][4], g2[2][4], g3[2][4];  // dH S_0^T, Z S_0^T, U dS^T, turned
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) g1[t][mt] = g2[t][mt] = g3[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+  // 10 tiles of dP and 10 of Z U^T: job, job + W, ..
+  constexpr int JOBS = (20 + W - 1) / W;
+  f32x4 jobs[JOBS];
+  int job_mat[JOBS], job_i[JOBS], job_j[JOBS];
+#pragma unroll
+  for (int x = 0; x < JOBS; ++x) {
+    jobs[x] = f32x4{0.f, 0.f, 0.f, 0.f};
+    const int job = min(x * W + wave, 19), tile = job % 10, i = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3;
+    job_mat[x] = job / 10;
+    job_i[x] = i;
+    job_j[x] = tile - i * (i + 1) / 2;
+  }
+  float zv[4 / (W < 4 ? W : 4)] = {};  // Z.V of tokens 16 mt + r
+  constexpr int MTS = 4 / (W < 4 ? W : 4);
+  const T* vrow = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
+  T* dvrow = (T*)p.dv + (int64_t)bh * p.S * p.DV;
+
+  const int steps = blocks / 2;
+  load(0);
+  for (int step = 0; step < steps; ++step) {
+    __syncthreads();
+    store(step);
+    __syncthreads();
+    if (step + 1 < steps) load(step + 1);
+    // a lane's 8 columns are of one block
+    float factor[SUMS];
+    products(2 * step + (gq >> 1), factor);
+    const float z_scale = scales[1][2 * step + (gq >> 1)];
+    _Float16 by[SUMS];
+#pragma unroll
+    for (int i = 0; i < SUMS; ++i) by[i] = (_Float16)(factor[i] / top[i]);
+    f16x8 s0[PK][2], ds[PK][2];
+#pragma unroll
+    for (int pl = 0; pl < PK; ++pl)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        s0[pl][t] = sta_frag(0, pl, 2 * wave + t);
+        ds[pl][t] = sta_frag(1, pl, 2 * wave + t);
+      }
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const f16x8 d = tok_frag(0, 0, mt) * by[DH_S], z = tok_frag(1, 0, mt) * by[Z_S], u = tok_frag(2, 0, mt) * by[U_DS];
+      f16x8 dl, zl, ul;
+      if constexpr (PK == 2) {
+        dl = tok_frag(0, 1, mt) * by[DH_S];
+        zl = tok_frag(1, 1, mt) * by[Z_S];
+        ul = tok_frag(2, 1, mt) * by[U_DS];
+      }
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        if constexpr (PK == 2) {
+          g1[t][mt] = mfma(s0[1][t], d, g1[t][mt]);
+          g1[t][mt] = mfma(s0[0][t], dl, g1[t][mt]);
+          g2[t][mt] = mfma(s0[1][t], z, g2[t][mt]);
+          g2[t][mt] = mfma(s0[0][t], zl, g2[t][mt]);
+          g3[t][mt] = mfma(ds[1][t], u, g3[t][mt]);
+          g3[t][mt] = mfma(ds[0][t], ul, g3[t][mt]);
+        }
+        g1[t][mt] = mfma(s0[0][t], d, g1[t][mt]);
+        g2[t][mt] = mfma(s0[0][t], z, g2[t][mt]);
+        g3[t][mt] = mfma(ds[0][t], u, g3[t][mt]);
+      }
+    }
+#pragma unroll
+    for (int x = 0; x < JOBS; ++x) {
+      const _Float16 share = job_mat[x] ? by[Z_U] : by[DH_U];
+      const f16x8 a = tok_frag(job_mat[x], 0, job_i[x]), u = tok_frag(2, 0, job_j[x]) * share;
+      if constexpr (PK == 2) {
+        jobs[x] = mfma(tok_frag(job_mat[x], 1, job_i[x]), u, jobs[x]);
+        jobs[x] = mfma(a, tok_frag(2, 1, job_j[x]) * share, jobs[x]);
+      }
+      jobs[x] = mfma(a, u, jobs[x]);
+    }
+    // dV = beta Z, and Z.V: a lane has 8 neighbours of a token
+    if (wave < 4) {
+#pragma unroll
+      for (int x = 0; x < MTS; ++x) {
+        const int mt = wave + x * W, t = t0 + 16 * mt + r, n = 32 * step + 8 * gq;
+        const f16x8 z = tok_frag(1, 0, mt);
+        f16x8 zl = {};
+        if constexpr (PK == 2) zl = tok_frag(1, 1, mt);
+        if (t < p.S) {
+          float zf[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) zf[e] = ((float)z[e] + (float)zl[e]) * z_scale;
+          const float beta = betas[16 * mt + r];
+          const T* from = vrow + t * p.vs[2] + n;
+          T* to = dvrow + (int64_t)t * p.DV + n;
+          struct alignas(16) Eight { T e[8]; };
+          if (p.wide_v && n + 8 <= p.DV) {
+            const Eight v = *(const Eight*)from;
+            Eight o;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+              zv[x] = fmaf(zf[e], to_f32(v.e[e]), zv[x]);
+              o.e[e] = from_f32<T>(beta * zf[e]);
+            }
+            *(Eight*)to = o;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e < p.DV) {
+                zv[x] = fmaf(zf[e], to_f32(from[e]), zv[x]);
+                to[e] = from_f32<T>(beta * zf[e]);
+              }
+          }
+        }
+      }
+    }
+  }
+  __syncthreads();
+
+  // ---- dP, dA to LDS; K beside
+#pragma unroll
+  for (int x = 0; x < JOBS; ++x) {
+    if (x * W + wave >= 20) continue;
+    float* to = job_mat[x] ? dam : dpm;
+    const float sc = job_mat[x] ? -top[Z_U] : top[DH_U];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) to[(16 * job_i[x] + 4 * gq + e) * GLD + 16 * job_j[x] + r] = jobs[x][e] * sc;
+  }
+  auto bring = [&](const char* img) {
+    for (int i = tid * 16; i < PK * PLANE; i += THREADS * 16) *(u32x4*)(areaA + i) = *(const u32x4*)(img + image * (PK * PLANE) + i);
+  };
+  bring(p.prep.k);
+  __syncthreads();
+  const float ksc = f->k, qsc = f->qs;
+#pragma unroll
+  for (int x = 0; x < (10 + W - 1) / W; ++x) {
+    const int tile = x * W + wave;
+    if (tile >= 10) continue;
+    const int i = tile < 1 ? 0 : tile < 3 ? 1 : tile < 6 ? 2 : 3, j = tile - i * (i + 1) / 2;
+    f32x4 y = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int s = 0; s < DKB; ++s) {
+      const f16x8 a = rows_frag<DKP>(areaA, i, s, r, gq), c = rows_frag<DKP>(areaA, j, s, r, gq);
+      if constexpr (PK == 2) {
+        y = mfma(rows_frag<DKP>(areaA + PLANE, i, s, r, gq), c, y);
+        y = mfma(a, rows_frag<DKP>(areaA + PLANE, j, s, r, gq), y);
+      }
+      y = mfma(a, c, y);
+    }
+#pragma unroll
+    for (int e = 0; e < 4; ++e) kkm[(16 * i + 4 * gq + e) * GLD + 16 * j + r] = y[e] * (ksc * ksc);
+  }
+  // sum over DQK's columns of this wave of K or Q times a turned accumulator, into red[slot][wave][token]
+  auto dots = [&](const f32x4 (&g)[2][4], int slot) {
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      float x = 0.f;
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const int tile = 2 * wave + t;
+        const char* at = areaA + piece_at<DKP>(16 * mt + r, 4 * (tile >> 1) + gq) + (tile & 1) * 8;
+        const f16x4 a = *(const f16x4*)at;
+        f16x4 al = {};
+        if constexpr (PK == 2) al = *(const f16x4*)(at + PLANE);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x = fmaf((float)a[e] + (float)al[e], g[t][mt][e], x);
+      }
+      x += __shfl_xor(x, 16, 64);
+      x += __shfl_xor(x, 32, 64);
+      if (gq == 0) red[(slot * 8 + wave) * L + 16 * mt + r] = x;
+    }
+  };
+  dots(g2, 0);  // k_i.(Z S_0^T)_i
+  dots(g3, 1);  // k_j.(U dS^T)_j
+  __syncthreads();
+
+  // ---- each pair of tokens: wave w has rows w, w + W, .., a lane a column
+  constexpr int ROWS = L / W;
+  float dps[ROWS], ee[ROWS], col = 0.f, mx[2] = {0.f, 0.f};
+  const f16_t* pf = p.prep.p + part * (2 * FRAG_PLANE);
+  const double bj = bs[lane];
+#pragma unroll
+  for (int x = 0; x < ROWS; ++x) {
+    const int i = x * W + wave, j = lane;
+    const bool on = j <= i, below = j < i;
+    const float dec = on ? exp_of(bs[i] - bj) : 0.f;
+    // P's operand order: lane (i % 16) + 16 of 4 columns, halves of 16 of each 32
+    const int at = (2 * (i >> 4) + (j >> 5)) * 512 + ((i & 15) + 16 * ((j >> 2) & 3)) * 8 + ((j >> 4) & 1) * 4 + (j & 3);
+    const float pv = on ? ((float)pf[at] + (float)pf[at + FRAG_PLANE]) * f->p : 0.f;
+    const float dp = on ? dpm[i * GLD + j] : 0.f, da = below ? dam[i * GLD + j] : 0.f, beta = betas[i];
+    const float nij = below ? dec * kkm[i * GLD + j] : 0.f;
+    const float bb = wave_sum_dpp(da * nij), pp = wave_sum_dpp(dp * pv);
+    if (lane == 63) {
+      rows[i] = pp;
+      rows[L + i] = bb;
+    }
+    col += fmaf(dp, pv, beta * (da * nij));
+    dps[x] = p.scale * dec * dp;
+    ee[x] = da * beta * dec;
+    mx[0] = fmaxf(mx[0], fabsf(dps[x]));
+    mx[1] = fmaxf(mx[1], fabsf(ee[x]));
+  }
+  red[(2 * 8 + wave) * L + lane] = col;
+  const float m0 = wave_max_all(mx[0]), m1 = wave_max_all(mx[1]), dot = wave_sum(ss_dot);
+  if (lane == 0) {
+    wred[wave] = m0;
+    wred[8 + wave] = m1;
+    wred[16 + wave] = dot;
+  }
+#pragma unroll
+  for (int x = 0; x < MTS; ++x) {
+    if (wave >= 4) continue;
+    float y = zv[x];
+    y += __shfl_xor(y, 16, 64);
+    y += __shfl_xor(y, 32, 64);
+    if (gq == 0) red[4 * 8 * L + 16 * (wave + x * W) + r] = y;
+  }
+  __syncthreads();  // dP and dA have been read: their place takes the operands
+  mx[0] = mx[1] = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    mx[0] = fmaxf(mx[0], wred[w]);
+    mx[1] = fmaxf(mx[1], wred[8 + w]);
+  }
+  const Pow2 sd = pow2_for(mx[0]), se = pow2_for(mx[1]);
+  // rows of 64 in f16, each 32 turned, piece p of row i at p ^ (i % 8): scale D o dP, its transpose, E + E^T
+  constexpr int MAT = L * L * 2;
+  auto put = [&](int mat, int i, int j, float x) {
+    char* at = areaB + mat * MAT + i * 128 + (((4 * (j >> 5) + ((j >> 2) & 3)) ^ (i & 7)) << 4) + ((j >> 4) & 1) * 8 + (j & 3) * 2;
+    const _Float16 hi = (_Float16)x;
+    *(_Float16*)at = hi;
+    if constexpr (PAIR) *(_Float16*)(at + 3 * MAT) = (_Float16)(x - (float)hi);
+  };
+#pragma unroll
+  for (int x = 0; x < ROWS; ++x) {
+    const int i = x * W + wave, j = lane;
+    const float dp = dps[x] * sd.up, e = ee[x] * se.up;
+    put(0, i, j, dp);
+    put(1, j, i, dp);
+    if (j <= i) put(2, i, j, e);
+    if (j < i) put(2, j, i, e);
+  }
+  __syncthreads();
+  auto pair_frag = [&](int mat, int pl, int mt, int s) {
+    const int i = 16 * mt + r;
+    return *(const f16x8*)(areaB + (pl * 3 + mat) * MAT + i * 128 + (((4 * s + gq) ^ (i & 7)) << 4));
+  };
+  // acc[t][mt] += (columns of the image in LDS)^T mat
+  auto add = [&](f32x4 (&acc)[2][4], int mat) {
+#pragma unroll
+    for (int s = 0; s < 2; ++s)
+#pragma unroll
+      for (int t = 0; t < 2; ++t) {
+        const f16x8 a = columns_frag<DKP>(areaA, 2 * wave + t, s, r, gq);
+        f16x8 al;
+        if constexpr (PK == 2) al = columns_frag<DKP>(areaA + PLANE, 2 * wave + t, s, r, gq);
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          const f16x8 x = pair_frag(mat, 0, mt, s);
+          if constexpr (PK == 2) acc[t][mt] = mfma(al, x, acc[t][mt]);
+          if constexpr (PAIR) acc[t][mt] = mfma(a, pair_frag(mat, 1, mt, s), acc[t][mt]);
+          acc[t][mt] = mfma(a, x, acc[t][mt]);
+        }
+      }
+  };
+  // dK's parts with the states, in units of K's scale and E's; then in those of Q's and D o dP's
+  f32x4 accq[2][4], acck[2][4];
+  const float ku = ksc * se.down, qu = qsc * sd.down;
+#pragma unroll
+  for (int mt = 0; mt < 4; ++mt) {
+    const float fo = f->out[16 * mt + r] / ksc * top[U_DS] / ku, fb = f->back[16 * mt + r] / ksc * top[Z_S] / ku;
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      acck[t][mt] = g3[t][mt] * fo - g2[t][mt] * fb;
+      accq[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+  }
+  add(accq, 0);
+  add(acck, 2);
+#pragma unroll
+  for (int t = 0; t < 2; ++t)
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) acck[t][mt] *= ku / qu;
+  __syncthreads();
+  bring(p.prep.q);
+  __syncthreads();
+  add(acck, 1);
+  dots(g1, 3);  // q_i.(dH S_0^T)_i
+  // ---- out
+  {
+    const bool own = p.group == 1;
+    auto write = [&](void* to, int tile, int token, f32x4 x) {
+      const int d = 16 * tile + 4 * gq;
+      auto as = [&](auto type) {
+        using O = decltype(type);
+        O* at = (O*)to + ((int64_t)bh * p.S + token) * p.DK + d;
+        struct alignas(4 * sizeof(O)) Four { O e[4]; } o;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) o.e[e] = from_f32<O>(x[e]);
+        if (p.DK % 4 == 0) {
+          if (d < p.DK) *(Four*)at = o;
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (d + e < p.DK) at[e] = o.e[e];
+        }
+      };
+      if (own) as(T{});
+      else as(float{});
+    };
+    const float fa = ksc * sd.down;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      const int token = t0 + 16 * mt + r;
+      const float fq = f->q[16 * mt + r] / qsc * top[DH_S];
+      if (token < p.S) {
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          write(p.dq, 2 * wave + t, token, g1[t][mt] * fq + accq[t][mt] * fa);
+          write(p.dk, 2 * wave + t, token, acck[t][mt] * qu);
+        }
+      }
+    }
+  }
+  __syncthreads();
+  // ---- the gates, a lane a token
+  if (wave != 0) return;
+  float kz = 0.f, ks = 0.f, qd = 0.f, cl = 0.f, dss = 0.f;
+#pragma unroll
+  for (int w = 0; w < W; ++w) {
+    kz += red[(0 * 8 + w) * L + lane];
+    ks += red[(1 * 8 + w) * L + lane];
+    cl += red[(2 * 8 + w) * L + lane];
+    qd += red[(3 * 8 + w) * L + lane];
+    dss += wred[16 + w];
+  }
+  kz *= ksc * top[Z_S];
+  const float sj = f->out[lane] * ks * top[U_DS];   // out has K's scale, which ks lacks
+  const float qi = f->q[lane] * qd * top[DH_S];
+  const float ci = f->in[lane] / ksc, beta = betas[lane];
+  const float dbeta = red[4 * 8 * L + lane] - ci * kz + rows[L + lane];
+  float db = rows[lane] + beta * rows[L + lane] - cl - sj + qi - beta * ci * kz;
+  const float sums = wave_sum(sj) + f->all * dss * top[S_DS];
+  if (lane == 63) db += sums;
+#pragma unroll
+  for (int o = 1; o < 64; o <<= 1) {
+    const float above = __shfl_down(db, o, 64);
+    if (lane + o < 64) db += above;
+  }
+  const int token = t0 + lane;
+  if (token >= p.S) return;
+  const int64_t at = (int64_t)bh * p.S + token;
+  auto gates = [&](auto type) {
+    using G = decltype(type);
+    ((G*)p.dg)[at] = from_f32<G>(db);
+    ((G*)p.dbeta)[at] = from_f32<G>(dbeta);
+  };
+  switch (p.gate_dtype) {
+    case XL_DTYPE_F32: gates(0.f); break;
+    case XL_DTYPE_BF16: gates(bf16_t{}); break;
+    default: gates(f16_t{}); break;
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ shared heads
+// to [B NHK, S DK] = sums over the group of from [B NHK, group, S DK]
+template <typename T>
+__global__ __launch_bounds__(256) void delta_join_kernel(const float* __restrict__ from, T* __restrict__ to, int group, int64_t per,
+                                                         int64_t count) {
+  for (int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x; i < count; i += (int64_t)gridDim.x * 256) {
+    const int64_t head = i / per;
+    const float* at = from + head * group * per + (i - head * per);
+    float x = 0.f;
+    for (int j = 0; j < group; ++j) x += at[j * per];
+    to[i] = from_f32<T>(x);
+  }
+}
+
+// ------------------------------------------------------------------------------------------------ host
+int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
+
+struct Layout {
+  int64_t prep, tok, sta, scales, partial;  // bytes of one of each
+  int blocks;
+  explicit Layout(const Shape& s) {
+    blocks = 2 * ((s.DV + 31) / 32);
+    prep = up256((int64_t)prep_bytes(s, true));
+    tok = up256(s.parts() * blocks * s.planes() * 16 * L * 2);
+    sta = up256(s.parts() * blocks * s.planes() * 16 * s.dkp() * 2);
+    scales = up256(s.parts() * blocks * 4);
+    partial = s.NH == s.NHK ? 0 : up256((int64_t)s.B * s.NH * s.S * s.DK * 4);
+  }
+  int64_t bytes() const { return prep + 3 * tok + 2 * sta + 5 * scales + 2 * partial; }
+};
+
+hipError_t launch(const void* kern, int64_t grid, int grid_y, int threads, int64_t lds, void* arg, hipStream_t st) {
+  void* args[] = {arg};
+  hipError_t e = lds > 65536 ? hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds) : hipSuccess;
+  return e != hipSuccess ? e : hipLaunchKernel(kern, dim3((unsigned)grid, grid_y), dim3(threads), args, (unsigned)lds, st);
+}
+
+template <typename T>
+int backward(const Shape& s, const void* v, const void* dh, const float* dc_last, void* dq, void* dk, void* dv, void* dg,
+             void* dbeta, float* dc0, const float* c0, const Prep& prep, const Kept& kept, float* dqp, float* dkp, hipStream_t st,
+             const char* who) {
+  const int group = s.NH / s.NHK, chunks = s.chunks();
+  TurnArgs turn{dh, kept, s.S, s.DV, chunks};
+  hipError_t e = launch((const void*)delta_turn_kernel<T>, s.parts(), (kept.blocks + 3) / 4, 256, 0, &turn, st);
+  if (e == hipSuccess)
+    if (const int rc = launch_scan(s, v, c0, nullptr, nullptr, prep, &kept, st, who)) return rc;
+  const int waves = kept.blocks >= 4 ? 4 : 2, slices = (kept.blocks + waves - 1) / waves;
+  BackArgs back{dc_last, dc0, prep, kept, s.NH, group, s.DK, s.DV, chunks, slices};
+  constexpr int S8 = is_f32<T>::value ? 1 : 2;
+  const int stages = s.dkp() == 256 ? S8 : 2;
+  const void* kern = s.dkp() == 64 ? (const void*)delta_back_kernel<T, 2, 2> : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2>
+                                                                                            : (const void*)delta_back_kernel<T, 8, S8>;
+  if (e == hipSuccess)
+    e = launch(kern, (int64_t)s.B * s.NH * slices, 1, 64 * waves, stages * 2 * s.image_bytes() + 2 * 2048, &back, st);
+  GradArgs grad{v, {s.vs[0], s.vs[1], s.vs[2]}, group == 1 ? dq : (void*)dqp, group == 1 ? dk : (void*)dkp, dv, dg, dbeta, prep, kept,
+                s.NH, group, s.S, s.DK, s.DV, chunks, s.dtype_gates, s.scale, false};
+  constexpr int VW = 16 / sizeof(T);
+  grad.wide_v = ((s.vs[0] | s.vs[1] | s.vs[2] | (int64_t)s.DV) % VW) == 0 && (((uintptr_t)v | (uintptr_t)dv) & 15) == 0;
+  const int lds = s.dkp() == 64 ? GradLds<T, 2>::BYTES : s.dkp() == 128 ? GradLds<T, 4>::BYTES : GradLds<T, 8>::BYTES;
+  kern = s.dkp() == 64 ? (const void*)delta_grad_kernel<T, 2> : s.dkp() == 128 ? (const void*)delta_grad_kernel<T, 4>
+                                                                              : (const void*)delta_grad_kernel<T, 8>;
+  if (e == hipSuccess) e = launch(kern, s.parts(), 1, s.dkp() * 2, lds, &grad, st);
+  if (e == hipSuccess && group > 1) {
+    const int64_t per = (int64_t)s.S * s.DK, count = (int64_t)s.B * s.NHK * per;
+    const unsigned grid = (unsigned)((count + 255) / 256 < 8192 ? (count + 255) / 256 : 8192);
+    delta_join_kernel<T><<<grid, 256, 0, st>>>(dqp, (T*)dq, group, per, count);
+    delta_join_kernel<T><<<grid, 256, 0, st>>>(dkp, (T*)dk, group, per, count);
+  }
+  if (e != hipSuccess) return set_error(XL_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
+  return check_launch(who);
+}
+
+}  // namespace
+}  // namespace delta
+}  // namespace xl
+
+extern "C" size_t xl_gated_delta_chunkwise_bwd_workspace_size(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv) {
+  using namespace xl;
+  delta::Shape s{B, NH, NHK, S, DQK, DV, {}, {}, {}, 1.f, dtype_qkv, dtype_qkv};
+  if (delta::check_shape("xl_gated_delta_chunkwise_bwd_workspace_size", s) != XL_OK) return 0;
+  return S == 0 ? 0 : (size_t)delta::Layout(s).bytes();
+}
+
+extern "C" int xl_gated_delta_chunkwise_bwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* g,
+                                            const void* beta, const float* c0, const void* dh, const float* dc_last, void* dq,
+                                            void* dk, void* dv, void* dg, void* dbeta, float* dc0, int B, int NH, int NHK,
+                                            int S, int DQK, int DV, float scale, int dtype_qkv, int dtype_gates,
+                                            void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace xl;
+  const char* who = "xl_gated_delta_chunkwise_bwd";
+  clear_error();
+  delta::Shape s{B, NH, NHK, S, DQK, DV, {}, {}, {}, scale, dtype_qkv, dtype_gates};
+  if (const int rc = delta::check_shape(who, s)) return rc;
+  if (S == 0) return set_error(XL_ERR_INVALID_ARG, "%s: no tokens", who);
+  if (!q || !k || !v || !g || !beta || !dh || !dq || !dk || !dv || !dg || !dbeta)
+    return set_error(XL_ERR_INVALID_ARG, "%s: null pointer", who);
+  if (((uintptr_t)dq | (uintptr_t)dk | (uintptr_t)dv) & 15)
+    return set_error(XL_ERR_INVALID_ARG, "%s: dq, dk and dv must be 16-byte aligned", who);
+  if (dc0 && dc0 == dc_last) return set_error(XL_ERR_INVALID_ARG, "%s: dc0 must not alias dc_last", who);
+  const delta::Layout lay(s);
+  if (!workspace || workspace_bytes < (size_t)lay.bytes() || ((uintptr_t)workspace & 255))
+    return set_error(XL_ERR_WORKSPACE, "%s: the workspace must be %zu bytes, 256-byte aligned", who, (size_t)lay.bytes());
+  if (const int rc = delta::set_strides(s, strides, who)) return rc;
+  const hipStream_t st = (hipStream_t)stream;
+  char* ws = (char*)workspace;
+  const delta::Prep prep = delta::prep_at(s, true, ws);
+  char* at = ws + lay.prep;
+  auto take = [&](int64_t bytes) {
+    char* x = at;
+    at += bytes;
+    return x;
+  };
+  delta::Kept kept{};
+  kept.u = (f16_t*)take(lay.tok);
+  kept.z = (f16_t*)take(lay.tok);
+  kept.dh = (f16_t*)take(lay.tok);
+  kept.s0 = (f16_t*)take(lay.sta);
+  kept.ds = (f16_t*)take(lay.sta);
+  for (float** x : {&kept.us, &kept.zs, &kept.dhs, &kept.s0s, &kept.dss}) *x = (float*)take(lay.scales);
+  kept.blocks = lay.blocks;
+  float *dqp = (float*)take(lay.partial), *dkp = (float*)take(lay.partial);
+  if (const int rc = delta::launch_prep(s, q, k, g, beta, prep, true, st, who)) return rc;
+  auto run = [&](auto t) {
+    return delta::backward<decltype(t)>(s, v, dh, dc_last, dq, dk, dv, dg, dbeta, dc0, c0, prep, kept, dqp, dkp, st, who);
+  };
+  if (dtype_qkv == XL_DTYPE_F32) return run(float{});
+  if (dtype_qkv == XL_DTYPE_BF16) return run(bf16_t{});
+  return run(f16_t{});
+}

@@ -18,14 +18,16 @@ struct ScanArgs {
   void* h;
   float* c_last;
   Prep prep;
+  Kept kept;
   int NH, group, S, DK, DV, chunks, slices;
 };
 
 // PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32)
-template <typename T, int DKB, int STAGES>
+// STATES: U and the state before each chunk are kept for the backward, and nothing else is written
+template <typename T, int DKB, int STAGES, bool STATES>
 __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
-  constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
-  constexpr bool PAIR = !std::is_same_v<T, bf16_t>;
+  constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = (STATES ? 1 : 2) * IMG;
+  constexpr bool PAIR = STATES ? PK == 2 : !std::is_same_v<T, bf16_t>;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int r = lane & 15, gq = lane >> 4;
@@ -43,7 +45,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
     const char* qi = p.prep.q + (image0 + chunk) * (int64_t)IMG;
     for (int i = wave; i < IMG / 1024; i += waves) {
       to_lds(lds_at + stage * STAGE + i * 1024, i * 1024 + lane * 16, ki);
-      to_lds(lds_at + stage * STAGE + IMG + i * 1024, i * 1024 + lane * 16, qi);
+      if constexpr (!STATES) to_lds(lds_at + stage * STAGE + IMG + i * 1024, i * 1024 + lane * 16, qi);
     }
   };
   auto fetch_factors = [&](int chunk) {
@@ -99,7 +101,9 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
   fetch_factors(0);
   load_v(0);
   load_t(0);
-  load_p(0);
+  if constexpr (!STATES) load_p(0);
+  const int block = n0 / 16;
+  const bool kept = STATES && block < p.kept.blocks;
   for (int c = 0; c < p.chunks; ++c) {
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     __builtin_amdgcn_s_barrier();
@@ -120,7 +124,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(st[t][e]));
     const float most = wave_max_all(m);
-    const Pow2 ss = pow2_for(most);
+    const Pow2 ss = pow2_for(most, 14, STATES ? KEPT : 100);
     f32x4 ks[4], hs[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) ks[mt] = hs[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -128,17 +132,25 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
     for (int s = 0; s < DKB; ++s) {
       f16x8 hi, lo;
       split8<true>(st[2 * s], st[2 * s + 1], ss.up, hi, lo);
+      if constexpr (STATES) {
+        if (kept) {
+          f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, PK, DKP) + r * DKP + s * 32 + gq * 8;
+          *(f16x8*)to = hi;
+          if constexpr (PK == 2) *(f16x8*)(to + 16 * DKP) = lo;
+        }
+      }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        const f16x8 k = rows_frag<DKP>(ki, mt, s, r, gq), q = rows_frag<DKP>(qi, mt, s, r, gq);
-        if constexpr (PK == 2) {
-          ks[mt] = mfma(rows_frag<DKP>(ki + PLANE, mt, s, r, gq), hi, ks[mt]);
-          hs[mt] = mfma(hi, rows_frag<DKP>(qi + PLANE, mt, s, r, gq), hs[mt]);
-        }
+        const f16x8 k = rows_frag<DKP>(ki, mt, s, r, gq);
+        if constexpr (PK == 2) ks[mt] = mfma(rows_frag<DKP>(ki + PLANE, mt, s, r, gq), hi, ks[mt]);
         ks[mt] = mfma(k, lo, ks[mt]);
-        if constexpr (PAIR) hs[mt] = mfma(lo, q, hs[mt]);
         ks[mt] = mfma(k, hi, ks[mt]);
-        hs[mt] = mfma(hi, q, hs[mt]);
+        if constexpr (!STATES) {
+          const f16x8 q = rows_frag<DKP>(qi, mt, s, r, gq);
+          if constexpr (PK == 2) hs[mt] = mfma(hi, rows_frag<DKP>(qi + PLANE, mt, s, r, gq), hs[mt]);
+          if constexpr (PAIR) hs[mt] = mfma(lo, q, hs[mt]);
+          hs[mt] = mfma(hi, q, hs[mt]);
+        }
       }
     }
     // ---- R
@@ -179,12 +191,25 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(u[mt][e]));
     }
     const float most_u = wave_max_all(m);
-    const Pow2 us = pow2_for(most_u);
-    // ---- H
-    {
-      f16x8 uh[2], ul[2];
+    const Pow2 us = pow2_for(most_u, 14, STATES ? KEPT : 100);
+    f16x8 uh[2], ul[2];
 #pragma unroll
-      for (int s = 0; s < 2; ++s) split8<PAIR>(u[2 * s], u[2 * s + 1], us.up, uh[s], ul[s]);
+    for (int s = 0; s < 2; ++s) split8<PAIR>(u[2 * s], u[2 * s + 1], us.up, uh[s], ul[s]);
+    if constexpr (STATES) {
+      if (kept) {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          f16_t* to = p.kept.u + kept_at(part0 + c, p.kept.blocks, block, PK, L) + r * L + s * 32 + gq * 8;
+          *(f16x8*)to = uh[s];
+          if constexpr (PK == 2) *(f16x8*)(to + 16 * L) = ul[s];
+        }
+        if (lane == 0) {
+          const int64_t at = (part0 + c) * p.kept.blocks + block;
+          p.kept.us[at] = us.down;
+          p.kept.s0s[at] = ss.down;
+        }
+      }
+    } else {  // ---- H
       f32x4 x[4];
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) x[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -263,28 +288,34 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
   }
 }
 
-template <typename T>
+template <typename T, bool STATES>
 const void* pick(int dkp, int& stages) {
   stages = 2;
-  if (dkp == 64) return (const void*)delta_scan_kernel<T, 2, 2>;
-  if (dkp == 128) return (const void*)delta_scan_kernel<T, 4, 2>;
-  if constexpr (is_f32<T>::value) {
-    stages = 1;
-    return (const void*)delta_scan_kernel<T, 8, 1>;
-  } else {
-    return (const void*)delta_scan_kernel<T, 8, 2>;
-  }
+  if (dkp == 64) return (const void*)delta_scan_kernel<T, 2, 2, STATES>;
+  if (dkp == 128) return (const void*)delta_scan_kernel<T, 4, 2, STATES>;
+  constexpr int S8 = is_f32<T>::value && !STATES ? 1 : 2;  // two chunks of K and Q pairs do not fit
+  stages = S8;
+  return (const void*)delta_scan_kernel<T, 8, S8, STATES>;
 }
 
-int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* c_last, const Prep& prep, hipStream_t st,
-                const char* who) {
-  ScanArgs a{v, {s.vs[0], s.vs[1], s.vs[2]}, c0, h, c_last, prep, s.NH, s.NH / s.NHK, s.S, s.DK, s.DV, s.chunks(), 0};
-  int stages;
-  const void* kern = s.dtype == XL_DTYPE_F32 ? pick<float>(s.dkp(), stages)
-                     : s.dtype == XL_DTYPE_BF16 ? pick<bf16_t>(s.dkp(), stages) : pick<f16_t>(s.dkp(), stages);
-  const int blocks = (s.DV + 15) / 16, waves = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
+}  // namespace
+
+int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* c_last, const Prep& prep, const Kept* kept,
+                hipStream_t st, const char* who) {
+  ScanArgs a{v, {s.vs[0], s.vs[1], s.vs[2]}, c0, h, c_last, prep, {}, s.NH, s.NH / s.NHK, s.S, s.DK, s.DV, s.chunks(), 0};
+  if (kept) a.kept = *kept;
+  int stages = 0;
+  const void* kern = nullptr;
+  auto choose = [&](auto t) {
+    using T = decltype(t);
+    kern = kept ? pick<T, true>(s.dkp(), stages) : pick<T, false>(s.dkp(), stages);
+  };
+  if (s.dtype == XL_DTYPE_F32) choose(float{});
+  else if (s.dtype == XL_DTYPE_BF16) choose(bf16_t{});
+  else choose(f16_t{});
+  const int blocks = kept ? kept->blocks : (s.DV + 15) / 16, waves = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
   a.slices = (blocks + waves - 1) / waves;
-  const int64_t lds = stages * 2 * s.image_bytes() + 2 * 1024;
+  const int64_t lds = stages * (kept ? 1 : 2) * s.image_bytes() + 2 * 1024;
   void* args[] = {&a};
   hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
   if (e == hipSuccess)
@@ -293,7 +324,6 @@ int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* 
   return check_launch(who);
 }
 
-}  // namespace
 }  // namespace delta
 }  // namespace xl
 
@@ -325,5 +355,5 @@ extern "C" int xl_gated_delta_chunkwise_fwd(const void* q, const void* k, const 
   const hipStream_t st = (hipStream_t)stream;
   const delta::Prep prep = delta::prep_at(s, false, (char*)workspace);
   if (const int rc = delta::launch_prep(s, q, k, g, beta, prep, false, st, who)) return rc;
-  return delta::launch_scan(s, v, c0, h, c_last, prep, st, who);
+  return delta::launch_scan(s, v, c0, h, c_last, prep, nullptr, st, who);
 }

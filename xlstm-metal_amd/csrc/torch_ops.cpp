@@ -937,6 +937,93 @@ std::tuple<Tensor, Tensor> gated_delta_chunkwise(const Tensor& q_, const Tensor&
   return {h, cl};
 }
 
+std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_delta_chunkwise_bwd(
+    const Tensor& q_, const Tensor& k_, const Tensor& v_, const Tensor& g_, const Tensor& beta_, const OptTensor& c0_,
+    const Tensor& dh_, const OptTensor& dc_last, double scale) {
+  const char* what = "gated_delta_chunkwise_bwd";
+  Gpu gpu(what, {&q_, &k_, &v_, &g_, &beta_, opt(c0_), &dh_, opt(dc_last)});
+  const DeltaShape s = delta_shapes(q_, k_, v_, g_, beta_, opt(c0_), true, what);
+  const DeltaSizes n(s, what);
+  XL_CHECK(dh_.sizes() == v_.sizes(), what, "dh must be (B, NH, S, DHV), got ", dh_.sizes());
+  XL_CHECK(!opt(dc_last) || dc_last->sizes() == at::IntArrayRef({s.B, s.NH, s.DQK, s.DV}), what,
+           "dc_last must be (B, NH, DHQK, DHV)");
+  int64_t st[9];
+  const Tensor q = delta_rows(q_, st), k = delta_rows(k_, st + 3), v = delta_rows(v_, st + 6);
+  const Tensor g = g_.contiguous(), beta = beta_.contiguous(), c0 = f32(c0_), dcl = f32(dc_last);
+  const Tensor dh = (dh_.scalar_type() == q.scalar_type() ? dh_ : dh_.to(q.scalar_type())).contiguous();
+  auto dense = [](const Tensor& t) { return at::empty(t.sizes(), t.options()); };
+  const Tensor dq = dense(q), dk = dense(k), dv = dense(v), dg = dense(g), dbeta = dense(beta);
+  const Tensor dc0 = c0.defined() ? dense(c0) : at::empty({0}, f32_on(q));
+  if (s.S == 0) {
+    if (c0.defined()) {
+      if (dcl.defined()) dc0.copy_(dcl);
+      else dc0.zero_();
+    }
+    return {dq, dk, dv, dg, dbeta, dc0};
+  }
+  const int dt = dtype_code(q, what);
+  const size_t ws_bytes = xl_gated_delta_chunkwise_bwd_workspace_size(n.B, n.NH, n.NHK, n.S, n.DQK, n.DV, dt);
+  const Tensor ws = at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte));
+  check_rc(xl_gated_delta_chunkwise_bwd(ptr(q), ptr(k), ptr(v), st, ptr(g), ptr(beta), ptr<float>(c0), ptr(dh),
+                                        ptr<float>(dcl), ptr(dq), ptr(dk), ptr(dv), ptr(dg), ptr(dbeta),
+                                        c0.defined() ? ptr<float>(dc0) : nullptr, n.B, n.NH, n.NHK, n.S, n.DQK, n.DV,
+                                        (float)scale, dt, dtype_code(g, what), ptr(ws), ws_bytes, gpu.st),
+           what);
+  return {dq, dk, dv, dg, dbeta, dc0};
+}
+
+using CallDelta = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                             const OptTensor&, double, bool);
+using DeltaBwd = SixTensors(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&, const OptTensor&,
+                            const Tensor&, const OptTensor&, double);
+
+std::tuple<Tensor, Tensor> call_delta(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g, const Tensor& beta,
+                                      const OptTensor& c0, double scale, bool ret) {
+  static const auto op =
+      c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::gated_delta_chunkwise", "").typed<CallDelta>();
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(q, k, v, g, beta, c0, scale, ret);
+}
+
+struct DeltaFn : public torch::autograd::Function<DeltaFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& q, const Tensor& k,
+                                                const Tensor& v, const Tensor& g, const Tensor& beta, const OptTensor& c0,
+                                                double scale, bool ret) {
+    ctx->save_for_backward({q, k, v, g, beta, c0.value_or(Tensor())});
+    ctx->saved_data["scale"] = scale;
+    ctx->saved_data["ret"] = ret;
+    ctx->set_materialize_grads(false);
+    auto [h, c] = call_delta(q, k, v, g, beta, c0, scale, ret);
+    return {h, c};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    static const auto bwd =
+        c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::gated_delta_chunkwise_bwd", "").typed<DeltaBwd>();
+    const auto saved = ctx->get_saved_variables();
+    auto given = [](const Tensor& t) { return t.defined() ? OptTensor(t) : OptTensor(); };
+    const Tensor none, &v = saved[2], &c0 = saved[5];
+    const OptTensor dcl = ctx->saved_data["ret"].toBool() ? given(grads[1]) : OptTensor();
+    if (!grads[0].defined() && !dcl) return {none, none, none, none, none, none, none, none};
+    const Tensor dh = grads[0].defined() ? grads[0] : at::zeros_symint(v.sym_sizes(), v.options());
+    auto [dq, dk, dv, dg, dbeta, dc0] = bwd.call(saved[0], saved[1], v, saved[3], saved[4], given(c0), dh, dcl,
+                                                 ctx->saved_data["scale"].toDouble());
+    return {dq, dk, dv, dg, dbeta, c0.defined() ? dc0.to(c0.scalar_type()) : none, none, none};
+  }
+};
+
+std::tuple<Tensor, Tensor> gated_delta_chunkwise_autograd(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& g,
+                                                          const Tensor& beta, const OptTensor& c0, double scale, bool ret) {
+  bool any = false;
+  const bool recorded = c10::GradMode::is_enabled();
+  for (const Tensor* t : {&q, &k, &v, &g, &beta, opt(c0)})
+    any = any || (t && t->defined() && ((recorded && t->requires_grad()) || t->_fw_grad(0).defined()));
+  if (!any) return call_delta(q, k, v, g, beta, c0, scale, ret);
+  const auto r = DeltaFn::apply(q, k, v, g, beta, c0, scale, ret);
+  return {r[0], r[1]};
+}
+
 // The operators that write an argument, under autograd's bookkeeping, on fake tensors as on real ones.  What they
 // write is updated outside autograd, whatever it requires (a leaf too; its own history stays), a backward through
 // the outputs raises, and the written tensors' version counters move (inference tensors have none).
@@ -1056,6 +1143,7 @@ TORCH_LIBRARY_IMPL(xlstm_hip, CUDA, m) {
   m.impl("layer_norm_bwd", layer_norm_bwd);
   m.impl("newton_schulz", newton_schulz);
   m.impl("gated_delta_chunkwise", gated_delta_chunkwise);
+  m.impl("gated_delta_chunkwise_bwd", gated_delta_chunkwise_bwd);
   m.impl("gated_delta_recurrent", gated_delta_recurrent);
   m.impl("gated_delta_step", gated_delta_step);
   m.impl("gated_delta_step_", gated_delta_step_);
@@ -1067,12 +1155,13 @@ TORCH_LIBRARY_IMPL(xlstm_hip, CUDA, m) {
   for (const char* op : {"soft_cap", "mlstm_step", "mlstm_chunkwise_bwd", "mlstm_sequence", "slstm_step",              \
                          "slstm_sequence", "causal_conv1d", "group_norm", "mh_rmsnorm_gate", "gate_proj_softcap",      \
                          "gate_proj2_softcap", "lm_head_softcap", "rms_norm", "silu_mul", "layer_norm_bwd",             \
-                         "newton_schulz", "gated_delta_recurrent", "gated_delta_step"})                                                                             \
+                         "newton_schulz", "gated_delta_chunkwise_bwd", "gated_delta_recurrent", "gated_delta_step"})                                                                             \
     m.impl(op, kernel());
 TORCH_LIBRARY_IMPL(xlstm_hip, Autograd, m) {
   if (!abi_matches()) return;
   m.impl("mlstm_chunkwise", mlstm_chunkwise_autograd);
   m.impl("layer_norm", layer_norm_autograd);
+  m.impl("gated_delta_chunkwise", gated_delta_chunkwise_autograd);
   m.impl("mlstm_step_", mlstm_step__autograd);
   m.impl("gated_delta_step_", gated_delta_step__autograd);
   m.impl("add_rmsnorm", add_rmsnorm_autograd);

@@ -4,8 +4,8 @@ Schemas and fake (meta) kernels are declared here, so the ops are traceable; the
 (csrc/torch_ops.cpp, lib/libxlstm_torch.so): they validate shapes and dtypes, allocate the outputs with
 torch's caching allocator (the library itself never allocates), pass raw pointers and the current HIP
 stream through the C-ABI and return without synchronising.  There is no CPU path: CPU tensors raise.
-``mlstm_chunkwise`` differentiates through the reference's custom backward and ``layer_norm`` through its own; a
-backward through any other op raises.
+``mlstm_chunkwise`` differentiates through the reference's custom backward, ``layer_norm`` and ``gated_delta_chunkwise``
+through their own; a backward through any other op raises.
 """
 
 from __future__ import annotations
@@ -81,6 +81,9 @@ _SCHEMAS = {
     # (h, the last state, or an empty placeholder); q, k [B, NHK, S, DQK], v [B, NH, S, DV], gates [B, NH, S]
     "gated_delta_chunkwise": ("(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? c0, float scale, bool "
                              "return_last_states) -> (Tensor, Tensor)"),
+    # dq, dk, dv, dg, dbeta and dc0 (float32; an empty placeholder without an initial state)
+    "gated_delta_chunkwise_bwd": ("(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? c0, Tensor dh, Tensor? "
+                                 "dc_last, float scale) -> (Tensor, Tensor, Tensor, Tensor, Tensor, Tensor)"),
     "gated_delta_recurrent": ("(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? c0, float scale, bool "
                              "return_last_states) -> (Tensor, Tensor)"),
     # one token: no S axis; the in-place form returns h
@@ -261,6 +264,12 @@ def _gated_delta(q, k, v, g, beta, c0, scale, return_last_states):
 
 _fake("gated_delta_chunkwise")(_gated_delta)
 _fake("gated_delta_recurrent")(_gated_delta)
+
+
+@_fake("gated_delta_chunkwise_bwd")
+def _(q, k, v, g, beta, c0, dh, dc_last, scale):
+    return tuple(t.new_empty(t.shape) for t in (q, k, v, g, beta)) + (
+        q.new_empty(c0.shape if c0 is not None else _EMPTY_SHAPE, dtype=torch.float32),)
 
 
 @_fake("gated_delta_step")
