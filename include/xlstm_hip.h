@@ -449,6 +449,22 @@ int xl_gated_delta_chunkwise_bwd(const void* q, const void* k, const void* v, co
                                  int DQK, int DV, float scale, int dtype_qkv, int dtype_gates, void* workspace,
                                  size_t workspace_bytes, void* stream);
 
+/*
+ * Gated linear unit: h = act(x w_gate^T) * (x w_up^T), x [T, D], weights [F, D], h [T, F], bf16 or f16 (float32:
+ * XL_ERR_UNSUPPORTED); act 0: SiLU, 1: GELU (by erf).  Products, activation and their product in float32, rounded once.  a and
+ * u: both products, float32 [T, keep_pitch] (keep_pitch at least F, a multiple of 8), for the backward, or both NULL.  Pointers 16-byte
+ * aligned.  T = 0: nothing.  Workspace (xl_gated_linear_workspace_size bytes, 256-byte aligned): none where D is a multiple of 8.
+ *
+ * Its gradients from dh [T, F], of x, and of both weights together; dx or both dw may be NULL.  T at least 1.
+ */
+size_t xl_gated_linear_workspace_size(int64_t T, int D, int F, int backward, int dtype);
+int xl_gated_linear_fwd(const void* x, const void* w_gate, const void* w_up, void* h, float* a, float* u,
+                        int64_t keep_pitch, int64_t T, int D, int F, int act, int dtype, void* workspace,
+                        size_t workspace_bytes, void* stream);
+int xl_gated_linear_bwd(const void* dh, const void* x, const void* w_gate, const void* w_up, const float* a,
+                        const float* u, int64_t keep_pitch, void* dx, void* dw_gate, void* dw_up, int64_t T, int D,
+                        int F, int act, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -1024,6 +1024,116 @@ std::tuple<Tensor, Tensor> gated_delta_chunkwise_autograd(const Tensor& q, const
   return {r[0], r[1]};
 }
 
+// ------------------------------------------------------------------ gated linear unit
+struct GluShape {
+  int64_t T;
+  int D, F, dtype;
+};
+GluShape glu_shape(const Tensor& x, const Tensor& wg, const Tensor& wu, const char* what) {
+  XL_CHECK(x.dim() >= 1, what, "x must have at least one axis");
+  XL_CHECK(wg.dim() == 2 && wg.size(1) == x.size(-1), what, "weight_gate must be (F, ", x.size(-1), "), got ", wg.sizes());
+  XL_CHECK(wu.sizes() == wg.sizes(), what, "weight_gate and weight_up must have the same shape, got ", wg.sizes(), " and ",
+           wu.sizes());
+  XL_CHECK(x.scalar_type() == wg.scalar_type() && wg.scalar_type() == wu.scalar_type(), what, "x and the weights must share a dtype");
+  XL_CHECK(wg.size(0) > 0 && wg.size(1) > 0, what, "weights must not be empty, got ", wg.sizes());
+  return {x.numel() / x.size(-1), i32(wg.size(1), what), i32(wg.size(0), what), dtype_code(x, what)};
+}
+
+std::tuple<Tensor, Tensor> gated_linear(const Tensor& x_, const Tensor& wg_, const Tensor& wu_, int64_t act, bool keep) {
+  const char* what = "gated_linear_unit";
+  Gpu gpu(what, {&x_, &wg_, &wu_});
+  const GluShape s = glu_shape(x_, wg_, wu_, what);
+  const Tensor x = prep(x_), wg = prep(wg_), wu = prep(wu_);
+  auto sizes = x_.sizes().vec();
+  sizes.back() = s.F;
+  const int64_t pitch = (s.F + 7) / 8 * 8;
+  const Tensor h = at::empty(sizes, x.options()), kept = at::empty({keep ? 2 : 0, s.T, pitch}, f32_on(x));
+  const size_t ws_bytes = xl_gated_linear_workspace_size(s.T, s.D, s.F, 0, s.dtype);
+  const Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, x.options().dtype(at::kByte)) : Tensor();
+  float* a = keep && s.T ? ptr<float>(kept) : nullptr;
+  check_rc(xl_gated_linear_fwd(ptr(x), ptr(wg), ptr(wu), ptr(h), a, a ? a + s.T * pitch : nullptr, pitch, s.T, s.D, s.F,
+                               i32(act, what), s.dtype, ptr(ws), ws_bytes, gpu.st),
+           what);
+  return {h, kept};
+}
+
+std::tuple<Tensor, Tensor, Tensor> gated_linear_bwd(const Tensor& dh_, const Tensor& x_, const Tensor& wg_, const Tensor& wu_,
+                                                    const Tensor& kept, int64_t act, std::array<bool, 3> mask) {
+  const char* what = "gated_linear_bwd";
+  Gpu gpu(what, {&dh_, &x_, &wg_, &wu_, &kept});
+  const GluShape s = glu_shape(x_, wg_, wu_, what);
+  const int64_t pitch = (s.F + 7) / 8 * 8;
+  XL_CHECK(dh_.dim() == x_.dim() && dh_.numel() == s.T * s.F && dh_.size(-1) == s.F, what, "dh must have the output's shape, got ",
+           dh_.sizes());
+  XL_CHECK(kept.sizes() == at::IntArrayRef({2, s.T, pitch}) && kept.scalar_type() == at::kFloat && kept.is_contiguous(), what,
+           "the kept values must be the forward's, got ", kept.sizes());
+  const Tensor x = prep(x_), wg = prep(wg_), wu = prep(wu_);
+  const Tensor dh = prep(dh_.scalar_type() == x.scalar_type() ? dh_ : dh_.to(x.scalar_type()));
+  const bool weights = mask[1] || mask[2];
+  auto made = [&](bool want, const Tensor& t) { return at::empty(want ? t.sizes() : at::IntArrayRef({0}), t.options()); };
+  const Tensor dx = made(mask[0], x), dwg = made(weights, wg), dwu = made(weights, wu);
+  if (s.T == 0) {
+    if (weights) {
+      dwg.zero_();
+      dwu.zero_();
+    }
+    return {dx, dwg, dwu};
+  }
+  const size_t ws_bytes = xl_gated_linear_workspace_size(s.T, s.D, s.F, 1, s.dtype);
+  const Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, x.options().dtype(at::kByte)) : Tensor();
+  const float* a = ptr<float>(kept);
+  check_rc(xl_gated_linear_bwd(ptr(dh), ptr(x), ptr(wg), ptr(wu), a, a + s.T * pitch, pitch, mask[0] ? ptr(dx) : nullptr,
+                               weights ? ptr(dwg) : nullptr, weights ? ptr(dwu) : nullptr, s.T, s.D, s.F, i32(act, what), s.dtype,
+                               ptr(ws), ws_bytes, gpu.st),
+           what);
+  return {dx, dwg, dwu};
+}
+
+using CallGlu = std::tuple<Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, c10::SymInt, bool);
+using GluBwd = std::tuple<Tensor, Tensor, Tensor>(const Tensor&, const Tensor&, const Tensor&, const Tensor&, const Tensor&,
+                                                  c10::SymInt, std::array<bool, 3>);
+
+std::tuple<Tensor, Tensor> call_glu(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::SymInt act, bool keep) {
+  static const auto op = c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::gated_linear", "").typed<CallGlu>();
+  at::AutoDispatchBelowADInplaceOrView below;
+  return op.call(x, wg, wu, act, keep);
+}
+
+// Gradients of h; the values kept for them are not differentiable.
+struct GluFn : public torch::autograd::Function<GluFn> {
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const Tensor& x, const Tensor& wg,
+                                                const Tensor& wu, c10::SymInt act, bool keep) {
+    auto [h, kept] = call_glu(x, wg, wu, act, true);
+    ctx->save_for_backward({x, wg, wu, kept});
+    ctx->saved_data["act"] = act;
+    ctx->mark_non_differentiable({kept});
+    ctx->set_materialize_grads(false);
+    return {h, kept};
+  }
+
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx,
+                                                 torch::autograd::variable_list grads) {
+    static const auto bwd =
+        c10::Dispatcher::singleton().findSchemaOrThrow("xlstm_hip::gated_linear_bwd", "").typed<GluBwd>();
+    const Tensor none;
+    if (!grads[0].defined()) return {none, none, none, none, none};
+    const auto saved = ctx->get_saved_variables();
+    std::array<bool, 3> mask = {};
+    for (size_t i = 0; i < 3; ++i) mask[i] = ctx->needs_input_grad(i);
+    auto [dx, dwg, dwu] = bwd.call(grads[0], saved[0], saved[1], saved[2], saved[3], ctx->saved_data["act"].toSymInt(), mask);
+    return {mask[0] ? dx : none, mask[1] ? dwg : none, mask[2] ? dwu : none, none, none};
+  }
+};
+
+std::tuple<Tensor, Tensor> gated_linear_autograd(const Tensor& x, const Tensor& wg, const Tensor& wu, c10::SymInt act, bool keep) {
+  bool any = false;
+  const bool recorded = c10::GradMode::is_enabled();
+  for (const Tensor* t : {&x, &wg, &wu}) any = any || (recorded && t->requires_grad()) || t->_fw_grad(0).defined();
+  if (!any) return call_glu(x, wg, wu, act, keep);
+  const auto r = GluFn::apply(x, wg, wu, act, keep);
+  return {r[0], r[1]};
+}
+
 // The operators that write an argument, under autograd's bookkeeping, on fake tensors as on real ones.  What they
 // write is updated outside autograd, whatever it requires (a leaf too; its own history stays), a backward through
 // the outputs raises, and the written tensors' version counters move (inference tensors have none).
@@ -1144,24 +1254,27 @@ TORCH_LIBRARY_IMPL(xlstm_hip, CUDA, m) {
   m.impl("newton_schulz", newton_schulz);
   m.impl("gated_delta_chunkwise", gated_delta_chunkwise);
   m.impl("gated_delta_chunkwise_bwd", gated_delta_chunkwise_bwd);
+  m.impl("gated_linear", gated_linear);
+  m.impl("gated_linear_bwd", gated_linear_bwd);
   m.impl("gated_delta_recurrent", gated_delta_recurrent);
   m.impl("gated_delta_step", gated_delta_step);
   m.impl("gated_delta_step_", gated_delta_step_);
 }
 
-// The chunkwise forward and the layer norm differentiate through their own backward; every other operator is
-// forward-only and a backward through it raises.
+// The chunkwise forwards, the layer norm and the gated linear unit differentiate through their own backward; every other
+// operator is forward-only and a backward through it raises.
 #define XL_FORWARD_ONLY(m, kernel)                                                                                     \
   for (const char* op : {"soft_cap", "mlstm_step", "mlstm_chunkwise_bwd", "mlstm_sequence", "slstm_step",              \
                          "slstm_sequence", "causal_conv1d", "group_norm", "mh_rmsnorm_gate", "gate_proj_softcap",      \
                          "gate_proj2_softcap", "lm_head_softcap", "rms_norm", "silu_mul", "layer_norm_bwd",             \
-                         "newton_schulz", "gated_delta_chunkwise_bwd", "gated_delta_recurrent", "gated_delta_step"})                                                                             \
+                         "newton_schulz", "gated_delta_chunkwise_bwd", "gated_delta_recurrent", "gated_delta_step", "gated_linear_bwd"})                                                                             \
     m.impl(op, kernel());
 TORCH_LIBRARY_IMPL(xlstm_hip, Autograd, m) {
   if (!abi_matches()) return;
   m.impl("mlstm_chunkwise", mlstm_chunkwise_autograd);
   m.impl("layer_norm", layer_norm_autograd);
   m.impl("gated_delta_chunkwise", gated_delta_chunkwise_autograd);
+  m.impl("gated_linear", gated_linear_autograd);
   m.impl("mlstm_step_", mlstm_step__autograd);
   m.impl("gated_delta_step_", gated_delta_step__autograd);
   m.impl("add_rmsnorm", add_rmsnorm_autograd);

@@ -18,6 +18,7 @@ from .backend import (
 )
 from .chunkwise import mlstm_chunkwise, mlstm_chunkwise__native_autograd, mlstm_chunkwise__native_custbw
 from .delta import gated_delta_chunkwise, gated_delta_recurrent, gated_delta_step, gated_delta_step_
+from .gated_linear import gated_linear_unit
 from .ops import chunkwise_algorithm
 from .mlstm_layers import (
     MultiHeadLayerNorm, MultiHeadRMSNorm, gate_proj_softcap, mh_rmsnorm_gate, mLSTMOutputCell, mLSTMProjectionCell,
@@ -51,6 +52,7 @@ __all__ = [
     "mh_rmsnorm_gate", "MultiHeadRMSNorm", "MultiHeadLayerNorm", "mLSTMOutputCell", "gate_proj_softcap",
     "mLSTMProjectionCell", "layer_norm", "multi_head_layer_norm", "newton_schulz",
     "gated_delta_chunkwise", "gated_delta_recurrent", "gated_delta_step", "gated_delta_step_",
+    "gated_linear_unit",
     "get_mlstm_kernel", "get_mlstm_step_kernel", "get_mlstm_sequence_kernel", "available_kernels",
     "wrap_chunkwise__arbitrary_sequence_length", "wrap_chunkwise__pad_zeros", "mLSTMBackendConfig",
     "mLSTMBackend", "load_library", "LIB_PATH",

@@ -68,6 +68,9 @@ SIGNATURES = {
     "xl_gated_delta_chunkwise_bwd_workspace_size": (_sz, [_i] * 7),
     "xl_gated_delta_chunkwise_bwd": (_i, [_vp] * 3 + [ctypes.POINTER(_i64)] + [_vp] * 2 + [_fp, _vp, _fp] + [_vp] * 5 + [_fp]
                                      + [_i] * 6 + [_f] + [_i] * 2 + [_vp, _sz, _vp]),
+    "xl_gated_linear_workspace_size": (_sz, [_i64] + [_i] * 4),
+    "xl_gated_linear_fwd": (_i, [_vp] * 4 + [_fp] * 2 + [_i64] * 2 + [_i] * 4 + [_vp, _sz, _vp]),
+    "xl_gated_linear_bwd": (_i, [_vp] * 4 + [_fp] * 2 + [_i64] + [_vp] * 3 + [_i64] + [_i] * 4 + [_vp, _sz, _vp]),
     "xl_newton_schulz": (_i, [_vp] * 2 + [_i64, _i, _i, ctypes.POINTER(_f), _i, _f, _i, _vp, _sz, _vp]),
 }
 

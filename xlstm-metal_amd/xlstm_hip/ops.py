@@ -4,8 +4,8 @@ Schemas and fake (meta) kernels are declared here, so the ops are traceable; the
 (csrc/torch_ops.cpp, lib/libxlstm_torch.so): they validate shapes and dtypes, allocate the outputs with
 torch's caching allocator (the library itself never allocates), pass raw pointers and the current HIP
 stream through the C-ABI and return without synchronising.  There is no CPU path: CPU tensors raise.
-``mlstm_chunkwise`` differentiates through the reference's custom backward, ``layer_norm`` and ``gated_delta_chunkwise``
-through their own; a backward through any other op raises.
+``mlstm_chunkwise`` differentiates through the reference's custom backward, ``layer_norm``, ``gated_delta_chunkwise``
+and ``gated_linear`` through their own; a backward through any other op raises.
 """
 
 from __future__ import annotations
@@ -22,7 +22,7 @@ __all__ = [
     "soft_cap_op", "mlstm_step_op", "mlstm_step_inplace_op", "mlstm_chunkwise_op", "mlstm_chunkwise_bwd_op", "mlstm_sequence_op",
     "slstm_step_op", "slstm_sequence_op", "causal_conv1d_op", "group_norm_op", "mh_rmsnorm_gate_op",
     "gate_proj_softcap_op", "gate_proj2_softcap_op", "lm_head_softcap_op", "rms_norm_op", "add_rmsnorm_op", "silu_mul_op",
-    "layer_norm_op", "newton_schulz_op", "gated_delta_chunkwise_op", "gated_delta_recurrent_op", "gated_delta_step_op",
+    "layer_norm_op", "newton_schulz_op", "gated_linear_op", "gated_delta_chunkwise_op", "gated_delta_recurrent_op", "gated_delta_step_op",
     "gated_delta_step_inplace_op",
     "chunkwise_workspace_bytes", "chunkwise_algorithm",
 ]
@@ -78,6 +78,11 @@ _SCHEMAS = {
                       "output_mask) -> (Tensor, Tensor, Tensor)"),
     # coefficients: a, b, c of each step
     "newton_schulz": ("(Tensor x, float[] coefficients, float eps) -> Tensor"),
+    # (act(x Wg^T) * (x Wu^T), the two products float32 [2, tokens, F rounded up to 8] where keep, for the backward); act: GLU_ACTS
+    "gated_linear": ("(Tensor x, Tensor weight_gate, Tensor weight_up, SymInt act, bool keep) -> (Tensor, Tensor)"),
+    # (dx, dweight_gate, dweight_up); what the mask leaves out is an empty placeholder (both weights' are formed together)
+    "gated_linear_bwd": ("(Tensor dh, Tensor x, Tensor weight_gate, Tensor weight_up, Tensor kept, SymInt act, bool[3] "
+                        "output_mask) -> (Tensor, Tensor, Tensor)"),
     # (h, the last state, or an empty placeholder); q, k [B, NHK, S, DQK], v [B, NH, S, DV], gates [B, NH, S]
     "gated_delta_chunkwise": ("(Tensor q, Tensor k, Tensor v, Tensor g, Tensor beta, Tensor? c0, float scale, bool "
                              "return_last_states) -> (Tensor, Tensor)"),
@@ -255,6 +260,19 @@ def _(x, coefficients, eps):
     return torch.empty_like(x, memory_format=torch.contiguous_format)
 
 
+@_fake("gated_linear")
+def _(x, weight_gate, weight_up, act, keep):
+    F = weight_gate.shape[0]
+    return (x.new_empty(tuple(x.shape[:-1]) + (F,)),
+            x.new_empty((2 if keep else 0, x.numel() // x.shape[-1], (F + 7) // 8 * 8), dtype=torch.float32))
+
+
+@_fake("gated_linear_bwd")
+def _(dh, x, weight_gate, weight_up, kept, act, output_mask):
+    wanted = (output_mask[0],) + (output_mask[1] or output_mask[2],) * 2
+    return tuple(t.new_empty(t.shape if w else _EMPTY_SHAPE) for t, w in zip((x, weight_gate, weight_up), wanted))
+
+
 def _gated_delta(q, k, v, g, beta, c0, scale, return_last_states):
     B, _, S, DQK = q.shape
     _, NH, _, DV = v.shape
@@ -299,12 +317,14 @@ add_rmsnorm_op = torch.ops.xlstm_hip.add_rmsnorm.default
 silu_mul_op = torch.ops.xlstm_hip.silu_mul.default
 layer_norm_op = torch.ops.xlstm_hip.layer_norm.default
 newton_schulz_op = torch.ops.xlstm_hip.newton_schulz.default
+gated_linear_op = torch.ops.xlstm_hip.gated_linear.default
 gated_delta_chunkwise_op = torch.ops.xlstm_hip.gated_delta_chunkwise.default
 gated_delta_recurrent_op = torch.ops.xlstm_hip.gated_delta_recurrent.default
 gated_delta_step_op = torch.ops.xlstm_hip.gated_delta_step.default
 gated_delta_step_inplace_op = torch.ops.xlstm_hip.gated_delta_step_.default
 
 CONV_ACTS = {None: 0, "silu": 1}
+GLU_ACTS = {"silu": 0, "gelu": 1}
 # csrc/torch_ops.cpp's own (0 where no kernel can run): the most rows of lm_head_softcap and the LDS of its
 # staging, and the input and forget gate of the tokens that the backward pads a ragged sequence with
 LM_HEAD_MAX_ROWS, LM_HEAD_MAX_LDS, _PAD_I, _PAD_F = (
