@@ -17,8 +17,8 @@ sigma(o), then out_proj).  The sLSTM layer is sLSTMProjectionCell (conv1d + SiLU
 kernels, z Linear) -> the sLSTM sequence kernel over the prompt and the step kernel per token
 -> sLSTMOutputCell (``group_norm_kernel``, out_proj).  The lm_head and the logit soft-cap are
 one kernel of this library (``lm_head_softcap``; ``fused_lm_head = False`` runs torch's Linear and
-then the soft_cap kernel instead).  Projections, FFN and embedding are torch (hipBLASLt GEMMs), the
-blocks' norms with the residual before them and the SwiGLU product one pass each; every mLSTM/sLSTM kernel is this library's.
+then the soft_cap kernel instead).  Projections, FFN and embedding are torch (hipBLASLt GEMMs; with ``StackConfig.fused_ffn``
+the FFN's first half is ``gated_linear_unit``), the blocks' norms with the residual before them and the SwiGLU product one pass each; every mLSTM/sLSTM kernel is this library's.
 
 Weights are N(0, init_std) in the model dtype (there is no checkpoint); the mLSTM forget-gate
 bias starts at +3 and the input-gate bias at 0, so the gates sit where a trained model keeps
@@ -42,6 +42,7 @@ from torch.autograd import forward_ad
 
 from .backend import (get_mlstm_kernel, get_mlstm_sequence_kernel, get_mlstm_step_kernel,
                       wrap_chunkwise__arbitrary_sequence_length)
+from .gated_linear import gated_linear_unit
 from .mlstm_layers import gate_pair_softcap, gate_proj_softcap, mLSTMOutputCell, mLSTMProjectionCell
 from .ops import add_rmsnorm_op, rms_norm_op, silu_mul_op
 from .recurrent import mlstm_recurrent_step_
@@ -76,6 +77,7 @@ class StackConfig:
     eps: float = 1e-6
     init_std: float = 0.02
     dtype: torch.dtype = torch.bfloat16
+    fused_ffn: bool = False       # the FFN's two projections, SiLU and product by gated_linear_unit (bf16, f16)
 
     @property
     def qk_head_dim(self) -> int:
@@ -146,13 +148,18 @@ class _RMSNorm(nn.Module):
 
 
 class _FFN(nn.Module):
-    def __init__(self, d: int, hidden: int) -> None:
+    """``fused``: gate, up, SiLU and product in one kernel, rounded once (three roundings otherwise); it differentiates."""
+
+    def __init__(self, d: int, hidden: int, fused: bool = False) -> None:
         super().__init__()
+        self.fused = fused
         self.proj_up = nn.Linear(d, hidden, bias=False)
         self.proj_up_gate = nn.Linear(d, hidden, bias=False)
         self.proj_down = nn.Linear(hidden, d, bias=False)
 
     def forward(self, x: Tensor) -> Tensor:
+        if self.fused and x.device.type == "cuda" and x.dtype in (torch.bfloat16, torch.float16):
+            return self.proj_down(gated_linear_unit(x, self.proj_up_gate.weight, self.proj_up.weight))
         gate, up = self.proj_up_gate(x), self.proj_up(x)
         if _one_pass(gate, up):
             return self.proj_down(silu_mul_op(gate, up))
@@ -183,7 +190,7 @@ class _mLSTMBlock(nn.Module):
         self.proj = mLSTMProjectionCell(d, NH, cfg.qk_head_dim, cfg.v_head_dim, gate_soft_cap=cfg.gate_soft_cap)
         self.out = mLSTMOutputCell(d, NH, cfg.v_head_dim, eps=cfg.eps)
         self.norm_ffn = _RMSNorm(d, cfg.norm_eps)
-        self.ffn = _FFN(d, cfg.ffn_dim)
+        self.ffn = _FFN(d, cfg.ffn_dim, cfg.fused_ffn)
         self._chunkwise = get_mlstm_kernel("chunkwise--native_autograd")
         self._sequence = get_mlstm_sequence_kernel("native_sequence__native")
         self._step = get_mlstm_step_kernel("native")
@@ -223,7 +230,7 @@ class _sLSTMBlock(nn.Module):
                                         gate_soft_cap=cfg.gate_soft_cap)
         self.out = sLSTMOutputCell(d, NH, self.H, eps=cfg.eps)
         self.norm_ffn = _RMSNorm(d, cfg.norm_eps)
-        self.ffn = _FFN(d, cfg.ffn_dim)
+        self.ffn = _FFN(d, cfg.ffn_dim, cfg.fused_ffn)
 
     def prefill(self, x: Tensor):
         B, S, d = x.shape
