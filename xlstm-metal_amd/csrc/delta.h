@@ -104,6 +104,23 @@ __device__ __forceinline__ void split8(const float (&x)[8], float scale, f16x8& 
   hi = __builtin_bit_cast(f16x8, h);
   lo = __builtin_bit_cast(f16x8, l);
 }
+// 16 bytes at a uniform base and a lane's 32-bit offset
+__device__ __forceinline__ f16x8 load16(const void* base, uint32_t at) { return *(const f16x8*)((const char*)base + at); }
+// 4 neighbours, rounded
+template <typename T>
+struct alignas(4 * sizeof(T)) Four {
+  T e[4];
+};
+template <typename T>
+__device__ __forceinline__ Four<T> rounded4(f32x4 v) {
+  if constexpr (is_f32<T>::value) {
+    return __builtin_bit_cast(Four<T>, v);
+  } else {
+    using pair = std::conditional_t<std::is_same_v<T, f16_t>, xl_f16x2, xl_bf16x2>;
+    return __builtin_bit_cast(Four<T>, (u32x2{__builtin_bit_cast(uint32_t, __builtin_convertvector((xl_f32x2{v[0], v[1]}), pair)),
+                                             __builtin_bit_cast(uint32_t, __builtin_convertvector((xl_f32x2{v[2], v[3]}), pair))}));
+  }
+}
 template <bool PAIR>
 __device__ __forceinline__ void split8(f32x4 a, f32x4 b, float scale, f16x8& hi, f16x8& lo) {
   const float x[8] = {a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
@@ -116,7 +133,31 @@ __device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const void
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 
-// Images of K and Q: [plane][64 tokens][DKP] f16, each 32 columns turned, the 16-byte piece p of token i at p ^ (i % 8).
+// The scans keep the state at a power-of-two scale: its planes are taken without a multiplication.  With max(c_L |S|, |w|)
+// below 2^(STATE + 1) and K's values below 2 the next state, c_L S + K^T w over 64 tokens, is below 129 2^(STATE + 1) = 33024.
+constexpr int STATE = 7;
+
+// max of |x| over a wave's piece of the state
+template <int N>
+__device__ __forceinline__ float state_max(const f32x4 (&st)[N]) {
+  float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], fabsf(st[t][e]));
+  return wave_max_all(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
+}
+template <int N>
+__device__ __forceinline__ float abs_max(const f32x4 (&x)[N]) {
+  float m[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+  for (int t = 0; t < N; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], fabsf(x[t][e]));
+  return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+
+// Images of K and Q: [plane][64 tokens][DKP] f16, the largest value in [1, 2), each 32 columns turned, the 16-byte piece p of token i at p ^ (i % 8).
 template <int DKP>
 __device__ __forceinline__ int piece_at(int token, int p) {
   return token * (DKP * 2) + ((p ^ (token & 7)) << 4);
@@ -138,16 +179,16 @@ __device__ __forceinline__ f16x8 columns_frag(const char* img, int t, int s, int
 constexpr int LOWER = 6;
 __device__ __host__ constexpr int lower_mt(int i) { return i < 2 ? i : 2 + (i - 2) / 2; }
 __device__ __host__ constexpr int lower_s(int i) { return i < 2 ? 0 : (i - 2) % 2; }
-__device__ __forceinline__ void load_lower(const f16_t* from, int lane, f16x8 (&to)[LOWER]) {
+__device__ __forceinline__ void load_lower(const f16_t* from, uint32_t lane, f16x8 (&to)[LOWER]) {
 #pragma unroll
-  for (int i = 0; i < LOWER; ++i) to[i] = *((const f16x8*)from + (2 * lower_mt(i) + lower_s(i)) * 64 + lane);
+  for (int i = 0; i < LOWER; ++i) to[i] = load16(from + (2 * lower_mt(i) + lower_s(i)) * 512, lane * 16);
 }
 // of a transposed one: row tiles 0 and 1 have both halves of k, 2 and 3 the second
 __device__ __host__ constexpr int upper_mt(int i) { return i < 4 ? i / 2 : i - 2; }
 __device__ __host__ constexpr int upper_s(int i) { return i < 4 ? i % 2 : 1; }
-__device__ __forceinline__ void load_upper(const f16_t* from, int lane, f16x8 (&to)[LOWER]) {
+__device__ __forceinline__ void load_upper(const f16_t* from, uint32_t lane, f16x8 (&to)[LOWER]) {
 #pragma unroll
-  for (int i = 0; i < LOWER; ++i) to[i] = *((const f16x8*)from + (2 * upper_mt(i) + upper_s(i)) * 64 + lane);
+  for (int i = 0; i < LOWER; ++i) to[i] = load16(from + (2 * upper_mt(i) + upper_s(i)) * 512, lane * 16);
 }
 
 // What the backward keeps of a scan for the chunks' gradients, by 16 columns n (a wave's): tokens x n, [plane][16 n][64 tokens,
@@ -183,6 +224,13 @@ struct Prep {
   f16_t *tt, *pt;    // T^T, P^T (2 planes)
   Factors* f;
 };
+
+// Waves of a scan's workgroups: up to 4 share a chunk's images, fewer where that leaves CUs without one.
+inline int scan_waves(int64_t heads, int blocks) {
+  int waves = 4;
+  while (waves > 1 && (heads * ((blocks + waves - 1) / waves) < 256 || waves / 2 >= blocks)) waves /= 2;
+  return waves;
+}
 
 int check_shape(const char* who, const Shape& s);
 // q, k, v strides from the caller's nine or of contiguous tensors

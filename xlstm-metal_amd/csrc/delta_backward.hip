@@ -860,7 +860,7 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
   hipError_t e = launch((const void*)delta_turn_kernel<T>, s.parts(), (kept.blocks + 3) / 4, 256, 0, &turn, st);
   if (e == hipSuccess)
     if (const int rc = launch_scan(s, v, c0, nullptr, nullptr, prep, &kept, st, who)) return rc;
-  const int waves = kept.blocks >= 4 ? 4 : 2, slices = (kept.blocks + waves - 1) / waves;
+  const int waves = scan_waves((int64_t)s.B * s.NH, kept.blocks), slices = (kept.blocks + waves - 1) / waves;
   BackArgs back{dc_last, dc0, prep, kept, s.NH, group, s.DK, s.DV, chunks, slices};
   constexpr int S8 = is_f32<T>::value ? 1 : 2;
   const int stages = s.dkp() == 256 ? S8 : 2;

@@ -51,32 +51,34 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
   auto fetch_factors = [&](int chunk) {
     if (wave == 0) to_lds(lds_at + STAGES * STAGE + (chunk & 1) * 1024, lane * 16, p.prep.f + part0 + chunk);
   };
-  // Rows 16 mt + 4 gq + e of column n.  Past the last token the last one is read again, for zeros; past the last column the
-  // last one: those columns are computed and not written.
+  // Rows 16 mt + 4 gq + e of column n.  Past the last token the last one is read again (its beta is 0 there: T has zeros in its
+  // column), past the last column the last one: those columns are computed and not written.
   const int nc = n < p.DV ? n : p.DV - 1, row_step = (int)p.vs[2];
   T vn[4][4];
+  uint32_t v_at[4][4];
+#pragma unroll
+  for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v_at[mt][e] = (uint32_t)((16 * mt + 4 * gq + e) * row_step + nc) * (uint32_t)sizeof(T);
   auto load_v = [&](int chunk) {
     const int t0 = chunk * L;
-    const T* base = v + t0 * p.vs[2];
-    if (t0 + L <= p.S) {
-      const uint32_t at = (uint32_t)(4 * gq * row_step + nc) * sizeof(T);
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) vn[mt][e] = *(const T*)((const char*)(base + (16 * mt + e) * p.vs[2]) + at);
-    } else {
+    if (t0 + L > p.S) {  // the last chunk, once
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int t = 16 * mt + 4 * gq + e;
-          const T x = base[(t0 + t < p.S ? t : 0) * p.vs[2] + nc];
-          vn[mt][e] = t0 + t < p.S ? x : from_f32<T>(0.f);
+          const int t = 16 * mt + 4 * gq + e, last = p.S - 1 - t0;
+          v_at[mt][e] = (uint32_t)((t < last ? t : last) * row_step + nc) * (uint32_t)sizeof(T);
         }
     }
+    const char* base = (const char*)(v + t0 * p.vs[2]);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vn[mt][e] = *(const T*)(base + v_at[mt][e]);
   };
 
-  f32x4 st[2 * DKB];
+  f32x4 st[2 * DKB];  // the state times 1 / st_down
 #pragma unroll
   for (int t = 0; t < 2 * DKB; ++t)
 #pragma unroll
@@ -84,8 +86,17 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       const int d = 16 * t + 4 * gq + e;
       st[t][e] = p.c0 && d < p.DK ? p.c0[((int64_t)bh * p.DK + d) * p.DV + nc] : 0.f;
     }
+  constexpr int LIMIT = STATES ? KEPT : 100;
+  float st_down;
+  {
+    const Pow2 sc = pow2_for(state_max(st), STATE, LIMIT);
+    st_down = sc.down;
+#pragma unroll
+    for (int t = 0; t < 2 * DKB; ++t) st[t] *= sc.up;
+  }
 
-  // T and P of the next chunk wait in registers, K, Q and the factors in LDS
+  // T, P and V of the next chunk wait in registers, K, Q and the factors in LDS.  What is loaded past the last chunk is that one's
+  // again: as many loads are under way after every chunk.
   f16x8 th[LOWER], tl[LOWER], ph[LOWER], pl[PAIR ? LOWER : 1];
   auto load_t = [&](int chunk) {
     const f16_t* from = p.prep.t + (part0 + chunk) * (2 * FRAG_PLANE);
@@ -97,6 +108,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
     load_lower(from, lane, ph);
     if constexpr (PAIR) load_lower(from + FRAG_PLANE, lane, pl);
   };
+  constexpr int LATER = 16 + 2 * LOWER;  // loads after a chunk's fetch, at least
   fetch(0, 0);
   fetch_factors(0);
   load_v(0);
@@ -104,34 +116,53 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
   if constexpr (!STATES) load_p(0);
   const int block = n0 / 16;
   const bool kept = STATES && block < p.kept.blocks;
+  const uint32_t h_at = (uint32_t)(r * p.DV + 4 * gq) * sizeof(T);
   for (int c = 0; c < p.chunks; ++c) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STAGES == 2 ? LATER : 0) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int stage = STAGES == 2 ? c & 1 : 0;
-    const bool more = c + 1 < p.chunks;
-    if (more) {
-      if (STAGES == 2) fetch(c + 1, stage ^ 1);
-      fetch_factors(c + 1);
+    const int stage = STAGES == 2 ? c & 1 : 0, next = c + 1 < p.chunks ? c + 1 : c;
+    if (next != c) {
+      if (STAGES == 2) fetch(next, stage ^ 1);
+      fetch_factors(next);
     }
     const char *ki = lds + stage * STAGE, *qi = ki + IMG;
     const Factors* f = (const Factors*)(lds + STAGES * STAGE + (c & 1) * 1024);
 
-    // ---- K S, and Q S turned
-    float m = 0.f;
+    // ---- K S, and Q S turned: the operands of the next 32 of DQK are read under the products of these
+    struct Rows {
+      f16x8 k[PK][4], q[STATES ? 1 : PK][4];
+    };
+    auto read = [&](Rows& to, int s) {
 #pragma unroll
-    for (int t = 0; t < 2 * DKB; ++t)
+      for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(st[t][e]));
-    const float most = wave_max_all(m);
-    const Pow2 ss = pow2_for(most, 14, STATES ? KEPT : 100);
+        for (int pl = 0; pl < PK; ++pl) {
+          to.k[pl][mt] = rows_frag<DKP>(ki + pl * PLANE, mt, s, r, gq);
+          if constexpr (!STATES) to.q[pl][mt] = rows_frag<DKP>(qi + pl * PLANE, mt, s, r, gq);
+        }
+    };
     f32x4 ks[4], hs[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) ks[mt] = hs[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    Rows rows[2];
+    read(rows[0], 0);
+    f32x4 in[4], out[4];
+    float fq[4];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      in[mt] = *(const f32x4*)&f->in[16 * mt + 4 * gq] * st_down;
+      out[mt] = *(const f32x4*)&f->out[16 * mt + 4 * gq];
+      if constexpr (!STATES) fq[mt] = f->q[16 * mt + r] * st_down;
+    }
+    const float keep = f->all, t_scale = f->t, p_scale = f->p;
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
+      if (s + 1 < DKB) read(rows[(s + 1) & 1], s + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      const Rows& x = rows[s & 1];
       f16x8 hi, lo;
-      split8<true>(st[2 * s], st[2 * s + 1], ss.up, hi, lo);
+      split8<true>(st[2 * s], st[2 * s + 1], 1.f, hi, lo);
       if constexpr (STATES) {
         if (kept) {
           f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, PK, DKP) + r * DKP + s * 32 + gq * 8;
@@ -141,60 +172,69 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       }
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        const f16x8 k = rows_frag<DKP>(ki, mt, s, r, gq);
-        if constexpr (PK == 2) ks[mt] = mfma(rows_frag<DKP>(ki + PLANE, mt, s, r, gq), hi, ks[mt]);
-        ks[mt] = mfma(k, lo, ks[mt]);
-        ks[mt] = mfma(k, hi, ks[mt]);
+        if constexpr (PK == 2) ks[mt] = mfma(x.k[1][mt], hi, ks[mt]);
+        ks[mt] = mfma(x.k[0][mt], hi, ks[mt]);
         if constexpr (!STATES) {
-          const f16x8 q = rows_frag<DKP>(qi, mt, s, r, gq);
-          if constexpr (PK == 2) hs[mt] = mfma(hi, rows_frag<DKP>(qi + PLANE, mt, s, r, gq), hs[mt]);
-          if constexpr (PAIR) hs[mt] = mfma(lo, q, hs[mt]);
-          hs[mt] = mfma(hi, q, hs[mt]);
+          if constexpr (PK == 2) hs[mt] = mfma(hi, x.q[1][mt], hs[mt]);
+          hs[mt] = mfma(hi, x.q[0][mt], hs[mt]);
         }
       }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        ks[mt] = mfma(x.k[0][mt], lo, ks[mt]);
+        if constexpr (PAIR && !STATES) hs[mt] = mfma(lo, x.q[0][mt], hs[mt]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
     }
     // ---- R
     f32x4 rr[4];
-    m = 0.f;
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const f32x4 in = *(const f32x4*)&f->in[16 * mt + 4 * gq];
+    for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        rr[mt][e] = to_f32(vn[mt][e]) - in[e] * (ks[mt][e] * ss.down);
-        m = fmaxf(m, fabsf(rr[mt][e]));
-      }
-    }
-    if (more) load_v(c + 1);
-    const Pow2 rs = pow2_for(wave_max_all(m));
+      for (int e = 0; e < 4; ++e) rr[mt][e] = fmaf(-in[mt][e], ks[mt][e], to_f32(vn[mt][e]));
+    load_v(next);
+    const Pow2 rs = pow2_for(wave_max_all(abs_max(rr)));
     f16x8 rh[2], rl[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) split8<true>(rr[2 * s], rr[2 * s + 1], rs.up, rh[s], rl[s]);
     // ---- U
     f32x4 u[4];
-    const float back = f->t * rs.down;
+    const float back = t_scale * rs.down;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) u[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < LOWER; ++i) {
-      f32x4& x = u[lower_mt(i)];
-      x = mfma(tl[i], rh[lower_s(i)], x);
-      x = mfma(th[i], rl[lower_s(i)], x);
-      x = mfma(th[i], rh[lower_s(i)], x);
-    }
-    if (more) load_t(c + 1);
-    m = 0.f;
+    for (int i = 0; i < LOWER; ++i) u[lower_mt(i)] = mfma(th[i], rh[lower_s(i)], u[lower_mt(i)]);
+#pragma unroll
+    for (int i = 0; i < LOWER; ++i) u[lower_mt(i)] = mfma(tl[i], rh[lower_s(i)], u[lower_mt(i)]);
+#pragma unroll
+    for (int i = 0; i < LOWER; ++i) u[lower_mt(i)] = mfma(th[i], rl[lower_s(i)], u[lower_mt(i)]);
+    load_t(next);
+    const float most = state_max(st) * st_down;  // not needed before w
+    // the first operands of the state's product
+    f16x8 columns[2][PK][2];
+    auto read_columns = [&](int t) {
+#pragma unroll
+      for (int pl = 0; pl < PK; ++pl)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) columns[t & 1][pl][s] = columns_frag<DKP>(ki + pl * PLANE, t, s, r, gq);
+    };
+    read_columns(0);
+    read_columns(1);
+    f32x4 w[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       u[mt] *= back;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(u[mt][e]));
+      w[mt] = u[mt] * out[mt];
     }
-    const float most_u = wave_max_all(m);
-    const Pow2 us = pow2_for(most_u, 14, STATES ? KEPT : 100);
-    f16x8 uh[2], ul[2];
+    const Pow2 us = pow2_for(wave_max_all(abs_max(u)), 14, LIMIT);
+    const Pow2 ws = pow2_for(fmaxf(wave_max_all(abs_max(w)), most * keep), STATE, LIMIT);
+    f16x8 uh[2], ul[2], wh[2], wl[2];
 #pragma unroll
-    for (int s = 0; s < 2; ++s) split8<PAIR>(u[2 * s], u[2 * s + 1], us.up, uh[s], ul[s]);
+    for (int s = 0; s < 2; ++s) {
+      split8<PAIR>(u[2 * s], u[2 * s + 1], us.up, uh[s], ul[s]);
+      split8<true>(w[2 * s], w[2 * s + 1], ws.up, wh[s], wl[s]);
+    }
+    f32x4 x[4];
     if constexpr (STATES) {
       if (kept) {
 #pragma unroll
@@ -206,75 +246,62 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
         if (lane == 0) {
           const int64_t at = (part0 + c) * p.kept.blocks + block;
           p.kept.us[at] = us.down;
-          p.kept.s0s[at] = ss.down;
+          p.kept.s0s[at] = st_down;
         }
       }
-    } else {  // ---- H
-      f32x4 x[4];
+    } else {  // ---- P U
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) x[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int i = 0; i < LOWER; ++i) {
         f32x4& y = x[lower_mt(i)];
+        y = mfma(uh[lower_s(i)], ph[i], y);
         if constexpr (PAIR) {
           y = mfma(ul[lower_s(i)], ph[i], y);
           y = mfma(uh[lower_s(i)], pl[i], y);
         }
-        y = mfma(uh[lower_s(i)], ph[i], y);
       }
-      if (more) load_p(c + 1);
-      const float pu = f->p * us.down;
-#pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        const int t = c * L + 16 * mt + r;
-        const float fq = f->q[16 * mt + r] * ss.down;
-        if (t < p.S) {
-          T* to = ho + (int64_t)t * p.DV + n0 + 4 * gq;
-          struct alignas(4 * sizeof(T)) Four { T e[4]; } out;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) out.e[e] = from_f32<T>(fmaf(x[mt][e], pu, hs[mt][e] * fq));
-          if (p.DV % 4 == 0) {
-            if (n0 + 4 * gq < p.DV) *(Four*)to = out;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-              if (n0 + 4 * gq + e < p.DV) to[e] = out.e[e];
-          }
-        }
-      }
+      load_p(next);
     }
     // ---- the state
-    const float keep = f->all;
-    m = most * keep;
-    f32x4 w[4];
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      w[mt] = u[mt] * *(const f32x4*)&f->out[16 * mt + 4 * gq];
-#pragma unroll
-      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(w[mt][e]));
-    }
-    const Pow2 ws = pow2_for(wave_max_all(m));
-    f16x8 wh[2], wl[2];
-#pragma unroll
-    for (int s = 0; s < 2; ++s) split8<true>(w[2 * s], w[2 * s + 1], ws.up, wh[s], wl[s]);
-    const float up = keep * ws.up;
+    const float up = keep * st_down * ws.up;
+    st_down = ws.down;
 #pragma unroll
     for (int t = 0; t < 2 * DKB; ++t) {
-      f32x4 x = st[t] * up;
+      f32x4 y = st[t] * up;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const f16x8 k = columns_frag<DKP>(ki, t, s, r, gq);
-        if constexpr (PK == 2) x = mfma(columns_frag<DKP>(ki + PLANE, t, s, r, gq), wh[s], x);
-        x = mfma(k, wl[s], x);
-        x = mfma(k, wh[s], x);
+        if constexpr (PK == 2) y = mfma(columns[t & 1][1][s], wh[s], y);
+        y = mfma(columns[t & 1][0][s], wl[s], y);
+        y = mfma(columns[t & 1][0][s], wh[s], y);
       }
-      st[t] = x * ws.down;
+      st[t] = y;
+      if (t + 2 < 2 * DKB) read_columns(t + 2);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+    // ---- H
+    if constexpr (!STATES) {
+      const float pu = p_scale * us.down;
+      const int t0 = c * L;
+      T* const to = ho + (int64_t)t0 * p.DV + n0;
+      const bool whole = t0 + L <= p.S && n0 + 16 <= p.DV && p.DV % 4 == 0;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        const Four<T> o = rounded4<T>(x[mt] * pu + hs[mt] * fq[mt]);
+        if (whole) {
+          *(Four<T>*)((char*)(to + (int64_t)(16 * mt) * p.DV) + h_at) = o;
+        } else if (t0 + 16 * mt + r < p.S) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n0 + 4 * gq + e < p.DV) to[(int64_t)(16 * mt + r) * p.DV + 4 * gq + e] = o.e[e];
+        }
+      }
     }
     if (STAGES == 1) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (more) fetch(c + 1, 0);
+      if (next != c) fetch(next, 0);
     }
   }
   if (p.c_last && n < p.DV) {
@@ -283,7 +310,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = 16 * t + 4 * gq + e;
-        if (d < p.DK) p.c_last[((int64_t)bh * p.DK + d) * p.DV + n] = st[t][e];
+        if (d < p.DK) p.c_last[((int64_t)bh * p.DK + d) * p.DV + n] = st[t][e] * st_down;
       }
   }
 }
@@ -313,7 +340,8 @@ int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* 
   if (s.dtype == XL_DTYPE_F32) choose(float{});
   else if (s.dtype == XL_DTYPE_BF16) choose(bf16_t{});
   else choose(f16_t{});
-  const int blocks = kept ? kept->blocks : (s.DV + 15) / 16, waves = blocks >= 4 ? 4 : blocks >= 2 ? 2 : 1;
+  const int blocks = kept ? kept->blocks : (s.DV + 15) / 16;
+  const int waves = scan_waves((int64_t)s.B * s.NH, blocks);
   a.slices = (blocks + waves - 1) / waves;
   const int64_t lds = stages * (kept ? 1 : 2) * s.image_bytes() + 2 * 1024;
   void* args[] = {&a};

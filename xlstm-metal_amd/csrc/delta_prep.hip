@@ -106,7 +106,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
       for (int e = 0; e < 8; ++e) m[0] = fmaxf(m[0], fabsf(x[s][e]));
     }
     block_max(m, red);
-    const Pow2 sc = m[0] > 0.f ? pow2_for(m[0], 10) : Pow2{1.f, 1.f};
+    const Pow2 sc = m[0] > 0.f ? pow2_for(m[0], 0) : Pow2{1.f, 1.f};
     scales[which] = sc.down;
     char* to = lds + which * PK * IMG;
 #pragma unroll
