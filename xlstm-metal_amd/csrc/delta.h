@@ -60,6 +60,17 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+
+// the scheduler's order here: N products, a few vector operations between them
+template <int N>
+__device__ __forceinline__ void interleave() {
+  mfma::static_for<0, N>([](auto) {
+    __builtin_amdgcn_sched_group_barrier(0x8, 1, 0);
+    __builtin_amdgcn_sched_group_barrier(0x2, 3, 0);
+  });
+}
+
 // 2^target / 2^exponent(m) and its inverse: m times the first is in [2^target, 2^(target + 1)); m >= 0, the same in the wave.
 // At most 2^limit either way (0 gets that); KEPT for scales of which two are multiplied.
 constexpr int KEPT = 60;
@@ -225,12 +236,8 @@ struct Prep {
   Factors* f;
 };
 
-// Waves of a scan's workgroups: up to 4 share a chunk's images, fewer where that leaves CUs without one.
-inline int scan_waves(int64_t heads, int blocks) {
-  int waves = 4;
-  while (waves > 1 && (heads * ((blocks + waves - 1) / waves) < 256 || waves / 2 >= blocks)) waves /= 2;
-  return waves;
-}
+// Waves of a scan's workgroups: 4 share a chunk's images, unless that leaves CUs without a workgroup.
+inline int scan_waves(int64_t heads, int blocks) { return heads * ((blocks + 3) / 4) < 256 ? 1 : 4; }
 
 int check_shape(const char* who, const Shape& s);
 // q, k, v strides from the caller's nine or of contiguous tensors

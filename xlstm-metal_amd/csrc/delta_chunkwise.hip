@@ -24,28 +24,31 @@ struct ScanArgs {
 
 // PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32)
 // STATES: U and the state before each chunk are kept for the backward, and nothing else is written
-template <typename T, int DKB, int STAGES, bool STATES>
-__global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
+template <typename T, int DKB, int STAGES, bool STATES, int W>
+__global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
   constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = (STATES ? 1 : 2) * IMG;
   constexpr bool PAIR = STATES ? PK == 2 : !std::is_same_v<T, bf16_t>;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r = lane & 15, gq = lane >> 4;
   const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
-  const int bh = __builtin_amdgcn_readfirstlane(all / p.slices), slice = all - bh * p.slices;
-  const int b = bh / p.NH, h = bh - b * p.NH;
-  const int64_t image0 = ((int64_t)b * (p.NH / p.group) + h / p.group) * p.chunks, part0 = (int64_t)bh * p.chunks;
-  const int n0 = (slice * waves + wave) * 16, n = n0 + r;
+  const int bh = uniform(all / p.slices), slice = all - bh * p.slices, b = uniform(bh / p.NH), h = bh - b * p.NH;
+  const int64_t image0 = ((int64_t)b * uniform(p.NH / p.group) + uniform(h / p.group)) * p.chunks, part0 = (int64_t)bh * p.chunks;
+  const int n0 = (slice * W + wave) * 16, n = n0 + r;
   const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
   T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
 
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
-  auto fetch = [&](int chunk, int stage) {
+  // a chunk's images, in DKB shares; a wave brings every W-th KB
+  constexpr int SHARE = STAGE / 1024 / DKB / W;
+  static_assert(SHARE * W * DKB * 1024 == STAGE);
+  auto fetch = [&](int chunk, int stage, int share) {
     const char* ki = p.prep.k + (image0 + chunk) * (int64_t)IMG;
-    const char* qi = p.prep.q + (image0 + chunk) * (int64_t)IMG;
-    for (int i = wave; i < IMG / 1024; i += waves) {
-      to_lds(lds_at + stage * STAGE + i * 1024, i * 1024 + lane * 16, ki);
-      if constexpr (!STATES) to_lds(lds_at + stage * STAGE + IMG + i * 1024, i * 1024 + lane * 16, qi);
+    const char* qi = p.prep.q + (image0 + chunk) * (int64_t)IMG - IMG;
+#pragma unroll
+    for (int j = 0; j < SHARE; ++j) {
+      const int i = (share * SHARE + j) * W;  // K's or Q's, for all waves
+      to_lds(lds_at + stage * STAGE + (i + wave) * 1024, (i + wave) * 1024 + lane * 16, STATES || i < IMG / 1024 ? ki : qi);
     }
   };
   auto fetch_factors = [&](int chunk) {
@@ -109,7 +112,8 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
     if constexpr (PAIR) load_lower(from + FRAG_PLANE, lane, pl);
   };
   constexpr int LATER = 16 + 2 * LOWER;  // loads after a chunk's fetch, at least
-  fetch(0, 0);
+#pragma unroll
+  for (int s = 0; s < DKB; ++s) fetch(0, 0, s);
   fetch_factors(0);
   load_v(0);
   load_t(0);
@@ -122,10 +126,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
     const int stage = STAGES == 2 ? c & 1 : 0, next = c + 1 < p.chunks ? c + 1 : c;
-    if (next != c) {
-      if (STAGES == 2) fetch(next, stage ^ 1);
-      fetch_factors(next);
-    }
+    if (next != c) fetch_factors(next);
     const char *ki = lds + stage * STAGE, *qi = ki + IMG;
     const Factors* f = (const Factors*)(lds + STAGES * STAGE + (c & 1) * 1024);
 
@@ -156,13 +157,16 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       if constexpr (!STATES) fq[mt] = f->q[16 * mt + r] * st_down;
     }
     const float keep = f->all, t_scale = f->t, p_scale = f->p;
+    f16x8 sh[2], sl[2];
+    split8<true>(st[0], st[1], 1.f, sh[0], sl[0]);
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
       if (s + 1 < DKB) read(rows[(s + 1) & 1], s + 1);
+      if (STAGES == 2) fetch(next, stage ^ 1, s);
       __builtin_amdgcn_sched_barrier(0);
       const Rows& x = rows[s & 1];
-      f16x8 hi, lo;
-      split8<true>(st[2 * s], st[2 * s + 1], 1.f, hi, lo);
+      const f16x8 hi = sh[s & 1], lo = sl[s & 1];
+      if (s + 1 < DKB) split8<true>(st[2 * s + 2], st[2 * s + 3], 1.f, sh[(s + 1) & 1], sl[(s + 1) & 1]);
       if constexpr (STATES) {
         if (kept) {
           f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, PK, DKP) + r * DKP + s * 32 + gq * 8;
@@ -184,6 +188,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
         ks[mt] = mfma(x.k[0][mt], lo, ks[mt]);
         if constexpr (PAIR && !STATES) hs[mt] = mfma(lo, x.q[0][mt], hs[mt]);
       }
+      interleave<8 + (STATES ? 0 : 4) + (PK == 2 ? 4 : 0)>();
       __builtin_amdgcn_sched_barrier(0);
     }
     // ---- R
@@ -211,15 +216,16 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
     load_t(next);
     const float most = state_max(st) * st_down;  // not needed before w
     // the first operands of the state's product
-    f16x8 columns[2][PK][2];
+    constexpr int AHEAD = 4;
+    f16x8 columns[AHEAD][PK][2];
     auto read_columns = [&](int t) {
 #pragma unroll
       for (int pl = 0; pl < PK; ++pl)
 #pragma unroll
-        for (int s = 0; s < 2; ++s) columns[t & 1][pl][s] = columns_frag<DKP>(ki + pl * PLANE, t, s, r, gq);
+        for (int s = 0; s < 2; ++s) columns[t % AHEAD][pl][s] = columns_frag<DKP>(ki + pl * PLANE, t, s, r, gq);
     };
-    read_columns(0);
-    read_columns(1);
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) read_columns(t);
     f32x4 w[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
@@ -271,12 +277,12 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       f32x4 y = st[t] * up;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        if constexpr (PK == 2) y = mfma(columns[t & 1][1][s], wh[s], y);
-        y = mfma(columns[t & 1][0][s], wl[s], y);
-        y = mfma(columns[t & 1][0][s], wh[s], y);
+        if constexpr (PK == 2) y = mfma(columns[t % AHEAD][1][s], wh[s], y);
+        y = mfma(columns[t % AHEAD][0][s], wl[s], y);
+        y = mfma(columns[t % AHEAD][0][s], wh[s], y);
       }
       st[t] = y;
-      if (t + 2 < 2 * DKB) read_columns(t + 2);
+      if (t + AHEAD < 2 * DKB) read_columns(t + AHEAD);
       __builtin_amdgcn_sched_barrier(0);
     }
     // ---- H
@@ -301,7 +307,10 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (next != c) fetch(next, 0);
+      if (next != c) {
+#pragma unroll
+        for (int s = 0; s < DKB; ++s) fetch(next, 0, s);
+      }
     }
   }
   if (p.c_last && n < p.DV) {
@@ -315,14 +324,14 @@ __global__ __launch_bounds__(256, 1) void delta_scan_kernel(ScanArgs p) {
   }
 }
 
-template <typename T, bool STATES>
+template <typename T, bool STATES, int W>
 const void* pick(int dkp, int& stages) {
   stages = 2;
-  if (dkp == 64) return (const void*)delta_scan_kernel<T, 2, 2, STATES>;
-  if (dkp == 128) return (const void*)delta_scan_kernel<T, 4, 2, STATES>;
+  if (dkp == 64) return (const void*)delta_scan_kernel<T, 2, 2, STATES, W>;
+  if (dkp == 128) return (const void*)delta_scan_kernel<T, 4, 2, STATES, W>;
   constexpr int S8 = is_f32<T>::value && !STATES ? 1 : 2;  // two chunks of K and Q pairs do not fit
   stages = S8;
-  return (const void*)delta_scan_kernel<T, 8, S8, STATES>;
+  return (const void*)delta_scan_kernel<T, 8, S8, STATES, W>;
 }
 
 }  // namespace
@@ -333,15 +342,15 @@ int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* 
   if (kept) a.kept = *kept;
   int stages = 0;
   const void* kern = nullptr;
+  const int blocks = kept ? kept->blocks : (s.DV + 15) / 16, waves = scan_waves((int64_t)s.B * s.NH, blocks);
   auto choose = [&](auto t) {
     using T = decltype(t);
-    kern = kept ? pick<T, true>(s.dkp(), stages) : pick<T, false>(s.dkp(), stages);
+    kern = waves == 4 ? kept ? pick<T, true, 4>(s.dkp(), stages) : pick<T, false, 4>(s.dkp(), stages)
+                      : kept ? pick<T, true, 1>(s.dkp(), stages) : pick<T, false, 1>(s.dkp(), stages);
   };
   if (s.dtype == XL_DTYPE_F32) choose(float{});
   else if (s.dtype == XL_DTYPE_BF16) choose(bf16_t{});
   else choose(f16_t{});
-  const int blocks = kept ? kept->blocks : (s.DV + 15) / 16;
-  const int waves = scan_waves((int64_t)s.B * s.NH, blocks);
   a.slices = (blocks + waves - 1) / waves;
   const int64_t lds = stages * (kept ? 1 : 2) * s.image_bytes() + 2 * 1024;
   void* args[] = {&a};
