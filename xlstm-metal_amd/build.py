@@ -42,6 +42,10 @@ CXXFLAGS = [
 EXTRA_FLAGS = {
     "chunkwise_fused.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
     "chunkwise_pipe.hip": ["-mllvm", "-amdgpu-sched-strategy=iterative-ilp"],
+    # the gated delta rule's kernels work on what their products leave: with results in accumulation registers a third of the
+    # vector operations are moves, and the scan at DQK 256 spills
+    "delta_chunkwise.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
+    "delta_backward.hip": ["-mllvm", "-amdgpu-mfma-vgpr-form"],
 }
 
 
