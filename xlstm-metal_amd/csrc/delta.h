@@ -72,15 +72,14 @@ __device__ __forceinline__ void interleave() {
 }
 
 // 2^target / 2^exponent(m) and its inverse: m times the first is in [2^target, 2^(target + 1)); m >= 0, the same in the wave.
-// At most 2^limit either way (0 gets that); KEPT for scales of which two are multiplied.
-constexpr int KEPT = 60;
+// At most 2^100 either way (0 gets that).
 struct Pow2 {
   float up, down;
 };
-__device__ __forceinline__ Pow2 pow2_for(float m, int target = 14, int limit = 100) {
+__device__ __forceinline__ Pow2 pow2_for(float m, int target = 14) {
   const int e = (int)(__float_as_uint(m) >> 23);
   int sh = e == 255 ? 0 : target + 127 - e;
-  sh = sh > limit ? limit : sh < -limit ? -limit : sh;
+  sh = sh > 100 ? 100 : sh < -100 ? -100 : sh;
   return {__uint_as_float((uint32_t)(127 + sh) << 23), __uint_as_float((uint32_t)(127 - sh) << 23)};
 }
 
@@ -101,16 +100,35 @@ __device__ __forceinline__ float wave_max_all(float x) {
 __device__ __forceinline__ uint32_t pk_f16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((xl_f32x2{a, b}), xl_f16x2));
 }
+// x as f16 planes, 8 values, x within f16's range.  one: 1 that the compiler does not know, for x - hi in one operation
+// (v_fma_mix_f32 reads hi as f16).
+__device__ __forceinline__ void split8(f32x4 x, f32x4 y, float one, f16x8& hi, f16x8& lo) {
+  u32x4 h, l;
+#pragma unroll
+  for (int j = 0; j < 4; ++j) {
+    const float a = j < 2 ? x[2 * j] : y[2 * j - 4], b = j < 2 ? x[2 * j + 1] : y[2 * j - 3];
+    const xl_f16x2 p = __builtin_convertvector((xl_f32x2{a, b}), xl_f16x2);
+    h[j] = __builtin_bit_cast(uint32_t, p);
+    l[j] = pk_f16(fmaf(a, one, -(float)p[0]), fmaf(b, one, -(float)p[1]));
+  }
+  hi = __builtin_bit_cast(f16x8, h);
+  lo = __builtin_bit_cast(f16x8, l);
+}
+__device__ __forceinline__ float opaque_one() {
+  float one = 1.f;
+  asm("" : "+s"(one));
+  return one;
+}
 // x * scale as f16 planes, 8 values
 template <bool PAIR>
 __device__ __forceinline__ void split8(const float (&x)[8], float scale, f16x8& hi, f16x8& lo) {
   u32x4 h, l = {};
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    const float a = x[2 * j] * scale, b = x[2 * j + 1] * scale;
-    const xl_f16x2 p = __builtin_convertvector((xl_f32x2{a, b}), xl_f16x2);
+    const float a = x[2 * j], b = x[2 * j + 1];
+    const xl_f16x2 p = __builtin_convertvector((xl_f32x2{a * scale, b * scale}), xl_f16x2);
     h[j] = __builtin_bit_cast(uint32_t, p);
-    if constexpr (PAIR) l[j] = pk_f16(a - (float)p[0], b - (float)p[1]);
+    if constexpr (PAIR) l[j] = pk_f16(fmaf(a, scale, -(float)p[0]), fmaf(b, scale, -(float)p[1]));
   }
   hi = __builtin_bit_cast(f16x8, h);
   lo = __builtin_bit_cast(f16x8, l);
@@ -147,6 +165,7 @@ __device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const void
 // The scans keep the state at a power-of-two scale: its planes are taken without a multiplication.  With max(c_L |S|, |w|)
 // below 2^(STATE + 1) and K's values below 2 the next state, c_L S + K^T w over 64 tokens, is below 129 2^(STATE + 1) = 33024.
 constexpr int STATE = 7;
+constexpr int STATE_BACK = 6;  // two products: 257 2^7 = 32896
 
 // max of |x| over a wave's piece of the state
 template <int N>
@@ -207,7 +226,7 @@ __device__ __forceinline__ void load_upper(const f16_t* from, uint32_t lane, f16
 struct Kept {
   f16_t *u, *z, *dh;   // tokens x n
   f16_t *s0, *ds;      // the state before the chunk, the gradient of the state behind it
-  float *us, *zs, *dhs, *s0s, *dss;  // values = planes * these (a block of zeros: the least)
+  float *us, *zs, *dhs, *s0s, *dss;  // values = planes * these, powers of two (a block of zeros: the least)
   int blocks;          // of a head, padded
 };
 __device__ __forceinline__ int64_t kept_at(int64_t part, int blocks, int block, int planes, int width) {

@@ -53,7 +53,7 @@ __global__ __launch_bounds__(256) void delta_turn_kernel(TurnArgs p) {
       x[s][e] = tile[32 * s + (e < 4 ? 4 * gq + e : 12 + 4 * gq + e)][16 * wave + r];
       m = fmaxf(m, fabsf(x[s][e]));
     }
-  const Pow2 sc = pow2_for(wave_max_all(m), 14, KEPT);
+  const Pow2 sc = pow2_for(wave_max_all(m));
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     f16x8 hi, lo;
@@ -74,26 +74,30 @@ struct BackArgs {
   int NH, group, DK, DV, chunks, slices;
 };
 
-template <typename T, int DKB, int STAGES>
-__global__ __launch_bounds__(256, 1) void delta_back_kernel(BackArgs p) {
+// As the forward's scan (delta_chunkwise.hip): operands are read ahead of their products, the next chunk's are on their way.
+template <typename T, int DKB, int STAGES, int W>
+__global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
   constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r = lane & 15, gq = lane >> 4;
   const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
-  const int bh = __builtin_amdgcn_readfirstlane(all / p.slices), slice = all - bh * p.slices;
-  const int b = bh / p.NH, h = bh - b * p.NH;
-  const int64_t image0 = ((int64_t)b * (p.NH / p.group) + h / p.group) * p.chunks, part0 = (int64_t)bh * p.chunks;
+  const int bh = uniform(all / p.slices), slice = all - bh * p.slices, b = uniform(bh / p.NH), h = bh - b * p.NH;
+  const int64_t image0 = ((int64_t)b * uniform(p.NH / p.group) + uniform(h / p.group)) * p.chunks, part0 = (int64_t)bh * p.chunks;
   // past the last block a wave computes it again and writes nothing
-  const int own = slice * waves + wave, block = own < p.kept.blocks ? own : p.kept.blocks - 1, n = block * 16 + r;
+  const int own = slice * W + wave, block = own < p.kept.blocks ? own : p.kept.blocks - 1, n = block * 16 + r;
   const bool mine = own < p.kept.blocks;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
-  auto fetch = [&](int chunk, int stage) {
+  // a chunk's images, in DKB shares; a wave brings every W-th KB
+  constexpr int SHARE = STAGE / 1024 / DKB / W;
+  static_assert(SHARE * W * DKB * 1024 == STAGE);
+  auto fetch = [&](int chunk, int stage, int share) {
     const char* ki = p.prep.k + (image0 + chunk) * (int64_t)IMG;
-    const char* qi = p.prep.q + (image0 + chunk) * (int64_t)IMG;
-    for (int i = wave; i < IMG / 1024; i += waves) {
-      to_lds(lds_at + stage * STAGE + i * 1024, i * 1024 + lane * 16, ki);
-      to_lds(lds_at + stage * STAGE + IMG + i * 1024, i * 1024 + lane * 16, qi);
+    const char* qi = p.prep.q + (image0 + chunk) * (int64_t)IMG - IMG;
+#pragma unroll
+    for (int j = 0; j < SHARE; ++j) {
+      const int i = (share * SHARE + j) * W;  // K's or Q's, for all waves
+      to_lds(lds_at + stage * STAGE + (i + wave) * 1024, (i + wave) * 1024 + lane * 16, i < IMG / 1024 ? ki : qi);
     }
   };
   auto fetch_factors = [&](int chunk) {
@@ -101,7 +105,7 @@ __global__ __launch_bounds__(256, 1) void delta_back_kernel(BackArgs p) {
     to_lds(lds_at + STAGES * STAGE + (chunk & 1) * 2048, lane * 16, p.prep.f + part0 + chunk);
     to_lds(lds_at + STAGES * STAGE + (chunk & 1) * 2048 + 1024, 1024 + lane * 16, p.prep.f + part0 + chunk);
   };
-  f32x4 st[2 * DKB];
+  f32x4 st[2 * DKB];  // the state's gradient times 1 / st_down
 #pragma unroll
   for (int t = 0; t < 2 * DKB; ++t)
 #pragma unroll
@@ -109,6 +113,13 @@ __global__ __launch_bounds__(256, 1) void delta_back_kernel(BackArgs p) {
       const int d = 16 * t + 4 * gq + e;
       st[t][e] = p.dc_last && d < p.DK && n < p.DV ? p.dc_last[((int64_t)bh * p.DK + d) * p.DV + n] : 0.f;
     }
+  float st_down;
+  {
+    const Pow2 sc = pow2_for(state_max(st), STATE_BACK);
+    st_down = sc.down;
+#pragma unroll
+    for (int t = 0; t < 2 * DKB; ++t) st[t] *= sc.up;
+  }
   f16x8 th[LOWER], tl[LOWER], ph[LOWER], pl[LOWER], dh[2], dl[2];
   float dh_scale = 0.f;
   auto load_t = [&](int chunk) {
@@ -122,85 +133,93 @@ __global__ __launch_bounds__(256, 1) void delta_back_kernel(BackArgs p) {
     load_upper(from + FRAG_PLANE, lane, pl);
   };
   auto load_dh = [&](int chunk) {
-    const f16_t* from = p.kept.dh + kept_at(part0 + chunk, p.kept.blocks, block, PK, L) + r * L + gq * 8;
+    const f16_t* from = p.kept.dh + kept_at(part0 + chunk, p.kept.blocks, block, PK, L);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
-      dh[s] = *(const f16x8*)(from + s * 32);
-      if constexpr (PK == 2) dl[s] = *(const f16x8*)(from + s * 32 + 16 * L);
+      dh[s] = load16(from, r * (L * 2) + gq * 16 + s * 64);
+      if constexpr (PK == 2) dl[s] = load16(from + 16 * L, r * (L * 2) + gq * 16 + s * 64);
     }
     dh_scale = p.kept.dhs[(part0 + chunk) * p.kept.blocks + block];
   };
+  const float one = opaque_one();
+  constexpr int LATER = 4 * LOWER + 2;  // loads after a chunk's fetch, at least
   const int last = p.chunks - 1;
-  fetch(last, STAGES == 2 ? last & 1 : 0);
+#pragma unroll
+  for (int s = 0; s < DKB; ++s) fetch(last, STAGES == 2 ? last & 1 : 0, s);
   fetch_factors(last);
-  load_t(last);
   load_p(last);
+  load_t(last);
   load_dh(last);
   for (int c = last; c >= 0; --c) {
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STAGES == 2 ? LATER : 0) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
-    const int stage = STAGES == 2 ? c & 1 : 0;
-    const bool more = c > 0;
-    if (more) {
-      if (STAGES == 2) fetch(c - 1, stage ^ 1);
-      fetch_factors(c - 1);
-    }
+    const int stage = STAGES == 2 ? c & 1 : 0, next = c > 0 ? c - 1 : c;
+    if (next != c) fetch_factors(next);
     const char *ki = lds + stage * STAGE, *qi = ki + IMG;
     const Factors* f = (const Factors*)(lds + STAGES * STAGE + (c & 1) * 2048);
     const int64_t at = (part0 + c) * p.kept.blocks + block;
     // ---- K dS; dS is kept
-    float m = 0.f;
+    f16x8 rows[2][PK][4];
+    auto read = [&](int s) {
 #pragma unroll
-    for (int t = 0; t < 2 * DKB; ++t)
+      for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(st[t][e]));
-    const float most = wave_max_all(m);
-    const Pow2 ss = pow2_for(most, 14, KEPT);
-    f32x4 ks[4];
+        for (int pl = 0; pl < PK; ++pl) rows[s & 1][pl][mt] = rows_frag<DKP>(ki + pl * PLANE, mt, s, r, gq);
+    };
+    read(0);
+    f32x4 ks[4], out[4], fq[4], fb[4];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) ks[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
-    f16_t* const to_ds = p.kept.ds + kept_at(part0 + c, p.kept.blocks, block, PK, DKP) + r * DKP + gq * 8;
+    for (int mt = 0; mt < 4; ++mt) {
+      ks[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      out[mt] = *(const f32x4*)&f->out[16 * mt + 4 * gq] * st_down;
+      fq[mt] = *(const f32x4*)&f->q[16 * mt + 4 * gq];
+      fb[mt] = *(const f32x4*)&f->back[16 * mt + 4 * gq];
+    }
+    const float keep = f->all, t_scale = f->tt, p_scale = f->p;
+    f16_t* const to_ds = p.kept.ds + kept_at(part0 + c, p.kept.blocks, block, PK, DKP);
+    f16x8 sh[2], sl[2];
+    split8(st[0], st[1], one, sh[0], sl[0]);
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
-      f16x8 hi, lo;
-      split8<true>(st[2 * s], st[2 * s + 1], ss.up, hi, lo);
+      if (s + 1 < DKB) read(s + 1);
+      if (STAGES == 2) fetch(next, stage ^ 1, s);
+      __builtin_amdgcn_sched_barrier(0);
+      const f16x8 hi = sh[s & 1], lo = sl[s & 1];
       if (mine) {
-        *(f16x8*)(to_ds + s * 32) = hi;
-        if constexpr (PK == 2) *(f16x8*)(to_ds + s * 32 + 16 * DKP) = lo;
+        *(f16x8*)((char*)to_ds + r * (DKP * 2) + gq * 16 + s * 64) = hi;
+        if constexpr (PK == 2) *(f16x8*)((char*)(to_ds + 16 * DKP) + r * (DKP * 2) + gq * 16 + s * 64) = lo;
       }
+      if (s + 1 < DKB) split8(st[2 * s + 2], st[2 * s + 3], one, sh[(s + 1) & 1], sl[(s + 1) & 1]);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        const f16x8 k = rows_frag<DKP>(ki, mt, s, r, gq);
-        if constexpr (PK == 2) ks[mt] = mfma(rows_frag<DKP>(ki + PLANE, mt, s, r, gq), hi, ks[mt]);
-        ks[mt] = mfma(k, lo, ks[mt]);
-        ks[mt] = mfma(k, hi, ks[mt]);
+        if constexpr (PK == 2) ks[mt] = mfma(rows[s & 1][1][mt], hi, ks[mt]);
+        ks[mt] = mfma(rows[s & 1][0][mt], hi, ks[mt]);
       }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) ks[mt] = mfma(rows[s & 1][0][mt], lo, ks[mt]);
+      interleave<8 + (PK == 2 ? 4 : 0)>();
+      __builtin_amdgcn_sched_barrier(0);
     }
     // ---- dU
     f32x4 x[4], du[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) x[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < LOWER; ++i) {
-      f32x4& y = x[upper_mt(i)];
-      if constexpr (PK == 2) y = mfma(ph[i], dl[upper_s(i)], y);
-      y = mfma(pl[i], dh[upper_s(i)], y);
-      y = mfma(ph[i], dh[upper_s(i)], y);
-    }
-    if (more) load_p(c - 1);
-    const float px = f->p * dh_scale;
-    m = 0.f;
+    for (int i = 0; i < LOWER; ++i) x[upper_mt(i)] = mfma(ph[i], dh[upper_s(i)], x[upper_mt(i)]);
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const f32x4 out = *(const f32x4*)&f->out[16 * mt + 4 * gq];
+    for (int i = 0; i < LOWER; ++i) x[upper_mt(i)] = mfma(pl[i], dh[upper_s(i)], x[upper_mt(i)]);
+    if constexpr (PK == 2) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        du[mt][e] = fmaf(x[mt][e], px, out[e] * (ks[mt][e] * ss.down));
-        m = fmaxf(m, fabsf(du[mt][e]));
-      }
+      for (int i = 0; i < LOWER; ++i) x[upper_mt(i)] = mfma(ph[i], dl[upper_s(i)], x[upper_mt(i)]);
     }
-    const Pow2 us = pow2_for(wave_max_all(m));
+    load_p(next);
+    const float px = p_scale * dh_scale;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) du[mt][e] = fmaf(x[mt][e], px, out[mt][e] * ks[mt][e]);
+    const Pow2 us = pow2_for(wave_max_all(abs_max(du)));
     f16x8 uh[2], ul[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) split8<true>(du[2 * s], du[2 * s + 1], us.up, uh[s], ul[s]);
@@ -209,83 +228,93 @@ __global__ __launch_bounds__(256, 1) void delta_back_kernel(BackArgs p) {
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) z[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < LOWER; ++i) {
-      f32x4& y = z[upper_mt(i)];
-      y = mfma(tl[i], uh[upper_s(i)], y);
-      y = mfma(th[i], ul[upper_s(i)], y);
-      y = mfma(th[i], uh[upper_s(i)], y);
-    }
-    if (more) load_t(c - 1);
-    const float back = f->tt * us.down;
-    m = 0.f;
+    for (int i = 0; i < LOWER; ++i) z[upper_mt(i)] = mfma(th[i], uh[upper_s(i)], z[upper_mt(i)]);
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      z[mt] *= back;
+    for (int i = 0; i < LOWER; ++i) z[upper_mt(i)] = mfma(tl[i], uh[upper_s(i)], z[upper_mt(i)]);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) m = fmaxf(m, fabsf(z[mt][e]));
-    }
-    const Pow2 zs = pow2_for(wave_max_all(m), 14, KEPT);
-    if (mine) {
-#pragma unroll
-      for (int s = 0; s < 2; ++s) {
-        f16x8 zh, zl;
-        split8<PK == 2>(z[2 * s], z[2 * s + 1], zs.up, zh, zl);
-        f16_t* to = p.kept.z + kept_at(part0 + c, p.kept.blocks, block, PK, L) + r * L + s * 32 + gq * 8;
-        *(f16x8*)to = zh;
-        if constexpr (PK == 2) *(f16x8*)(to + 16 * L) = zl;
-      }
-      if (lane == 0) {
-        p.kept.zs[at] = zs.down;
-        p.kept.dss[at] = ss.down;
-      }
-    }
-    // ---- dS: Q^T w1 + K^T w2
+    for (int i = 0; i < LOWER; ++i) z[upper_mt(i)] = mfma(th[i], ul[upper_s(i)], z[upper_mt(i)]);
+    load_t(next);
+    // what does not wait for Z: w1, the state's size, the first operands of the state's products
     f32x4 w1[4], w2[4];
-    const float keep = f->all;
-    m = most * keep;
+    const float most = state_max(st) * st_down;
+    constexpr int AHEAD = PK == 2 ? 2 : 4;
+    f16x8 kc[AHEAD][PK][2], qc[AHEAD][PK][2];
+    auto read_columns = [&](int t) {
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const f32x4 fq = *(const f32x4*)&f->q[16 * mt + 4 * gq], fb = *(const f32x4*)&f->back[16 * mt + 4 * gq];
+      for (int pl = 0; pl < PK; ++pl)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          kc[t % AHEAD][pl][s] = columns_frag<DKP>(ki + pl * PLANE, t, s, r, gq);
+          qc[t % AHEAD][pl][s] = columns_frag<DKP>(qi + pl * PLANE, t, s, r, gq);
+        }
+    };
+#pragma unroll
+    for (int t = 0; t < AHEAD; ++t) read_columns(t);
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float d = (float)dh[mt >> 1][(mt & 1) * 4 + e];
         if constexpr (PK == 2) d += (float)dl[mt >> 1][(mt & 1) * 4 + e];
-        w1[mt][e] = fq[e] * (d * dh_scale);
-        w2[mt][e] = -fb[e] * z[mt][e];
-        m = fmaxf(m, fmaxf(fabsf(w1[mt][e]), fabsf(w2[mt][e])));
+        w1[mt][e] = fq[mt][e] * (d * dh_scale);
       }
+    load_dh(next);
+    const float back = t_scale * us.down;
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      z[mt] *= back;
+      w2[mt] = -fb[mt] * z[mt];
     }
-    if (more) load_dh(c - 1);
-    const Pow2 ws = pow2_for(wave_max_all(m));
-    f16x8 w1h[2], w1l[2], w2h[2], w2l[2];
+    const Pow2 zs = pow2_for(wave_max_all(abs_max(z)));
+    const Pow2 ws = pow2_for(fmaxf(wave_max_all(fmaxf(abs_max(w1), abs_max(w2))), most * keep), STATE_BACK);
+    f16x8 w1h[2], w1l[2], w2h[2], w2l[2], zh[2], zl[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       split8<true>(w1[2 * s], w1[2 * s + 1], ws.up, w1h[s], w1l[s]);
       split8<true>(w2[2 * s], w2[2 * s + 1], ws.up, w2h[s], w2l[s]);
+      split8<PK == 2>(z[2 * s], z[2 * s + 1], zs.up, zh[s], zl[s]);
     }
-    const float up = keep * ws.up;
-#pragma unroll
-    for (int t = 0; t < 2 * DKB; ++t) {
-      f32x4 y = st[t] * up;
+    if (mine) {
+      f16_t* to = p.kept.z + kept_at(part0 + c, p.kept.blocks, block, PK, L);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const f16x8 k = columns_frag<DKP>(ki, t, s, r, gq), q = columns_frag<DKP>(qi, t, s, r, gq);
-        if constexpr (PK == 2) {
-          y = mfma(columns_frag<DKP>(qi + PLANE, t, s, r, gq), w1h[s], y);
-          y = mfma(columns_frag<DKP>(ki + PLANE, t, s, r, gq), w2h[s], y);
-        }
-        y = mfma(q, w1l[s], y);
-        y = mfma(k, w2l[s], y);
-        y = mfma(q, w1h[s], y);
-        y = mfma(k, w2h[s], y);
+        *(f16x8*)((char*)to + r * (L * 2) + gq * 16 + s * 64) = zh[s];
+        if constexpr (PK == 2) *(f16x8*)((char*)(to + 16 * L) + r * (L * 2) + gq * 16 + s * 64) = zl[s];
       }
-      st[t] = y * ws.down;
+      if (lane == 0) {
+        p.kept.zs[at] = zs.down;
+        p.kept.dss[at] = st_down;
+      }
+    }
+    // ---- dS: Q^T w1 + K^T w2
+    const float up = keep * st_down * ws.up;
+    st_down = ws.down;
+#pragma unroll
+    for (int t = 0; t < 2 * DKB; ++t) {
+      f32x4 y = st[t] * up, y2 = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        if constexpr (PK == 2) {
+          y = mfma(qc[t % AHEAD][1][s], w1h[s], y);
+          y2 = mfma(kc[t % AHEAD][1][s], w2h[s], y2);
+        }
+        y = mfma(qc[t % AHEAD][0][s], w1l[s], y);
+        y2 = mfma(kc[t % AHEAD][0][s], w2l[s], y2);
+        y = mfma(qc[t % AHEAD][0][s], w1h[s], y);
+        y2 = mfma(kc[t % AHEAD][0][s], w2h[s], y2);
+      }
+      st[t] = y + y2;
+      if (t + AHEAD < 2 * DKB) read_columns(t + AHEAD);
+      __builtin_amdgcn_sched_barrier(0);
     }
     if (STAGES == 1) {
       asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
       __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      if (more) fetch(c - 1, 0);
+      if (next != c) {
+#pragma unroll
+        for (int s = 0; s < DKB; ++s) fetch(next, 0, s);
+      }
     }
   }
   if (p.dc0 && mine && n < p.DV) {
@@ -294,7 +323,7 @@ __global__ __launch_bounds__(256, 1) void delta_back_kernel(BackArgs p) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int d = 16 * t + 4 * gq + e;
-        if (d < p.DK) p.dc0[((int64_t)bh * p.DK + d) * p.DV + n] = st[t][e];
+        if (d < p.DK) p.dc0[((int64_t)bh * p.DK + d) * p.DV + n] = st[t][e] * st_down;
       }
   }
 }
@@ -356,28 +385,33 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   const int blocks = p.kept.blocks;
   const int64_t blk0 = part * blocks;
 
-  // ---- Blocks of columns have scales of their own; a product's sum over the columns takes the largest of its two scales'
-  // product, and one operand of a smaller block the factor that is left.
+  // ---- Blocks of columns have scales of their own (exponents here); a product's sum over the columns takes the largest of its
+  // two scales' product, and one operand of a smaller block the factor that is left.
   const float* const scales[5] = {p.kept.dhs + blk0, p.kept.zs + blk0, p.kept.us + blk0, p.kept.s0s + blk0, p.kept.dss + blk0};
   enum { DH_S, Z_S, U_DS, DH_U, Z_U, S_DS, SUMS };
-  auto products = [&](int block, float (&to)[SUMS]) {
-    const float dh = scales[0][block], z = scales[1][block], u = scales[2][block], s0 = scales[3][block], ds = scales[4][block];
-    to[DH_S] = dh * s0;
-    to[Z_S] = z * s0;
-    to[U_DS] = u * ds;
-    to[DH_U] = dh * u;
-    to[Z_U] = z * u;
-    to[S_DS] = s0 * ds;
+  auto products = [&](int block, int (&to)[SUMS]) {
+    int e[5];
+#pragma unroll
+    for (int i = 0; i < 5; ++i) e[i] = (int)(__float_as_uint(scales[i][block]) >> 23) - 127;
+    to[DH_S] = e[0] + e[3];
+    to[Z_S] = e[1] + e[3];
+    to[U_DS] = e[2] + e[4];
+    to[DH_U] = e[0] + e[2];
+    to[Z_U] = e[1] + e[2];
+    to[S_DS] = e[3] + e[4];
   };
-  float top[SUMS] = {};
+  auto power = [](int e) { return e < -126 ? 0.f : __uint_as_float((uint32_t)(e + 127) << 23); };  // e <= 0
+  int top[SUMS];
+#pragma unroll
+  for (int i = 0; i < SUMS; ++i) top[i] = -1000;
   for (int j = lane; j < blocks; j += 64) {
-    float x[SUMS];
+    int x[SUMS];
     products(j, x);
 #pragma unroll
-    for (int i = 0; i < SUMS; ++i) top[i] = fmaxf(top[i], x[i]);
+    for (int i = 0; i < SUMS; ++i) top[i] = max(top[i], x[i]);
   }
 #pragma unroll
-  for (int i = 0; i < SUMS; ++i) top[i] = wave_max_all(top[i]);
+  for (int i = 0; i < SUMS; ++i) top[i] = (int)wave_max_all((float)(top[i] + 1000)) - 1000;
   if (tid < L) {
     bs[tid] = f->b[tid];
     betas[tid] = f->beta[tid];
@@ -434,7 +468,9 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) x = fmaf((float)a[e] + (float)al[e], (float)d[e] + (float)dl[e], x);
       const int block = 2 * step + ((((i / PK) * THREADS + tid) / (DKP / 8)) >> 4);
-      ss_dot = fmaf(x, scales[3][block] * scales[4][block] / top[S_DS], ss_dot);
+      int e[SUMS];
+      products(block, e);
+      ss_dot = fmaf(x, power(e[S_DS] - top[S_DS]), ss_dot);
     }
   };
   // operands, k = the 32 columns: tokens 16 mt .. of matrix mat (0 dH, 1 Z, 2 U); DQK's columns 16 t .. of S_0 (0), dS (1)
@@ -482,12 +518,12 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
     __syncthreads();
     if (step + 1 < steps) load(step + 1);
     // a lane's 8 columns are of one block
-    float factor[SUMS];
+    int factor[SUMS];
     products(2 * step + (gq >> 1), factor);
     const float z_scale = scales[1][2 * step + (gq >> 1)];
     _Float16 by[SUMS];
 #pragma unroll
-    for (int i = 0; i < SUMS; ++i) by[i] = (_Float16)(factor[i] / top[i]);
+    for (int i = 0; i < SUMS; ++i) by[i] = (_Float16)power(factor[i] - top[i]);
     f16x8 s0[PK][2], ds[PK][2];
 #pragma unroll
     for (int pl = 0; pl < PK; ++pl)
@@ -574,9 +610,9 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   for (int x = 0; x < JOBS; ++x) {
     if (x * W + wave >= 20) continue;
     float* to = job_mat[x] ? dam : dpm;
-    const float sc = job_mat[x] ? -top[Z_U] : top[DH_U];
+    const int sc = job_mat[x] ? top[Z_U] : top[DH_U];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) to[(16 * job_i[x] + 4 * gq + e) * GLD + 16 * job_j[x] + r] = jobs[x][e] * sc;
+    for (int e = 0; e < 4; ++e) to[(16 * job_i[x] + 4 * gq + e) * GLD + 16 * job_j[x] + r] = ldexpf(job_mat[x] ? -jobs[x][e] : jobs[x][e], sc);
   }
   auto bring = [&](const char* img) {
     for (int i = tid * 16; i < PK * PLANE; i += THREADS * 16) *(u32x4*)(areaA + i) = *(const u32x4*)(img + image * (PK * PLANE) + i);
@@ -720,7 +756,7 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   const float ku = ksc * se.down, qu = qsc * sd.down;
 #pragma unroll
   for (int mt = 0; mt < 4; ++mt) {
-    const float fo = f->out[16 * mt + r] / ksc * top[U_DS] / ku, fb = f->back[16 * mt + r] / ksc * top[Z_S] / ku;
+    const float fo = ldexpf(f->out[16 * mt + r] / ksc / ku, top[U_DS]), fb = ldexpf(f->back[16 * mt + r] / ksc / ku, top[Z_S]);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       acck[t][mt] = g3[t][mt] * fo - g2[t][mt] * fb;
@@ -764,7 +800,7 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       const int token = t0 + 16 * mt + r;
-      const float fq = f->q[16 * mt + r] / qsc * top[DH_S];
+      const float fq = ldexpf(f->q[16 * mt + r] / qsc, top[DH_S]);
       if (token < p.S) {
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
@@ -786,13 +822,13 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
     qd += red[(3 * 8 + w) * L + lane];
     dss += wred[16 + w];
   }
-  kz *= ksc * top[Z_S];
-  const float sj = f->out[lane] * ks * top[U_DS];   // out has K's scale, which ks lacks
-  const float qi = f->q[lane] * qd * top[DH_S];
+  kz = ldexpf(kz * ksc, top[Z_S]);
+  const float sj = ldexpf(f->out[lane] * ks, top[U_DS]);   // out has K's scale, which ks lacks
+  const float qi = ldexpf(f->q[lane] * qd, top[DH_S]);
   const float ci = f->in[lane] / ksc, beta = betas[lane];
   const float dbeta = red[4 * 8 * L + lane] - ci * kz + rows[L + lane];
   float db = rows[lane] + beta * rows[L + lane] - cl - sj + qi - beta * ci * kz;
-  const float sums = wave_sum(sj) + f->all * dss * top[S_DS];
+  const float sums = wave_sum(sj) + ldexpf(f->all * dss, top[S_DS]);
   if (lane == 63) db += sums;
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1) {
@@ -864,8 +900,11 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
   BackArgs back{dc_last, dc0, prep, kept, s.NH, group, s.DK, s.DV, chunks, slices};
   constexpr int S8 = is_f32<T>::value ? 1 : 2;
   const int stages = s.dkp() == 256 ? S8 : 2;
-  const void* kern = s.dkp() == 64 ? (const void*)delta_back_kernel<T, 2, 2> : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2>
-                                                                                            : (const void*)delta_back_kernel<T, 8, S8>;
+  const void* kern =
+      waves == 4 ? s.dkp() == 64    ? (const void*)delta_back_kernel<T, 2, 2, 4>
+                   : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2, 4> : (const void*)delta_back_kernel<T, 8, S8, 4>
+      : s.dkp() == 64    ? (const void*)delta_back_kernel<T, 2, 2, 1>
+        : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2, 1> : (const void*)delta_back_kernel<T, 8, S8, 1>;
   if (e == hipSuccess)
     e = launch(kern, (int64_t)s.B * s.NH * slices, 1, 64 * waves, stages * 2 * s.image_bytes() + 2 * 2048, &back, st);
   GradArgs grad{v, {s.vs[0], s.vs[1], s.vs[2]}, group == 1 ? dq : (void*)dqp, group == 1 ? dk : (void*)dkp, dv, dg, dbeta, prep, kept,

@@ -89,10 +89,9 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
       const int d = 16 * t + 4 * gq + e;
       st[t][e] = p.c0 && d < p.DK ? p.c0[((int64_t)bh * p.DK + d) * p.DV + nc] : 0.f;
     }
-  constexpr int LIMIT = STATES ? KEPT : 100;
   float st_down;
   {
-    const Pow2 sc = pow2_for(state_max(st), STATE, LIMIT);
+    const Pow2 sc = pow2_for(state_max(st), STATE);
     st_down = sc.down;
 #pragma unroll
     for (int t = 0; t < 2 * DKB; ++t) st[t] *= sc.up;
@@ -111,6 +110,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
     load_lower(from, lane, ph);
     if constexpr (PAIR) load_lower(from + FRAG_PLANE, lane, pl);
   };
+  const float one = opaque_one();
   constexpr int LATER = 16 + 2 * LOWER;  // loads after a chunk's fetch, at least
 #pragma unroll
   for (int s = 0; s < DKB; ++s) fetch(0, 0, s);
@@ -158,7 +158,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
     }
     const float keep = f->all, t_scale = f->t, p_scale = f->p;
     f16x8 sh[2], sl[2];
-    split8<true>(st[0], st[1], 1.f, sh[0], sl[0]);
+    split8(st[0], st[1], one, sh[0], sl[0]);
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
       if (s + 1 < DKB) read(rows[(s + 1) & 1], s + 1);
@@ -166,7 +166,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
       __builtin_amdgcn_sched_barrier(0);
       const Rows& x = rows[s & 1];
       const f16x8 hi = sh[s & 1], lo = sl[s & 1];
-      if (s + 1 < DKB) split8<true>(st[2 * s + 2], st[2 * s + 3], 1.f, sh[(s + 1) & 1], sl[(s + 1) & 1]);
+      if (s + 1 < DKB) split8(st[2 * s + 2], st[2 * s + 3], one, sh[(s + 1) & 1], sl[(s + 1) & 1]);
       if constexpr (STATES) {
         if (kept) {
           f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, PK, DKP) + r * DKP + s * 32 + gq * 8;
@@ -232,8 +232,8 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
       u[mt] *= back;
       w[mt] = u[mt] * out[mt];
     }
-    const Pow2 us = pow2_for(wave_max_all(abs_max(u)), 14, LIMIT);
-    const Pow2 ws = pow2_for(fmaxf(wave_max_all(abs_max(w)), most * keep), STATE, LIMIT);
+    const Pow2 us = pow2_for(wave_max_all(abs_max(u)));
+    const Pow2 ws = pow2_for(fmaxf(wave_max_all(abs_max(w)), most * keep), STATE);
     f16x8 uh[2], ul[2], wh[2], wl[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {

@@ -25,27 +25,31 @@ struct PrepArgs {
 
 constexpr int MLD = 68;  // row length of 64 x 64 float32 matrices in LDS
 
+// 8 values as they lie; zeros past n
 template <typename T>
-__device__ __forceinline__ void load8(const T* p, int from, int n, bool wide, float (&x)[8]) {
+struct Raw8 {
+  u32x4 w[sizeof(T) / 2];
+};
+template <typename T>
+__device__ __forceinline__ Raw8<T> load8(const T* p, int from, int n, bool wide) {
+  Raw8<T> x;
   if (wide && from + 8 <= n) {
-    if constexpr (is_f32<T>::value) {
-      const f32x4 a = *(const f32x4*)(p + from), b = *(const f32x4*)(p + from + 4);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        x[e] = a[e];
-        x[4 + e] = b[e];
-      }
-    } else {
-      const u32x4 raw = *(const u32x4*)(p + from);
-      struct V { T e[8]; };
-      const V v = __builtin_bit_cast(V, raw);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) x[e] = to_f32(v.e[e]);
-    }
+    for (int i = 0; i < (int)sizeof(T) / 2; ++i) x.w[i] = *(const u32x4*)(p + from + 4 * i);
   } else {
+    struct V { T e[8]; } v;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) x[e] = from + e < n ? to_f32(p[from + e]) : 0.f;
+    for (int e = 0; e < 8; ++e) v.e[e] = from + e < n ? p[from + e] : from_f32<T>(0.f);
+    x = __builtin_bit_cast(Raw8<T>, v);
   }
+  return x;
+}
+template <typename T>
+__device__ __forceinline__ void values8(const Raw8<T>& raw, float (&x)[8]) {
+  struct V { T e[8]; };
+  const V v = __builtin_bit_cast(V, raw);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) x[e] = to_f32(v.e[e]);
 }
 
 __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
@@ -89,30 +93,58 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
   // ---- K and Q: a row's 32 columns are one piece of 8 of each of 4 threads
   const int row = tid >> 2, c = tid & 3;
   float scales[2];  // K, Q = planes * these
+  Raw8<T> raw[2][DKB];  // both under way at once
+  const bool there = t0 + row < p.S;  // past the last token: its row again, for zeros
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
     const int64_t* st = which ? p.qs : p.ks;
-    const T* from = (const T*)(which ? p.q : p.k) + b * st[0] + hk * st[1] + (int64_t)(t0 + row) * st[2];
-    float x[DKB][8], m[1] = {0.f};
+    const T* from = (const T*)(which ? p.q : p.k) + b * st[0] + hk * st[1] + (int64_t)(there ? t0 + row : p.S - 1) * st[2];
+#pragma unroll
+    for (int s = 0; s < DKB; ++s) raw[which][s] = load8(from, 32 * s + 8 * c, p.DK, p.wide);
+  }
+  float gt = 0.f, bt = 0.f;
+  auto load_gates = [&](int64_t bh) {
+    const int64_t at = bh * p.S + (t0 + lane < p.S ? t0 + lane : p.S - 1);
+    auto gates = [&](auto type) {
+      using G = decltype(type);
+      gt = to_f32(((const G*)p.g)[at]);
+      bt = to_f32(((const G*)p.beta)[at]);
+    };
+    switch (p.gate_dtype) {
+      case XL_DTYPE_F32: gates(0.f); break;
+      case XL_DTYPE_BF16: gates(bf16_t{}); break;
+      default: gates(f16_t{}); break;
+    }
+    if (t0 + lane >= p.S) gt = bt = 0.f;
+  };
+  load_gates((int64_t)b * p.NH + hk * group);
+  float m2[2] = {0.f, 0.f};
+#pragma unroll
+  for (int which = 0; which < 2; ++which)
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
-      if (t0 + row < p.S) {
-        load8(from, 32 * s + 8 * c, p.DK, p.wide, x[s]);
-      } else {
+      float x[8];
+      values8(raw[which][s], x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[s][e] = 0.f;
-      }
-#pragma unroll
-      for (int e = 0; e < 8; ++e) m[0] = fmaxf(m[0], fabsf(x[s][e]));
+      for (int e = 0; e < 8; ++e) m2[which] = fmaxf(m2[which], there ? fabsf(x[e]) : 0.f);
     }
-    block_max(m, red);
-    const Pow2 sc = m[0] > 0.f ? pow2_for(m[0], 0) : Pow2{1.f, 1.f};
+  block_max(m2, red);
+#pragma unroll
+  for (int which = 0; which < 2; ++which) {
+    const Pow2 sc = m2[which] > 0.f ? pow2_for(m2[which], 0) : Pow2{1.f, 1.f};
     scales[which] = sc.down;
+    const float up = there ? sc.up : 0.f;
     char* to = lds + which * PK * IMG;
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
       f16x8 hi, lo;
-      split8<PK == 2>(x[s], sc.up, hi, lo);
+      float x[8];
+      values8(raw[which][s], x);
+      if (!there) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] = 0.f;
+      }
+      split8<PK == 2>(x, up, hi, lo);
       // values 8 c + 0..3 and 4..7 of the 32: groups 2 c, 2 c + 1 of 4, the second four groups in the upper halves
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
@@ -163,20 +195,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
     const int h = hk * group + rep;
     const int64_t bh = (int64_t)b * p.NH + h, part = bh * p.chunks + chunk;
     // ---- running sums of g, a lane a token
-    const int token = t0 + lane;
-    float gt = 0.f, bt = 0.f;
-    auto gates = [&](auto type) {
-      using G = decltype(type);
-      if (token < p.S) {
-        gt = to_f32(((const G*)p.g)[bh * p.S + token]);
-        bt = to_f32(((const G*)p.beta)[bh * p.S + token]);
-      }
-    };
-    switch (p.gate_dtype) {
-      case XL_DTYPE_F32: gates(0.f); break;
-      case XL_DTYPE_BF16: gates(bf16_t{}); break;
-      default: gates(f16_t{}); break;
-    }
+    if (rep) load_gates(bh);
     gt = gt < CLAMP_G ? CLAMP_G : gt;
     double sum = (double)gt;
 #pragma unroll
