@@ -47,9 +47,10 @@ struct Factors {
   float q[L];      // scale c_i 2^q      Q S
   float out[L];    // c_L / c_i 2^k      U into the state
   float all;       // c_L
+  float most;      // the largest of out
   float t, tt, p;  // T diag(beta), T and P = planes * these
   float k, qs;     // K, Q = planes * these
-  float pad[58];   // the scans take the first 1 KB into LDS
+  float pad[57];   // the scans take the first 1 KB into LDS
   float back[L];   // beta_i c_i 2^k     Z into the state's gradient
   float beta[L];
   double b[L];     // running sums of g
@@ -60,6 +61,12 @@ __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
 }
 
+// A barrier for what lies in LDS; loads from memory stay under way (__syncthreads would wait for them).
+__device__ __forceinline__ void lds_barrier() {
+  asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // the scheduler's order here: N products, a few vector operations between them
@@ -83,41 +90,56 @@ __device__ __forceinline__ Pow2 pow2_for(float m, int target = 14) {
   return {__uint_as_float((uint32_t)(127 + sh) << 23), __uint_as_float((uint32_t)(127 - sh) << 23)};
 }
 
-// max over the wave, in every lane (scalar)
-__device__ __forceinline__ float wave_max_all(float x) {
-#define XL_DPP_MAX(CTRL, ROWMASK) \
-  x = fmaxf(x, __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, ROWMASK, 0xf, false)));
-  XL_DPP_MAX(0x111, 0xf)  // row_shr:1 (what is shifted in is 0: x is not negative)
+// max over the wave of x >= 0, in every lane (scalar); by the bits, which order as the values do (a NaN is the largest)
+__device__ __forceinline__ float wave_max_all(float value) {
+  uint32_t x = __float_as_uint(value);
+#define XL_DPP_MAX(CTRL, ROWMASK) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWMASK, 0xf, false));
+  XL_DPP_MAX(0x111, 0xf)  // row_shr:1 (what is shifted in is 0)
   XL_DPP_MAX(0x112, 0xf)
   XL_DPP_MAX(0x114, 0xf)
   XL_DPP_MAX(0x118, 0xf)
   XL_DPP_MAX(0x142, 0xa)  // row_bcast:15
   XL_DPP_MAX(0x143, 0xc)  // row_bcast:31
 #undef XL_DPP_MAX
-  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), 63));
+  return __int_as_float(__builtin_amdgcn_readlane((int)x, 63));
 }
 
 __device__ __forceinline__ uint32_t pk_f16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((xl_f32x2{a, b}), xl_f16x2));
 }
-// x as f16 planes, 8 values, x within f16's range.  one: 1 that the compiler does not know, for x - hi in one operation
-// (v_fma_mix_f32 reads hi as f16).
-__device__ __forceinline__ void split8(f32x4 x, f32x4 y, float one, f16x8& hi, f16x8& lo) {
+// x as f16 planes, 8 values, x within f16's range
+__device__ __forceinline__ void split8(f32x4 x, f32x4 y, f16x8& hi, f16x8& lo) {
   u32x4 h, l;
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
     const float a = j < 2 ? x[2 * j] : y[2 * j - 4], b = j < 2 ? x[2 * j + 1] : y[2 * j - 3];
     const xl_f16x2 p = __builtin_convertvector((xl_f32x2{a, b}), xl_f16x2);
     h[j] = __builtin_bit_cast(uint32_t, p);
-    l[j] = pk_f16(fmaf(a, one, -(float)p[0]), fmaf(b, one, -(float)p[1]));
+    l[j] = pk_f16(a - (float)p[0], b - (float)p[1]);
   }
   hi = __builtin_bit_cast(f16x8, h);
   lo = __builtin_bit_cast(f16x8, l);
 }
-__device__ __forceinline__ float opaque_one() {
-  float one = 1.f;
-  asm("" : "+s"(one));
-  return one;
+// x * scale as planes, 4 values
+__device__ __forceinline__ void split4(f32x4 x, float scale, f16x4& hi, f16x4& lo) {
+  u32x2 h, l;
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const float a = x[2 * j], b = x[2 * j + 1];
+    const xl_f16x2 p = __builtin_convertvector((xl_f32x2{a * scale, b * scale}), xl_f16x2);
+    h[j] = __builtin_bit_cast(uint32_t, p);
+    l[j] = pk_f16(fmaf(a, scale, -(float)p[0]), fmaf(b, scale, -(float)p[1]));
+  }
+  hi = __builtin_bit_cast(f16x4, h);
+  lo = __builtin_bit_cast(f16x4, l);
+}
+__device__ __forceinline__ f16x8 join(f16x4 a, f16x4 b) {
+  return f16x8{a[0], a[1], a[2], a[3], b[0], b[1], b[2], b[3]};
+}
+// a / b of powers of two, as f16 (0 below its range); a <= b
+__device__ __forceinline__ _Float16 ratio(float a, float b) {
+  const int e = (int)(__float_as_uint(a) >> 23) - (int)(__float_as_uint(b) >> 23);
+  return e < -24 ? (_Float16)0.f : (_Float16)__uint_as_float((uint32_t)(127 + e) << 23);
 }
 // x * scale as f16 planes, 8 values
 template <bool PAIR>
@@ -167,16 +189,7 @@ __device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const void
 constexpr int STATE = 7;
 constexpr int STATE_BACK = 6;  // two products: 257 2^7 = 32896
 
-// max of |x| over a wave's piece of the state
-template <int N>
-__device__ __forceinline__ float state_max(const f32x4 (&st)[N]) {
-  float m[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-  for (int t = 0; t < N; ++t)
-#pragma unroll
-    for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], fabsf(st[t][e]));
-  return wave_max_all(fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3])));
-}
+// max of |x| of a lane's
 template <int N>
 __device__ __forceinline__ float abs_max(const f32x4 (&x)[N]) {
   float m[4] = {0.f, 0.f, 0.f, 0.f};
@@ -185,6 +198,11 @@ __device__ __forceinline__ float abs_max(const f32x4 (&x)[N]) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) m[e] = fmaxf(m[e], fabsf(x[t][e]));
   return fmaxf(fmaxf(m[0], m[1]), fmaxf(m[2], m[3]));
+}
+// max of |x| over a wave's piece of the state
+template <int N>
+__device__ __forceinline__ float state_max(const f32x4 (&st)[N]) {
+  return wave_max_all(abs_max(st));
 }
 
 // Images of K and Q: [plane][64 tokens][DKP] f16, the largest value in [1, 2), each 32 columns turned, the 16-byte piece p of token i at p ^ (i % 8).
@@ -254,9 +272,6 @@ struct Prep {
   f16_t *tt, *pt;    // T^T, P^T (2 planes)
   Factors* f;
 };
-
-// Waves of a scan's workgroups: 4 share a chunk's images, unless that leaves CUs without a workgroup.
-inline int scan_waves(int64_t heads, int blocks) { return heads * ((blocks + 3) / 4) < 256 ? 1 : 4; }
 
 int check_shape(const char* who, const Shape& s);
 // q, k, v strides from the caller's nine or of contiguous tensors

@@ -141,7 +141,6 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
     }
     dh_scale = p.kept.dhs[(part0 + chunk) * p.kept.blocks + block];
   };
-  const float one = opaque_one();
   constexpr int LATER = 4 * LOWER + 2;  // loads after a chunk's fetch, at least
   const int last = p.chunks - 1;
 #pragma unroll
@@ -179,7 +178,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
     const float keep = f->all, t_scale = f->tt, p_scale = f->p;
     f16_t* const to_ds = p.kept.ds + kept_at(part0 + c, p.kept.blocks, block, PK, DKP);
     f16x8 sh[2], sl[2];
-    split8(st[0], st[1], one, sh[0], sl[0]);
+    split8(st[0], st[1], sh[0], sl[0]);
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
       if (s + 1 < DKB) read(s + 1);
@@ -190,7 +189,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
         *(f16x8*)((char*)to_ds + r * (DKP * 2) + gq * 16 + s * 64) = hi;
         if constexpr (PK == 2) *(f16x8*)((char*)(to_ds + 16 * DKP) + r * (DKP * 2) + gq * 16 + s * 64) = lo;
       }
-      if (s + 1 < DKB) split8(st[2 * s + 2], st[2 * s + 3], one, sh[(s + 1) & 1], sl[(s + 1) & 1]);
+      if (s + 1 < DKB) split8(st[2 * s + 2], st[2 * s + 3], sh[(s + 1) & 1], sl[(s + 1) & 1]);
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
         if constexpr (PK == 2) ks[mt] = mfma(rows[s & 1][1][mt], hi, ks[mt]);
@@ -896,7 +895,7 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
   hipError_t e = launch((const void*)delta_turn_kernel<T>, s.parts(), (kept.blocks + 3) / 4, 256, 0, &turn, st);
   if (e == hipSuccess)
     if (const int rc = launch_scan(s, v, c0, nullptr, nullptr, prep, &kept, st, who)) return rc;
-  const int waves = scan_waves((int64_t)s.B * s.NH, kept.blocks), slices = (kept.blocks + waves - 1) / waves;
+  const int waves = (int64_t)s.B * s.NH * ((kept.blocks + 3) / 4) < 256 ? 1 : 4, slices = (kept.blocks + waves - 1) / waves;
   BackArgs back{dc_last, dc0, prep, kept, s.NH, group, s.DK, s.DV, chunks, slices};
   constexpr int S8 = is_f32<T>::value ? 1 : 2;
   const int stages = s.dkp() == 256 ? S8 : 2;

@@ -1,10 +1,17 @@
 // Gated delta rule by chunks, second kernel: the scan over a head's chunks (delta.h has the formulas).
 //
-// A wave takes 16 columns through the sequence, its [DQK, 16] piece of the state in float32 registers; the waves of a
-// workgroup share the chunk's images of K and Q in LDS, filled straight from memory a chunk ahead, and nothing else.  Per
-// chunk: K S and Q S (one pass over the state, which is split into f16 planes on the way), R = V - diag(c) K S, U = T R,
-// H = Q S + P U, S = c_L S + K^T U.  U comes out of T R as the B operand of the next two products; H is formed turned
-// (columns down, tokens across), so that a lane holds four neighbours of a row.
+// Every 16 columns of V, U and the state go through the sequence by themselves.  PARTS waves (2 or 4) take a block of 16: a wave
+// has its part of the state's rows (DQK / PARTS, float32 registers) and as large a part of a chunk's tokens.  Per chunk:
+//
+//   1  K S and Q S over the wave's rows, all tokens; the others' tokens go to LDS
+//   2  R = V - diag(c) K S of the wave's tokens, to LDS as f16 planes
+//   3  U = T R of the wave's tokens, to LDS as f16 planes, decayed for the state and as it is for H
+//   4  S = c_L S + K^T U of the wave's rows; H = Q S + P U of the wave's tokens
+//
+// A wave on its own (the first form) is a chain of some 800 vector operations and 100 products a chunk that little can
+// overlap: 3.1 us a chunk at DQK 128, 4.7 at 256.  CB blocks of one workgroup share the chunk's images of K and Q in LDS, filled
+// straight from memory: K a chunk ahead, Q from where this chunk's has been read; T, P, V of the next chunk wait in
+// registers.  H is formed turned (columns down, tokens across), so that a lane holds four neighbours of a row.
 #include "delta.h"
 
 namespace xl {
@@ -23,10 +30,395 @@ struct ScanArgs {
 };
 
 // PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32)
-// STATES: U and the state before each chunk are kept for the backward, and nothing else is written
-template <typename T, int DKB, int STAGES, bool STATES, int W>
-__global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
-  constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = (STATES ? 1 : 2) * IMG;
+// LDS of a scan's workgroup: KST stages of K, one of Q, two chunks' factors, and each block's exchanges
+template <int DKB, int PK, int PARTS, int CB, int KST, bool WITH_Q, bool WIDE_U>
+struct ScanLds {
+  static constexpr int IMG = PK * L * DKB * 32 * 2;
+  static constexpr int Q = KST * IMG, FACTORS = Q + (WITH_Q ? IMG : 0), BLOCKS = FACTORS + 2 * 1024;
+  // of a block: sums of the others' parts (then of Q S), R, U decayed, U, scales
+  static constexpr int SUMS = 0, R = 4 * (PARTS - 1) * 1024, UD = R + 4096, U = UD + 4096, SCALES = U + (WIDE_U ? 4096 : 2048);
+  static constexpr int BLOCK = SCALES + 64, BYTES = BLOCKS + CB * BLOCK;
+};
+
+// STATES: U and the state before each chunk are kept for the backward, and nothing else is written.
+// PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32).
+template <typename T, int DKB, int PARTS, int CB, int KST, bool STATES>
+__global__ __launch_bounds__(64 * PARTS * CB) void delta_scan_kernel(ScanArgs p) {
+  constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE;
+  constexpr int WAVES = PARTS * CB, TPW = 4 / PARTS, NB = DKB / PARTS;  // a wave's tiles of 16 tokens, its 32s of DQK
+  constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
+  using Lds = ScanLds<DKB, PK, PARTS, CB, KST, !STATES, PAIR>;
+  static_assert(DKB % PARTS == 0 && Lds::BYTES <= 160 * 1024);
+  extern __shared__ __align__(1024) char lds[];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), cb = wave / PARTS, part = wave % PARTS;
+  const int r = lane & 15, gq = lane >> 4;
+  const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
+  const int bh = uniform(all / p.slices), slice = all - bh * p.slices, b = uniform(bh / p.NH), h = bh - b * p.NH;
+  const int64_t image0 = ((int64_t)b * uniform(p.NH / p.group) + uniform(h / p.group)) * p.chunks, part0 = (int64_t)bh * p.chunks;
+  const int block = slice * CB + cb, n0 = block * 16, n = n0 + r;
+  const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
+  T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
+  const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
+  char* const mine = lds + Lds::BLOCKS + cb * Lds::BLOCK;
+  float* const scales = (float*)(mine + Lds::SCALES);  // [R, U, state][part]
+  // partial sums of tile mt by the parts that do not own it
+  auto sums_at = [&](int mt, int from) {
+    return (f32x4*)(mine + Lds::SUMS) + (mt * (PARTS - 1) + from - (from > mt / TPW ? 1 : 0)) * 64 + lane;
+  };
+
+  auto fetch = [&](const char* images, int chunk, int to) {
+    const char* img = images + (image0 + chunk) * (int64_t)IMG;
+#pragma unroll
+    for (int i = 0; i < IMG / 1024; i += WAVES)
+      if (IMG / 1024 % WAVES == 0 || i + wave < IMG / 1024)
+        to_lds(lds_at + to + (i + wave) * 1024, (i + wave) * 1024 + lane * 16, img);
+  };
+  auto fetch_factors = [&](int chunk) {
+    if (wave == 0) to_lds(lds_at + Lds::FACTORS + (chunk & 1) * 1024, lane * 16, p.prep.f + part0 + chunk);
+  };
+  // Tokens 16 mt + 4 gq + e of column n, mt of this wave.  Past the last token the last one is read again (its beta is 0 there: T
+  // has zeros in its column), past the last column the last one: those columns are computed and not written.
+  const int nc = n < p.DV ? n : p.DV - 1, row_step = (int)p.vs[2];
+  T vn[TPW][4];
+  uint32_t v_at[TPW][4];
+#pragma unroll
+  for (int x = 0; x < TPW; ++x)
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      v_at[x][e] = (uint32_t)((16 * (part * TPW + x) + 4 * gq + e) * row_step + nc) * (uint32_t)sizeof(T);
+  auto load_v = [&](int chunk) {
+    const int t0 = chunk * L;
+    if (t0 + L > p.S) {  // the last chunk, once
+#pragma unroll
+      for (int x = 0; x < TPW; ++x)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int t = 16 * (part * TPW + x) + 4 * gq + e, last = p.S - 1 - t0;
+          v_at[x][e] = (uint32_t)((t < last ? t : last) * row_step + nc) * (uint32_t)sizeof(T);
+        }
+    }
+    const char* base = (const char*)(v + t0 * p.vs[2]);
+#pragma unroll
+    for (int x = 0; x < TPW; ++x)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) vn[x][e] = *(const T*)(base + v_at[x][e]);
+  };
+  // T's and P's rows of the wave's tokens, both halves of k
+  f16x8 th[TPW][2], tl[TPW][2], ph[TPW][2], pl[PAIR ? TPW : 1][2];
+  auto load_rows = [&](const f16_t* from, f16x8 (&to)[TPW][2]) {
+#pragma unroll
+    for (int x = 0; x < TPW; ++x)
+#pragma unroll
+      for (int s = 0; s < 2; ++s) to[x][s] = load16(from + (2 * (part * TPW + x) + s) * 512, lane * 16);
+  };
+  auto load_t = [&](int chunk) {
+    const f16_t* from = p.prep.t + (part0 + chunk) * (2 * FRAG_PLANE);
+    load_rows(from, th);
+    load_rows(from + FRAG_PLANE, tl);
+  };
+  auto load_p = [&](int chunk) {
+    const f16_t* from = p.prep.p + (part0 + chunk) * (2 * FRAG_PLANE);
+    load_rows(from, ph);
+    if constexpr (PAIR) load_rows(from + FRAG_PLANE, pl);
+  };
+
+  f32x4 st[2 * NB];  // the wave's rows of the state, times 1 / st_down (the same for all parts)
+#pragma unroll
+  for (int t = 0; t < 2 * NB; ++t)
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const int d = 16 * (2 * NB * part + t) + 4 * gq + e;
+      st[t][e] = p.c0 && d < p.DK ? p.c0[((int64_t)bh * p.DK + d) * p.DV + nc] : 0.f;
+    }
+  auto largest = [&](const float* of) {
+    float m = of[0];
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) m = fmaxf(m, of[i]);
+    return __int_as_float(uniform(__float_as_int(m)));
+  };
+  float st_down, most = state_max(st);
+  if (lane == 0) scales[2 * PARTS + part] = most;
+  __syncthreads();
+  {
+    const Pow2 sc = pow2_for(largest(scales + 2 * PARTS), STATE);
+    st_down = sc.down;
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t) st[t] *= sc.up;
+  }
+
+  // What is loaded past the last chunk is that one's again: as many loads are under way after every chunk.
+  constexpr int LATER = 4 * TPW + 4 * TPW;  // loads after a chunk's images, at least (V, T)
+  fetch(p.prep.k, 0, 0);
+  if constexpr (!STATES) fetch(p.prep.q, 0, Lds::Q);
+  fetch_factors(0);
+  load_v(0);
+  load_t(0);
+  if constexpr (!STATES) load_p(0);
+  const bool kept = STATES && block < p.kept.blocks;
+  const uint32_t h_at = (uint32_t)(r * p.DV + 4 * gq) * sizeof(T);
+  for (int c = 0; c < p.chunks; ++c) {
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(KST == 2 ? LATER : 0) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    const int stage = KST == 2 ? (c & 1) * IMG : 0, next = c + 1 < p.chunks ? c + 1 : c;
+    const char *ki = lds + stage, *qi = lds + Lds::Q;
+    const Factors* f = (const Factors*)(lds + Lds::FACTORS + (c & 1) * 1024);
+
+    // ---- 1: K S, and Q S turned, over the wave's rows
+    f32x4 ks[4], hs[STATES ? 1 : 4], in[TPW], out[TPW];
+    float fq[TPW];
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      ks[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      if constexpr (!STATES) hs[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+    }
+#pragma unroll
+    for (int s = 0; s < NB; ++s) {
+      const int sb = part * NB + s;
+      f16x8 k[PK][4], q[STATES ? 1 : PK][4], hi, lo;
+#pragma unroll
+      for (int pl = 0; pl < PK; ++pl)
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          k[pl][mt] = rows_frag<DKP>(ki + pl * PLANE, mt, sb, r, gq);
+          if constexpr (!STATES) q[pl][mt] = rows_frag<DKP>(qi + pl * PLANE, mt, sb, r, gq);
+        }
+      split8(st[2 * s], st[2 * s + 1], hi, lo);
+      if constexpr (STATES) {
+        if (kept) {
+          f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, PK, DKP);
+          *(f16x8*)((char*)to + r * (DKP * 2) + gq * 16 + sb * 64) = hi;
+          if constexpr (PK == 2) *(f16x8*)((char*)(to + 16 * DKP) + r * (DKP * 2) + gq * 16 + sb * 64) = lo;
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        if constexpr (PK == 2) ks[mt] = mfma(k[1][mt], hi, ks[mt]);
+        ks[mt] = mfma(k[0][mt], hi, ks[mt]);
+        ks[mt] = mfma(k[0][mt], lo, ks[mt]);
+      }
+      if constexpr (!STATES) {
+#pragma unroll
+        for (int mt = 0; mt < 4; ++mt) {
+          if constexpr (PK == 2) hs[mt] = mfma(hi, q[1][mt], hs[mt]);
+          hs[mt] = mfma(hi, q[0][mt], hs[mt]);
+          if constexpr (PAIR) hs[mt] = mfma(lo, q[0][mt], hs[mt]);
+        }
+      }
+    }
+    f32x4 own[TPW];  // the wave's own tokens
+#pragma unroll
+    for (int mt = 0; mt < 4; ++mt) {
+      if (mt / TPW == part) own[mt % TPW] = ks[mt];
+      else *sums_at(mt, part) = ks[mt];
+    }
+#pragma unroll
+    for (int x = 0; x < TPW; ++x) {
+      const int mt = part * TPW + x;
+      in[x] = *(const f32x4*)&f->in[16 * mt + 4 * gq] * st_down;
+      out[x] = *(const f32x4*)&f->out[16 * mt + 4 * gq];
+      if constexpr (!STATES) fq[x] = f->q[16 * mt + r] * st_down;
+    }
+    const float keep = f->all, t_scale = f->t, p_scale = f->p;
+    const Pow2 decayed = pow2_for(f->most, 0);  // U decayed is below 2 decayed.down times U
+    most = state_max(st) * st_down;
+    if (lane == 0) scales[2 * PARTS + part] = most;
+    lds_barrier();  // Q has been read too: its place takes the next chunk's; K's other stage has been free since the chunk began
+    if (next != c) {
+      if (KST == 2) fetch(p.prep.k, next, stage ^ IMG);
+      if constexpr (!STATES) fetch(p.prep.q, next, Lds::Q);
+      fetch_factors(next);
+    }
+    // ---- 2: R
+    f32x4 rr[TPW];
+#pragma unroll
+    for (int x = 0; x < TPW; ++x) {
+      const int mt = part * TPW + x;
+#pragma unroll
+      for (int i = 0; i < PARTS - 1; ++i) own[x] += *((const f32x4*)(mine + Lds::SUMS) + (mt * (PARTS - 1) + i) * 64 + lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e) rr[x][e] = fmaf(-in[x][e], own[x][e], to_f32(vn[x][e]));
+    }
+    load_v(next);
+    const Pow2 rs = pow2_for(wave_max_all(abs_max(rr)));
+#pragma unroll
+    for (int x = 0; x < TPW; ++x) {
+      f16x4 hi, lo;
+      split4(rr[x], rs.up, hi, lo);
+      *((f16x8*)(mine + Lds::R) + (part * TPW + x) * 64 + lane) = join(hi, lo);
+    }
+    if (lane == 0) scales[part] = rs.down;
+    lds_barrier();
+    // ---- 3: U
+    f16x8 rh[2], rl[2];
+    const float r_down = largest(scales);
+    auto planes = [&](const f16x8* from, const float* of, float down, f16x8 (&hi)[2], f16x8 (&lo)[2]) {
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        f16x4 h[2], l[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const f16x8 x = from[(2 * s + i) * 64 + lane] * ratio(__int_as_float(uniform(__float_as_int(of[(2 * s + i) / TPW]))), down);
+          h[i] = f16x4{x[0], x[1], x[2], x[3]};
+          l[i] = f16x4{x[4], x[5], x[6], x[7]};
+        }
+        hi[s] = join(h[0], h[1]);
+        lo[s] = join(l[0], l[1]);
+      }
+    };
+    planes((const f16x8*)(mine + Lds::R), scales, r_down, rh, rl);
+    f32x4 u[TPW], w[TPW];
+    const float back = t_scale * r_down;
+#pragma unroll
+    for (int x = 0; x < TPW; ++x) {
+      f32x4 y = {0.f, 0.f, 0.f, 0.f}, y2 = y;
+      y = mfma(tl[x][0], rh[0], y);
+      y2 = mfma(th[x][0], rl[0], y2);
+      if (part * TPW + x >= 2) {
+        y = mfma(tl[x][1], rh[1], y);
+        y2 = mfma(th[x][1], rl[1], y2);
+        y = mfma(th[x][1], rh[1], y);
+      }
+      y2 = mfma(th[x][0], rh[0], y2);
+      u[x] = (y + y2) * back;
+      w[x] = u[x] * out[x];
+    }
+    load_t(next);
+    const Pow2 us = pow2_for(wave_max_all(abs_max(u)));
+    const float ws_up = us.up * decayed.up * 0.5f;
+#pragma unroll
+    for (int x = 0; x < TPW; ++x) {
+      const int mt = part * TPW + x;
+      f16x4 hi, lo;
+      split4(w[x], ws_up, hi, lo);
+      *((f16x8*)(mine + Lds::UD) + mt * 64 + lane) = join(hi, lo);
+      if constexpr (!STATES) {
+        split4(u[x], us.up, hi, lo);
+        if constexpr (PAIR) *((f16x8*)(mine + Lds::U) + mt * 64 + lane) = join(hi, lo);
+        else *((f16x4*)(mine + Lds::U) + mt * 64 + lane) = hi;
+      }
+    }
+    if (lane == 0) scales[PARTS + part] = us.down;
+    if constexpr (!STATES) {
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        if (mt / TPW == part) own[mt % TPW] = hs[mt];
+        else *sums_at(mt, part) = hs[mt];
+      }
+    }
+    lds_barrier();
+    // ---- 4: the state
+    const float u_down = largest(scales + PARTS), w_down = u_down * decayed.down * 2.f;
+    // U decayed is below 2^15 w_down
+    const Pow2 sc = pow2_for(fmaxf(largest(scales + 2 * PARTS) * keep, w_down * 32767.f), STATE);
+    f16x8 wh[2], wl[2];
+    planes((const f16x8*)(mine + Lds::UD), scales + PARTS, u_down, wh, wl);
+    const _Float16 shift = (_Float16)(w_down * sc.up);  // to the state's scale: 2^-8 or less
+#pragma unroll
+    for (int s = 0; s < 2; ++s) {
+      wh[s] *= shift;
+      wl[s] *= shift;
+    }
+    const float up = keep * st_down * sc.up;
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t) {
+      f32x4 y = st[t] * up, y2 = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int s = 0; s < 2; ++s) {
+        const f16x8 k = columns_frag<DKP>(ki, 2 * NB * part + t, s, r, gq);
+        if constexpr (PK == 2) y2 = mfma(columns_frag<DKP>(ki + PLANE, 2 * NB * part + t, s, r, gq), wh[s], y2);
+        y2 = mfma(k, wl[s], y2);
+        y = mfma(k, wh[s], y);
+      }
+      st[t] = y + y2;
+    }
+    if constexpr (STATES) {
+      if (kept) {
+        const _Float16 by = ratio(us.down, u_down);
+#pragma unroll
+        for (int x = 0; x < TPW; ++x) {
+          const int mt = part * TPW + x;
+          f16x4 hi, lo;
+          split4(u[x], us.up, hi, lo);
+          char* to = (char*)(p.kept.u + kept_at(part0 + c, p.kept.blocks, block, PK, L)) + r * (L * 2) + (mt >> 1) * 64 + gq * 16 + (mt & 1) * 8;
+          *(f16x4*)to = hi * by;
+          if constexpr (PK == 2) *(f16x4*)(to + 16 * L * 2) = lo * by;
+        }
+        if (lane == 0 && part == 0) {
+          const int64_t at = (part0 + c) * p.kept.blocks + block;
+          p.kept.us[at] = u_down;
+          p.kept.s0s[at] = st_down;
+        }
+      }
+    } else {  // ---- H
+      f16x8 uh[2], ul[2];
+      if constexpr (PAIR) {
+        planes((const f16x8*)(mine + Lds::U), scales + PARTS, u_down, uh, ul);
+      } else {
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          f16x4 x[2];
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            x[i] = *((const f16x4*)(mine + Lds::U) + (2 * s + i) * 64 + lane) *
+                   ratio(__int_as_float(uniform(__float_as_int(scales[PARTS + (2 * s + i) / TPW]))), u_down);
+          uh[s] = join(x[0], x[1]);
+        }
+      }
+      const float pu = p_scale * u_down;
+      const int t0 = c * L;
+      T* const to = ho + (int64_t)t0 * p.DV + n0;
+      const bool whole = t0 + L <= p.S && n0 + 16 <= p.DV && p.DV % 4 == 0;
+#pragma unroll
+      for (int x = 0; x < TPW; ++x) {
+        const int mt = part * TPW + x;
+#pragma unroll
+        for (int i = 0; i < PARTS - 1; ++i) own[x] += *((const f32x4*)(mine + Lds::SUMS) + (mt * (PARTS - 1) + i) * 64 + lane);
+        f32x4 y = {0.f, 0.f, 0.f, 0.f};
+        y = mfma(uh[0], ph[x][0], y);
+        if constexpr (PAIR) {
+          y = mfma(ul[0], ph[x][0], y);
+          y = mfma(uh[0], pl[x][0], y);
+        }
+        if (mt >= 2) {
+          y = mfma(uh[1], ph[x][1], y);
+          if constexpr (PAIR) {
+            y = mfma(ul[1], ph[x][1], y);
+            y = mfma(uh[1], pl[x][1], y);
+          }
+        }
+        const Four<T> o = rounded4<T>(y * pu + own[x] * fq[x]);
+        if (whole) {
+          *(Four<T>*)((char*)(to + (int64_t)(16 * mt) * p.DV) + h_at) = o;
+        } else if (t0 + 16 * mt + r < p.S) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            if (n0 + 4 * gq + e < p.DV) to[(int64_t)(16 * mt + r) * p.DV + 4 * gq + e] = o.e[e];
+        }
+      }
+      load_p(next);
+    }
+    st_down = sc.down;
+    if (KST == 1) {
+      lds_barrier();
+      if (next != c) fetch(p.prep.k, next, 0);
+    }
+  }
+  if (p.c_last && n < p.DV) {
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        const int d = 16 * (2 * NB * part + t) + 4 * gq + e;
+        if (d < p.DK) p.c_last[((int64_t)bh * p.DK + d) * p.DV + n] = st[t][e] * st_down;
+      }
+  }
+}
+
+// A block by one wave, W blocks a workgroup.
+template <typename T, int DKB, int STAGES, bool STATES>
+__global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
+  constexpr int W = 4, DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = (STATES ? 1 : 2) * IMG;
   constexpr bool PAIR = STATES ? PK == 2 : !std::is_same_v<T, bf16_t>;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -110,7 +502,6 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
     load_lower(from, lane, ph);
     if constexpr (PAIR) load_lower(from + FRAG_PLANE, lane, pl);
   };
-  const float one = opaque_one();
   constexpr int LATER = 16 + 2 * LOWER;  // loads after a chunk's fetch, at least
 #pragma unroll
   for (int s = 0; s < DKB; ++s) fetch(0, 0, s);
@@ -157,8 +548,9 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
       if constexpr (!STATES) fq[mt] = f->q[16 * mt + r] * st_down;
     }
     const float keep = f->all, t_scale = f->t, p_scale = f->p;
+    const Pow2 decayed = pow2_for(f->most, 0);  // U decayed is below 2 decayed.down times U
     f16x8 sh[2], sl[2];
-    split8(st[0], st[1], one, sh[0], sl[0]);
+    split8(st[0], st[1], sh[0], sl[0]);
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
       if (s + 1 < DKB) read(rows[(s + 1) & 1], s + 1);
@@ -166,7 +558,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
       __builtin_amdgcn_sched_barrier(0);
       const Rows& x = rows[s & 1];
       const f16x8 hi = sh[s & 1], lo = sl[s & 1];
-      if (s + 1 < DKB) split8(st[2 * s + 2], st[2 * s + 3], one, sh[(s + 1) & 1], sl[(s + 1) & 1]);
+      if (s + 1 < DKB) split8(st[2 * s + 2], st[2 * s + 3], sh[(s + 1) & 1], sl[(s + 1) & 1]);
       if constexpr (STATES) {
         if (kept) {
           f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, PK, DKP) + r * DKP + s * 32 + gq * 8;
@@ -233,7 +625,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
       w[mt] = u[mt] * out[mt];
     }
     const Pow2 us = pow2_for(wave_max_all(abs_max(u)));
-    const Pow2 ws = pow2_for(fmaxf(wave_max_all(abs_max(w)), most * keep), STATE);
+    const Pow2 ws = pow2_for(fmaxf(us.down * decayed.down * 65534.f, most * keep), STATE);  // U is below 2^15 us.down
     f16x8 uh[2], ul[2], wh[2], wl[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -324,14 +716,26 @@ __global__ __launch_bounds__(64 * W, 1) void delta_scan_kernel(ScanArgs p) {
   }
 }
 
-template <typename T, bool STATES, int W>
-const void* pick(int dkp, int& stages) {
-  stages = 2;
-  if (dkp == 64) return (const void*)delta_scan_kernel<T, 2, 2, STATES, W>;
-  if (dkp == 128) return (const void*)delta_scan_kernel<T, 4, 2, STATES, W>;
-  constexpr int S8 = is_f32<T>::value && !STATES ? 1 : 2;  // two chunks of K and Q pairs do not fit
-  stages = S8;
-  return (const void*)delta_scan_kernel<T, 8, S8, STATES, W>;
+struct Choice {
+  const void* kern;
+  int threads, blocks, lds;  // threads of a workgroup, its blocks of 16 columns
+};
+// Few blocks: one a workgroup, by as many waves as there are 32s of DQK, up to 4.  Many: one a wave, 4 a workgroup.  us, both ways:
+//   256 blocks, DQK 128, 64 chunks     171 (a wave), 155 (4 waves)
+//   1024 blocks, DQK 256, 128 chunks   590 (a wave), 834 (2 waves a block, 4 blocks a workgroup: T and P come to each)
+template <typename T, int DKB, bool STATES>
+Choice choice(bool many) {
+  constexpr int PK = is_f32<T>::value ? 2 : 1, KST = DKB == 8 && PK == 2 && !STATES ? 1 : 2;  // K's pairs twice and Q's do not fit
+  constexpr int PARTS = DKB < 4 ? DKB : 4;
+  constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
+  if (many)
+    return {(const void*)delta_scan_wave_kernel<T, DKB, KST, STATES>, 256, 4, KST * (STATES ? 1 : 2) * PK * L * DKB * 64 + 2 * 1024};
+  return {(const void*)delta_scan_kernel<T, DKB, PARTS, 1, KST, STATES>, 64 * PARTS, 1,
+          ScanLds<DKB, PK, PARTS, 1, KST, !STATES, PAIR>::BYTES};
+}
+template <typename T, bool STATES>
+Choice pick(int dkp, bool many) {
+  return dkp == 64 ? choice<T, 2, STATES>(many) : dkp == 128 ? choice<T, 4, STATES>(many) : choice<T, 8, STATES>(many);
 }
 
 }  // namespace
@@ -340,23 +744,21 @@ int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* 
                 hipStream_t st, const char* who) {
   ScanArgs a{v, {s.vs[0], s.vs[1], s.vs[2]}, c0, h, c_last, prep, {}, s.NH, s.NH / s.NHK, s.S, s.DK, s.DV, s.chunks(), 0};
   if (kept) a.kept = *kept;
-  int stages = 0;
-  const void* kern = nullptr;
-  const int blocks = kept ? kept->blocks : (s.DV + 15) / 16, waves = scan_waves((int64_t)s.B * s.NH, blocks);
+  const int blocks = kept ? kept->blocks : (s.DV + 15) / 16;
+  const bool many = (int64_t)s.B * s.NH * ((blocks + 3) / 4) >= 256;
+  Choice use{};
   auto choose = [&](auto t) {
     using T = decltype(t);
-    kern = waves == 4 ? kept ? pick<T, true, 4>(s.dkp(), stages) : pick<T, false, 4>(s.dkp(), stages)
-                      : kept ? pick<T, true, 1>(s.dkp(), stages) : pick<T, false, 1>(s.dkp(), stages);
+    use = kept ? pick<T, true>(s.dkp(), many) : pick<T, false>(s.dkp(), many);
   };
   if (s.dtype == XL_DTYPE_F32) choose(float{});
   else if (s.dtype == XL_DTYPE_BF16) choose(bf16_t{});
   else choose(f16_t{});
-  a.slices = (blocks + waves - 1) / waves;
-  const int64_t lds = stages * (kept ? 1 : 2) * s.image_bytes() + 2 * 1024;
+  a.slices = (blocks + use.blocks - 1) / use.blocks;
   void* args[] = {&a};
-  hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);
+  hipError_t e = hipFuncSetAttribute(use.kern, hipFuncAttributeMaxDynamicSharedMemorySize, use.lds);
   if (e == hipSuccess)
-    e = hipLaunchKernel(kern, dim3((unsigned)((int64_t)s.B * s.NH * a.slices)), dim3(64 * waves), args, (unsigned)lds, st);
+    e = hipLaunchKernel(use.kern, dim3((unsigned)((int64_t)s.B * s.NH * a.slices)), dim3(use.threads), args, (unsigned)use.lds, st);
   if (e != hipSuccess) return set_error(XL_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
   return check_launch(who);
 }

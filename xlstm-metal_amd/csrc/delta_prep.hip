@@ -212,7 +212,9 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
       f->b[lane] = sum;
       f->in[lane] = in * scales[0];
       f->q[lane] = in * scales[1] * p.scale;
-      f->out[lane] = exp_of(last - sum) * scales[0];
+      const float out = exp_of(last - sum) * scales[0], most = wave_max_all(out);
+      f->out[lane] = out;
+      if (lane == 0) f->most = most;
       f->back[lane] = bt * in * scales[0];
       f->beta[lane] = bt;
     }
