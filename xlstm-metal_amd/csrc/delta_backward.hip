@@ -29,6 +29,7 @@ struct TurnArgs {
   const void* dh;
   Kept kept;
   int S, DV, chunks;
+  bool wide;  // 16-byte loads
 };
 
 template <typename T>
@@ -38,10 +39,24 @@ __global__ __launch_bounds__(256) void delta_turn_kernel(TurnArgs p) {
   const int64_t part = blockIdx.x;
   const int64_t bh = part / p.chunks;
   const int t0 = (int)(part - bh * p.chunks) * L, n0 = blockIdx.y * 64;
-  const int row = threadIdx.x >> 2, c = (threadIdx.x & 3) * 16;
-  const T* from = (const T*)p.dh + (bh * p.S + t0 + row) * p.DV + n0 + c;
+  // 8 lanes a row, 8 values each
 #pragma unroll
-  for (int e = 0; e < 16; ++e) tile[row][c + e] = t0 + row < p.S && n0 + c + e < p.DV ? to_f32(from[e]) : 0.f;
+  for (int half = 0; half < 2; ++half) {
+    const int row = half * 32 + (threadIdx.x >> 3), c = (threadIdx.x & 7) * 8;
+    const T* from = (const T*)p.dh + (bh * p.S + t0 + row) * p.DV + n0 + c;
+    float x[8];
+    if (t0 + row < p.S && n0 + c + 8 <= p.DV && p.wide) {
+      struct alignas(16) Eight { T e[8]; };
+      const Eight v = *(const Eight*)from;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = to_f32(v.e[e]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = t0 + row < p.S && n0 + c + e < p.DV ? to_f32(from[e]) : 0.f;
+    }
+#pragma unroll
+    for (int e = 0; e < 8; ++e) tile[row][c + e] = x[e];
+  }
   __syncthreads();
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r = lane & 15, gq = lane >> 4, block = blockIdx.y * 4 + wave;
   if (block >= p.kept.blocks) return;
@@ -354,8 +369,9 @@ struct GradLds {
   static constexpr int STAGE = PK * (3 * TOK + 2 * STA), IMAGE = PK * L * DKP * 2;
   static constexpr int KK = L * GLD * 4;
   static constexpr int A = STAGE > IMAGE + KK ? STAGE : IMAGE + KK;  // the columns; then K or Q, and K K^T
-  static constexpr int B = 2 * KK > 6 * L * L * 2 ? 2 * KK : 6 * L * L * 2;  // dP, dA; then their operands
-  static constexpr int SMALL = 6 * 8 * L * 4 + 64 * 4 + L * 8 + 4 * L * 4;
+  static constexpr int OPERANDS = (std::is_same_v<T, bf16_t> ? 3 : 6) * L * L * 2;
+  static constexpr int B = 2 * KK > OPERANDS ? 2 * KK : OPERANDS;  // dP, dA; then their operands
+  static constexpr int SMALL = (4 * DKB + 1) * L * 4 + 64 * 4 + L * 8 + 3 * L * 4;
   static constexpr int BYTES = A + B + SMALL;
 };
 
@@ -369,10 +385,10 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   char *areaA = lds, *areaB = lds + Lds::A;
   float* kkm = (float*)(lds + Lds::IMAGE);
   float *dpm = (float*)areaB, *dam = (float*)(areaB + Lds::KK);
-  float* red = (float*)(areaB + Lds::B);  // [6][8][L]
-  float* wred = red + 6 * 8 * L;          // [64]
+  float* red = (float*)(areaB + Lds::B);  // [4][W][L], [L]
+  float* wred = red + (4 * W + 1) * L;    // [64]
   double* bs = (double*)(wred + 64);
-  float* betas = (float*)(bs + L);        // [L], then row sums [2][L], spare [L]
+  float* betas = (float*)(bs + L);        // [L], then row sums [2][L]
   float* rows = betas + L;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, gq = lane >> 4;
@@ -654,7 +670,7 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
       }
       x += __shfl_xor(x, 16, 64);
       x += __shfl_xor(x, 32, 64);
-      if (gq == 0) red[(slot * 8 + wave) * L + 16 * mt + r] = x;
+      if (gq == 0) red[(slot * W + wave) * L + 16 * mt + r] = x;
     }
   };
   dots(g2, 0);  // k_i.(Z S_0^T)_i
@@ -687,7 +703,7 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
     mx[0] = fmaxf(mx[0], fabsf(dps[x]));
     mx[1] = fmaxf(mx[1], fabsf(ee[x]));
   }
-  red[(2 * 8 + wave) * L + lane] = col;
+  red[(2 * W + wave) * L + lane] = col;
   const float m0 = wave_max_all(mx[0]), m1 = wave_max_all(mx[1]), dot = wave_sum(ss_dot);
   if (lane == 0) {
     wred[wave] = m0;
@@ -700,7 +716,7 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
     float y = zv[x];
     y += __shfl_xor(y, 16, 64);
     y += __shfl_xor(y, 32, 64);
-    if (gq == 0) red[4 * 8 * L + 16 * (wave + x * W) + r] = y;
+    if (gq == 0) red[4 * W * L + 16 * (wave + x * W) + r] = y;
   }
   __syncthreads();  // dP and dA have been read: their place takes the operands
   mx[0] = mx[1] = 0.f;
@@ -815,17 +831,17 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   float kz = 0.f, ks = 0.f, qd = 0.f, cl = 0.f, dss = 0.f;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
-    kz += red[(0 * 8 + w) * L + lane];
-    ks += red[(1 * 8 + w) * L + lane];
-    cl += red[(2 * 8 + w) * L + lane];
-    qd += red[(3 * 8 + w) * L + lane];
+    kz += red[(0 * W + w) * L + lane];
+    ks += red[(1 * W + w) * L + lane];
+    cl += red[(2 * W + w) * L + lane];
+    qd += red[(3 * W + w) * L + lane];
     dss += wred[16 + w];
   }
   kz = ldexpf(kz * ksc, top[Z_S]);
   const float sj = ldexpf(f->out[lane] * ks, top[U_DS]);   // out has K's scale, which ks lacks
   const float qi = ldexpf(f->q[lane] * qd, top[DH_S]);
   const float ci = f->in[lane] / ksc, beta = betas[lane];
-  const float dbeta = red[4 * 8 * L + lane] - ci * kz + rows[L + lane];
+  const float dbeta = red[4 * W * L + lane] - ci * kz + rows[L + lane];
   float db = rows[lane] + beta * rows[L + lane] - cl - sj + qi - beta * ci * kz;
   const float sums = wave_sum(sj) + ldexpf(f->all * dss, top[S_DS]);
   if (lane == 63) db += sums;
@@ -891,7 +907,7 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
              void* dbeta, float* dc0, const float* c0, const Prep& prep, const Kept& kept, float* dqp, float* dkp, hipStream_t st,
              const char* who) {
   const int group = s.NH / s.NHK, chunks = s.chunks();
-  TurnArgs turn{dh, kept, s.S, s.DV, chunks};
+  TurnArgs turn{dh, kept, s.S, s.DV, chunks, s.DV % 8 == 0 && ((uintptr_t)dh & 15) == 0};
   hipError_t e = launch((const void*)delta_turn_kernel<T>, s.parts(), (kept.blocks + 3) / 4, 256, 0, &turn, st);
   if (e == hipSuccess)
     if (const int rc = launch_scan(s, v, c0, nullptr, nullptr, prep, &kept, st, who)) return rc;
