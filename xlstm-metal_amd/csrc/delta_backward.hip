@@ -404,10 +404,10 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   // two scales' product, and one operand of a smaller block the factor that is left.
   const float* const scales[5] = {p.kept.dhs + blk0, p.kept.zs + blk0, p.kept.us + blk0, p.kept.s0s + blk0, p.kept.dss + blk0};
   enum { DH_S, Z_S, U_DS, DH_U, Z_U, S_DS, SUMS };
-  auto products = [&](int block, int (&to)[SUMS]) {
+  auto products = [&](const float (&of)[5], int (&to)[SUMS]) {
     int e[5];
 #pragma unroll
-    for (int i = 0; i < 5; ++i) e[i] = (int)(__float_as_uint(scales[i][block]) >> 23) - 127;
+    for (int i = 0; i < 5; ++i) e[i] = (int)(__float_as_uint(of[i]) >> 23) - 127;
     to[DH_S] = e[0] + e[3];
     to[Z_S] = e[1] + e[3];
     to[U_DS] = e[2] + e[4];
@@ -421,7 +421,8 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   for (int i = 0; i < SUMS; ++i) top[i] = -1000;
   for (int j = lane; j < blocks; j += 64) {
     int x[SUMS];
-    products(j, x);
+    const float of[5] = {scales[0][j], scales[1][j], scales[2][j], scales[3][j], scales[4][j]};
+    products(of, x);
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) top[i] = max(top[i], x[i]);
   }
@@ -435,7 +436,12 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   // ---- staging: pieces of 16 bytes, through registers
   constexpr int TOK_PIECES = 3 * PK * 256, TOK_PER = (TOK_PIECES + THREADS - 1) / THREADS, STA_PER = 2 * PK;  // of each state
   u32x4 tok[TOK_PER], sta[2][STA_PER];
+  float coming[2][5];  // the scales of a step's two blocks
   auto load = [&](int step) {
+#pragma unroll
+    for (int half = 0; half < 2; ++half)
+#pragma unroll
+      for (int i = 0; i < 5; ++i) coming[half][i] = scales[i][2 * step + half];
 #pragma unroll
     for (int i = 0; i < TOK_PER; ++i) {
       const int at = i * THREADS + tid;
@@ -456,7 +462,7 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
       }
   };
   float ss_dot = 0.f;  // <dS, S_0>
-  auto store = [&](int step) {
+  auto store = [&] {
 #pragma unroll
     for (int i = 0; i < TOK_PER; ++i) {
       const int at = i * THREADS + tid;
@@ -482,9 +488,8 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
       float x = 0.f;
 #pragma unroll
       for (int e = 0; e < 8; ++e) x = fmaf((float)a[e] + (float)al[e], (float)d[e] + (float)dl[e], x);
-      const int block = 2 * step + ((((i / PK) * THREADS + tid) / (DKP / 8)) >> 4);
       int e[SUMS];
-      products(block, e);
+      products(coming[i / PK], e);  // THREADS pieces are a block
       ss_dot = fmaf(x, power(e[S_DS] - top[S_DS]), ss_dot);
     }
   };
@@ -528,14 +533,16 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   const int steps = blocks / 2;
   load(0);
   for (int step = 0; step < steps; ++step) {
-    __syncthreads();
-    store(step);
-    __syncthreads();
+    lds_barrier();
+    store();
+    float of[5];  // a lane's 8 columns are of one block
+#pragma unroll
+    for (int i = 0; i < 5; ++i) of[i] = gq >> 1 ? coming[1][i] : coming[0][i];
+    lds_barrier();
     if (step + 1 < steps) load(step + 1);
-    // a lane's 8 columns are of one block
     int factor[SUMS];
-    products(2 * step + (gq >> 1), factor);
-    const float z_scale = scales[1][2 * step + (gq >> 1)];
+    products(of, factor);
+    const float z_scale = of[1];
     _Float16 by[SUMS];
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) by[i] = (_Float16)power(factor[i] - top[i]);
@@ -618,7 +625,30 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
       }
     }
   }
-  __syncthreads();
+  // K and the wave's rows of P are on their way meanwhile
+  u32x4 image_regs[4 * PK];
+  auto bring = [&](const char* img) {
+#pragma unroll
+    for (int i = 0; i < 4 * PK; ++i) image_regs[i] = *(const u32x4*)(img + image * (PK * PLANE) + (i * THREADS + tid) * 16);
+  };
+  auto put_image = [&] {
+#pragma unroll
+    for (int i = 0; i < 4 * PK; ++i) *(u32x4*)(areaA + (i * THREADS + tid) * 16) = image_regs[i];
+  };
+  static_assert(4 * THREADS * 16 == PLANE);
+  bring(p.prep.k);
+  constexpr int ROWS = L / W;
+  f16_t ph[ROWS], pl[ROWS];
+  const f16_t* pf = p.prep.p + part * (2 * FRAG_PLANE);
+#pragma unroll
+  for (int x = 0; x < ROWS; ++x) {
+    // P's operand order: lane (i % 16) + 16 of 4 columns, halves of 16 of each 32
+    const int i = x * W + wave, j = lane;
+    const int at = (2 * (i >> 4) + (j >> 5)) * 512 + ((i & 15) + 16 * ((j >> 2) & 3)) * 8 + ((j >> 4) & 1) * 4 + (j & 3);
+    ph[x] = pf[at];
+    pl[x] = pf[at + FRAG_PLANE];
+  }
+  lds_barrier();
 
   // ---- dP, dA to LDS; K beside
 #pragma unroll
@@ -629,11 +659,9 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
 #pragma unroll
     for (int e = 0; e < 4; ++e) to[(16 * job_i[x] + 4 * gq + e) * GLD + 16 * job_j[x] + r] = ldexpf(job_mat[x] ? -jobs[x][e] : jobs[x][e], sc);
   }
-  auto bring = [&](const char* img) {
-    for (int i = tid * 16; i < PK * PLANE; i += THREADS * 16) *(u32x4*)(areaA + i) = *(const u32x4*)(img + image * (PK * PLANE) + i);
-  };
-  bring(p.prep.k);
-  __syncthreads();
+  put_image();
+  bring(p.prep.q);
+  lds_barrier();
   const float ksc = f->k, qsc = f->qs;
 #pragma unroll
   for (int x = 0; x < (10 + W - 1) / W; ++x) {
@@ -675,21 +703,18 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   };
   dots(g2, 0);  // k_i.(Z S_0^T)_i
   dots(g3, 1);  // k_j.(U dS^T)_j
-  __syncthreads();
+  lds_barrier();
 
   // ---- each pair of tokens: wave w has rows w, w + W, .., a lane a column
-  constexpr int ROWS = L / W;
   float dps[ROWS], ee[ROWS], col = 0.f, mx[2] = {0.f, 0.f};
-  const f16_t* pf = p.prep.p + part * (2 * FRAG_PLANE);
   const double bj = bs[lane];
+  const float p_scale = f->p;
 #pragma unroll
   for (int x = 0; x < ROWS; ++x) {
     const int i = x * W + wave, j = lane;
     const bool on = j <= i, below = j < i;
     const float dec = on ? exp_of(bs[i] - bj) : 0.f;
-    // P's operand order: lane (i % 16) + 16 of 4 columns, halves of 16 of each 32
-    const int at = (2 * (i >> 4) + (j >> 5)) * 512 + ((i & 15) + 16 * ((j >> 2) & 3)) * 8 + ((j >> 4) & 1) * 4 + (j & 3);
-    const float pv = on ? ((float)pf[at] + (float)pf[at + FRAG_PLANE]) * f->p : 0.f;
+    const float pv = on ? ((float)ph[x] + (float)pl[x]) * p_scale : 0.f;
     const float dp = on ? dpm[i * GLD + j] : 0.f, da = below ? dam[i * GLD + j] : 0.f, beta = betas[i];
     const float nij = below ? dec * kkm[i * GLD + j] : 0.f;
     const float bb = wave_sum_dpp(da * nij), pp = wave_sum_dpp(dp * pv);
@@ -718,7 +743,7 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
     y += __shfl_xor(y, 32, 64);
     if (gq == 0) red[4 * W * L + 16 * (wave + x * W) + r] = y;
   }
-  __syncthreads();  // dP and dA have been read: their place takes the operands
+  lds_barrier();  // dP and dA have been read: their place takes the operands
   mx[0] = mx[1] = 0.f;
 #pragma unroll
   for (int w = 0; w < W; ++w) {
@@ -743,7 +768,7 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
     if (j <= i) put(2, i, j, e);
     if (j < i) put(2, j, i, e);
   }
-  __syncthreads();
+  lds_barrier();
   auto pair_frag = [&](int mat, int pl, int mt, int s) {
     const int i = 16 * mt + r;
     return *(const f16x8*)(areaB + (pl * 3 + mat) * MAT + i * 128 + (((4 * s + gq) ^ (i & 7)) << 4));
@@ -784,9 +809,9 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   for (int t = 0; t < 2; ++t)
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) acck[t][mt] *= ku / qu;
-  __syncthreads();
-  bring(p.prep.q);
-  __syncthreads();
+  lds_barrier();
+  put_image();
+  lds_barrier();
   add(acck, 1);
   dots(g1, 3);  // q_i.(dH S_0^T)_i
   // ---- out
@@ -825,7 +850,7 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
       }
     }
   }
-  __syncthreads();
+  lds_barrier();
   // ---- the gates, a lane a token
   if (wave != 0) return;
   float kz = 0.f, ks = 0.f, qd = 0.f, cl = 0.f, dss = 0.f;
