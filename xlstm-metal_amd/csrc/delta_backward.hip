@@ -376,8 +376,9 @@ struct GradLds {
 };
 
 // DKB waves: a wave has 32 of DQK's columns of dQ and dK, turned (columns down, tokens across), and its share of the 64 x 64 tiles.
+// At DQK 128 two workgroups fit a CU with 256 registers a lane (16-bit types: 167 us at 8192 tokens, 187 without; float32 would spill).
 template <typename T, int DKB>
-__global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
+__global__ __launch_bounds__(64 * DKB, DKB == 4 && !is_f32<T>::value ? 2 : 1) void delta_grad_kernel(GradArgs p) {
   using Lds = GradLds<T, DKB>;
   constexpr int PK = Lds::PK, DKP = Lds::DKP, PLANE = L * DKP * 2, TOK = Lds::TOK, STA = Lds::STA, W = DKB, THREADS = 64 * W;
   constexpr bool PAIR = !std::is_same_v<T, bf16_t>;
@@ -437,6 +438,26 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
   constexpr int TOK_PIECES = 3 * PK * 256, TOK_PER = (TOK_PIECES + THREADS - 1) / THREADS, STA_PER = 2 * PK;  // of each state
   u32x4 tok[TOK_PER], sta[2][STA_PER];
   float coming[2][5];  // the scales of a step's two blocks
+  // V of a token and 8 neighbours: wave w has tokens 16 w + r (and 16 (w + 2) + r where there are two)
+  constexpr int MTS = 4 / (W < 4 ? W : 4);
+  struct alignas(16) Eight { T e[8]; };
+  Eight v8[MTS];
+  const T* vrow = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
+  T* dvrow = (T*)p.dv + (int64_t)bh * p.S * p.DV;
+  auto load_v = [&](int step) {
+    if (wave >= 4) return;
+#pragma unroll
+    for (int x = 0; x < MTS; ++x) {
+      const int t = t0 + 16 * (wave + x * W) + r, n = 32 * step + 8 * gq;
+      const T* from = vrow + (t < p.S ? t : p.S - 1) * p.vs[2] + n;
+      if (p.wide_v && n + 8 <= p.DV) {
+        v8[x] = *(const Eight*)from;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v8[x].e[e] = n + e < p.DV ? from[e] : from_f32<T>(0.f);
+      }
+    }
+  };
   auto load = [&](int step) {
 #pragma unroll
     for (int half = 0; half < 2; ++half)
@@ -525,13 +546,11 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
     job_i[x] = i;
     job_j[x] = tile - i * (i + 1) / 2;
   }
-  float zv[4 / (W < 4 ? W : 4)] = {};  // Z.V of tokens 16 mt + r
-  constexpr int MTS = 4 / (W < 4 ? W : 4);
-  const T* vrow = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
-  T* dvrow = (T*)p.dv + (int64_t)bh * p.S * p.DV;
+  float zv[MTS] = {};  // Z.V of tokens 16 mt + r
 
   const int steps = blocks / 2;
   load(0);
+  load_v(0);
   for (int step = 0; step < steps; ++step) {
     lds_barrier();
     store();
@@ -539,10 +558,42 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
 #pragma unroll
     for (int i = 0; i < 5; ++i) of[i] = gq >> 1 ? coming[1][i] : coming[0][i];
     lds_barrier();
-    if (step + 1 < steps) load(step + 1);
+    // dV = beta Z, and Z.V: a lane has 8 neighbours of a token
+    if (wave < 4) {
+#pragma unroll
+      for (int x = 0; x < MTS; ++x) {
+        const int mt = wave + x * W, t = t0 + 16 * mt + r, n = 32 * step + 8 * gq;
+        const f16x8 z = tok_frag(1, 0, mt);
+        f16x8 zl = {};
+        if constexpr (PK == 2) zl = tok_frag(1, 1, mt);
+        if (t < p.S) {
+          float zf[8];
+#pragma unroll
+          for (int e = 0; e < 8; ++e) zf[e] = ((float)z[e] + (float)zl[e]) * of[1];
+          const float beta = betas[16 * mt + r];
+          T* to = dvrow + (int64_t)t * p.DV + n;
+          Eight o;
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            zv[x] = fmaf(zf[e], to_f32(v8[x].e[e]), zv[x]);
+            o.e[e] = from_f32<T>(beta * zf[e]);
+          }
+          if (p.wide_v && n + 8 <= p.DV) {
+            *(Eight*)to = o;
+          } else {
+#pragma unroll
+            for (int e = 0; e < 8; ++e)
+              if (n + e < p.DV) to[e] = o.e[e];
+          }
+        }
+      }
+    }
+    if (step + 1 < steps) {
+      load(step + 1);
+      load_v(step + 1);
+    }
     int factor[SUMS];
     products(of, factor);
-    const float z_scale = of[1];
     _Float16 by[SUMS];
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) by[i] = (_Float16)power(factor[i] - top[i]);
@@ -587,42 +638,6 @@ __global__ __launch_bounds__(64 * DKB) void delta_grad_kernel(GradArgs p) {
         jobs[x] = mfma(a, tok_frag(2, 1, job_j[x]) * share, jobs[x]);
       }
       jobs[x] = mfma(a, u, jobs[x]);
-    }
-    // dV = beta Z, and Z.V: a lane has 8 neighbours of a token
-    if (wave < 4) {
-#pragma unroll
-      for (int x = 0; x < MTS; ++x) {
-        const int mt = wave + x * W, t = t0 + 16 * mt + r, n = 32 * step + 8 * gq;
-        const f16x8 z = tok_frag(1, 0, mt);
-        f16x8 zl = {};
-        if constexpr (PK == 2) zl = tok_frag(1, 1, mt);
-        if (t < p.S) {
-          float zf[8];
-#pragma unroll
-          for (int e = 0; e < 8; ++e) zf[e] = ((float)z[e] + (float)zl[e]) * z_scale;
-          const float beta = betas[16 * mt + r];
-          const T* from = vrow + t * p.vs[2] + n;
-          T* to = dvrow + (int64_t)t * p.DV + n;
-          struct alignas(16) Eight { T e[8]; };
-          if (p.wide_v && n + 8 <= p.DV) {
-            const Eight v = *(const Eight*)from;
-            Eight o;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-              zv[x] = fmaf(zf[e], to_f32(v.e[e]), zv[x]);
-              o.e[e] = from_f32<T>(beta * zf[e]);
-            }
-            *(Eight*)to = o;
-          } else {
-#pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (n + e < p.DV) {
-                zv[x] = fmaf(zf[e], to_f32(from[e]), zv[x]);
-                to[e] = from_f32<T>(beta * zf[e]);
-              }
-          }
-        }
-      }
     }
   }
   // K and the wave's rows of P are on their way meanwhile
