@@ -62,6 +62,25 @@ def test_step(gpu_case, B, NH, NHK, DQK, DV, dtype, gate):
     assert c2 is x[5] and torch.equal(h, h2) and torch.equal(c, c2)
 
 
+# many heads: the decode step's own kernels, by their widths, rows and ragged columns
+@pytest.mark.parametrize("B,NH,NHK,DQK,DV", [(32, 8, 8, 128, 256), (64, 8, 4, 256, 512), (32, 8, 8, 100, 256), (64, 4, 1, 64, 64),
+                                             (40, 8, 8, 33, 100), (64, 4, 4, 200, 196), (64, 4, 4, 1, 4)])
+@pytest.mark.parametrize("dtype,gate", [(BF16, F32), (F16, F16), (F32, F32)])
+def test_step_of_many_heads(gpu_case, B, NH, NHK, DQK, DV, dtype, gate):
+    test_step(gpu_case, B, NH, NHK, DQK, DV, dtype, gate)
+
+
+# many blocks of columns: the scans' form of one wave a block
+MANY = [(32, 8, 8, 70, 64, 64), (16, 8, 4, 130, 128, 100), (32, 8, 8, 65, 256, 40), (8, 16, 16, 64, 200, 128)]
+
+
+@pytest.mark.parametrize("shape", MANY)
+@pytest.mark.parametrize("dtype,gate", [(BF16, F32), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("state", [False, True])
+def test_chunkwise_of_many_heads(gpu_case, shape, dtype, gate, state):
+    test_chunkwise(gpu_case, shape, dtype, gate, state)
+
+
 def test_step_on_an_odd_address(gpu_case):
     import xlstm_hip
     x = make(2, 2, 2, 1, 64, 32, BF16, BF16, seed=3)

@@ -106,6 +106,13 @@ def test_gradients(gpu_case, shape, dtype, gate, state, last):
     check_all(*inputs(shape, dtype, gate, sum(shape), state, last))
 
 
+# many blocks of columns: the scans' form of one wave a block
+@pytest.mark.parametrize("shape", [(32, 8, 8, 70, 64, 64), (16, 8, 4, 130, 128, 100), (32, 8, 8, 65, 256, 40)])
+@pytest.mark.parametrize("dtype,gate", [(BF16, BF16), (F16, F16), (F32, F32)])
+def test_gradients_of_many_heads(gpu_case, shape, dtype, gate):
+    check_all(*inputs(shape, dtype, gate, sum(shape), True, True))
+
+
 def test_last_state_alone(gpu_case):
     x, _, dc = inputs((1, 2, 2, 100, 64, 32), F32, F32, 3)
     check_all(x, None, dc)

@@ -4,8 +4,8 @@
 //
 // A workgroup takes 32 columns of a head's state through all tokens, in float32 registers: 4 waves x 8 lane groups share
 // the rows, a lane holds 4 columns of every 32nd row.  S^T k and S^T q of the state before the token are summed
-// together (h = scale (a S^T q + (q.k) d)), so a token costs one reduction and one barrier.  One token is bound by the state's
-// bytes, in and out once.
+// together (h = scale (a S^T q + (q.k) d)), so a token costs one reduction and one barrier; the next token's values are on their way
+// meanwhile.  One token of many heads is bound by the state's bytes, in and out once, and has a kernel of its own.
 #include "delta.h"
 
 namespace xl {
@@ -13,6 +13,7 @@ namespace delta {
 namespace {
 
 constexpr int COLS = 32, RWAVES = 4;
+static_assert(MAX_DQK == 64 * RWAVES);  // a thread for each value of q and k
 
 struct RecArgs {
   const void *q, *k, *v, *g, *beta;
@@ -23,6 +24,15 @@ struct RecArgs {
   float scale;
   bool wide;  // 16-byte accesses to the state
 };
+
+// x + what the lanes 8, 16 and 32 away have: the sum over a wave's 8 row groups
+__device__ __forceinline__ float sum_groups(float x) {
+  x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));  // row_ror:8
+  const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = __uint_as_float(y[0]) + __uint_as_float(y[1]);
+  const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return __uint_as_float(z[0]) + __uint_as_float(z[1]);
+}
 
 template <typename T, typename G, int NI>
 __global__ __launch_bounds__(256) void delta_recurrent_kernel(RecArgs p) {
@@ -59,32 +69,51 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(RecArgs p) {
       }
     }
   }
-  float qn = 0.f, kn = 0.f;  // thread tid has value tid of the next token's q and k
-  if (tid < p.DK && p.S > 0) {
-    qn = to_f32(q[tid]);
-    kn = to_f32(k[tid]);
+  // Thread tid has value tid of a token's q and k.  What is loaded past the last token or value is the last one's.  No branch around a load: the compiler would wait for it at the branch's end.
+  const int dc = tid < p.DK ? tid : p.DK - 1;
+  T qn{}, kn{};
+  auto load_qk = [&](int t) {
+    const int64_t at = (int64_t)(t < p.S ? t : p.S - 1) * p.DK + dc;
+    qn = q[at];
+    kn = k[at];
+  };
+  if (p.S > 0) {
+    load_qk(0);
+    qk_s[0][0][tid] = to_f32(qn);
+    qk_s[0][1][tid] = to_f32(kn);
+    load_qk(1);
   }
-  if (tid < MAX_DQK) {
-    qk_s[0][0][tid] = qn;
-    qk_s[0][1][tid] = kn;
-  }
-  __syncthreads();
+  T vn[4];
+  G gn{}, bn{};
+  int vcol[4];
+#pragma unroll
+  for (int e = 0; e < 4; ++e) vcol[e] = col + e < p.DV ? col + e : p.DV - 1;
+  auto load = [&](int t) {
+    t = t < p.S ? t : p.S - 1;
+    gn = gp[t];
+    bn = bp[t];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) vn[e] = v[(int64_t)t * p.DV + vcol[e]];
+  };
+  if (p.S > 0) load(0);
+  lds_barrier();
   for (int t = 0; t < p.S; ++t) {
     const int at = t & 1;
-    if (t + 1 < p.S && tid < p.DK) {
-      qn = to_f32(q[(int64_t)(t + 1) * p.DK + tid]);
-      kn = to_f32(k[(int64_t)(t + 1) * p.DK + tid]);
-    }
-    const float a = expf(to_f32(gp[t])), beta = to_f32(bp[t]);
+    const float a = expf(to_f32(gn)), beta = to_f32(bn);
     float vt[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) vt[e] = col + e < p.DV ? to_f32(v[(int64_t)t * p.DV + col + e]) : 0.f;
+    for (int e = 0; e < 4; ++e) vt[e] = to_f32(vn[e]);
+    qk_s[at ^ 1][0][tid] = to_f32(qn);  // the next token's, read a token ago
+    qk_s[at ^ 1][1][tid] = to_f32(kn);
+    load(t + 1);
+    load_qk(t + 2);
     f32x4 ks = {0.f, 0.f, 0.f, 0.f}, qs = {0.f, 0.f, 0.f, 0.f};
     float kk[NI], dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const float qi = qk_s[at][0][row0 + 32 * i];
-      kk[i] = qk_s[at][1][row0 + 32 * i];
+      const bool there = row0 + 32 * i < p.DK;
+      const float qi = there ? qk_s[at][0][row0 + 32 * i] : 0.f;
+      kk[i] = there ? qk_s[at][1][row0 + 32 * i] : 0.f;
       dot = fmaf(qi, kk[i], dot);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -93,24 +122,17 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(RecArgs p) {
       }
     }
 #pragma unroll
-    for (int o = 8; o < 64; o <<= 1) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        ks[e] += __shfl_xor(ks[e], o, 64);
-        qs[e] += __shfl_xor(qs[e], o, 64);
-      }
-      dot += __shfl_xor(dot, o, 64);
+    for (int e = 0; e < 4; ++e) {
+      ks[e] = sum_groups(ks[e]);
+      qs[e] = sum_groups(qs[e]);
     }
+    dot = sum_groups(dot);
     if (lane < 8) {
       *(f32x4*)&sums[at][wave][0][lane * 4] = ks;
       *(f32x4*)&sums[at][wave][1][lane * 4] = qs;
       if (lane == 0) dots[at][wave] = dot;
     }
-    if (tid < MAX_DQK) {
-      qk_s[at ^ 1][0][tid] = qn;
-      qk_s[at ^ 1][1][tid] = kn;
-    }
-    __syncthreads();
+    lds_barrier();
     ks = qs = f32x4{0.f, 0.f, 0.f, 0.f};
     dot = 0.f;
 #pragma unroll
@@ -146,6 +168,97 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(RecArgs p) {
         if (col + e < p.DV) to[e] = st[i][e];
     }
   }
+}
+
+// One token of many heads: 1024 threads a workgroup, COLS columns (256: a wave reads whole KBs of a row), every thread's rows read
+// before the first is written.  S^T k and S^T q are summed over a thread's rows, then over the row groups in LDS.
+constexpr int STEP_THREADS = 1024;
+
+template <typename T, typename G, int COLS, int DKP>
+__global__ __launch_bounds__(STEP_THREADS) void delta_step_kernel(RecArgs p) {
+  constexpr int CG = COLS / 4, RG = STEP_THREADS / CG, RPT = DKP / RG, LANES = STEP_THREADS / COLS;
+  static_assert(RG == 4 * LANES && DKP % RG == 0);
+  __shared__ float q_s[DKP], k_s[DKP], sums[2][RG][COLS + 4], d_s[COLS], dots[STEP_THREADS / 64];
+  const int tid = threadIdx.x, tiles = (p.DV + COLS - 1) / COLS;
+  const int bh = uniform(blockIdx.x / tiles), tile = blockIdx.x - bh * tiles, b = uniform(bh / p.NH), h = bh - b * p.NH;
+  const int64_t bhk = (int64_t)b * uniform(p.NH / p.group) + uniform(h / p.group);
+  const int cg = tid % CG, rg = tid / CG, col = tile * COLS + cg * 4, colc = col < p.DV ? col : 0;
+  // the small values first, then the rows (past DQK: row 0 again, against zeros), all under way at once
+  const G graw = ((const G*)p.g)[bh], braw = ((const G*)p.beta)[bh];
+  const int d0 = tid < p.DK ? tid : 0;
+  const T qraw = ((const T*)p.q)[bhk * p.DK + d0], kraw = ((const T*)p.k)[bhk * p.DK + d0];
+  const int own = tile * COLS + tid / LANES;  // the column that this thread helps to sum
+  const T vraw = ((const T*)p.v)[(int64_t)bh * p.DV + (own < p.DV ? own : 0)];
+  asm volatile("" ::: "memory");
+  const int64_t state = (int64_t)bh * p.DK * p.DV + colc;
+  f32x4 st[RPT];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = rg + RG * i;
+    st[i] = __builtin_nontemporal_load((const f32x4*)(p.c0 + state + (int64_t)(r < p.DK ? r : 0) * p.DV));
+  }
+  const float qv = tid < p.DK ? to_f32(qraw) : 0.f, kv = tid < p.DK ? to_f32(kraw) : 0.f;
+  if (tid < DKP) {
+    q_s[tid] = qv;
+    k_s[tid] = kv;
+  }
+  const float part = wave_sum(qv * kv);
+  if ((tid & 63) == 0) dots[tid >> 6] = part;
+  const float a = expf(to_f32(graw)), beta = to_f32(braw);
+  lds_barrier();
+  float kk[RPT];
+  f32x4 ks = {0.f, 0.f, 0.f, 0.f}, qs = ks;
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    kk[i] = k_s[rg + RG * i];
+    const float qi = q_s[rg + RG * i];
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      ks[e] = fmaf(kk[i], st[i][e], ks[e]);
+      qs[e] = fmaf(qi, st[i][e], qs[e]);
+    }
+  }
+  *(f32x4*)&sums[0][rg][cg * 4] = ks;
+  *(f32x4*)&sums[1][rg][cg * 4] = qs;
+  lds_barrier();
+  {
+    const int c = tid / LANES, l = tid % LANES;
+    float x[2];
+#pragma unroll
+    for (int m = 0; m < 2; ++m) {
+      x[m] = (sums[m][l][c] + sums[m][l + LANES][c]) + (sums[m][l + 2 * LANES][c] + sums[m][l + 3 * LANES][c]);
+#pragma unroll
+      for (int o = 1; o < LANES; o <<= 1) x[m] += __shfl_xor(x[m], o, 64);
+    }
+    if (l == 0 && own < p.DV) {
+      float dot = 0.f;
+#pragma unroll
+      for (int w = 0; w < (DKP + 63) / 64; ++w) dot += dots[w];
+      const float d = beta * (to_f32(vraw) - a * x[0]);
+      d_s[c] = d;
+      ((T*)p.h)[(int64_t)bh * p.DV + own] = from_f32<T>(p.scale * fmaf(dot, d, a * x[1]));
+    }
+  }
+  lds_barrier();
+  if (col >= p.DV) return;
+  const f32x4 d = *(const f32x4*)&d_s[cg * 4];
+#pragma unroll
+  for (int i = 0; i < RPT; ++i) {
+    const int r = rg + RG * i;
+    if (r >= p.DK) continue;
+    f32x4 x;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) x[e] = fmaf(kk[i], d[e], a * st[i][e]);
+    __builtin_nontemporal_store(x, (f32x4*)(p.c_last + state + (int64_t)r * p.DV));
+  }
+}
+
+template <typename T, typename G, int COLS>
+const void* pick_step(int DK) {
+  if constexpr (COLS == 64)
+    return DK <= 64 ? (const void*)delta_step_kernel<T, G, COLS, 64> : DK <= 128 ? (const void*)delta_step_kernel<T, G, COLS, 128>
+                                                                                : (const void*)delta_step_kernel<T, G, COLS, 256>;
+  return DK <= 128 ? (const void*)delta_step_kernel<T, G, 256, 128> : (const void*)delta_step_kernel<T, G, 256, 256>;
 }
 
 template <typename T, typename G>
@@ -196,17 +309,29 @@ int launch_recurrent(const Shape& s, const void* q, const void* k, const void* v
                      const float* c0, void* h, float* c_last, hipStream_t st, const char* who) {
   RecArgs a{q, k, v, g, beta, c0, h, c_last, s.NH, s.NH / s.NHK, s.S, s.DK, s.DV, s.scale, false};
   a.wide = s.DV % 4 == 0 && (((uintptr_t)c0 | (uintptr_t)c_last) & 15) == 0;
+  // One token: 1 KB rows where that gives every CU a workgroup, else 256-byte ones, else the kernel of several tokens (us, bf16, 256 x
+  // 512 states: 128 heads 25 and 40, 8 heads STEP8).
+  const int64_t heads = (int64_t)s.B * s.NH;
+  const bool one = s.S == 1 && c0 && c_last && a.wide;
+  const int cols = one && s.DV % 256 == 0 && heads * (s.DV / 256) >= 256 ? 256 : one && heads * ((s.DV + 63) / 64) >= 256 ? 64 : 0;
   const void* kern = nullptr;
   auto with_gate = [&](auto t) {
     using T = decltype(t);
-    kern = s.dtype_gates == XL_DTYPE_F32 ? pick<T, float>(s.DK) : s.dtype_gates == XL_DTYPE_BF16 ? pick<T, bf16_t>(s.DK) : pick<T, f16_t>(s.DK);
+    auto of = [&](auto g) {
+      using G = decltype(g);
+      kern = cols == 256 ? pick_step<T, G, 256>(s.DK) : cols == 64 ? pick_step<T, G, 64>(s.DK) : pick<T, G>(s.DK);
+    };
+    if (s.dtype_gates == XL_DTYPE_F32) of(float{});
+    else if (s.dtype_gates == XL_DTYPE_BF16) of(bf16_t{});
+    else of(f16_t{});
   };
   if (s.dtype == XL_DTYPE_F32) with_gate(float{});
   else if (s.dtype == XL_DTYPE_BF16) with_gate(bf16_t{});
   else with_gate(f16_t{});
-  const unsigned grid = (unsigned)((int64_t)s.B * s.NH * ((s.DV + COLS - 1) / COLS));
+  const int width = cols ? cols : COLS;
+  const unsigned grid = (unsigned)(heads * ((s.DV + width - 1) / width));
   void* args[] = {&a};
-  const hipError_t e = hipLaunchKernel(kern, dim3(grid), dim3(256), args, 0, st);
+  const hipError_t e = hipLaunchKernel(kern, dim3(grid), dim3(cols ? STEP_THREADS : 256), args, 0, st);
   if (e != hipSuccess) return set_error(XL_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
   return check_launch(who);
 }
