@@ -94,6 +94,17 @@ def test_large_tiles(gpu_case, T, D, F):
         check(g, v, bar, name)
 
 
+@pytest.mark.parametrize("T,D,F", [(70, 136, 2731), (5, 264, 5504), (777, 512, 5504), (4200, 72, 130), (2500, 200, 1025), (4096, 512, 256)])
+@pytest.mark.parametrize("dtype", [BF16, F16])
+def test_sums_in_parts(gpu_case, T, D, F, dtype):
+    """Few tiles and a long sum: dx over the features, the weights' over the tokens, in parts that do not divide their slices."""
+    x, wg, wu, dh = inputs(T, D, F, dtype, T + 1)
+    first = run(x, wg, wu, dh)
+    for g, (v, bar), name in zip(first, reference(x, wg, wu, dh, "silu"), NAMES):
+        check(g, v, bar, name)
+    assert all(torch.equal(a, b) for a, b in zip(first, run(x, wg, wu, dh)))
+
+
 @pytest.mark.parametrize("M", [1, 2, 7, 8, 15, 16])
 @pytest.mark.parametrize("D,F", [(4096, 1000), (24, 17), (2048, 5504)])
 @pytest.mark.parametrize("dtype", [BF16, F16])

@@ -4,9 +4,10 @@
 //   da = dh u act'(a),  du = dh act(a),  dx = da Wg + du Wu,  dWg = da^T x,  dWu = du^T x
 //
 // The forward is one product of x with both weights: a tile holds the same rows of Wg and of Wu, a wave has a and u of the
-// same values in its registers, and only h goes to memory (for training a and u too, in float32: the gradients' factors keep their
-// bits).  Backward: da and du once, zero-padded to whole slices; dx as one product over both weights' rows; the weights'
-// gradients as one launch of two.  Up to 16 tokens the weights are streamed past them instead.
+// same values in its registers, and only h goes to memory (for training a and u too, in float32: the gradients' factors
+// keep their bits).  Backward: da and du once, zero-padded to whole slices; dx as one product over both weights' rows; the
+// weights' gradients as one launch of two; both in parts of K where tiles are few.  Up to 16 tokens the weights are streamed
+// past them instead.
 //
 // Products: 16 x 16 blocks of v_mfma_f32_16x16x32, sums in registers; slices of 64 of K of both operands in LDS, STAGES of
 // them, filled straight from memory STAGES - 1 ahead; a wave holds the operands of 32 of a slice's 64 and multiplies them
@@ -15,6 +16,7 @@
 // that transpose.  The loads write LDS in lane order, so each lane fetches what belongs at its place.
 #include <math.h>
 
+#include <algorithm>
 #include <type_traits>
 
 #include "common.h"
@@ -31,6 +33,7 @@ typedef __attribute__((address_space(3))) char lds_char;
 
 enum Act { SILU = 0, GELU = 1 };
 enum Product { FWD, DX, DW };  // h; dx; dWg and dWu
+enum Part { WHOLE, PART, JOIN };  // a tile; a part of its sum over K; the tile from its parts, added in order
 
 template <typename T>
 __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
@@ -99,9 +102,11 @@ struct Args {
   int64_t keep_pitch;
   int act;
   bool wide;  // 16-byte stores of out
+  int splits;      // parts of K
+  float* partial;  // their sums, by [tile][part]
 };
 
-template <int BL, int BR, int WL, int WR, int STAGES, int MODE, typename T>
+template <int BL, int BR, int WL, int WR, int STAGES, int MODE, int PARTS, typename T>
 __global__ __launch_bounds__(64 * WL * WR) void glu_product_kernel(Args p) {
   constexpr int THREADS = 64 * WL * WR, BK = 64, TL = BL / WL / 16, TR = BR / WR / 16;
   constexpr bool LC = MODE != FWD, RC = MODE == DW;  // by columns
@@ -116,7 +121,8 @@ __global__ __launch_bounds__(64 * WL * WR) void glu_product_kernel(Args p) {
   const int wl = wave / WR, wr = wave % WR;
 
   // neighbours share operands, on one XCD
-  const int tiles = p.left_tiles * p.right_tiles, all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
+  const int tiles = p.left_tiles * p.right_tiles, job = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
+  const int all = PARTS == PART ? __builtin_amdgcn_readfirstlane(job / p.splits) : job, split = PARTS == PART ? job - all * p.splits : 0;
   const int b = __builtin_amdgcn_readfirstlane(all / tiles), t = all - b * tiles;
   constexpr int G = 4;
   const int group = t / (G * p.left_tiles), rows = min(G, p.right_tiles - group * G), in = t - group * G * p.left_tiles;
@@ -158,7 +164,9 @@ __global__ __launch_bounds__(64 * WL * WR) void glu_product_kernel(Args p) {
     for (int i = 0; i < BR / PER; ++i)
       from_r[i] = (uint32_t)(min(i * PER + (tid >> 3), p.rights - 1 - br * BR) * lr + piece);
   }
-  const int per_weight = (p.K + BK - 1) / BK, slices = MODE == DX ? 2 * per_weight : per_weight;
+  const int per_weight = (p.K + BK - 1) / BK, whole = MODE == DX ? 2 * per_weight : per_weight;
+  const int first = PARTS == PART ? __builtin_amdgcn_readfirstlane((int)((int64_t)whole * split / p.splits)) : 0;
+  const int slices = PARTS == PART ? __builtin_amdgcn_readfirstlane((int)((int64_t)whole * (split + 1) / p.splits)) : whole;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds + wave * 1024;
   auto fetch_one = [&](auto I, int slice, int stage) {
     constexpr int i = I.value;
@@ -241,24 +249,41 @@ __global__ __launch_bounds__(64 * WL * WR) void glu_product_kernel(Args p) {
   // Past the end the last slice is loaded again, and read, but not multiplied: the same number of loads is under way after
   // every slice.
   using Behind = std::integral_constant<int, LOADS*(STAGES - 2)>;
-  Half h0, h1;
+  // a lane's sums of a part: one f32x4 a block, the workgroup's side by side
+  auto part_at = [&](int of, int at) { return (f32x4*)p.partial + (((int64_t)all * p.splits + of) * (TL * TR) + at) * THREADS + tid; };
+  if constexpr (PARTS == JOIN) {
+    for (int of = 0; of < p.splits; ++of)
 #pragma unroll
-  for (int k = 0; k < STAGES - 1; ++k)
-    mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(k, slices - 1), k); });
-  landed(Behind{});
-  mfma::static_for<0, READS>([&](auto R) { read_one(R, h0, 0, 0); });
-  mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(STAGES - 1, slices - 1), STAGES - 1); });
-  int stage = 0;
-  for (int k = 0; k < slices; ++k) {
-    const int next = stage + 1 == STAGES ? 0 : stage + 1, ahead = min(k + STAGES, slices - 1);
-    multiply(h0, h1, stage * STAGE, 1, [](auto) {});
-    landed(Behind{});  // slice k + 1 is there, slice k has been read
-    multiply(h1, h0, next * STAGE, 0, [&](auto I) {
-      mfma::static_for<LOADS * I.value / TL, LOADS * (I.value + 1) / TL>([&](auto X) { fetch_one(X, ahead, stage); });
-    });
-    stage = next;
+      for (int i = 0; i < TL; ++i)
+#pragma unroll
+        for (int j = 0; j < TR; ++j) acc[i][j] += *part_at(of, i * TR + j);
+  } else {
+    Half h0, h1;
+#pragma unroll
+    for (int k = 0; k < STAGES - 1; ++k)
+      mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(first + k, slices - 1), k); });
+    landed(Behind{});
+    mfma::static_for<0, READS>([&](auto R) { read_one(R, h0, 0, 0); });
+    mfma::static_for<0, LOADS>([&](auto I) { fetch_one(I, min(first + STAGES - 1, slices - 1), STAGES - 1); });
+    int stage = 0;
+    for (int k = first; k < slices; ++k) {
+      const int next = stage + 1 == STAGES ? 0 : stage + 1, ahead = min(k + STAGES, slices - 1);
+      multiply(h0, h1, stage * STAGE, 1, [](auto) {});
+      landed(Behind{});  // slice k + 1 is there, slice k has been read
+      multiply(h1, h0, next * STAGE, 0, [&](auto I) {
+        mfma::static_for<LOADS * I.value / TL, LOADS * (I.value + 1) / TL>([&](auto X) { fetch_one(X, ahead, stage); });
+      });
+      stage = next;
+    }
+    landed(std::integral_constant<int, 0>{});
   }
-  landed(std::integral_constant<int, 0>{});
+  if constexpr (PARTS == PART) {
+#pragma unroll
+    for (int i = 0; i < TL; ++i)
+#pragma unroll
+      for (int j = 0; j < TR; ++j) *part_at(split, i * TR + j) = acc[i][j];
+    return;
+  }
 
   // A lane has left 4 quad .. 4 quad + 3 of right `row` of each block: 16 rows at a time, turned in the wave's own part of LDS
   constexpr int OUT = MODE == FWD ? TL / 2 : TL, LDW = OUT * 16 + 4, EACH = OUT * 2;
@@ -414,42 +439,101 @@ unsigned grid_of(int64_t count) {
   return (unsigned)(n < 16384 ? n : 16384);
 }
 
-template <int BL, int BR, int WL, int WR, int STAGES, int MODE, typename T>
-int launch_tiles(Args a, const char* who, hipStream_t st) {
+template <int BL, int BR, int WL, int WR, int STAGES, int MODE, int PARTS, typename T>
+int launch_part(const Args& a, const char* who, hipStream_t st) {
   constexpr int TL = BL / WL / 16, OUT = MODE == FWD ? TL / 2 : TL;
-  constexpr int STRIPS = WL * WR * 16 * (OUT * 16 + 4) * 4, SLICES = STAGES * (BL + BR) * 128, LDS = SLICES > STRIPS ? SLICES : STRIPS;
+  constexpr int STRIPS = WL * WR * 16 * (OUT * 16 + 4) * 4, SLICES = PARTS == JOIN ? 0 : STAGES * (BL + BR) * 128;
+  constexpr int LDS = SLICES > STRIPS ? SLICES : STRIPS;
   static_assert(LDS <= 160 * 1024);
-  auto kernel = glu_product_kernel<BL, BR, WL, WR, STAGES, MODE, T>;
+  auto kernel = glu_product_kernel<BL, BR, WL, WR, STAGES, MODE, PARTS, T>;
   if (LDS > 64 * 1024) {
     const hipError_t e = hipFuncSetAttribute((const void*)kernel, hipFuncAttributeMaxDynamicSharedMemorySize, LDS);
     if (e != hipSuccess) return set_error(XL_ERR_LAUNCH, "%s: %s", who, hipGetErrorString(e));
   }
-  constexpr int LEFT = MODE == FWD ? BL / 2 : BL;
-  a.left_tiles = (a.lefts + LEFT - 1) / LEFT;
-  a.right_tiles = (a.rights + BR - 1) / BR;
-  const int64_t tiles = (int64_t)a.left_tiles * a.right_tiles * (MODE == DW ? 2 : 1);
+  const int64_t tiles = (int64_t)a.left_tiles * a.right_tiles * (MODE == DW ? 2 : 1) * (PARTS == PART ? a.splits : 1);
   if (tiles > 0x7fffffff) return set_error(XL_ERR_UNSUPPORTED, "%s: too many tiles", who);
   hipLaunchKernelGGL(kernel, dim3((unsigned)tiles), dim3(64 * WL * WR), LDS, st, a);
   return check_launch(who);
 }
 
+// Tiles: the cheapest by the rounds of the chip that they take, us a slice of K and round, and what a round costs besides (its first
+// loads, its end).  Measured, whole products in us: 777 tokens of 2048 to 5504, h: 256 x 192 46, 256 x 256 53, 128 x 128 63, 64 x 64
+// 75; 1333 of 1000 to 2731: 128 x 128 29, 256 x 192 32, 256 x 256 37; 300 of 1024 to 2752: 64 x 64 10, 128 x 128 14; 128 of 4096 to
+// 10944: 128 x 128 in four stages 43, in two 57, 64 x 64 47; 8192 of those: 256 x 256 1127, 256 x 192 1239, 128 x 128 1512.  (256 x 128,
+// 128 x 256, 128 x 64 and 256 x 64 were nowhere better by more than 10 %.)
+enum Tile { T256, T192, T128_2, T128_4, T64, TILES };
+struct Shape {
+  int bl, br;
+  double slice, round;
+};
+constexpr Shape SHAPES[TILES] = {{256, 256, 1.6, 5.0}, {256, 192, 1.28, 4.5}, {128, 128, 0.57, 2.5}, {128, 128, 0.52, 3.0}, {64, 64, 0.215, 2.0}};
+
+// A product's tile and the parts of its K.  A sum over many slices of few tiles is split, its parts kept in float32 and joined by a
+// second launch: 4 us, what it writes and reads, and 25 bytes a ns that one workgroup reads.  Measured with da and du, us: dx of 777
+// tokens of 2048 to 5504 87 whole, 72 in two parts of 128 x 128; of 128 tokens of 4096 to 10944 101 and 54; of 64 of 2048 to 5504 57 and
+// 21.  h has two sums a tile and long K only with many tiles: whole.
+struct Plan {
+  int tile = T64, splits = 1;
+  int64_t tiles = 0;
+  size_t partial() const { return splits > 1 ? (size_t)tiles * splits * SHAPES[tile].bl * SHAPES[tile].br * 4 : 0; }
+};
+Plan plan(int mode, int64_t lefts, int64_t rights, int64_t K) {
+  const int64_t whole = (K + 63) / 64 * (mode == DX ? 2 : 1);
+  Plan best;
+  double least = INFINITY;
+  for (int tile = 0; tile < TILES; ++tile) {
+    if (tile == T192 && mode != FWD) continue;
+    const Shape& s = SHAPES[tile];
+    const int64_t l = mode == FWD ? s.bl / 2 : s.bl, tiles = (lefts + l - 1) / l * ((rights + s.br - 1) / s.br) * (mode == DW ? 2 : 1);
+    for (int splits = 1; splits <= (mode == FWD ? 1 : 8); ++splits) {
+      if (splits > 1 && whole < 8 * splits) break;
+      const int64_t rounds = (tiles * splits + CUS - 1) / CUS, slices = (whole + splits - 1) / splits;
+      if (tile == T128_4 && rounds > 1) continue;
+      double us = rounds * (slices * s.slice + s.round);
+      if (tile == T128_2 && rounds == 1) us += slices * 0.1;
+      if (splits > 1) us += 4.0 + std::max((double)tiles * splits * s.bl * s.br * 8 / 4.5e6, (double)splits * s.bl * s.br * 4 / 25e3);
+      if (us < least) {
+        least = us;
+        best.tile = tile;
+        best.splits = splits;
+        best.tiles = tiles;
+      }
+    }
+  }
+  return best;
+}
+
+template <int BL, int BR, int WL, int WR, int STAGES, int MODE, typename T>
+int launch_tiles(Args a, const char* who, hipStream_t st) {
+  constexpr int LEFT = MODE == FWD ? BL / 2 : BL;
+  a.left_tiles = (a.lefts + LEFT - 1) / LEFT;
+  a.right_tiles = (a.rights + BR - 1) / BR;
+  if constexpr (MODE != FWD) {
+    if (a.splits > 1) {
+      const int rc = launch_part<BL, BR, WL, WR, STAGES, MODE, PART, T>(a, who, st);
+      return rc ? rc : launch_part<BL, BR, WL, WR, STAGES, MODE, JOIN, T>(a, who, st);
+    }
+  }
+  return launch_part<BL, BR, WL, WR, STAGES, MODE, WHOLE, T>(a, who, st);
+}
+
 template <int MODE, typename T>
-int launch_product(const Args& a, const char* who, hipStream_t st) {
-  auto rounds = [&](int bl, int br) {
-    const int64_t l = MODE == FWD ? bl / 2 : bl;
-    const int64_t tiles = (a.lefts + l - 1) / l * ((a.rights + br - 1) / br) * (MODE == DW ? 2 : 1);
-    return (double)((tiles + CUS - 1) / CUS);
-  };
-  const double c256 = 3.2 * rounds(256, 256), c128 = 1.0 * rounds(128, 128), c64 = 0.45 * rounds(64, 64);
-  if (c256 <= c128 && c256 <= c64) return launch_tiles<256, 256, 2, 4, 2, MODE, T>(a, who, st);
-  if (c128 <= c64) return launch_tiles<128, 128, 2, 2, 2, MODE, T>(a, who, st);
+int launch_product(Args a, char* partial, const char* who, hipStream_t st) {
+  const Plan use = plan(MODE, a.lefts, a.rights, a.K);
+  a.splits = use.splits;
+  a.partial = (float*)partial;
+  if (use.tile == T256) return launch_tiles<256, 256, 2, 4, 2, MODE, T>(a, who, st);
+  if constexpr (MODE == FWD)
+    if (use.tile == T192) return launch_tiles<256, 192, 2, 4, 2, MODE, T>(a, who, st);
+  if (use.tile == T128_2) return launch_tiles<128, 128, 2, 2, 2, MODE, T>(a, who, st);
+  if (use.tile == T128_4) return launch_tiles<128, 128, 2, 2, 4, MODE, T>(a, who, st);
   return launch_tiles<64, 64, 2, 2, 4, MODE, T>(a, who, st);
 }
 
 // What both directions need in workspace: x and the weights by rows of whole 16 bytes, where D is not a multiple of 8; the
-// backward da and du besides.
+// backward da and du besides, and the sums of a product's parts (dx's, then the weights').
 struct Layout {
-  int64_t Dp, Fp, Tp, x, w, factor;
+  int64_t Dp, Fp, Tp, x, w, factor, partial = 0;
   Layout(int64_t tokens, int D, int F, bool backward) {
     const bool pad = D % 8 != 0 && (backward || tokens > 0);
     Dp = up_to(D, 8);
@@ -458,8 +542,12 @@ struct Layout {
     x = pad ? up_to(tokens * Dp * 2, 256) : 0;
     w = pad ? up_to((int64_t)F * Dp * 2, 256) : 0;
     factor = backward ? up_to(Tp * Fp * 2, 256) : 0;
+    if (backward && tokens > 0) {
+      const size_t dx = plan(DX, D, tokens, Fp).partial(), dw = plan(DW, D, F, Tp).partial();
+      partial = (int64_t)(dx > dw ? dx : dw);
+    }
   }
-  int64_t bytes() const { return x + 2 * w + 2 * factor; }
+  int64_t bytes() const { return x + 2 * w + 2 * factor + partial; }
 };
 
 int check_sizes(const char* who, int64_t tokens, int D, int F, int act, int dtype) {
@@ -506,7 +594,7 @@ int forward(const void* x, const void* wg, const void* wu, void* h, float* a, fl
   p.keep_pitch = keep_pitch;
   p.act = act;
   p.wide = F % 8 == 0;
-  return launch_product<FWD, T>(p, who, st);
+  return launch_product<FWD, T>(p, nullptr, who, st);
 }
 
 template <typename T>
@@ -521,6 +609,7 @@ int backward(const void* dh, const void* x, const void* wg, const void* wu, cons
     }
   }
   T *da = (T*)(ws + lay.x + 2 * lay.w), *du = (T*)((char*)da + lay.factor);
+  char* const partial = (char*)du + lay.factor;
   const int64_t pieces = lay.Tp * (lay.Fp / 8);
   glu_factors_kernel<T><<<grid_of(pieces), 256, 0, st>>>((const T*)dh, a, u, keep_pitch, da, du, tokens, F, (int)lay.Fp, pieces, act,
                                                        F % 8 == 0);
@@ -540,7 +629,7 @@ int backward(const void* dh, const void* x, const void* wg, const void* wu, cons
     p.out[0] = dx;
     p.out_pitch = D;
     p.wide = D % 8 == 0;
-    if (const int rc = launch_product<DX, T>(p, who, st)) return rc;
+    if (const int rc = launch_product<DX, T>(p, partial, who, st)) return rc;
   }
   if (dwg) {
     Args p{};
@@ -557,7 +646,7 @@ int backward(const void* dh, const void* x, const void* wg, const void* wu, cons
     p.out[1] = dwu;
     p.out_pitch = D;
     p.wide = D % 8 == 0;
-    if (const int rc = launch_product<DW, T>(p, who, st)) return rc;
+    if (const int rc = launch_product<DW, T>(p, partial, who, st)) return rc;
   }
   return XL_OK;
 }
