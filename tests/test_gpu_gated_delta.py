@@ -81,6 +81,24 @@ def test_chunkwise_of_many_heads(gpu_case, shape, dtype, gate, state):
     test_chunkwise(gpu_case, shape, dtype, gate, state)
 
 
+@pytest.mark.parametrize("B,NH,DK,DV", [(2, 128, 100, 256), (1, 3, 70, 33), (1, 2, 1, 1), (3, 100, 256, 255), (1, 5, 129, 66)])
+def test_step_of_any_columns(gpu_case, B, NH, DK, DV):
+    """One token from a state: columns that nothing divides, the wide kernel's too, also where the state's address is odd."""
+    import xlstm_hip
+    x = make(B, NH, NH, 1, DK, DV, BF16, F32, seed=DK + DV)
+    one = [t[:, :, 0] for t in x[:5]]
+    h, c = xlstm_hip.gated_delta_step(*one, x[5])
+    hr, cr, hb, cb = reference(*x, recurrent_ku(DK))
+    check(c, cr, cb, "C")
+    check(h[:, :, None], hr, hb, "h")
+    held = torch.full((x[5].numel() + 2,), 7.0, device=dev())
+    odd = held[1:-1].view(x[5].shape)
+    odd.copy_(x[5])
+    h2, _ = xlstm_hip.gated_delta_step_(*one, odd)
+    assert torch.equal(h, h2) and torch.equal(odd, c) and float(held[0]) == float(held[-1]) == 7.0
+    assert torch.equal(xlstm_hip.gated_delta_recurrent(*x)[:, :, 0], h)
+
+
 def test_step_on_an_odd_address(gpu_case):
     import xlstm_hip
     x = make(2, 2, 2, 1, 64, 32, BF16, BF16, seed=3)

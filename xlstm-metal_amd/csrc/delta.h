@@ -9,8 +9,8 @@
 //   H = scale diag(c) Q S + P U,   S' = c_L S + (diag(c_L / c_j) K)^T U
 //
 // T and P do not know the state: a first kernel (delta_prep) forms them for all chunks at once.  What is left of a chunk
-// acts on each column of V, U and S by itself: a wave takes 16 columns through the whole sequence, its [DQK, 16] piece
-// of the state in float32 registers, and no wave waits for another.
+// acts on each column of V, U and S by itself: a scan takes blocks of 16 columns through the whole sequence, a block's [DQK, 16]
+// piece of the state in float32 registers, and no block waits for another.
 //
 // All products are on the matrix cores in f16 with float32 sums.  Every operand stands at a power-of-two scale that
 // puts its largest value high in f16's range (of a chunk's K or Q, of T and P, and of a wave's S, V - diag(c) K S, U), so any
@@ -88,6 +88,12 @@ __device__ __forceinline__ Pow2 pow2_for(float m, int target = 14) {
   int sh = e == 255 ? 0 : target + 127 - e;
   sh = sh > 100 ? 100 : sh < -100 ? -100 : sh;
   return {__uint_as_float((uint32_t)(127 + sh) << 23), __uint_as_float((uint32_t)(127 - sh) << 23)};
+}
+
+// exp(x): float32's rounding of x alone would cost |x| 2^-24 of the result
+__device__ __forceinline__ float exp_of(double x) {
+  const float hi = (float)x, e = expf(hi);
+  return fmaf(e, (float)(x - (double)hi), e);
 }
 
 // max over the wave of x >= 0, in every lane (scalar); by the bits, which order as the values do (a NaN is the largest)
@@ -205,7 +211,8 @@ __device__ __forceinline__ float state_max(const f32x4 (&st)[N]) {
   return wave_max_all(abs_max(st));
 }
 
-// Images of K and Q: [plane][64 tokens][DKP] f16, the largest value in [1, 2), each 32 columns turned, the 16-byte piece p of token i at p ^ (i % 8).
+// Images of K and Q: [plane][64 tokens][DKP] f16, the largest value in [1, 2), each 32 columns turned, the 16-byte piece p of
+// token i at p ^ (i % 8).
 template <int DKP>
 __device__ __forceinline__ int piece_at(int token, int p) {
   return token * (DKP * 2) + ((p ^ (token & 7)) << 4);

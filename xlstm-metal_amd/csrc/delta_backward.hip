@@ -356,12 +356,6 @@ struct GradArgs {
 
 constexpr int GLD = 65;
 
-// exp(x): float32's rounding of x alone would cost |x| 2^-24 of the result
-__device__ __forceinline__ float exp_of(double x) {
-  const float hi = (float)x, e = expf(hi);
-  return fmaf(e, (float)(x - (double)hi), e);
-}
-
 template <typename T, int DKB>
 struct GradLds {
   static constexpr int PK = is_f32<T>::value ? 2 : 1, DKP = DKB * 32;

@@ -1,17 +1,19 @@
 // Gated delta rule by chunks, second kernel: the scan over a head's chunks (delta.h has the formulas).
 //
-// Every 16 columns of V, U and the state go through the sequence by themselves.  PARTS waves (2 or 4) take a block of 16: a wave
-// has its part of the state's rows (DQK / PARTS, float32 registers) and as large a part of a chunk's tokens.  Per chunk:
+// Every 16 columns of V, U and the state go through the sequence by themselves: heads times DV / 16 chains, each chunk's step of
+// which is bound by the time of dependent products, reductions and LDS exchanges, not by bytes or operations.  Where such
+// blocks are many, a wave takes one, four of them share the chunk's images in LDS (delta_scan_wave_kernel).  Where they are
+// few, up to four waves take one (delta_scan_kernel): a wave has its part of the state's rows (float32 registers) and as
+// large a part of a chunk's tokens.  Per chunk:
 //
 //   1  K S and Q S over the wave's rows, all tokens; the others' tokens go to LDS
 //   2  R = V - diag(c) K S of the wave's tokens, to LDS as f16 planes
 //   3  U = T R of the wave's tokens, to LDS as f16 planes, decayed for the state and as it is for H
 //   4  S = c_L S + K^T U of the wave's rows; H = Q S + P U of the wave's tokens
 //
-// A wave on its own (the first form) is a chain of some 800 vector operations and 100 products a chunk that little can
-// overlap: 3.1 us a chunk at DQK 128, 4.7 at 256.  CB blocks of one workgroup share the chunk's images of K and Q in LDS, filled
-// straight from memory: K a chunk ahead, Q from where this chunk's has been read; T, P, V of the next chunk wait in
-// registers.  H is formed turned (columns down, tokens across), so that a lane holds four neighbours of a row.
+// The images of K and Q come to LDS straight from memory: K a chunk ahead, Q from where this chunk's has been read; T, P, V of the
+// next chunk wait in registers.  H is formed turned (columns down, tokens across): a lane holds four neighbours of a row.
+// Measured (bf16): 8192 tokens of 4 heads of 128 x 256 155 us, 1.2 a chunk; 8192 of 16 x 4 of 256 x 256 in 64 heads' blocks 590.
 #include "delta.h"
 
 namespace xl {
@@ -29,52 +31,48 @@ struct ScanArgs {
   int NH, group, S, DK, DV, chunks, slices;
 };
 
-// PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32)
-// LDS of a scan's workgroup: KST stages of K, one of Q, two chunks' factors, and each block's exchanges
-template <int DKB, int PK, int PARTS, int CB, int KST, bool WITH_Q, bool WIDE_U>
+// LDS of a scan's workgroup: KST stages of K, one of Q, two chunks' factors, and the exchanges
+template <int DKB, int PK, int PARTS, int KST, bool WITH_Q, bool WIDE_U>
 struct ScanLds {
   static constexpr int IMG = PK * L * DKB * 32 * 2;
-  static constexpr int Q = KST * IMG, FACTORS = Q + (WITH_Q ? IMG : 0), BLOCKS = FACTORS + 2 * 1024;
-  // of a block: sums of the others' parts (then of Q S), R, U decayed, U, scales
-  static constexpr int SUMS = 0, R = 4 * (PARTS - 1) * 1024, UD = R + 4096, U = UD + 4096, SCALES = U + (WIDE_U ? 4096 : 2048);
-  static constexpr int BLOCK = SCALES + 64, BYTES = BLOCKS + CB * BLOCK;
+  static constexpr int Q = KST * IMG, FACTORS = Q + (WITH_Q ? IMG : 0);
+  // sums of the others' parts (then of Q S), R, U decayed, U, scales
+  static constexpr int SUMS = FACTORS + 2 * 1024, R = SUMS + 4 * (PARTS - 1) * 1024, UD = R + 4096, U = UD + 4096, SCALES = U + (WIDE_U ? 4096 : 2048);
+  static constexpr int BYTES = SCALES + 64;
 };
 
 // STATES: U and the state before each chunk are kept for the backward, and nothing else is written.
 // PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32).
-template <typename T, int DKB, int PARTS, int CB, int KST, bool STATES>
-__global__ __launch_bounds__(64 * PARTS * CB) void delta_scan_kernel(ScanArgs p) {
+template <typename T, int DKB, int PARTS, int KST, bool STATES>
+__global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
   constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE;
-  constexpr int WAVES = PARTS * CB, TPW = 4 / PARTS, NB = DKB / PARTS;  // a wave's tiles of 16 tokens, its 32s of DQK
+  constexpr int TPW = 4 / PARTS, NB = DKB / PARTS;  // a wave's tiles of 16 tokens, its 32s of DQK
   constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
-  using Lds = ScanLds<DKB, PK, PARTS, CB, KST, !STATES, PAIR>;
-  static_assert(DKB % PARTS == 0 && Lds::BYTES <= 160 * 1024);
+  using Lds = ScanLds<DKB, PK, PARTS, KST, !STATES, PAIR>;
+  static_assert(DKB % PARTS == 0 && IMG / 1024 % PARTS == 0 && Lds::BYTES <= 160 * 1024);
   extern __shared__ __align__(1024) char lds[];
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), cb = wave / PARTS, part = wave % PARTS;
+  const int lane = threadIdx.x & 63, part = uniform(threadIdx.x >> 6);
   const int r = lane & 15, gq = lane >> 4;
   const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
-  const int bh = uniform(all / p.slices), slice = all - bh * p.slices, b = uniform(bh / p.NH), h = bh - b * p.NH;
+  const int bh = uniform(all / p.slices), block = all - bh * p.slices, b = uniform(bh / p.NH), h = bh - b * p.NH;
   const int64_t image0 = ((int64_t)b * uniform(p.NH / p.group) + uniform(h / p.group)) * p.chunks, part0 = (int64_t)bh * p.chunks;
-  const int block = slice * CB + cb, n0 = block * 16, n = n0 + r;
+  const int n0 = block * 16, n = n0 + r;
   const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
   T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
-  char* const mine = lds + Lds::BLOCKS + cb * Lds::BLOCK;
-  float* const scales = (float*)(mine + Lds::SCALES);  // [R, U, state][part]
+  float* const scales = (float*)(lds + Lds::SCALES);  // [R, U, state][part]
   // partial sums of tile mt by the parts that do not own it
   auto sums_at = [&](int mt, int from) {
-    return (f32x4*)(mine + Lds::SUMS) + (mt * (PARTS - 1) + from - (from > mt / TPW ? 1 : 0)) * 64 + lane;
+    return (f32x4*)(lds + Lds::SUMS) + (mt * (PARTS - 1) + from - (from > mt / TPW ? 1 : 0)) * 64 + lane;
   };
 
   auto fetch = [&](const char* images, int chunk, int to) {
     const char* img = images + (image0 + chunk) * (int64_t)IMG;
 #pragma unroll
-    for (int i = 0; i < IMG / 1024; i += WAVES)
-      if (IMG / 1024 % WAVES == 0 || i + wave < IMG / 1024)
-        to_lds(lds_at + to + (i + wave) * 1024, (i + wave) * 1024 + lane * 16, img);
+    for (int i = 0; i < IMG / 1024; i += PARTS) to_lds(lds_at + to + (i + part) * 1024, (i + part) * 1024 + lane * 16, img);
   };
   auto fetch_factors = [&](int chunk) {
-    if (wave == 0) to_lds(lds_at + Lds::FACTORS + (chunk & 1) * 1024, lane * 16, p.prep.f + part0 + chunk);
+    if (part == 0) to_lds(lds_at + Lds::FACTORS + (chunk & 1) * 1024, lane * 16, p.prep.f + part0 + chunk);
   };
   // Tokens 16 mt + 4 gq + e of column n, mt of this wave.  Past the last token the last one is read again (its beta is 0 there: T
   // has zeros in its column), past the last column the last one: those columns are computed and not written.
@@ -235,7 +233,7 @@ __global__ __launch_bounds__(64 * PARTS * CB) void delta_scan_kernel(ScanArgs p)
     for (int x = 0; x < TPW; ++x) {
       const int mt = part * TPW + x;
 #pragma unroll
-      for (int i = 0; i < PARTS - 1; ++i) own[x] += *((const f32x4*)(mine + Lds::SUMS) + (mt * (PARTS - 1) + i) * 64 + lane);
+      for (int i = 0; i < PARTS - 1; ++i) own[x] += *((const f32x4*)(lds + Lds::SUMS) + (mt * (PARTS - 1) + i) * 64 + lane);
 #pragma unroll
       for (int e = 0; e < 4; ++e) rr[x][e] = fmaf(-in[x][e], own[x][e], to_f32(vn[x][e]));
     }
@@ -245,7 +243,7 @@ __global__ __launch_bounds__(64 * PARTS * CB) void delta_scan_kernel(ScanArgs p)
     for (int x = 0; x < TPW; ++x) {
       f16x4 hi, lo;
       split4(rr[x], rs.up, hi, lo);
-      *((f16x8*)(mine + Lds::R) + (part * TPW + x) * 64 + lane) = join(hi, lo);
+      *((f16x8*)(lds + Lds::R) + (part * TPW + x) * 64 + lane) = join(hi, lo);
     }
     if (lane == 0) scales[part] = rs.down;
     lds_barrier();
@@ -266,7 +264,7 @@ __global__ __launch_bounds__(64 * PARTS * CB) void delta_scan_kernel(ScanArgs p)
         lo[s] = join(l[0], l[1]);
       }
     };
-    planes((const f16x8*)(mine + Lds::R), scales, r_down, rh, rl);
+    planes((const f16x8*)(lds + Lds::R), scales, r_down, rh, rl);
     f32x4 u[TPW], w[TPW];
     const float back = t_scale * r_down;
 #pragma unroll
@@ -291,11 +289,11 @@ __global__ __launch_bounds__(64 * PARTS * CB) void delta_scan_kernel(ScanArgs p)
       const int mt = part * TPW + x;
       f16x4 hi, lo;
       split4(w[x], ws_up, hi, lo);
-      *((f16x8*)(mine + Lds::UD) + mt * 64 + lane) = join(hi, lo);
+      *((f16x8*)(lds + Lds::UD) + mt * 64 + lane) = join(hi, lo);
       if constexpr (!STATES) {
         split4(u[x], us.up, hi, lo);
-        if constexpr (PAIR) *((f16x8*)(mine + Lds::U) + mt * 64 + lane) = join(hi, lo);
-        else *((f16x4*)(mine + Lds::U) + mt * 64 + lane) = hi;
+        if constexpr (PAIR) *((f16x8*)(lds + Lds::U) + mt * 64 + lane) = join(hi, lo);
+        else *((f16x4*)(lds + Lds::U) + mt * 64 + lane) = hi;
       }
     }
     if (lane == 0) scales[PARTS + part] = us.down;
@@ -312,7 +310,7 @@ __global__ __launch_bounds__(64 * PARTS * CB) void delta_scan_kernel(ScanArgs p)
     // U decayed is below 2^15 w_down
     const Pow2 sc = pow2_for(fmaxf(largest(scales + 2 * PARTS) * keep, w_down * 32767.f), STATE);
     f16x8 wh[2], wl[2];
-    planes((const f16x8*)(mine + Lds::UD), scales + PARTS, u_down, wh, wl);
+    planes((const f16x8*)(lds + Lds::UD), scales + PARTS, u_down, wh, wl);
     const _Float16 shift = (_Float16)(w_down * sc.up);  // to the state's scale: 2^-8 or less
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
@@ -353,14 +351,14 @@ __global__ __launch_bounds__(64 * PARTS * CB) void delta_scan_kernel(ScanArgs p)
     } else {  // ---- H
       f16x8 uh[2], ul[2];
       if constexpr (PAIR) {
-        planes((const f16x8*)(mine + Lds::U), scales + PARTS, u_down, uh, ul);
+        planes((const f16x8*)(lds + Lds::U), scales + PARTS, u_down, uh, ul);
       } else {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
           f16x4 x[2];
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            x[i] = *((const f16x4*)(mine + Lds::U) + (2 * s + i) * 64 + lane) *
+            x[i] = *((const f16x4*)(lds + Lds::U) + (2 * s + i) * 64 + lane) *
                    ratio(__int_as_float(uniform(__float_as_int(scales[PARTS + (2 * s + i) / TPW]))), u_down);
           uh[s] = join(x[0], x[1]);
         }
@@ -373,7 +371,7 @@ __global__ __launch_bounds__(64 * PARTS * CB) void delta_scan_kernel(ScanArgs p)
       for (int x = 0; x < TPW; ++x) {
         const int mt = part * TPW + x;
 #pragma unroll
-        for (int i = 0; i < PARTS - 1; ++i) own[x] += *((const f32x4*)(mine + Lds::SUMS) + (mt * (PARTS - 1) + i) * 64 + lane);
+        for (int i = 0; i < PARTS - 1; ++i) own[x] += *((const f32x4*)(lds + Lds::SUMS) + (mt * (PARTS - 1) + i) * 64 + lane);
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
         y = mfma(uh[0], ph[x][0], y);
         if constexpr (PAIR) {
@@ -730,8 +728,8 @@ Choice choice(bool many) {
   constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
   if (many)
     return {(const void*)delta_scan_wave_kernel<T, DKB, KST, STATES>, 256, 4, KST * (STATES ? 1 : 2) * PK * L * DKB * 64 + 2 * 1024};
-  return {(const void*)delta_scan_kernel<T, DKB, PARTS, 1, KST, STATES>, 64 * PARTS, 1,
-          ScanLds<DKB, PK, PARTS, 1, KST, !STATES, PAIR>::BYTES};
+  return {(const void*)delta_scan_kernel<T, DKB, PARTS, KST, STATES>, 64 * PARTS, 1,
+          ScanLds<DKB, PK, PARTS, KST, !STATES, PAIR>::BYTES};
 }
 template <typename T, bool STATES>
 Choice pick(int dkp, bool many) {

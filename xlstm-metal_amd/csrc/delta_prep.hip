@@ -56,12 +56,6 @@ __device__ __forceinline__ f32x4 mfma4(float a, float b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0);
 }
 
-// exp(x): float32's rounding of x alone would cost |x| 2^-24 of the result
-__device__ __forceinline__ float exp_of(double x) {
-  const float hi = (float)x, e = expf(hi);
-  return fmaf(e, (float)(x - (double)hi), e);
-}
-
 // max over the workgroup of N values a thread
 template <int N>
 __device__ __forceinline__ void block_max(float (&m)[N], float (*red)[8]) {

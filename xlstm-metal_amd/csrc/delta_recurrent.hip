@@ -4,8 +4,9 @@
 //
 // A workgroup takes 32 columns of a head's state through all tokens, in float32 registers: 4 waves x 8 lane groups share
 // the rows, a lane holds 4 columns of every 32nd row.  S^T k and S^T q of the state before the token are summed
-// together (h = scale (a S^T q + (q.k) d)), so a token costs one reduction and one barrier; the next token's values are on their way
-// meanwhile.  One token of many heads is bound by the state's bytes, in and out once, and has a kernel of its own.
+// together (h = scale (a S^T q + (q.k) d)), so a token costs one reduction and one barrier; the next token's values are on their
+// way meanwhile.  13 tokens of 32 heads of 128 x 256 (bf16): 16.9 us, 1 a token, bound by that reduction's latency.  One token
+// is bound by the state's bytes, in and out once, and has a kernel of its own.
 #include "delta.h"
 
 namespace xl {
@@ -170,7 +171,7 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(RecArgs p) {
   }
 }
 
-// One token of many heads: 1024 threads a workgroup, COLS columns (256: a wave reads whole KBs of a row), every thread's rows read
+// One token: 1024 threads a workgroup, COLS columns (256: a wave reads whole KBs of a row), every thread's rows read
 // before the first is written.  S^T k and S^T q are summed over a thread's rows, then over the row groups in LDS.
 constexpr int STEP_THREADS = 1024;
 
@@ -192,10 +193,20 @@ __global__ __launch_bounds__(STEP_THREADS) void delta_step_kernel(RecArgs p) {
   asm volatile("" ::: "memory");
   const int64_t state = (int64_t)bh * p.DK * p.DV + colc;
   f32x4 st[RPT];
+  if (p.wide) {
 #pragma unroll
-  for (int i = 0; i < RPT; ++i) {
-    const int r = rg + RG * i;
-    st[i] = __builtin_nontemporal_load((const f32x4*)(p.c0 + state + (int64_t)(r < p.DK ? r : 0) * p.DV));
+    for (int i = 0; i < RPT; ++i) {
+      const int r = rg + RG * i;
+      st[i] = __builtin_nontemporal_load((const f32x4*)(p.c0 + state + (int64_t)(r < p.DK ? r : 0) * p.DV));
+    }
+  } else {  // columns past the last: that one again
+#pragma unroll
+    for (int i = 0; i < RPT; ++i) {
+      const int r = rg + RG * i;
+      const float* from = p.c0 + state + (int64_t)(r < p.DK ? r : 0) * p.DV;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[i][e] = from[colc + e < p.DV ? e : p.DV - 1 - colc];
+    }
   }
   const float qv = tid < p.DK ? to_f32(qraw) : 0.f, kv = tid < p.DK ? to_f32(kraw) : 0.f;
   if (tid < DKP) {
@@ -240,7 +251,7 @@ __global__ __launch_bounds__(STEP_THREADS) void delta_step_kernel(RecArgs p) {
     }
   }
   lds_barrier();
-  if (col >= p.DV) return;
+  if (col >= p.DV || !p.c_last) return;
   const f32x4 d = *(const f32x4*)&d_s[cg * 4];
 #pragma unroll
   for (int i = 0; i < RPT; ++i) {
@@ -249,7 +260,14 @@ __global__ __launch_bounds__(STEP_THREADS) void delta_step_kernel(RecArgs p) {
     f32x4 x;
 #pragma unroll
     for (int e = 0; e < 4; ++e) x[e] = fmaf(kk[i], d[e], a * st[i][e]);
-    __builtin_nontemporal_store(x, (f32x4*)(p.c_last + state + (int64_t)r * p.DV));
+    float* const to = p.c_last + state + (int64_t)r * p.DV;
+    if (p.wide) {
+      __builtin_nontemporal_store(x, (f32x4*)to);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (col + e < p.DV) to[e] = x[e];
+    }
   }
 }
 
@@ -309,11 +327,12 @@ int launch_recurrent(const Shape& s, const void* q, const void* k, const void* v
                      const float* c0, void* h, float* c_last, hipStream_t st, const char* who) {
   RecArgs a{q, k, v, g, beta, c0, h, c_last, s.NH, s.NH / s.NHK, s.S, s.DK, s.DV, s.scale, false};
   a.wide = s.DV % 4 == 0 && (((uintptr_t)c0 | (uintptr_t)c_last) & 15) == 0;
-  // One token: 1 KB rows where that gives every CU a workgroup, else 256-byte ones, else the kernel of several tokens (us, bf16, 256 x
-  // 512 states: 128 heads 25 and 40, 8 heads STEP8).
+  // One token from a state: 1 KB rows where that gives every CU a workgroup, else 256-byte ones, else the kernel of
+  // several tokens.  bf16, us, in that order: 8 heads of 128 x 256 6.1, 4.3, 5.3; 64 heads 6.7, 5.7, 7.5; 256 heads 12.4, 14.9, 17.6;
+  // 16 heads of 256 x 512 9.6, 6.0, 10.4; 128 heads 23.9, 26.8, 41.0 (268 MB: 5.6 TB/s).
   const int64_t heads = (int64_t)s.B * s.NH;
-  const bool one = s.S == 1 && c0 && c_last && a.wide;
-  const int cols = one && s.DV % 256 == 0 && heads * (s.DV / 256) >= 256 ? 256 : one && heads * ((s.DV + 63) / 64) >= 256 ? 64 : 0;
+  const bool one = s.S == 1 && c0;
+  const int cols = !one ? 0 : s.DV % 256 == 0 && heads * (s.DV / 256) >= 256 ? 256 : 64;
   const void* kern = nullptr;
   auto with_gate = [&](auto t) {
     using T = decltype(t);
