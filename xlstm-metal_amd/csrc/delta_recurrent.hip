@@ -2,19 +2,18 @@
 //
 //   S = a S + k d^T,  d = beta (v - a S^T k),  h = scale S^T q,  a = exp(g)
 //
-// A workgroup takes 32 columns of a head's state through all tokens, in float32 registers: 4 waves x 8 lane groups share
-// the rows, a lane holds 4 columns of every 32nd row.  S^T k and S^T q of the state before the token are summed
-// together (h = scale (a S^T q + (q.k) d)), so a token costs one reduction and one barrier; the next token's values are on their
-// way meanwhile.  13 tokens of 32 heads of 128 x 256 (bf16): 16.9 us, 1 a token, bound by that reduction's latency.  One token
-// is bound by the state's bytes, in and out once, and has a kernel of its own.
+// A workgroup takes 32 or 16 columns of a head's state through all tokens, in float32 registers: 4 waves x 8 or 16 lane
+// groups share the rows, a lane holds 4 columns of every 32nd or 64th row.  S^T k and S^T q of the state before the token are
+// summed together (h = scale (a S^T q + (q.k) d)), so a token costs one reduction and one barrier, whose latency bounds it:
+// 13 tokens of 32 heads of 128 x 256 (bf16) 11.0 us, 0.6 a token.  Tokens' values come 8 tokens at a time and a block ahead.
+// One token is bound by the state's bytes, in and out once, and has a kernel of its own.
 #include "delta.h"
 
 namespace xl {
 namespace delta {
 namespace {
 
-constexpr int COLS = 32, RWAVES = 4;
-static_assert(MAX_DQK == 64 * RWAVES);  // a thread for each value of q and k
+constexpr int RWAVES = 4;
 
 struct RecArgs {
   const void *q, *k, *v, *g, *beta;
@@ -23,27 +22,40 @@ struct RecArgs {
   float* c_last;
   int NH, group, S, DK, DV;
   float scale;
-  bool wide;  // 16-byte accesses to the state
+  bool wide;    // 16-byte accesses to the state
+  bool wide_h;  // 4 values of h at once
 };
 
-// x + what the lanes 8, 16 and 32 away have: the sum over a wave's 8 row groups
-__device__ __forceinline__ float sum_groups(float x) {
+// x + what the lanes G, 2 G .. 32 away have: the sum over a wave's lane groups
+template <int G>
+__device__ __forceinline__ float sum_row(float x) {
   x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x128, 0xf, 0xf, false));  // row_ror:8
-  const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  x = __uint_as_float(y[0]) + __uint_as_float(y[1]);
-  const auto z = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-  return __uint_as_float(z[0]) + __uint_as_float(z[1]);
+  if (G == 4) x += __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), 0x124, 0xf, 0xf, false));  // row_ror:4
+  return x;
+}
+// both sums over halves of the wave: a's in its lower half (of 32 or, alternately, of 16 lanes), b's in the upper
+__device__ __forceinline__ float fold32(float a, float b) {
+  const auto y = __builtin_amdgcn_permlane32_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
+}
+__device__ __forceinline__ float fold16(float a, float b) {
+  const auto y = __builtin_amdgcn_permlane16_swap(__float_as_uint(a), __float_as_uint(b), false, false);
+  return __uint_as_float(y[0]) + __uint_as_float(y[1]);
 }
 
-template <typename T, typename G, int NI>
+template <typename T, typename G, int COLS, int DKP>
 __global__ __launch_bounds__(256) void delta_recurrent_kernel(RecArgs p) {
-  __shared__ float qk_s[2][2][MAX_DQK];
+  constexpr int QUADS = COLS / 4, RSTEP = RWAVES * 64 / QUADS, NI = DKP / RSTEP;
+  static_assert(NI * RSTEP == DKP);
+  // a block of tokens' values, brought by one load a thread for each of PASSES tokens of q and k, for v, g and beta
+  constexpr int TOKENS = 8, AT_ONCE = 256 / DKP, PASSES = TOKENS / AT_ONCE;
+  __shared__ float q_s[TOKENS][DKP], k_s[TOKENS][DKP], v_s[TOKENS][COLS], gates[TOKENS][2];
   __shared__ float sums[2][RWAVES][2][COLS];
   __shared__ float dots[2][RWAVES];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lg = lane >> 3;
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, lg = lane / QUADS, quad = lane % QUADS;
   const int slices = (p.DV + COLS - 1) / COLS;
   const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
-  const int bh = all / slices, col = (all - bh * slices) * COLS + (lane & 7) * 4;
+  const int bh = all / slices, col = (all - bh * slices) * COLS + quad * 4;
   const int b = bh / p.NH, h = bh - b * p.NH, bhk = b * (p.NH / p.group) + h / p.group;
   const T* q = (const T*)p.q + (int64_t)bhk * p.S * p.DK;
   const T* k = (const T*)p.k + (int64_t)bhk * p.S * p.DK;
@@ -51,70 +63,75 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(RecArgs p) {
   T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
   const G *gp = (const G*)p.g + (int64_t)bh * p.S, *bp = (const G*)p.beta + (int64_t)bh * p.S;
   const int64_t state = (int64_t)bh * p.DK * p.DV;
-  const int row0 = wave * 8 + lg;
-  const bool whole = p.wide && col < p.DV;  // a multiple of 4 columns
+  const int row0 = wave * (64 / QUADS) + lg;
 
+  // Rows past DQK are the first again, against zeros, and columns past DV the last.
   f32x4 st[NI];
+  const int colc = min(col, p.DV - 1);
+  if (p.c0 && p.wide) {
 #pragma unroll
-  for (int i = 0; i < NI; ++i) {
-    const int r = row0 + 32 * i;
-    st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
-    if (p.c0 && r < p.DK) {
-      const float* from = p.c0 + state + (int64_t)r * p.DV + col;
-      if (whole) {
-        st[i] = __builtin_nontemporal_load((const f32x4*)from);
-      } else {
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < p.DV) st[i][e] = from[e];
-      }
+    for (int i = 0; i < NI; ++i) {
+      const int r = row0 + RSTEP * i;
+      st[i] = __builtin_nontemporal_load((const f32x4*)(p.c0 + state + (int64_t)(r < p.DK ? r : 0) * p.DV + (col < p.DV ? col : 0)));
     }
-  }
-  // Thread tid has value tid of a token's q and k.  What is loaded past the last token or value is the last one's.  No branch around a load: the compiler would wait for it at the branch's end.
-  const int dc = tid < p.DK ? tid : p.DK - 1;
-  T qn{}, kn{};
-  auto load_qk = [&](int t) {
-    const int64_t at = (int64_t)(t < p.S ? t : p.S - 1) * p.DK + dc;
-    qn = q[at];
-    kn = k[at];
-  };
-  if (p.S > 0) {
-    load_qk(0);
-    qk_s[0][0][tid] = to_f32(qn);
-    qk_s[0][1][tid] = to_f32(kn);
-    load_qk(1);
-  }
-  T vn[4];
-  G gn{}, bn{};
-  int vcol[4];
+  } else if (p.c0) {
 #pragma unroll
-  for (int e = 0; e < 4; ++e) vcol[e] = col + e < p.DV ? col + e : p.DV - 1;
-  auto load = [&](int t) {
-    t = t < p.S ? t : p.S - 1;
+    for (int i = 0; i < NI; ++i) {
+      const int r = row0 + RSTEP * i;
+      const float* from = p.c0 + state + (int64_t)(r < p.DK ? r : 0) * p.DV;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) st[i][e] = from[min(colc + e, p.DV - 1)];
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < NI; ++i) st[i] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+  // What is loaded past the last token or column is the last one's, past the last value a zero.  No branch around a load: the
+  // compiler would wait for it at the branch's end.
+  T qn[PASSES], kn[PASSES], vn{};
+  G gn{}, bn{};
+  const int value = tid % DKP, vtoken = tid / COLS, vcol = (all - bh * slices) * COLS + tid % COLS;
+  const bool there = value < p.DK;
+  auto load = [&](int t0) {
+#pragma unroll
+    for (int i = 0; i < PASSES; ++i) {
+      const int64_t at = (int64_t)min(t0 + i * AT_ONCE + tid / DKP, p.S - 1) * p.DK + (there ? value : 0);
+      qn[i] = q[at];
+      kn[i] = k[at];
+    }
+    vn = v[(int64_t)min(t0 + vtoken, p.S - 1) * p.DV + min(vcol, p.DV - 1)];
+    const int t = min(t0 + (tid & (TOKENS - 1)), p.S - 1);
     gn = gp[t];
     bn = bp[t];
-#pragma unroll
-    for (int e = 0; e < 4; ++e) vn[e] = v[(int64_t)t * p.DV + vcol[e]];
   };
   if (p.S > 0) load(0);
-  lds_barrier();
-  for (int t = 0; t < p.S; ++t) {
-    const int at = t & 1;
-    const float a = expf(to_f32(gn)), beta = to_f32(bn);
-    float vt[4];
+  // here, not at its first use: in the loop that wait would be for every token's stores too
 #pragma unroll
-    for (int e = 0; e < 4; ++e) vt[e] = to_f32(vn[e]);
-    qk_s[at ^ 1][0][tid] = to_f32(qn);  // the next token's, read a token ago
-    qk_s[at ^ 1][1][tid] = to_f32(kn);
-    load(t + 1);
-    load_qk(t + 2);
+  for (int i = 0; i < NI; ++i) asm volatile("" : "+v"(st[i]));
+  for (int t = 0; t < p.S; ++t) {
+    const int at = t & 1, in = t & (TOKENS - 1);
+    if (in == 0) {  // the block before has been read: each token's values before its barrier
+#pragma unroll
+      for (int i = 0; i < PASSES; ++i) {
+        q_s[i * AT_ONCE + tid / DKP][value] = there ? to_f32(qn[i]) : 0.f;
+        k_s[i * AT_ONCE + tid / DKP][value] = there ? to_f32(kn[i]) : 0.f;
+      }
+      if (vtoken < TOKENS) v_s[vtoken][tid % COLS] = to_f32(vn);
+      if (tid < TOKENS) {
+        gates[tid][0] = expf(to_f32(gn));
+        gates[tid][1] = to_f32(bn);
+      }
+      load(t + TOKENS);
+      lds_barrier();
+    }
+    const float a = gates[in][0], beta = gates[in][1];
+    const f32x4 vt = *(const f32x4*)&v_s[in][quad * 4];
     f32x4 ks = {0.f, 0.f, 0.f, 0.f}, qs = {0.f, 0.f, 0.f, 0.f};
     float kk[NI], dot = 0.f;
 #pragma unroll
     for (int i = 0; i < NI; ++i) {
-      const bool there = row0 + 32 * i < p.DK;
-      const float qi = there ? qk_s[at][0][row0 + 32 * i] : 0.f;
-      kk[i] = there ? qk_s[at][1][row0 + 32 * i] : 0.f;
+      const float qi = q_s[in][row0 + RSTEP * i];
+      kk[i] = k_s[in][row0 + RSTEP * i];
       dot = fmaf(qi, kk[i], dot);
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -122,26 +139,25 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(RecArgs p) {
         qs[e] = fmaf(qi, st[i][e], qs[e]);
       }
     }
+    // lanes below 32 get the sums of S^T k, the others S^T q's; of those, 16 lanes the columns 0 and 2, 16 the columns 1 and 3
+    float y[4];
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      ks[e] = sum_groups(ks[e]);
-      qs[e] = sum_groups(qs[e]);
+    for (int e = 0; e < 4; ++e) y[e] = fold32(ks[e], qs[e]);
+    const float s02[2] = {sum_row<QUADS>(fold16(y[0], y[1])), sum_row<QUADS>(fold16(y[2], y[3]))};
+    dot = fold32(dot, dot);
+    dot = sum_row<QUADS>(fold16(dot, dot));
+    if ((lane & 15) < QUADS) {
+      float* to = &sums[at][wave][lane >> 5][quad * 4 + (lane >> 4 & 1)];
+      to[0] = s02[0];
+      to[2] = s02[1];
     }
-    dot = sum_groups(dot);
-    if (lane < 8) {
-      *(f32x4*)&sums[at][wave][0][lane * 4] = ks;
-      *(f32x4*)&sums[at][wave][1][lane * 4] = qs;
-      if (lane == 0) dots[at][wave] = dot;
-    }
+    if (lane == 0) dots[at][wave] = dot;
     lds_barrier();
-    ks = qs = f32x4{0.f, 0.f, 0.f, 0.f};
-    dot = 0.f;
+    f32x4 part[RWAVES];
 #pragma unroll
-    for (int w = 0; w < RWAVES; ++w) {
-      ks += *(const f32x4*)&sums[at][w][0][(lane & 7) * 4];
-      qs += *(const f32x4*)&sums[at][w][1][(lane & 7) * 4];
-      dot += dots[at][w];
-    }
+    for (int w = 0; w < RWAVES; ++w) part[w] = *(const f32x4*)&sums[at][w][0][quad * 4];
+    __builtin_amdgcn_sched_barrier(0);  // all four under way at once
+    ks = (part[0] + part[1]) + (part[2] + part[3]);
     f32x4 d;
 #pragma unroll
     for (int e = 0; e < 4; ++e) d[e] = beta * (vt[e] - a * ks[e]);
@@ -149,20 +165,36 @@ __global__ __launch_bounds__(256) void delta_recurrent_kernel(RecArgs p) {
     for (int i = 0; i < NI; ++i)
 #pragma unroll
       for (int e = 0; e < 4; ++e) st[i][e] = fmaf(kk[i], d[e], a * st[i][e]);
-    if (wave == 0 && lg == 0) {
+    if (wave == (t & (RWAVES - 1)) && lg == 0) {  // the waves in turn
+      dot = 0.f;
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        if (col + e < p.DV) ho[(int64_t)t * p.DV + col + e] = from_f32<T>(p.scale * fmaf(dot, d[e], a * qs[e]));
+      for (int w = 0; w < RWAVES; ++w) {
+        part[w] = *(const f32x4*)&sums[at][w][1][quad * 4];
+        dot += dots[at][w];
+      }
+      qs = (part[0] + part[1]) + (part[2] + part[3]);
+      f32x4 y;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) y[e] = p.scale * fmaf(dot, d[e], a * qs[e]);
+      const Four<T> o = rounded4<T>(y);
+      T* const to = ho + (int64_t)t * p.DV + col;
+      if (p.wide_h) {
+        if (col < p.DV) *(Four<T>*)to = o;
+      } else {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < p.DV) to[e] = o.e[e];
+      }
     }
   }
   if (!p.c_last) return;
 #pragma unroll
   for (int i = 0; i < NI; ++i) {
-    const int r = row0 + 32 * i;
+    const int r = row0 + RSTEP * i;
     if (r >= p.DK) continue;
     float* to = p.c_last + state + (int64_t)r * p.DV + col;
-    if (whole) {
-      *(f32x4*)to = st[i];
+    if (p.wide) {
+      if (col < p.DV) *(f32x4*)to = st[i];
     } else {
 #pragma unroll
       for (int e = 0; e < 4; ++e)
@@ -279,10 +311,10 @@ const void* pick_step(int DK) {
   return DK <= 128 ? (const void*)delta_step_kernel<T, G, 256, 128> : (const void*)delta_step_kernel<T, G, 256, 256>;
 }
 
-template <typename T, typename G>
+template <typename T, typename G, int COLS>
 const void* pick(int DK) {
-  return DK <= 64 ? (const void*)delta_recurrent_kernel<T, G, 2> : DK <= 128 ? (const void*)delta_recurrent_kernel<T, G, 4>
-                                                                             : (const void*)delta_recurrent_kernel<T, G, 8>;
+  return DK <= 64 ? (const void*)delta_recurrent_kernel<T, G, COLS, 64> : DK <= 128 ? (const void*)delta_recurrent_kernel<T, G, COLS, 128>
+                                                                                 : (const void*)delta_recurrent_kernel<T, G, COLS, 256>;
 }
 
 }  // namespace
@@ -325,20 +357,27 @@ int set_strides(Shape& s, const int64_t* strides, const char* who) {
 
 int launch_recurrent(const Shape& s, const void* q, const void* k, const void* v, const void* g, const void* beta,
                      const float* c0, void* h, float* c_last, hipStream_t st, const char* who) {
-  RecArgs a{q, k, v, g, beta, c0, h, c_last, s.NH, s.NH / s.NHK, s.S, s.DK, s.DV, s.scale, false};
+  RecArgs a{q, k, v, g, beta, c0, h, c_last, s.NH, s.NH / s.NHK, s.S, s.DK, s.DV, s.scale, false, false};
+  a.wide_h = s.DV % 4 == 0 && (uintptr_t)h % 16 == 0;
   a.wide = s.DV % 4 == 0 && (((uintptr_t)c0 | (uintptr_t)c_last) & 15) == 0;
   // One token from a state: 1 KB rows where that gives every CU a workgroup, else 256-byte ones, else the kernel of
   // several tokens.  bf16, us, in that order: 8 heads of 128 x 256 6.1, 4.3, 5.3; 64 heads 6.7, 5.7, 7.5; 256 heads 12.4, 14.9, 17.6;
   // 16 heads of 256 x 512 9.6, 6.0, 10.4; 128 heads 23.9, 26.8, 41.0 (268 MB: 5.6 TB/s).
   const int64_t heads = (int64_t)s.B * s.NH;
   const bool one = s.S == 1 && c0;
-  const int cols = !one ? 0 : s.DV % 256 == 0 && heads * (s.DV / 256) >= 256 ? 256 : 64;
+  const int step = !one ? 0 : s.DV % 256 == 0 && heads * (s.DV / 256) >= 256 ? 256 : 64;
+  // Several: 16 columns a workgroup where 32 give a CU one at most, for 13 tokens of 128 x 256 us of 16 and 32: 8 heads 10.2, 11.3; 32
+  // heads 12.2, 12.5; 64 heads 17.5, 14.8; 128 heads 28.9, 21.4.
+  const int width = step ? step : heads * ((s.DV + 31) / 32) <= 256 ? 16 : 32;
   const void* kern = nullptr;
   auto with_gate = [&](auto t) {
     using T = decltype(t);
     auto of = [&](auto g) {
       using G = decltype(g);
-      kern = cols == 256 ? pick_step<T, G, 256>(s.DK) : cols == 64 ? pick_step<T, G, 64>(s.DK) : pick<T, G>(s.DK);
+      kern = step == 256 ? pick_step<T, G, 256>(s.DK)
+             : step == 64 ? pick_step<T, G, 64>(s.DK)
+             : width == 16 ? pick<T, G, 16>(s.DK)
+                           : pick<T, G, 32>(s.DK);
     };
     if (s.dtype_gates == XL_DTYPE_F32) of(float{});
     else if (s.dtype_gates == XL_DTYPE_BF16) of(bf16_t{});
@@ -347,10 +386,9 @@ int launch_recurrent(const Shape& s, const void* q, const void* k, const void* v
   if (s.dtype == XL_DTYPE_F32) with_gate(float{});
   else if (s.dtype == XL_DTYPE_BF16) with_gate(bf16_t{});
   else with_gate(f16_t{});
-  const int width = cols ? cols : COLS;
   const unsigned grid = (unsigned)(heads * ((s.DV + width - 1) / width));
   void* args[] = {&a};
-  const hipError_t e = hipLaunchKernel(kern, dim3(grid), dim3(cols ? STEP_THREADS : 256), args, 0, st);
+  const hipError_t e = hipLaunchKernel(kern, dim3(grid), dim3(step ? STEP_THREADS : 256), args, 0, st);
   if (e != hipSuccess) return set_error(XL_ERR_LAUNCH, "%s: launch failed: %s", who, hipGetErrorString(e));
   return check_launch(who);
 }
