@@ -37,7 +37,7 @@ struct ScanLds {
   static constexpr int IMG = PK * L * DKB * 32 * 2;
   static constexpr int Q = KST * IMG, FACTORS = Q + (WITH_Q ? IMG : 0);
   // sums of the others' parts (then of Q S), R, U decayed, U, scales
-  static constexpr int SUMS = FACTORS + 2 * 1024, R = SUMS + 4 * (PARTS - 1) * 1024, UD = R + 4096, U = UD + 4096, SCALES = U + (WIDE_U ? 4096 : 2048);
+  static constexpr int SUMS = FACTORS + 2 * 1024, R = SUMS + 4 * PARTS * 1024, UD = R + 4096, U = UD + 4096, SCALES = U + (WIDE_U ? 4096 : 2048);
   static constexpr int BYTES = SCALES + 64;
 };
 
@@ -61,9 +61,15 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
   T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
   float* const scales = (float*)(lds + Lds::SCALES);  // [R, U, state][part]
-  // partial sums of tile mt by the parts that do not own it
-  auto sums_at = [&](int mt, int from) {
-    return (f32x4*)(lds + Lds::SUMS) + (mt * (PARTS - 1) + from - (from > mt / TPW ? 1 : 0)) * 64 + lane;
+  // sums over part `from`'s rows of token tile mt (its owner's own too: to leave those out took branches that cost more)
+  auto sums_at = [&](int mt, int from) { return (f32x4*)(lds + Lds::SUMS) + (mt * PARTS + from) * 64 + lane; };
+  auto sum_of = [&](int mt) {
+    f32x4 x[PARTS];
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) x[i] = *sums_at(mt, i);
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) x[0] += x[i];
+    return x[0];
   };
 
   auto fetch = [&](const char* images, int chunk, int to) {
@@ -204,12 +210,8 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
         }
       }
     }
-    f32x4 own[TPW];  // the wave's own tokens
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      if (mt / TPW == part) own[mt % TPW] = ks[mt];
-      else *sums_at(mt, part) = ks[mt];
-    }
+    for (int mt = 0; mt < 4; ++mt) *sums_at(mt, part) = ks[mt];
 #pragma unroll
     for (int x = 0; x < TPW; ++x) {
       const int mt = part * TPW + x;
@@ -231,11 +233,9 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     f32x4 rr[TPW];
 #pragma unroll
     for (int x = 0; x < TPW; ++x) {
-      const int mt = part * TPW + x;
+      const f32x4 sum = sum_of(part * TPW + x);
 #pragma unroll
-      for (int i = 0; i < PARTS - 1; ++i) own[x] += *((const f32x4*)(lds + Lds::SUMS) + (mt * (PARTS - 1) + i) * 64 + lane);
-#pragma unroll
-      for (int e = 0; e < 4; ++e) rr[x][e] = fmaf(-in[x][e], own[x][e], to_f32(vn[x][e]));
+      for (int e = 0; e < 4; ++e) rr[x][e] = fmaf(-in[x][e], sum[e], to_f32(vn[x][e]));
     }
     load_v(next);
     const Pow2 rs = pow2_for(wave_max_all(abs_max(rr)));
@@ -299,10 +299,7 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     if (lane == 0) scales[PARTS + part] = us.down;
     if constexpr (!STATES) {
 #pragma unroll
-      for (int mt = 0; mt < 4; ++mt) {
-        if (mt / TPW == part) own[mt % TPW] = hs[mt];
-        else *sums_at(mt, part) = hs[mt];
-      }
+      for (int mt = 0; mt < 4; ++mt) *sums_at(mt, part) = hs[mt];
     }
     lds_barrier();
     // ---- 4: the state
@@ -370,8 +367,7 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
 #pragma unroll
       for (int x = 0; x < TPW; ++x) {
         const int mt = part * TPW + x;
-#pragma unroll
-        for (int i = 0; i < PARTS - 1; ++i) own[x] += *((const f32x4*)(lds + Lds::SUMS) + (mt * (PARTS - 1) + i) * 64 + lane);
+        const f32x4 qs = sum_of(mt);
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
         y = mfma(uh[0], ph[x][0], y);
         if constexpr (PAIR) {
@@ -385,7 +381,7 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
             y = mfma(uh[1], pl[x][1], y);
           }
         }
-        const Four<T> o = rounded4<T>(y * pu + own[x] * fq[x]);
+        const Four<T> o = rounded4<T>(y * pu + qs * fq[x]);
         if (whole) {
           *(Four<T>*)((char*)(to + (int64_t)(16 * mt) * p.DV) + h_at) = o;
         } else if (t0 + 16 * mt + r < p.S) {
