@@ -67,6 +67,11 @@ __device__ __forceinline__ void lds_barrier() {
   __builtin_amdgcn_s_barrier();
   asm volatile("" ::: "memory");
 }
+// Every load and store under way, also to the compiler, which counts what it knows of
+__device__ __forceinline__ void wait_loads() {
+  __builtin_amdgcn_s_waitcnt(0x0f70);  // vmcnt(0)
+  asm volatile("" ::: "memory");
+}
 __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
 
 // the scheduler's order here: N products, a few vector operations between them
@@ -187,6 +192,9 @@ __device__ __forceinline__ void split8(f32x4 a, f32x4 b, float scale, f16x8& hi,
 // 16 bytes a lane from global memory into LDS, at lds + 16 * lane (lds the same in the whole wave).  Whoever reads what it
 // writes waits for it by vmcnt, and then for everybody at a barrier.  m0 has to be written one wait state before.
 __device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const void* base) {
+  // a base that the compiler has moved to vector registers comes back
+  base = (const void*)((uint64_t)(uint32_t)uniform((int)((uint64_t)base >> 32)) << 32 | (uint32_t)uniform((int)(uint64_t)base));
+  lds = (uint32_t)uniform((int)lds);
   asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, %2" ::"s"(lds), "v"(offset), "s"(base) : "memory");
 }
 

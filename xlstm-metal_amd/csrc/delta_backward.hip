@@ -331,6 +331,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
       }
     }
   }
+  wait_loads();
   if (p.dc0 && mine && n < p.DV) {
 #pragma unroll
     for (int t = 0; t < 2 * DKB; ++t)

@@ -72,10 +72,20 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     return x[0];
   };
 
-  auto fetch = [&](const char* images, int chunk, int to) {
+  // Images, a quarter at a time: a CU takes 64 bytes a clock, and a wave whose load has to queue stands still.
+  constexpr int QUARTER = IMG / 1024 / PARTS / 4;
+  static_assert(QUARTER * PARTS * 4 * 1024 == IMG);
+  auto fetch = [&](const char* images, int chunk, int to, int quarter) {
     const char* img = images + (image0 + chunk) * (int64_t)IMG;
 #pragma unroll
-    for (int i = 0; i < IMG / 1024; i += PARTS) to_lds(lds_at + to + (i + part) * 1024, (i + part) * 1024 + lane * 16, img);
+    for (int j = 0; j < QUARTER; ++j) {
+      const int i = (quarter * QUARTER + j) * PARTS + part;
+      to_lds(lds_at + to + i * 1024, i * 1024 + lane * 16, img);
+    }
+  };
+  auto fetch_all = [&](const char* images, int chunk, int to) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) fetch(images, chunk, to, i);
   };
   auto fetch_factors = [&](int chunk) {
     if (part == 0) to_lds(lds_at + Lds::FACTORS + (chunk & 1) * 1024, lane * 16, p.prep.f + part0 + chunk);
@@ -108,7 +118,7 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
       for (int e = 0; e < 4; ++e) vn[x][e] = *(const T*)(base + v_at[x][e]);
   };
   // T's and P's rows of the wave's tokens, both halves of k
-  f16x8 th[TPW][2], tl[TPW][2], ph[TPW][2], pl[PAIR ? TPW : 1][2];
+  f16x8 th[TPW][2], tl[TPW][2], ph[TPW][2], pl[TPW][2], ph_next[TPW][2], pl_next[TPW][2];
   auto load_rows = [&](const f16_t* from, f16x8 (&to)[TPW][2]) {
 #pragma unroll
     for (int x = 0; x < TPW; ++x)
@@ -122,8 +132,8 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
   };
   auto load_p = [&](int chunk) {
     const f16_t* from = p.prep.p + (part0 + chunk) * (2 * FRAG_PLANE);
-    load_rows(from, ph);
-    if constexpr (PAIR) load_rows(from + FRAG_PLANE, pl);
+    load_rows(from, ph_next);
+    if constexpr (PAIR) load_rows(from + FRAG_PLANE, pl_next);
   };
 
   f32x4 st[2 * NB];  // the wave's rows of the state, times 1 / st_down (the same for all parts)
@@ -150,21 +160,55 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     for (int t = 0; t < 2 * NB; ++t) st[t] *= sc.up;
   }
 
-  // What is loaded past the last chunk is that one's again: as many loads are under way after every chunk.
-  constexpr int LATER = 4 * TPW + 4 * TPW;  // loads after a chunk's images, at least (V, T)
-  fetch(p.prep.k, 0, 0);
-  if constexpr (!STATES) fetch(p.prep.q, 0, Lds::Q);
+  fetch_all(p.prep.k, 0, 0);
+  if constexpr (!STATES) fetch_all(p.prep.q, 0, Lds::Q);
   fetch_factors(0);
   load_v(0);
   load_t(0);
   if constexpr (!STATES) load_p(0);
   const bool kept = STATES && block < p.kept.blocks;
   const uint32_t h_at = (uint32_t)(r * p.DV + 4 * gq) * sizeof(T);
+  Four<T> o[TPW];  // the chunk's H, written when the next one's loads have been waited for
+  auto store_h = [&](int chunk) {
+    const int t0 = chunk * L;
+    T* const to = ho + (int64_t)t0 * p.DV + n0;
+    const bool whole = t0 + L <= p.S && n0 + 16 <= p.DV && p.DV % 4 == 0;
+#pragma unroll
+    for (int x = 0; x < TPW; ++x) {
+      const int mt = part * TPW + x;
+      if (whole) {
+        *(Four<T>*)((char*)(to + (int64_t)(16 * mt) * p.DV) + h_at) = o[x];
+      } else if (t0 + 16 * mt + r < p.S) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (n0 + 4 * gq + e < p.DV) to[(int64_t)(16 * mt + r) * p.DV + 4 * gq + e] = o[x].e[e];
+      }
+    }
+  };
   for (int c = 0; c < p.chunks; ++c) {
-    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)" ::"n"(KST == 2 ? LATER : 0) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    // The chunk's only wait for memory.  The compiler does not count the loads into LDS: a wait of its own for a register,
+    // behind them, would be for some of them too, and they have only just left.
+    wait_loads();
+    lds_barrier();
     const int stage = KST == 2 ? (c & 1) * IMG : 0, next = c + 1 < p.chunks ? c + 1 : c;
+    if constexpr (!STATES) {
+      if (c) store_h(c - 1);
+#pragma unroll
+      for (int x = 0; x < TPW; ++x)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+          ph[x][s] = ph_next[x][s];
+          if constexpr (PAIR) pl[x][s] = pl_next[x][s];
+        }
+    }
+    // past the last chunk the last one comes again, unread
+    auto next_k = [&](int quarter) {
+      if (KST == 2) fetch(p.prep.k, next, stage ^ IMG, quarter);
+    };
+    auto next_q = [&](int quarter) {
+      if constexpr (!STATES) fetch(p.prep.q, next, Lds::Q, quarter);
+    };
+    next_k(0);
     const char *ki = lds + stage, *qi = lds + Lds::Q;
     const Factors* f = (const Factors*)(lds + Lds::FACTORS + (c & 1) * 1024);
 
@@ -183,10 +227,14 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
 #pragma unroll
       for (int pl = 0; pl < PK; ++pl)
 #pragma unroll
-        for (int mt = 0; mt < 4; ++mt) {
-          k[pl][mt] = rows_frag<DKP>(ki + pl * PLANE, mt, sb, r, gq);
-          if constexpr (!STATES) q[pl][mt] = rows_frag<DKP>(qi + pl * PLANE, mt, sb, r, gq);
-        }
+        for (int mt = 0; mt < 4; ++mt) k[pl][mt] = rows_frag<DKP>(ki + pl * PLANE, mt, sb, r, gq);
+      if constexpr (!STATES) {
+#pragma unroll
+        for (int pl = 0; pl < PK; ++pl)
+#pragma unroll
+          for (int mt = 0; mt < 4; ++mt) q[pl][mt] = rows_frag<DKP>(qi + pl * PLANE, mt, sb, r, gq);
+      }
+      __builtin_amdgcn_sched_barrier(0);  // every read under way at once, here and below
       split8(st[2 * s], st[2 * s + 1], hi, lo);
       if constexpr (STATES) {
         if (kept) {
@@ -210,6 +258,7 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
         }
       }
     }
+    next_k(1);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) *sums_at(mt, part) = ks[mt];
 #pragma unroll
@@ -223,12 +272,9 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     const Pow2 decayed = pow2_for(f->most, 0);  // U decayed is below 2 decayed.down times U
     most = state_max(st) * st_down;
     if (lane == 0) scales[2 * PARTS + part] = most;
-    lds_barrier();  // Q has been read too: its place takes the next chunk's; K's other stage has been free since the chunk began
-    if (next != c) {
-      if (KST == 2) fetch(p.prep.k, next, stage ^ IMG);
-      if constexpr (!STATES) fetch(p.prep.q, next, Lds::Q);
-      fetch_factors(next);
-    }
+    lds_barrier();  // Q has been read too: its place takes the next chunk's
+    fetch_factors(next);
+    next_q(0);
     // ---- 2: R
     f32x4 rr[TPW];
 #pragma unroll
@@ -238,6 +284,7 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
       for (int e = 0; e < 4; ++e) rr[x][e] = fmaf(-in[x][e], sum[e], to_f32(vn[x][e]));
     }
     load_v(next);
+    if constexpr (!STATES) load_p(next);
     const Pow2 rs = pow2_for(wave_max_all(abs_max(rr)));
 #pragma unroll
     for (int x = 0; x < TPW; ++x) {
@@ -245,26 +292,41 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
       split4(rr[x], rs.up, hi, lo);
       *((f16x8*)(lds + Lds::R) + (part * TPW + x) * 64 + lane) = join(hi, lo);
     }
+    next_k(2);
     if (lane == 0) scales[part] = rs.down;
     lds_barrier();
     // ---- 3: U
-    f16x8 rh[2], rl[2];
-    const float r_down = largest(scales);
-    auto planes = [&](const f16x8* from, const float* of, float down, f16x8 (&hi)[2], f16x8 (&lo)[2]) {
+    f16x8 raw[4], rh[2], rl[2];
+    float of[PARTS];
+    auto read_scales = [&](int from, float (&to)[PARTS]) {
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) to[i] = scales[from * PARTS + i];
+    };
+    auto read4 = [&](int at) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) raw[i] = *((const f16x8*)(lds + at) + i * 64 + lane);
+    };
+    read_scales(0, of);
+    read4(Lds::R);
+    __builtin_amdgcn_sched_barrier(0);
+    // of a part's scale to the largest's
+    auto shifts = [&](const float (&of)[PARTS], float down, _Float16 (&by)[PARTS]) {
+#pragma unroll
+      for (int i = 0; i < PARTS; ++i) by[i] = ratio(__int_as_float(uniform(__float_as_int(of[i]))), down);
+    };
+    auto planes = [&](const _Float16 (&by)[PARTS], f16x8 (&hi)[2], f16x8 (&lo)[2]) {
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        f16x4 h[2], l[2];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const f16x8 x = from[(2 * s + i) * 64 + lane] * ratio(__int_as_float(uniform(__float_as_int(of[(2 * s + i) / TPW]))), down);
-          h[i] = f16x4{x[0], x[1], x[2], x[3]};
-          l[i] = f16x4{x[4], x[5], x[6], x[7]};
-        }
-        hi[s] = join(h[0], h[1]);
-        lo[s] = join(l[0], l[1]);
+        const f16x8 a = raw[2 * s] * by[2 * s / TPW], b = raw[2 * s + 1] * by[(2 * s + 1) / TPW];
+        hi[s] = join(f16x4{a[0], a[1], a[2], a[3]}, f16x4{b[0], b[1], b[2], b[3]});
+        lo[s] = join(f16x4{a[4], a[5], a[6], a[7]}, f16x4{b[4], b[5], b[6], b[7]});
       }
     };
-    planes((const f16x8*)(lds + Lds::R), scales, r_down, rh, rl);
+    _Float16 by[PARTS];
+    const float r_down = largest(of);
+    shifts(of, r_down, by);
+    planes(by, rh, rl);
+    next_q(1);
     f32x4 u[TPW], w[TPW];
     const float back = t_scale * r_down;
 #pragma unroll
@@ -296,6 +358,8 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
         else *((f16x4*)(lds + Lds::U) + mt * 64 + lane) = hi;
       }
     }
+    next_k(3);
+    next_q(2);
     if (lane == 0) scales[PARTS + part] = us.down;
     if constexpr (!STATES) {
 #pragma unroll
@@ -303,27 +367,53 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     }
     lds_barrier();
     // ---- 4: the state
-    const float u_down = largest(scales + PARTS), w_down = u_down * decayed.down * 2.f;
+    f16x8 kc[2 * NB][PK][2], raw_u[PAIR ? 4 : 1];
+    f16x4 half_u[PAIR || STATES ? 1 : 4];
+    f32x4 qs[STATES ? 1 : TPW];
+    float of_u[PARTS], of_s[PARTS];
+    read_scales(1, of_u);
+    read_scales(2, of_s);
+    read4(Lds::UD);
+#pragma unroll
+    for (int t = 0; t < 2 * NB; ++t)
+#pragma unroll
+      for (int pl = 0; pl < PK; ++pl)
+#pragma unroll
+        for (int s = 0; s < 2; ++s) kc[t][pl][s] = columns_frag<DKP>(ki + pl * PLANE, 2 * NB * part + t, s, r, gq);
+    if constexpr (!STATES) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        if constexpr (PAIR) raw_u[i] = *((const f16x8*)(lds + Lds::U) + i * 64 + lane);
+        else half_u[i] = *((const f16x4*)(lds + Lds::U) + i * 64 + lane);
+      }
+    }
+    __builtin_amdgcn_sched_barrier(0);
+    const float u_down = largest(of_u), w_down = u_down * decayed.down * 2.f;
     // U decayed is below 2^15 w_down
-    const Pow2 sc = pow2_for(fmaxf(largest(scales + 2 * PARTS) * keep, w_down * 32767.f), STATE);
+    const Pow2 sc = pow2_for(fmaxf(largest(of_s) * keep, w_down * 32767.f), STATE);
     f16x8 wh[2], wl[2];
-    planes((const f16x8*)(lds + Lds::UD), scales + PARTS, u_down, wh, wl);
+    shifts(of_u, u_down, by);
+    planes(by, wh, wl);
+    if constexpr (!STATES) {
+#pragma unroll
+      for (int x = 0; x < TPW; ++x) qs[x] = sum_of(part * TPW + x);
+    }
     const _Float16 shift = (_Float16)(w_down * sc.up);  // to the state's scale: 2^-8 or less
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       wh[s] *= shift;
       wl[s] *= shift;
     }
+    next_q(3);
     const float up = keep * st_down * sc.up;
 #pragma unroll
     for (int t = 0; t < 2 * NB; ++t) {
       f32x4 y = st[t] * up, y2 = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
-        const f16x8 k = columns_frag<DKP>(ki, 2 * NB * part + t, s, r, gq);
-        if constexpr (PK == 2) y2 = mfma(columns_frag<DKP>(ki + PLANE, 2 * NB * part + t, s, r, gq), wh[s], y2);
-        y2 = mfma(k, wl[s], y2);
-        y = mfma(k, wh[s], y);
+        if constexpr (PK == 2) y2 = mfma(kc[t][1][s], wh[s], y2);
+        y2 = mfma(kc[t][0][s], wl[s], y2);
+        y = mfma(kc[t][0][s], wh[s], y);
       }
       st[t] = y + y2;
     }
@@ -348,26 +438,17 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     } else {  // ---- H
       f16x8 uh[2], ul[2];
       if constexpr (PAIR) {
-        planes((const f16x8*)(lds + Lds::U), scales + PARTS, u_down, uh, ul);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) raw[i] = raw_u[i];
+        planes(by, uh, ul);
       } else {
 #pragma unroll
-        for (int s = 0; s < 2; ++s) {
-          f16x4 x[2];
-#pragma unroll
-          for (int i = 0; i < 2; ++i)
-            x[i] = *((const f16x4*)(lds + Lds::U) + (2 * s + i) * 64 + lane) *
-                   ratio(__int_as_float(uniform(__float_as_int(scales[PARTS + (2 * s + i) / TPW]))), u_down);
-          uh[s] = join(x[0], x[1]);
-        }
+        for (int s = 0; s < 2; ++s) uh[s] = join(half_u[2 * s] * by[2 * s / TPW], half_u[2 * s + 1] * by[(2 * s + 1) / TPW]);
       }
       const float pu = p_scale * u_down;
-      const int t0 = c * L;
-      T* const to = ho + (int64_t)t0 * p.DV + n0;
-      const bool whole = t0 + L <= p.S && n0 + 16 <= p.DV && p.DV % 4 == 0;
 #pragma unroll
       for (int x = 0; x < TPW; ++x) {
         const int mt = part * TPW + x;
-        const f32x4 qs = sum_of(mt);
         f32x4 y = {0.f, 0.f, 0.f, 0.f};
         y = mfma(uh[0], ph[x][0], y);
         if constexpr (PAIR) {
@@ -381,23 +462,17 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
             y = mfma(uh[1], pl[x][1], y);
           }
         }
-        const Four<T> o = rounded4<T>(y * pu + qs * fq[x]);
-        if (whole) {
-          *(Four<T>*)((char*)(to + (int64_t)(16 * mt) * p.DV) + h_at) = o;
-        } else if (t0 + 16 * mt + r < p.S) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (n0 + 4 * gq + e < p.DV) to[(int64_t)(16 * mt + r) * p.DV + 4 * gq + e] = o.e[e];
-        }
+        o[x] = rounded4<T>(y * pu + qs[x] * fq[x]);
       }
-      load_p(next);
     }
     st_down = sc.down;
     if (KST == 1) {
       lds_barrier();
-      if (next != c) fetch(p.prep.k, next, 0);
+      fetch_all(p.prep.k, next, 0);
     }
   }
+  if constexpr (!STATES) store_h(p.chunks - 1);
+  wait_loads();
   if (p.c_last && n < p.DV) {
 #pragma unroll
     for (int t = 0; t < 2 * NB; ++t)
@@ -699,6 +774,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
       }
     }
   }
+  wait_loads();
   if (p.c_last && n < p.DV) {
 #pragma unroll
     for (int t = 0; t < 2 * DKB; ++t)
