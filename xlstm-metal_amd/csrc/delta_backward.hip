@@ -156,7 +156,6 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
     }
     dh_scale = p.kept.dhs[(part0 + chunk) * p.kept.blocks + block];
   };
-  constexpr int LATER = 4 * LOWER + 2;  // loads after a chunk's fetch, at least
   const int last = p.chunks - 1;
 #pragma unroll
   for (int s = 0; s < DKB; ++s) fetch(last, STAGES == 2 ? last & 1 : 0, s);
@@ -165,9 +164,10 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
   load_t(last);
   load_dh(last);
   for (int c = last; c >= 0; --c) {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STAGES == 2 ? LATER : 0) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    // The chunk's only wait for memory.  The compiler does not count the loads into LDS: a wait of its own for a register,
+    // behind them, would be for all of them too, and they have only just left.
+    wait_loads();
+    lds_barrier();
     const int stage = STAGES == 2 ? c & 1 : 0, next = c > 0 ? c - 1 : c;
     if (next != c) fetch_factors(next);
     const char *ki = lds + stage * STAGE, *qi = ki + IMG;
