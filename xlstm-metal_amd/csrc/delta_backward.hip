@@ -90,11 +90,12 @@ struct BackArgs {
 };
 
 // As the forward's scan (delta_chunkwise.hip): operands are read ahead of their products, the next chunk's are on their way.
+// Four waves take a block each and bring the images together; a wave on its own has a second one that only brings them.
 template <typename T, int DKB, int STAGES, int W>
-__global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
+__global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(BackArgs p) {
   constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
-  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  const int lane = threadIdx.x & 63, in = uniform(threadIdx.x >> 6), wave = W == 1 ? 0 : in;
   const int r = lane & 15, gq = lane >> 4;
   const int all = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
   const int bh = uniform(all / p.slices), slice = all - bh * p.slices, b = uniform(bh / p.NH), h = bh - b * p.NH;
@@ -120,6 +121,25 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
     to_lds(lds_at + STAGES * STAGE + (chunk & 1) * 2048, lane * 16, p.prep.f + part0 + chunk);
     to_lds(lds_at + STAGES * STAGE + (chunk & 1) * 2048 + 1024, 1024 + lane * 16, p.prep.f + part0 + chunk);
   };
+  const int last = p.chunks - 1;
+  if (W == 1 && in == 1) {
+    for (int c = last; c >= 0; --c) {  // the other wave's barriers
+      if (c == last || STAGES == 1) {
+#pragma unroll
+        for (int s = 0; s < DKB; ++s) fetch(c, STAGES == 2 ? c & 1 : 0, s);
+        fetch_factors(c);
+      }
+      wait_loads();
+      lds_barrier();
+      if (STAGES == 2 && c > 0) {
+#pragma unroll
+        for (int s = 0; s < DKB; ++s) fetch(c - 1, (c - 1) & 1, s);
+        fetch_factors(c - 1);
+      }
+      if (STAGES == 1) lds_barrier();
+    }
+    return;
+  }
   f32x4 st[2 * DKB];  // the state's gradient times 1 / st_down
 #pragma unroll
   for (int t = 0; t < 2 * DKB; ++t)
@@ -156,10 +176,11 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
     }
     dh_scale = p.kept.dhs[(part0 + chunk) * p.kept.blocks + block];
   };
-  const int last = p.chunks - 1;
+  if (W != 1) {
 #pragma unroll
-  for (int s = 0; s < DKB; ++s) fetch(last, STAGES == 2 ? last & 1 : 0, s);
-  fetch_factors(last);
+    for (int s = 0; s < DKB; ++s) fetch(last, STAGES == 2 ? last & 1 : 0, s);
+    fetch_factors(last);
+  }
   load_p(last);
   load_t(last);
   load_dh(last);
@@ -169,7 +190,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
     wait_loads();
     lds_barrier();
     const int stage = STAGES == 2 ? c & 1 : 0, next = c > 0 ? c - 1 : c;
-    if (next != c) fetch_factors(next);
+    if (W != 1 && next != c) fetch_factors(next);
     const char *ki = lds + stage * STAGE, *qi = ki + IMG;
     const Factors* f = (const Factors*)(lds + STAGES * STAGE + (c & 1) * 2048);
     const int64_t at = (part0 + c) * p.kept.blocks + block;
@@ -197,7 +218,7 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
       if (s + 1 < DKB) read(s + 1);
-      if (STAGES == 2) fetch(next, stage ^ 1, s);
+      if (W != 1 && STAGES == 2) fetch(next, stage ^ 1, s);
       __builtin_amdgcn_sched_barrier(0);
       const f16x8 hi = sh[s & 1], lo = sl[s & 1];
       if (mine) {
@@ -322,10 +343,8 @@ __global__ __launch_bounds__(64 * W, 1) void delta_back_kernel(BackArgs p) {
       __builtin_amdgcn_sched_barrier(0);
     }
     if (STAGES == 1) {
-      asm volatile("s_waitcnt lgkmcnt(0)" ::: "memory");
-      __builtin_amdgcn_s_barrier();
-      asm volatile("" ::: "memory");
-      if (next != c) {
+      lds_barrier();
+      if (W != 1 && next != c) {
 #pragma unroll
         for (int s = 0; s < DKB; ++s) fetch(next, 0, s);
       }
@@ -956,7 +975,7 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
       : s.dkp() == 64    ? (const void*)delta_back_kernel<T, 2, 2, 1>
         : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2, 1> : (const void*)delta_back_kernel<T, 8, S8, 1>;
   if (e == hipSuccess)
-    e = launch(kern, (int64_t)s.B * s.NH * slices, 1, 64 * waves, stages * 2 * s.image_bytes() + 2 * 2048, &back, st);
+    e = launch(kern, (int64_t)s.B * s.NH * slices, 1, waves == 1 ? 128 : 64 * waves, stages * 2 * s.image_bytes() + 2 * 2048, &back, st);
   GradArgs grad{v, {s.vs[0], s.vs[1], s.vs[2]}, group == 1 ? dq : (void*)dqp, group == 1 ? dk : (void*)dkp, dv, dg, dbeta, prep, kept,
                 s.NH, group, s.S, s.DK, s.DV, chunks, s.dtype_gates, s.scale, false};
   constexpr int VW = 16 / sizeof(T);
