@@ -44,12 +44,12 @@ struct ScanLds {
 // STATES: U and the state before each chunk are kept for the backward, and nothing else is written.
 // PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32).
 template <typename T, int DKB, int PARTS, int KST, bool STATES>
-__global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
+__global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p) {
   constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE;
   constexpr int TPW = 4 / PARTS, NB = DKB / PARTS;  // a wave's tiles of 16 tokens, its 32s of DQK
   constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
   using Lds = ScanLds<DKB, PK, PARTS, KST, !STATES, PAIR>;
-  static_assert(DKB % PARTS == 0 && IMG / 1024 % PARTS == 0 && Lds::BYTES <= 160 * 1024);
+  static_assert(DKB % PARTS == 0 && Lds::BYTES <= 160 * 1024);
   extern __shared__ __align__(1024) char lds[];
   const int lane = threadIdx.x & 63, part = uniform(threadIdx.x >> 6);
   const int r = lane & 15, gq = lane >> 4;
@@ -72,24 +72,35 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     return x[0];
   };
 
-  // Images, a quarter at a time: a CU takes 64 bytes a clock, and a wave whose load has to queue stands still.
-  constexpr int QUARTER = IMG / 1024 / PARTS / 4;
-  static_assert(QUARTER * PARTS * 4 * 1024 == IMG);
-  auto fetch = [&](const char* images, int chunk, int to, int quarter) {
-    const char* img = images + (image0 + chunk) * (int64_t)IMG;
+  if (part == PARTS) {  // brings the images: a wave whose load into LDS has to queue stands still
+    auto fetch = [&](const char* images, int chunk, int to) {
+      const char* img = images + (image0 + chunk) * (int64_t)IMG;
 #pragma unroll
-    for (int j = 0; j < QUARTER; ++j) {
-      const int i = (quarter * QUARTER + j) * PARTS + part;
-      to_lds(lds_at + to + i * 1024, i * 1024 + lane * 16, img);
+      for (int i = 0; i < IMG / 1024; ++i) to_lds(lds_at + to + i * 1024, i * 1024 + lane * 16, img);
+    };
+    auto fetch_factors = [&](int chunk) { to_lds(lds_at + Lds::FACTORS + (chunk & 1) * 1024, lane * 16, p.prep.f + part0 + chunk); };
+    fetch(p.prep.k, 0, 0);
+    if constexpr (!STATES) fetch(p.prep.q, 0, Lds::Q);
+    fetch_factors(0);
+    lds_barrier();  // the other waves' barriers: of the first state,
+    for (int c = 0; c < p.chunks; ++c) {
+      wait_loads();
+      lds_barrier();  // a chunk's begin,
+      if (KST == 2 && c + 1 < p.chunks) fetch(p.prep.k, c + 1, ((c + 1) & 1) * IMG);
+      lds_barrier();  // the partial sums: Q has been read,
+      if (c + 1 < p.chunks) {
+        if constexpr (!STATES) fetch(p.prep.q, c + 1, Lds::Q);
+        fetch_factors(c + 1);
+      }
+      lds_barrier();  // R,
+      lds_barrier();  // U
+      if (KST == 1) {
+        lds_barrier();
+        if (c + 1 < p.chunks) fetch(p.prep.k, c + 1, 0);
+      }
     }
-  };
-  auto fetch_all = [&](const char* images, int chunk, int to) {
-#pragma unroll
-    for (int i = 0; i < 4; ++i) fetch(images, chunk, to, i);
-  };
-  auto fetch_factors = [&](int chunk) {
-    if (part == 0) to_lds(lds_at + Lds::FACTORS + (chunk & 1) * 1024, lane * 16, p.prep.f + part0 + chunk);
-  };
+    return;
+  }
   // Tokens 16 mt + 4 gq + e of column n, mt of this wave.  Past the last token the last one is read again (its beta is 0 there: T
   // has zeros in its column), past the last column the last one: those columns are computed and not written.
   const int nc = n < p.DV ? n : p.DV - 1, row_step = (int)p.vs[2];
@@ -160,9 +171,6 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     for (int t = 0; t < 2 * NB; ++t) st[t] *= sc.up;
   }
 
-  fetch_all(p.prep.k, 0, 0);
-  if constexpr (!STATES) fetch_all(p.prep.q, 0, Lds::Q);
-  fetch_factors(0);
   load_v(0);
   load_t(0);
   if constexpr (!STATES) load_p(0);
@@ -186,8 +194,7 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     }
   };
   for (int c = 0; c < p.chunks; ++c) {
-    // The chunk's only wait for memory.  The compiler does not count the loads into LDS: a wait of its own for a register,
-    // behind them, would be for some of them too, and they have only just left.
+    // The chunk's only wait for memory: T, V and P left a good part of a chunk ago.
     wait_loads();
     lds_barrier();
     const int stage = KST == 2 ? (c & 1) * IMG : 0, next = c + 1 < p.chunks ? c + 1 : c;
@@ -201,14 +208,6 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
           if constexpr (PAIR) pl[x][s] = pl_next[x][s];
         }
     }
-    // past the last chunk the last one comes again, unread
-    auto next_k = [&](int quarter) {
-      if (KST == 2) fetch(p.prep.k, next, stage ^ IMG, quarter);
-    };
-    auto next_q = [&](int quarter) {
-      if constexpr (!STATES) fetch(p.prep.q, next, Lds::Q, quarter);
-    };
-    next_k(0);
     const char *ki = lds + stage, *qi = lds + Lds::Q;
     const Factors* f = (const Factors*)(lds + Lds::FACTORS + (c & 1) * 1024);
 
@@ -258,7 +257,6 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
         }
       }
     }
-    next_k(1);
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) *sums_at(mt, part) = ks[mt];
 #pragma unroll
@@ -272,9 +270,7 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     const Pow2 decayed = pow2_for(f->most, 0);  // U decayed is below 2 decayed.down times U
     most = state_max(st) * st_down;
     if (lane == 0) scales[2 * PARTS + part] = most;
-    lds_barrier();  // Q has been read too: its place takes the next chunk's
-    fetch_factors(next);
-    next_q(0);
+    lds_barrier();
     // ---- 2: R
     f32x4 rr[TPW];
 #pragma unroll
@@ -292,7 +288,6 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
       split4(rr[x], rs.up, hi, lo);
       *((f16x8*)(lds + Lds::R) + (part * TPW + x) * 64 + lane) = join(hi, lo);
     }
-    next_k(2);
     if (lane == 0) scales[part] = rs.down;
     lds_barrier();
     // ---- 3: U
@@ -326,7 +321,6 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
     const float r_down = largest(of);
     shifts(of, r_down, by);
     planes(by, rh, rl);
-    next_q(1);
     f32x4 u[TPW], w[TPW];
     const float back = t_scale * r_down;
 #pragma unroll
@@ -358,8 +352,6 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
         else *((f16x4*)(lds + Lds::U) + mt * 64 + lane) = hi;
       }
     }
-    next_k(3);
-    next_q(2);
     if (lane == 0) scales[PARTS + part] = us.down;
     if constexpr (!STATES) {
 #pragma unroll
@@ -404,7 +396,6 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
       wh[s] *= shift;
       wl[s] *= shift;
     }
-    next_q(3);
     const float up = keep * st_down * sc.up;
 #pragma unroll
     for (int t = 0; t < 2 * NB; ++t) {
@@ -466,10 +457,7 @@ __global__ __launch_bounds__(64 * PARTS) void delta_scan_kernel(ScanArgs p) {
       }
     }
     st_down = sc.down;
-    if (KST == 1) {
-      lds_barrier();
-      fetch_all(p.prep.k, next, 0);
-    }
+    if (KST == 1) lds_barrier();
   }
   if constexpr (!STATES) store_h(p.chunks - 1);
   wait_loads();
@@ -800,7 +788,7 @@ Choice choice(bool many) {
   constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
   if (many)
     return {(const void*)delta_scan_wave_kernel<T, DKB, KST, STATES>, 256, 4, KST * (STATES ? 1 : 2) * PK * L * DKB * 64 + 2 * 1024};
-  return {(const void*)delta_scan_kernel<T, DKB, PARTS, KST, STATES>, 64 * PARTS, 1,
+  return {(const void*)delta_scan_kernel<T, DKB, PARTS, KST, STATES>, 64 * PARTS + 64, 1,
           ScanLds<DKB, PK, PARTS, KST, !STATES, PAIR>::BYTES};
 }
 template <typename T, bool STATES>
