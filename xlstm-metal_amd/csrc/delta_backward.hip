@@ -90,7 +90,8 @@ struct BackArgs {
 };
 
 // As the forward's scan (delta_chunkwise.hip): operands are read ahead of their products, the next chunk's are on their way.
-// Four waves take a block each and bring the images together; a wave on its own has a second one that only brings them.
+// Four waves take a block each and bring the images together; a wave on its own has a second one that only brings them (a load into
+// LDS that has to queue stops its wave: 177 us without, 157 with, at 8192 tokens of 128 x 256, 2.5 a chunk).
 template <typename T, int DKB, int STAGES, int W>
 __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(BackArgs p) {
   constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
@@ -965,17 +966,22 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
   hipError_t e = launch((const void*)delta_turn_kernel<T>, s.parts(), (kept.blocks + 3) / 4, 256, 0, &turn, st);
   if (e == hipSuccess)
     if (const int rc = launch_scan(s, v, c0, nullptr, nullptr, prep, &kept, st, who)) return rc;
-  const int waves = (int64_t)s.B * s.NH * ((kept.blocks + 3) / 4) < 256 ? 1 : 4, slices = (kept.blocks + waves - 1) / waves;
-  BackArgs back{dc_last, dc0, prep, kept, s.NH, group, s.DK, s.DV, chunks, slices};
   constexpr int S8 = is_f32<T>::value ? 1 : 2;
   const int stages = s.dkp() == 256 ? S8 : 2;
+  // A lone wave a block where two workgroups a CU (one, if no two fit) take all blocks, else four blocks a workgroup.  us of whole calls,
+  // 2048 tokens, lone waves and fours: bf16 128 x 256, 256 blocks 252, 277; 512 433, 454; 768 626, 572; 1024 755, 689; 64 x 256, 512
+  // blocks 346, 357; 1024 637, 577; 256 x 512, 512 blocks 597, 548; float32 128 x 256, 512 blocks of 1024 tokens 362, 349.
+  const int64_t scan_lds = stages * 2 * s.image_bytes() + 2 * 2048;
+  const int waves = (int64_t)s.B * s.NH * kept.blocks <= (scan_lds <= 80 * 1024 ? 512 : 256) ? 1 : 4;
+  const int slices = (kept.blocks + waves - 1) / waves;
+  BackArgs back{dc_last, dc0, prep, kept, s.NH, group, s.DK, s.DV, chunks, slices};
   const void* kern =
       waves == 4 ? s.dkp() == 64    ? (const void*)delta_back_kernel<T, 2, 2, 4>
                    : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2, 4> : (const void*)delta_back_kernel<T, 8, S8, 4>
       : s.dkp() == 64    ? (const void*)delta_back_kernel<T, 2, 2, 1>
         : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2, 1> : (const void*)delta_back_kernel<T, 8, S8, 1>;
   if (e == hipSuccess)
-    e = launch(kern, (int64_t)s.B * s.NH * slices, 1, waves == 1 ? 128 : 64 * waves, stages * 2 * s.image_bytes() + 2 * 2048, &back, st);
+    e = launch(kern, (int64_t)s.B * s.NH * slices, 1, waves == 1 ? 128 : 64 * waves, scan_lds, &back, st);
   GradArgs grad{v, {s.vs[0], s.vs[1], s.vs[2]}, group == 1 ? dq : (void*)dqp, group == 1 ? dk : (void*)dkp, dv, dg, dbeta, prep, kept,
                 s.NH, group, s.S, s.DK, s.DV, chunks, s.dtype_gates, s.scale, false};
   constexpr int VW = 16 / sizeof(T);

@@ -11,9 +11,10 @@
 //   3  U = T R of the wave's tokens, to LDS as f16 planes, decayed for the state and as it is for H
 //   4  S = c_L S + K^T U of the wave's rows; H = Q S + P U of the wave's tokens
 //
-// The images of K and Q come to LDS straight from memory: K a chunk ahead, Q from where this chunk's has been read; T, P, V of the
-// next chunk wait in registers.  H is formed turned (columns down, tokens across): a lane holds four neighbours of a row.
-// Measured (bf16): 8192 tokens of 4 heads of 128 x 256 155 us, 1.2 a chunk; 8192 of 16 x 4 of 256 x 256 in 64 heads' blocks 590.
+// The images of K and Q come to LDS straight from memory, K a chunk ahead, Q into the place of this chunk's when it has been read;
+// in delta_scan_kernel by a wave of its own (a load into LDS that has to queue stops its wave).  T, P and V of the next chunk wait in
+// registers.  H is formed turned (columns down, tokens across): a lane holds four neighbours of a row.  Measured (bf16): 2 x 4096 tokens
+// of 8 heads of 128 x 256 136 us, 2.1 a chunk; 4 x 8192 of 8 heads of 256 x 512 580, 4.5 a chunk.
 #include "delta.h"
 
 namespace xl {
@@ -778,9 +779,9 @@ struct Choice {
   const void* kern;
   int threads, blocks, lds;  // threads of a workgroup, its blocks of 16 columns
 };
-// Few blocks: one a workgroup, by as many waves as there are 32s of DQK, up to 4.  Many: one a wave, 4 a workgroup.  us, both ways:
-//   256 blocks, DQK 128, 64 chunks     171 (a wave), 155 (4 waves)
-//   1024 blocks, DQK 256, 128 chunks   590 (a wave), 834 (2 waves a block, 4 blocks a workgroup: T and P come to each)
+// At most a block of columns a CU: by as many waves as there are 32s of DQK, up to 4.  More: one a wave, 4 a workgroup.  us of whole
+// calls of bf16, 2048 tokens, both ways (waves of a block, a wave): 128 x 256, 256 blocks 91, 112; 512 171, 128; 1024 316, 165; 2048
+// 613, 335; 64 x 256, 512 blocks 104, 98; 256 x 512, 512 blocks 181, 147; 1024 365, 180.
 template <typename T, int DKB, bool STATES>
 Choice choice(bool many) {
   constexpr int PK = is_f32<T>::value ? 2 : 1, KST = DKB == 8 && PK == 2 && !STATES ? 1 : 2;  // K's pairs twice and Q's do not fit
@@ -803,7 +804,7 @@ int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* 
   ScanArgs a{v, {s.vs[0], s.vs[1], s.vs[2]}, c0, h, c_last, prep, {}, s.NH, s.NH / s.NHK, s.S, s.DK, s.DV, s.chunks(), 0};
   if (kept) a.kept = *kept;
   const int blocks = kept ? kept->blocks : (s.DV + 15) / 16;
-  const bool many = (int64_t)s.B * s.NH * ((blocks + 3) / 4) >= 256;
+  const bool many = (int64_t)s.B * s.NH * blocks > 256;
   Choice use{};
   auto choose = [&](auto t) {
     using T = decltype(t);
