@@ -14,7 +14,7 @@
 // The images of K and Q come to LDS straight from memory, K a chunk ahead, Q into the place of this chunk's when it has been read;
 // in delta_scan_kernel by a wave of its own (a load into LDS that has to queue stops its wave).  T, P and V of the next chunk wait in
 // registers.  H is formed turned (columns down, tokens across): a lane holds four neighbours of a row.  Measured (bf16): 2 x 4096 tokens
-// of 8 heads of 128 x 256 136 us, 2.1 a chunk; 4 x 8192 of 8 heads of 256 x 512 580, 4.5 a chunk.
+// of 8 heads of 128 x 256 136 us, 2.1 a chunk; 4 x 8192 of 8 heads of 256 x 512 520 to 560, 4.2 a chunk.
 #include "delta.h"
 
 namespace xl {
@@ -548,7 +548,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
   }
 
   // T, P and V of the next chunk wait in registers, K, Q and the factors in LDS.  What is loaded past the last chunk is that one's
-  // again: as many loads are under way after every chunk.
+  // again.
   f16x8 th[LOWER], tl[LOWER], ph[LOWER], pl[PAIR ? LOWER : 1];
   auto load_t = [&](int chunk) {
     const f16_t* from = p.prep.t + (part0 + chunk) * (2 * FRAG_PLANE);
@@ -560,7 +560,6 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
     load_lower(from, lane, ph);
     if constexpr (PAIR) load_lower(from + FRAG_PLANE, lane, pl);
   };
-  constexpr int LATER = 16 + 2 * LOWER;  // loads after a chunk's fetch, at least
 #pragma unroll
   for (int s = 0; s < DKB; ++s) fetch(0, 0, s);
   fetch_factors(0);
@@ -571,9 +570,10 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
   const bool kept = STATES && block < p.kept.blocks;
   const uint32_t h_at = (uint32_t)(r * p.DV + 4 * gq) * sizeof(T);
   for (int c = 0; c < p.chunks; ++c) {
-    asm volatile("s_waitcnt vmcnt(%0)" ::"n"(STAGES == 2 ? LATER : 0) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
+    // The chunk's only wait for memory: the compiler does not count the loads into LDS, and its waits for a register behind them were
+    // for some of them too (666 us, 627 so).
+    wait_loads();
+    lds_barrier();
     const int stage = STAGES == 2 ? c & 1 : 0, next = c + 1 < p.chunks ? c + 1 : c;
     if (next != c) fetch_factors(next);
     const char *ki = lds + stage * STAGE, *qi = ki + IMG;
