@@ -18,6 +18,10 @@
 // are added at a term's later token and taken off at its earlier one, so what does not pass t cancels to float32's rounding.)
 //
 // Heads of v that share q and k write their dQ and dK in float32, and a last kernel adds them in order.
+//
+// Measured (bf16, 2 x 4096 tokens of 8 heads of 128 x 256), us: first kernel 37, dH by columns 17, states 121, scan backwards
+// 155, chunks' gradients 165.  The scans are bound by the chain of one chunk's step; the last by its waits between products
+// (its 377 MB are 73 us of a copy).
 #include "delta.h"
 
 namespace xl {

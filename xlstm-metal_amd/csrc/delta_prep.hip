@@ -7,6 +7,9 @@
 // T by 16 x 16 blocks, in float32: each wave inverts one diagonal block by substitution (a lane a column), then walks down
 // its block column, T_ij = -T_ii sum_l A_il T_lj, with v_mfma_f32_16x16x4_f32, whose result is the next one's operand as it
 // stands.  Everything a scan reads as an operand (T diag(beta), P) is written in operand order, 16 bytes a lane.
+//
+// Large: bound by memory (bf16, 4 x 8192 tokens of 8 heads of 256: 136 to 144 us for 0.64 GB in and out, which a copy takes
+// 124 for); few chunks: by the chain of one (13 chunks of 8 heads of 128: 12.8 us).
 #include "delta.h"
 
 namespace xl {
@@ -304,6 +307,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
     block_max(m, red);
 #pragma unroll
     for (int mat = 0; mat < MATS; ++mat) {
+      constexpr bool P_LO = BWD || !std::is_same_v<T, bf16_t>;  // bf16's scan takes P as one plane
       const float up = pow2_for(m[mat], 10).up;
       f16_t* to = (mat == 0 ? p.out.t : mat == 1 ? p.out.p : mat == 2 ? p.out.tt : p.out.pt) + part * (2 * FRAG_PLANE);
 #pragma unroll
@@ -312,7 +316,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
         split8<true>(x[mat][half], up, hi, lo);
         f16_t* at = to + ((wave + 4 * half) * 64 + lane) * 8;
         *(f16x8*)at = hi;
-        *(f16x8*)(at + FRAG_PLANE) = lo;
+        if (mat != 1 || P_LO) *(f16x8*)(at + FRAG_PLANE) = lo;
       }
     }
     if (tid == 0) {
