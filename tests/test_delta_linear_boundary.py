@@ -52,6 +52,12 @@ def test_delta_refuses(lib, which):
         assert delta(lib, which, S=0, q=None, h=None) == 0  # nothing to do
 
 
+@pytest.mark.parametrize("which", ["recurrent_fwd", "chunkwise_fwd", "chunkwise_bwd"])
+def test_delta_refuses_more_threads_than_a_launch_has(lib, which):
+    assert delta(lib, which, B=1 << 19, NH=1, NHK=1, S=1, DQK=1, DV=1024) == -2 and b"too large" in lib.xl_last_error()
+    assert delta(lib, which, B=(1 << 24) - 1, NH=1, NHK=1, S=1, DQK=1, DV=33) == -2
+
+
 def test_delta_workspace_sizes(lib):
     fwd, bwd = lib.xl_gated_delta_chunkwise_workspace_size, lib.xl_gated_delta_chunkwise_bwd_workspace_size
     assert fwd(1, 2, 2, 0, 64, 64, 1) == bwd(1, 2, 2, 0, 64, 64, 1) == 0

@@ -245,3 +245,24 @@ def test_no_tokens(gpu_case):
 def test_long(gpu_case):
     """2000 tokens, shared heads, against the 64-bit recurrence."""
     check_all(*inputs((1, 4, 2, 2000, 64, 32), F32, F32, 13))
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 2, 500, 64, 64), (2, 2, 1, 130, 128, 100), (1, 1, 1, 200, 256, 32)])
+def test_float16_is_off_by_its_rounding(gpu_case, shape):
+    """float16's operands in the backward are pairs (2^-22): by the bar's count 10 x (2^-22 + 4.5 2^-24) = 5.1e-6 of the parts' norm
+    beside the gradient's own rounding to float16 (2e-4 in norm), of which 2 parts' and the cancellation of dg's sums (20 for keys of
+    norm 1 and decays near 1) make 2e-4 at most.  One plane's 10 x 2^-11 would be 10 to 20 times that."""
+    B, NH, NHK, S, DK, DV = shape
+    import xlstm_hip
+    r = torch.Generator().manual_seed(S)
+    n = lambda *s: torch.randn(*s, generator=r)  # noqa: E731
+    unit = lambda t: torch.nn.functional.normalize(t, dim=-1)  # noqa: E731
+    x = [t.to(F16).to(dev()) for t in (unit(n(B, NHK, S, DK)), unit(n(B, NHK, S, DK)), n(B, NH, S, DV), -0.2 * torch.rand(B, NH, S, generator=r),
+                                       torch.rand(B, NH, S, generator=r))] + [None]
+    dh = n(B, NH, S, DV).to(F16).to(dev())
+    scale = DK ** -0.5
+    got = gradients(lambda q, k, v, g, b, c: xlstm_hip.gated_delta_chunkwise(q, k, v, g, b, c, scale, True), x, dh, None)
+    want = gradients(lambda q, k, v, g, b, c: plain(q, k, v, g, b, c, scale), x, dh, None, torch.float64)
+    for name, a, w in zip(NAMES, got, want):
+        err, rounding = float((a.double() - w).norm()), float((w.to(F16).double() - w).norm())
+        assert err <= rounding + 2e-4 * float(w.norm()), f"{name}: {err / float(w.norm()):.2e}"

@@ -38,7 +38,7 @@ struct TurnArgs {
 
 template <typename T>
 __global__ __launch_bounds__(256) void delta_turn_kernel(TurnArgs p) {
-  constexpr int PK = is_f32<T>::value ? 2 : 1;
+  constexpr int PK = PLANES<T, true>;
   __shared__ float tile[L][65];
   const int64_t part = blockIdx.x;
   const int64_t bh = part / p.chunks;
@@ -98,7 +98,7 @@ struct BackArgs {
 // LDS that has to queue stops its wave: 177 us without, 157 with, at 8192 tokens of 128 x 256, 2.5 a chunk).
 template <typename T, int DKB, int STAGES, int W>
 __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(BackArgs p) {
-  constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
+  constexpr int DKP = DKB * 32, PK = PLANES<T, true>, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
   const int lane = threadIdx.x & 63, in = uniform(threadIdx.x >> 6), wave = W == 1 ? 0 : in;
   const int r = lane & 15, gq = lane >> 4;
@@ -383,7 +383,7 @@ constexpr int GLD = 65;
 
 template <typename T, int DKB>
 struct GradLds {
-  static constexpr int PK = is_f32<T>::value ? 2 : 1, DKP = DKB * 32;
+  static constexpr int PK = PLANES<T, true>, DKP = DKB * 32;
   static constexpr int TOK = 32 * L * 2, STA = 32 * DKP * 2;  // 32 columns of one plane
   static constexpr int STAGE = PK * (3 * TOK + 2 * STA), IMAGE = PK * L * DKP * 2;
   static constexpr int KK = L * GLD * 4;
@@ -395,9 +395,9 @@ struct GradLds {
 };
 
 // DKB waves: a wave has 32 of DQK's columns of dQ and dK, turned (columns down, tokens across), and its share of the 64 x 64 tiles.
-// At DQK 128 two workgroups fit a CU with 256 registers a lane (16-bit types: 167 us at 8192 tokens, 187 without; float32 would spill).
+// At DQK 128 two workgroups fit a CU with 256 registers a lane (bf16: 165 us at 8192 tokens, 187 without; pairs would spill).
 template <typename T, int DKB>
-__global__ __launch_bounds__(64 * DKB, DKB == 4 && !is_f32<T>::value ? 2 : 1) void delta_grad_kernel(GradArgs p) {
+__global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1)) void delta_grad_kernel(GradArgs p) {
   using Lds = GradLds<T, DKB>;
   constexpr int PK = Lds::PK, DKP = Lds::DKP, PLANE = L * DKP * 2, TOK = Lds::TOK, STA = Lds::STA, W = DKB, THREADS = 64 * W;
   constexpr bool PAIR = !std::is_same_v<T, bf16_t>;
@@ -947,8 +947,8 @@ struct Layout {
   explicit Layout(const Shape& s) {
     blocks = 2 * ((s.DV + 31) / 32);
     prep = up256((int64_t)prep_bytes(s, true));
-    tok = up256(s.parts() * blocks * s.planes() * 16 * L * 2);
-    sta = up256(s.parts() * blocks * s.planes() * 16 * s.dkp() * 2);
+    tok = up256(s.parts() * blocks * s.planes(true) * 16 * L * 2);
+    sta = up256(s.parts() * blocks * s.planes(true) * 16 * s.dkp() * 2);
     scales = up256(s.parts() * blocks * 4);
     partial = s.NH == s.NHK ? 0 : up256((int64_t)s.B * s.NH * s.S * s.DK * 4);
   }
@@ -970,12 +970,12 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
   hipError_t e = launch((const void*)delta_turn_kernel<T>, s.parts(), (kept.blocks + 3) / 4, 256, 0, &turn, st);
   if (e == hipSuccess)
     if (const int rc = launch_scan(s, v, c0, nullptr, nullptr, prep, &kept, st, who)) return rc;
-  constexpr int S8 = is_f32<T>::value ? 1 : 2;
+  constexpr int S8 = PLANES<T, true> == 2 ? 1 : 2;
   const int stages = s.dkp() == 256 ? S8 : 2;
   // A lone wave a block where two workgroups a CU (one, if no two fit) take all blocks, else four blocks a workgroup.  us of whole calls,
   // 2048 tokens, lone waves and fours: bf16 128 x 256, 256 blocks 252, 277; 512 433, 454; 768 626, 572; 1024 755, 689; 64 x 256, 512
   // blocks 346, 357; 1024 637, 577; 256 x 512, 512 blocks 597, 548; float32 128 x 256, 512 blocks of 1024 tokens 362, 349.
-  const int64_t scan_lds = stages * 2 * s.image_bytes() + 2 * 2048;
+  const int64_t scan_lds = stages * 2 * s.image_bytes(true) + 2 * 2048;
   const int waves = (int64_t)s.B * s.NH * kept.blocks <= (scan_lds <= 80 * 1024 ? 512 : 256) ? 1 : 4;
   const int slices = (kept.blocks + waves - 1) / waves;
   BackArgs back{dc_last, dc0, prep, kept, s.NH, group, s.DK, s.DV, chunks, slices};

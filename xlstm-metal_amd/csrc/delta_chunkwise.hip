@@ -46,7 +46,7 @@ struct ScanLds {
 // PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32).
 template <typename T, int DKB, int PARTS, int KST, bool STATES>
 __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p) {
-  constexpr int DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE;
+  constexpr int DKP = DKB * 32, PK = PLANES<T, STATES>, PLANE = L * DKP * 2, IMG = PK * PLANE;
   constexpr int TPW = 4 / PARTS, NB = DKB / PARTS;  // a wave's tiles of 16 tokens, its 32s of DQK
   constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
   using Lds = ScanLds<DKB, PK, PARTS, KST, !STATES, PAIR>;
@@ -476,7 +476,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
 // A block by one wave, W blocks a workgroup.
 template <typename T, int DKB, int STAGES, bool STATES>
 __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
-  constexpr int W = 4, DKP = DKB * 32, PK = is_f32<T>::value ? 2 : 1, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = (STATES ? 1 : 2) * IMG;
+  constexpr int W = 4, DKP = DKB * 32, PK = PLANES<T, STATES>, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = (STATES ? 1 : 2) * IMG;
   constexpr bool PAIR = STATES ? PK == 2 : !std::is_same_v<T, bf16_t>;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -784,7 +784,7 @@ struct Choice {
 // 613, 335; 64 x 256, 512 blocks 104, 98; 256 x 512, 512 blocks 181, 147; 1024 365, 180.
 template <typename T, int DKB, bool STATES>
 Choice choice(bool many) {
-  constexpr int PK = is_f32<T>::value ? 2 : 1, KST = DKB == 8 && PK == 2 && !STATES ? 1 : 2;  // K's pairs twice and Q's do not fit
+  constexpr int PK = PLANES<T, STATES>, KST = DKB == 8 && PK == 2 && !STATES ? 1 : 2;  // K's pairs twice and Q's do not fit
   constexpr int PARTS = DKB < 4 ? DKB : 4;
   constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
   if (many)

@@ -329,6 +329,8 @@ int check_shape(const char* who, const Shape& s) {
   const int64_t heads = (int64_t)s.B * s.NH, chunks = s.chunks() + 1;
   if (heads >= (1 << 24) || heads * chunks * ((s.DV + 15) / 16) >= ((int64_t)1 << 31))
     return set_error(XL_ERR_UNSUPPORTED, "%s: B NH S DV too large", who);
+  // a launch has fewer than 2^32 threads: 256 for 32 columns of a head
+  if (heads * ((s.DV + 31) / 32) >= (1 << 24)) return set_error(XL_ERR_UNSUPPORTED, "%s: B NH DV too large", who);
   return XL_OK;
 }
 
@@ -364,7 +366,7 @@ int launch_recurrent(const Shape& s, const void* q, const void* k, const void* v
   // several tokens.  bf16, us, in that order: 8 heads of 128 x 256 6.1, 4.3, 5.3; 64 heads 6.7, 5.7, 7.5; 256 heads 12.4, 14.9, 17.6;
   // 16 heads of 256 x 512 9.6, 6.0, 10.4; 128 heads 23.9, 26.8, 41.0 (268 MB: 5.6 TB/s).
   const int64_t heads = (int64_t)s.B * s.NH;
-  const bool one = s.S == 1 && c0;
+  const bool one = s.S == 1 && c0 && heads * ((s.DV + 63) / 64) < (1 << 22);  // 2^32 threads
   const int step = !one ? 0 : s.DV % 256 == 0 && heads * (s.DV / 256) >= 256 ? 256 : 64;
   // Several: 16 columns a workgroup where 32 give a CU one at most, for 13 tokens of 128 x 256 us of 16 and 32: 8 heads 10.2, 11.3; 32
   // heads 12.2, 12.5; 64 heads 17.5, 14.8; 128 heads 28.9, 21.4.

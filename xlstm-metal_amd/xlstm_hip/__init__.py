@@ -4,8 +4,9 @@ Drop-in for the torch-native kernel API of MLXPorts/xLSTM-metal: chunkwise
 mLSTM prefill and its custom backward, recurrent decode step and sequence, sLSTM step and sequence,
 the sLSTM layer's causal conv1d + SiLU and per-head GroupNorm, the mLSTM
 output cell's multi-head RMSNorm x sigmoid(o), soft_cap and the logit
-projection with its soft-cap epilogue, and for training a layer norm with its
-gradients and the orthogonalisation of updates,
+projection with its soft-cap epilogue, for training a layer norm with its
+gradients and the orthogonalisation of updates, and beside them the gated delta
+rule and the gated linear unit of a feed-forward block, both with gradients,
 each a ``torch.library`` op (``xlstm_hip::*``, native kernels in
 ``lib/libxlstm_torch.so``) calling hand-written HIP kernels in
 ``lib/libxlstm_hip.so`` through a C-ABI.
