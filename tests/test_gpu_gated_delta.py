@@ -46,6 +46,13 @@ def test_recurrent(gpu_case, shape, dtype, gate, state):
     assert torch.equal(h, xlstm_hip.gated_delta_recurrent(*x))
 
 
+@pytest.mark.parametrize("shape", [(64, 8, 4, 11, 100, 50), (40, 8, 8, 3, 256, 64), (32, 16, 16, 17, 33, 33), (8, 33, 11, 8, 64, 31)])
+@pytest.mark.parametrize("dtype,gate", [(BF16, F32), (F16, F16), (F32, F32)])
+@pytest.mark.parametrize("state", [False, True])
+def test_recurrent_of_many_heads(gpu_case, shape, dtype, gate, state):
+    test_recurrent(gpu_case, shape, dtype, gate, state)
+
+
 @pytest.mark.parametrize("B,NH,NHK,DQK,DV", [(1, 8, 8, 128, 256), (5, 4, 2, 64, 40), (3, 3, 1, 33, 7), (16, 8, 8, 256, 512)])
 @pytest.mark.parametrize("dtype,gate", [(BF16, BF16), (F16, F32), (F32, F32)])
 def test_step(gpu_case, B, NH, NHK, DQK, DV, dtype, gate):

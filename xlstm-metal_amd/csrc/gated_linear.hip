@@ -328,8 +328,11 @@ __global__ __launch_bounds__(64 * WL * WR) void glu_product_kernel(Args p) {
 }
 
 // ------------------------------------------------------------------------------------------------ few tokens
-// 16 rows of Wg and of Wu a workgroup, its waves share K; the parts meet in LDS.  Tokens past T read the last one again.
-constexpr int FEW_WAVES = 8, FEW_KB = 4, FEW_TOKENS = 16;
+// 16 rows of Wg and of Wu a workgroup, its waves share K; the parts meet in LDS.  Tokens past T read the last one again.  Bound by
+// memory: 8 tokens of 4096 to 10944 43 us, 4.2 TB/s.  Waves and 32s of K that each has under way, us for those 8 tokens, 8 of 2048 to
+// 5504 and 4 of 8192 to 1024: 8 and 2 43.2, 15.9, 23.8; 8 and 4 45.2, 17.8, 25.4; 4 and 2 42.0, 14.9, 27.4; 4 and 8 42.7, 16.5, 29.6;
+// 16 and 2 43.6, 17.3, 24.4; 8 and 1 49.4, 17.4, 25.5.
+constexpr int FEW_WAVES = 8, FEW_KB = 2, FEW_TOKENS = 16;
 
 template <typename T>
 __global__ __launch_bounds__(64 * FEW_WAVES) void glu_few_kernel(const T* __restrict__ x, const T* __restrict__ wg,
