@@ -461,44 +461,46 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   constexpr int MTS = 4 / (W < 4 ? W : 4);
   struct alignas(16) Eight { T e[8]; };
   Eight v8[MTS];
-  const T* vrow = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
-  T* dvrow = (T*)p.dv + (int64_t)bh * p.S * p.DV;
+  // Bases that are the same for all and 32-bit offsets: addresses of each lane's own would leave no registers for what is under way.
+  const char* const vrows = (const char*)((const T*)p.v + b * p.vs[0] + h * p.vs[1] + t0 * p.vs[2]);
+  char* const dvrows = (char*)((T*)p.dv + ((int64_t)bh * p.S + t0) * p.DV);
+  const int last = p.S - 1 - t0;
   auto load_v = [&](int step) {
     if (wave >= 4) return;
+    const int n = 32 * step + 8 * gq;
 #pragma unroll
     for (int x = 0; x < MTS; ++x) {
-      const int t = t0 + 16 * (wave + x * W) + r, n = 32 * step + 8 * gq;
-      const T* from = vrow + (t < p.S ? t : p.S - 1) * p.vs[2] + n;
-      if (p.wide_v && n + 8 <= p.DV) {
-        v8[x] = *(const Eight*)from;
+      const char* from = vrows + (uint32_t)(min(16 * (wave + x * W) + r, last) * (int)p.vs[2]) * (uint32_t)sizeof(T);
+      if (p.wide_v) {  // past the last column the first ones, against Z's zeros
+        v8[x] = *(const Eight*)(from + (uint32_t)(n < p.DV ? n : 0) * (uint32_t)sizeof(T));
       } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v8[x].e[e] = n + e < p.DV ? from[e] : from_f32<T>(0.f);
+        for (int e = 0; e < 8; ++e) v8[x].e[e] = n + e < p.DV ? ((const T*)from)[n + e] : from_f32<T>(0.f);
       }
     }
   };
+  auto tok_of = [&](const f16_t* kept) { return (const char*)(kept + kept_at(part, blocks, 0, PK, L)); };
+  auto sta_of = [&](const f16_t* kept) { return (const char*)(kept + kept_at(part, blocks, 0, PK, DKP)); };
   auto load = [&](int step) {
 #pragma unroll
     for (int half = 0; half < 2; ++half)
 #pragma unroll
       for (int i = 0; i < 5; ++i) coming[half][i] = scales[i][2 * step + half];
+    const uint32_t tok_step = step * (uint32_t)(2 * PK * 16 * L * 2), sta_step = step * (uint32_t)(2 * PK * 16 * DKP * 2);
 #pragma unroll
     for (int i = 0; i < TOK_PER; ++i) {
-      const int at = i * THREADS + tid;
-      if (at >= TOK_PIECES) continue;
-      const int mat = at / (PK * 256), rest = at - mat * (PK * 256), pl = rest >> 8, row = (rest >> 3) & 31, piece = rest & 7;
-      const int block = 2 * step + (row >> 4);
-      const f16_t* base = mat == 0 ? p.kept.dh : mat == 1 ? p.kept.z : p.kept.u;
-      tok[i] = *(const u32x4*)(base + kept_at(part, blocks, block, PK, L) + pl * 16 * L + (row & 15) * L + piece * 8);
+      const int at = min(i * THREADS + tid, TOK_PIECES - 1), mat = uniform(at / (PK * 256)), rest = at - mat * (PK * 256);
+      const int pl = rest >> 8, row = (rest >> 3) & 31, piece = rest & 7;
+      const uint32_t off = ((row >> 4) * PK + pl) * (16 * L * 2) + (row & 15) * (L * 2) + piece * 16;
+      tok[i] = __builtin_bit_cast(u32x4, load16(tok_of(mat == 0 ? p.kept.dh : mat == 1 ? p.kept.z : p.kept.u), tok_step + off));
     }
 #pragma unroll
     for (int mat = 0; mat < 2; ++mat)
 #pragma unroll
       for (int i = 0; i < STA_PER; ++i) {
         const int at = (i / PK) * THREADS + tid, pl = i % PK, row = at / (DKP / 8), piece = at % (DKP / 8);
-        const int block = 2 * step + (row >> 4);
-        sta[mat][i] = *(const u32x4*)((mat ? p.kept.ds : p.kept.s0) + kept_at(part, blocks, block, PK, DKP) + pl * 16 * DKP +
-                                      (row & 15) * DKP + piece * 8);
+        const uint32_t off = ((row >> 4) * PK + pl) * (16 * DKP * 2) + (row & 15) * (DKP * 2) + piece * 16;
+        sta[mat][i] = __builtin_bit_cast(u32x4, load16(sta_of(mat ? p.kept.ds : p.kept.s0), sta_step + off));
       }
   };
   float ss_dot = 0.f;  // <dS, S_0>
@@ -590,19 +592,23 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
 #pragma unroll
           for (int e = 0; e < 8; ++e) zf[e] = ((float)z[e] + (float)zl[e]) * of[1];
           const float beta = betas[16 * mt + r];
-          T* to = dvrow + (int64_t)t * p.DV + n;
-          Eight o;
+          char* const to = dvrows + (uint32_t)((t - t0) * p.DV + n) * (uint32_t)sizeof(T);
+          f32x4 dv[2];
 #pragma unroll
           for (int e = 0; e < 8; ++e) {
             zv[x] = fmaf(zf[e], to_f32(v8[x].e[e]), zv[x]);
-            o.e[e] = from_f32<T>(beta * zf[e]);
+            dv[e >> 2][e & 3] = beta * zf[e];
           }
-          if (p.wide_v && n + 8 <= p.DV) {
-            *(Eight*)to = o;
-          } else {
 #pragma unroll
-            for (int e = 0; e < 8; ++e)
-              if (n + e < p.DV) to[e] = o.e[e];
+          for (int q = 0; q < 2; ++q) {
+            const Four<T> o = rounded4<T>(dv[q]);
+            if (p.wide_v) {
+              if (n < p.DV) ((Four<T>*)to)[q] = o;
+            } else {
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                if (n + 4 * q + e < p.DV) ((T*)to)[4 * q + e] = o.e[e];
+            }
           }
         }
       }
@@ -850,39 +856,41 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   dots(g1, 3);  // q_i.(dH S_0^T)_i
   // ---- out
   {
-    const bool own = p.group == 1;
-    auto write = [&](void* to, int tile, int token, f32x4 x) {
-      const int d = 16 * tile + 4 * gq;
-      auto as = [&](auto type) {
-        using O = decltype(type);
-        O* at = (O*)to + ((int64_t)bh * p.S + token) * p.DK + d;
-        struct alignas(4 * sizeof(O)) Four { O e[4]; } o;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) o.e[e] = from_f32<O>(x[e]);
-        if (p.DK % 4 == 0) {
-          if (d < p.DK) *(Four*)at = o;
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            if (d + e < p.DK) at[e] = o.e[e];
-        }
-      };
-      if (own) as(T{});
-      else as(float{});
-    };
     const float fa = ksc * sd.down;
+    float fq[4];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) {
-      const int token = t0 + 16 * mt + r;
-      const float fq = ldexpf(f->q[16 * mt + r] / qsc, top[DH_S]);
-      if (token < p.S) {
+    for (int mt = 0; mt < 4; ++mt) fq[mt] = ldexpf(f->q[16 * mt + r] / qsc, top[DH_S]);
+    auto write = [&](auto type, auto whole) {
+      using O = decltype(type);
+      const int d = 32 * wave + 4 * gq;
+      const int64_t at = ((int64_t)bh * p.S + t0 + r) * p.DK + d;
+#pragma unroll
+      for (int mt = 0; mt < 4; ++mt) {
+        if (t0 + 16 * mt + r >= p.S) continue;
+        O *const q = (O*)p.dq + at + (int64_t)(16 * mt) * p.DK, *const k = (O*)p.dk + at + (int64_t)(16 * mt) * p.DK;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          write(p.dq, 2 * wave + t, token, g1[t][mt] * fq + accq[t][mt] * fa);
-          write(p.dk, 2 * wave + t, token, acck[t][mt] * qu);
+          const Four<O> oq = rounded4<O>(g1[t][mt] * fq[mt] + accq[t][mt] * fa), ok = rounded4<O>(acck[t][mt] * qu);
+          if constexpr (decltype(whole)::value) {
+            if (d + 16 * t < p.DK) {
+              *(Four<O>*)(q + 16 * t) = oq;
+              *(Four<O>*)(k + 16 * t) = ok;
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (d + 16 * t + e < p.DK) {
+                q[16 * t + e] = oq.e[e];
+                k[16 * t + e] = ok.e[e];
+              }
+          }
         }
       }
-    }
+    };
+    using Yes = std::true_type;
+    using No = std::false_type;
+    if (p.group == 1) p.DK % 4 == 0 ? write(T{}, Yes{}) : write(T{}, No{});
+    else p.DK % 4 == 0 ? write(float{}, Yes{}) : write(float{}, No{});
   }
   lds_barrier();
   // ---- the gates, a lane a token
@@ -989,7 +997,7 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
   GradArgs grad{v, {s.vs[0], s.vs[1], s.vs[2]}, group == 1 ? dq : (void*)dqp, group == 1 ? dk : (void*)dkp, dv, dg, dbeta, prep, kept,
                 s.NH, group, s.S, s.DK, s.DV, chunks, s.dtype_gates, s.scale, false};
   constexpr int VW = 16 / sizeof(T);
-  grad.wide_v = ((s.vs[0] | s.vs[1] | s.vs[2] | (int64_t)s.DV) % VW) == 0 && (((uintptr_t)v | (uintptr_t)dv) & 15) == 0;
+  grad.wide_v = s.DV % 8 == 0 && ((s.vs[0] | s.vs[1] | s.vs[2]) % VW) == 0 && (((uintptr_t)v | (uintptr_t)dv) & 15) == 0;
   const int lds = s.dkp() == 64 ? GradLds<T, 2>::BYTES : s.dkp() == 128 ? GradLds<T, 4>::BYTES : GradLds<T, 8>::BYTES;
   kern = s.dkp() == 64 ? (const void*)delta_grad_kernel<T, 2> : s.dkp() == 128 ? (const void*)delta_grad_kernel<T, 4>
                                                                               : (const void*)delta_grad_kernel<T, 8>;
