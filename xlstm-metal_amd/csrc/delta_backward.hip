@@ -447,7 +447,7 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
     for (int i = 0; i < SUMS; ++i) top[i] = max(top[i], x[i]);
   }
 #pragma unroll
-  for (int i = 0; i < SUMS; ++i) top[i] = (int)wave_max_all((float)(top[i] + 1000)) - 1000;
+  for (int i = 0; i < SUMS; ++i) top[i] = uniform((int)wave_max_all((float)(top[i] + 1000)) - 1000);
   if (tid < L) {
     bs[tid] = f->b[tid];
     betas[tid] = f->beta[tid];
@@ -613,15 +613,14 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
         }
       }
     }
-    if (step + 1 < steps) {
-      load(step + 1);
-      load_v(step + 1);
-    }
     int factor[SUMS];
     products(of, factor);
     _Float16 by[SUMS];
 #pragma unroll
     for (int i = 0; i < SUMS; ++i) by[i] = (_Float16)power(factor[i] - top[i]);
+    __builtin_amdgcn_sched_barrier(0);
+    load(step + 1 < steps ? step + 1 : step);  // past the last step that one again
+    load_v(step + 1 < steps ? step + 1 : step);
     f16x8 s0[PK][2], ds[PK][2];
 #pragma unroll
     for (int pl = 0; pl < PK; ++pl)
