@@ -20,7 +20,7 @@
 // Heads of v that share q and k write their dQ and dK in float32, and a last kernel adds them in order.
 //
 // Measured (bf16, 2 x 4096 tokens of 8 heads of 128 x 256), us: first kernel 37, dH by columns 17, states 121, scan backwards
-// 155, chunks' gradients 165.  The scans are bound by the chain of one chunk's step; the last by its waits between products
+// 155, chunks' gradients 133.  The scans are bound by the chain of one chunk's step; the last by its waits between products
 // (its 377 MB are 73 us of a copy).
 #include "delta.h"
 
@@ -395,7 +395,7 @@ struct GradLds {
 };
 
 // DKB waves: a wave has 32 of DQK's columns of dQ and dK, turned (columns down, tokens across), and its share of the 64 x 64 tiles.
-// At DQK 128 two workgroups fit a CU with 256 registers a lane (bf16: 165 us at 8192 tokens, 187 without; pairs would spill).
+// At DQK 128 two workgroups fit a CU with 256 registers a lane (bf16: 165 us against 187, measured before it came to 133; pairs would spill).
 template <typename T, int DKB>
 __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1)) void delta_grad_kernel(GradArgs p) {
   using Lds = GradLds<T, DKB>;
