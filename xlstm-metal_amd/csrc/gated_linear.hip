@@ -45,6 +45,12 @@ __device__ __forceinline__ f32x4 mfma16(u32x4 a, u32x4 b, f32x4 c) {
 
 // 16 bytes from float32, two values by one conversion
 template <typename T>
+__device__ __forceinline__ T rounded1(float v) {
+  using pair = std::conditional_t<std::is_same_v<T, f16_t>, xl_f16x2, xl_bf16x2>;
+  const uint16_t x = (uint16_t)__builtin_bit_cast(uint32_t, __builtin_convertvector((xl_f32x2{v, 0.f}), pair));
+  return __builtin_bit_cast(T, x);
+}
+template <typename T>
 __device__ __forceinline__ u32x4 rounded8(const float (&v)[8]) {
   using pair = std::conditional_t<std::is_same_v<T, f16_t>, xl_f16x2, xl_bf16x2>;
   u32x4 raw;
@@ -101,7 +107,7 @@ struct Args {
   float *a, *u;  // FWD: a, u [T, keep_pitch], or null
   int64_t keep_pitch;
   int act;
-  bool wide;  // 16-byte stores of out
+  bool wide;  // rows of out are multiples of 8 values
   int splits;      // parts of K
   float* partial;  // their sums, by [tile][part]
 };
@@ -309,19 +315,20 @@ __global__ __launch_bounds__(64 * WL * WR) void glu_product_kernel(Args p) {
       *(f32x4*)(strip + row * LDW + i * 16 + quad * 4) = v;
     }
     wave_fence();
+    if (p.wide) {
 #pragma unroll
-    for (int h = 0; h < (16 * EACH + 63) / 64; ++h) {
-      const int at = h * 64 + lane, r = at / EACH, c = at % EACH * 8, m = r0 + j * 16 + r, n = l0 + c;
-      if (r >= 16 || m >= p.rights || n >= p.lefts) continue;
-      const f32x4 v0 = *(const f32x4*)(strip + r * LDW + c), v1 = *(const f32x4*)(strip + r * LDW + c + 4);
-      const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
-      T* to = out + m * p.out_pitch + n;
-      if (p.wide && n + 8 <= p.lefts) {
-        *(u32x4*)to = rounded8<T>(v);
-      } else {
-#pragma unroll
-        for (int q = 0; q < 8; ++q)
-          if (n + q < p.lefts) to[q] = from_f32<T>(v[q]);
+      for (int h = 0; h < (16 * EACH + 63) / 64; ++h) {
+        const int at = h * 64 + lane, r = at / EACH, c = at % EACH * 8, m = r0 + j * 16 + r, n = l0 + c;
+        if (r >= 16 || m >= p.rights || n >= p.lefts) continue;
+        const f32x4 v0 = *(const f32x4*)(strip + r * LDW + c), v1 = *(const f32x4*)(strip + r * LDW + c + 4);
+        const float v[8] = {v0[0], v0[1], v0[2], v0[3], v1[0], v1[1], v1[2], v1[3]};
+        *(u32x4*)(out + m * p.out_pitch + n) = rounded8<T>(v);
+      }
+    } else {  // rows of any address: neighbouring lanes write neighbouring values
+#pragma unroll 4
+      for (int h = 0; h < 4 * OUT; ++h) {
+        const int at = h * 64 + lane, r = at / (OUT * 16), c = at % (OUT * 16), m = r0 + j * 16 + r, n = l0 + c;
+        if (m < p.rights && n < p.lefts) out[m * p.out_pitch + n] = rounded1<T>(strip[r * LDW + c]);
       }
     }
   }
