@@ -417,7 +417,7 @@ int xl_newton_schulz(const void* g, void* x, int64_t batch, int m, int n, const 
  * Gated delta rule: with a = exp(g), the state C [DQK, DV] goes to a C + k (beta (v - (a C)^T k))^T at every token, and h =
  * scale C^T q.  q, k [B, NHK, S, DQK], v, h [B, NH, S, DV] of dtype_qkv, head i of v with head i / (NH / NHK) of q and k;
  * g, beta [B, NH, S] of dtype_gates (g = -inf: a = 0); c0 [B, NH, DQK, DV] float32 or NULL (zeros), c_last the last state or
- * NULL.  DQK up to 256.  S = 0 copies c0 to c_last.
+ * NULL.  DQK up to 256, B NH DV below 2^29.  S = 0 copies c0 to c_last.
  *
  * Token by token, in float32, everything contiguous; c_last may be c0.
  */
@@ -452,8 +452,9 @@ int xl_gated_delta_chunkwise_bwd(const void* q, const void* k, const void* v, co
 /*
  * Gated linear unit: h = act(x w_gate^T) * (x w_up^T), x [T, D], weights [F, D], h [T, F], bf16 or f16 (float32:
  * XL_ERR_UNSUPPORTED); act 0: SiLU, 1: GELU (by erf).  Products, activation and their product in float32, rounded once.  a and
- * u: both products, float32 [T, keep_pitch] (keep_pitch at least F, a multiple of 8), for the backward, or both NULL.  Pointers 16-byte
- * aligned.  T = 0: nothing.  Workspace (xl_gated_linear_workspace_size bytes, 256-byte aligned): none where D is a multiple of 8.
+ * u: both products, float32 [T, keep_pitch] (keep_pitch at least F, a multiple of 8), for the backward, or both NULL.  Pointers
+ * 16-byte aligned.  T up to 2^28, D and F up to 2^22; T = 0: nothing.  Workspace (xl_gated_linear_workspace_size bytes, 256-byte
+ * aligned): none forward where D is a multiple of 8.
  *
  * Its gradients from dh [T, F], of x, and of both weights together; dx or both dw may be NULL.  T at least 1.
  */
