@@ -745,7 +745,10 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   lds_barrier();
 
   // ---- each pair of tokens: wave w has rows w, w + W, .., a lane a column
-  float dps[ROWS], ee[ROWS], col = 0.f, mx[2] = {0.f, 0.f};
+  // dQ takes scale D o dP against K's planes, dK its transpose against Q's and E + E^T against K's: the planes' scales enter here, and
+  // dK's two have one scale between them, so that their sum is in one unit.  (A chunk without a pair of tokens has zeros for E, one without
+  // dH for dP: in units of its own the other part could be past float32's range.)
+  float dpk[ROWS], dpq[ROWS], ee[ROWS], col = 0.f, mx[2] = {0.f, 0.f};
   const double bj = bs[lane];
   const float p_scale = f->p;
 #pragma unroll
@@ -762,10 +765,11 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
       rows[L + i] = bb;
     }
     col += fmaf(dp, pv, beta * (da * nij));
-    dps[x] = p.scale * dec * dp;
-    ee[x] = da * beta * dec;
-    mx[0] = fmaxf(mx[0], fabsf(dps[x]));
-    mx[1] = fmaxf(mx[1], fabsf(ee[x]));
+    dpk[x] = p.scale * dec * dp * ksc;
+    dpq[x] = p.scale * dec * dp * qsc;
+    ee[x] = da * beta * dec * ksc;
+    mx[0] = fmaxf(mx[0], fabsf(dpk[x]));
+    mx[1] = fmaxf(mx[1], fmaxf(fabsf(dpq[x]), fabsf(ee[x])));
   }
   red[(2 * W + wave) * L + lane] = col;
   const float m0 = wave_max_all(mx[0]), m1 = wave_max_all(mx[1]), dot = wave_sum(ss_dot);
@@ -789,7 +793,7 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
     mx[0] = fmaxf(mx[0], wred[w]);
     mx[1] = fmaxf(mx[1], wred[8 + w]);
   }
-  const Pow2 sd = pow2_for(mx[0]), se = pow2_for(mx[1]);
+  const Pow2 sq = pow2_for(mx[0]), sk = pow2_for(mx[1]);
   // rows of 64 in f16, each 32 turned, piece p of row i at p ^ (i % 8): scale D o dP, its transpose, E + E^T
   constexpr int MAT = L * L * 2;
   auto put = [&](int mat, int i, int j, float x) {
@@ -801,9 +805,9 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
 #pragma unroll
   for (int x = 0; x < ROWS; ++x) {
     const int i = x * W + wave, j = lane;
-    const float dp = dps[x] * sd.up, e = ee[x] * se.up;
-    put(0, i, j, dp);
-    put(1, j, i, dp);
+    const float e = ee[x] * sk.up;
+    put(0, i, j, dpk[x] * sq.up);
+    put(1, j, i, dpq[x] * sk.up);
     if (j <= i) put(2, i, j, e);
     if (j < i) put(2, j, i, e);
   }
@@ -830,24 +834,19 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
         }
       }
   };
-  // dK's parts with the states, in units of K's scale and E's; then in those of Q's and D o dP's
+  // dK's parts with the states (in g3 from here)
   f32x4 accq[2][4], acck[2][4];
-  const float ku = ksc * se.down, qu = qsc * sd.down;
 #pragma unroll
   for (int mt = 0; mt < 4; ++mt) {
-    const float fo = ldexpf(f->out[16 * mt + r] / ksc / ku, top[U_DS]), fb = ldexpf(f->back[16 * mt + r] / ksc / ku, top[Z_S]);
+    const float fo = ldexpf(f->out[16 * mt + r] / ksc, top[U_DS]), fb = ldexpf(f->back[16 * mt + r] / ksc, top[Z_S]);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
-      acck[t][mt] = g3[t][mt] * fo - g2[t][mt] * fb;
-      accq[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
+      g3[t][mt] = g3[t][mt] * fo - g2[t][mt] * fb;
+      accq[t][mt] = acck[t][mt] = f32x4{0.f, 0.f, 0.f, 0.f};
     }
   }
   add(accq, 0);
   add(acck, 2);
-#pragma unroll
-  for (int t = 0; t < 2; ++t)
-#pragma unroll
-    for (int mt = 0; mt < 4; ++mt) acck[t][mt] *= ku / qu;
   lds_barrier();
   put_image();
   lds_barrier();
@@ -855,7 +854,6 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   dots(g1, 3);  // q_i.(dH S_0^T)_i
   // ---- out
   {
-    const float fa = ksc * sd.down;
     float fq[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) fq[mt] = ldexpf(f->q[16 * mt + r] / qsc, top[DH_S]);
@@ -869,7 +867,7 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
         O *const q = (O*)p.dq + at + (int64_t)(16 * mt) * p.DK, *const k = (O*)p.dk + at + (int64_t)(16 * mt) * p.DK;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          const Four<O> oq = rounded4<O>(g1[t][mt] * fq[mt] + accq[t][mt] * fa), ok = rounded4<O>(acck[t][mt] * qu);
+          const Four<O> oq = rounded4<O>(g1[t][mt] * fq[mt] + accq[t][mt] * sq.down), ok = rounded4<O>(g3[t][mt] + acck[t][mt] * sk.down);
           if constexpr (decltype(whole)::value) {
             if (d + 16 * t < p.DK) {
               *(Four<O>*)(q + 16 * t) = oq;
