@@ -340,7 +340,8 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     }
     load_t(next);
     const Pow2 us = pow2_for(wave_max_all(abs_max(u)));
-    const float ws_up = us.up * decayed.up * 0.5f;
+    // at most 2^126: U of zeros has the largest scale there is, and keys far below 1 another
+    const float ws_up = fminf(us.up * decayed.up * 0.5f, 0x1p126f);
 #pragma unroll
     for (int x = 0; x < TPW; ++x) {
       const int mt = part * TPW + x;
@@ -381,11 +382,15 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    const float u_down = largest(of_u), w_down = u_down * decayed.down * 2.f;
+    const float u_down = largest(of_u);
+    float of_w[PARTS];  // the inverses of the parts' ws_up
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) of_w[i] = fmaxf(of_u[i] * decayed.down * 2.f, 0x1p-126f);
+    const float w_down = largest(of_w);
     // U decayed is below 2^15 w_down
     const Pow2 sc = pow2_for(fmaxf(largest(of_s) * keep, w_down * 32767.f), STATE);
     f16x8 wh[2], wl[2];
-    shifts(of_u, u_down, by);
+    shifts(of_w, w_down, by);
     planes(by, wh, wl);
     if constexpr (!STATES) {
 #pragma unroll
@@ -429,6 +434,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       }
     } else {  // ---- H
       f16x8 uh[2], ul[2];
+      shifts(of_u, u_down, by);
       if constexpr (PAIR) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) raw[i] = raw_u[i];
