@@ -1,16 +1,18 @@
-"""The gated delta rule on the GPU where sizes are far apart: gradients beside a matrix of zeros, keys far below 1.
+"""The gated delta rule on the GPU where sizes are far apart: gradients beside a matrix of zeros, keys far below 1, rows of one chunk
+far from each other.
 
-Bars of gradients are those of test_gpu_gated_delta_bwd; of h and the state delta_reference's, but that what a token adds to the state is taken
-at its key's length (``tight``)."""
+Bars of gradients are those of test_gpu_gated_delta_bwd, of a head or (``token_parts``) of each token's own terms; of h and the state
+delta_reference's, but that what a token adds to the state is taken at its key's length (``tight``)."""
 
 import pytest
 import torch
 
 from delta_reference import CHUNK_KU, check, make
-from test_gpu_gated_delta_bwd import check_all, inputs
+from helpers import dev
+from test_gpu_gated_delta_bwd import BAR, check_all, gradients, inputs, plain
 
 pytestmark = pytest.mark.gpu
-F32, BF16 = torch.float32, torch.bfloat16
+F32, BF16, F16 = torch.float32, torch.bfloat16, torch.float16
 
 
 # ------------------------------------------------------------------ gradients beside zeros
@@ -96,3 +98,89 @@ def test_small_keys(gpu_case, shape, dtype, ks, state):
     h, c = xlstm_hip.gated_delta_chunkwise(*x, return_last_states=True)
     check(c, cr, cb, "C")
     check(h, hr, hb, "h")
+
+
+# ------------------------------------------------------------------ rows of one chunk far apart
+def row_sizes(kind, S):
+    """(of q's rows, of k's): a token's own size."""
+    one, t = torch.ones(S), torch.arange(S)
+    far = 10.0 ** -(6.0 * torch.rand(S, generator=torch.Generator().manual_seed(S)))
+    small = torch.where(t % 5 == 2, 1e-6, 1.0)
+    # keys that grow in the middle of a chunk: those before it are small beside their chunk's largest
+    early = torch.where(t < 40, 1e-6, 1.0)
+    return {"q": (far, one), "q small": (small, one), "k early": (one, early), "k late": (one, early.flip(0)), "both": (far.flip(0), far)}[kind]
+
+
+KINDS = ["q", "q small", "k early", "k late", "both"]
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 2, 140, 64, 48), (1, 2, 1, 100, 200, 40), (40, 8, 8, 70, 128, 20)])
+@pytest.mark.parametrize("dtype", [F32, BF16, F16])
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("state", [False, True])
+def test_rows_far_apart(gpu_case, shape, dtype, kind, state):
+    """h of every token to its own size, whatever the other tokens' queries and keys are."""
+    import xlstm_hip
+    if dtype == F16:  # its own numbers end at 2^-24: rows of 1e-3 at the least, and h on a scale that its numbers hold
+        sizes = [s.clamp_min(1e-3) for s in row_sizes(kind, shape[3])]
+    else:
+        sizes = row_sizes(kind, shape[3])
+    q, k, v, g, beta, c0 = make(*shape, F32, F32, seed=41, state=state)
+    q, k = (t * s.to(dev())[:, None] for t, s in zip((q, k), sizes))
+    x = (q.to(dtype), k.to(dtype), v.to(dtype), g, beta, c0)
+    hr, cr, hb, cb = tight(*x, planes=dtype == BF16)
+    h, c = xlstm_hip.gated_delta_chunkwise(*x, return_last_states=True)
+    check(c, cr, cb, "C")
+    check(h, hr, hb, "h")
+
+
+def token_parts(x, dh, scale):
+    """Sizes of a token's dq, dk and dv before anything cancels, without an initial or last state: norms of the sums' terms."""
+    q, k, v, g, beta = (t.double() for t in x[:5])
+    rep = v.shape[1] // q.shape[1]
+    q, k = q.repeat_interleave(rep, 1), k.repeat_interleave(rep, 1)
+    C, U, Gs = v.new_zeros(*v.shape[:2], q.shape[-1], v.shape[-1]), torch.empty_like(v), torch.empty_like(v)
+    for t in range(v.shape[2]):
+        C = C * torch.exp(g[:, :, t, None, None])
+        U[:, :, t] = beta[:, :, t, None] * (v[:, :, t] - (k[:, :, t, :, None] * C).sum(-2))
+        C = C + k[:, :, t, :, None] * U[:, :, t, None, :]
+    G = torch.zeros_like(C)
+    for t in reversed(range(v.shape[2])):
+        G = G + scale * q[:, :, t, :, None] * dh.double()[:, :, t, None, :]
+        Gs[:, :, t] = (k[:, :, t, :, None] * G).sum(-2)  # dU = Z
+        G = torch.exp(g[:, :, t, None, None]) * (G - k[:, :, t, :, None] * (beta[:, :, t, None] * Gs[:, :, t])[..., None, :])
+    b = g.cumsum(-1)
+    low = torch.ones(g.shape[-1], g.shape[-1], dtype=torch.bool, device=g.device).tril()
+    D = torch.exp((b[..., :, None] - b[..., None, :]).masked_fill(~low, -torch.inf))
+    n = lambda t: t.norm(dim=-1)  # noqa: E731
+    lq, lk, ld, lu, lz = n(q), n(k), n(dh.double()), n(U), n(Gs)
+    M = D * low.double().tril(-1)
+    dq = scale * (D * ld[..., :, None] * lu[..., None, :] @ lk[..., None])[..., 0]
+    dk = scale * ((D * ld[..., :, None] * lu[..., None, :]).mT @ lq[..., None])[..., 0]
+    E = M * (beta * lz)[..., :, None] * lu[..., None, :]
+    dk = dk + ((E + E.mT) @ lk[..., None])[..., 0]
+    dv = scale * ((D * lq[..., :, None] * lk[..., None, :]).mT @ ld[..., None])[..., 0]
+    dv = beta * (lz + dv + lk * (M.mT @ (beta * lz * lk)[..., None])[..., 0])
+    share = lambda t: t.view(t.shape[0], -1, rep, t.shape[-1]).sum(2)  # noqa: E731
+    return share(dq), share(dk), dv
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 2, 140, 64, 48), (1, 2, 1, 100, 200, 40), (16, 8, 8, 70, 128, 48)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_gradients_of_rows_far_apart(gpu_case, shape, kind):
+    """dq, dk and dv of every token to the size of its own terms, float32: 10 pairs' roundings of 2^-22 (test_gpu_gated_delta_bwd's
+    count, twice).  Queries and keys have rows 2^-20 of the largest, so products of both have 2^-40.  The operands that are formed of such
+    (dU, Z, and what K and Q are multiplied with for dQ and dK) stand at 2^14 of their block or chunk and f16 ends at 2^-24: each value
+    is off by 2^-39 of the largest, and 64 of them, of random sign, with factors up to 1, by sqrt(64) of that, with two or three operands one behind the
+    other by 2^-34 of the largest token's."""
+    import xlstm_hip
+    x, dh, _ = inputs(shape, F32, F32, 43, state=False, last=False)
+    x = [t * s.to(dev())[:, None] for t, s in zip(x[:2], row_sizes(kind, shape[3]))] + list(x[2:])
+    scale = shape[4] ** -0.5
+    got = gradients(lambda *y: (xlstm_hip.gated_delta_chunkwise(*y, scale=scale), None), x, dh, None)
+    want = gradients(lambda *y: plain(*y, scale), x, dh, None, torch.float64)
+    for a, w, part, name in zip(got, want, token_parts(x, dh, scale), ("dq", "dk", "dv")):
+        err = (a.double() - w).norm(dim=-1)
+        largest = torch.cat([c.amax(-1, keepdim=True).expand_as(c) for c in part.split(64, -1)], -1)
+        worst = float(((err - 2.0 ** -34 * largest) / part.clamp_min(1e-300)).max())
+        assert worst <= BAR[F32], f"{name}: {worst:.3e} of a token's terms"

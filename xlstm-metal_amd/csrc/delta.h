@@ -12,15 +12,19 @@
 // acts on each column of V, U and S by itself: a scan takes blocks of 16 columns through the whole sequence, a block's [DQK, 16]
 // piece of the state in float32 registers, and no block waits for another.
 //
-// All products are on the matrix cores in f16 with float32 sums.  Every operand stands at a power-of-two scale that
-// puts its largest value high in f16's range (of a chunk's K or Q, of T and P, and of a wave's S, V - diag(c) K S, U), so any
-// input's range is kept; float32 values enter as pairs hi + lo of f16 (22 bits), and a product of two pairs is three.
+// All products are on the matrix cores in f16 with float32 sums.  Every operand stands at a power-of-two scale that puts its
+// largest value high in f16's range: each row of K, of Q and of P at its own, so that a token's h has its bits beside tokens of other
+// sizes; T at a chunk's; S, V - diag(c) K S and U at a block of columns'.  Largest values from 2^-86 to 2^110 are kept.  float32 values enter
+// as pairs hi + lo of f16 (22 bits), and a product of two pairs is three.  f16 ends at 2^-24: a value x times below its operand's largest is
+// off by 2^-25 of that where this stands at 1 (K, Q), by 2^-39 where at 2^14 (R, U), if that is more than 2^-22 (one plane: 2^-11) of itself.
 //
 // Operand layout of v_mfma_f32_16x16x32_f16: lane l = 16 g + r holds row (A) or column (B) r, k = 8 g .. 8 g + 7; the result's
 // column is r, its rows 4 g .. 4 g + 3.  Two results below each other (16 rows each) hold 4 g + e and 16 + 4 g + e of 32 rows:
 // they are the next product's B operand as they stand if its A operand has k in that order.  "Turned" 32s have it: piece g
 // of 8 values holds 4 g .. 4 g + 3, 16 + 4 g .. 16 + 4 g + 3.
 #pragma once
+
+#include <stddef.h>
 
 #include "common.h"
 #include "mfma_bf16.h"
@@ -45,21 +49,27 @@ constexpr int FRAGS = 8;        // 16 x 32 operands of a 64 x 64 matrix: row til
 constexpr int FRAG_PLANE = FRAGS * 64 * 8;  // f16 values of one plane
 constexpr float CLAMP_G = -1e4f;  // exp() of it is 0: a reset (-inf) keeps the sums finite
 
-// Per head and chunk, by the first kernel: per-token factors (f16 planes' scales folded in) and scales.
+// Per head and chunk, by the first kernel: per-token factors (the scales of K's and Q's rows, 2^k_i and 2^q_i, folded in) and scales, the bytes
+// as biased exponents.  A row of zeros has scale 0 (its out must not raise `most`).
 struct Factors {
-  float in[L];     // c_i 2^k            K S
-  float q[L];      // scale c_i 2^q      Q S
-  float out[L];    // c_L / c_i 2^k      U into the state
-  float all;       // c_L
-  float most;      // the largest of out
-  float t, tt, p;  // T diag(beta), T and P = planes * these
-  float k, qs;     // K, Q = planes * these
-  float pad[57];   // the scans take the first 1 KB into LDS
-  float back[L];   // beta_i c_i 2^k     Z into the state's gradient
-  float beta[L];
-  double b[L];     // running sums of g
+  float in[L];      // c_i 2^k_i          K S
+  float q[L];       // scale c_i 2^q_i    Q S
+  float out[L];     // c_L / c_i 2^k_i    U into the state
+  float all;        // c_L
+  float most;       // the largest of out
+  float t, tt;      // T diag(beta), T^T = planes * these
+  uint8_t p[L];     // P's rows = planes * these
+  float pad[44];    // the scan takes the first 1 KB into LDS
+  float back[L];    // beta_i in_i        Z into the state's gradient
+  float pt[L];      // P^T's rows
+  uint8_t k[L], qs[L];  // K's and Q's rows
+  float pad2[32];
+  float beta[L];    // the scan backwards takes 2 KB
+  double b[L];      // running sums of g
 };
-static_assert(sizeof(Factors) == 2048);
+static_assert(sizeof(Factors) == 2560 && offsetof(Factors, back) == 1024 && offsetof(Factors, b) == 2048);
+__device__ __forceinline__ float power_of(uint32_t exponent) { return __uint_as_float(exponent << 23); }
+__device__ __forceinline__ uint8_t exponent_of(float power) { return (uint8_t)(__float_as_uint(power) >> 23); }
 
 __device__ __forceinline__ f32x4 mfma(f16x8 a, f16x8 b, f32x4 c) {
   return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
@@ -87,7 +97,7 @@ __device__ __forceinline__ void interleave() {
   });
 }
 
-// 2^target / 2^exponent(m) and its inverse: m times the first is in [2^target, 2^(target + 1)); m >= 0, the same in the wave.
+// 2^target / 2^exponent(m) and its inverse: m times the first is in [2^target, 2^(target + 1)); m >= 0.
 // At most 2^100 either way (0 gets that).
 struct Pow2 {
   float up, down;
@@ -223,8 +233,8 @@ __device__ __forceinline__ float state_max(const f32x4 (&st)[N]) {
   return wave_max_all(abs_max(st));
 }
 
-// Images of K and Q: [plane][64 tokens][DKP] f16, the largest value in [1, 2), each 32 columns turned, the 16-byte piece p of
-// token i at p ^ (i % 8).
+// Images of K and Q: [plane][64 tokens][DKP] f16, each token's largest value in [1, 2), each 32 columns turned, the 16-byte piece p
+// of token i at p ^ (i % 8).
 template <int DKP>
 __device__ __forceinline__ int piece_at(int token, int p) {
   return token * (DKP * 2) + ((p ^ (token & 7)) << 4);

@@ -208,15 +208,16 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
         for (int pl = 0; pl < PK; ++pl) rows[s & 1][pl][mt] = rows_frag<DKP>(ki + pl * PLANE, mt, s, r, gq);
     };
     read(0);
-    f32x4 ks[4], out[4], fq[4], fb[4];
+    f32x4 ks[4], out[4], fq[4], fb[4], fp[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       ks[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
       out[mt] = *(const f32x4*)&f->out[16 * mt + 4 * gq] * st_down;
       fq[mt] = *(const f32x4*)&f->q[16 * mt + 4 * gq];
       fb[mt] = *(const f32x4*)&f->back[16 * mt + 4 * gq];
+      fp[mt] = *(const f32x4*)&f->pt[16 * mt + 4 * gq] * dh_scale;
     }
-    const float keep = f->all, t_scale = f->tt, p_scale = f->p;
+    const float keep = f->all, t_scale = f->tt;
     f16_t* const to_ds = p.kept.ds + kept_at(part0 + c, p.kept.blocks, block, PK, DKP);
     f16x8 sh[2], sl[2];
     split8(st[0], st[1], sh[0], sl[0]);
@@ -254,11 +255,10 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
       for (int i = 0; i < LOWER; ++i) x[upper_mt(i)] = mfma(ph[i], dl[upper_s(i)], x[upper_mt(i)]);
     }
     load_p(next);
-    const float px = p_scale * dh_scale;
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) du[mt][e] = fmaf(x[mt][e], px, out[mt][e] * ks[mt][e]);
+      for (int e = 0; e < 4; ++e) du[mt][e] = fmaf(x[mt][e], fp[mt][e], out[mt][e] * ks[mt][e]);
     const Pow2 us = pow2_for(wave_max_all(abs_max(du)));
     f16x8 uh[2], ul[2];
 #pragma unroll
@@ -390,7 +390,7 @@ struct GradLds {
   static constexpr int A = STAGE > IMAGE + KK ? STAGE : IMAGE + KK;  // the columns; then K or Q, and K K^T
   static constexpr int OPERANDS = (std::is_same_v<T, bf16_t> ? 3 : 6) * L * L * 2;
   static constexpr int B = 2 * KK > OPERANDS ? 2 * KK : OPERANDS;  // dP, dA; then their operands
-  static constexpr int SMALL = (4 * DKB + 1) * L * 4 + 64 * 4 + L * 8 + 3 * L * 4;
+  static constexpr int SMALL = (4 * DKB + 1) * L * 4 + 64 * 4 + L * 8 + 4 * L * 4;
   static constexpr int BYTES = A + B + SMALL;
 };
 
@@ -410,6 +410,7 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   double* bs = (double*)(wred + 64);
   float* betas = (float*)(bs + L);        // [L], then row sums [2][L]
   float* rows = betas + L;
+  float* ksc = rows + 2 * L;              // the scales of K's rows
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, gq = lane >> 4;
   const int64_t part = mfma::xcd_contiguous(blockIdx.x, gridDim.x);
@@ -451,6 +452,7 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   if (tid < L) {
     bs[tid] = f->b[tid];
     betas[tid] = f->beta[tid];
+    ksc[tid] = power_of(f->k[tid]);
   }
 
   // ---- staging: pieces of 16 bytes, through registers
@@ -701,7 +703,6 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   put_image();
   bring(p.prep.q);
   lds_barrier();
-  const float ksc = f->k, qsc = f->qs;
 #pragma unroll
   for (int x = 0; x < (10 + W - 1) / W; ++x) {
     const int tile = x * W + wave;
@@ -718,7 +719,7 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
       y = mfma(a, c, y);
     }
 #pragma unroll
-    for (int e = 0; e < 4; ++e) kkm[(16 * i + 4 * gq + e) * GLD + 16 * j + r] = y[e] * (ksc * ksc);
+    for (int e = 0; e < 4; ++e) kkm[(16 * i + 4 * gq + e) * GLD + 16 * j + r] = y[e] * (ksc[16 * i + 4 * gq + e] * ksc[16 * j + r]);
   }
   // sum over DQK's columns of this wave of K or Q times a turned accumulator, into red[slot][wave][token]
   auto dots = [&](const f32x4 (&g)[2][4], int slot) {
@@ -745,18 +746,20 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   lds_barrier();
 
   // ---- each pair of tokens: wave w has rows w, w + W, .., a lane a column
-  // dQ takes scale D o dP against K's planes, dK its transpose against Q's and E + E^T against K's: the planes' scales enter here, and
-  // dK's two have one scale between them, so that their sum is in one unit.  (A chunk without a pair of tokens has zeros for E, one without
+  // dQ takes scale D o dP against K's planes, dK its transpose against Q's and E + E^T against K's: the scales of the planes' rows enter
+  // here, and dK's two have one scale between them, so that their sum is in one unit.  (A chunk without a pair of tokens has zeros for E, one without
   // dH for dP: in units of its own the other part could be past float32's range.)
-  float dpk[ROWS], dpq[ROWS], ee[ROWS], col = 0.f, mx[2] = {0.f, 0.f};
+  float dps[ROWS], ee[ROWS], col = 0.f, mx[2] = {0.f, 0.f};
   const double bj = bs[lane];
-  const float p_scale = f->p;
+  // a lane's token's; a row's are read from its lane
+  const float kj = ksc[lane], qj = power_of(f->qs[lane]), pj = power_of(f->p[lane]);
+  auto of_row = [&](float x, int i) { return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), i)); };
 #pragma unroll
   for (int x = 0; x < ROWS; ++x) {
     const int i = x * W + wave, j = lane;
     const bool on = j <= i, below = j < i;
     const float dec = on ? exp_of(bs[i] - bj) : 0.f;
-    const float pv = on ? ((float)ph[x] + (float)pl[x]) * p_scale : 0.f;
+    const float pv = on ? ((float)ph[x] + (float)pl[x]) * of_row(pj, i) : 0.f;
     const float dp = on ? dpm[i * GLD + j] : 0.f, da = below ? dam[i * GLD + j] : 0.f, beta = betas[i];
     const float nij = below ? dec * kkm[i * GLD + j] : 0.f;
     const float bb = wave_sum_dpp(da * nij), pp = wave_sum_dpp(dp * pv);
@@ -765,11 +768,10 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
       rows[L + i] = bb;
     }
     col += fmaf(dp, pv, beta * (da * nij));
-    dpk[x] = p.scale * dec * dp * ksc;
-    dpq[x] = p.scale * dec * dp * qsc;
-    ee[x] = da * beta * dec * ksc;
-    mx[0] = fmaxf(mx[0], fabsf(dpk[x]));
-    mx[1] = fmaxf(mx[1], fmaxf(fabsf(dpq[x]), fabsf(ee[x])));
+    dps[x] = p.scale * dec * dp;
+    ee[x] = da * beta * dec;
+    mx[0] = fmaxf(mx[0], fabsf(dps[x]) * kj);
+    mx[1] = fmaxf(mx[1], fmaxf(fabsf(dps[x]) * of_row(qj, i), fabsf(ee[x]) * fmaxf(kj, of_row(kj, i))));
   }
   red[(2 * W + wave) * L + lane] = col;
   const float m0 = wave_max_all(mx[0]), m1 = wave_max_all(mx[1]), dot = wave_sum(ss_dot);
@@ -805,11 +807,10 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
 #pragma unroll
   for (int x = 0; x < ROWS; ++x) {
     const int i = x * W + wave, j = lane;
-    const float e = ee[x] * sk.up;
-    put(0, i, j, dpk[x] * sq.up);
-    put(1, j, i, dpq[x] * sk.up);
-    if (j <= i) put(2, i, j, e);
-    if (j < i) put(2, j, i, e);
+    put(0, i, j, dps[x] * kj * sq.up);
+    put(1, j, i, dps[x] * of_row(qj, i) * sk.up);
+    if (j <= i) put(2, i, j, ee[x] * kj * sk.up);
+    if (j < i) put(2, j, i, ee[x] * of_row(kj, i) * sk.up);
   }
   lds_barrier();
   auto pair_frag = [&](int mat, int pl, int mt, int s) {
@@ -838,7 +839,8 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   f32x4 accq[2][4], acck[2][4];
 #pragma unroll
   for (int mt = 0; mt < 4; ++mt) {
-    const float fo = ldexpf(f->out[16 * mt + r] / ksc, top[U_DS]), fb = ldexpf(f->back[16 * mt + r] / ksc, top[Z_S]);
+    const double bt = bs[16 * mt + r];
+    const float fo = ldexpf(exp_of(bs[L - 1] - bt), top[U_DS]), fb = ldexpf(betas[16 * mt + r] * exp_of(bt), top[Z_S]);
 #pragma unroll
     for (int t = 0; t < 2; ++t) {
       g3[t][mt] = g3[t][mt] * fo - g2[t][mt] * fb;
@@ -856,7 +858,7 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
   {
     float fq[4];
 #pragma unroll
-    for (int mt = 0; mt < 4; ++mt) fq[mt] = ldexpf(f->q[16 * mt + r] / qsc, top[DH_S]);
+    for (int mt = 0; mt < 4; ++mt) fq[mt] = ldexpf(p.scale * exp_of(bs[16 * mt + r]), top[DH_S]);
     auto write = [&](auto type, auto whole) {
       using O = decltype(type);
       const int d = 32 * wave + 4 * gq;
@@ -901,12 +903,12 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
     qd += red[(3 * W + w) * L + lane];
     dss += wred[16 + w];
   }
-  kz = ldexpf(kz * ksc, top[Z_S]);
-  const float sj = ldexpf(f->out[lane] * ks, top[U_DS]);   // out has K's scale, which ks lacks
+  const float ckz = ldexpf(f->in[lane] * kz, top[Z_S]);    // in and out have K's scale, which kz and ks lack
+  const float sj = ldexpf(f->out[lane] * ks, top[U_DS]);
   const float qi = ldexpf(f->q[lane] * qd, top[DH_S]);
-  const float ci = f->in[lane] / ksc, beta = betas[lane];
-  const float dbeta = red[4 * W * L + lane] - ci * kz + rows[L + lane];
-  float db = rows[lane] + beta * rows[L + lane] - cl - sj + qi - beta * ci * kz;
+  const float beta = betas[lane];
+  const float dbeta = red[4 * W * L + lane] - ckz + rows[L + lane];
+  float db = rows[lane] + beta * rows[L + lane] - cl - sj + qi - beta * ckz;
   const float sums = wave_sum(sj) + ldexpf(f->all * dss, top[S_DS]);
   if (lane == 63) db += sums;
 #pragma unroll

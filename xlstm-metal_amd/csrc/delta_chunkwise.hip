@@ -61,7 +61,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
   const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
   T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
-  float* const scales = (float*)(lds + Lds::SCALES);  // [R, U, state][part]
+  float* const scales = (float*)(lds + Lds::SCALES);  // [R, U, state, U decayed][part]
   // sums over part `from`'s rows of token tile mt (its owner's own too: to leave those out took branches that cost more)
   auto sums_at = [&](int mt, int from) { return (f32x4*)(lds + Lds::SUMS) + (mt * PARTS + from) * 64 + lane; };
   auto sum_of = [&](int mt) {
@@ -214,7 +214,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
 
     // ---- 1: K S, and Q S turned, over the wave's rows
     f32x4 ks[4], hs[STATES ? 1 : 4], in[TPW], out[TPW];
-    float fq[TPW];
+    float fq[TPW], fp[TPW];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       ks[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -265,9 +265,12 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       const int mt = part * TPW + x;
       in[x] = *(const f32x4*)&f->in[16 * mt + 4 * gq] * st_down;
       out[x] = *(const f32x4*)&f->out[16 * mt + 4 * gq];
-      if constexpr (!STATES) fq[x] = f->q[16 * mt + r] * st_down;
+      if constexpr (!STATES) {
+        fq[x] = f->q[16 * mt + r] * st_down;
+        fp[x] = power_of(f->p[16 * mt + r]);
+      }
     }
-    const float keep = f->all, t_scale = f->t, p_scale = f->p;
+    const float keep = f->all, t_scale = f->t;
     const Pow2 decayed = pow2_for(f->most, 0);  // U decayed is below 2 decayed.down times U
     most = state_max(st) * st_down;
     if (lane == 0) scales[2 * PARTS + part] = most;
@@ -341,7 +344,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     load_t(next);
     const Pow2 us = pow2_for(wave_max_all(abs_max(u)));
     // at most 2^126: U of zeros has the largest scale there is, and keys far below 1 another
-    const float ws_up = fminf(us.up * decayed.up * 0.5f, 0x1p126f);
+    const float ws_up = fminf(us.up * decayed.up * 0.5f, 0x1p126f), ws_down = fmaxf(us.down * decayed.down * 2.f, 0x1p-126f);
 #pragma unroll
     for (int x = 0; x < TPW; ++x) {
       const int mt = part * TPW + x;
@@ -354,7 +357,10 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
         else *((f16x4*)(lds + Lds::U) + mt * 64 + lane) = hi;
       }
     }
-    if (lane == 0) scales[PARTS + part] = us.down;
+    if (lane == 0) {
+      scales[PARTS + part] = us.down;
+      scales[3 * PARTS + part] = ws_down;
+    }
     if constexpr (!STATES) {
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) *sums_at(mt, part) = hs[mt];
@@ -364,9 +370,10 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     f16x8 kc[2 * NB][PK][2], raw_u[PAIR ? 4 : 1];
     f16x4 half_u[PAIR || STATES ? 1 : 4];
     f32x4 qs[STATES ? 1 : TPW];
-    float of_u[PARTS], of_s[PARTS];
+    float of_u[PARTS], of_s[PARTS], of_w[PARTS];
     read_scales(1, of_u);
     read_scales(2, of_s);
+    read_scales(3, of_w);
     read4(Lds::UD);
 #pragma unroll
     for (int t = 0; t < 2 * NB; ++t)
@@ -382,11 +389,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    const float u_down = largest(of_u);
-    float of_w[PARTS];  // the inverses of the parts' ws_up
-#pragma unroll
-    for (int i = 0; i < PARTS; ++i) of_w[i] = fmaxf(of_u[i] * decayed.down * 2.f, 0x1p-126f);
-    const float w_down = largest(of_w);
+    const float u_down = largest(of_u), w_down = largest(of_w);
     // U decayed is below 2^15 w_down
     const Pow2 sc = pow2_for(fmaxf(largest(of_s) * keep, w_down * 32767.f), STATE);
     f16x8 wh[2], wl[2];
@@ -443,7 +446,6 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
 #pragma unroll
         for (int s = 0; s < 2; ++s) uh[s] = join(half_u[2 * s] * by[2 * s / TPW], half_u[2 * s + 1] * by[(2 * s + 1) / TPW]);
       }
-      const float pu = p_scale * u_down;
 #pragma unroll
       for (int x = 0; x < TPW; ++x) {
         const int mt = part * TPW + x;
@@ -460,7 +462,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
             y = mfma(uh[1], pl[x][1], y);
           }
         }
-        o[x] = rounded4<T>(y * pu + qs[x] * fq[x]);
+        o[x] = rounded4<T>(y * (fp[x] * u_down) + qs[x] * fq[x]);
       }
     }
     st_down = sc.down;
@@ -604,14 +606,17 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
     Rows rows[2];
     read(rows[0], 0);
     f32x4 in[4], out[4];
-    float fq[4];
+    float fq[4], fp[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       in[mt] = *(const f32x4*)&f->in[16 * mt + 4 * gq] * st_down;
       out[mt] = *(const f32x4*)&f->out[16 * mt + 4 * gq];
-      if constexpr (!STATES) fq[mt] = f->q[16 * mt + r] * st_down;
+      if constexpr (!STATES) {
+        fq[mt] = f->q[16 * mt + r] * st_down;
+        fp[mt] = power_of(f->p[16 * mt + r]);
+      }
     }
-    const float keep = f->all, t_scale = f->t, p_scale = f->p;
+    const float keep = f->all, t_scale = f->t;
     const Pow2 decayed = pow2_for(f->most, 0);  // U decayed is below 2 decayed.down times U
     f16x8 sh[2], sl[2];
     split8(st[0], st[1], sh[0], sl[0]);
@@ -743,13 +748,12 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
     }
     // ---- H
     if constexpr (!STATES) {
-      const float pu = p_scale * us.down;
       const int t0 = c * L;
       T* const to = ho + (int64_t)t0 * p.DV + n0;
       const bool whole = t0 + L <= p.S && n0 + 16 <= p.DV && p.DV % 4 == 0;
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) {
-        const Four<T> o = rounded4<T>(x[mt] * pu + hs[mt] * fq[mt]);
+        const Four<T> o = rounded4<T>(x[mt] * (fp[mt] * us.down) + hs[mt] * fq[mt]);
         if (whole) {
           *(Four<T>*)((char*)(to + (int64_t)(16 * mt) * p.DV) + h_at) = o;
         } else if (t0 + 16 * mt + r < p.S) {

@@ -1,7 +1,7 @@
 // Gated delta rule by chunks, first kernel: what of a chunk does not depend on the state (delta.h has the formulas).
 //
-// A workgroup of 4 waves takes one chunk of one head of q and k: it brings K and Q to f16 planes at a power-of-two scale (their
-// images go to memory as the scans' LDS wants them), forms K K^T and Q K^T once, and for each head of v that shares them
+// A workgroup of 4 waves takes one chunk of one head of q and k: it brings K and Q to f16 planes, each token at a power-of-two scale of
+// its own (their images go to memory as the scans' LDS wants them), forms K K^T and Q K^T once, and for each head of v that shares them
 // the sums of g (in float64: differences of sums of strong decays keep their bits), A, T = (I + A)^-1 and P.
 //
 // T by 16 x 16 blocks, in float32: each wave inverts one diagonal block by substitution (a lane a column), then walks down
@@ -79,6 +79,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
   extern __shared__ __align__(1024) char lds[];  // the images of K and Q; then A, T and P
   __shared__ double bs[L];
   __shared__ float betas[L], red[4][8];
+  __shared__ float ksc[L], qsc[L];  // rows of K, Q = planes * these; 0 for rows of zeros
   float *Am = (float*)lds, *Tm = Am + L * MLD, *Pm = Tm + L * MLD;
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, gq = lane >> 4;
@@ -89,7 +90,6 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
 
   // ---- K and Q: a row's 32 columns are one piece of 8 of each of 4 threads
   const int row = tid >> 2, c = tid & 3;
-  float scales[2];  // K, Q = planes * these
   Raw8<T> raw[2][DKB];  // both under way at once
   const bool there = t0 + row < p.S;  // past the last token: its row again, for zeros
 #pragma unroll
@@ -117,7 +117,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
   load_gates((int64_t)b * p.NH + hk * group);
   float m2[2] = {0.f, 0.f};
 #pragma unroll
-  for (int which = 0; which < 2; ++which)
+  for (int which = 0; which < 2; ++which) {
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
       float x[8];
@@ -125,11 +125,13 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
 #pragma unroll
       for (int e = 0; e < 8; ++e) m2[which] = fmaxf(m2[which], there ? fabsf(x[e]) : 0.f);
     }
-  block_max(m2, red);
+    m2[which] = fmaxf(m2[which], __shfl_xor(m2[which], 1, 64));
+    m2[which] = fmaxf(m2[which], __shfl_xor(m2[which], 2, 64));
+  }
 #pragma unroll
   for (int which = 0; which < 2; ++which) {
-    const Pow2 sc = m2[which] > 0.f ? pow2_for(m2[which], 0) : Pow2{1.f, 1.f};
-    scales[which] = sc.down;
+    const Pow2 sc = m2[which] == 0.f ? Pow2{1.f, 0.f} : pow2_for(m2[which], 0);
+    if (c == 0) (which ? qsc : ksc)[row] = sc.down;
     const float up = there ? sc.up : 0.f;
     char* to = lds + which * PK * IMG;
 #pragma unroll
@@ -205,36 +207,40 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
       bs[lane] = sum;
       betas[lane] = bt;
       Factors* f = p.out.f + part;
-      const float in = exp_of(sum);
+      const float in = exp_of(sum), ks = ksc[lane], qs = qsc[lane];
       f->b[lane] = sum;
-      f->in[lane] = in * scales[0];
-      f->q[lane] = in * scales[1] * p.scale;
-      const float out = exp_of(last - sum) * scales[0], most = wave_max_all(out);
+      f->in[lane] = in * ks;
+      f->q[lane] = in * qs * p.scale;
+      const float out = exp_of(last - sum) * ks, most = wave_max_all(out);
       f->out[lane] = out;
       if (lane == 0) f->most = most;
-      f->back[lane] = bt * in * scales[0];
+      f->back[lane] = bt * in * ks;
+      f->k[lane] = exponent_of(ks);
+      f->qs[lane] = exponent_of(qs);
       f->beta[lane] = bt;
     }
     __syncthreads();
     // ---- A and P
     double bi[4];
-    float be[4];
+    float be[4], sp[4];
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
-      bi[e] = bs[16 * wave + 4 * gq + e];
-      be[e] = betas[16 * wave + 4 * gq + e] * (scales[0] * scales[0]);
+      const int i = 16 * wave + 4 * gq + e;
+      bi[e] = bs[i];
+      be[e] = betas[i] * ksc[i];
+      sp[e] = p.scale * qsc[i];
     }
-    const float sp = p.scale * scales[0] * scales[1];
 #pragma unroll
     for (int jt = 0; jt < 4; ++jt) {
       const int j = 16 * jt + r;
       const double bj = bs[j];
+      const float kj = ksc[j];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 16 * wave + 4 * gq + e;
-        const float dec = jt <= wave && j <= i ? exp_of(bi[e] - bj) : 0.f;
+        const float dec = jt <= wave && j <= i ? exp_of(bi[e] - bj) * kj : 0.f;
         Am[i * MLD + j] = j < i ? be[e] * dec * kk[jt][e] : 0.f;
-        Pm[i * MLD + j] = j <= i ? sp * dec * qk[jt][e] : 0.f;
+        Pm[i * MLD + j] = j <= i ? sp[e] * dec * qk[jt][e] : 0.f;
         Tm[i * MLD + j] = 0.f;
       }
     }
@@ -283,50 +289,61 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
       for (int e = 0; e < 4; ++e) Tm[(16 * (wave + d) + 4 * gq + e) * MLD + 16 * wave + r] = col[d][e];
     }
     __syncthreads();
-    // ---- operands: wave w has frags w and w + 4 of each matrix
-    constexpr int MATS = BWD ? 4 : 2;  // T diag(beta), P; T^T, P^T
-    float x[MATS][2][8], m[MATS];
-#pragma unroll
-    for (int mat = 0; mat < MATS; ++mat) m[mat] = 0.f;
-#pragma unroll
-    for (int half = 0; half < 2; ++half) {
-      const int frag = wave + 4 * half, i = 16 * (frag >> 1) + r, s = frag & 1;
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const int j = 32 * s + (e < 4 ? 4 * gq + e : 12 + 4 * gq + e);
-        x[0][half][e] = Tm[i * MLD + j] * betas[j];
-        x[1][half][e] = Pm[i * MLD + j];
-        if constexpr (BWD) {
-          x[2][half][e] = Tm[j * MLD + i];
-          x[3][half][e] = Pm[j * MLD + i];
-        }
-#pragma unroll
-        for (int mat = 0; mat < MATS; ++mat) m[mat] = fmaxf(m[mat], fabsf(x[mat][half][e]));
-      }
-    }
-    block_max(m, red);
-#pragma unroll
-    for (int mat = 0; mat < MATS; ++mat) {
-      constexpr bool P_LO = BWD || !std::is_same_v<T, bf16_t>;  // bf16's scan takes P as one plane
-      const float up = pow2_for(m[mat], 10).up;
-      f16_t* to = (mat == 0 ? p.out.t : mat == 1 ? p.out.p : mat == 2 ? p.out.tt : p.out.pt) + part * (2 * FRAG_PLANE);
+    // ---- operands: wave w has the 16 rows 16 w .. of each matrix, both halves of k
+    constexpr int FORMS = BWD ? 2 : 1;  // P, T diag(beta); P^T, T^T
+    Factors* f = p.out.f + part;
+    const int i = 16 * wave + r;
+    auto column = [&](int half, int e) { return 32 * half + (e < 4 ? 4 * gq + e : 12 + 4 * gq + e); };
+    auto write = [&](f16_t* to, const float (&x)[2][8], float up, bool with_lo) {
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         f16x8 hi, lo;
-        split8<true>(x[mat][half], up, hi, lo);
-        f16_t* at = to + ((wave + 4 * half) * 64 + lane) * 8;
+        split8<true>(x[half], up, hi, lo);
+        f16_t* at = to + part * (2 * FRAG_PLANE) + ((2 * wave + half) * 64 + lane) * 8;
         *(f16x8*)at = hi;
-        if (mat != 1 || P_LO) *(f16x8*)(at + FRAG_PLANE) = lo;
+        if (with_lo) *(f16x8*)(at + FRAG_PLANE) = lo;
+      }
+    };
+#pragma unroll
+    for (int turned = 0; turned < FORMS; ++turned) {  // P: a scale a row
+      float x[2][8], m = 0.f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = column(half, e);
+          x[half][e] = turned ? Pm[j * MLD + i] : Pm[i * MLD + j];
+          m = fmaxf(m, fabsf(x[half][e]));
+        }
+      m = fmaxf(m, __shfl_xor(m, 16, 64));
+      m = fmaxf(m, __shfl_xor(m, 32, 64));
+      const Pow2 sc = pow2_for(m, 10);
+      write(turned ? p.out.pt : p.out.p, x, sc.up, BWD || !std::is_same_v<T, bf16_t>);  // bf16's scan takes P as one plane
+      if (gq == 0) {
+        if (turned) f->pt[i] = sc.down;
+        else f->p[i] = exponent_of(sc.down);
       }
     }
+    float x[FORMS][2][8], m[FORMS];
+#pragma unroll
+    for (int turned = 0; turned < FORMS; ++turned) {  // T: one scale
+      m[turned] = 0.f;
+#pragma unroll
+      for (int half = 0; half < 2; ++half)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          const int j = column(half, e);
+          x[turned][half][e] = turned ? Tm[j * MLD + i] : Tm[i * MLD + j] * betas[j];
+          m[turned] = fmaxf(m[turned], fabsf(x[turned][half][e]));
+        }
+    }
+    block_max(m, red);
+#pragma unroll
+    for (int turned = 0; turned < FORMS; ++turned) write(turned ? p.out.tt : p.out.t, x[turned], pow2_for(m[turned], 10).up, true);
     if (tid == 0) {
-      Factors* f = p.out.f + part;
       f->all = exp_of(last);
       f->t = pow2_for(m[0], 10).down;
-      f->p = pow2_for(m[1], 10).down;
-      f->tt = BWD ? pow2_for(m[BWD ? 2 : 0], 10).down : 0.f;
-      f->k = scales[0];
-      f->qs = scales[1];
+      f->tt = BWD ? pow2_for(m[FORMS - 1], 10).down : 0.f;
     }
     __syncthreads();
   }
