@@ -98,14 +98,14 @@ __device__ __forceinline__ void interleave() {
 }
 
 // 2^target / 2^exponent(m) and its inverse: m times the first is in [2^target, 2^(target + 1)); m >= 0.
-// At most 2^100 either way (0 gets that).
+// At most 2^most either way (0 gets that).
 struct Pow2 {
   float up, down;
 };
-__device__ __forceinline__ Pow2 pow2_for(float m, int target = 14) {
+__device__ __forceinline__ Pow2 pow2_for(float m, int target = 14, int most = 100) {
   const int e = (int)(__float_as_uint(m) >> 23);
   int sh = e == 255 ? 0 : target + 127 - e;
-  sh = sh > 100 ? 100 : sh < -100 ? -100 : sh;
+  sh = sh > most ? most : sh < -100 ? -100 : sh;
   return {__uint_as_float((uint32_t)(127 + sh) << 23), __uint_as_float((uint32_t)(127 - sh) << 23)};
 }
 

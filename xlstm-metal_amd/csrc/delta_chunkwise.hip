@@ -61,7 +61,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
   const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
   T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
-  float* const scales = (float*)(lds + Lds::SCALES);  // [R, U, state, U decayed][part]
+  float* const scales = (float*)(lds + Lds::SCALES);  // [R, U, state][part]
   // sums over part `from`'s rows of token tile mt (its owner's own too: to leave those out took branches that cost more)
   auto sums_at = [&](int mt, int from) { return (f32x4*)(lds + Lds::SUMS) + (mt * PARTS + from) * 64 + lane; };
   auto sum_of = [&](int mt) {
@@ -272,6 +272,8 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     }
     const float keep = f->all, t_scale = f->t;
     const Pow2 decayed = pow2_for(f->most, 0);  // U decayed is below 2 decayed.down times U
+    // The product of both scales is at most 2^126: U of zeros would have the largest there is, and keys far below 1 have another.
+    const int most_up = min(100, 254 - (int)(__float_as_uint(decayed.up) >> 23));
     most = state_max(st) * st_down;
     if (lane == 0) scales[2 * PARTS + part] = most;
     lds_barrier();
@@ -342,9 +344,8 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       w[x] = u[x] * out[x];
     }
     load_t(next);
-    const Pow2 us = pow2_for(wave_max_all(abs_max(u)));
-    // at most 2^126: U of zeros has the largest scale there is, and keys far below 1 another
-    const float ws_up = fminf(us.up * decayed.up * 0.5f, 0x1p126f), ws_down = fmaxf(us.down * decayed.down * 2.f, 0x1p-126f);
+    const Pow2 us = pow2_for(wave_max_all(abs_max(u)), 14, most_up);
+    const float ws_up = us.up * decayed.up * 0.5f;
 #pragma unroll
     for (int x = 0; x < TPW; ++x) {
       const int mt = part * TPW + x;
@@ -357,10 +358,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
         else *((f16x4*)(lds + Lds::U) + mt * 64 + lane) = hi;
       }
     }
-    if (lane == 0) {
-      scales[PARTS + part] = us.down;
-      scales[3 * PARTS + part] = ws_down;
-    }
+    if (lane == 0) scales[PARTS + part] = us.down;
     if constexpr (!STATES) {
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) *sums_at(mt, part) = hs[mt];
@@ -370,10 +368,9 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     f16x8 kc[2 * NB][PK][2], raw_u[PAIR ? 4 : 1];
     f16x4 half_u[PAIR || STATES ? 1 : 4];
     f32x4 qs[STATES ? 1 : TPW];
-    float of_u[PARTS], of_s[PARTS], of_w[PARTS];
+    float of_u[PARTS], of_s[PARTS];
     read_scales(1, of_u);
     read_scales(2, of_s);
-    read_scales(3, of_w);
     read4(Lds::UD);
 #pragma unroll
     for (int t = 0; t < 2 * NB; ++t)
@@ -389,11 +386,11 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    const float u_down = largest(of_u), w_down = largest(of_w);
+    const float u_down = largest(of_u), w_down = u_down * decayed.down * 2.f;
     // U decayed is below 2^15 w_down
     const Pow2 sc = pow2_for(fmaxf(largest(of_s) * keep, w_down * 32767.f), STATE);
     f16x8 wh[2], wl[2];
-    shifts(of_w, w_down, by);
+    shifts(of_u, u_down, by);
     planes(by, wh, wl);
     if constexpr (!STATES) {
 #pragma unroll
@@ -437,7 +434,6 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       }
     } else {  // ---- H
       f16x8 uh[2], ul[2];
-      shifts(of_u, u_down, by);
       if constexpr (PAIR) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) raw[i] = raw_u[i];
