@@ -36,7 +36,7 @@
 extern "C" {
 #endif
 
-#define XL_ABI_VERSION 5
+#define XL_ABI_VERSION 6
 
 enum xl_dtype { XL_DTYPE_F32 = 0, XL_DTYPE_BF16 = 1, XL_DTYPE_F16 = 2 };
 
@@ -439,10 +439,13 @@ int xl_gated_delta_chunkwise_fwd(const void* q, const void* k, const void* v, co
 /*
  * Its gradients: dq, dk [B, NHK, S, DQK] and dv [B, NH, S, DV] of dtype_qkv, dg, dbeta [B, NH, S] of dtype_gates, all
  * contiguous (dq, dk and dv 16-byte aligned), and dc0 float32 or NULL, from dh [B, NH, S, DV] of dtype_qkv, contiguous, and
- * dc_last, the gradient of the last state, float32 or NULL.  S at least 1.  The workspace
- * (xl_gated_delta_chunkwise_bwd_workspace_size bytes, 256-byte aligned) holds every chunk's state and its gradient.
+ * dc_last, the gradient of the last state, float32 or NULL.  S at least 1.  The workspace, 256-byte aligned, holds every chunk's
+ * state and its gradient: xl_gated_delta_chunkwise_bwd_workspace_size bytes for gates of any type,
+ * xl_gated_delta_chunkwise_bwd_workspace_size_gates for those of dtype_gates (fewer where q, k, v and gates are bf16).
  */
 size_t xl_gated_delta_chunkwise_bwd_workspace_size(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv);
+size_t xl_gated_delta_chunkwise_bwd_workspace_size_gates(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv,
+                                                         int dtype_gates);
 int xl_gated_delta_chunkwise_bwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* g,
                                  const void* beta, const float* c0, const void* dh, const float* dc_last, void* dq,
                                  void* dk, void* dv, void* dg, void* dbeta, float* dc0, int B, int NH, int NHK, int S,

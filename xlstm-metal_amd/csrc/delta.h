@@ -40,10 +40,13 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef __attribute__((address_space(3))) char lds_char;
 
 constexpr int L = 64;           // tokens of a chunk
-// f16 planes of K and Q and of what the backward keeps of U, Z and the states: pairs for float32, and for f16's backward, where one
-// plane's rounding is as large as the inputs' own and the differences that dg is made of show it (bf16's own is 8 times that)
-template <typename T, bool BWD>
-constexpr int PLANES = is_f32<T>::value || (BWD && std::is_same_v<T, f16_t>) ? 2 : 1;
+// f16 planes of K and Q: pairs for float32; 16-bit values have their bits in one
+template <typename T>
+constexpr int PLANES = is_f32<T>::value ? 2 : 1;
+// Planes that the backward keeps of U, Z, dH and the states (KEPT, 0 in the forward): pairs, but one where inputs and gates are bf16, whose own
+// rounding is 8 times a plane's.  The gates' gradients are made of differences that show it: one plane takes a float32 dg 3e-5 to
+// 6e-4 of its terms off, pairs below 1e-5.
+inline int kept_planes(int dtype, int dtype_gates) { return dtype == XL_DTYPE_BF16 && dtype_gates == XL_DTYPE_BF16 ? 1 : 2; }
 constexpr int MAX_DQK = 256;
 constexpr int FRAGS = 8;        // 16 x 32 operands of a 64 x 64 matrix: row tile mt, half s of k at 2 mt + s
 constexpr int FRAG_PLANE = FRAGS * 64 * 8;  // f16 values of one plane
@@ -288,10 +291,10 @@ struct Shape {
   int dtype, dtype_gates;
   int chunks() const { return (S + L - 1) / L; }
   int dkp() const { return DK <= 64 ? 64 : DK <= 128 ? 128 : 256; }
-  int planes(bool backward) const { return dtype == XL_DTYPE_F32 || (backward && dtype == XL_DTYPE_F16) ? 2 : 1; }
+  int kept() const { return kept_planes(dtype, dtype_gates); }
   int64_t images() const { return (int64_t)B * NHK * chunks(); }
   int64_t parts() const { return (int64_t)B * NH * chunks(); }
-  int64_t image_bytes(bool backward) const { return (int64_t)planes(backward) * L * dkp() * 2; }
+  int64_t image_bytes() const { return (int64_t)(dtype == XL_DTYPE_F32 ? 2 : 1) * L * dkp() * 2; }
 };
 
 // What the first kernel writes; transposed forms for the backward only.

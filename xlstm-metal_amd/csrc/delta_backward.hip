@@ -36,9 +36,8 @@ struct TurnArgs {
   bool wide;  // 16-byte loads
 };
 
-template <typename T>
+template <typename T, int KEPT>
 __global__ __launch_bounds__(256) void delta_turn_kernel(TurnArgs p) {
-  constexpr int PK = PLANES<T, true>;
   __shared__ float tile[L][65];
   const int64_t part = blockIdx.x;
   const int64_t bh = part / p.chunks;
@@ -76,10 +75,10 @@ __global__ __launch_bounds__(256) void delta_turn_kernel(TurnArgs p) {
 #pragma unroll
   for (int s = 0; s < 2; ++s) {
     f16x8 hi, lo;
-    split8<PK == 2>(x[s], sc.up, hi, lo);
-    f16_t* to = p.kept.dh + kept_at(part, p.kept.blocks, block, PK, L) + r * L + s * 32 + gq * 8;
+    split8<KEPT == 2>(x[s], sc.up, hi, lo);
+    f16_t* to = p.kept.dh + kept_at(part, p.kept.blocks, block, KEPT, L) + r * L + s * 32 + gq * 8;
     *(f16x8*)to = hi;
-    if constexpr (PK == 2) *(f16x8*)(to + 16 * L) = lo;
+    if constexpr (KEPT == 2) *(f16x8*)(to + 16 * L) = lo;
   }
   if (lane == 0) p.kept.dhs[part * p.kept.blocks + block] = sc.down;
 }
@@ -96,9 +95,9 @@ struct BackArgs {
 // As the forward's scan (delta_chunkwise.hip): operands are read ahead of their products, the next chunk's are on their way.
 // Four waves take a block each and bring the images together; a wave on its own has a second one that only brings them (a load into
 // LDS that has to queue stops its wave: 177 us without, 157 with, at 8192 tokens of 128 x 256, 2.5 a chunk).
-template <typename T, int DKB, int STAGES, int W>
+template <typename T, int DKB, int STAGES, int W, int KEPT>
 __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(BackArgs p) {
-  constexpr int DKP = DKB * 32, PK = PLANES<T, true>, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
+  constexpr int DKP = DKB * 32, PK = PLANES<T>, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = 2 * IMG;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
   const int lane = threadIdx.x & 63, in = uniform(threadIdx.x >> 6), wave = W == 1 ? 0 : in;
   const int r = lane & 15, gq = lane >> 4;
@@ -173,11 +172,11 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
     load_upper(from + FRAG_PLANE, lane, pl);
   };
   auto load_dh = [&](int chunk) {
-    const f16_t* from = p.kept.dh + kept_at(part0 + chunk, p.kept.blocks, block, PK, L);
+    const f16_t* from = p.kept.dh + kept_at(part0 + chunk, p.kept.blocks, block, KEPT, L);
 #pragma unroll
     for (int s = 0; s < 2; ++s) {
       dh[s] = load16(from, r * (L * 2) + gq * 16 + s * 64);
-      if constexpr (PK == 2) dl[s] = load16(from + 16 * L, r * (L * 2) + gq * 16 + s * 64);
+      if constexpr (KEPT == 2) dl[s] = load16(from + 16 * L, r * (L * 2) + gq * 16 + s * 64);
     }
     dh_scale = p.kept.dhs[(part0 + chunk) * p.kept.blocks + block];
   };
@@ -218,7 +217,7 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
       fp[mt] = *(const f32x4*)&f->pt[16 * mt + 4 * gq] * dh_scale;
     }
     const float keep = f->all, t_scale = f->tt;
-    f16_t* const to_ds = p.kept.ds + kept_at(part0 + c, p.kept.blocks, block, PK, DKP);
+    f16_t* const to_ds = p.kept.ds + kept_at(part0 + c, p.kept.blocks, block, KEPT, DKP);
     f16x8 sh[2], sl[2];
     split8(st[0], st[1], sh[0], sl[0]);
 #pragma unroll
@@ -229,7 +228,7 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
       const f16x8 hi = sh[s & 1], lo = sl[s & 1];
       if (mine) {
         *(f16x8*)((char*)to_ds + r * (DKP * 2) + gq * 16 + s * 64) = hi;
-        if constexpr (PK == 2) *(f16x8*)((char*)(to_ds + 16 * DKP) + r * (DKP * 2) + gq * 16 + s * 64) = lo;
+        if constexpr (KEPT == 2) *(f16x8*)((char*)(to_ds + 16 * DKP) + r * (DKP * 2) + gq * 16 + s * 64) = lo;
       }
       if (s + 1 < DKB) split8(st[2 * s + 2], st[2 * s + 3], sh[(s + 1) & 1], sl[(s + 1) & 1]);
 #pragma unroll
@@ -250,7 +249,7 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
     for (int i = 0; i < LOWER; ++i) x[upper_mt(i)] = mfma(ph[i], dh[upper_s(i)], x[upper_mt(i)]);
 #pragma unroll
     for (int i = 0; i < LOWER; ++i) x[upper_mt(i)] = mfma(pl[i], dh[upper_s(i)], x[upper_mt(i)]);
-    if constexpr (PK == 2) {
+    if constexpr (KEPT == 2) {
 #pragma unroll
       for (int i = 0; i < LOWER; ++i) x[upper_mt(i)] = mfma(ph[i], dl[upper_s(i)], x[upper_mt(i)]);
     }
@@ -295,7 +294,7 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         float d = (float)dh[mt >> 1][(mt & 1) * 4 + e];
-        if constexpr (PK == 2) d += (float)dl[mt >> 1][(mt & 1) * 4 + e];
+        if constexpr (KEPT == 2) d += (float)dl[mt >> 1][(mt & 1) * 4 + e];
         w1[mt][e] = fq[mt][e] * (d * dh_scale);
       }
     load_dh(next);
@@ -312,14 +311,14 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
     for (int s = 0; s < 2; ++s) {
       split8<true>(w1[2 * s], w1[2 * s + 1], ws.up, w1h[s], w1l[s]);
       split8<true>(w2[2 * s], w2[2 * s + 1], ws.up, w2h[s], w2l[s]);
-      split8<PK == 2>(z[2 * s], z[2 * s + 1], zs.up, zh[s], zl[s]);
+      split8<KEPT == 2>(z[2 * s], z[2 * s + 1], zs.up, zh[s], zl[s]);
     }
     if (mine) {
-      f16_t* to = p.kept.z + kept_at(part0 + c, p.kept.blocks, block, PK, L);
+      f16_t* to = p.kept.z + kept_at(part0 + c, p.kept.blocks, block, KEPT, L);
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         *(f16x8*)((char*)to + r * (L * 2) + gq * 16 + s * 64) = zh[s];
-        if constexpr (PK == 2) *(f16x8*)((char*)(to + 16 * L) + r * (L * 2) + gq * 16 + s * 64) = zl[s];
+        if constexpr (KEPT == 2) *(f16x8*)((char*)(to + 16 * L) + r * (L * 2) + gq * 16 + s * 64) = zl[s];
       }
       if (lane == 0) {
         p.kept.zs[at] = zs.down;
@@ -381,11 +380,11 @@ struct GradArgs {
 
 constexpr int GLD = 65;
 
-template <typename T, int DKB>
+template <typename T, int DKB, int KEPT>
 struct GradLds {
-  static constexpr int PK = PLANES<T, true>, DKP = DKB * 32;
+  static constexpr int DKP = DKB * 32;
   static constexpr int TOK = 32 * L * 2, STA = 32 * DKP * 2;  // 32 columns of one plane
-  static constexpr int STAGE = PK * (3 * TOK + 2 * STA), IMAGE = PK * L * DKP * 2;
+  static constexpr int STAGE = KEPT * (3 * TOK + 2 * STA), IMAGE = PLANES<T> * L * DKP * 2;
   static constexpr int KK = L * GLD * 4;
   static constexpr int A = STAGE > IMAGE + KK ? STAGE : IMAGE + KK;  // the columns; then K or Q, and K K^T
   static constexpr int OPERANDS = (std::is_same_v<T, bf16_t> ? 3 : 6) * L * L * 2;
@@ -396,10 +395,10 @@ struct GradLds {
 
 // DKB waves: a wave has 32 of DQK's columns of dQ and dK, turned (columns down, tokens across), and its share of the 64 x 64 tiles.
 // At DQK 128 two workgroups fit a CU with 256 registers a lane (bf16: 165 us against 187, measured before it came to 133; pairs would spill).
-template <typename T, int DKB>
-__global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1)) void delta_grad_kernel(GradArgs p) {
-  using Lds = GradLds<T, DKB>;
-  constexpr int PK = Lds::PK, DKP = Lds::DKP, PLANE = L * DKP * 2, TOK = Lds::TOK, STA = Lds::STA, W = DKB, THREADS = 64 * W;
+template <typename T, int DKB, int KEPT>
+__global__ __launch_bounds__(64 * DKB, (DKB == 4 && KEPT == 1 ? 2 : 1)) void delta_grad_kernel(GradArgs p) {
+  using Lds = GradLds<T, DKB, KEPT>;
+  constexpr int PK = KEPT, PI = PLANES<T>, DKP = Lds::DKP, PLANE = L * DKP * 2, TOK = Lds::TOK, STA = Lds::STA, W = DKB, THREADS = 64 * W;
   constexpr bool PAIR = !std::is_same_v<T, bf16_t>;
   extern __shared__ __align__(1024) char lds[];
   char *areaA = lds, *areaB = lds + Lds::A;
@@ -667,14 +666,14 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
     }
   }
   // K and the wave's rows of P are on their way meanwhile
-  u32x4 image_regs[4 * PK];
+  u32x4 image_regs[4 * PI];
   auto bring = [&](const char* img) {
 #pragma unroll
-    for (int i = 0; i < 4 * PK; ++i) image_regs[i] = *(const u32x4*)(img + image * (PK * PLANE) + (i * THREADS + tid) * 16);
+    for (int i = 0; i < 4 * PI; ++i) image_regs[i] = *(const u32x4*)(img + image * (PI * PLANE) + (i * THREADS + tid) * 16);
   };
   auto put_image = [&] {
 #pragma unroll
-    for (int i = 0; i < 4 * PK; ++i) *(u32x4*)(areaA + (i * THREADS + tid) * 16) = image_regs[i];
+    for (int i = 0; i < 4 * PI; ++i) *(u32x4*)(areaA + (i * THREADS + tid) * 16) = image_regs[i];
   };
   static_assert(4 * THREADS * 16 == PLANE);
   bring(p.prep.k);
@@ -712,7 +711,7 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
 #pragma unroll
     for (int s = 0; s < DKB; ++s) {
       const f16x8 a = rows_frag<DKP>(areaA, i, s, r, gq), c = rows_frag<DKP>(areaA, j, s, r, gq);
-      if constexpr (PK == 2) {
+      if constexpr (PI == 2) {
         y = mfma(rows_frag<DKP>(areaA + PLANE, i, s, r, gq), c, y);
         y = mfma(a, rows_frag<DKP>(areaA + PLANE, j, s, r, gq), y);
       }
@@ -732,7 +731,7 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
         const char* at = areaA + piece_at<DKP>(16 * mt + r, 4 * (tile >> 1) + gq) + (tile & 1) * 8;
         const f16x4 a = *(const f16x4*)at;
         f16x4 al = {};
-        if constexpr (PK == 2) al = *(const f16x4*)(at + PLANE);
+        if constexpr (PI == 2) al = *(const f16x4*)(at + PLANE);
 #pragma unroll
         for (int e = 0; e < 4; ++e) x = fmaf((float)a[e] + (float)al[e], g[t][mt][e], x);
       }
@@ -825,11 +824,11 @@ __global__ __launch_bounds__(64 * DKB, (DKB == 4 && PLANES<T, true> == 1 ? 2 : 1
       for (int t = 0; t < 2; ++t) {
         const f16x8 a = columns_frag<DKP>(areaA, 2 * wave + t, s, r, gq);
         f16x8 al;
-        if constexpr (PK == 2) al = columns_frag<DKP>(areaA + PLANE, 2 * wave + t, s, r, gq);
+        if constexpr (PI == 2) al = columns_frag<DKP>(areaA + PLANE, 2 * wave + t, s, r, gq);
 #pragma unroll
         for (int mt = 0; mt < 4; ++mt) {
           const f16x8 x = pair_frag(mat, 0, mt, s);
-          if constexpr (PK == 2) acc[t][mt] = mfma(al, x, acc[t][mt]);
+          if constexpr (PI == 2) acc[t][mt] = mfma(al, x, acc[t][mt]);
           if constexpr (PAIR) acc[t][mt] = mfma(a, pair_frag(mat, 1, mt, s), acc[t][mt]);
           acc[t][mt] = mfma(a, x, acc[t][mt]);
         }
@@ -954,8 +953,8 @@ struct Layout {
   explicit Layout(const Shape& s) {
     blocks = 2 * ((s.DV + 31) / 32);
     prep = up256((int64_t)prep_bytes(s, true));
-    tok = up256(s.parts() * blocks * s.planes(true) * 16 * L * 2);
-    sta = up256(s.parts() * blocks * s.planes(true) * 16 * s.dkp() * 2);
+    tok = up256(s.parts() * blocks * s.kept() * 16 * L * 2);
+    sta = up256(s.parts() * blocks * s.kept() * 16 * s.dkp() * 2);
     scales = up256(s.parts() * blocks * 4);
     partial = s.NH == s.NHK ? 0 : up256((int64_t)s.B * s.NH * s.S * s.DK * 4);
   }
@@ -968,38 +967,38 @@ hipError_t launch(const void* kern, int64_t grid, int grid_y, int threads, int64
   return e != hipSuccess ? e : hipLaunchKernel(kern, dim3((unsigned)grid, grid_y), dim3(threads), args, (unsigned)lds, st);
 }
 
-template <typename T>
+template <typename T, int KEPT>
 int backward(const Shape& s, const void* v, const void* dh, const float* dc_last, void* dq, void* dk, void* dv, void* dg,
              void* dbeta, float* dc0, const float* c0, const Prep& prep, const Kept& kept, float* dqp, float* dkp, hipStream_t st,
              const char* who) {
   const int group = s.NH / s.NHK, chunks = s.chunks();
   TurnArgs turn{dh, kept, s.S, s.DV, chunks, s.DV % 8 == 0 && ((uintptr_t)dh & 15) == 0};
-  hipError_t e = launch((const void*)delta_turn_kernel<T>, s.parts(), (kept.blocks + 3) / 4, 256, 0, &turn, st);
+  hipError_t e = launch((const void*)delta_turn_kernel<T, KEPT>, s.parts(), (kept.blocks + 3) / 4, 256, 0, &turn, st);
   if (e == hipSuccess)
     if (const int rc = launch_scan(s, v, c0, nullptr, nullptr, prep, &kept, st, who)) return rc;
-  constexpr int S8 = PLANES<T, true> == 2 ? 1 : 2;
+  constexpr int S8 = PLANES<T> == 2 ? 1 : 2;
   const int stages = s.dkp() == 256 ? S8 : 2;
   // A lone wave a block where two workgroups a CU (one, if no two fit) take all blocks, else four blocks a workgroup.  us of whole calls,
   // 2048 tokens, lone waves and fours: bf16 128 x 256, 256 blocks 252, 277; 512 433, 454; 768 626, 572; 1024 755, 689; 64 x 256, 512
   // blocks 346, 357; 1024 637, 577; 256 x 512, 512 blocks 597, 548; float32 128 x 256, 512 blocks of 1024 tokens 362, 349.
-  const int64_t scan_lds = stages * 2 * s.image_bytes(true) + 2 * 2048;
+  const int64_t scan_lds = stages * 2 * s.image_bytes() + 2 * 2048;
   const int waves = (int64_t)s.B * s.NH * kept.blocks <= (scan_lds <= 80 * 1024 ? 512 : 256) ? 1 : 4;
   const int slices = (kept.blocks + waves - 1) / waves;
   BackArgs back{dc_last, dc0, prep, kept, s.NH, group, s.DK, s.DV, chunks, slices};
   const void* kern =
-      waves == 4 ? s.dkp() == 64    ? (const void*)delta_back_kernel<T, 2, 2, 4>
-                   : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2, 4> : (const void*)delta_back_kernel<T, 8, S8, 4>
-      : s.dkp() == 64    ? (const void*)delta_back_kernel<T, 2, 2, 1>
-        : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2, 1> : (const void*)delta_back_kernel<T, 8, S8, 1>;
+      waves == 4 ? s.dkp() == 64    ? (const void*)delta_back_kernel<T, 2, 2, 4, KEPT>
+                   : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2, 4, KEPT> : (const void*)delta_back_kernel<T, 8, S8, 4, KEPT>
+      : s.dkp() == 64    ? (const void*)delta_back_kernel<T, 2, 2, 1, KEPT>
+        : s.dkp() == 128 ? (const void*)delta_back_kernel<T, 4, 2, 1, KEPT> : (const void*)delta_back_kernel<T, 8, S8, 1, KEPT>;
   if (e == hipSuccess)
     e = launch(kern, (int64_t)s.B * s.NH * slices, 1, waves == 1 ? 128 : 64 * waves, scan_lds, &back, st);
   GradArgs grad{v, {s.vs[0], s.vs[1], s.vs[2]}, group == 1 ? dq : (void*)dqp, group == 1 ? dk : (void*)dkp, dv, dg, dbeta, prep, kept,
                 s.NH, group, s.S, s.DK, s.DV, chunks, s.dtype_gates, s.scale, false};
   constexpr int VW = 16 / sizeof(T);
   grad.wide_v = s.DV % 8 == 0 && ((s.vs[0] | s.vs[1] | s.vs[2]) % VW) == 0 && (((uintptr_t)v | (uintptr_t)dv) & 15) == 0;
-  const int lds = s.dkp() == 64 ? GradLds<T, 2>::BYTES : s.dkp() == 128 ? GradLds<T, 4>::BYTES : GradLds<T, 8>::BYTES;
-  kern = s.dkp() == 64 ? (const void*)delta_grad_kernel<T, 2> : s.dkp() == 128 ? (const void*)delta_grad_kernel<T, 4>
-                                                                              : (const void*)delta_grad_kernel<T, 8>;
+  const int lds = s.dkp() == 64 ? GradLds<T, 2, KEPT>::BYTES : s.dkp() == 128 ? GradLds<T, 4, KEPT>::BYTES : GradLds<T, 8, KEPT>::BYTES;
+  kern = s.dkp() == 64 ? (const void*)delta_grad_kernel<T, 2, KEPT> : s.dkp() == 128 ? (const void*)delta_grad_kernel<T, 4, KEPT>
+                                                                                    : (const void*)delta_grad_kernel<T, 8, KEPT>;
   if (e == hipSuccess) e = launch(kern, s.parts(), 1, s.dkp() * 2, lds, &grad, st);
   if (e == hipSuccess && group > 1) {
     const int64_t per = (int64_t)s.S * s.DK, count = (int64_t)s.B * s.NHK * per;
@@ -1015,11 +1014,17 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
 }  // namespace delta
 }  // namespace xl
 
-extern "C" size_t xl_gated_delta_chunkwise_bwd_workspace_size(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv) {
+extern "C" size_t xl_gated_delta_chunkwise_bwd_workspace_size_gates(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv,
+                                                                    int dtype_gates) {
   using namespace xl;
-  delta::Shape s{B, NH, NHK, S, DQK, DV, {}, {}, {}, 1.f, dtype_qkv, dtype_qkv};
+  delta::Shape s{B, NH, NHK, S, DQK, DV, {}, {}, {}, 1.f, dtype_qkv, dtype_gates};
   if (delta::check_shape("xl_gated_delta_chunkwise_bwd_workspace_size", s) != XL_OK) return 0;
   return S == 0 ? 0 : (size_t)delta::Layout(s).bytes();
+}
+
+// float32 gates keep pairs whatever q, k and v are
+extern "C" size_t xl_gated_delta_chunkwise_bwd_workspace_size(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv) {
+  return xl_gated_delta_chunkwise_bwd_workspace_size_gates(B, NH, NHK, S, DQK, DV, dtype_qkv, XL_DTYPE_F32);
 }
 
 extern "C" int xl_gated_delta_chunkwise_bwd(const void* q, const void* k, const void* v, const int64_t* strides, const void* g,
@@ -1061,10 +1066,11 @@ extern "C" int xl_gated_delta_chunkwise_bwd(const void* q, const void* k, const 
   kept.blocks = lay.blocks;
   float *dqp = (float*)take(lay.partial), *dkp = (float*)take(lay.partial);
   if (const int rc = delta::launch_prep(s, q, k, g, beta, prep, true, st, who)) return rc;
-  auto run = [&](auto t) {
-    return delta::backward<decltype(t)>(s, v, dh, dc_last, dq, dk, dv, dg, dbeta, dc0, c0, prep, kept, dqp, dkp, st, who);
+  auto run = [&](auto t, auto planes) {
+    return delta::backward<decltype(t), decltype(planes)::value>(s, v, dh, dc_last, dq, dk, dv, dg, dbeta, dc0, c0, prep, kept, dqp, dkp, st, who);
   };
-  if (dtype_qkv == XL_DTYPE_F32) return run(float{});
-  if (dtype_qkv == XL_DTYPE_BF16) return run(bf16_t{});
-  return run(f16_t{});
+  using Pairs = std::integral_constant<int, 2>;
+  if (dtype_qkv == XL_DTYPE_F32) return run(float{}, Pairs{});
+  if (dtype_qkv == XL_DTYPE_F16) return run(f16_t{}, Pairs{});
+  return s.kept() == 2 ? run(bf16_t{}, Pairs{}) : run(bf16_t{}, std::integral_constant<int, 1>{});
 }

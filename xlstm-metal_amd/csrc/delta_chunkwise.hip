@@ -42,11 +42,12 @@ struct ScanLds {
   static constexpr int BYTES = SCALES + 64;
 };
 
-// STATES: U and the state before each chunk are kept for the backward, and nothing else is written.
+// KEPT: U and the state before each chunk are kept for the backward, in as many planes, and nothing else is written; 0: the forward.
 // PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32).
-template <typename T, int DKB, int PARTS, int KST, bool STATES>
+template <typename T, int DKB, int PARTS, int KST, int KEPT>
 __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p) {
-  constexpr int DKP = DKB * 32, PK = PLANES<T, STATES>, PLANE = L * DKP * 2, IMG = PK * PLANE;
+  constexpr bool STATES = KEPT != 0;
+  constexpr int DKP = DKB * 32, PK = PLANES<T>, PLANE = L * DKP * 2, IMG = PK * PLANE;
   constexpr int TPW = 4 / PARTS, NB = DKB / PARTS;  // a wave's tiles of 16 tokens, its 32s of DQK
   constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
   using Lds = ScanLds<DKB, PK, PARTS, KST, !STATES, PAIR>;
@@ -238,9 +239,9 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       split8(st[2 * s], st[2 * s + 1], hi, lo);
       if constexpr (STATES) {
         if (kept) {
-          f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, PK, DKP);
+          f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, KEPT, DKP);
           *(f16x8*)((char*)to + r * (DKP * 2) + gq * 16 + sb * 64) = hi;
-          if constexpr (PK == 2) *(f16x8*)((char*)(to + 16 * DKP) + r * (DKP * 2) + gq * 16 + sb * 64) = lo;
+          if constexpr (KEPT == 2) *(f16x8*)((char*)(to + 16 * DKP) + r * (DKP * 2) + gq * 16 + sb * 64) = lo;
         }
       }
 #pragma unroll
@@ -422,9 +423,9 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
           const int mt = part * TPW + x;
           f16x4 hi, lo;
           split4(u[x], us.up, hi, lo);
-          char* to = (char*)(p.kept.u + kept_at(part0 + c, p.kept.blocks, block, PK, L)) + r * (L * 2) + (mt >> 1) * 64 + gq * 16 + (mt & 1) * 8;
+          char* to = (char*)(p.kept.u + kept_at(part0 + c, p.kept.blocks, block, KEPT, L)) + r * (L * 2) + (mt >> 1) * 64 + gq * 16 + (mt & 1) * 8;
           *(f16x4*)to = hi * by;
-          if constexpr (PK == 2) *(f16x4*)(to + 16 * L * 2) = lo * by;
+          if constexpr (KEPT == 2) *(f16x4*)(to + 16 * L * 2) = lo * by;
         }
         if (lane == 0 && part == 0) {
           const int64_t at = (part0 + c) * p.kept.blocks + block;
@@ -478,10 +479,11 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
 }
 
 // A block by one wave, W blocks a workgroup.
-template <typename T, int DKB, int STAGES, bool STATES>
+template <typename T, int DKB, int STAGES, int KEPT>
 __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
-  constexpr int W = 4, DKP = DKB * 32, PK = PLANES<T, STATES>, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = (STATES ? 1 : 2) * IMG;
-  constexpr bool PAIR = STATES ? PK == 2 : !std::is_same_v<T, bf16_t>;
+  constexpr bool STATES = KEPT != 0;
+  constexpr int W = 4, DKP = DKB * 32, PK = PLANES<T>, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = (STATES ? 1 : 2) * IMG;
+  constexpr bool PAIR = STATES ? KEPT == 2 : !std::is_same_v<T, bf16_t>;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int r = lane & 15, gq = lane >> 4;
@@ -626,9 +628,9 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
       if (s + 1 < DKB) split8(st[2 * s + 2], st[2 * s + 3], sh[(s + 1) & 1], sl[(s + 1) & 1]);
       if constexpr (STATES) {
         if (kept) {
-          f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, PK, DKP) + r * DKP + s * 32 + gq * 8;
+          f16_t* to = p.kept.s0 + kept_at(part0 + c, p.kept.blocks, block, KEPT, DKP) + r * DKP + s * 32 + gq * 8;
           *(f16x8*)to = hi;
-          if constexpr (PK == 2) *(f16x8*)(to + 16 * DKP) = lo;
+          if constexpr (KEPT == 2) *(f16x8*)(to + 16 * DKP) = lo;
         }
       }
 #pragma unroll
@@ -702,9 +704,9 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
       if (kept) {
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
-          f16_t* to = p.kept.u + kept_at(part0 + c, p.kept.blocks, block, PK, L) + r * L + s * 32 + gq * 8;
+          f16_t* to = p.kept.u + kept_at(part0 + c, p.kept.blocks, block, KEPT, L) + r * L + s * 32 + gq * 8;
           *(f16x8*)to = uh[s];
-          if constexpr (PK == 2) *(f16x8*)(to + 16 * L) = ul[s];
+          if constexpr (KEPT == 2) *(f16x8*)(to + 16 * L) = ul[s];
         }
         if (lane == 0) {
           const int64_t at = (part0 + c) * p.kept.blocks + block;
@@ -788,19 +790,20 @@ struct Choice {
 // At most a block of columns a CU: by as many waves as there are 32s of DQK, up to 4.  More: one a wave, 4 a workgroup.  us of whole
 // calls of bf16, 2048 tokens, both ways (waves of a block, a wave): 128 x 256, 256 blocks 91, 112; 512 171, 128; 1024 316, 165; 2048
 // 613, 335; 64 x 256, 512 blocks 104, 98; 256 x 512, 512 blocks 181, 147; 1024 365, 180.
-template <typename T, int DKB, bool STATES>
+template <typename T, int DKB, int KEPT>
 Choice choice(bool many) {
-  constexpr int PK = PLANES<T, STATES>, KST = DKB == 8 && PK == 2 && !STATES ? 1 : 2;  // K's pairs twice and Q's do not fit
+  constexpr bool STATES = KEPT != 0;
+  constexpr int PK = PLANES<T>, KST = DKB == 8 && PK == 2 && !STATES ? 1 : 2;  // K's pairs twice and Q's do not fit
   constexpr int PARTS = DKB < 4 ? DKB : 4;
   constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
   if (many)
-    return {(const void*)delta_scan_wave_kernel<T, DKB, KST, STATES>, 256, 4, KST * (STATES ? 1 : 2) * PK * L * DKB * 64 + 2 * 1024};
-  return {(const void*)delta_scan_kernel<T, DKB, PARTS, KST, STATES>, 64 * PARTS + 64, 1,
+    return {(const void*)delta_scan_wave_kernel<T, DKB, KST, KEPT>, 256, 4, KST * (STATES ? 1 : 2) * PK * L * DKB * 64 + 2 * 1024};
+  return {(const void*)delta_scan_kernel<T, DKB, PARTS, KST, KEPT>, 64 * PARTS + 64, 1,
           ScanLds<DKB, PK, PARTS, KST, !STATES, PAIR>::BYTES};
 }
-template <typename T, bool STATES>
+template <typename T, int KEPT>
 Choice pick(int dkp, bool many) {
-  return dkp == 64 ? choice<T, 2, STATES>(many) : dkp == 128 ? choice<T, 4, STATES>(many) : choice<T, 8, STATES>(many);
+  return dkp == 64 ? choice<T, 2, KEPT>(many) : dkp == 128 ? choice<T, 4, KEPT>(many) : choice<T, 8, KEPT>(many);
 }
 
 }  // namespace
@@ -814,7 +817,9 @@ int launch_scan(const Shape& s, const void* v, const float* c0, void* h, float* 
   Choice use{};
   auto choose = [&](auto t) {
     using T = decltype(t);
-    use = kept ? pick<T, true>(s.dkp(), many) : pick<T, false>(s.dkp(), many);
+    if (!kept) use = pick<T, 0>(s.dkp(), many);
+    else if (s.kept() == 2) use = pick<T, 2>(s.dkp(), many);
+    else if constexpr (std::is_same_v<T, bf16_t>) use = pick<T, 1>(s.dkp(), many);
   };
   if (s.dtype == XL_DTYPE_F32) choose(float{});
   else if (s.dtype == XL_DTYPE_BF16) choose(bf16_t{});

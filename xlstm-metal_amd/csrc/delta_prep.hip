@@ -75,7 +75,7 @@ __device__ __forceinline__ void block_max(float (&m)[N], float (*red)[8]) {
 
 template <typename T, int DKB, bool BWD>
 __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
-  constexpr int DKP = DKB * 32, PK = PLANES<T, BWD>, IMG = L * DKP * 2;
+  constexpr int DKP = DKB * 32, PK = PLANES<T>, IMG = L * DKP * 2;
   extern __shared__ __align__(1024) char lds[];  // the images of K and Q; then A, T and P
   __shared__ double bs[L];
   __shared__ float betas[L], red[4][8];
@@ -361,11 +361,11 @@ int64_t up256(int64_t n) { return (n + 255) & ~(int64_t)255; }
 
 size_t prep_bytes(const Shape& s, bool backward) {
   const int64_t frags = up256(s.parts() * 2 * FRAG_PLANE * 2);
-  return 2 * up256(s.images() * s.image_bytes(backward)) + (backward ? 4 : 2) * frags + up256(s.parts() * (int64_t)sizeof(Factors));
+  return 2 * up256(s.images() * s.image_bytes()) + (backward ? 4 : 2) * frags + up256(s.parts() * (int64_t)sizeof(Factors));
 }
 
 Prep prep_at(const Shape& s, bool backward, char* ws) {
-  const int64_t image = up256(s.images() * s.image_bytes(backward)), frags = up256(s.parts() * 2 * FRAG_PLANE * 2);
+  const int64_t image = up256(s.images() * s.image_bytes()), frags = up256(s.parts() * 2 * FRAG_PLANE * 2);
   Prep p{};
   p.k = ws;
   p.q = p.k + image;
@@ -393,7 +393,7 @@ int launch_prep(const Shape& s, const void* q, const void* k, const void* g, con
   const void* kern = s.dtype == XL_DTYPE_F32    ? backward ? pick<float, true>(s.dkp()) : pick<float, false>(s.dkp())
                      : s.dtype == XL_DTYPE_BF16 ? backward ? pick<bf16_t, true>(s.dkp()) : pick<bf16_t, false>(s.dkp())
                                                 : backward ? pick<f16_t, true>(s.dkp()) : pick<f16_t, false>(s.dkp());
-  int64_t lds = 2 * s.image_bytes(backward);
+  int64_t lds = 2 * s.image_bytes();
   if (lds < 3 * L * MLD * 4) lds = 3 * L * MLD * 4;
   void* args[] = {&a};
   hipError_t e = hipFuncSetAttribute(kern, hipFuncAttributeMaxDynamicSharedMemorySize, (int)lds);

@@ -961,13 +961,13 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_delta_chunkwise
     }
     return {dq, dk, dv, dg, dbeta, dc0};
   }
-  const int dt = dtype_code(q, what);
-  const size_t ws_bytes = xl_gated_delta_chunkwise_bwd_workspace_size(n.B, n.NH, n.NHK, n.S, n.DQK, n.DV, dt);
+  const int dt = dtype_code(q, what), dg_t = dtype_code(g, what);
+  const size_t ws_bytes = xl_gated_delta_chunkwise_bwd_workspace_size_gates(n.B, n.NH, n.NHK, n.S, n.DQK, n.DV, dt, dg_t);
   const Tensor ws = at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte));
   check_rc(xl_gated_delta_chunkwise_bwd(ptr(q), ptr(k), ptr(v), st, ptr(g), ptr(beta), ptr<float>(c0), ptr(dh),
                                         ptr<float>(dcl), ptr(dq), ptr(dk), ptr(dv), ptr(dg), ptr(dbeta),
                                         c0.defined() ? ptr<float>(dc0) : nullptr, n.B, n.NH, n.NHK, n.S, n.DQK, n.DV,
-                                        (float)scale, dt, dtype_code(g, what), ptr(ws), ws_bytes, gpu.st),
+                                        (float)scale, dt, dg_t, ptr(ws), ws_bytes, gpu.st),
            what);
   return {dq, dk, dv, dg, dbeta, dc0};
 }

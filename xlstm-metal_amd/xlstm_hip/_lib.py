@@ -66,6 +66,7 @@ SIGNATURES = {
     "xl_gated_delta_chunkwise_fwd": (_i, [_vp] * 3 + [ctypes.POINTER(_i64)] + [_vp] * 2 + [_fp, _vp, _fp] + [_i] * 6 + [_f]
                                      + [_i] * 2 + [_vp, _sz, _vp]),
     "xl_gated_delta_chunkwise_bwd_workspace_size": (_sz, [_i] * 7),
+    "xl_gated_delta_chunkwise_bwd_workspace_size_gates": (_sz, [_i] * 8),
     "xl_gated_delta_chunkwise_bwd": (_i, [_vp] * 3 + [ctypes.POINTER(_i64)] + [_vp] * 2 + [_fp, _vp, _fp] + [_vp] * 5 + [_fp]
                                      + [_i] * 6 + [_f] + [_i] * 2 + [_vp, _sz, _vp]),
     "xl_gated_linear_workspace_size": (_sz, [_i64] + [_i] * 4),
@@ -74,7 +75,7 @@ SIGNATURES = {
     "xl_newton_schulz": (_i, [_vp] * 2 + [_i64, _i, _i, ctypes.POINTER(_f), _i, _f, _i, _vp, _sz, _vp]),
 }
 
-ABI_VERSION = 5
+ABI_VERSION = 6
 
 _lib = None
 _lock = threading.Lock()
