@@ -1,5 +1,5 @@
 """The gated delta rule on the GPU where sizes are far apart: gradients beside a matrix of zeros, keys far below 1, rows of one chunk
-far from each other.
+far from each other, columns that are not finite.
 
 Bars of gradients are those of test_gpu_gated_delta_bwd, of a head or (``token_parts``) of each token's own terms; of h and the state
 delta_reference's, but that what a token adds to the state is taken at its key's length (``tight``)."""
@@ -7,7 +7,7 @@ delta_reference's, but that what a token adds to the state is taken at its key's
 import pytest
 import torch
 
-from delta_reference import CHUNK_KU, check, make
+from delta_reference import CHUNK_KU, check, make, reference
 from helpers import dev
 from test_gpu_gated_delta_bwd import BAR, check_all, gradients, inputs, plain
 
@@ -184,3 +184,50 @@ def test_gradients_of_rows_far_apart(gpu_case, shape, kind):
         largest = torch.cat([c.amax(-1, keepdim=True).expand_as(c) for c in part.split(64, -1)], -1)
         worst = float(((err - 2.0 ** -34 * largest) / part.clamp_min(1e-300)).max())
         assert worst <= BAR[F32], f"{name}: {worst:.3e} of a token's terms"
+
+
+# ------------------------------------------------------------------ columns that are not finite
+@pytest.mark.parametrize("shape", [(1, 2, 2, 200, 64, 48), (1, 1, 1, 140, 256, 40), (40, 8, 8, 140, 64, 20)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("value", [float("inf"), float("nan")])
+@pytest.mark.parametrize("size", [1.0, 1e7, 1e-7])
+def test_not_finite_stays_in_its_column(gpu_case, shape, dtype, value, size):
+    """One value of v, or of the state, that is not finite: the 15 columns beside it keep their results, and so does
+    what its own column had in earlier chunks."""
+    import xlstm_hip
+    x = list(make(*shape, F32, F32, seed=51))
+    x[2], x[5] = x[2] * size, x[5] * size
+    x[:3] = (t.to(dtype) for t in x[:3])
+    hr, cr, hb, cb = reference(*x, CHUNK_KU, planes=dtype == BF16)
+    others = torch.arange(shape[5], device=dev()) != 3
+    for where in ("v", "c"):
+        y = [t.clone() for t in x]
+        if where == "v":
+            y[2][0, -1, 130, 3] = value
+        else:
+            y[5][0, -1, 5, 3] = value
+        h, c = xlstm_hip.gated_delta_chunkwise(*y, return_last_states=True)
+        check(h[..., others], hr[..., others], hb[..., others], f"h, {where}")
+        check(c[..., others], cr[..., others], cb[..., others], f"C, {where}")
+        check(h[:, :-1], hr[:, :-1], hb[:, :-1], f"h of other heads, {where}")
+        if where == "v":
+            check(h[:, :, :128], hr[:, :, :128], hb[:, :, :128], "h of earlier chunks")
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 2, 100, 64, 48), (16, 8, 8, 70, 128, 48)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+def test_gradients_beside_a_column_that_is_not_finite(gpu_case, shape, dtype):
+    """dH of one column is infinite: dv and dc0 of the other columns are what they were (dq, dk and the gates' sum over all of them)."""
+    import xlstm_hip
+    (q, k, v, g, beta, c0), dh, dc = inputs(shape, dtype, F32, 52)
+    x, dh, dc = (q, k, v, g, beta, c0), dh * 1e6, dc * 1e6
+    fn = lambda *y: xlstm_hip.gated_delta_chunkwise(*y, return_last_states=True)  # noqa: E731
+    want = gradients(lambda *y: plain(*y, shape[4] ** -0.5), x, dh, dc, torch.float64)
+    spoilt = dh.clone()
+    spoilt[:, :, 37, 3] = float("inf")
+    got = gradients(fn, x, spoilt, dc)
+    others = torch.arange(shape[5], device=dev()) != 3
+    for i in (2, 5):
+        a, w = (t[..., others].double().flatten(2) for t in (got[i], want[i]))
+        worst = float(((a - w).norm(dim=-1) / w.norm(dim=-1)).max())
+        assert worst <= BAR[dtype] + torch.finfo(got[i].dtype).eps / 2, f"{i}: {worst:.3e}"

@@ -118,9 +118,11 @@ __device__ __forceinline__ float exp_of(double x) {
   return fmaf(e, (float)(x - (double)hi), e);
 }
 
-// max over the wave of x >= 0, in every lane (scalar); by the bits, which order as the values do (a NaN is the largest)
+// max over the wave of x >= 0, in every lane (scalar); by the bits, which order as the values do.  A lane's infinity or NaN does not count: a
+// lane has values of one column, and its neighbours keep their scale.
 __device__ __forceinline__ float wave_max_all(float value) {
   uint32_t x = __float_as_uint(value);
+  x = x < 0x7f800000u ? x : 0u;
 #define XL_DPP_MAX(CTRL, ROWMASK) x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, CTRL, ROWMASK, 0xf, false));
   XL_DPP_MAX(0x111, 0xf)  // row_shr:1 (what is shifted in is 0)
   XL_DPP_MAX(0x112, 0xf)
