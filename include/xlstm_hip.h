@@ -427,7 +427,7 @@ int xl_gated_delta_recurrent_fwd(const void* q, const void* k, const void* v, co
 
 /*
  * By chunks of 64 tokens, any S.  strides (host memory): element strides of batch, head and token of q, k and v, values
- * contiguous, or NULL for contiguous tensors.  h 16-byte aligned, c_last apart from c0.  Workspace:
+ * contiguous, or NULL for contiguous tensors; a token stride is 0 to 2^22 (any for one token).  h 16-byte aligned, c_last apart from c0.  Workspace:
  * xl_gated_delta_chunkwise_workspace_size bytes, 256-byte aligned.
  */
 size_t xl_gated_delta_chunkwise_workspace_size(int B, int NH, int NHK, int S, int DQK, int DV, int dtype_qkv);

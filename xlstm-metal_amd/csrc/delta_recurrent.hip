@@ -336,14 +336,15 @@ int check_shape(const char* who, const Shape& s) {
 
 int set_strides(Shape& s, const int64_t* strides, const char* who) {
   if (strides) {
-    for (int i = 0; i < 3; ++i)  // a token stride is multiplied by up to 63 in 32 bits
-      if (strides[3 * i + 2] < 0 || strides[3 * i + 2] > MAX_TOKEN_STRIDE)
+    for (int i = 0; i < 3; ++i)  // a token stride is multiplied by up to 63 in 32 bits; one token's is never stepped
+      if (s.S > 1 && (strides[3 * i + 2] < 0 || strides[3 * i + 2] > MAX_TOKEN_STRIDE))
         return set_error(XL_ERR_UNSUPPORTED, "%s: token strides must be 0 to %d elements", who, MAX_TOKEN_STRIDE);
     for (int i = 0; i < 3; ++i) {
       s.qs[i] = strides[i];
       s.ks[i] = strides[3 + i];
       s.vs[i] = strides[6 + i];
     }
+    if (s.S <= 1) s.qs[2] = s.ks[2] = s.vs[2] = 0;
     return XL_OK;
   }
   auto dense = [&](int64_t (&to)[3], int heads, int D) {

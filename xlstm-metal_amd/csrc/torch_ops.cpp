@@ -858,9 +858,10 @@ struct DeltaSizes {
   DeltaSizes(const DeltaShape& s, const char* w)
       : B(i32(s.B, w)), NH(i32(s.NH, w)), NHK(i32(s.NHK, w)), S(i32(s.S, w)), DQK(i32(s.DQK, w)), DV(i32(s.DV, w)) {}
 };
-// q, k and v as they lie where their last axis is contiguous (strides: batch, head, token of each)
+// q, k and v as they lie where their last axis is contiguous (strides: batch, head, token of each; of one token any, which contiguous()
+// would leave as it is)
 Tensor delta_rows(const Tensor& t, int64_t* strides) {
-  const Tensor r = (t.size(3) <= 1 || t.stride(3) == 1) && t.stride(2) <= (1 << 22) ? t : t.contiguous();
+  const Tensor r = (t.size(3) <= 1 || t.stride(3) == 1) && (t.size(2) <= 1 || t.stride(2) <= (1 << 22)) ? t : t.contiguous();
   for (int d = 0; d < 3; ++d) strides[d] = r.stride(d);
   return r;
 }
