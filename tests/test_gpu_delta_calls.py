@@ -1,4 +1,4 @@
-"""Calls of the gated delta rule at the edges of their shapes: one token under any stride."""
+"""Calls of the gated delta rule at the edges of their shapes: one token under any stride, an empty batch."""
 
 import pytest
 import torch
@@ -30,3 +30,23 @@ def test_one_token_under_any_stride(gpu_case):
         h, c = xlstm_hip.gated_delta_chunkwise(*z, return_last_states=True)
         found.append(torch.autograd.grad(h.float().sum() + c.sum(), z))
     assert all(torch.equal(a, b) for a, b in zip(*found))
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_empty_batch(gpu_case, dtype):
+    """No sequences: empty results and gradients, as without tokens."""
+    import xlstm_hip
+    x = [t[:0] for t in make(1, 4, 2, 70, 64, 48, dtype, F32, seed=2)]
+    for op in (xlstm_hip.gated_delta_chunkwise, xlstm_hip.gated_delta_recurrent):
+        h, c = op(*x, return_last_states=True)
+        assert h.shape == (0, 4, 70, 48) and h.dtype == dtype and c.shape == (0, 4, 64, 48) and c.dtype == F32
+        assert op(*x[:5]).shape == (0, 4, 70, 48)
+    one = [t[:, :, 0] for t in x[:5]]
+    h, c = xlstm_hip.gated_delta_step(*one, x[5])
+    assert h.shape == (0, 4, 48) and c.shape == (0, 4, 64, 48)
+    h, c = xlstm_hip.gated_delta_step_(*one, x[5])
+    assert h.shape == (0, 4, 48) and c is x[5]
+    y = [t.detach().requires_grad_(True) for t in x]
+    h, c = xlstm_hip.gated_delta_chunkwise(*y, return_last_states=True)
+    for g, t in zip(torch.autograd.grad((h, c), y, (torch.ones_like(h), torch.ones_like(c))), y):
+        assert g.shape == t.shape and g.dtype == t.dtype

@@ -876,6 +876,7 @@ std::tuple<Tensor, Tensor> gated_delta_recurrent(const Tensor& q_, const Tensor&
   const Tensor q = q_.contiguous(), k = k_.contiguous(), v = v_.contiguous(), g = g_.contiguous(), beta = beta_.contiguous();
   const Tensor c0 = f32(c0_), h = at::empty({s.B, s.NH, s.S, s.DV}, q.options());
   const Tensor cl = return_last_states ? at::empty({s.B, s.NH, s.DQK, s.DV}, f32_on(q)) : at::empty({0}, f32_on(q));
+  if (s.B == 0) return {h, cl};
   check_rc(xl_gated_delta_recurrent_fwd(ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr<float>(c0), ptr(h),
                                         return_last_states ? ptr<float>(cl) : nullptr, n.B, n.NH, n.NHK, n.S, n.DQK, n.DV,
                                         (float)scale, dtype_code(q, what), dtype_code(g, what), gpu.st),
@@ -890,6 +891,7 @@ Tensor launch_delta_step(const Tensor& q_, const Tensor& k_, const Tensor& v_, c
   const DeltaSizes n(s, what);
   const Tensor q = q_.contiguous(), k = k_.contiguous(), v = v_.contiguous(), g = g_.contiguous(), beta = beta_.contiguous();
   const Tensor h = at::empty({s.B, s.NH, s.DV}, q.options());
+  if (s.B == 0) return h;
   check_rc(xl_gated_delta_recurrent_fwd(ptr(q), ptr(k), ptr(v), ptr(g), ptr(beta), ptr<float>(c), ptr(h), ptr<float>(c_new), n.B,
                                         n.NH, n.NHK, 1, n.DQK, n.DV, (float)scale, dtype_code(q, what), dtype_code(g, what),
                                         gpu.st),
@@ -928,6 +930,7 @@ std::tuple<Tensor, Tensor> gated_delta_chunkwise(const Tensor& q_, const Tensor&
   const Tensor g = g_.contiguous(), beta = beta_.contiguous(), c0 = f32(c0_);
   const Tensor h = at::empty({s.B, s.NH, s.S, s.DV}, q.options());
   const Tensor cl = return_last_states ? at::empty({s.B, s.NH, s.DQK, s.DV}, f32_on(q)) : at::empty({0}, f32_on(q));
+  if (s.B == 0) return {h, cl};
   const int dt = dtype_code(q, what);
   const size_t ws_bytes = xl_gated_delta_chunkwise_workspace_size(n.B, n.NH, n.NHK, n.S, n.DQK, n.DV, dt);
   const Tensor ws = ws_bytes ? at::empty({(int64_t)ws_bytes}, q.options().dtype(at::kByte)) : Tensor();
@@ -955,7 +958,7 @@ std::tuple<Tensor, Tensor, Tensor, Tensor, Tensor, Tensor> gated_delta_chunkwise
   auto dense = [](const Tensor& t) { return at::empty(t.sizes(), t.options()); };
   const Tensor dq = dense(q), dk = dense(k), dv = dense(v), dg = dense(g), dbeta = dense(beta);
   const Tensor dc0 = c0.defined() ? dense(c0) : at::empty({0}, f32_on(q));
-  if (s.S == 0) {
+  if (s.S == 0 || s.B == 0) {
     if (c0.defined()) {
       if (dcl.defined()) dc0.copy_(dcl);
       else dc0.zero_();
