@@ -147,8 +147,17 @@ class _RMSNorm(nn.Module):
         return F.rms_norm(x.float(), (x.shape[-1],), self.weight.float(), self.eps).to(x.dtype)
 
 
+def _plain_linear(m: nn.Module) -> bool:
+    """Whether a call of m is its weight's product and nothing else: an nn.Linear as it is, without bias or hooks."""
+    return (type(m) is nn.Linear and m.bias is None and "forward" not in m.__dict__
+            and not (m._forward_pre_hooks or m._forward_hooks or m._backward_pre_hooks or m._backward_hooks)
+            and not nn.modules.module._has_any_global_hook())
+
+
 class _FFN(nn.Module):
-    """``fused``: gate, up, SiLU and product in one kernel, rounded once (three roundings otherwise); it differentiates."""
+    """``fused``: gate, up, SiLU and product in one kernel, rounded once (three roundings otherwise); it differentiates.  Where that kernel
+    would pass something by (forward derivatives, torch.func's transforms, autocast, a projection's hooks or another module in its place)
+    the projections are called."""
 
     def __init__(self, d: int, hidden: int, fused: bool = False) -> None:
         super().__init__()
@@ -157,8 +166,14 @@ class _FFN(nn.Module):
         self.proj_up_gate = nn.Linear(d, hidden, bias=False)
         self.proj_down = nn.Linear(hidden, d, bias=False)
 
+    def _one_kernel(self, x: Tensor) -> bool:
+        gate, up = self.proj_up_gate, self.proj_up
+        return (x.device.type == "cuda" and x.dtype in (torch.bfloat16, torch.float16) and _plain_linear(gate) and _plain_linear(up)
+                and gate.weight.dtype == up.weight.dtype == x.dtype and forward_ad._current_level < 0
+                and not torch._C._are_functorch_transforms_active() and not torch.is_autocast_enabled())
+
     def forward(self, x: Tensor) -> Tensor:
-        if self.fused and x.device.type == "cuda" and x.dtype in (torch.bfloat16, torch.float16):
+        if self.fused and self._one_kernel(x):
             return self.proj_down(gated_linear_unit(x, self.proj_up_gate.weight, self.proj_up.weight))
         gate, up = self.proj_up_gate(x), self.proj_up(x)
         if _one_pass(gate, up):
