@@ -60,10 +60,11 @@ __device__ __forceinline__ u32x4 rounded8(const float (&v)[8]) {
   return raw;
 }
 
-// act(a) and its derivative; exp by the hardware's exp2, a few units of float32 off, far below a 16-bit result's rounding
+// act(a) and its derivative; exp by the hardware's exp2, a few units of float32 off, far below a 16-bit result's rounding.  GELU by erfc:
+// 1 + erf cancels below zero (at a = -4 to 11 bits).
 __device__ __forceinline__ float act_of(float a, int act) {
   if (act == SILU) return a * __builtin_amdgcn_rcpf(1.f + __builtin_amdgcn_exp2f(a * -1.4426950408889634f));
-  return 0.5f * a * (1.f + erff(a * 0.70710678118654752f));
+  return 0.5f * a * erfcf(a * -0.70710678118654752f);
 }
 __device__ __forceinline__ float act_grad(float a, int act, float& value) {
   if (act == SILU) {
@@ -71,7 +72,7 @@ __device__ __forceinline__ float act_grad(float a, int act, float& value) {
     value = a * s;
     return s * fmaf(a, 1.f - s, 1.f);
   }
-  const float phi = 0.5f * (1.f + erff(a * 0.70710678118654752f));
+  const float phi = 0.5f * erfcf(a * -0.70710678118654752f);
   value = a * phi;
   return fmaf(a * 0.3989422804014327f, __builtin_amdgcn_exp2f(a * a * -0.72134752044448170f), phi);
 }
