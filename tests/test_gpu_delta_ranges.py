@@ -231,3 +231,21 @@ def test_gradients_beside_a_column_that_is_not_finite(gpu_case, shape, dtype):
         a, w = (t[..., others].double().flatten(2) for t in (got[i], want[i]))
         worst = float(((a - w).norm(dim=-1) / w.norm(dim=-1)).max())
         assert worst <= BAR[dtype] + torch.finfo(got[i].dtype).eps / 2, f"{i}: {worst:.3e}"
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 2, 140, 64, 48), (40, 8, 8, 70, 64, 20)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("which", [0, 1, 2])
+def test_rows_of_zeros(gpu_case, shape, dtype, which):
+    """Tokens whose q, k or v is zeros, alone and a chunk of them, beside others: their h, and dk or dq, which do not vanish."""
+    import xlstm_hip
+    x, dh, dc = inputs(shape, dtype, F32, 61)
+    x[which][:, :, 3:9] = 0
+    x[which][:, :, -1] = 0
+    x[which][:, :, 64:] = 0
+    hr, cr, hb, cb = tight(*x, planes=dtype == BF16)
+    h, c = xlstm_hip.gated_delta_chunkwise(*x, return_last_states=True)
+    check(c, cr, cb, "C")
+    check(h, hr, hb, "h")
+    if shape[0] == 1:
+        check_all(x, dh, dc)

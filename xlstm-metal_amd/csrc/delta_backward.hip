@@ -19,8 +19,8 @@
 //
 // Heads of v that share q and k write their dQ and dK in float32, and a last kernel adds them in order.
 //
-// Measured (bf16, 2 x 4096 tokens of 8 heads of 128 x 256), us: first kernel 37, dH by columns 17, states 121, scan backwards
-// 155, chunks' gradients 133.  The scans are bound by the chain of one chunk's step; the last by its waits between products
+// Measured (2 x 4096 tokens of 8 heads of 128 x 256), us: first kernel 37, dH by columns 17, states 125, scan backwards 161, chunks'
+// gradients 135 for bf16 inputs and gates; with float32 gates, which keep pairs, 37, 22, 146, 183, 270.  The scans are bound by the chain of one chunk's step; the last by its waits between products
 // (its 377 MB are 73 us of a copy).
 #include "delta.h"
 
@@ -394,7 +394,8 @@ struct GradLds {
 };
 
 // DKB waves: a wave has 32 of DQK's columns of dQ and dK, turned (columns down, tokens across), and its share of the 64 x 64 tiles.
-// At DQK 128 two workgroups fit a CU with 256 registers a lane (bf16: 165 us against 187, measured before it came to 133; pairs would spill).
+// At DQK 128 two workgroups fit a CU with 256 registers a lane (bf16: 165 us against 187, measured before it came to 135; pairs would spill).
+// bf16's dQ and dK take D o dP and E in one plane, whose rounding is an eighth of their own.
 template <typename T, int DKB, int KEPT>
 __global__ __launch_bounds__(64 * DKB, (DKB == 4 && KEPT == 1 ? 2 : 1)) void delta_grad_kernel(GradArgs p) {
   using Lds = GradLds<T, DKB, KEPT>;
@@ -980,7 +981,8 @@ int backward(const Shape& s, const void* v, const void* dh, const float* dc_last
   const int stages = s.dkp() == 256 ? S8 : 2;
   // A lone wave a block where two workgroups a CU (one, if no two fit) take all blocks, else four blocks a workgroup.  us of whole calls,
   // 2048 tokens, lone waves and fours: bf16 128 x 256, 256 blocks 252, 277; 512 433, 454; 768 626, 572; 1024 755, 689; 64 x 256, 512
-  // blocks 346, 357; 1024 637, 577; 256 x 512, 512 blocks 597, 548; float32 128 x 256, 512 blocks of 1024 tokens 362, 349.
+  // blocks 346, 357; 1024 637, 577; 256 x 512, 512 blocks 597, 548; float32 128 x 256, 512 blocks of 1024 tokens 362, 349; f16
+  // 128 x 256, 256 blocks 420, 468; 512 748, 785; 768 1040, 983; 256 x 512, 512 blocks 1188, 1151.
   const int64_t scan_lds = stages * 2 * s.image_bytes() + 2 * 2048;
   const int waves = (int64_t)s.B * s.NH * kept.blocks <= (scan_lds <= 80 * 1024 ? 512 : 256) ? 1 : 4;
   const int slices = (kept.blocks + waves - 1) / waves;

@@ -14,7 +14,7 @@
 // The images of K and Q come to LDS straight from memory, K a chunk ahead, Q into the place of this chunk's when it has been read;
 // in delta_scan_kernel by a wave of its own (a load into LDS that has to queue stops its wave).  T, P and V of the next chunk wait in
 // registers.  H is formed turned (columns down, tokens across): a lane holds four neighbours of a row.  Measured (bf16): 2 x 4096 tokens
-// of 8 heads of 128 x 256 136 us, 2.1 a chunk; 4 x 8192 of 8 heads of 256 x 512 520 to 560, 4.2 a chunk.
+// of 8 heads of 128 x 256 139 to 144 us, 2.2 a chunk; 4 x 8192 of 8 heads of 256 x 512 575 to 630, 4.5 to 4.9 a chunk.
 #include "delta.h"
 
 namespace xl {
@@ -43,7 +43,9 @@ struct ScanLds {
 };
 
 // KEPT: U and the state before each chunk are kept for the backward, in as many planes, and nothing else is written; 0: the forward.
-// PAIR: the outputs' products too are of pairs (f16, whose own rounding is near a single plane's, and float32).
+// PAIR: the outputs' products too are of pairs (f16, whose own rounding is a single plane's, and float32).  bf16's h, off by up to
+// 2^-8 by its own rounding, takes P, U and the state in one plane there, 2^-11 each (pairs: 4 to 12 % of a call); its U and state are
+// formed of pairs.
 template <typename T, int DKB, int PARTS, int KST, int KEPT>
 __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p) {
   constexpr bool STATES = KEPT != 0;

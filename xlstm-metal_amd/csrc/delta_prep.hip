@@ -8,7 +8,7 @@
 // its block column, T_ij = -T_ii sum_l A_il T_lj, with v_mfma_f32_16x16x4_f32, whose result is the next one's operand as it
 // stands.  Everything a scan reads as an operand (T diag(beta), P) is written in operand order, 16 bytes a lane.
 //
-// Large: bound by memory (bf16, 4 x 8192 tokens of 8 heads of 256: 136 to 144 us for 0.64 GB in and out, which a copy takes
+// Large: bound by memory (bf16, 4 x 8192 tokens of 8 heads of 256: 144 to 153 us for 0.64 GB in and out, which a copy takes
 // 124 for); few chunks: by the chain of one (13 chunks of 8 heads of 128: 12.8 us).
 #include "delta.h"
 

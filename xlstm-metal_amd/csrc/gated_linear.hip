@@ -392,7 +392,8 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void glu_few_kernel(const T* __rest
 }
 
 // ------------------------------------------------------------------------------------------------ da, du
-// [Tp, Fp], zero past T and F; 8 values a thread
+// [Tp, Fp], zero past T and F; 8 values a thread.  Rounded once, to the type, for the matrix cores, as a block of two 16-bit projections rounds
+// them too: the weights' gradients have two roundings, and float16's da and du end at 65504 and 2^-25, as dh does.
 template <typename T>
 __global__ __launch_bounds__(256) void glu_factors_kernel(const T* __restrict__ dh, const float* __restrict__ a,
                                                           const float* __restrict__ u, int64_t keep_pitch, T* __restrict__ da,

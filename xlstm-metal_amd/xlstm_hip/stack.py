@@ -77,7 +77,7 @@ class StackConfig:
     eps: float = 1e-6
     init_std: float = 0.02
     dtype: torch.dtype = torch.bfloat16
-    fused_ffn: bool = False       # the FFN's two projections, SiLU and product by gated_linear_unit (bf16, f16)
+    fused_ffn: bool = False       # the FFN's two projections, SiLU and product by gated_linear_unit (bf16, f16); changes roundings
 
     @property
     def qk_head_dim(self) -> int:
