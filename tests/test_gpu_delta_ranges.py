@@ -249,3 +249,40 @@ def test_rows_of_zeros(gpu_case, shape, dtype, which):
     check(h, hr, hb, "h")
     if shape[0] == 1:
         check_all(x, dh, dc)
+
+
+# ------------------------------------------------------------------ small writes into a large state
+@pytest.mark.parametrize("shape", [(40, 8, 8, 640, 64, 20)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("by", ["beta", "k"])
+def test_small_writes_add_up(gpu_case, shape, dtype, by):
+    """Tokens that each write 1e-6 or less of the state, without decay (gates all but closed, or short keys): thousands of them are seen.
+
+    Bar, of the largest value of the state (a column's block has one scale): a chunk rounds the state to float32 and takes its writes
+    at 2^-31 of it, 64 of them: 2^-22 in all; a write is off by 16 2^-22 of itself (delta_reference)."""
+    import xlstm_hip
+    B, NH, _, S, DQK, DV = shape
+    r = torch.Generator().manual_seed(71)
+    unit = torch.nn.functional.normalize(torch.randn(B, NH, 1, DQK, generator=r), dim=-1).expand(B, NH, S, DQK)
+    v = torch.rand(B, NH, S, DV, generator=r) + 0.5
+    size = {"beta": (1e-6, 1.0), "k": (0.7, 2.0 ** -20)}[by]
+    q, k, v = unit.to(dtype).to(dev()), (unit * size[1]).to(dtype).to(dev()), v.to(dtype).to(dev())
+    g, beta = torch.zeros(B, NH, S, device=dev()), torch.full((B, NH, S), size[0], device=dev())
+    # a state that does not answer to the keys: every token writes beta v
+    c0 = torch.randn(B, NH, DQK, DV, generator=r).to(dev())
+    u = k[:, :, 0].double() / k[:, :, 0].double().norm(dim=-1, keepdim=True)
+    c0 = (c0.double() - u[..., None] * (u[..., None] * c0.double()).sum(-2, keepdim=True)).float()
+    want = c0.double()
+    kd, vd, bd = k[:, :, 0].double(), v.double(), float(beta[0, 0, 0].double())
+    # k is the same at every token: C's part along it goes to x - beta |k|^2 x + beta v by itself
+    along, n2 = (kd[..., None] * want).sum(-2), (kd ** 2).sum(-1)[..., None]
+    total = torch.zeros_like(along)
+    for t in range(S):
+        d = bd * (vd[:, :, t] - along)
+        along, total = along + n2 * d, total + d
+    want = want + kd[..., None] * total[..., None, :]
+    _, c = xlstm_hip.gated_delta_chunkwise(q, k, v, g, beta, c0, return_last_states=True)
+    chunks = (S + 63) // 64
+    bar = chunks * 2.0 ** -22 * float(want.abs().max()) + CHUNK_KU * float((kd[..., None] * total[..., None, :]).abs().max())
+    err = float((c.double() - want).abs().max())
+    assert err <= bar, f"{err:.3e} over {bar:.3e}; written {float((want - c0).abs().max()):.3e}"

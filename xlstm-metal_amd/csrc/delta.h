@@ -219,9 +219,14 @@ __device__ __forceinline__ void to_lds(uint32_t lds, uint32_t offset, const void
 
 // The scans keep the state at a power-of-two scale: its planes are taken without a multiplication.  With max(c_L |S|, |w|)
 // below 2^(STATE + 1) and K's values below 2 the next state, c_L S + K^T w over 64 tokens, is below 129 2^(STATE + 1) = 33024.
+// A chunk's products are summed from zero and added to the state once: in the matrix cores' sums every one of them would
+// round the state, towards zero.
 constexpr int STATE = 7;
 constexpr int STATE_BACK = 6;  // two products: 257 2^7 = 32896
 
+__device__ __forceinline__ f32x4 fma4(f32x4 x, float a, f32x4 y) {
+  return f32x4{fmaf(x[0], a, y[0]), fmaf(x[1], a, y[1]), fmaf(x[2], a, y[2]), fmaf(x[3], a, y[3])};
+}
 // max of |x| of a lane's
 template <int N>
 __device__ __forceinline__ float abs_max(const f32x4 (&x)[N]) {

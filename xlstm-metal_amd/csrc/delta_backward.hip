@@ -330,7 +330,7 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
     st_down = ws.down;
 #pragma unroll
     for (int t = 0; t < 2 * DKB; ++t) {
-      f32x4 y = st[t] * up, y2 = f32x4{0.f, 0.f, 0.f, 0.f};
+      f32x4 y = {0.f, 0.f, 0.f, 0.f}, y2 = y;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if constexpr (PK == 2) {
@@ -342,7 +342,7 @@ __global__ __launch_bounds__(W == 1 ? 128 : 64 * W, 1) void delta_back_kernel(Ba
         y = mfma(qc[t % AHEAD][0][s], w1h[s], y);
         y2 = mfma(kc[t % AHEAD][0][s], w2h[s], y2);
       }
-      st[t] = y + y2;
+      st[t] = fma4(st[t], up, y + y2);
       if (t + AHEAD < 2 * DKB) read_columns(t + AHEAD);
       __builtin_amdgcn_sched_barrier(0);
     }

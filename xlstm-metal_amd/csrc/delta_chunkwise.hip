@@ -408,14 +408,14 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     const float up = keep * st_down * sc.up;
 #pragma unroll
     for (int t = 0; t < 2 * NB; ++t) {
-      f32x4 y = st[t] * up, y2 = {0.f, 0.f, 0.f, 0.f};
+      f32x4 y = {0.f, 0.f, 0.f, 0.f}, y2 = y;
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if constexpr (PK == 2) y2 = mfma(kc[t][1][s], wh[s], y2);
         y2 = mfma(kc[t][0][s], wl[s], y2);
         y = mfma(kc[t][0][s], wh[s], y);
       }
-      st[t] = y + y2;
+      st[t] = fma4(st[t], up, y + y2);
     }
     if constexpr (STATES) {
       if (kept) {
@@ -735,14 +735,14 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
     st_down = ws.down;
 #pragma unroll
     for (int t = 0; t < 2 * DKB; ++t) {
-      f32x4 y = st[t] * up;
+      f32x4 y = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int s = 0; s < 2; ++s) {
         if constexpr (PK == 2) y = mfma(columns[t % AHEAD][1][s], wh[s], y);
         y = mfma(columns[t % AHEAD][0][s], wl[s], y);
         y = mfma(columns[t % AHEAD][0][s], wh[s], y);
       }
-      st[t] = y;
+      st[t] = fma4(st[t], up, y);
       if (t + AHEAD < 2 * DKB) read_columns(t + AHEAD);
       __builtin_amdgcn_sched_barrier(0);
     }
