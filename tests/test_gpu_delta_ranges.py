@@ -252,7 +252,7 @@ def test_rows_of_zeros(gpu_case, shape, dtype, which):
 
 
 # ------------------------------------------------------------------ small writes into a large state
-@pytest.mark.parametrize("shape", [(40, 8, 8, 640, 64, 20)])
+@pytest.mark.parametrize("shape", [(1, 2, 2, 2560, 64, 48), (1, 1, 1, 1920, 256, 32), (1, 2, 2, 1280, 128, 64), (40, 8, 8, 640, 64, 20)])
 @pytest.mark.parametrize("dtype", [F32, BF16])
 @pytest.mark.parametrize("by", ["beta", "k"])
 def test_small_writes_add_up(gpu_case, shape, dtype, by):

@@ -392,18 +392,23 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     const float u_down = largest(of_u), w_down = u_down * decayed.down * 2.f;
     // U decayed is below 2^15 w_down
     const Pow2 sc = pow2_for(fmaxf(largest(of_s) * keep, w_down * 32767.f), STATE);
+    // U decayed from its parts' scales to the state's, in two steps of 2^-24 at most: as one f16 factor what is 2^-25 or less (writes of 2^-17 of the
+    // state and below) would be 0
     f16x8 wh[2], wl[2];
+    _Float16 by2[PARTS];
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+      const float x = of_u[i] * (decayed.down * 2.f) * sc.up;
+      by[i] = (_Float16)fmaxf(x, 0x1p-24f);
+      by2[i] = (_Float16)fminf(x * 0x1p24f, 1.f);
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) raw[i] = raw[i] * by[i / TPW];
+    planes(by2, wh, wl);
     shifts(of_u, u_down, by);
-    planes(by, wh, wl);
     if constexpr (!STATES) {
 #pragma unroll
       for (int x = 0; x < TPW; ++x) qs[x] = sum_of(part * TPW + x);
-    }
-    const _Float16 shift = (_Float16)(w_down * sc.up);  // to the state's scale: 2^-8 or less
-#pragma unroll
-    for (int s = 0; s < 2; ++s) {
-      wh[s] *= shift;
-      wl[s] *= shift;
     }
     const float up = keep * st_down * sc.up;
 #pragma unroll
