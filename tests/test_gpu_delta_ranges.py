@@ -286,3 +286,33 @@ def test_small_writes_add_up(gpu_case, shape, dtype, by):
     bar = chunks * 2.0 ** -22 * float(want.abs().max()) + CHUNK_KU * float((kd[..., None] * total[..., None, :]).abs().max())
     err = float((c.double() - want).abs().max())
     assert err <= bar, f"{err:.3e} over {bar:.3e}; written {float((want - c0).abs().max()):.3e}"
+
+
+@pytest.mark.parametrize("shape", [(1, 2, 2, 200, 64, 48), (1, 1, 1, 200, 256, 32), (40, 8, 8, 140, 128, 20)])
+@pytest.mark.parametrize("size", [1e6, 1e8])
+def test_large_values_at_short_keys(gpu_case, shape, size):
+    """A token in 16 whose v is 1e6 (1e8) times the others' and whose k as much shorter: its U is large, what it writes is not, and the state and
+    the other tokens' writes keep their bits, float32.
+
+    Bar: 16 2^-22 of the state's columns and of the chunk's writes (delta_reference), at q's length; and U is off by 2^-39 of its block's
+    largest: of a state of 64 tokens' (random signs) 2^-36 of it, twice that where a chunk's products take it again."""
+    import xlstm_hip
+    q, k, v, g, beta, _ = make(*shape, F32, F32, seed=81, state=False)
+    rare = (torch.arange(shape[3], device=dev()) % 16 == 5)[:, None]
+    k, v = torch.where(rare, k / size, k), torch.where(rare, v * size, v)
+    hr, cr, hb, cb = tight(q, k, v, g, beta, None)
+    B, NH, S = g.shape
+    kd, scale = k.double().repeat_interleave(NH // k.shape[1], 1), shape[4] ** -0.5
+    C, bar, writes = torch.zeros_like(cr), torch.empty_like(hr), 0.0
+    lq = q.double().norm(dim=-1).repeat_interleave(NH // k.shape[1], 1)
+    most, largest = 0.0, float(v.abs().max())
+    for t in range(S):
+        C = C * torch.exp(g[:, :, t].double())[..., None, None]
+        d = beta[:, :, t, None].double() * (v[:, :, t].double() - (kd[:, :, t, :, None] * C).sum(-2))
+        C = C + kd[:, :, t, :, None] * d[..., None, :]
+        most = torch.maximum(torch.as_tensor(most, device=dev()), C.norm(dim=-2))
+        writes = writes + (kd[:, :, t].norm(dim=-1, keepdim=True) * d).abs()
+        bar[:, :, t] = scale * lq[:, :, t, None] * (CHUNK_KU * (most + writes) + 2.0 ** -35 * largest)
+    h, c = xlstm_hip.gated_delta_chunkwise(q, k, v, g, beta, return_last_states=True)
+    err = (h.double() - hr).abs() / bar
+    assert float(err.max()) <= 1, f"h: {float(err.max()):.2f} of the bar"

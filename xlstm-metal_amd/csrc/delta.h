@@ -53,16 +53,15 @@ constexpr int FRAG_PLANE = FRAGS * 64 * 8;  // f16 values of one plane
 constexpr float CLAMP_G = -1e4f;  // exp() of it is 0: a reset (-inf) keeps the sums finite
 
 // Per head and chunk, by the first kernel: per-token factors (the scales of K's and Q's rows, 2^k_i and 2^q_i, folded in) and scales, the bytes
-// as biased exponents.  A row of zeros has scale 0 (its out must not raise `most`).
+// as biased exponents.  A row of zeros has scale 0.
 struct Factors {
   float in[L];      // c_i 2^k_i          K S
   float q[L];       // scale c_i 2^q_i    Q S
   float out[L];     // c_L / c_i 2^k_i    U into the state
   float all;        // c_L
-  float most;       // the largest of out
   float t, tt;      // T diag(beta), T^T = planes * these
   uint8_t p[L];     // P's rows = planes * these
-  float pad[44];    // the scan takes the first 1 KB into LDS
+  float pad[45];    // the scan takes the first 1 KB into LDS
   float back[L];    // beta_i in_i        Z into the state's gradient
   float pt[L];      // P^T's rows
   uint8_t k[L], qs[L];  // K's and Q's rows
@@ -101,14 +100,14 @@ __device__ __forceinline__ void interleave() {
 }
 
 // 2^target / 2^exponent(m) and its inverse: m times the first is in [2^target, 2^(target + 1)); m >= 0.
-// At most 2^most either way (0 gets that).
+// At most 2^100 either way (0 gets that).
 struct Pow2 {
   float up, down;
 };
-__device__ __forceinline__ Pow2 pow2_for(float m, int target = 14, int most = 100) {
+__device__ __forceinline__ Pow2 pow2_for(float m, int target = 14) {
   const int e = (int)(__float_as_uint(m) >> 23);
   int sh = e == 255 ? 0 : target + 127 - e;
-  sh = sh > most ? most : sh < -100 ? -100 : sh;
+  sh = sh > 100 ? 100 : sh < -100 ? -100 : sh;
   return {__uint_as_float((uint32_t)(127 + sh) << 23), __uint_as_float((uint32_t)(127 - sh) << 23)};
 }
 

@@ -64,7 +64,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
   const T* v = (const T*)p.v + b * p.vs[0] + h * p.vs[1];
   T* ho = (T*)p.h + (int64_t)bh * p.S * p.DV;
   const uint32_t lds_at = (uint32_t)(uintptr_t)(lds_char*)lds;
-  float* const scales = (float*)(lds + Lds::SCALES);  // [R, U, state][part]
+  float* const scales = (float*)(lds + Lds::SCALES);  // [R, U, state, U decayed][part]
   // sums over part `from`'s rows of token tile mt (its owner's own too: to leave those out took branches that cost more)
   auto sums_at = [&](int mt, int from) { return (f32x4*)(lds + Lds::SUMS) + (mt * PARTS + from) * 64 + lane; };
   auto sum_of = [&](int mt) {
@@ -274,9 +274,6 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       }
     }
     const float keep = f->all, t_scale = f->t;
-    const Pow2 decayed = pow2_for(f->most, 0);  // U decayed is below 2 decayed.down times U
-    // The product of both scales is at most 2^126: U of zeros would have the largest there is, and keys far below 1 have another.
-    const int most_up = min(100, 254 - (int)(__float_as_uint(decayed.up) >> 23));
     most = state_max(st) * st_down;
     if (lane == 0) scales[2 * PARTS + part] = most;
     lds_barrier();
@@ -347,13 +344,12 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       w[x] = u[x] * out[x];
     }
     load_t(next);
-    const Pow2 us = pow2_for(wave_max_all(abs_max(u)), 14, most_up);
-    const float ws_up = us.up * decayed.up * 0.5f;
+    const Pow2 us = pow2_for(wave_max_all(abs_max(u))), ws = pow2_for(wave_max_all(abs_max(w)));
 #pragma unroll
     for (int x = 0; x < TPW; ++x) {
       const int mt = part * TPW + x;
       f16x4 hi, lo;
-      split4(w[x], ws_up, hi, lo);
+      split4(w[x], ws.up, hi, lo);
       *((f16x8*)(lds + Lds::UD) + mt * 64 + lane) = join(hi, lo);
       if constexpr (!STATES) {
         split4(u[x], us.up, hi, lo);
@@ -361,7 +357,10 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
         else *((f16x4*)(lds + Lds::U) + mt * 64 + lane) = hi;
       }
     }
-    if (lane == 0) scales[PARTS + part] = us.down;
+    if (lane == 0) {
+      scales[PARTS + part] = us.down;
+      scales[3 * PARTS + part] = ws.down;
+    }
     if constexpr (!STATES) {
 #pragma unroll
       for (int mt = 0; mt < 4; ++mt) *sums_at(mt, part) = hs[mt];
@@ -371,9 +370,10 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     f16x8 kc[2 * NB][PK][2], raw_u[PAIR ? 4 : 1];
     f16x4 half_u[PAIR || STATES ? 1 : 4];
     f32x4 qs[STATES ? 1 : TPW];
-    float of_u[PARTS], of_s[PARTS];
+    float of_u[PARTS], of_s[PARTS], of_w[PARTS];
     read_scales(1, of_u);
     read_scales(2, of_s);
+    read_scales(3, of_w);
     read4(Lds::UD);
 #pragma unroll
     for (int t = 0; t < 2 * NB; ++t)
@@ -389,16 +389,16 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
       }
     }
     __builtin_amdgcn_sched_barrier(0);
-    const float u_down = largest(of_u), w_down = u_down * decayed.down * 2.f;
-    // U decayed is below 2^15 w_down
-    const Pow2 sc = pow2_for(fmaxf(largest(of_s) * keep, w_down * 32767.f), STATE);
+    const float u_down = largest(of_u);
+    // U decayed is below 2^15 of its scale
+    const Pow2 sc = pow2_for(fmaxf(largest(of_s) * keep, largest(of_w) * 32767.f), STATE);
     // U decayed from its parts' scales to the state's, in two steps of 2^-24 at most: as one f16 factor what is 2^-25 or less (writes of 2^-17 of the
     // state and below) would be 0
     f16x8 wh[2], wl[2];
     _Float16 by2[PARTS];
 #pragma unroll
     for (int i = 0; i < PARTS; ++i) {
-      const float x = of_u[i] * (decayed.down * 2.f) * sc.up;
+      const float x = of_w[i] * sc.up;
       by[i] = (_Float16)fmaxf(x, 0x1p-24f);
       by2[i] = (_Float16)fminf(x * 0x1p24f, 1.f);
     }
@@ -622,7 +622,6 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
       }
     }
     const float keep = f->all, t_scale = f->t;
-    const Pow2 decayed = pow2_for(f->most, 0);  // U decayed is below 2 decayed.down times U
     f16x8 sh[2], sl[2];
     split8(st[0], st[1], sh[0], sl[0]);
 #pragma unroll
@@ -680,7 +679,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
 #pragma unroll
     for (int i = 0; i < LOWER; ++i) u[lower_mt(i)] = mfma(th[i], rl[lower_s(i)], u[lower_mt(i)]);
     load_t(next);
-    const float most = state_max(st) * st_down;  // not needed before w
+    const float most = abs_max(st) * (st_down * keep);  // a lane's, not needed before w
     // the first operands of the state's product
     constexpr int AHEAD = 4;
     f16x8 columns[AHEAD][PK][2];
@@ -699,7 +698,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
       w[mt] = u[mt] * out[mt];
     }
     const Pow2 us = pow2_for(wave_max_all(abs_max(u)));
-    const Pow2 ws = pow2_for(fmaxf(us.down * decayed.down * 65534.f, most * keep), STATE);  // U is below 2^15 us.down
+    const Pow2 ws = pow2_for(wave_max_all(fmaxf(abs_max(w), most)), STATE);
     f16x8 uh[2], ul[2], wh[2], wl[2];
 #pragma unroll
     for (int s = 0; s < 2; ++s) {

@@ -211,9 +211,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
       f->b[lane] = sum;
       f->in[lane] = in * ks;
       f->q[lane] = in * qs * p.scale;
-      const float out = exp_of(last - sum) * ks, most = wave_max_all(out);
-      f->out[lane] = out;
-      if (lane == 0) f->most = most;
+      f->out[lane] = exp_of(last - sum) * ks;
       f->back[lane] = bt * in * ks;
       f->k[lane] = exponent_of(ks);
       f->qs[lane] = exponent_of(qs);
