@@ -316,3 +316,27 @@ def test_large_values_at_short_keys(gpu_case, shape, size):
     h, c = xlstm_hip.gated_delta_chunkwise(q, k, v, g, beta, return_last_states=True)
     err = (h.double() - hr).abs() / bar
     assert float(err.max()) <= 1, f"h: {float(err.max()):.2f} of the bar"
+
+
+# ------------------------------------------------------------------ padding
+@pytest.mark.parametrize("shape", [(1, 2, 2, 150, 64, 48), (1, 2, 1, 100, 200, 40), (40, 8, 8, 140, 64, 20)])
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("large", [1.0, 1e9, 1e15])
+def test_padding_of_any_values(gpu_case, shape, dtype, large):
+    """Tokens of g and beta 0, scattered and a run over a chunk's border, with whatever is in their q, k and v: the others' h and the state are
+    those of the sequence without them."""
+    import xlstm_hip
+    x = make(*shape, dtype, F32, seed=91)
+    S = shape[3]
+    t = torch.arange(S)
+    pad = (t % 7 == 3) | ((t > 50) & (t < 75))
+    y = [a.clone() for a in x]
+    y[3][:, :, pad], y[4][:, :, pad] = 0, 0
+    keep = (~pad).to(dev())
+    hr, cr, hb, cb = reference(*[a[:, :, keep] for a in y[:5]], y[5], CHUNK_KU, planes=dtype == BF16)
+    for i in range(3):
+        y[i][:, :, pad] *= large
+    h, c = xlstm_hip.gated_delta_chunkwise(*y, return_last_states=True)
+    # chunks are cut where they would not be without the padding: a second chunk's start as large as the first's
+    check(c, cr, 2 * cb, "C")
+    check(h[:, :, keep], hr, 2 * hb, "h")

@@ -5,7 +5,7 @@
 //
 // In a chunk, with b_i = g_1 + .. + g_i, c_i = exp(b_i), D_ij = exp(b_i - b_j) and S the state before it (rows i, j are tokens):
 //
-//   A_ij = beta_i D_ij k_i.k_j (j < i),  T = (I + A)^-1,  U = T diag(beta) (V - diag(c) K S),  P_ij = scale D_ij q_i.k_j (j <= i)
+//   A_ij = beta_i D_ij k_i.k_j (j < i),  T = (I + A)^-1,  U = T R,  R = diag(beta) (V - diag(c) K S),  P_ij = scale D_ij q_i.k_j (j <= i)
 //   H = scale diag(c) Q S + P U,   S' = c_L S + (diag(c_L / c_j) K)^T U
 //
 // T and P do not know the state: a first kernel (delta_prep) forms them for all chunks at once.  What is left of a chunk
@@ -14,7 +14,7 @@
 //
 // All products are on the matrix cores in f16 with float32 sums.  Every operand stands at a power-of-two scale that puts its
 // largest value high in f16's range: each row of K, of Q and of P at its own, so that a token's h has its bits beside tokens of other
-// sizes; T at a chunk's; S, V - diag(c) K S and U at a block of columns'.  Largest values from 2^-86 to 2^110 are kept.  float32 values enter
+// sizes; T at a chunk's; S, R and U at a block of columns'.  Largest values from 2^-86 to 2^110 are kept.  float32 values enter
 // as pairs hi + lo of f16 (22 bits), and a product of two pairs is three.  f16 ends at 2^-24: a value x times below its operand's largest is
 // off by 2^-25 of that where this stands at 1 (K, Q), by 2^-39 where at 2^14 (R, U), if that is more than 2^-22 (one plane: 2^-11) of itself.
 //
@@ -55,21 +55,21 @@ constexpr float CLAMP_G = -1e4f;  // exp() of it is 0: a reset (-inf) keeps the 
 // Per head and chunk, by the first kernel: per-token factors (the scales of K's and Q's rows, 2^k_i and 2^q_i, folded in) and scales, the bytes
 // as biased exponents.  A row of zeros has scale 0.
 struct Factors {
-  float in[L];      // c_i 2^k_i          K S
-  float q[L];       // scale c_i 2^q_i    Q S
-  float out[L];     // c_L / c_i 2^k_i    U into the state
-  float all;        // c_L
-  float t, tt;      // T diag(beta), T^T = planes * these
+  float back[L];    // beta_i c_i 2^k_i    K S; Z into the state's gradient
+  float q[L];       // scale c_i 2^q_i     Q S
+  float out[L];     // c_L / c_i 2^k_i     U into the state
+  float beta[L];    // the scan by several waves takes this 1 KB into LDS, and what follows to P's rows into registers,
+  float all, t;     // c_L; T = planes * t
   uint8_t p[L];     // P's rows = planes * these
-  float pad[45];    // the scan takes the first 1 KB into LDS
-  float back[L];    // beta_i in_i        Z into the state's gradient
+  float tt;         // T^T
+  float pad[45];    // that by one wave 1.25 KB,
   float pt[L];      // P^T's rows
+  float in[L];      // c_i 2^k_i
   uint8_t k[L], qs[L];  // K's and Q's rows
-  float pad2[32];
-  float beta[L];    // the scan backwards takes 2 KB
+  float pad2[32];   // the scan backwards 2 KB
   double b[L];      // running sums of g
 };
-static_assert(sizeof(Factors) == 2560 && offsetof(Factors, back) == 1024 && offsetof(Factors, b) == 2048);
+static_assert(sizeof(Factors) == 2560 && offsetof(Factors, all) == 1024 && offsetof(Factors, b) == 2048);
 __device__ __forceinline__ float power_of(uint32_t exponent) { return __uint_as_float(exponent << 23); }
 __device__ __forceinline__ uint8_t exponent_of(float power) { return (uint8_t)(__float_as_uint(power) >> 23); }
 
@@ -306,7 +306,7 @@ struct Shape {
 // What the first kernel writes; transposed forms for the backward only.
 struct Prep {
   char *k, *q;       // images
-  f16_t *t, *p;      // [part][plane][FRAG_PLANE]: T diag(beta) (2 planes), P
+  f16_t *t, *p;      // [part][plane][FRAG_PLANE]: T (2 planes), P; columns of tokens of beta 0: delta_prep.hip
   f16_t *tt, *pt;    // T^T, P^T (2 planes)
   Factors* f;
 };

@@ -7,7 +7,7 @@
 // large a part of a chunk's tokens.  Per chunk:
 //
 //   1  K S and Q S over the wave's rows, all tokens; the others' tokens go to LDS
-//   2  R = V - diag(c) K S of the wave's tokens, to LDS as f16 planes
+//   2  R = diag(beta) (V - diag(c) K S) of the wave's tokens, to LDS as f16 planes
 //   3  U = T R of the wave's tokens, to LDS as f16 planes, decayed for the state and as it is for H
 //   4  S = c_L S + K^T U of the wave's rows; H = Q S + P U of the wave's tokens
 //
@@ -105,8 +105,8 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     }
     return;
   }
-  // Tokens 16 mt + 4 gq + e of column n, mt of this wave.  Past the last token the last one is read again (its beta is 0 there: T
-  // has zeros in its column), past the last column the last one: those columns are computed and not written.
+  // Tokens 16 mt + 4 gq + e of column n, mt of this wave.  Past the last token the last one is read again (beta is 0 there),
+  // past the last column the last one: those columns are computed and not written.
   const int nc = n < p.DV ? n : p.DV - 1, row_step = (int)p.vs[2];
   T vn[TPW][4];
   uint32_t v_at[TPW][4];
@@ -140,10 +140,19 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
 #pragma unroll
       for (int s = 0; s < 2; ++s) to[x][s] = load16(from + (2 * (part * TPW + x) + s) * 512, lane * 16);
   };
+  float all_next, t_next;  // the next chunk's factors that are not in LDS
+  uint8_t p_next[TPW];
   auto load_t = [&](int chunk) {
     const f16_t* from = p.prep.t + (part0 + chunk) * (2 * FRAG_PLANE);
     load_rows(from, th);
     load_rows(from + FRAG_PLANE, tl);
+    const Factors* f = p.prep.f + part0 + chunk;
+    all_next = f->all;
+    t_next = f->t;
+    if constexpr (!STATES) {
+#pragma unroll
+      for (int x = 0; x < TPW; ++x) p_next[x] = f->p[16 * (part * TPW + x) + r];
+    }
   };
   auto load_p = [&](int chunk) {
     const f16_t* from = p.prep.p + (part0 + chunk) * (2 * FRAG_PLANE);
@@ -216,8 +225,19 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     const Factors* f = (const Factors*)(lds + Lds::FACTORS + (c & 1) * 1024);
 
     // ---- 1: K S, and Q S turned, over the wave's rows
-    f32x4 ks[4], hs[STATES ? 1 : 4], in[TPW], out[TPW];
+    f32x4 ks[4], hs[STATES ? 1 : 4], in[TPW], bv[TPW], out[TPW];
     float fq[TPW], fp[TPW];
+#pragma unroll
+    for (int x = 0; x < TPW; ++x) {
+      const int mt = part * TPW + x;
+      in[x] = *(const f32x4*)&f->back[16 * mt + 4 * gq];
+      bv[x] = *(const f32x4*)&f->beta[16 * mt + 4 * gq];
+      out[x] = *(const f32x4*)&f->out[16 * mt + 4 * gq];
+      if constexpr (!STATES) {
+        fq[x] = f->q[16 * mt + r];
+        fp[x] = power_of(p_next[x]);
+      }
+    }
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
       ks[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -265,15 +285,12 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     for (int mt = 0; mt < 4; ++mt) *sums_at(mt, part) = ks[mt];
 #pragma unroll
     for (int x = 0; x < TPW; ++x) {
-      const int mt = part * TPW + x;
-      in[x] = *(const f32x4*)&f->in[16 * mt + 4 * gq] * st_down;
-      out[x] = *(const f32x4*)&f->out[16 * mt + 4 * gq];
-      if constexpr (!STATES) {
-        fq[x] = f->q[16 * mt + r] * st_down;
-        fp[x] = power_of(f->p[16 * mt + r]);
-      }
+      in[x] *= st_down;
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bv[x][e] *= to_f32(vn[x][e]);
+      if constexpr (!STATES) fq[x] *= st_down;
     }
-    const float keep = f->all, t_scale = f->t;
+    const float keep = all_next, t_scale = t_next;
     most = state_max(st) * st_down;
     if (lane == 0) scales[2 * PARTS + part] = most;
     lds_barrier();
@@ -283,7 +300,7 @@ __global__ __launch_bounds__(64 * PARTS + 64) void delta_scan_kernel(ScanArgs p)
     for (int x = 0; x < TPW; ++x) {
       const f32x4 sum = sum_of(part * TPW + x);
 #pragma unroll
-      for (int e = 0; e < 4; ++e) rr[x][e] = fmaf(-in[x][e], sum[e], to_f32(vn[x][e]));
+      for (int e = 0; e < 4; ++e) rr[x][e] = fmaf(-in[x][e], sum[e], bv[x][e]);
     }
     load_v(next);
     if constexpr (!STATES) load_p(next);
@@ -490,6 +507,7 @@ template <typename T, int DKB, int STAGES, int KEPT>
 __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
   constexpr bool STATES = KEPT != 0;
   constexpr int W = 4, DKP = DKB * 32, PK = PLANES<T>, PLANE = L * DKP * 2, IMG = PK * PLANE, STAGE = (STATES ? 1 : 2) * IMG;
+  constexpr int FACTORS = 1280;  // of a chunk's Factors, in LDS
   constexpr bool PAIR = STATES ? KEPT == 2 : !std::is_same_v<T, bf16_t>;
   extern __shared__ __align__(1024) char lds[];  // STAGES of K and Q; two chunks' factors
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
@@ -515,10 +533,12 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
     }
   };
   auto fetch_factors = [&](int chunk) {
-    if (wave == 0) to_lds(lds_at + STAGES * STAGE + (chunk & 1) * 1024, lane * 16, p.prep.f + part0 + chunk);
+    if (wave >= 2) return;  // 1.25 KB: the second wave's KB lies over the first's
+    const uint32_t from = wave * (FACTORS - 1024);
+    to_lds(lds_at + STAGES * STAGE + (chunk & 1) * FACTORS + from, from + lane * 16, p.prep.f + part0 + chunk);
   };
-  // Rows 16 mt + 4 gq + e of column n.  Past the last token the last one is read again (its beta is 0 there: T has zeros in its
-  // column), past the last column the last one: those columns are computed and not written.
+  // Rows 16 mt + 4 gq + e of column n.  Past the last token the last one is read again (beta is 0 there), past the last column the
+  // last one: those columns are computed and not written.
   const int nc = n < p.DV ? n : p.DV - 1, row_step = (int)p.vs[2];
   T vn[4][4];
   uint32_t v_at[4][4];
@@ -590,7 +610,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
     const int stage = STAGES == 2 ? c & 1 : 0, next = c + 1 < p.chunks ? c + 1 : c;
     if (next != c) fetch_factors(next);
     const char *ki = lds + stage * STAGE, *qi = ki + IMG;
-    const Factors* f = (const Factors*)(lds + STAGES * STAGE + (c & 1) * 1024);
+    const Factors* f = (const Factors*)(lds + STAGES * STAGE + (c & 1) * FACTORS);
 
     // ---- K S, and Q S turned: the operands of the next 32 of DQK are read under the products of these
     struct Rows {
@@ -610,11 +630,14 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
     for (int mt = 0; mt < 4; ++mt) ks[mt] = hs[mt] = f32x4{0.f, 0.f, 0.f, 0.f};
     Rows rows[2];
     read(rows[0], 0);
-    f32x4 in[4], out[4];
+    f32x4 in[4], bv[4], out[4];
     float fq[4], fp[4];
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt) {
-      in[mt] = *(const f32x4*)&f->in[16 * mt + 4 * gq] * st_down;
+      in[mt] = *(const f32x4*)&f->back[16 * mt + 4 * gq] * st_down;
+      bv[mt] = *(const f32x4*)&f->beta[16 * mt + 4 * gq];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) bv[mt][e] *= to_f32(vn[mt][e]);
       out[mt] = *(const f32x4*)&f->out[16 * mt + 4 * gq];
       if constexpr (!STATES) {
         fq[mt] = f->q[16 * mt + r] * st_down;
@@ -661,7 +684,7 @@ __global__ __launch_bounds__(256, 1) void delta_scan_wave_kernel(ScanArgs p) {
 #pragma unroll
     for (int mt = 0; mt < 4; ++mt)
 #pragma unroll
-      for (int e = 0; e < 4; ++e) rr[mt][e] = fmaf(-in[mt][e], ks[mt][e], to_f32(vn[mt][e]));
+      for (int e = 0; e < 4; ++e) rr[mt][e] = fmaf(-in[mt][e], ks[mt][e], bv[mt][e]);
     load_v(next);
     const Pow2 rs = pow2_for(wave_max_all(abs_max(rr)));
     f16x8 rh[2], rl[2];
@@ -803,7 +826,7 @@ Choice choice(bool many) {
   constexpr int PARTS = DKB < 4 ? DKB : 4;
   constexpr bool PAIR = !STATES && !std::is_same_v<T, bf16_t>;
   if (many)
-    return {(const void*)delta_scan_wave_kernel<T, DKB, KST, KEPT>, 256, 4, KST * (STATES ? 1 : 2) * PK * L * DKB * 64 + 2 * 1024};
+    return {(const void*)delta_scan_wave_kernel<T, DKB, KST, KEPT>, 256, 4, KST * (STATES ? 1 : 2) * PK * L * DKB * 64 + 2 * 1280};
   return {(const void*)delta_scan_kernel<T, DKB, PARTS, KST, KEPT>, 64 * PARTS + 64, 1,
           ScanLds<DKB, PK, PARTS, KST, !STATES, PAIR>::BYTES};
 }

@@ -6,7 +6,9 @@
 //
 // T by 16 x 16 blocks, in float32: each wave inverts one diagonal block by substitution (a lane a column), then walks down
 // its block column, T_ij = -T_ii sum_l A_il T_lj, with v_mfma_f32_16x16x4_f32, whose result is the next one's operand as it
-// stands.  Everything a scan reads as an operand (T diag(beta), P) is written in operand order, 16 bytes a lane.
+// stands.  Everything a scan reads as an operand (T, P) is written in operand order, 16 bytes a lane.
+// A token of beta 0 has U = 0, whatever its values: its columns of A, T and P, which only U meets, are left out, so that padding does not set
+// their scales (in the backward T's alone: dbeta needs the transposed ones).
 //
 // Large: bound by memory (bf16, 4 x 8192 tokens of 8 heads of 256: 144 to 153 us for 0.64 GB in and out, which a copy takes
 // 124 for); few chunks: by the chain of one (13 chunks of 8 heads of 128: 12.8 us).
@@ -232,7 +234,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
     for (int jt = 0; jt < 4; ++jt) {
       const int j = 16 * jt + r;
       const double bj = bs[j];
-      const float kj = ksc[j];
+      const float kj = BWD || betas[j] != 0.f ? ksc[j] : 0.f;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const int i = 16 * wave + 4 * gq + e;
@@ -288,7 +290,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
     }
     __syncthreads();
     // ---- operands: wave w has the 16 rows 16 w .. of each matrix, both halves of k
-    constexpr int FORMS = BWD ? 2 : 1;  // P, T diag(beta); P^T, T^T
+    constexpr int FORMS = BWD ? 2 : 1;  // P, T; P^T, T^T
     Factors* f = p.out.f + part;
     const int i = 16 * wave + r;
     auto column = [&](int half, int e) { return 32 * half + (e < 4 ? 4 * gq + e : 12 + 4 * gq + e); };
@@ -331,7 +333,7 @@ __global__ __launch_bounds__(256) void delta_prep_kernel(PrepArgs p) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
           const int j = column(half, e);
-          x[turned][half][e] = turned ? Tm[j * MLD + i] : Tm[i * MLD + j] * betas[j];
+          x[turned][half][e] = turned ? Tm[j * MLD + i] : BWD && betas[j] == 0.f ? 0.f : Tm[i * MLD + j];
           m[turned] = fmaxf(m[turned], fabsf(x[turned][half][e]));
         }
     }

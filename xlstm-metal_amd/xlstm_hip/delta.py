@@ -32,8 +32,8 @@ def gated_delta_chunkwise(q: Tensor, k: Tensor, v: Tensor, g: Tensor, beta: Tens
     """h, or (h, C after the last token), for prompts and training: any S, on the matrix cores by chunks of 64 tokens.
 
     q, k and v are read in place where their last axis is contiguous (a projection's transposed views).  Tokens with g and
-    beta 0 leave the state alone: pad with them.  A value that is not finite spoils the h of its chunk from its first token on, one of v or of the
-    state that of its own column only.
+    beta 0 leave the state alone, whatever finite q, k and v they have: pad with them.  A value that is not finite spoils the h of
+    its chunk from its first token on, one of v or of the state that of its own column only.
     """
     h, c = gated_delta_chunkwise_op(q, k, v, g, beta, c_initial, _scale(q, scale), return_last_states)
     return (h, c) if return_last_states else h
