@@ -19,8 +19,8 @@
 //
 // Heads of v that share q and k write their dQ and dK in float32, and a last kernel adds them in order.
 //
-// Measured (2 x 4096 tokens of 8 heads of 128 x 256), us: first kernel 37, dH by columns 17, states 125, scan backwards 161, chunks'
-// gradients 135 for bf16 inputs and gates; with float32 gates, which keep pairs, 37, 22, 146, 183, 270.  The scans are bound by the chain of one chunk's step; the last by its waits between products
+// Measured (2 x 4096 tokens of 8 heads of 128 x 256), us: first kernel 37, dH by columns 17, states 124, scan backwards 163, chunks'
+// gradients 134 for bf16 inputs and gates; with float32 gates, which keep pairs, 37, 22, 149, 189, 270.  The scans are bound by the chain of one chunk's step; the last by its waits between products
 // (its 377 MB are 73 us of a copy).
 #include "delta.h"
 

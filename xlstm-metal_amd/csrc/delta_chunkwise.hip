@@ -14,7 +14,7 @@
 // The images of K and Q come to LDS straight from memory, K a chunk ahead, Q into the place of this chunk's when it has been read;
 // in delta_scan_kernel by a wave of its own (a load into LDS that has to queue stops its wave).  T, P and V of the next chunk wait in
 // registers.  H is formed turned (columns down, tokens across): a lane holds four neighbours of a row.  Measured (bf16): 2 x 4096 tokens
-// of 8 heads of 128 x 256 139 to 144 us, 2.2 a chunk; 4 x 8192 of 8 heads of 256 x 512 575 to 630, 4.5 to 4.9 a chunk.
+// of 8 heads of 128 x 256 138 to 145 us, 2.2 a chunk; 4 x 8192 of 8 heads of 256 x 512 580 to 627, 4.5 to 4.9 a chunk.
 #include "delta.h"
 
 namespace xl {

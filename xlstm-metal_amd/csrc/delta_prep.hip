@@ -10,7 +10,7 @@
 // A token of beta 0 has U = 0, whatever its values: its columns of A, T and P, which only U meets, are left out, so that padding does not set
 // their scales (in the backward T's alone: dbeta needs the transposed ones).
 //
-// Large: bound by memory (bf16, 4 x 8192 tokens of 8 heads of 256: 144 to 153 us for 0.64 GB in and out, which a copy takes
+// Large: bound by memory (bf16, 4 x 8192 tokens of 8 heads of 256: 144 to 152 us for 0.64 GB in and out, which a copy takes
 // 124 for); few chunks: by the chain of one (13 chunks of 8 heads of 128: 12.8 us).
 #include "delta.h"
 
